@@ -77,6 +77,11 @@ SIGNATURES: dict[str, list] = {
     "cin_moe_combine": [_p, _i32, _i64, _p, _i32, _i64, _p, _i64, _i64, _i64, _i64, _p, _i64, _p],
     "cin_moe_combine_backward": [_p, _i64, _p, _i32, _i64, _p, _i32, _i64, _p, _p, _i64, _i64, _i64,
                                  _i64, _p, _i32, _i64, _p, _p],
+    "cin_moe_gate": [_p, _i32, _i64, _p, _i64, _i64, _i64, _i32, _i64, _i64, _i32, _i32, ctypes.c_float, _p, _p,
+                     _p, _p],
+    "cin_moe_gate_backward": [_p, _i32, _i64, _i64, _i64, _i64, _i32, _i32, ctypes.c_float, _p, _p, _p, _p, _p],
+    "cin_rotary": [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i64] * 2 + [_i32, _i64, _i64, _i64, _p, _p, _i64, _i64,
+                                                                           _i64, _i64, _p, _i64, _i64, _i32, _i32, _p],
 }
 
 # entry points that return something other than an int status
@@ -133,6 +138,15 @@ def call(name: str, *args) -> None:
         if rc == CIN_ERR_ARG:
             raise ValueError(msg)
         raise CinnamonLibraryError(msg)
+
+
+def call_on(t: torch.Tensor, name: str, *args) -> None:
+    """call() with t's device current: a launch goes to the current device."""
+    if t.get_device() == torch._C._cuda_getDevice():
+        call(name, *args)
+    else:
+        with torch.cuda.device(t.device):
+            call(name, *args)
 
 
 def dtype_code(t) -> int:

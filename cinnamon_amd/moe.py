@@ -4,13 +4,14 @@ Counterpart of the permute -> grouped experts -> unpermute block of the referenc
 MoE.forward (src/layers.py:126-157):
 
   reference                                      here
+  sigmoid, bias, top-k, renormalized weights     moe_gate: one launch, and one for the gradient
   expanded_idx.sort(), token_indices, bincount,  moe_route: stable counting sort on the
   cumsum, max_expert_tokens = .item()            device, int64 expert ranges, no host sync
   sorted_x = flat_x[token_indices] (bf16),       moe_gather_quantize: the 1x128 quantizer
   then the experts quantize it                   reads x rows through the permutation
   sorted_out * sorted_scores, scatter_add_       moe_combine: per-token sum in sorted order
 
-``routed_experts`` chains them with layers.experts_forward/backward; its gradients reach
+``routed_experts`` chains those after moe_gate with layers.experts_forward/backward; its gradients reach
 x, the expert weights and the routing scores.  Every launch is a cinnamon_amd:: torch
 operator (torch.compile traces through it).  The sort is stable, so within an expert the
 rows keep token order (the reference's unstable sort may order them differently; each
@@ -22,15 +23,159 @@ from __future__ import annotations
 import torch
 
 from . import layers
-from ._lib import call, dtype_code, ptr, stream_of
-from .kernels import _cdiv, _require, _run_detached, _scale_buf, custom_op
+from ._lib import call, call_on, dtype_code, ptr, stream_of
+from .kernels import _cdiv, _plain_eager, _require, _run_detached, _scale_buf, custom_op
 
 _ROUTE_CHUNK = 1024  # assignments per route workgroup (csrc/moe.hip kChunk)
 MAX_EXPERTS = 4096
 MAX_TOP_K = 16
+MAX_GROUPS = 64
 
-__all__ = ["moe_route", "moe_gather_quantize", "moe_gather_sum", "moe_combine",
+__all__ = ["moe_gate", "moe_route", "moe_gather_quantize", "moe_gather_sum", "moe_combine",
            "moe_combine_backward", "RoutedExpertsFunction", "routed_experts"]
+
+
+# ---------------------------------------------------------------------------
+# The gate (reference src/layers.py:122-126)
+# ---------------------------------------------------------------------------
+_SCORES = {"sigmoid": 0, "softmax": 1}
+
+
+def moe_gate(logits: torch.Tensor, top_k: int, bias: torch.Tensor | None = None, score: str = "sigmoid",
+             n_groups: int = 1, top_groups: int | None = None, group_top: int = 2, renormalize: bool = True,
+             scale: float = 1.0, return_scores: bool = False):
+    """The chosen experts of each token and their weights, from the router's logits [n_tokens, E]
+    (bf16, fp16 or fp32): (top_idx int64 [n_tokens, top_k], top_scores fp32 [n_tokens, top_k]) for
+    routed_experts, and with return_scores all scores fp32 [n_tokens, E] (for a balance loss).
+
+      scores = sigmoid(logits) or softmax(logits); choice = scores + bias (fp32 [E], only chooses);
+      with n_groups > 1, E / n_groups neighbouring experts form a group, a group counts by the sum of
+      its group_top (1 or 2) largest choices, and only the best top_groups groups stay;
+      top_idx: the top_k largest choices left, falling, ties to the lowest index; choices are
+      compared in 64 bits; NaN counts as the greatest, as in torch.topk;
+      top_scores = scale * scores[top_idx], divided by (their sum + 1e-9) with renormalize.
+
+    Differentiable in logits, through top_scores and scores; no gradient reaches bias."""
+    _require(logits.is_cuda, "Input must be on CUDA")
+    _require(logits.ndim == 2, "logits must be [n_tokens, n_experts]")
+    _require(logits.dtype in (torch.bfloat16, torch.float16, torch.float32), "logits must be bf16, fp16 or fp32")
+    E = logits.shape[1]
+    _require(1 <= E <= MAX_EXPERTS, f"n_experts must be in [1, {MAX_EXPERTS}]")
+    _require(score in _SCORES, "score must be 'sigmoid' or 'softmax'")
+    _require(1 <= n_groups <= MAX_GROUPS and E % n_groups == 0, f"n_groups must divide n_experts and be in [1, {MAX_GROUPS}]")
+    top_groups = n_groups if top_groups is None else top_groups
+    _require(1 <= top_groups <= n_groups, "top_groups must be in [1, n_groups]")
+    _require(group_top in (1, 2), "group_top must be 1 or 2")
+    _require(1 <= top_k <= min(MAX_TOP_K, top_groups * (E // n_groups)),
+             f"top_k must be in [1, {MAX_TOP_K}] and within the experts of the kept groups")
+    if bias is not None:
+        _require(bias.shape == (E,) and bias.device == logits.device, "bias must be [n_experts] on logits' device")
+        _require(bias.dtype == torch.float32, "bias must be fp32")
+        bias = bias.detach()
+    options = (int(top_k), _SCORES[score], int(n_groups), int(top_groups), int(group_top), bool(renormalize),
+               float(scale), bool(return_scores))
+    if _plain_eager(logits, bias):
+        if torch.is_grad_enabled() and logits.requires_grad:
+            out = _MoeGate.apply(logits, bias, *options)
+        else:
+            out = _launch_gate(logits, bias, *options)
+    else:
+        out = _gate_op(logits, bias, *options)
+    return out if return_scores else out[:2]
+
+
+def _gate_rows(logits):
+    return logits if logits.stride(1) == 1 and logits.stride(0) >= logits.shape[1] else logits.contiguous()
+
+
+def _launch_gate(logits, bias, top_k, score, n_groups, top_groups, group_top, renormalize, scale, return_scores):
+    lg = _gate_rows(logits)
+    T, E = lg.shape
+    dev = lg.device
+    idx = torch.empty((T, top_k), dtype=torch.int64, device=dev)
+    w = torch.empty((T, top_k), dtype=torch.float32, device=dev)
+    scores = torch.empty((T, E) if return_scores else (0,), dtype=torch.float32, device=dev)
+    bias = None if bias is None else bias.contiguous()
+    call_on(lg, "cin_moe_gate", ptr(lg), dtype_code(lg), max(lg.stride(0), E), ptr(bias), T, E, top_k, score, n_groups,
+            top_groups, group_top, int(renormalize), scale, ptr(idx), ptr(w), ptr(scores) if return_scores else 0,
+            stream_of(lg))
+    return idx, w, scores
+
+
+def _launch_gate_backward(logits, idx, gw, gs, score, renormalize, scale):
+    """Gradient of the logits; gw or gs may be None."""
+    lg = _gate_rows(logits)
+    T, E = lg.shape
+    out = torch.empty((T, E), dtype=lg.dtype, device=lg.device)
+    gw = None if gw is None else gw.float().contiguous()
+    gs = None if gs is None else gs.float().contiguous()
+    call_on(lg, "cin_moe_gate_backward", ptr(lg), dtype_code(lg), max(lg.stride(0), E), T, E, idx.shape[1], score,
+            int(renormalize), scale, ptr(idx.contiguous()), ptr(gw), ptr(gs), ptr(out), stream_of(lg))
+    return out
+
+
+class _MoeGate(torch.autograd.Function):
+    """moe_gate in eager mode, its two launches called directly."""
+
+    @staticmethod
+    def forward(ctx, logits, bias, *options):
+        idx, w, scores = _launch_gate(logits, bias, *options)
+        ctx.save_for_backward(logits, idx)
+        ctx.options = options
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(*((idx,) if options[-1] else (idx, scores)))
+        return idx, w, scores
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, _gidx, gw, gs):
+        if gw is None and gs is None:
+            return (None,) * 10
+        _k, score, _g, _tg, _gt, renormalize, scale, _rs = ctx.options
+        return (_launch_gate_backward(*ctx.saved_tensors, gw, gs, score, renormalize, scale),) + (None,) * 9
+
+
+@custom_op("moe_gate", "(Tensor logits, Tensor? bias, int top_k, int score, int n_groups, int top_groups, int group_top, "
+           "bool renormalize, float scale, bool return_scores) -> (Tensor, Tensor, Tensor)")
+def _gate_op(logits, bias, *options):
+    # without return_scores the last output is an empty placeholder
+    return _launch_gate(logits, bias, *options)
+
+
+@_gate_op.register_fake
+def _(logits, bias, top_k, score, n_groups, top_groups, group_top, renormalize, scale, return_scores):
+    T, E = logits.shape
+    return (logits.new_empty((T, top_k), dtype=torch.int64), logits.new_empty((T, top_k), dtype=torch.float32),
+            logits.new_empty((T, E) if return_scores else (0,), dtype=torch.float32))
+
+
+@custom_op("moe_gate_backward", "(Tensor logits, Tensor idx, Tensor gw, Tensor? gs, int score, bool renormalize, "
+           "float scale) -> Tensor")
+def _gate_bwd_op(logits, idx, gw, gs, score, renormalize, scale):
+    return _launch_gate_backward(logits, idx, gw, gs, score, renormalize, scale)
+
+
+@_gate_bwd_op.register_fake
+def _(logits, idx, gw, gs, score, renormalize, scale):
+    return logits.new_empty(logits.shape)
+
+
+def _gate_setup(ctx, inputs, output):
+    logits, _bias, _k, score, _g, _tg, _gt, renormalize, scale, return_scores = inputs
+    idx, _w, scores = output
+    ctx.save_for_backward(logits, idx)
+    ctx.mark_non_differentiable(*((idx,) if return_scores else (idx, scores)))
+    ctx.options = score, renormalize, scale, return_scores
+
+
+def _gate_backward(ctx, _gidx, gw, gs):
+    logits, idx = ctx.saved_tensors
+    score, renormalize, scale, return_scores = ctx.options
+    dz = _gate_bwd_op(logits, idx, gw, gs if return_scores else None, score, renormalize, scale)
+    return (dz,) + (None,) * 9
+
+
+_gate_op.register_autograd(_gate_backward, setup_context=_gate_setup)
 
 
 # ---------------------------------------------------------------------------

@@ -512,6 +512,46 @@ int cin_moe_combine_backward(const float* dout, int64_t sdm, const void* y, int 
                              const int32_t* inv, int64_t T, int64_t k, int64_t A, int64_t N,
                              void* dy, int dy_dtype, int64_t sdym, float* dscores, void* stream);
 
+/*
+ * The experts' gate (reference src/layers.py:122-126): scores s = sigmoid (score 0) or softmax
+ * (score 1) of a token's E logits, choices s + bias (bias [E] fp32 or null), experts outside the
+ * best top_groups of `groups` groups of E / groups neighbours left out (a group counts by the sum
+ * of its group_top, 1 or 2, largest choices), then the k largest choices, falling, ties to the
+ * lowest index; compared in 64 bits, NaN as the greatest.
+ *   logits [T, E] of dtype, row stride ldl; idx [T, k] int64; weights [T, k] fp32 =
+ *   scale * s[idx], with renormalize divided by (their sum + 1e-9); scores [T, E] fp32 or null.
+ * E <= 4096, k <= 16 and within the kept groups, groups <= 64.
+ */
+int cin_moe_gate(const void* logits, int dtype, int64_t ldl, const float* bias, int64_t T, int64_t E,
+                 int64_t k, int score, int64_t groups, int64_t top_groups, int group_top,
+                 int renormalize, float scale, int64_t* idx, float* weights, float* scores,
+                 void* stream);
+
+/*
+ * Gradient of cin_moe_gate's logits from those of its weights [T, k] and scores [T, E] (fp32,
+ * either null for none); idx as the forward returned it; dlogits [T, E] of dtype, contiguous.
+ */
+int cin_moe_gate_backward(const void* logits, int dtype, int64_t ldl, int64_t T, int64_t E, int64_t k,
+                          int score, int renormalize, float scale, const int64_t* idx,
+                          const float* gweights, const float* gscores, void* dlogits, void* stream);
+
+/*
+ * Rotary positions (reference src/attention.py:9-128): the channel pairs of [start, start + rot)
+ * of q [B, L, H, D] and k [B, L, Hk, D] turned by the angle of the token's position,
+ *   y0 = x0 cos - x1 sin, y1 = x0 sin + x1 cos    (inverse: sin negated, the gradient),
+ * pairs (2i, 2i + 1) if interleaved, else (i, i + rot / 2); the other channels copied.  cos and
+ * sin [P, rot / 2] fp32 with row stride ldt; positions int64 with strides (spb, spl), or null for
+ * 0 .. L - 1 (L <= P).  A token at a negative position is copied as it is, one at P or beyond
+ * gives NaN in its rotated channels.  Batch, token and head strides per tensor, channels adjacent;
+ * H or Hk may be 0.  Outputs must not overlap the inputs.
+ */
+int cin_rotary(const void* q, int64_t sqb, int64_t sql, int64_t sqh, void* q_out, int64_t soqb,
+               int64_t soql, int64_t soqh, int64_t H, const void* k, int64_t skb, int64_t skl,
+               int64_t skh, void* k_out, int64_t sokb, int64_t sokl, int64_t sokh, int64_t Hk,
+               int dtype, int64_t B, int64_t L, int64_t D, const float* cos, const float* sin,
+               int64_t P, int64_t ldt, int64_t rot, int64_t start, const int64_t* positions,
+               int64_t spb, int64_t spl, int interleaved, int inverse, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
