@@ -1,0 +1,810 @@
+// Output projection and softmax cross entropy over a large vocabulary on gfx950, without keeping
+// the logits.
+//
+//   z[t, v]  = x[t] . w[v]                 loss_t = log(sum_v exp(z[t, v])) - z[t, y_t]
+//   dz[t, v] = g_t (exp(z[t, v] - max_t) / total_t - [v = y_t])
+//   dx       = dz w                        dw = dz^T x
+//
+// Rows whose target is ignore_index are taken out first (x is copied without them), so that no
+// product runs over them.  Forward: one product whose tiles leave only each row's maximum and sum
+// of exponentials and the target's logit.  Backward: by pieces of the vocabulary, a product that
+// ends in dz of the piece (in x's type), then dx += dz w and dw = dz^T x of the piece.
+//
+// One kernel runs the three products, on the matrix units in x's type (bf16, fp16 or fp32) with
+// fp32 sums.  An operand is read along K (its rows hold K) or across it (its rows are K), so no
+// transposed copy of x, w or dz is ever made.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "cin_common.h"
+#include "cin_gemm_tile.h"
+#include "cin_grouped.h"
+#include "cin_runtime.h"
+
+using namespace cin;
+
+namespace {
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr uint32_t kOut = 0x80000000u;  // an out-of-range lane offset
+
+typedef unsigned int v4u __attribute__((ext_vector_type(4)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+
+template <int DT>
+constexpr int kEs = DT == CIN_DT_F32 ? 4 : 2;
+
+// Workgroup tile of 16 MT WM x 16 NT WN, K steps of 128 bytes.
+template <int WM_, int WN_, int MT_, int NT_>
+struct Cfg {
+  static constexpr int WM = WM_, WN = WN_, MT = MT_, NT = NT_;
+  static constexpr int kThreads = 64 * WM * WN, TM = 16 * MT * WM, TN = 16 * NT * WN;
+  static constexpr int kStage = (TM + TN) * 128;
+  static constexpr int kCStride = TN * 2 + 16;  // a staged row of 16-bit results; rows 4 banks apart
+  static constexpr int kBytes = 2 * kStage > TM * kCStride ? 2 * kStage : TM * kCStride;
+};
+
+// What a product ends in.
+enum Epi {
+  kStats,  // the row's maximum and sum of exponentials over the tile, and the target's logit
+  kGrad,   // dz, in the operands' type
+  kSlab,   // fp32 partial sums (added to what is there with `add`)
+  kFinal   // times a device scalar, in the operands' type
+};
+
+struct GemmArgs {
+  const void *A, *B;
+  int64_t lda, ldb;
+  int64_t M, N, K;     // N: columns to compute; K: a multiple of a K step where an operand holds K in its rows
+  const int* n;        // rows there are, in place of M (or of K for kFinal)
+  int splits;          // parts of K, one slab each
+  int64_t ldc, slab;   // elements between rows of C, between slabs
+  void* C;
+  int add;
+  int64_t v0, V;       // first column of the piece and columns of the vocabulary
+  int64_t wa, wb;      // columns there are of an operand that is read across K
+  float2* part;        // [T, tiles_n]
+  float* ztarget;
+  const int* target;
+  const float *rowmax, *inv, *coef, *out_scale;
+};
+
+// One operand of ROWS tile rows (of M or N) and a 128-byte K step, moved global -> LDS by DMA.
+// Along K: LDS rows are tile rows of 128 bytes, 16-byte chunk c of row r at slot c ^ f(r).
+// Across K: LDS rows are the step's K rows of ROWS elements, in granules of 16 elements, granule
+// q of row r at q ^ f(r): the rows that one transposing read takes together lie on other banks.
+template <int DT, int ROWS, int THREADS, bool ACROSS>
+struct Operand {
+  static constexpr int es = kEs<DT>, BK = 128 / es;
+  static constexpr int kOps = ROWS * 8 / THREADS;
+  static constexpr int kCpr = ACROSS ? ROWS * es / 16 : 8;  // 16-byte chunks of an LDS row
+  static constexpr int kGc = es;                            // chunks of a granule (across)
+  static constexpr int kGran = kCpr / kGc;
+  static_assert(ROWS * 8 % THREADS == 0, "whole operations");
+  uint32_t voff[kOps];
+  __amdgpu_buffer_rsrc_t rsrc;
+  const uint8_t* p;
+  int64_t ldb, kleft, width;
+  uint32_t lds;
+
+  __device__ static inline int f(int r) {
+    if constexpr (!ACROSS) return swz_f(r);
+    if constexpr (es == 2) return ((r & 3) | ((r >> 3 & 1) << 2)) & (kGran - 1);
+    return (r >> 2) & 3 & (kGran - 1);
+  }
+  // r0: the tile's first row (along) or column (across); valid: rows (along) or columns (across)
+  // from there on; k0, k1: the K range that there is
+  __device__ __forceinline__ void init(const void* base, int64_t ld, int64_t r0, int64_t valid, int64_t k0, int64_t k1,
+                                       int tid, uint32_t lds0) {
+    ldb = ld * es;
+    width = valid * es;
+    lds = lds0 + (uint32_t)__builtin_amdgcn_readfirstlane(tid >> 6) * 1024;
+    kleft = k1 - k0;
+    if constexpr (ACROSS) {
+      p = static_cast<const uint8_t*>(base) + k0 * ldb + r0 * es;
+    } else {
+      const int rows = (int)(valid < ROWS ? valid : ROWS);
+      p = static_cast<const uint8_t*>(base) + r0 * ldb + k0 * es;
+      rsrc = make_rsrc(p, (rows - 1) * ldb + kleft * es);
+    }
+#pragma unroll
+    for (int i = 0; i < kOps; ++i) {
+      const int slot = i * THREADS + tid, r = slot / kCpr, c = slot % kCpr;
+      if constexpr (ACROSS) {
+        voff[i] = (uint32_t)(r * ldb) + (uint32_t)((((c / kGc) ^ f(r)) * kGc + c % kGc) * 16);
+      } else {
+        voff[i] = r < valid ? (uint32_t)(r * ldb) + (uint32_t)((c ^ f(r)) * 16) : kOut;
+      }
+    }
+  }
+  __device__ __forceinline__ void fetch(int kt, uint32_t stage) {
+    uint32_t so = 0;
+    if constexpr (ACROSS) {
+      const int64_t left = kleft - (int64_t)kt * BK;
+      // K rows past the last read as zero, and nothing is read past the last row's end
+      rsrc = make_rsrc(p + (int64_t)kt * BK * ldb, ((left < BK ? left : BK) - 1) * ldb + width);
+    } else {
+      so = (uint32_t)kt * 128;
+    }
+#pragma unroll
+    for (int i = 0; i < kOps; ++i) dma16(rsrc, voff[i], so, lds + stage + i * THREADS * 16);
+  }
+  // 16 bytes a lane: K elements 8 kq .. + 7 of half ks (fp32: 4 kq .. + 3) of tile row r16 + l16
+  __device__ static __forceinline__ v4u frag(const uint8_t* st, int r16, int ks, int l16, int kq) {
+    if constexpr (!ACROSS) {
+      return *reinterpret_cast<const v4u*>(st + (r16 + l16) * 128 + (((4 * ks + kq) ^ f(r16 + l16)) << 4));
+    } else if constexpr (es == 2) {
+      v4u v;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int k = 32 * ks + 8 * kq + 4 * h + (l16 >> 2);
+        const uint8_t* q = st + k * (ROWS * 2) + ((((r16 >> 4)) ^ f(k)) << 5) + (l16 & 3) * 8;
+        const s4 t = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)q);
+        const uint2 u = __builtin_bit_cast(uint2, t);
+        v[2 * h] = u.x;
+        v[2 * h + 1] = u.y;
+      }
+      return v;
+    } else {
+      v4u v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int k = 16 * ks + 4 * kq + e;
+        v[e] = *reinterpret_cast<const uint32_t*>(st + k * (ROWS * 4) + ((((r16 >> 4)) ^ f(k)) << 6) + l16 * 4);
+      }
+      return v;
+    }
+  }
+};
+
+// c += a b over a half step: lane (l16, kq) holds column l16 of b and rows 4 kq .. + 3 of a
+template <int DT>
+__device__ __forceinline__ v4f mma(v4u a, v4u b, v4f c) {
+  if constexpr (DT == CIN_DT_BF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+  if constexpr (DT == CIN_DT_F16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[e]), __uint_as_float(b[e]), c, 0, 0, 0);
+  return c;
+}
+
+__device__ inline float exp_of(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
+
+template <class C, int DT, int EPI>
+__global__ __launch_bounds__(C::kThreads, 2) void k_ce_gemm(GemmArgs g) {
+  constexpr bool kAcrossA = EPI == kFinal, kAcrossB = EPI == kSlab || EPI == kFinal;
+  constexpr int MT = C::MT, NT = C::NT, BK = 128 / kEs<DT>;
+  __shared__ __attribute__((aligned(128))) uint8_t smem[C::kBytes];
+  const int64_t rows = __builtin_amdgcn_readfirstlane(*g.n);
+  const int64_t M = EPI == kFinal ? g.M : rows, Kall = EPI == kFinal ? rows : g.K;
+  const uint32_t tiles_m = (uint32_t)cdiv(M, C::TM), tiles_n = (uint32_t)cdiv(g.N, C::TN);
+  const uint32_t total = tiles_m * tiles_n;
+  if (blockIdx.x >= total) return;
+  uint32_t tm, tn;
+  raster<4>(xcd_remap(blockIdx.x, total), tiles_m, tiles_n, tm, tn);
+  const int64_t m0 = (int64_t)tm * C::TM, n0 = (int64_t)tn * C::TN;
+  int64_t k0 = 0, k1 = Kall;
+  if constexpr (EPI == kSlab) {
+    const int64_t per = cdiv(cdiv(Kall, BK), g.splits) * BK;
+    k0 = blockIdx.y * per;
+    k1 = k0 + per < Kall ? k0 + per : Kall;
+  }
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / C::WN, wn = wave % C::WN;
+  const int l16 = lane & 15, kq = lane >> 4;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)smem;
+  Operand<DT, C::TM, C::kThreads, kAcrossA> oa;
+  Operand<DT, C::TN, C::kThreads, kAcrossB> ob;
+  v4f acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+  const int nk = k1 > k0 ? (int)((k1 - k0 + BK - 1) / BK) : 0;
+  if (nk > 0) {
+    // w has rows up to the vocabulary's end, as tile rows or as K
+    oa.init(g.A, g.lda, m0, (kAcrossA ? g.wa : M) - m0, k0, k1, tid, lds0);
+    ob.init(g.B, g.ldb, n0, (kAcrossB ? g.wb : g.V - g.v0) - n0, k0,
+            EPI == kSlab && k1 > g.V - g.v0 ? g.V - g.v0 : k1, tid, lds0 + C::TM * 128);
+    oa.fetch(0, 0);
+    ob.fetch(0, 0);
+  }
+  for (int kt = 0; kt < nk; ++kt) {
+    wait_dma();
+    lds_barrier();
+    const uint32_t st = (kt & 1) * C::kStage;
+    if (kt + 1 < nk) {
+      oa.fetch(kt + 1, C::kStage - st);
+      ob.fetch(kt + 1, C::kStage - st);
+    }
+    const uint8_t* sa = smem + st;
+    const uint8_t* sb = sa + C::TM * 128;
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      v4u bf[NT];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) bf[j] = ob.frag(sb, (wn * NT + j) * 16, ks, l16, kq);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const v4u af = oa.frag(sa, (wm * MT + i) * 16, ks, l16, kq);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = mma<DT>(bf[j], af, acc[i][j]);
+      }
+    }
+  }
+  lds_barrier();
+  // the lane holds rows m0 + (wm MT + i) 16 + l16, columns n0 + (wn NT + j) 16 + 4 kq + r
+  const int64_t nl = n0 + wn * NT * 16 + 4 * kq;
+  if constexpr (EPI == kStats) {
+    float2* st = reinterpret_cast<float2*>(smem);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const int ml = (wm * MT + i) * 16 + l16;
+      const bool in = m0 + ml < M;
+      const int64_t at = (in ? g.target[m0 + ml] : -1) - nl;
+      float mx = -__builtin_inff();
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (at == j * 16 + r) g.ztarget[m0 + ml] = acc[i][j][r];
+          if (nl + j * 16 + r >= g.N) acc[i][j][r] = -__builtin_inff();
+          mx = fmaxf(mx, acc[i][j][r]);
+        }
+      mx = fmaxf(mx, __shfl_xor(mx, 16));
+      mx = fmaxf(mx, __shfl_xor(mx, 32));
+      float s = 0.0f;
+      // (a wave with no column of the vocabulary, or nothing but -inf, adds nothing)
+      const float ref = mx == -__builtin_inff() ? 0.0f : mx;
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s += exp_of(acc[i][j][r] - ref);
+      s += __shfl_xor(s, 16);
+      s += __shfl_xor(s, 32);
+      if (kq == 0) st[wn * C::TM + ml] = make_float2(mx, s);
+    }
+    __syncthreads();
+    for (int m = tid; m < C::TM; m += C::kThreads) {
+      if (m0 + m >= M) continue;
+      float2 a = st[m];
+      float s = 0.0f;
+#pragma unroll
+      for (int w = 1; w < C::WN; ++w) a.x = fmaxf(a.x, st[w * C::TM + m].x);
+      const float ref = a.x == -__builtin_inff() ? 0.0f : a.x;
+#pragma unroll
+      for (int w = 0; w < C::WN; ++w) s += st[w * C::TM + m].y * exp_of(st[w * C::TM + m].x - ref);
+      g.part[(m0 + m) * tiles_n + tn] = make_float2(a.x, s);
+    }
+    return;
+  }
+  if constexpr (EPI == kSlab) {
+    float* out = static_cast<float*>(g.C) + blockIdx.y * g.slab;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const int64_t m = m0 + (wm * MT + i) * 16 + l16;
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const int64_t n = nl + j * 16;
+        if (m >= M || n >= g.N) continue;  // (N is a multiple of 4)
+        float4* q = reinterpret_cast<float4*>(out + m * g.ldc + n);
+        float4 v = make_float4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
+        if (g.add) {
+          const float4 o = *q;
+          v = make_float4(v.x + o.x, v.y + o.y, v.z + o.z, v.w + o.w);
+        }
+        *q = v;
+      }
+    }
+    return;
+  }
+  const float scale = EPI == kFinal ? *g.out_scale : 1.0f;
+  if constexpr (EPI == kGrad) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const int64_t m = m0 + (wm * MT + i) * 16 + l16;
+      const bool in = m < M;
+      const float mx = in ? g.rowmax[m] : 0.0f, inv = in ? g.inv[m] : 0.0f, cf = in ? g.coef[m] : 0.0f;
+      const int64_t at = (in ? g.target[m] : -1) - g.v0 - nl;
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float p = exp_of(acc[i][j][r] - mx) * inv;
+          // columns past the vocabulary are part of the next products' K
+          acc[i][j][r] = g.v0 + nl + j * 16 + r < g.V ? (at == j * 16 + r ? p - 1.0f : p) * cf : 0.0f;
+        }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[i][j][r] *= scale;
+  }
+  const int64_t N = g.N;
+  if constexpr (DT == CIN_DT_F32) {
+    float* out = static_cast<float*>(g.C);
+    const bool whole = (g.ldc & 3) == 0 && ((uintptr_t)out & 15) == 0;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const int64_t m = m0 + (wm * MT + i) * 16 + l16;
+      if (m >= M) continue;
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const int64_t n = nl + j * 16;
+        if (whole && n + 4 <= N) {
+          *reinterpret_cast<float4*>(out + m * g.ldc + n) = make_float4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (n + r < N) out[m * g.ldc + n + r] = acc[i][j][r];
+        }
+      }
+    }
+  } else {
+    // rows through LDS, so that the stores run along them
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+        *reinterpret_cast<uint2*>(smem + ((wm * MT + i) * 16 + l16) * C::kCStride + ((wn * NT + j) * 16 + kq * 4) * 2) =
+            make_uint2(f32x2_to_half2_bits<DT>(acc[i][j][0], acc[i][j][1]),
+                       f32x2_to_half2_bits<DT>(acc[i][j][2], acc[i][j][3]));
+    __syncthreads();
+    uint16_t* out = static_cast<uint16_t*>(g.C);
+    const bool whole = (g.ldc & 7) == 0 && ((uintptr_t)out & 15) == 0;
+    constexpr int kChunks = C::TN / 8;
+    for (int q = tid; q < C::TM * kChunks; q += C::kThreads) {
+      const int m = q / kChunks, n = (q % kChunks) * 8;
+      if (m0 + m >= M || n0 + n >= N) continue;
+      const v4u v = *reinterpret_cast<const v4u*>(smem + m * C::kCStride + n * 2);
+      uint16_t* d = out + (m0 + m) * g.ldc + n0 + n;
+      if (whole && n0 + n + 8 <= N) {
+        *reinterpret_cast<v4u*>(d) = v;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (n0 + n + e < N) d[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Rows
+// ---------------------------------------------------------------------------
+constexpr int kRowThreads = 1024, kRowPer = 8;
+
+// The rows that count, in order: map[i] the row, target[i] its target (-1 outside the vocabulary),
+// pos[t] = i or -1 for an ignored row (whose loss is 0), n their number.  One workgroup.
+__global__ __launch_bounds__(kRowThreads) void k_ce_rows(const int64_t* __restrict__ y, int64_t T, int64_t V, int64_t ignore,
+                                                         int* __restrict__ map, int* __restrict__ pos,
+                                                         int* __restrict__ target, int* __restrict__ n,
+                                                         float* __restrict__ rowloss) {
+  __shared__ int wsum[kRowThreads / 64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int base = 0;
+  for (int64_t t0 = 0; t0 < T; t0 += kRowThreads * kRowPer) {
+    const int64_t first = t0 + (int64_t)tid * kRowPer;
+    int64_t v[kRowPer];
+    int mine = 0;
+#pragma unroll
+    for (int j = 0; j < kRowPer; ++j) {
+      v[j] = first + j < T ? y[first + j] : ignore;
+      mine += v[j] != ignore;
+    }
+    int incl = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(incl, d);
+      if (lane >= d) incl += o;
+    }
+    if (lane == 63) wsum[wave] = incl;
+    __syncthreads();
+    int before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < kRowThreads / 64; ++w) {
+      if (w < wave) before += wsum[w];
+      all += wsum[w];
+    }
+    int i = base + before + incl - mine;
+#pragma unroll
+    for (int j = 0; j < kRowPer; ++j) {
+      if (first + j >= T) break;
+      if (v[j] == ignore) {
+        pos[first + j] = -1;
+        rowloss[first + j] = 0.0f;
+      } else {
+        map[i] = (int)(first + j);
+        target[i] = v[j] >= 0 && v[j] < V ? (int)v[j] : -1;
+        pos[first + j] = i++;
+      }
+    }
+    base += all;
+    __syncthreads();
+  }
+  if (tid == 0) *n = base;
+}
+
+// Rows of x (all, or map's first *n) with zeros up to Dp columns.
+template <int ES>
+__global__ __launch_bounds__(256) void k_ce_copy(const void* __restrict__ x, int64_t ldx, int64_t rows, int64_t D,
+                                                 const int* __restrict__ map, const int* __restrict__ n,
+                                                 void* __restrict__ out, int64_t Dp) {
+  using E = std::conditional_t<ES == 4, uint32_t, uint16_t>;
+  constexpr int kPer = 16 / ES;
+  const int64_t pieces = Dp / kPer, have = n ? *n : rows;
+  const bool whole = ((uintptr_t)x & 15) == 0 && ldx % kPer == 0;
+  for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < have * pieces; q += (int64_t)gridDim.x * 256) {
+    const int64_t i = q / pieces, c = (q - i * pieces) * kPer;
+    const E* s = static_cast<const E*>(x) + (map ? (int64_t)map[i] : i) * ldx + c;
+    E* d = static_cast<E*>(out) + i * Dp + c;
+    if (whole && c + kPer <= D) {
+      *reinterpret_cast<v4u*>(d) = *reinterpret_cast<const v4u*>(s);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) d[e] = c + e < D ? s[e] : (E)0;
+    }
+  }
+}
+
+// A wave per row: the tiles' maxima and sums joined, the row's loss (NaN for a target outside the
+// vocabulary).
+__global__ __launch_bounds__(256) void k_ce_join(const float2* __restrict__ part, int tiles, const int* __restrict__ n,
+                                                 const int* __restrict__ map, const int* __restrict__ target,
+                                                 const float* __restrict__ ztarget, float* __restrict__ rowmax,
+                                                 float* __restrict__ inv, float* __restrict__ rowloss) {
+  const int lane = threadIdx.x & 63;
+  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (i >= *n) return;
+  float m = -__builtin_inff(), s = 0.0f;
+  for (int t = lane; t < tiles; t += 64) m = fmaxf(m, part[i * tiles + t].x);
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+  for (int t = lane; t < tiles; t += 64) {
+    const float2 p = part[i * tiles + t];
+    s += p.y * exp_of(p.x - m);
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) s += __shfl_xor(s, o);
+  if (lane == 0) {
+    rowmax[i] = m;
+    inv[i] = 1.0f / s;
+    rowloss[map[i]] = target[i] < 0 ? __builtin_nanf("") : (m - ztarget[i]) + logf(s);
+  }
+}
+
+// Sum of a value a thread over the workgroup, in 64 bits.
+__device__ inline double block_sum(double v) {
+  __shared__ double w[16];
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
+  if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = v;
+  __syncthreads();
+  double s = 0;
+  for (int i = 0; i < (int)blockDim.x / 64; ++i) s += w[i];
+  __syncthreads();
+  return s;
+}
+
+// The rows' sum, over their number with `mean` (0 / 0 is NaN).
+__global__ __launch_bounds__(1024) void k_ce_loss(const float* __restrict__ rowloss, int64_t T, const int* __restrict__ n,
+                                                  int mean, float* __restrict__ loss) {
+  double s = 0;
+  for (int64_t t = threadIdx.x; t < T; t += 1024) s += rowloss[t];
+  s = block_sum(s);
+  if (threadIdx.x == 0) *loss = (float)(mean ? s / *n : s);
+}
+
+// What dz is scaled by: coef[i] = g_i 2^a with all products in range (fp16 holds 2^-24 .. 65504,
+// and p - 1 lies in [-1, 1]: top 2^15), and out_scale = 2^-a times what all rows share.  A gradient
+// shared by all rows (stride 0) stays out of coef.  One workgroup.
+__global__ __launch_bounds__(1024) void k_ce_coef(const float* __restrict__ grad, int64_t stride, int mean, int half,
+                                                  const int* __restrict__ n, const int* __restrict__ map,
+                                                  const int* __restrict__ target, float* __restrict__ coef,
+                                                  float* __restrict__ out_scale) {
+  __shared__ float wmax[16];
+  const int rows = *n;
+  const float top = half ? 32768.0f : 1.0f;
+  float s = top, out = 1.0f / top;
+  if (stride == 0) {
+    out *= mean ? grad[0] / (float)rows : grad[0];
+  } else {
+    float m = 0.0f;
+    for (int i = threadIdx.x; i < rows; i += 1024) m = fmaxf(m, fabsf(grad[(int64_t)map[i] * stride]));
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+    if ((threadIdx.x & 63) == 0) wmax[threadIdx.x >> 6] = m;
+    __syncthreads();
+    for (int w = 0; w < 16; ++w) m = fmaxf(m, wmax[w]);
+    if (m > 0.0f && m < __builtin_inff()) {
+      int e;
+      frexpf(m, &e);  // m <= 2^e
+      e = e < -100 ? -100 : (e > 100 ? 100 : e);
+      s = ldexpf(top, -e);
+      out = ldexpf(1.0f / top, e);
+    }
+  }
+  for (int i = threadIdx.x; i < rows; i += 1024) {
+    const float g = stride == 0 ? s : grad[(int64_t)map[i] * stride] * s;
+    coef[i] = target[i] < 0 ? __builtin_nanf("") : g;
+  }
+  if (threadIdx.x == 0) *out_scale = rows ? out : 0.0f;
+}
+
+// dx[t] = out_scale * the sum of the slabs' row pos[t], zero for an ignored row.
+template <int DT>
+__global__ __launch_bounds__(256) void k_ce_dx(const float* __restrict__ slabs, int64_t slab, int splits, int64_t Dp,
+                                               const int* __restrict__ pos, const float* __restrict__ out_scale,
+                                               int64_t T, int64_t D, void* __restrict__ dx) {
+  const float scale = *out_scale;
+  const int64_t pieces = Dp / 4;
+  const bool whole = D % 4 == 0;
+  for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < T * pieces; q += (int64_t)gridDim.x * 256) {
+    const int64_t t = q / pieces, c = (q - t * pieces) * 4;
+    if (c >= D) continue;
+    const int i = pos[t];
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (i >= 0) {
+      for (int s = 0; s < splits; ++s) {
+        const float4 b = *reinterpret_cast<const float4*>(slabs + s * slab + i * Dp + c);
+        a = make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
+      }
+    }
+    const float v[4] = {a.x * scale, a.y * scale, a.z * scale, a.w * scale};
+    const int64_t at = t * D + c;
+    if constexpr (DT == CIN_DT_F32) {
+      float* d = static_cast<float*>(dx) + at;
+      if (whole)
+        *reinterpret_cast<float4*>(d) = make_float4(v[0], v[1], v[2], v[3]);
+      else
+        for (int e = 0; e < 4; ++e)
+          if (c + e < D) d[e] = v[e];
+    } else {
+      uint16_t* d = static_cast<uint16_t*>(dx) + at;
+      const uint2 h = make_uint2(f32x2_to_half2_bits<DT>(v[0], v[1]), f32x2_to_half2_bits<DT>(v[2], v[3]));
+      if (whole)
+        *reinterpret_cast<uint2*>(d) = h;
+      else
+        for (int e = 0; e < 4; ++e)
+          if (c + e < D) d[e] = (uint16_t)((e < 2 ? h.x : h.y) >> (16 * (e & 1)));
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------
+using Big = Cfg<2, 4, 8, 4>;  // 256 x 256, 8 waves of 128 x 64
+
+constexpr int64_t kMaxT = (int64_t)1 << 30, kMaxV = (int64_t)1 << 30, kMaxD = (int64_t)1 << 18;
+constexpr int64_t kPieceBytes = (int64_t)1 << 30;  // dz of one piece
+constexpr int64_t kMaxPiece = (int64_t)1 << 20;    // its columns: 256 rows lie within 2^31 bytes
+
+int64_t align_up(int64_t v, int64_t a) { return cdiv(v, a) * a; }
+
+struct Plan {
+  int es;
+  int64_t Dp;           // columns of x and w as the products read them
+  int64_t tiles_n;      // column tiles of the forward product
+  int64_t piece, ldz;   // columns of a piece, elements between rows of dz
+  int splits;           // slabs of dx
+  // bytes
+  int64_t part, ztarget, dz, slabs, coef;
+};
+
+Plan make_plan(int dtype, int64_t T, int64_t D, int64_t V) {
+  Plan p;
+  p.es = dtype == CIN_DT_F32 ? 4 : 2;
+  p.Dp = align_up(D, 128 / p.es);
+  p.tiles_n = cdiv(V, Big::TN);
+  const int64_t Tp = T > 0 ? T : 1;
+  int64_t most = align_up(kPieceBytes / (Tp * p.es) + 1, Big::TN);
+  if (most > kMaxPiece) most = kMaxPiece;
+  const int64_t pieces = cdiv(V, most);
+  p.piece = align_up(cdiv(V, pieces), Big::TN);
+  p.ldz = p.piece + 64;  // rows not a multiple of 16 KiB apart
+  const int64_t tiles = cdiv(Tp, Big::TM) * cdiv(p.Dp, Big::TN);
+  int64_t s = tiles >= 192 ? 1 : 256 / tiles;
+  const int64_t steps = p.piece * p.es / 128;
+  if (s > steps / 8) s = steps / 8;
+  p.splits = (int)(s < 1 ? 1 : s);
+  p.part = align_up(Tp * p.tiles_n * 8, 256);
+  p.ztarget = align_up(Tp * 4, 256);
+  p.dz = align_up(Tp * p.ldz * p.es, 256);
+  p.slabs = align_up(p.splits * Tp * p.Dp * 4, 256);
+  p.coef = align_up((Tp + 1) * 4, 256);
+  return p;
+}
+
+int check(const char* name, int dtype, int64_t T, int64_t D, int64_t V) {
+  CIN_CHECK_ARG(dtype == CIN_DT_BF16 || dtype == CIN_DT_F32 || dtype == CIN_DT_F16, "%s: bad dtype %d", name, dtype);
+  CIN_CHECK_ARG(T >= 0 && T < kMaxT, "%s: T must be in [0, 2^30)", name);
+  CIN_CHECK_ARG(V >= 1 && V < kMaxV, "%s: V must be in [1, 2^30)", name);
+  CIN_CHECK_ARG(D >= 1 && D <= kMaxD, "%s: D must be in [1, 2^18]", name);
+  CIN_CHECK_ARG(cdiv(T, 256) * cdiv(V, 256) < ((int64_t)1 << 31), "%s: T x V is too large", name);
+  return CIN_OK;
+}
+
+bool w_fits(const void* w, int dtype, int64_t ldw) {
+  const int es = dtype == CIN_DT_F32 ? 4 : 2;
+  return ((uintptr_t)w & 15) == 0 && ldw * es % 16 == 0 && ldw <= 4 * kMaxD;
+}
+
+template <class F>
+void with_dtype(int dtype, F f) {
+  if (dtype == CIN_DT_F32)
+    f(std::integral_constant<int, CIN_DT_F32>{});
+  else if (dtype == CIN_DT_F16)
+    f(std::integral_constant<int, CIN_DT_F16>{});
+  else
+    f(std::integral_constant<int, CIN_DT_BF16>{});
+}
+
+template <int EPI>
+void gemm(int dtype, const GemmArgs& g, int64_t max_m, hipStream_t s) {
+  with_dtype(dtype, [&](auto dt) {
+    const int64_t tiles = cdiv(max_m, Big::TM) * cdiv(g.N, Big::TN);
+    hipLaunchKernelGGL((k_ce_gemm<Big, dt(), EPI>), dim3((unsigned)tiles, (unsigned)g.splits), Big::kThreads, 0, s, g);
+  });
+}
+
+void copy_rows(int es, const void* x, int64_t ldx, int64_t rows, int64_t D, const int* map, const int* n, void* out,
+               int64_t Dp, hipStream_t s) {
+  const int64_t blocks = cdiv(rows * (Dp * es / 16), 256);
+  const unsigned grid = (unsigned)(blocks < 8192 ? blocks : 8192);
+  if (es == 4)
+    hipLaunchKernelGGL(k_ce_copy<4>, grid, 256, 0, s, x, ldx, rows, D, map, n, out, Dp);
+  else
+    hipLaunchKernelGGL(k_ce_copy<2>, grid, 256, 0, s, x, ldx, rows, D, map, n, out, Dp);
+}
+
+// The int32 state: n, then map, pos and target of T entries each.
+struct IntState {
+  int *n, *map, *pos, *target;
+  IntState(int32_t* p, int64_t T) : n(p), map(p + 4), pos(map + T), target(pos + T) {}
+};
+
+}  // namespace
+
+extern "C" {
+
+int64_t cin_linear_ce_workspace(int dtype, int64_t T, int64_t D, int64_t V, int backward) {
+  if (check("linear_ce_workspace", dtype, T, D, V)) return -1;
+  const Plan p = make_plan(dtype, T, D, V);
+  return backward ? p.dz + p.slabs + p.coef : p.part + p.ztarget;
+}
+
+int cin_linear_ce_forward(const void* x, int dtype, int64_t T, int64_t D, int64_t ldx, const void* w, int64_t V,
+                          int64_t ldw, const int64_t* target, int64_t ignore_index, int mean, void* xc, void* wp,
+                          int32_t* state_i, float* state_f, float* rowloss, float* loss, void* workspace,
+                          int64_t workspace_bytes, void* stream) {
+  const char* name = "linear_ce_forward";
+  if (int rc = check(name, dtype, T, D, V)) return rc;
+  CIN_CHECK_ARG(ldx >= D && ldw >= D, "%s: rows overlap", name);
+  CIN_CHECK_ARG(state_i && w && (T == 0 || (x && target && xc && state_f && rowloss)), "%s: null pointer", name);
+  const Plan p = make_plan(dtype, T, D, V);
+  CIN_CHECK_ARG(wp || (w_fits(w, dtype, ldw) && p.Dp == D), "%s: w needs a padded copy", name);
+  CIN_CHECK_ARG(workspace_bytes >= p.part + p.ztarget && workspace, "%s: workspace needs %lld bytes", name,
+                (long long)(p.part + p.ztarget));
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const IntState st(state_i, T);
+  float2* part = static_cast<float2*>(workspace);
+  float* zt = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.part);
+  hipLaunchKernelGGL(k_ce_rows, 1, kRowThreads, 0, s, target, T, V, ignore_index, st.map, st.pos, st.target, st.n, rowloss);
+  if (T > 0) {
+    copy_rows(p.es, x, ldx, T, D, st.map, st.n, xc, p.Dp, s);
+    if (wp) copy_rows(p.es, w, ldw, V, D, nullptr, nullptr, wp, p.Dp, s);
+    GemmArgs g{};
+    g.A = xc;
+    g.lda = p.Dp;
+    g.B = wp ? wp : w;
+    g.ldb = wp ? p.Dp : ldw;
+    g.N = g.V = V;
+    g.K = p.Dp;
+    g.n = st.n;
+    g.splits = 1;
+    g.part = part;
+    g.ztarget = zt;
+    g.target = st.target;
+    gemm<kStats>(dtype, g, T, s);
+    hipLaunchKernelGGL(k_ce_join, (unsigned)cdiv(T, 4), 256, 0, s, part, (int)p.tiles_n, st.n, st.map, st.target, zt,
+                       state_f, state_f + T, rowloss);
+  }
+  if (loss) hipLaunchKernelGGL(k_ce_loss, 1, 1024, 0, s, rowloss, T, st.n, mean, loss);
+  return cin_check_launch(name);
+}
+
+int cin_linear_ce_backward(const void* xc, int dtype, int64_t T, int64_t D, const void* w, int64_t V, int64_t ldw,
+                           const int32_t* state_i, const float* state_f, const float* grad, int64_t grad_stride,
+                           int mean, void* dx, void* dw, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* name = "linear_ce_backward";
+  if (int rc = check(name, dtype, T, D, V)) return rc;
+  const Plan p = make_plan(dtype, T, D, V);
+  CIN_CHECK_ARG(w_fits(w, dtype, ldw) && ldw >= p.Dp, "%s: w's rows must be padded as the forward's", name);
+  CIN_CHECK_ARG(grad_stride >= 0, "%s: negative gradient stride", name);
+  CIN_CHECK_ARG(T > 0 && state_i && state_f && xc && w && grad, "%s: null pointer", name);
+  CIN_CHECK_ARG(workspace && workspace_bytes >= p.dz + p.slabs + p.coef, "%s: workspace needs %lld bytes", name,
+                (long long)(p.dz + p.slabs + p.coef));
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const IntState st(const_cast<int32_t*>(state_i), T);
+  char* ws = static_cast<char*>(workspace);
+  void* dz = ws;
+  float* slabs = reinterpret_cast<float*>(ws + p.dz);
+  float* out_scale = reinterpret_cast<float*>(ws + p.dz + p.slabs);
+  float* coef = out_scale + 1;
+  hipLaunchKernelGGL(k_ce_coef, 1, 1024, 0, s, grad, grad_stride, mean, dtype == CIN_DT_F16, st.n, st.map, st.target, coef,
+                     out_scale);
+  const char* wb = static_cast<const char*>(w);
+  for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
+    const int64_t cols = v0 + p.piece < V ? p.piece : V - v0;
+    GemmArgs g{};
+    g.A = xc;
+    g.lda = p.Dp;
+    g.B = wb + v0 * ldw * p.es;
+    g.ldb = ldw;
+    g.N = align_up(cols, 128 / p.es);  // with the zeros that fill the next product's last K step
+    g.K = p.Dp;
+    g.n = st.n;
+    g.splits = 1;
+    g.C = dz;
+    g.ldc = p.ldz;
+    g.v0 = v0;
+    g.V = V;
+    g.target = st.target;
+    g.rowmax = state_f;
+    g.inv = state_f + T;
+    g.coef = coef;
+    gemm<kGrad>(dtype, g, T, s);
+    GemmArgs h{};
+    h.n = st.n;
+    h.A = dz;
+    h.lda = p.ldz;
+    h.wa = p.ldz;
+    h.wb = p.Dp;
+    h.v0 = v0;
+    h.V = V;
+    if (dx) {
+      h.B = g.B;
+      h.ldb = ldw;
+      h.N = p.Dp;
+      h.K = g.N;
+      h.splits = p.splits;
+      h.C = slabs;
+      h.ldc = p.Dp;
+      h.slab = T * p.Dp;
+      h.add = v0 > 0;
+      gemm<kSlab>(dtype, h, T, s);
+    }
+    if (dw) {
+      h.B = xc;
+      h.ldb = p.Dp;
+      h.M = cols;
+      h.N = D;
+      h.splits = 1;
+      h.C = static_cast<char*>(dw) + v0 * D * p.es;
+      h.ldc = D;
+      h.out_scale = out_scale;
+      gemm<kFinal>(dtype, h, cols, s);
+    }
+  }
+  if (dx) {
+    const int64_t blocks = cdiv(T * (p.Dp / 4), 256);
+    with_dtype(dtype, [&](auto dt) {
+      hipLaunchKernelGGL(k_ce_dx<dt()>, (unsigned)(blocks < 16384 ? blocks : 16384), 256, 0, s, slabs, T * p.Dp, p.splits,
+                         p.Dp, st.pos, out_scale, T, D, dx);
+    });
+  }
+  return cin_check_launch(name);
+}
+
+}  // extern "C"

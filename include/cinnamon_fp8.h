@@ -552,6 +552,33 @@ int cin_rotary(const void* q, int64_t sqb, int64_t sql, int64_t sqh, void* q_out
                int64_t P, int64_t ldt, int64_t rot, int64_t start, const int64_t* positions,
                int64_t spb, int64_t spl, int interleaved, int inverse, void* stream);
 
+/*
+ * Output projection and softmax cross entropy without keeping the logits (reference src/model.py,
+ * lm_head, and the cross entropy of src/train.py:355-372): for rows t whose target y_t is not
+ * ignore_index, loss_t = log sum_v exp(x_t . w_v) - x_t . w_{y_t}; an ignored row's loss is 0, a
+ * target outside [0, V) gives NaN.
+ *   x [T, D] (row stride ldx) and w [V, D] (row stride ldw) of dtype; target [T] int64.
+ *   rowloss [T] fp32; loss [1] fp32 or null: their sum, with mean over the rows that count.
+ * For the backward the forward fills xc [T, Dp] of dtype, state_i [4 + 3 T] int32 and state_f
+ * [2 T] fp32, Dp = D rounded up to 128 bytes; and wp [V, Dp] of dtype, a padded copy of w that is
+ * needed (else null) where Dp != D or w's rows do not start on 16 bytes.
+ *   workspace: cin_linear_ce_workspace(dtype, T, D, V, backward) bytes, 16-byte aligned (-1 for
+ *   sizes that are refused).
+ * Backward: w and ldw as the products read them (wp and Dp where there is a copy); grad fp32, of
+ * the loss (grad_stride 0, with mean divided by the rows that count) or of each row (grad_stride
+ * elements apart); dx [T, D] and dw [V, D] of dtype, contiguous, either null.  Gradients are
+ * bit-identical from call to call.
+ */
+int64_t cin_linear_ce_workspace(int dtype, int64_t T, int64_t D, int64_t V, int backward);
+int cin_linear_ce_forward(const void* x, int dtype, int64_t T, int64_t D, int64_t ldx, const void* w,
+                          int64_t V, int64_t ldw, const int64_t* target, int64_t ignore_index, int mean,
+                          void* xc, void* wp, int32_t* state_i, float* state_f, float* rowloss,
+                          float* loss, void* workspace, int64_t workspace_bytes, void* stream);
+int cin_linear_ce_backward(const void* xc, int dtype, int64_t T, int64_t D, const void* w, int64_t V,
+                           int64_t ldw, const int32_t* state_i, const float* state_f, const float* grad,
+                           int64_t grad_stride, int mean, void* dx, void* dw, void* workspace,
+                           int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,430 @@
+"""lm_head.linear_cross_entropy against its definition in 64 bits (GPU), and its refusals (CPU).
+
+Tolerances.  u = 2^-24, step = half a step of the type (bf16 2^-8, fp16 2^-11, fp32 u).
+  logits     fp32 sums of D exact products: within D u S, S = sum_d |x_d w_d|, e = D u max S
+  loss       2 e (maximum and target's logit), and 64 u for the exponentials, their sum and the log
+  dz         its own rounding, step |dz|, and p (2 e + 16 u + 64 u); fp16 is scaled so that the
+             largest row gradient tops 2^15: what lies under fp16's least number is off by 2^-39 of it
+  dx, dw     the sum of dz's errors times |w| or |x|, K u sum |dz w| for K fp32 additions, and the
+             output's rounding
+These hold for each value in the worst case.  Roundings point both ways, so over a whole tensor the
+norm of the error stays under that of one rounding to the type and of sqrt(K) fp32 ones: twice the
+step (one for dz, one for the output), and 4 sqrt(K + D) u.
+"""
+import math
+
+import pytest
+import torch
+import torch.nn.functional as F
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+from cinnamon_amd import _lib, lm_head
+
+U = 2.0 ** -24
+DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+STEP = {"bf16": 2.0 ** -8, "fp16": 2.0 ** -11, "fp32": U}
+LEAST = {"bf16": 1e-37, "fp16": 2.0 ** -24, "fp32": 1e-37}
+
+
+def reference(x, w, y, ignore=-100, reduction="mean", grad=None):
+    """loss, dx, dw in 64 bits and the worst-case error of each value."""
+    dt = {v: k for k, v in DT.items()}[x.dtype]
+    x, w, y = x.detach().double(), w.detach().double(), y.reshape(-1).long()
+    x = x.reshape(-1, x.shape[-1])
+    (T, D), V = x.shape, w.shape[0]
+    kept = y != ignore
+    n = int(kept.sum())
+    z = x @ w.t()
+    e = D * U * (x.abs() @ w.abs().t()).amax(1, keepdim=True)
+    lse = torch.logsumexp(z, 1, keepdim=True)
+    at = torch.where(kept, y, 0)[:, None]
+    rows = torch.where(kept, (lse - z.gather(1, at))[:, 0], 0)
+    rtol = torch.where(kept, 2 * e[:, 0] + 64 * U + 2 * U * rows, 0)
+    loss = {"none": rows, "sum": rows.sum(), "mean": rows.sum() / n if n else torch.tensor(math.nan)}[reduction]
+    ltol = {"none": rtol, "sum": rtol.sum(), "mean": rtol.sum() / max(n, 1)}[reduction]
+    g = torch.ones(T, dtype=torch.float64, device=x.device) if grad is None else grad.double().reshape(-1).expand(T)
+    g = torch.where(kept, g, 0) / (max(n, 1) if reduction == "mean" else 1)
+    p = torch.exp(z - lse)
+    dz = p.scatter_add(1, at, -torch.ones_like(at, dtype=torch.float64)) * g[:, None]
+    dz_err = STEP[dt] * dz.abs() + p * g.abs()[:, None] * (2 * e + 80 * U) + 4 * U * dz.abs()
+    if dt == "fp16":
+        dz_err = dz_err + 2.0 ** -39 * g.abs().max()
+    dz_err = torch.where(kept[:, None], dz_err, 0)
+    dx, dw = dz @ w, dz.t() @ x
+    dx_tol = dz_err @ w.abs() + V * U * (dz.abs() @ w.abs()) + STEP[dt] * dx.abs()
+    dw_tol = dz_err.t() @ x.abs() + T * U * (dz.abs().t() @ x.abs()) + STEP[dt] * dw.abs()
+    return (loss, ltol), (dx, dx_tol), (dw, dw_tol)
+
+
+def near(got, ref, tol, dt, K):
+    got = got.detach().double().reshape(ref.shape)
+    assert torch.isfinite(got).all()
+    d = (got - ref).abs()
+    bound = 1.01 * tol + LEAST[dt]
+    assert (d <= bound).all(), (d / bound).max().item()
+    norm = 2 * STEP[dt] + 4 * math.sqrt(K) * U
+    assert d.norm() <= norm * ref.norm() + LEAST[dt] * math.sqrt(d.numel()), (d.norm() / ref.norm()).item()
+
+
+def make(T, V, D, dt, ignored, dev, seed=1, ignore=-100):
+    g = torch.Generator().manual_seed(seed)
+    w = torch.randn(V, D, generator=g) * (2 / math.sqrt(D))
+    y = torch.randint(0, V, (T,), generator=g)
+    x = torch.randn(T, D, generator=g) + torch.rand(T, 1, generator=g) * 2 * w[y]
+    y = torch.where(torch.rand(T, generator=g) < ignored, ignore, y)
+    return x.to(DT[dt]).to(dev), w.to(DT[dt]).to(dev), y.to(dev), g
+
+
+SHAPES = [
+    # T, V, D, ignored
+    (1, 1, 1, 0.0), (1, 1000, 64, 0.0), (2, 7, 130, 0.0), (16, 3201, 96, 0.0), (65, 64, 8, 0.3), (255, 257, 64, 0.0),
+    (257, 513, 129, 0.5), (300, 2049, 192, 0.1), (513, 5003, 320, 0.4), (1000, 300, 777, 0.9), (130, 1024, 1024, 0.0),
+    (3, 20011, 33, 0.0),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
+def test_loss_and_gradients(dev, shape, dt):
+    T, V, D, ignored = shape
+    x, w, y, g = make(T, V, D, dt, ignored, dev)
+    for reduction in ("mean", "sum", "none"):
+        grad = torch.randn(T, generator=g).to(dev) if reduction == "none" else torch.randn((), generator=g).to(dev)
+        if reduction == "mean" and int((y >= 0).sum()) == 0:
+            y = y.clone()
+            y[0] = 0
+        (loss, ltol), (dx, dxt), (dw, dwt) = reference(x, w, y, reduction=reduction, grad=grad)
+        with torch.no_grad():
+            plain = lm_head.linear_cross_entropy(x, w, y, reduction=reduction)
+        xl, wl = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        got = lm_head.linear_cross_entropy(xl, wl, y, reduction=reduction)
+        assert got.dtype == torch.float32 and got.shape == loss.shape and torch.equal(plain, got.detach())
+        assert ((got.detach().double() - loss).abs() <= ltol).all()
+        a, b = torch.autograd.grad(got, [xl, wl], grad)
+        assert a.dtype == b.dtype == x.dtype and a.shape == x.shape and b.shape == w.shape
+        near(a, dx, dxt, dt, V + D)
+        near(b, dw, dwt, dt, T + D)
+        assert (a[y == -100] == 0).all()
+        if reduction == "sum":  # one gradient alone
+            (a1,) = torch.autograd.grad(lm_head.linear_cross_entropy(xl, w, y, reduction=reduction), [xl], grad)
+            (b1,) = torch.autograd.grad(lm_head.linear_cross_entropy(x, wl, y, reduction=reduction), [wl], grad)
+            assert torch.equal(a1, a) and torch.equal(b1, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("T,V,D", [(3, (1 << 20) + 1000, 64), (9000, 70001, 64)])
+def test_more_than_one_piece_of_the_vocabulary(dev, T, V, D, dt):
+    if dt == "fp32" and T > 100:
+        V = 35001
+    x, w, y, g = make(T, V, D, dt, 0.1, dev)
+    y[0] = V - 1
+    (loss, ltol), (dx, dxt), (dw, dwt) = reference(x, w, y)
+    xl, wl = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    got = lm_head.linear_cross_entropy(xl, wl, y)
+    assert (got.detach().double() - loss).abs() <= ltol
+    a, b = torch.autograd.grad(got, [xl, wl])
+    near(a, dx, dxt, dt, V + D)
+    near(b, dw, dwt, dt, T + D)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+def test_ignored_and_impossible_targets(dev, dt):
+    x, w, y, g = make(40, 300, 72, dt, 0.0, dev)
+
+    def run(y, **kw):
+        xl, wl = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        loss = lm_head.linear_cross_entropy(xl, wl, y, **kw)
+        return (loss.detach(), *torch.autograd.grad(loss.sum(), [xl, wl]))
+
+    none = torch.full_like(y, -100)
+    for reduction, want in (("sum", 0.0), ("mean", math.nan), ("none", 0.0)):
+        loss, dx, dw = run(none, reduction=reduction)
+        assert torch.isnan(loss).all() if math.isnan(want) else (loss == want).all()
+        assert (dx == 0).all() and (dw == 0).all()
+    # an ignore_index inside the vocabulary
+    yi = torch.where(torch.arange(40, device=dev) % 3 == 0, 7, y)
+    (loss, ltol), (dx, dxt), (dw, dwt) = reference(x, w, yi, ignore=7)
+    got = run(yi, ignore_index=7)
+    assert (got[0].double() - loss).abs() <= ltol
+    near(got[1], dx, dxt, dt, 372)
+    near(got[2], dw, dwt, dt, 112)
+    # impossible targets: their rows only in the loss and in dx
+    for bad in (300, -1, 2 ** 40, -(2 ** 40)):
+        yb = y.clone()
+        yb[5] = bad
+        loss, dx, dw = run(yb, reduction="none")
+        assert torch.isnan(loss[5]) and torch.isfinite(loss).sum() == 39
+        assert torch.isnan(dx[5]).all() and torch.isfinite(dx).sum() == 39 * 72 and torch.isnan(dw).all()
+        assert torch.isnan(run(yb)[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+def test_strides_shapes_and_targets_types(dev, dt):
+    T, V, D = 60, 500, 128
+    x, w, y, g = make(T, V, D, dt, 0.2, dev)
+    (loss, ltol), (dx, dxt), (dw, dwt) = reference(x, w, y)
+    wide = torch.zeros(T, D + 9, dtype=x.dtype, device=dev)
+    wide[:, 5:5 + D] = x
+    ww = torch.zeros(V, 2 * D + 8, dtype=x.dtype, device=dev)
+    ww[:, :D] = w
+    wo = torch.zeros(V * D + 1, dtype=x.dtype, device=dev)
+    wo[1:] = w.reshape(-1)
+    xs = [x, wide[:, 5:5 + D], x.t().contiguous().t(), x.view(3, 20, D), x.view(3, 20, D).transpose(0, 1).contiguous().transpose(0, 1)]
+    ws = [w, ww[:, :D], w.t().contiguous().t(), wo[1:].view(V, D), w.repeat_interleave(2, 0)[::2]]
+    for i, xv in enumerate(xs):
+        for wv in ws if i == 0 else ws[:1]:
+            xl, wl = xv.detach().requires_grad_(True), wv.detach().requires_grad_(True)
+            yv = y.view(xv.shape[:-1]).to([torch.int64, torch.int32, torch.int16][i % 3])
+            got = lm_head.linear_cross_entropy(xl, wl, yv)
+            assert (got.detach().double() - loss).abs() <= ltol
+            a, b = torch.autograd.grad(got, [xl, wl])
+            near(a, dx, dxt, dt, V + D)
+            near(b, dw, dwt, dt, T + D)
+    rows = lm_head.linear_cross_entropy(xs[3], w, y.view(3, 20), reduction="none")
+    assert rows.shape == (3, 20)
+    # a token's row repeated (rows that overlap)
+    one = x[:1].expand(T, D)
+    (loss, ltol), (dx, dxt), (dw, dwt) = reference(one, w, y, reduction="sum")
+    xl, wl = one.detach().requires_grad_(True), w.clone().requires_grad_(True)
+    got = lm_head.linear_cross_entropy(xl, wl, y, reduction="sum")
+    a, b = torch.autograd.grad(got, [xl, wl])
+    near(a, dx, dxt, dt, V + D)
+    near(b, dw, dwt, dt, T + D)
+    # a single token without a batch dimension
+    got = lm_head.linear_cross_entropy(x[0], w, y[0].abs().clamp(max=V - 1), reduction="none")
+    assert got.shape == ()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+def test_no_tokens(dev, dt):
+    w = torch.randn(50, 64, device=dev).to(DT[dt]).requires_grad_(True)
+    x = torch.empty(0, 64, device=dev, dtype=DT[dt], requires_grad=True)
+    y = torch.empty(0, dtype=torch.int64, device=dev)
+    assert torch.isnan(lm_head.linear_cross_entropy(x, w, y))
+    assert lm_head.linear_cross_entropy(x, w, y, reduction="none").shape == (0,)
+    loss = lm_head.linear_cross_entropy(x, w, y, reduction="sum")
+    assert loss.item() == 0.0
+    dx, dw = torch.autograd.grad(loss, [x, w])
+    assert dx.shape == (0, 64) and (dw == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("reduction", ["sum", "none"])
+def test_gradients_far_from_one(dev, dt, reduction):
+    """A loss scaled up or averaged over very many rows, and rows whose gradients differ widely."""
+    x, w, y, g = make(64, 400, 64, dt, 0.0, dev)
+    for size in (2.0 ** -18, 1.0, 2.0 ** 6):
+        grad = torch.tensor(size, device=dev)
+        if reduction == "none":
+            grad = (torch.randn(64, generator=g).exp2() * size).to(dev)
+        _, (dx, dxt), (dw, dwt) = reference(x, w, y, reduction=reduction, grad=grad)
+        xl, wl = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        a, b = torch.autograd.grad(lm_head.linear_cross_entropy(xl, wl, y, reduction=reduction), [xl, wl], grad)
+        near(a, dx, dxt, dt, 464)
+        near(b, dw, dwt, dt, 128)
+    # a gradient expanded over the rows, and one of zeros
+    xl, wl = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    rows = lm_head.linear_cross_entropy(xl, wl, y, reduction="none")
+    _, (dx, dxt), (dw, dwt) = reference(x, w, y, reduction="none")
+    a, b = torch.autograd.grad(rows.sum(), [xl, wl], retain_graph=True)
+    near(a, dx, dxt, dt, 464)
+    near(b, dw, dwt, dt, 128)
+    a, b = torch.autograd.grad(rows, [xl, wl], torch.zeros_like(rows))
+    assert (a == 0).all() and (b == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+def test_large_logits_do_not_overflow(dev, dt):
+    x = torch.zeros(8, 64, device=dev, dtype=DT[dt])
+    w = torch.zeros(300, 64, device=dev, dtype=DT[dt])
+    x[:, 0] = 100.0
+    w[:, 0] = torch.linspace(-100, 100, 300, device=dev).to(DT[dt])
+    y = torch.tensor([0, 299, 298, 150, 1, 299, 299, 2], device=dev)
+    xl, wl = x.requires_grad_(True), w.requires_grad_(True)
+    rows = lm_head.linear_cross_entropy(xl, wl, y, reduction="none")
+    z = x.detach().double() @ w.detach().double().t()
+    want = torch.logsumexp(z, 1) - z.gather(1, y[:, None])[:, 0]
+    # logits of 10^4 are exact here (one product each): the loss is fp32's rounding of 2 * 10^4
+    assert ((rows.detach().double() - want).abs() <= 4 * U * 2e4).all()
+    a, b = torch.autograd.grad(rows.sum(), [xl, wl])
+    assert torch.isfinite(a).all() and torch.isfinite(b).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+def test_gradient_against_differences(dev, dt):
+    x, w, y, g = make(6, 50, 70, dt, 0.0, dev)
+    xl, wl = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    dx, dw = torch.autograd.grad(lm_head.linear_cross_entropy(xl, wl, y), [xl, wl])
+
+    def value(x, w):
+        return F.cross_entropy(x @ w.t(), y).item()
+
+    xd, wd = x.double(), w.double()
+    h = 1e-5  # the difference's own error is about h^2 = 1e-10 and 1e-15 / h = 1e-10
+    for t, d in ((0, 0), (3, 69), (5, 33)):
+        a, b = xd.clone(), xd.clone()
+        a[t, d] += h
+        b[t, d] -= h
+        want = (value(a, wd) - value(b, wd)) / (2 * h)
+        assert abs(dx[t, d].item() - want) <= 3 * STEP[dt] * dx[t].abs().max().item() + 1e-6
+    for v, d in ((int(y[0]), 0), (49, 69), (int(y[3]), 33)):
+        a, b = wd.clone(), wd.clone()
+        a[v, d] += h
+        b[v, d] -= h
+        want = (value(xd, a) - value(xd, b)) / (2 * h)
+        assert abs(dw[v, d].item() - want) <= 3 * STEP[dt] * dw.abs().max().item() + 1e-6
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+def test_repeat_stream_and_graph(dev, dt):
+    T, V, D = 700, 3000, 200
+    x, w, y, g = make(T, V, D, dt, 0.3, dev)
+
+    def step(x, w, y):
+        loss = lm_head.linear_cross_entropy(x, w, y)
+        return (loss, *torch.autograd.grad(loss, [x, w]))
+
+    def leaves():
+        return x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+
+    want = [t.detach().clone() for t in step(*leaves(), y)]
+    assert all(torch.equal(a, b) for a, b in zip(want, step(*leaves(), y)))
+    lv = leaves()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step(*lv, y)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    del got, lv
+    sx, sw = torch.zeros_like(x).requires_grad_(True), torch.zeros_like(w).requires_grad_(True)
+    sy = torch.zeros_like(y)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(sx, sw, sy)
+    for r in range(3):  # other inputs, and another number of ignored rows, each time
+        yr = torch.where(torch.rand(T, generator=g).to(dev) < 0.3 * r, -100, y.clamp(min=0).roll(r))
+        with torch.no_grad():
+            sx.copy_(x.roll(r, 0))
+            sw.copy_(w.roll(r, 0))
+            sy.copy_(yr)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step(x.roll(r, 0).requires_grad_(True), w.roll(r, 0).requires_grad_(True), yr)
+        assert all(torch.equal(a, b) for a, b in zip(want, out)), r
+
+
+@pytest.mark.gpu
+def test_compiles(dev):
+    x, w, y, g = make(100, 400, 100, "bf16", 0.2, dev)
+
+    def step(x, w):
+        return lm_head.linear_cross_entropy(x * 2, w, y) + lm_head.linear_cross_entropy(x, w, y, reduction="none").sum()
+
+    grads = []
+    for f in (step, torch.compile(step, backend="aot_eager", fullgraph=True)):
+        xl, wl = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        loss = f(xl, wl)
+        grads.append((loss.detach(), *torch.autograd.grad(loss, [xl, wl])))
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
+    for D in (100, 128):
+        x, w, y, g = make(50, 300, D, "bf16", 0.2, dev)
+        torch.library.opcheck(torch.ops.cinnamon_amd.linear_ce_forward, (x, w, y, -100, 2),
+                              test_utils=("test_schema", "test_faketensor"))
+
+
+@pytest.mark.gpu
+def test_a_model_step_with_tied_heads(dev):
+    """Main and next-but-one losses over one tied weight, as the training step composes them, with
+    gradients through a norm, against the same step on plain logits in 64 bits."""
+    torch.manual_seed(5)
+    B, L, D, V = 2, 65, 128, 1000
+    emb = torch.randn(V, D, device=dev) * 0.05
+    ids = torch.randint(0, V, (B, L + 1), device=dev)
+    mix = torch.randn(D, D, device=dev) / math.sqrt(D)
+
+    def step(emb, mix, loss_of):
+        h = F.embedding(ids[:, :-1], emb) @ mix
+        h = h * torch.rsqrt(h.pow(2).mean(-1, keepdim=True) + 1e-6)
+        main = loss_of(h, emb, ids[:, 1:])
+        mtp = loss_of(h[:, :-1], emb, ids[:, 2:])
+        return main + 0.3 * mtp
+
+    ref = [t.double().requires_grad_(True) for t in (emb, mix)]
+    want = step(*ref, lambda h, w, y: F.cross_entropy((h @ w.t()).reshape(-1, V), y.reshape(-1)))
+    dwant = torch.autograd.grad(want, ref)
+    got = [t.clone().requires_grad_(True) for t in (emb, mix)]
+    loss = step(*got, lm_head.linear_cross_entropy)
+    dgot = torch.autograd.grad(loss, got)
+    # fp32 throughout: sums of at most 1000 terms in each of three chained products
+    assert abs(loss.item() - want.item()) <= 3 * math.sqrt(1000) * U * want.item()
+    for a, b in zip(dgot, dwant):
+        assert (a - b).norm() <= 12 * math.sqrt(1000) * U * b.norm()
+
+
+def test_refusals():
+    with FakeTensorMode():
+        def fake(*shape, dtype=torch.bfloat16):
+            return torch.empty(*shape, dtype=dtype, device="cuda")
+
+        i64 = torch.int64
+        x, w, y = fake(4, 64), fake(100, 64), fake(4, dtype=i64)
+        f = lm_head.linear_cross_entropy
+        for bad in [
+            lambda: f(torch.empty(4, 64, dtype=torch.bfloat16), w, y),
+            lambda: f(x, torch.empty(100, 64, dtype=torch.bfloat16), y),
+            lambda: f(x, w, torch.zeros(4, dtype=i64)),
+            lambda: f(x, fake(100, 32), y),
+            lambda: f(x, fake(100, 64, 1), y),
+            lambda: f(x, w, fake(5, dtype=i64)),
+            lambda: f(x, w, fake(4, 1, dtype=i64)),
+            lambda: f(x, fake(100, 64, dtype=torch.float32), y),
+            lambda: f(fake(4, 64, dtype=torch.float64), fake(100, 64, dtype=torch.float64), y),
+            lambda: f(x, w, fake(4, dtype=torch.float32)),
+            lambda: f(x, w, fake(4, dtype=torch.bool)),
+            lambda: f(x, w, y, reduction="max"),
+            lambda: f(x, fake(0, 64), y),
+            lambda: f(fake(4, 0), fake(100, 0), y),
+        ]:
+            with pytest.raises(AssertionError):
+                bad()
+        assert f(x, w, y).shape == () and f(x, w, y).dtype == torch.float32
+        assert f(fake(2, 2, 65), fake(100, 65), fake(2, 2, dtype=i64), reduction="none").shape == (2, 2)
+
+
+_FWD = [16, 0, 4, 64, 64, 16, 100, 64, 16, -100, 1, 16, None, 16, 16, 16, 16, 16, 1 << 30, None]
+_BWD = [16, 0, 4, 64, 16, 100, 64, 16, 16, 16, 0, 1, 16, 16, 16, 1 << 30, None]
+
+
+@pytest.mark.parametrize("name,ok,at,value", [
+    ("cin_linear_ce_forward", _FWD, 1, 4), ("cin_linear_ce_forward", _FWD, 2, -1), ("cin_linear_ce_forward", _FWD, 3, 0),
+    ("cin_linear_ce_forward", _FWD, 3, 1 << 19), ("cin_linear_ce_forward", _FWD, 4, 63), ("cin_linear_ce_forward", _FWD, 6, 0),
+    ("cin_linear_ce_forward", _FWD, 7, 63), ("cin_linear_ce_forward", _FWD, 7, 65), ("cin_linear_ce_forward", _FWD, 5, 20),
+    ("cin_linear_ce_forward", _FWD, 0, None), ("cin_linear_ce_forward", _FWD, 8, None), ("cin_linear_ce_forward", _FWD, 11, None),
+    ("cin_linear_ce_forward", _FWD, 13, None), ("cin_linear_ce_forward", _FWD, 17, None), ("cin_linear_ce_forward", _FWD, 18, 10),
+    ("cin_linear_ce_backward", _BWD, 1, 4), ("cin_linear_ce_backward", _BWD, 2, 0), ("cin_linear_ce_backward", _BWD, 6, 65),
+    ("cin_linear_ce_backward", _BWD, 4, 18), ("cin_linear_ce_backward", _BWD, 9, None), ("cin_linear_ce_backward", _BWD, 10, -1),
+    ("cin_linear_ce_backward", _BWD, 14, None), ("cin_linear_ce_backward", _BWD, 15, 100), ("cin_linear_ce_backward", _BWD, 3, 65),
+])
+def test_c_refusals(name, ok, at, value):
+    args = list(ok)
+    args[at] = value
+    with pytest.raises(ValueError):
+        _lib.call(name, *args)
+
+
+def test_workspace_grows_with_the_call_and_is_bounded():
+    ws = _lib.load().cin_linear_ce_workspace
+    assert ws(0, -1, 64, 100, 1) == -1 and ws(0, 4, 64, 100, 0) > 0
+    for T, D, V in ((1, 64, 100), (8192, 4096, 131072), (100000, 1024, 200000)):
+        # a piece of the logits' gradient, and partial sums of x's gradient
+        assert 0 < ws(0, T, D, V, 1) <= (1 << 30) + T * 1024 + 256 * 2 * T + 4 * T * D * 4 + (256 << 20)
