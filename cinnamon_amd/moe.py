@@ -21,6 +21,7 @@ sorted position order, the order of a sequential scatter_add_).
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import layers
 from ._lib import call, call_on, dtype_code, ptr, stream_of
@@ -85,20 +86,20 @@ def moe_gate(logits: torch.Tensor, top_k: int, bias: torch.Tensor | None = None,
 
 
 def _gate_rows(logits):
-    return logits if logits.stride(1) == 1 and logits.stride(0) >= logits.shape[1] else logits.contiguous()
+    return logits if logits.is_contiguous() or (logits.stride(1) == 1 and logits.stride(0) >= logits.shape[1]) \
+        else logits.contiguous()
 
 
 def _launch_gate(logits, bias, top_k, score, n_groups, top_groups, group_top, renormalize, scale, return_scores):
+    """(idx, weights, scores or None)"""
     lg = _gate_rows(logits)
     T, E = lg.shape
-    dev = lg.device
-    idx = torch.empty((T, top_k), dtype=torch.int64, device=dev)
-    w = torch.empty((T, top_k), dtype=torch.float32, device=dev)
-    scores = torch.empty((T, E) if return_scores else (0,), dtype=torch.float32, device=dev)
+    idx = lg.new_empty((T, top_k), dtype=torch.int64)
+    w = lg.new_empty((T, top_k), dtype=torch.float32)
+    scores = lg.new_empty((T, E), dtype=torch.float32) if return_scores else None
     bias = None if bias is None else bias.contiguous()
-    call_on(lg, "cin_moe_gate", ptr(lg), dtype_code(lg), max(lg.stride(0), E), ptr(bias), T, E, top_k, score, n_groups,
-            top_groups, group_top, int(renormalize), scale, ptr(idx), ptr(w), ptr(scores) if return_scores else 0,
-            stream_of(lg))
+    call_on(lg, "cin_moe_gate", lg.data_ptr(), dtype_code(lg), max(lg.stride(0), E), ptr(bias), T, E, top_k, score,
+            n_groups, top_groups, group_top, renormalize, scale, idx.data_ptr(), w.data_ptr(), ptr(scores), stream_of(lg))
     return idx, w, scores
 
 
@@ -106,11 +107,11 @@ def _launch_gate_backward(logits, idx, gw, gs, score, renormalize, scale):
     """Gradient of the logits; gw or gs may be None."""
     lg = _gate_rows(logits)
     T, E = lg.shape
-    out = torch.empty((T, E), dtype=lg.dtype, device=lg.device)
-    gw = None if gw is None else gw.float().contiguous()
-    gs = None if gs is None else gs.float().contiguous()
+    out = lg.new_empty((T, E))
+    gw = None if gw is None else gw.contiguous()
+    gs = None if gs is None else gs.contiguous()
     call_on(lg, "cin_moe_gate_backward", ptr(lg), dtype_code(lg), max(lg.stride(0), E), T, E, idx.shape[1], score,
-            int(renormalize), scale, ptr(idx.contiguous()), ptr(gw), ptr(gs), ptr(out), stream_of(lg))
+            renormalize, scale, idx.data_ptr(), ptr(gw), ptr(gs), out.data_ptr(), stream_of(lg))
     return out
 
 
@@ -123,23 +124,29 @@ class _MoeGate(torch.autograd.Function):
         ctx.save_for_backward(logits, idx)
         ctx.options = options
         ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(*((idx,) if options[-1] else (idx, scores)))
+        ctx.mark_non_differentiable(idx)
         return idx, w, scores
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, _gidx, gw, gs):
-        if gw is None and gs is None:
-            return (None,) * 10
-        _k, score, _g, _tg, _gt, renormalize, scale, _rs = ctx.options
-        return (_launch_gate_backward(*ctx.saved_tensors, gw, gs, score, renormalize, scale),) + (None,) * 9
+    def backward(ctx, *grads):
+        # (the wrapper costs 4 us of host time a call; only a graph of the gradient needs it)
+        f = _gate_gradient if not torch.is_grad_enabled() else once_differentiable(_gate_gradient)
+        return f(ctx, *grads)
+
+
+def _gate_gradient(ctx, _gidx, gw, gs):
+    if gw is None and gs is None:
+        return (None,) * 10
+    _k, score, _g, _tg, _gt, renormalize, scale, _rs = ctx.options
+    return (_launch_gate_backward(*ctx.saved_tensors, gw, gs, score, renormalize, scale),) + (None,) * 9
 
 
 @custom_op("moe_gate", "(Tensor logits, Tensor? bias, int top_k, int score, int n_groups, int top_groups, int group_top, "
            "bool renormalize, float scale, bool return_scores) -> (Tensor, Tensor, Tensor)")
 def _gate_op(logits, bias, *options):
     # without return_scores the last output is an empty placeholder
-    return _launch_gate(logits, bias, *options)
+    idx, w, scores = _launch_gate(logits, bias, *options)
+    return idx, w, scores if scores is not None else logits.new_empty((0,), dtype=torch.float32)
 
 
 @_gate_op.register_fake

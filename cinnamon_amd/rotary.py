@@ -10,6 +10,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from ._lib import call_on, dtype_code, ptr, stream_of
 from .kernels import _plain_eager, _require, custom_op
@@ -83,19 +84,20 @@ def apply_rotary(q: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k: torch
     _require(cos.ndim == 2 and cos.shape == sin.shape and cos.dtype == sin.dtype == torch.float32,
              "cos and sin must be fp32 [P, rot / 2]")
     _require(cos.device == q.device and sin.device == q.device, "cos and sin must be on q's device")
-    _require(not (torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad)),
+    _require(not (cos.requires_grad or sin.requires_grad) or not torch.is_grad_enabled(),
              "cos and sin carry no gradient: detach them")
-    rot, L = 2 * cos.shape[1], q.shape[1]
-    _require(rot >= 2 and start >= 0 and start + rot <= q.shape[-1],
-             f"the rotated channels [{start}, {start + rot}) must lie within the head")
+    (P, half), L = cos.shape, q.shape[1]
+    _require(half >= 1 and start >= 0 and start + 2 * half <= q.shape[-1],
+             "the rotated channels [start, start + rot) must lie within the head")
     if positions is None:
-        _require(L <= cos.shape[0], f"{L} positions, but the tables hold {cos.shape[0]}")
+        _require(L <= P, "more tokens than the tables hold positions")
     else:
         _require(positions.device == q.device and not positions.dtype.is_floating_point
                  and not positions.dtype.is_complex and positions.dtype != torch.bool,
                  "positions must be integers on q's device")
         _require(tuple(positions.shape) in ((L,), (q.shape[0], L)), "positions must be [L] or [B, L]")
-        positions = positions.to(torch.int64)
+        if positions.dtype != torch.int64:
+            positions = positions.to(torch.int64)
     args = (q, k, cos, sin, positions, bool(interleaved), int(start))
     if _plain_eager(*args):
         if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
@@ -108,12 +110,10 @@ def apply_rotary(q: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k: torch
 
 
 def _rows(t):
-    return t if t.stride(-1) == 1 else t.contiguous()
-
-
-def _strides(t):
-    """Batch, token and head strides and the number of heads."""
-    return (t.stride(0), t.stride(1), t.stride(2), t.shape[2]) if t.ndim == 4 else (t.stride(0), t.stride(1), 0, 1)
+    """t with adjacent channels and token and head strides that fit in 32 bits."""
+    if t.is_contiguous() or (t.stride(-1) == 1 and max(t.stride()[1:-1]) < 1 << 31):
+        return t
+    return t.contiguous()
 
 
 def _empty(x):
@@ -122,26 +122,41 @@ def _empty(x):
     return out if out.stride(-1) == 1 else torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
+_NO_SIDE = (0,) * 9
+
+
+def _side(t):
+    """(output, the arguments of one tensor: both pointers, their batch, token and head strides,
+    the heads)"""
+    if t.is_contiguous():
+        out = torch.empty_like(t)
+        shape = t.shape
+        H = shape[2] if len(shape) == 4 else 1
+        D = shape[-1]
+        l = H * D
+        b = shape[1] * l
+        return out, (t.data_ptr(), b, l, D, out.data_ptr(), b, l, D, H)
+    t = _rows(t)
+    out = _empty(t)
+
+    def strides(x):
+        return (x.stride(0), x.stride(1), x.stride(2) if x.ndim == 4 else 0)
+
+    return out, (t.data_ptr(), *strides(t), out.data_ptr(), *strides(out), t.shape[2] if t.ndim == 4 else 1)
+
+
 def _launch(q, k, cos, sin, positions, interleaved, start, inverse):
     """(q's result, k's); a tensor that is None gives None."""
-    outs, sides = [], []
-    for t in (q, k):
-        if t is None:
-            outs.append(None)
-            sides += [0, 0, 0, 0, 0, 0, 0, 0, 0]
-            continue
-        t = _rows(t)
-        o = _empty(t)
-        outs.append(o)
-        b, l, h, heads = _strides(t)
-        sides += [ptr(t), b, l, h, ptr(o), *_strides(o)[:3], heads]
+    oq, sq = (None, _NO_SIDE) if q is None else _side(q)
+    ok, sk = (None, _NO_SIDE) if k is None else _side(k)
     t = q if q is not None else k
-    B, L, D = t.shape[0], t.shape[1], t.shape[-1]
+    shape = t.shape
     cos, sin = cos.contiguous(), sin.contiguous()
+    P, half = cos.shape
     spb, spl = (0, 0) if positions is None else (positions.stride(0) if positions.ndim == 2 else 0, positions.stride(-1))
-    call_on(t, "cin_rotary", *sides, dtype_code(t), B, L, D, ptr(cos), ptr(sin), cos.shape[0],
-            cos.shape[1], 2 * cos.shape[1], start, ptr(positions), spb, spl, int(interleaved), int(inverse), stream_of(t))
-    return tuple(outs)
+    call_on(t, "cin_rotary", *sq, *sk, dtype_code(t), shape[0], shape[1], shape[-1], cos.data_ptr(), sin.data_ptr(), P,
+            half, 2 * half, start, ptr(positions), spb, spl, interleaved, inverse, stream_of(t))
+    return oq, ok
 
 
 class _Rotary(torch.autograd.Function):
@@ -155,13 +170,18 @@ class _Rotary(torch.autograd.Function):
         return _launch(q, k, cos, sin, positions, interleaved, start, False)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, gq, gk):
-        gq = gq if ctx.needs_input_grad[0] else None
-        gk = gk if ctx.needs_input_grad[1] else None
-        if gq is None and gk is None:
-            return (None,) * 7
-        return (*_launch(gq, gk, *ctx.saved_tensors, *ctx.options, True), None, None, None, None, None)
+        # (the wrapper costs 4 us of host time a call; only a graph of the gradient needs it)
+        f = _rotary_turn_back if not torch.is_grad_enabled() else once_differentiable(_rotary_turn_back)
+        return f(ctx, gq, gk)
+
+
+def _rotary_turn_back(ctx, gq, gk):
+    need_q, need_k = ctx.needs_input_grad[:2]
+    gq, gk = gq if need_q else None, gk if need_k else None
+    if gq is None and gk is None:
+        return (None,) * 7
+    return (*_launch(gq, gk, *ctx.saved_tensors, *ctx.options, True), None, None, None, None, None)
 
 
 @custom_op("rotary", "(Tensor q, Tensor? k, Tensor cos, Tensor sin, Tensor? positions, bool interleaved, int start, "

@@ -542,8 +542,8 @@ int cin_moe_gate_backward(const void* logits, int dtype, int64_t ldl, int64_t T,
  * pairs (2i, 2i + 1) if interleaved, else (i, i + rot / 2); the other channels copied.  cos and
  * sin [P, rot / 2] fp32 with row stride ldt; positions int64 with strides (spb, spl), or null for
  * 0 .. L - 1 (L <= P).  A token at a negative position is copied as it is, one at P or beyond
- * gives NaN in its rotated channels.  Batch, token and head strides per tensor, channels adjacent;
- * H or Hk may be 0.  Outputs must not overlap the inputs.
+ * gives NaN in its rotated channels.  Batch, token and head strides per tensor (the last two below
+ * 2^31), channels adjacent; H or Hk may be 0.  Outputs must not overlap the inputs.
  */
 int cin_rotary(const void* q, int64_t sqb, int64_t sql, int64_t sqh, void* q_out, int64_t soqb,
                int64_t soql, int64_t soqh, int64_t H, const void* k, int64_t skb, int64_t skl,
