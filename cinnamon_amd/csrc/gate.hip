@@ -12,11 +12,15 @@
 //   ds     = gs;  ds[idx_j] += scale * (gw_j - sum_i gw_i s[idx_i] / total) / total
 //   dz     = ds s (1 - s)  or  s (ds - sum_e ds_e s_e)
 //
-// Scores are ordered in 64 bits: neighbours in the order may differ by less than 32 bits hold.
-// NaN counts as the greatest value, in a row and among groups.
+// Choices are ordered as they compare in 64 bits: neighbours in the order may differ by less than
+// 32 bits hold.  A token is first ranked in 32 bits; where every difference that decides exceeds
+// the error bound (or is one of equal logits and biases, a true tie), that is the order, else its
+// wave ranks it again in 64 bits (about one token in a thousand with random logits).  NaN counts as the greatest value, in a row and among groups.
 //
 // A token's experts lie over LANES lanes, EPL consecutive ones a lane, so that the order of the
 // lanes is the order of the indices: the lowest of equal candidates is the first lane of a ballot.
+// Up to 256 experts a token takes 16 lanes (a DPP row): maxima and sums need no LDS, and the rounds
+// of the top k serve four tokens at once.  Bound by VALU issue: see the rates at the launch.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -55,201 +59,466 @@ __device__ inline uint64_t key_of(double v) {
 __device__ inline double value_of(uint64_t k) {
   return __longlong_as_double((long long)(k >> 63 ? k & ~(1ull << 63) : ~k));
 }
+__device__ inline uint32_t key_of(float v) {  // (not for NaN)
+  const uint32_t b = __float_as_uint(v + 0.0f);
+  return b >> 31 ? ~b : b | (1u << 31);
+}
+__device__ inline float value_of(uint32_t k) { return __uint_as_float(k >> 31 ? k & ~(1u << 31) : ~k); }
 
-template <int LANES, class V>
-__device__ inline V lanes_max(V v) {
+template <int CTRL>
+__device__ inline uint32_t moved(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xF, 0xF, true);
+}
+// f over the token's lanes, every lane getting the result: within a DPP row by quad permutations,
+// a half mirror and a mirror, across rows by swaps through LDS.
+template <int LANES, class F>
+__device__ inline uint32_t over_lanes(uint32_t v, F f) {
+  static_assert(LANES == 16 || LANES == 64, "a DPP row or a wave");
+  v = f(v, moved<0xB1>(v));
+  v = f(v, moved<0x4E>(v));
+  v = f(v, moved<0x141>(v));
+  v = f(v, moved<0x140>(v));
+  if constexpr (LANES == 64) {
+    v = f(v, (uint32_t)__shfl_xor((int)v, 16));
+    v = f(v, (uint32_t)__shfl_xor((int)v, 32));
+  }
+  return v;
+}
+template <int LANES>
+__device__ inline uint32_t lanes_max(uint32_t v) {
+  return over_lanes<LANES>(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+}
+template <int LANES>
+__device__ inline float lanes_sum(float v) {
+  return __uint_as_float(over_lanes<LANES>(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  }));
+}
+// the maximum, NaN where there is one
+template <int LANES>
+__device__ inline float lanes_max_nan(float v) {
+  return __uint_as_float(over_lanes<LANES>(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+    const float x = __uint_as_float(a), y = __uint_as_float(b);
+    return y > x || y != y ? b : a;
+  }));
+}
+template <int LANES>
+__device__ inline uint64_t lanes_max(uint64_t v) {
 #pragma unroll
   for (int o = 1; o < LANES; o <<= 1) {
-    const V u = __shfl_xor(v, o);
+    const uint64_t u = __shfl_xor(v, o);
     v = u > v ? u : v;
   }
   return v;
 }
-template <int LANES, class V>
-__device__ inline V lanes_sum(V v) {
+template <int LANES>
+__device__ inline double lanes_sum(double v) {
 #pragma unroll
   for (int o = 1; o < LANES; o <<= 1) v += __shfl_xor(v, o);
   return v;
 }
 
-// The first lane of this lane's token for which `mine` holds, or -1.
+// Whether this lane is the first of its token for which `mine` holds.
 template <int LANES>
-__device__ inline int first_lane(bool mine, int lane) {
-  uint64_t m = __ballot(mine);
-  if constexpr (LANES < 64) m = (m >> (lane & ~(LANES - 1))) & ((1ull << LANES) - 1);
-  return m ? __builtin_ctzll(m) : -1;
+__device__ inline bool is_first(bool mine, int lane) {
+  const uint64_t m = __ballot(mine);
+  if constexpr (LANES == 64) return lane == (int)__builtin_ctzll(m | (1ull << 63));
+  const uint32_t w = lane & 32 ? (uint32_t)(m >> 32) : (uint32_t)m;
+  const uint32_t row = (w >> (lane & 16)) & 0xffffu;
+  return (lane & 15) == __builtin_ctz(row | 0x10000u);
+}
+// Whether `mine` holds on any lane of the token.
+template <int LANES>
+__device__ inline bool any_lane(bool mine, int lane) {
+  const uint64_t m = __ballot(mine);
+  if constexpr (LANES == 64) return m != 0;
+  const uint32_t w = lane & 32 ? (uint32_t)(m >> 32) : (uint32_t)m;
+  return ((w >> (lane & 16)) & 0xffffu) != 0;
 }
 
-// Scores of the token's experts, EPL a lane; z holds -inf past E.
-template <int LANES, int EPL, class F>
-__device__ inline void scores(int kind, const float (&z)[EPL], F (&s)[EPL]) {
-  if (kind == kSigmoid) {
+// LDS written by lanes of a wave and read by others of the same wave: accesses of one wave are
+// carried out in order, so only the compiler has to keep them so.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// EPL neighbours from any element's address, `other` past n.
+template <int DT, int EPL>
+__device__ __forceinline__ void load_row(const void* p, int64_t row, int e0, int n, float other, float (&v)[EPL]) {
+  constexpr int es = DT == CIN_DT_F32 ? 4 : 2;
+  const uint8_t* q = static_cast<const uint8_t*>(p) + (row + e0) * es;
+  if (e0 + EPL <= n) {
+    if constexpr (DT == CIN_DT_F32) {
+      __builtin_memcpy(v, q, 4 * EPL);
+    } else {
+      uint16_t h[EPL];
+      __builtin_memcpy(h, q, 2 * EPL);
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) s[j] = 1 / (1 + exp(-(F)z[j]));
-  } else {
-    F m = z[0];
-#pragma unroll
-    for (int j = 0; j < EPL; ++j) m = z[j] > m || z[j] != z[j] ? (F)z[j] : m;
-#pragma unroll
-    for (int o = 1; o < LANES; o <<= 1) {
-      const F u = __shfl_xor(m, o);
-      m = u > m || u != u ? u : m;
+      for (int j = 0; j < EPL; ++j) v[j] = half_bits_to_f32(DT, h[j]);
     }
-    F t = 0;
+  } else {
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) t += s[j] = exp((F)z[j] - m);
-    t = lanes_sum<LANES>(t);
-#pragma unroll
-    for (int j = 0; j < EPL; ++j) s[j] /= t;
+    for (int j = 0; j < EPL; ++j) v[j] = e0 + j < n ? load_elem(q, DT, j) : other;
   }
 }
 
-template <int EPL>
-__device__ inline void load_logits(const GateArgs& a, int64_t t, int e0, float (&z)[EPL]) {
+// 1 / (1 + e^-z) and e^d in 32 bits within 8 roundings, below 1e-37 in absolute terms; NaN stays.  The
+// exponential's argument is formed in two parts, as a rounded one is off by |d| of its last bits.
+__device__ inline float exp_of(float d) {
+  d = d > 88.7f ? 88.7f : d;
+  d = d < -104.0f ? -104.0f : d;
+  const float t = d * 1.44269504f, lo = __builtin_fmaf(d, 1.44269504f, -t) + d * 1.92596299e-8f;
+  const float e = __builtin_amdgcn_exp2f(t);
+  return __builtin_fmaf(e, lo * 0.693147182f, e);
+}
+__device__ inline float sigmoid_of(float z) { return __builtin_amdgcn_rcpf(1.0f + exp_of(-z)); }
+
+// Scores of the token's experts; z holds -inf past E.  top: an upper bound of them (softmax).
+template <int LANES, int EPL>
+__device__ inline void scores(int kind, const float (&z)[EPL], float (&s)[EPL], float& top, float& zmax, float& inv) {
+  top = 1.0f;
+  zmax = 0.0f;
+  inv = 1.0f;
+  if (kind == kSigmoid) {
 #pragma unroll
-  for (int j = 0; j < EPL; ++j)
-    z[j] = e0 + j < a.E ? load_elem(a.logits, a.dtype, t * a.ldl + e0 + j) : -__builtin_inff();
+    for (int j = 0; j < EPL; ++j) s[j] = sigmoid_of(z[j]);
+  } else {
+    float m = z[0], t = 0.0f;
+#pragma unroll
+    for (int j = 1; j < EPL; ++j) m = z[j] > m || z[j] != z[j] ? z[j] : m;
+    m = lanes_max_nan<LANES>(m);
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) t += s[j] = exp_of(z[j] - m);
+    t = lanes_sum<LANES>(t);
+    top = inv = 1.0f / t;
+    zmax = m;
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) s[j] *= inv;
+  }
+}
+// Groups that stay, as a mask: lanes share a group's keys, `part` of `parts` each.  `margin` gets
+// the difference between the last group that stays, `worst`, and the first that does not.
+template <int LANES, class K, class F>
+__device__ inline uint64_t keep_groups(const GateArgs& a, const K* keys, int lane, F& margin, F& worst) {
+  constexpr int kPer = kGateMaxGroups / LANES;  // groups of a lane
+  const int sub = lane & (LANES - 1), n = a.E / a.groups;
+  K best[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) best[i] = 0;
+  if (2 * a.groups <= LANES) {
+    // 2, 4 or 8 lanes a group
+    int parts = 2;
+    while (2 * parts * a.groups <= LANES && parts < 8) parts *= 2;
+    const int g = sub / parts, part = sub % parts;
+    K k1 = 0, k2 = 0;
+    if (g < a.groups)
+      for (int e = part; e < n; e += parts) {
+        const K v = keys[g * n + e];
+        k2 = v > k1 ? k1 : (v > k2 ? v : k2);
+        k1 = v > k1 ? v : k1;
+      }
+    for (int o = 1; o < parts; o <<= 1) {
+      const K o1 = __shfl_xor(k1, o), o2 = __shfl_xor(k2, o);
+      const K lo = k1 < o1 ? k1 : o1, hi2 = k2 > o2 ? k2 : o2;
+      k1 = k1 > o1 ? k1 : o1;
+      k2 = lo > hi2 ? lo : hi2;
+    }
+    // group sub's result to lane sub
+    const int from = (lane & ~(LANES - 1)) + (sub * parts) % LANES;
+    k1 = __shfl(k1, from);
+    k2 = __shfl(k2, from);
+    if (sub < a.groups) best[0] = a.group_top == 1 || n == 1 ? k1 : key_of(value_of(k1) + value_of(k2));
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int g = sub + i * LANES;
+      K k1 = 0, k2 = 0;
+      if (g < a.groups)
+        for (int e = 0; e < n; ++e) {
+          const K v = keys[g * n + e];
+          k2 = v > k1 ? k1 : (v > k2 ? v : k2);
+          k1 = v > k1 ? v : k1;
+        }
+      best[i] = g >= a.groups ? 0 : (a.group_top == 1 || n == 1 ? k1 : key_of(value_of(k1) + value_of(k2)));
+    }
+  }
+  uint64_t kept = 0;
+  K last = 0;
+  for (int r = 0; r <= a.top_groups; ++r) {
+    // the best group left, the lowest of equals: lane sub holds groups sub, sub + LANES, ..
+    K m = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) m = best[i] > m ? best[i] : m;
+    const K top = lanes_max<LANES>(m);
+    if (r == a.top_groups) {
+      worst = value_of(last);
+      margin = worst - value_of(top);
+      break;
+    }
+    last = top;
+    bool done = false;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      uint64_t mine = __ballot(!done && best[i] == top);
+      if constexpr (LANES < 64) mine = (mine >> (lane & ~(LANES - 1))) & ((1ull << LANES) - 1);
+      if (mine && !done) {
+        const int at = (int)__builtin_ctzll(mine);
+        kept |= 1ull << (at + i * LANES);
+        if (sub == at) best[i] = 0;
+        done = true;
+      }
+    }
+  }
+  return kept;
 }
 
-// One token a wave: its keys through LDS for the groups, then k rounds of a maximum.
-template <int LANES, int EPL, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void k_gate_fwd(GateArgs a, int64_t* __restrict__ idx, float* __restrict__ w,
+// The k largest keys, the lowest index of equals: lane r's key, and the expert in chosen[r]; keys
+// taken become 0.
+template <int LANES, int EPL>
+__device__ inline uint32_t top_k(int k, int lane, uint32_t (&key)[EPL], int* chosen) {
+  const int sub = lane & (LANES - 1);
+  uint32_t mine = 0;
+  for (int r = 0; r < k; ++r) {
+    uint32_t m = key[0];
+#pragma unroll
+    for (int j = 1; j < EPL; ++j) m = key[j] > m ? key[j] : m;
+    const uint32_t top = lanes_max<LANES>(m);
+    mine = sub == r ? top : mine;
+    if (is_first<LANES>(m == top, lane)) {
+      int at = EPL - 1;
+#pragma unroll
+      for (int j = EPL - 2; j >= 0; --j) at = key[j] == top ? j : at;
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) key[j] = j == at ? 0 : key[j];
+      chosen[r] = sub * EPL + at;
+    }
+  }
+  wave_sync();
+  return mine;
+}
+
+// Token t's ranking in 64 bits by the whole wave, its keys in LDS: lane r < k gets the r-th expert
+// and its score.
+template <int DT>
+__device__ inline void rank64(const GateArgs& a, int64_t t, int lane, uint64_t* keys, int& my_e, double& my_s) {
+  const int64_t row = t * a.ldl;
+  double m = -__builtin_inf(), total = 0;
+  if (a.score == kSoftmax) {
+    for (int e = lane; e < a.E; e += 64) {
+      const double z = load_elem(a.logits, DT, row + e);
+      m = z > m || z != z ? z : m;
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const double u = __shfl_xor(m, o);
+      m = u > m || u != u ? u : m;
+    }
+    for (int e = lane; e < a.E; e += 64) total += exp((double)load_elem(a.logits, DT, row + e) - m);
+    total = lanes_sum<64>(total);
+  }
+  const auto score = [&](int e) {
+    const double z = load_elem(a.logits, DT, row + e);
+    return a.score == kSoftmax ? exp(z - m) / total : 1 / (1 + exp(-z));
+  };
+  wave_sync();
+  for (int e = lane; e < a.E; e += 64) keys[e] = key_of(score(e) + (a.bias ? (double)a.bias[e] : 0.0));
+  wave_sync();
+  if (a.top_groups < a.groups) {
+    double margin, worst;
+    const uint64_t kept = keep_groups<64, uint64_t, double>(a, keys, lane, margin, worst);
+    const int n = a.E / a.groups;
+    wave_sync();
+    for (int e = lane; e < a.E; e += 64)
+      if (!(kept >> (e / n) & 1)) keys[e] = 0;
+    wave_sync();
+  }
+  my_e = 0;
+  for (int r = 0; r < a.k; ++r) {
+    uint64_t best = 0;
+    int at = 0;  // the lane's first expert with it
+    for (int e = lane; e < a.E; e += 64) {
+      const uint64_t v = keys[e];
+      at = v > best ? e : at;
+      best = v > best ? v : best;
+    }
+    const uint64_t top = lanes_max<64>(best);
+    int e = best == top ? at : a.E;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int u = __shfl_xor(e, o);
+      e = u < e ? u : e;
+    }
+    if (lane == r) my_e = e;
+    if (lane == 0) keys[e] = 0;
+    wave_sync();
+  }
+  my_s = lane < a.k ? score(my_e) : 0.0;
+}
+
+template <int LANES, int EPL, int WAVES, int DT>
+__global__ __launch_bounds__(64 * WAVES, EPL <= 16 ? 4 : 1) void k_gate_fwd(GateArgs a, int64_t* __restrict__ idx, float* __restrict__ w,
                                                          float* __restrict__ all) {
   constexpr int kTokens = 64 / LANES * WAVES;
-  __shared__ uint64_t sk[kTokens][LANES * EPL];
+  __shared__ uint64_t keys64[WAVES][LANES * EPL];   // of the token a wave ranks in 64 bits
+  __shared__ uint32_t keys32[kTokens][LANES * EPL];
+  __shared__ int chosen[kTokens][kGateMaxTopK];
   const int lane = threadIdx.x & 63, sub = lane & (LANES - 1);
   const int slot = threadIdx.x / LANES;
   const int64_t t0 = (int64_t)blockIdx.x * kTokens + slot;
   const bool live = t0 < a.T;
   const int64_t t = live ? t0 : a.T - 1;  // (a token past the end repeats the last one and stores nothing)
   const int e0 = sub * EPL;
-  float z[EPL];
-  double s[EPL];
-  uint64_t key[EPL];
-  load_logits(a, t, e0, z);
-  scores<LANES, EPL>(a.score, z, s);
+  const bool limited = a.top_groups < a.groups;
+  float z[EPL], b[EPL], s[EPL];
+  load_row<DT, EPL>(a.logits, t * a.ldl, e0, a.E, -__builtin_inff(), z);
+  if (a.bias) {
+    load_row<CIN_DT_F32, EPL>(a.bias, 0, e0, a.E, 0.0f, b);
+  } else {
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) b[j] = 0.0f;
+  }
+  float top, zmax, inv;
+  scores<LANES, EPL>(a.score, z, s, top, zmax, inv);
   if (all && live) {
+    float* q = all + t * a.E + e0;
+    if (e0 + EPL <= a.E) {
+      __builtin_memcpy(q, s, 4 * EPL);
+    } else {
 #pragma unroll
-    for (int j = 0; j < EPL; ++j)
-      if (e0 + j < a.E) all[t * a.E + e0 + j] = (float)s[j];
+      for (int j = 0; j < EPL; ++j)
+        if (e0 + j < a.E) q[j] = s[j];
+    }
   }
+  // Without a bias, and with groups that count by one expert, the logits order as the choices do:
+  // exactly, but where 64 bits cannot tell two scores apart (neighbours closer than 1e-10, sigmoids
+  // above 10, scores under e^-600).  Else in 32 bits, u = 2^-24: a score is off by less than
+  // (24 + EPL) u of itself, a choice by its rounding too.
+  const bool direct = !a.bias && (!limited || a.group_top == 1);
+  constexpr float kU = 5.9604644775390625e-8f, kS = (48 + 2 * EPL) * kU, kC = 4 * kU;
+  const auto bound = [&](float c) { return direct ? 1e-10f : kS * (a.bias ? top : fabsf(c)) + kC * fabsf(c); };
+  const auto blurred = [&](float c) { return direct && !(c - zmax > -600.0f && (a.score == kSoftmax || c < 10.0f)); };
+  uint32_t key[EPL];
+  bool doubt = false;
 #pragma unroll
-  for (int j = 0; j < EPL; ++j)
-    key[j] = e0 + j < a.E ? key_of(s[j] + (a.bias ? (double)a.bias[e0 + j] : 0.0)) : 0;
-  if (a.groups > 1 && a.top_groups < a.groups) {
+  for (int j = 0; j < EPL; ++j) {
+    const float c = direct ? z[j] : s[j] + b[j];
+    key[j] = e0 + j < a.E ? key_of(c) : 0;
+    doubt |= e0 + j < a.E && !(c < __builtin_inff());  // NaN or infinite
+  }
+  if (limited) {
+    uint32_t* keys = keys32[slot];
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) keys[e0 + j] = key[j];
+    wave_sync();
+    float margin, worst;
+    const uint64_t kept = keep_groups<LANES, uint32_t, float>(a, keys, lane, margin, worst);
+    // two choices of up to `most` each on either side
     const int n = a.E / a.groups;
-#pragma unroll
-    for (int j = 0; j < EPL; ++j) sk[slot][e0 + j] = key[j];
-    __syncthreads();
-    // lane g < G ranks group g (LANES >= G, or a lane takes several)
-    uint64_t kept = 0;
-    uint64_t best[kGateMaxGroups / LANES > 0 ? kGateMaxGroups / LANES : 1];
-    constexpr int kPer = sizeof(best) / sizeof(best[0]);
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int g = sub * kPer + i;
-      uint64_t k1 = 0, k2 = 0;
-      if (g < a.groups)
-        for (int e = 0; e < n; ++e) {
-          const uint64_t v = sk[slot][g * n + e];
-          k2 = v > k1 ? k1 : (v > k2 ? v : k2);
-          k1 = v > k1 ? v : k1;
-        }
-      best[i] = g >= a.groups ? 0 : (a.group_top == 1 || n == 1 ? k1 : key_of(value_of(k1) + value_of(k2)));
-    }
-    for (int r = 0; r < a.top_groups; ++r) {
-      uint64_t m = 0;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) m = best[i] > m ? best[i] : m;
-      const uint64_t top = lanes_max<LANES>(m);
-      const int from = first_lane<LANES>(m == top, lane);
-      int g = 0;
-#pragma unroll
-      for (int i = kPer - 1; i >= 0; --i) g = best[i] == top ? i : g;
-      if (sub == from) {
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) best[i] = i == g ? 0 : best[i];
-      }
-      kept |= 1ull << __shfl(sub * kPer + g, (lane & ~(LANES - 1)) + from);
-    }
-#pragma unroll
-    for (int j = 0; j < EPL; ++j)
-      if (e0 + j < a.E && !(kept >> ((e0 + j) / n) & 1)) key[j] = 0;
-  }
-  // k rounds; lane j keeps the j-th expert and its score
-  int my_e = 0;
-  double my_s = 0;
-  for (int r = 0; r < a.k; ++r) {
-    uint64_t m = 0;
-#pragma unroll
-    for (int j = 0; j < EPL; ++j) m = key[j] > m ? key[j] : m;
-    const uint64_t top = lanes_max<LANES>(m);
-    const int from = first_lane<LANES>(m == top, lane);
-    int at = 0;
-#pragma unroll
-    for (int j = EPL - 1; j >= 0; --j) at = key[j] == top ? j : at;
-    double sv = 0;
+    int g = e0 / n, left = n - (e0 - g * n);  // the group of e0 + j and its experts from there on
+    float most = 0.0f;
 #pragma unroll
     for (int j = 0; j < EPL; ++j) {
-      sv = j == at ? s[j] : sv;
-      if (sub == from && j == at) key[j] = 0;
+      most = fmaxf(most, e0 + j < a.E ? fabsf(value_of(key[j])) : 0.0f);
+      if (!(kept >> g & 1)) key[j] = 0;
+      if (--left == 0) {
+        ++g;
+        left = n;
+      }
     }
-    const int src = (lane & ~(LANES - 1)) + from;
-    const int e = __shfl(e0 + at, src);
-    sv = __shfl(sv, src);
-    if (sub == r) {
-      my_e = e;
-      my_s = sv;
+    most = __uint_as_float(lanes_max<LANES>(__float_as_uint(most)));
+    doubt |= !(margin > 4 * bound(most) || (direct && margin == 0.0f)) || blurred(worst);
+  }
+  // lane r < k: the r-th expert, its choice, logit and bias (the lanes from k on as lane k - 1)
+  float my_c = value_of(top_k<LANES, EPL>(a.k, lane, key, chosen[slot]));
+  const int first = lane & ~(LANES - 1), last = first + a.k - 1;
+  int my_e = chosen[slot][sub < a.k ? sub : a.k - 1];
+  const auto z_of = [&](int e) { return load_elem(a.logits, DT, t * a.ldl + e); };
+  const float my_z = z_of(my_e), my_b = a.bias ? a.bias[my_e] : 0.0f;
+  const float my_s = a.score == kSigmoid ? sigmoid_of(my_z) : exp_of(my_z - zmax) * inv;
+  // in doubt: neighbours in the order that are near and no true tie, an expert not taken that is
+  // near the last one taken, and scores that 32 bits hardly hold
+  const int up = sub > 0 ? lane - 1 : lane;
+  const float c1 = __shfl(my_c, up), z1 = __shfl(my_z, up), b1 = __shfl(my_b, up);
+  doubt |= sub < a.k && ((sub > 0 && !(c1 - my_c > bound(fmaxf(fabsf(c1), fabsf(my_c)))) && !(z1 == my_z && b1 == my_b)) ||
+                         my_s < 1e-30f || !(fabsf(my_c) < __builtin_inff()) || blurred(my_c));
+  const float cl = __shfl(my_c, last), zl = __shfl(my_z, last), bl = __shfl(my_b, last), least = cl - bound(cl);
+  // (a key is 0 for an expert taken or left out: below that of any choice)
+  const uint32_t near = least < __builtin_inff() ? key_of(least) : 1u;
+  uint64_t at = 0;
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) at |= (uint64_t)(key[j] >= near) << j;
+  for (; at; at &= at - 1) {
+    const int e = e0 + (int)__builtin_ctzll(at);
+    doubt |= !(z_of(e) == zl && (a.bias ? a.bias[e] : 0.0f) == bl);
+  }
+  const float total = lanes_sum<LANES>(sub < a.k ? my_s : 0.0f) + (float)kEps;
+  float wt = (a.renormalize ? my_s / total : my_s) * a.scale;
+  const uint64_t doubts = __ballot(doubt);
+#pragma unroll 1
+  for (int q = 0; q < 64 / LANES; ++q) {
+    if (!(doubts >> (q * LANES) & (LANES == 64 ? ~0ull : (1ull << LANES % 64) - 1))) continue;  // the whole wave
+    int e;
+    double v;
+    rank64<DT>(a, __shfl(t, q * LANES), lane, keys64[threadIdx.x >> 6], e, v);
+    const double sum = lanes_sum<64>(v) + kEps;
+    const float wv = (float)((a.renormalize ? v / sum : v) * (double)a.scale);
+    const int e_r = __shfl(e, sub);
+    const float w_r = __shfl(wv, sub);
+    if (lane / LANES == q) {
+      my_e = e_r;
+      wt = w_r;
     }
   }
-  if (sub >= a.k) my_s = 0;
-  const double total = lanes_sum<LANES>(my_s) + kEps;
   if (live && sub < a.k) {
     idx[t * a.k + sub] = my_e;
-    w[t * a.k + sub] = (float)((a.renormalize ? my_s / total : my_s) * (double)a.scale);
+    w[t * a.k + sub] = wt;
   }
 }
 
-// Gradient of the logits; gs null: no gradient of the scores.
+// Gradient of the logits; gw or gs null: no gradient of the weights, of the scores.  The chosen
+// experts' terms go to their places through LDS.
 template <int LANES, int EPL, int WAVES, int DT>
 __global__ __launch_bounds__(64 * WAVES) void k_gate_bwd(GateArgs a, const int64_t* __restrict__ idx,
                                                          const float* __restrict__ gw, const float* __restrict__ gs,
                                                          void* __restrict__ dz) {
   constexpr int kTokens = 64 / LANES * WAVES;
+  __shared__ float place[kTokens][LANES * EPL];
   const int lane = threadIdx.x & 63, sub = lane & (LANES - 1);
-  const int64_t t0 = (int64_t)blockIdx.x * kTokens + threadIdx.x / LANES;
+  const int slot = threadIdx.x / LANES;
+  const int64_t t0 = (int64_t)blockIdx.x * kTokens + slot;
   const bool live = t0 < a.T;
   const int64_t t = live ? t0 : a.T - 1;
   const int e0 = sub * EPL;
+  const bool mine = gw && sub < a.k;
+  const int64_t e = mine ? idx[t * a.k + sub] : 0;
+  const bool there = mine && e >= 0 && e < a.E;
+  const float ze = there ? load_elem(a.logits, DT, t * a.ldl + e) : 0.0f;
+  const float g = there ? gw[t * a.k + sub] * a.scale : 0.0f;
   float z[EPL], s[EPL], ds[EPL];
-  load_logits(a, t, e0, z);
-  scores<LANES, EPL>(a.score, z, s);
+  load_row<DT, EPL>(a.logits, t * a.ldl, e0, a.E, -__builtin_inff(), z);
+  if (gs) {
+    load_row<CIN_DT_F32, EPL>(gs, t * a.E, e0, a.E, 0.0f, ds);
+  } else {
 #pragma unroll
-  for (int j = 0; j < EPL; ++j) ds[j] = gs && e0 + j < a.E ? gs[t * a.E + e0 + j] : 0.0f;
+    for (int j = 0; j < EPL; ++j) ds[j] = 0.0f;
+  }
+  float top, zmax, inv;
+  scores<LANES, EPL>(a.score, z, s, top, zmax, inv);
   if (gw) {
-    // lane j of the token: the chosen expert j, its weight's gradient and its score
-    const int my_e = sub < a.k ? (int)idx[t * a.k + sub] : -1;
-    const float g = sub < a.k ? gw[t * a.k + sub] * a.scale : 0.0f;
-    float my_s = 0.0f;
-    for (int r = 0; r < a.k; ++r) {
-      const int e = __shfl(my_e, (lane & ~(LANES - 1)) + r);
-      float v = 0.0f;
-#pragma unroll
-      for (int j = 0; j < EPL; ++j) v = e0 + j == e ? s[j] : v;
-      const float got = __shfl(v, (lane & ~(LANES - 1)) + e / EPL);
-      if (sub == r) my_s = got;
-    }
+    const float se = there ? (a.score == kSigmoid ? sigmoid_of(ze) : exp_of(ze - zmax) * inv) : 0.0f;
     float d = g;
     if (a.renormalize) {
-      const float total = lanes_sum<LANES>(my_s) + (float)kEps;
-      d = (g - lanes_sum<LANES>(g * my_s) / total) / total;
+      const float total = lanes_sum<LANES>(se) + (float)kEps;
+      d = (g - lanes_sum<LANES>(g * se) / total) / total;
     }
-    for (int r = 0; r < a.k; ++r) {
-      const int e = __shfl(my_e, (lane & ~(LANES - 1)) + r);
-      const float v = __shfl(d, (lane & ~(LANES - 1)) + r);
 #pragma unroll
-      for (int j = 0; j < EPL; ++j) ds[j] += e0 + j == e ? v : 0.0f;
-    }
+    for (int j = 0; j < EPL; ++j) place[slot][e0 + j] = 0.0f;
+    wave_sync();
+    if (there) place[slot][e] = d;
+    wave_sync();
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) ds[j] += place[slot][e0 + j];
   }
   if (a.score == kSoftmax) {
     float u = 0.0f;
@@ -263,29 +532,59 @@ __global__ __launch_bounds__(64 * WAVES) void k_gate_bwd(GateArgs a, const int64
     for (int j = 0; j < EPL; ++j) ds[j] = ds[j] * s[j] * (1.0f - s[j]);
   }
   if (!live) return;
+  constexpr int es = DT == CIN_DT_F32 ? 4 : 2;
+  uint8_t* q = static_cast<uint8_t*>(dz) + (t * a.E + e0) * es;
+  if (e0 + EPL <= a.E) {
+    if constexpr (DT == CIN_DT_F32) {
+      __builtin_memcpy(q, ds, 4 * EPL);
+    } else {
+      uint16_t h[EPL];
 #pragma unroll
-  for (int j = 0; j < EPL; ++j) {
-    if (e0 + j >= a.E) continue;
-    const int64_t at = t * a.E + e0 + j;
-    if constexpr (DT == CIN_DT_F32)
-      static_cast<float*>(dz)[at] = ds[j];
-    else
-      static_cast<uint16_t*>(dz)[at] = (uint16_t)f32_to_half_bits(DT, ds[j]);
+      for (int j = 0; j < EPL; ++j) h[j] = (uint16_t)f32_to_half_bits(DT, ds[j]);
+      __builtin_memcpy(q, h, 2 * EPL);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) {
+      if (e0 + j >= a.E) continue;
+      if constexpr (DT == CIN_DT_F32)
+        reinterpret_cast<float*>(q)[j] = ds[j];
+      else
+        reinterpret_cast<uint16_t*>(q)[j] = (uint16_t)f32_to_half_bits(DT, ds[j]);
+    }
   }
 }
 
-// launch(lanes, experts a lane, waves a workgroup)
+// launch(lanes, experts a lane, waves a workgroup, dtype)
 template <class F>
-void with_experts(int E, F launch) {
+void with_experts(int E, int dtype, F launch) {
   using std::integral_constant;
-  if (E <= 64)
-    launch(integral_constant<int, 64>{}, integral_constant<int, 1>{}, integral_constant<int, 4>{});
+  auto go = [&](auto lanes, auto epl, auto waves) {
+    if (dtype == CIN_DT_F32)
+      launch(lanes, epl, waves, integral_constant<int, CIN_DT_F32>{});
+    else if (dtype == CIN_DT_F16)
+      launch(lanes, epl, waves, integral_constant<int, CIN_DT_F16>{});
+    else
+      launch(lanes, epl, waves, integral_constant<int, CIN_DT_BF16>{});
+  };
+  const integral_constant<int, 16> row{};
+  const integral_constant<int, 64> wave{};
+  const integral_constant<int, 4> four{};
+  const integral_constant<int, 1> one{};
+  if (E <= 16)
+    go(row, integral_constant<int, 1>{}, four);
+  else if (E <= 32)
+    go(row, integral_constant<int, 2>{}, four);
+  else if (E <= 64)
+    go(row, integral_constant<int, 4>{}, four);
+  else if (E <= 128)
+    go(row, integral_constant<int, 8>{}, four);
   else if (E <= 256)
-    launch(integral_constant<int, 64>{}, integral_constant<int, 4>{}, integral_constant<int, 4>{});
+    go(row, integral_constant<int, 16>{}, four);
   else if (E <= 1024)
-    launch(integral_constant<int, 64>{}, integral_constant<int, 16>{}, integral_constant<int, 2>{});
+    go(wave, integral_constant<int, 16>{}, one);
   else
-    launch(integral_constant<int, 64>{}, integral_constant<int, 64>{}, integral_constant<int, 1>{});
+    go(wave, integral_constant<int, 64>{}, one);
 }
 
 int gate_args(const char* name, GateArgs& a, const void* logits, int dtype, int64_t ldl, const float* bias, int64_t T,
@@ -320,9 +619,9 @@ int cin_moe_gate(const void* logits, int dtype, int64_t ldl, const float* bias, 
     return rc;
   if (T == 0) return CIN_OK;
   CIN_CHECK_ARG(idx && weights, "moe_gate: null pointer");
-  with_experts((int)E, [&](auto lanes, auto epl, auto waves) {
+  with_experts((int)E, dtype, [&](auto lanes, auto epl, auto waves, auto dt) {
     constexpr int kTokens = 64 / lanes() * waves();
-    hipLaunchKernelGGL((k_gate_fwd<lanes(), epl(), waves()>), (unsigned)cdiv(T, kTokens), 64 * waves(), 0,
+    hipLaunchKernelGGL((k_gate_fwd<lanes(), epl(), waves(), dt()>), (unsigned)cdiv(T, kTokens), 64 * waves(), 0,
                        static_cast<hipStream_t>(stream), a, idx, weights, scores_out);
   });
   return cin_check_launch("moe_gate");
@@ -336,18 +635,10 @@ int cin_moe_gate_backward(const void* logits, int dtype, int64_t ldl, int64_t T,
     return rc;
   if (T == 0) return CIN_OK;
   CIN_CHECK_ARG(idx && dlogits, "moe_gate_backward: null pointer");
-  with_experts((int)E, [&](auto lanes, auto epl, auto waves) {
+  with_experts((int)E, dtype, [&](auto lanes, auto epl, auto waves, auto dt) {
     constexpr int kTokens = 64 / lanes() * waves();
-    auto go = [&](auto dt) {
-      hipLaunchKernelGGL((k_gate_bwd<lanes(), epl(), waves(), dt()>), (unsigned)cdiv(T, kTokens), 64 * waves(), 0,
-                         static_cast<hipStream_t>(stream), a, idx, gweights, gscores, dlogits);
-    };
-    if (dtype == CIN_DT_F32)
-      go(std::integral_constant<int, CIN_DT_F32>{});
-    else if (dtype == CIN_DT_F16)
-      go(std::integral_constant<int, CIN_DT_F16>{});
-    else
-      go(std::integral_constant<int, CIN_DT_BF16>{});
+    hipLaunchKernelGGL((k_gate_bwd<lanes(), epl(), waves(), dt()>), (unsigned)cdiv(T, kTokens), 64 * waves(), 0,
+                       static_cast<hipStream_t>(stream), a, idx, gweights, gscores, dlogits);
   });
   return cin_check_launch("moe_gate_backward");
 }
