@@ -126,7 +126,7 @@ struct Operand {
     if constexpr (ACROSS) {
       const int64_t left = kleft - (int64_t)kt * BK;
       // K rows past the last read as zero, and nothing is read past the last row's end
-      rsrc = make_rsrc(p + (int64_t)kt * BK * ldb, ((left < BK ? left : BK) - 1) * ldb + width);
+      rsrc = make_rsrc(p + (int64_t)kt * BK * ldb, left > 0 ? ((left < BK ? left : BK) - 1) * ldb + width : 0);
     } else {
       so = (uint32_t)kt * 128;
     }
@@ -244,20 +244,35 @@ __global__ __launch_bounds__(C::kThreads, 2) void k_ce_gemm(GemmArgs g) {
   const int64_t nl = n0 + wn * NT * 16 + 4 * kq;
   if constexpr (EPI == kStats) {
     float2* st = reinterpret_cast<float2*>(smem);
+    if (n0 + C::TN > g.N) {  // columns past the vocabulary add nothing
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (nl + j * 16 + r >= g.N) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) acc[i][j][r] = -__builtin_inff();
+          }
+    }
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       const int ml = (wm * MT + i) * 16 + l16;
       const bool in = m0 + ml < M;
+      // (few waves hold a row's target)
       const int64_t at = (in ? g.target[m0 + ml] : -1) - nl;
-      float mx = -__builtin_inff();
+      if (at >= 0 && at < NT * 16 && (at & 15) < 4) {
+        float z = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) z = (int)at == j * 16 + r ? acc[i][j][r] : z;
+        g.ztarget[m0 + ml] = z;
+      }
+      float mx = acc[i][0][0];
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if (at == j * 16 + r) g.ztarget[m0 + ml] = acc[i][j][r];
-          if (nl + j * 16 + r >= g.N) acc[i][j][r] = -__builtin_inff();
-          mx = fmaxf(mx, acc[i][j][r]);
-        }
+        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, acc[i][j][r]);
       mx = fmaxf(mx, __shfl_xor(mx, 16));
       mx = fmaxf(mx, __shfl_xor(mx, 32));
       float s = 0.0f;
@@ -312,15 +327,28 @@ __global__ __launch_bounds__(C::kThreads, 2) void k_ce_gemm(GemmArgs g) {
       const int64_t m = m0 + (wm * MT + i) * 16 + l16;
       const bool in = m < M;
       const float mx = in ? g.rowmax[m] : 0.0f, inv = in ? g.inv[m] : 0.0f, cf = in ? g.coef[m] : 0.0f;
-      const int64_t at = (in ? g.target[m] : -1) - g.v0 - nl;
+      const float pc = inv * cf;
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float p = exp_of(acc[i][j][r] - mx) * inv;
-          // columns past the vocabulary are part of the next products' K
-          acc[i][j][r] = g.v0 + nl + j * 16 + r < g.V ? (at == j * 16 + r ? p - 1.0f : p) * cf : 0.0f;
-        }
+        for (int r = 0; r < 4; ++r) acc[i][j][r] = exp_of(acc[i][j][r] - mx) * pc;
+      const int64_t at = (in ? g.target[m] : -1) - g.v0 - nl;
+      if (at >= 0 && at < NT * 16 && (at & 15) < 4) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[i][j][r] -= (int)at == j * 16 + r ? cf : 0.0f;
+      }
+    }
+    if (g.v0 + n0 + C::TN > g.V) {  // columns past the vocabulary are part of the next products' K
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (g.v0 + nl + j * 16 + r >= g.V) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) acc[i][j][r] = 0.0f;
+          }
     }
   } else {
 #pragma unroll
