@@ -10,8 +10,11 @@
 // of exponentials and the target's logit.  Backward: by pieces of the vocabulary, a product that
 // ends in dz of the piece (in x's type), then dx += dz w and dw = dz^T x of the piece.
 //
-// One kernel runs the three products, on the matrix units in x's type (bf16, fp16 or fp32) with
-// fp32 sums.  An operand is read along K (its rows hold K) or across it (its rows are K), so no
+// One kernel runs the three products on the matrix units, with fp32 sums.  fp32 values are held as
+// three bf16 ones (x = x0 + x1 + x2, each the rounding of what is left, exact to 2^-26), and their
+// product is the six products of planes down to x0 y2, the small ones first: what is dropped lies
+// under 2^-26 of |x y|, and the sums are those of fp32 products (2046 x 32000 x 1024: 0.72 ms, 187
+// TFLOP/s; on the fp32 matrix units, in the same tiles, 1.04 ms).  An operand is read along K (its rows hold K) or across it (its rows are K), so no
 // transposed copy of x, w or dz is ever made.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -35,8 +38,8 @@ typedef short s4 __attribute__((ext_vector_type(4)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 
-template <int DT>
-constexpr int kEs = DT == CIN_DT_F32 ? 4 : 2;
+constexpr int kEs = 2;  // bytes of an operand's element: bf16 or fp16
+constexpr int BK = 64;  // elements of a K step
 
 // Workgroup tile of 16 MT WM x 16 NT WN, K steps of 128 bytes.
 template <int WM_, int WN_, int MT_, int NT_>
@@ -51,18 +54,19 @@ struct Cfg {
 // What a product ends in.
 enum Epi {
   kStats,  // the row's maximum and sum of exponentials over the tile, and the target's logit
-  kGrad,   // dz, in the operands' type
+  kGrad,   // dz, in the operands' type (three planes of it for fp32)
   kSlab,   // fp32 partial sums (added to what is there with `add`)
-  kFinal   // times a device scalar, in the operands' type
+  kFinal   // times a device scalar, in x's type
 };
 
 struct GemmArgs {
   const void *A, *B;
   int64_t lda, ldb;
+  int64_t plane_a, plane_b;  // bytes between the planes of an fp32 operand
   int64_t M, N, K;     // N: columns to compute; K: a multiple of a K step where an operand holds K in its rows
   const int* n;        // rows there are, in place of M (or of K for kFinal)
   int splits;          // parts of K, one slab each
-  int64_t ldc, slab;   // elements between rows of C, between slabs
+  int64_t ldc, slab;   // elements between rows of C, between slabs (or planes of dz)
   void* C;
   int add;
   int64_t v0, V;       // first column of the piece and columns of the vocabulary
@@ -77,67 +81,66 @@ struct GemmArgs {
 // Along K: LDS rows are tile rows of 128 bytes, 16-byte chunk c of row r at slot c ^ f(r).
 // Across K: LDS rows are the step's K rows of ROWS elements, in granules of 16 elements, granule
 // q of row r at q ^ f(r): the rows that one transposing read takes together lie on other banks.
-template <int DT, int ROWS, int THREADS, bool ACROSS>
+template <int ROWS, int THREADS, bool ACROSS>
 struct Operand {
-  static constexpr int es = kEs<DT>, BK = 128 / es;
   static constexpr int kOps = ROWS * 8 / THREADS;
-  static constexpr int kCpr = ACROSS ? ROWS * es / 16 : 8;  // 16-byte chunks of an LDS row
-  static constexpr int kGc = es;                            // chunks of a granule (across)
-  static constexpr int kGran = kCpr / kGc;
+  static constexpr int kCpr = ACROSS ? ROWS * kEs / 16 : 8;  // 16-byte chunks of an LDS row
+  static constexpr int kGran = kCpr / 2;                     // granules of 16 elements (across)
   static_assert(ROWS * 8 % THREADS == 0, "whole operations");
   uint32_t voff[kOps];
-  __amdgpu_buffer_rsrc_t rsrc;
   const uint8_t* p;
-  int64_t ldb, kleft, width;
+  int64_t ldb, kleft, bytes;
   uint32_t lds;
 
   __device__ static inline int f(int r) {
     if constexpr (!ACROSS) return swz_f(r);
-    if constexpr (es == 2) return ((r & 3) | ((r >> 3 & 1) << 2)) & (kGran - 1);
-    return (r >> 2) & 3 & (kGran - 1);
+    return ((r & 3) | ((r >> 3 & 1) << 2)) & (kGran - 1);
   }
   // r0: the tile's first row (along) or column (across); valid: rows (along) or columns (across)
   // from there on; k0, k1: the K range that there is
   __device__ __forceinline__ void init(const void* base, int64_t ld, int64_t r0, int64_t valid, int64_t k0, int64_t k1,
                                        int tid, uint32_t lds0) {
-    ldb = ld * es;
-    width = valid * es;
+    ldb = ld * kEs;
     lds = lds0 + (uint32_t)__builtin_amdgcn_readfirstlane(tid >> 6) * 1024;
     kleft = k1 - k0;
     if constexpr (ACROSS) {
-      p = static_cast<const uint8_t*>(base) + k0 * ldb + r0 * es;
+      p = static_cast<const uint8_t*>(base) + k0 * ldb + r0 * kEs;
+      bytes = valid * kEs;  // of the last K row
     } else {
       const int rows = (int)(valid < ROWS ? valid : ROWS);
-      p = static_cast<const uint8_t*>(base) + r0 * ldb + k0 * es;
-      rsrc = make_rsrc(p, (rows - 1) * ldb + kleft * es);
+      p = static_cast<const uint8_t*>(base) + r0 * ldb + k0 * kEs;
+      bytes = (rows - 1) * ldb + kleft * kEs;
     }
 #pragma unroll
     for (int i = 0; i < kOps; ++i) {
       const int slot = i * THREADS + tid, r = slot / kCpr, c = slot % kCpr;
       if constexpr (ACROSS) {
-        voff[i] = (uint32_t)(r * ldb) + (uint32_t)((((c / kGc) ^ f(r)) * kGc + c % kGc) * 16);
+        voff[i] = (uint32_t)(r * ldb) + (uint32_t)((((c / 2) ^ f(r)) * 2 + c % 2) * 16);
       } else {
         voff[i] = r < valid ? (uint32_t)(r * ldb) + (uint32_t)((c ^ f(r)) * 16) : kOut;
       }
     }
   }
-  __device__ __forceinline__ void fetch(int kt, uint32_t stage) {
+  // K step kt of the plane that lies `plane` bytes on
+  __device__ __forceinline__ void fetch(int kt, int64_t plane, uint32_t stage) {
+    __amdgpu_buffer_rsrc_t rsrc;
     uint32_t so = 0;
     if constexpr (ACROSS) {
       const int64_t left = kleft - (int64_t)kt * BK;
       // K rows past the last read as zero, and nothing is read past the last row's end
-      rsrc = make_rsrc(p + (int64_t)kt * BK * ldb, left > 0 ? ((left < BK ? left : BK) - 1) * ldb + width : 0);
+      rsrc = make_rsrc(p + plane + (int64_t)kt * BK * ldb, left > 0 ? ((left < BK ? left : BK) - 1) * ldb + bytes : 0);
     } else {
-      so = (uint32_t)kt * 128;
+      rsrc = make_rsrc(p + plane, bytes);
+      so = (uint32_t)__builtin_amdgcn_readfirstlane(kt) * 128;
     }
 #pragma unroll
     for (int i = 0; i < kOps; ++i) dma16(rsrc, voff[i], so, lds + stage + i * THREADS * 16);
   }
-  // 16 bytes a lane: K elements 8 kq .. + 7 of half ks (fp32: 4 kq .. + 3) of tile row r16 + l16
+  // 16 bytes a lane: K elements 8 kq .. + 7 of half ks of tile row r16 + l16
   __device__ static __forceinline__ v4u frag(const uint8_t* st, int r16, int ks, int l16, int kq) {
     if constexpr (!ACROSS) {
       return *reinterpret_cast<const v4u*>(st + (r16 + l16) * 128 + (((4 * ks + kq) ^ f(r16 + l16)) << 4));
-    } else if constexpr (es == 2) {
+    } else {
       v4u v;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -149,14 +152,6 @@ struct Operand {
         v[2 * h + 1] = u.y;
       }
       return v;
-    } else {
-      v4u v;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int k = 16 * ks + 4 * kq + e;
-        v[e] = *reinterpret_cast<const uint32_t*>(st + k * (ROWS * 4) + ((((r16 >> 4)) ^ f(k)) << 6) + l16 * 4);
-      }
-      return v;
     }
   }
 };
@@ -164,14 +159,17 @@ struct Operand {
 // c += a b over a half step: lane (l16, kq) holds column l16 of b and rows 4 kq .. + 3 of a
 template <int DT>
 __device__ __forceinline__ v4f mma(v4u a, v4u b, v4f c) {
-  if constexpr (DT == CIN_DT_BF16)
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
   if constexpr (DT == CIN_DT_F16)
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-    c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[e]), __uint_as_float(b[e]), c, 0, 0, 0);
-  return c;
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+}
+
+// The planes of the products of an fp32 operand pair, small terms first.
+constexpr int kPairs32 = 6;
+__device__ inline void planes_of(int seg, int& a, int& b) {
+  a = seg == 0 ? 2 : (seg == 1 || seg == 3 ? 1 : 0);
+  b = seg == 2 ? 2 : (seg == 1 || seg == 4 ? 1 : 0);
 }
 
 __device__ inline float exp_of(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
@@ -179,7 +177,7 @@ __device__ inline float exp_of(float d) { return __builtin_amdgcn_exp2f(d * kLog
 template <class C, int DT, int EPI>
 __global__ __launch_bounds__(C::kThreads, 2) void k_ce_gemm(GemmArgs g) {
   constexpr bool kAcrossA = EPI == kFinal, kAcrossB = EPI == kSlab || EPI == kFinal;
-  constexpr int MT = C::MT, NT = C::NT, BK = 128 / kEs<DT>;
+  constexpr int MT = C::MT, NT = C::NT, kSegs = DT == CIN_DT_F32 ? kPairs32 : 1;
   __shared__ __attribute__((aligned(128))) uint8_t smem[C::kBytes];
   const int64_t rows = __builtin_amdgcn_readfirstlane(*g.n);
   const int64_t M = EPI == kFinal ? g.M : rows, Kall = EPI == kFinal ? rows : g.K;
@@ -200,8 +198,8 @@ __global__ __launch_bounds__(C::kThreads, 2) void k_ce_gemm(GemmArgs g) {
   const int wm = wave / C::WN, wn = wave % C::WN;
   const int l16 = lane & 15, kq = lane >> 4;
   const uint32_t lds0 = (uint32_t)(uintptr_t)smem;
-  Operand<DT, C::TM, C::kThreads, kAcrossA> oa;
-  Operand<DT, C::TN, C::kThreads, kAcrossB> ob;
+  Operand<C::TM, C::kThreads, kAcrossA> oa;
+  Operand<C::TN, C::kThreads, kAcrossB> ob;
   v4f acc[MT][NT];
 #pragma unroll
   for (int i = 0; i < MT; ++i)
@@ -213,17 +211,30 @@ __global__ __launch_bounds__(C::kThreads, 2) void k_ce_gemm(GemmArgs g) {
     oa.init(g.A, g.lda, m0, (kAcrossA ? g.wa : M) - m0, k0, k1, tid, lds0);
     ob.init(g.B, g.ldb, n0, (kAcrossB ? g.wb : g.V - g.v0) - n0, k0,
             EPI == kSlab && k1 > g.V - g.v0 ? g.V - g.v0 : k1, tid, lds0 + C::TM * 128);
-    oa.fetch(0, 0);
-    ob.fetch(0, 0);
   }
-  for (int kt = 0; kt < nk; ++kt) {
+  int fk = 0, seg = 0;  // the K step and pair of planes that are fetched next
+  const auto fetch = [&](uint32_t stage) {
+    int64_t pa = 0, pb = 0;
+    if constexpr (kSegs > 1) {
+      int ia, ib;
+      planes_of(seg, ia, ib);
+      pa = ia * g.plane_a;
+      pb = ib * g.plane_b;
+    }
+    oa.fetch(fk, pa, stage);
+    ob.fetch(fk, pb, stage);
+    if (++fk == nk) {
+      fk = 0;
+      ++seg;
+    }
+  };
+  const int steps = nk * kSegs;
+  if (steps > 0) fetch(0);
+  for (int kt = 0; kt < steps; ++kt) {
     wait_dma();
     lds_barrier();
     const uint32_t st = (kt & 1) * C::kStage;
-    if (kt + 1 < nk) {
-      oa.fetch(kt + 1, C::kStage - st);
-      ob.fetch(kt + 1, C::kStage - st);
-    }
+    if (kt + 1 < steps) fetch(C::kStage - st);
     const uint8_t* sa = smem + st;
     const uint8_t* sb = sa + C::TM * 128;
 #pragma unroll
@@ -359,7 +370,7 @@ __global__ __launch_bounds__(C::kThreads, 2) void k_ce_gemm(GemmArgs g) {
         for (int r = 0; r < 4; ++r) acc[i][j][r] *= scale;
   }
   const int64_t N = g.N;
-  if constexpr (DT == CIN_DT_F32) {
+  if constexpr (DT == CIN_DT_F32 && EPI == kFinal) {
     float* out = static_cast<float*>(g.C);
     const bool whole = (g.ldc & 3) == 0 && ((uintptr_t)out & 15) == 0;
 #pragma unroll
@@ -378,19 +389,30 @@ __global__ __launch_bounds__(C::kThreads, 2) void k_ce_gemm(GemmArgs g) {
         }
       }
     }
-  } else {
-    // rows through LDS, so that the stores run along them
+    return;
+  }
+  // 16-bit rows through LDS, so that the stores run along them; for fp32 one plane after the other
+  constexpr int kHalf = DT == CIN_DT_F16 ? CIN_DT_F16 : CIN_DT_BF16;
+  constexpr int kChunks = C::TN / 8;
+  const bool whole = (g.ldc & 7) == 0 && ((uintptr_t)g.C & 15) == 0;
+#pragma unroll 1
+  for (int plane = 0; plane < (DT == CIN_DT_F32 ? 3 : 1); ++plane) {
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
-        *reinterpret_cast<uint2*>(smem + ((wm * MT + i) * 16 + l16) * C::kCStride + ((wn * NT + j) * 16 + kq * 4) * 2) =
-            make_uint2(f32x2_to_half2_bits<DT>(acc[i][j][0], acc[i][j][1]),
-                       f32x2_to_half2_bits<DT>(acc[i][j][2], acc[i][j][3]));
+      for (int j = 0; j < NT; ++j) {
+        const uint2 h = make_uint2(f32x2_to_half2_bits<kHalf>(acc[i][j][0], acc[i][j][1]),
+                                   f32x2_to_half2_bits<kHalf>(acc[i][j][2], acc[i][j][3]));
+        *reinterpret_cast<uint2*>(smem + ((wm * MT + i) * 16 + l16) * C::kCStride + ((wn * NT + j) * 16 + kq * 4) * 2) = h;
+        if constexpr (DT == CIN_DT_F32) {
+          acc[i][j][0] -= bf16_lo(h.x);
+          acc[i][j][1] -= bf16_hi(h.x);
+          acc[i][j][2] -= bf16_lo(h.y);
+          acc[i][j][3] -= bf16_hi(h.y);
+        }
+      }
     __syncthreads();
-    uint16_t* out = static_cast<uint16_t*>(g.C);
-    const bool whole = (g.ldc & 7) == 0 && ((uintptr_t)out & 15) == 0;
-    constexpr int kChunks = C::TN / 8;
+    uint16_t* out = static_cast<uint16_t*>(g.C) + plane * g.slab;
     for (int q = tid; q < C::TM * kChunks; q += C::kThreads) {
       const int m = q / kChunks, n = (q % kChunks) * 8;
       if (m0 + m >= M || n0 + n >= N) continue;
@@ -404,6 +426,7 @@ __global__ __launch_bounds__(C::kThreads, 2) void k_ce_gemm(GemmArgs g) {
           if (n0 + n + e < N) d[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
       }
     }
+    if constexpr (DT == CIN_DT_F32) __syncthreads();
   }
 }
 
@@ -463,24 +486,39 @@ __global__ __launch_bounds__(kRowThreads) void k_ce_rows(const int64_t* __restri
   if (tid == 0) *n = base;
 }
 
-// Rows of x (all, or map's first *n) with zeros up to Dp columns.
-template <int ES>
+// Rows of x (all, or map's first *n) with zeros up to Dp columns; fp32 rows as three bf16 planes.
+template <bool F32>
 __global__ __launch_bounds__(256) void k_ce_copy(const void* __restrict__ x, int64_t ldx, int64_t rows, int64_t D,
                                                  const int* __restrict__ map, const int* __restrict__ n,
-                                                 void* __restrict__ out, int64_t Dp) {
-  using E = std::conditional_t<ES == 4, uint32_t, uint16_t>;
-  constexpr int kPer = 16 / ES;
-  const int64_t pieces = Dp / kPer, have = n ? *n : rows;
-  const bool whole = ((uintptr_t)x & 15) == 0 && ldx % kPer == 0;
+                                                 uint16_t* __restrict__ out, int64_t Dp, int64_t plane) {
+  using E = std::conditional_t<F32, float, uint16_t>;
+  const int64_t pieces = Dp / 8, have = n ? *n : rows;
+  const bool whole = ((uintptr_t)x & 15) == 0 && ldx % (16 / (int)sizeof(E)) == 0;
   for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < have * pieces; q += (int64_t)gridDim.x * 256) {
-    const int64_t i = q / pieces, c = (q - i * pieces) * kPer;
+    const int64_t i = q / pieces, c = (q - i * pieces) * 8;
     const E* s = static_cast<const E*>(x) + (map ? (int64_t)map[i] : i) * ldx + c;
-    E* d = static_cast<E*>(out) + i * Dp + c;
-    if (whole && c + kPer <= D) {
-      *reinterpret_cast<v4u*>(d) = *reinterpret_cast<const v4u*>(s);
+    uint16_t* d = out + i * Dp + c;
+    E v[8];
+    if (whole && c + 8 <= D) {
+      __builtin_memcpy(v, __builtin_assume_aligned(s, 16), sizeof(v));
     } else {
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) d[e] = c + e < D ? s[e] : (E)0;
+      for (int e = 0; e < 8; ++e) v[e] = c + e < D ? s[e] : (E)0;
+    }
+    if constexpr (F32) {
+#pragma unroll
+      for (int p = 0; p < 3; ++p) {
+        v4u h;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          h[e] = f32x2_to_bf16x2_bits(v[2 * e], v[2 * e + 1]);
+          v[2 * e] -= bf16_lo(h[e]);
+          v[2 * e + 1] -= bf16_hi(h[e]);
+        }
+        *reinterpret_cast<v4u*>(d + p * plane) = h;
+      }
+    } else {
+      __builtin_memcpy(__builtin_assume_aligned(d, 16), v, 16);
     }
   }
 }
@@ -621,7 +659,7 @@ constexpr int64_t kMaxPiece = (int64_t)1 << 20;    // its columns: 256 rows lie 
 int64_t align_up(int64_t v, int64_t a) { return cdiv(v, a) * a; }
 
 struct Plan {
-  int es;
+  int planes;           // of an operand: 3 for fp32
   int64_t Dp;           // columns of x and w as the products read them
   int64_t tiles_n;      // column tiles of the forward product
   int64_t piece, ldz;   // columns of a piece, elements between rows of dz
@@ -632,23 +670,23 @@ struct Plan {
 
 Plan make_plan(int dtype, int64_t T, int64_t D, int64_t V) {
   Plan p;
-  p.es = dtype == CIN_DT_F32 ? 4 : 2;
-  p.Dp = align_up(D, 128 / p.es);
+  p.planes = dtype == CIN_DT_F32 ? 3 : 1;
+  p.Dp = align_up(D, BK);
   p.tiles_n = cdiv(V, Big::TN);
   const int64_t Tp = T > 0 ? T : 1;
-  int64_t most = align_up(kPieceBytes / (Tp * p.es) + 1, Big::TN);
+  int64_t most = align_up(kPieceBytes / (Tp * kEs * p.planes) + 1, Big::TN);
   if (most > kMaxPiece) most = kMaxPiece;
   const int64_t pieces = cdiv(V, most);
   p.piece = align_up(cdiv(V, pieces), Big::TN);
   p.ldz = p.piece + 64;  // rows not a multiple of 16 KiB apart
   const int64_t tiles = cdiv(Tp, Big::TM) * cdiv(p.Dp, Big::TN);
   int64_t s = tiles >= 192 ? 1 : 256 / tiles;
-  const int64_t steps = p.piece * p.es / 128;
+  const int64_t steps = p.piece / BK;
   if (s > steps / 8) s = steps / 8;
   p.splits = (int)(s < 1 ? 1 : s);
   p.part = align_up(Tp * p.tiles_n * 8, 256);
   p.ztarget = align_up(Tp * 4, 256);
-  p.dz = align_up(Tp * p.ldz * p.es, 256);
+  p.dz = align_up(p.planes * Tp * p.ldz * kEs, 256);
   p.slabs = align_up(p.splits * Tp * p.Dp * 4, 256);
   p.coef = align_up((Tp + 1) * 4, 256);
   return p;
@@ -663,9 +701,8 @@ int check(const char* name, int dtype, int64_t T, int64_t D, int64_t V) {
   return CIN_OK;
 }
 
-bool w_fits(const void* w, int dtype, int64_t ldw) {
-  const int es = dtype == CIN_DT_F32 ? 4 : 2;
-  return ((uintptr_t)w & 15) == 0 && ldw * es % 16 == 0 && ldw <= 4 * kMaxD;
+bool w_fits(const void* w, int64_t ldw) {
+  return ((uintptr_t)w & 15) == 0 && ldw * kEs % 16 == 0 && ldw <= 4 * kMaxD;
 }
 
 template <class F>
@@ -686,14 +723,15 @@ void gemm(int dtype, const GemmArgs& g, int64_t max_m, hipStream_t s) {
   });
 }
 
-void copy_rows(int es, const void* x, int64_t ldx, int64_t rows, int64_t D, const int* map, const int* n, void* out,
+void copy_rows(bool f32, const void* x, int64_t ldx, int64_t rows, int64_t D, const int* map, const int* n, void* out,
                int64_t Dp, hipStream_t s) {
-  const int64_t blocks = cdiv(rows * (Dp * es / 16), 256);
+  const int64_t blocks = cdiv(rows * (Dp / 8), 256);
   const unsigned grid = (unsigned)(blocks < 8192 ? blocks : 8192);
-  if (es == 4)
-    hipLaunchKernelGGL(k_ce_copy<4>, grid, 256, 0, s, x, ldx, rows, D, map, n, out, Dp);
+  uint16_t* o = static_cast<uint16_t*>(out);
+  if (f32)
+    hipLaunchKernelGGL(k_ce_copy<true>, grid, 256, 0, s, x, ldx, rows, D, map, n, o, Dp, rows * Dp);
   else
-    hipLaunchKernelGGL(k_ce_copy<2>, grid, 256, 0, s, x, ldx, rows, D, map, n, out, Dp);
+    hipLaunchKernelGGL(k_ce_copy<false>, grid, 256, 0, s, x, ldx, rows, D, map, n, o, Dp, rows * Dp);
 }
 
 // The int32 state: n, then map, pos and target of T entries each.
@@ -721,7 +759,8 @@ int cin_linear_ce_forward(const void* x, int dtype, int64_t T, int64_t D, int64_
   CIN_CHECK_ARG(ldx >= D && ldw >= D, "%s: rows overlap", name);
   CIN_CHECK_ARG(state_i && w && (T == 0 || (x && target && xc && state_f && rowloss)), "%s: null pointer", name);
   const Plan p = make_plan(dtype, T, D, V);
-  CIN_CHECK_ARG(wp || (w_fits(w, dtype, ldw) && p.Dp == D), "%s: w needs a padded copy", name);
+  const bool f32 = dtype == CIN_DT_F32;
+  CIN_CHECK_ARG(wp || (!f32 && w_fits(w, ldw) && p.Dp == D), "%s: w needs a padded copy", name);
   CIN_CHECK_ARG(workspace_bytes >= p.part + p.ztarget && workspace, "%s: workspace needs %lld bytes", name,
                 (long long)(p.part + p.ztarget));
   hipStream_t s = static_cast<hipStream_t>(stream);
@@ -730,13 +769,15 @@ int cin_linear_ce_forward(const void* x, int dtype, int64_t T, int64_t D, int64_
   float* zt = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.part);
   hipLaunchKernelGGL(k_ce_rows, 1, kRowThreads, 0, s, target, T, V, ignore_index, st.map, st.pos, st.target, st.n, rowloss);
   if (T > 0) {
-    copy_rows(p.es, x, ldx, T, D, st.map, st.n, xc, p.Dp, s);
-    if (wp) copy_rows(p.es, w, ldw, V, D, nullptr, nullptr, wp, p.Dp, s);
+    copy_rows(f32, x, ldx, T, D, st.map, st.n, xc, p.Dp, s);
+    if (wp) copy_rows(f32, w, ldw, V, D, nullptr, nullptr, wp, p.Dp, s);
     GemmArgs g{};
     g.A = xc;
     g.lda = p.Dp;
     g.B = wp ? wp : w;
     g.ldb = wp ? p.Dp : ldw;
+    g.plane_a = T * p.Dp * kEs;
+    g.plane_b = V * p.Dp * kEs;
     g.N = g.V = V;
     g.K = p.Dp;
     g.n = st.n;
@@ -758,7 +799,8 @@ int cin_linear_ce_backward(const void* xc, int dtype, int64_t T, int64_t D, cons
   const char* name = "linear_ce_backward";
   if (int rc = check(name, dtype, T, D, V)) return rc;
   const Plan p = make_plan(dtype, T, D, V);
-  CIN_CHECK_ARG(w_fits(w, dtype, ldw) && ldw >= p.Dp, "%s: w's rows must be padded as the forward's", name);
+  CIN_CHECK_ARG(w_fits(w, ldw) && (dtype == CIN_DT_F32 ? ldw == p.Dp : ldw >= p.Dp),
+                "%s: w's rows must be padded as the forward's", name);
   CIN_CHECK_ARG(grad_stride >= 0, "%s: negative gradient stride", name);
   CIN_CHECK_ARG(T > 0 && state_i && state_f && xc && w && grad, "%s: null pointer", name);
   CIN_CHECK_ARG(workspace && workspace_bytes >= p.dz + p.slabs + p.coef, "%s: workspace needs %lld bytes", name,
@@ -778,14 +820,17 @@ int cin_linear_ce_backward(const void* xc, int dtype, int64_t T, int64_t D, cons
     GemmArgs g{};
     g.A = xc;
     g.lda = p.Dp;
-    g.B = wb + v0 * ldw * p.es;
+    g.B = wb + v0 * ldw * kEs;
     g.ldb = ldw;
-    g.N = align_up(cols, 128 / p.es);  // with the zeros that fill the next product's last K step
+    g.plane_a = T * p.Dp * kEs;
+    g.plane_b = V * p.Dp * kEs;
+    g.N = align_up(cols, BK);  // with the zeros that fill the next product's last K step
     g.K = p.Dp;
     g.n = st.n;
     g.splits = 1;
     g.C = dz;
     g.ldc = p.ldz;
+    g.slab = T * p.ldz;
     g.v0 = v0;
     g.V = V;
     g.target = st.target;
@@ -799,11 +844,13 @@ int cin_linear_ce_backward(const void* xc, int dtype, int64_t T, int64_t D, cons
     h.lda = p.ldz;
     h.wa = p.ldz;
     h.wb = p.Dp;
+    h.plane_a = T * p.ldz * kEs;
     h.v0 = v0;
     h.V = V;
     if (dx) {
       h.B = g.B;
       h.ldb = ldw;
+      h.plane_b = g.plane_b;
       h.N = p.Dp;
       h.K = g.N;
       h.splits = p.splits;
@@ -816,10 +863,11 @@ int cin_linear_ce_backward(const void* xc, int dtype, int64_t T, int64_t D, cons
     if (dw) {
       h.B = xc;
       h.ldb = p.Dp;
+      h.plane_b = g.plane_a;
       h.M = cols;
       h.N = D;
       h.splits = 1;
-      h.C = static_cast<char*>(dw) + v0 * D * p.es;
+      h.C = static_cast<char*>(dw) + v0 * D * (dtype == CIN_DT_F32 ? 4 : 2);
       h.ldc = D;
       h.out_scale = out_scale;
       gemm<kFinal>(dtype, h, cols, s);
