@@ -17,6 +17,7 @@
 // TFLOP/s; on the fp32 matrix units, in the same tiles, 1.04 ms).  An operand is read along K (its rows hold K) or across it (its rows are K), so no
 // transposed copy of x, w or dz is ever made.
 #include <hip/hip_runtime.h>
+#include <math.h>
 #include <stdint.h>
 
 #include <type_traits>
@@ -41,14 +42,21 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 constexpr int kEs = 2;  // bytes of an operand's element: bf16 or fp16
 constexpr int BK = 64;  // elements of a K step
 
-// Workgroup tile of 16 MT WM x 16 NT WN, K steps of 128 bytes.
-template <int WM_, int WN_, int MT_, int NT_>
+// s_waitcnt vmcnt(N): everything but the last N vector memory operations has completed
+template <int N>
+__device__ __forceinline__ void wait_dma_but() {
+  static_assert(N >= 0 && N < 64, "vmcnt has 6 bits");
+  __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | (N >> 4 << 14));
+}
+
+// Workgroup tile of 16 MT WM x 16 NT WN, K steps of 128 bytes in STAGES LDS stages.
+template <int WM_, int WN_, int MT_, int NT_, int STAGES>
 struct Cfg {
-  static constexpr int WM = WM_, WN = WN_, MT = MT_, NT = NT_;
+  static constexpr int WM = WM_, WN = WN_, MT = MT_, NT = NT_, kStages = STAGES;
   static constexpr int kThreads = 64 * WM * WN, TM = 16 * MT * WM, TN = 16 * NT * WN;
   static constexpr int kStage = (TM + TN) * 128;
   static constexpr int kCStride = TN * 2 + 16;  // a staged row of 16-bit results; rows 4 banks apart
-  static constexpr int kBytes = 2 * kStage > TM * kCStride ? 2 * kStage : TM * kCStride;
+  static constexpr int kBytes = STAGES * kStage > TM * kCStride ? STAGES * kStage : TM * kCStride;
 };
 
 // What a product ends in.
@@ -229,12 +237,21 @@ __global__ __launch_bounds__(C::kThreads, 2) void k_ce_gemm(GemmArgs g) {
     }
   };
   const int steps = nk * kSegs;
-  if (steps > 0) fetch(0);
+  constexpr int kStages = C::kStages;
+  constexpr int kOps = decltype(oa)::kOps + decltype(ob)::kOps;
+#pragma unroll
+  for (int q = 0; q < kStages - 1; ++q)
+    if (q < steps) fetch(q * C::kStage);
   for (int kt = 0; kt < steps; ++kt) {
-    wait_dma();
+    // step kt has landed once no more than the kStages - 2 behind it are on their way
+    if (kStages > 2 && kt + kStages - 2 < steps)
+      wait_dma_but<(kStages - 2) * kOps>();
+    else
+      wait_dma();
     lds_barrier();
-    const uint32_t st = (kt & 1) * C::kStage;
-    if (kt + 1 < steps) fetch(C::kStage - st);
+    const uint32_t st = (kt % kStages) * C::kStage;
+    // where step kt - 1 was, read by all
+    if (kt + kStages - 1 < steps) fetch((kt + kStages - 1) % kStages * C::kStage);
     const uint8_t* sa = smem + st;
     const uint8_t* sb = sa + C::TM * 128;
 #pragma unroll
@@ -433,18 +450,23 @@ __global__ __launch_bounds__(C::kThreads, 2) void k_ce_gemm(GemmArgs g) {
 // ---------------------------------------------------------------------------
 // Rows
 // ---------------------------------------------------------------------------
-constexpr int kRowThreads = 1024, kRowPer = 8;
+constexpr int kRowPer = 8;  // targets a thread looks at together
+
+// The int32 state: the rows that count, workgroups that are done, and T entries each of map, pos, target.
+struct IntState {
+  int *n, *done, *map, *pos, *target;
+  IntState(int32_t* p, int64_t T) : n(p), done(p + 1), map(p + 4), pos(map + T), target(pos + T) {}
+};
 
 // The rows that count, in order: map[i] the row, target[i] its target (-1 outside the vocabulary),
-// pos[t] = i or -1 for an ignored row (whose loss is 0), n their number.  One workgroup.
-__global__ __launch_bounds__(kRowThreads) void k_ce_rows(const int64_t* __restrict__ y, int64_t T, int64_t V, int64_t ignore,
-                                                         int* __restrict__ map, int* __restrict__ pos,
-                                                         int* __restrict__ target, int* __restrict__ n,
-                                                         float* __restrict__ rowloss) {
-  __shared__ int wsum[kRowThreads / 64];
+// pos[t] = i or -1 for an ignored row (whose loss is 0), n their number.  One workgroup of THREADS.
+template <int THREADS>
+__device__ __forceinline__ int find_rows(const int64_t* __restrict__ y, int64_t T, int64_t V, int64_t ignore,
+                                         const IntState& st, float* __restrict__ rowloss, bool write, int* lds_map) {
+  __shared__ int wsum[THREADS / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int base = 0;
-  for (int64_t t0 = 0; t0 < T; t0 += kRowThreads * kRowPer) {
+  for (int64_t t0 = 0; t0 < T; t0 += THREADS * kRowPer) {
     const int64_t first = t0 + (int64_t)tid * kRowPer;
     int64_t v[kRowPer];
     int mine = 0;
@@ -463,7 +485,7 @@ __global__ __launch_bounds__(kRowThreads) void k_ce_rows(const int64_t* __restri
     __syncthreads();
     int before = 0, all = 0;
 #pragma unroll
-    for (int w = 0; w < kRowThreads / 64; ++w) {
+    for (int w = 0; w < THREADS / 64; ++w) {
       if (w < wave) before += wsum[w];
       all += wsum[w];
     }
@@ -471,81 +493,95 @@ __global__ __launch_bounds__(kRowThreads) void k_ce_rows(const int64_t* __restri
 #pragma unroll
     for (int j = 0; j < kRowPer; ++j) {
       if (first + j >= T) break;
-      if (v[j] == ignore) {
-        pos[first + j] = -1;
-        rowloss[first + j] = 0.0f;
-      } else {
-        map[i] = (int)(first + j);
-        target[i] = v[j] >= 0 && v[j] < V ? (int)v[j] : -1;
-        pos[first + j] = i++;
+      const bool kept = v[j] != ignore;
+      if (lds_map && kept) lds_map[i] = (int)(first + j);
+      if (write) {
+        if (kept) {
+          st.map[i] = (int)(first + j);
+          st.target[i] = v[j] >= 0 && v[j] < V ? (int)v[j] : -1;
+        } else {
+          rowloss[first + j] = 0.0f;
+        }
+        st.pos[first + j] = kept ? i : -1;
       }
+      i += kept;
     }
     base += all;
     __syncthreads();
   }
-  if (tid == 0) *n = base;
+  if (write && tid == 0) {
+    *st.n = base;
+    *st.done = 0;
+  }
+  return base;
+}
+
+__global__ __launch_bounds__(1024) void k_ce_rows(const int64_t* __restrict__ y, int64_t T, int64_t V, int64_t ignore,
+                                                  IntState st, float* __restrict__ rowloss) {
+  find_rows<1024>(y, T, V, ignore, st, rowloss, true, nullptr);
 }
 
 // Rows of x (all, or map's first *n) with zeros up to Dp columns; fp32 rows as three bf16 planes.
 template <bool F32>
+__device__ __forceinline__ void copy_piece(const void* __restrict__ x, int64_t ldx, int64_t D, bool whole, int64_t row, int64_t i,
+                                           int64_t c, uint16_t* __restrict__ out, int64_t Dp, int64_t plane) {
+  using E = std::conditional_t<F32, float, uint16_t>;
+  const E* s = static_cast<const E*>(x) + row * ldx + c;
+  uint16_t* d = out + i * Dp + c;
+  E v[8];
+  if (whole && c + 8 <= D) {
+    __builtin_memcpy(v, __builtin_assume_aligned(s, 16), sizeof(v));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = c + e < D ? s[e] : (E)0;
+  }
+  if constexpr (F32) {
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+      v4u h;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        h[e] = f32x2_to_bf16x2_bits(v[2 * e], v[2 * e + 1]);
+        v[2 * e] -= bf16_lo(h[e]);
+        v[2 * e + 1] -= bf16_hi(h[e]);
+      }
+      *reinterpret_cast<v4u*>(d + p * plane) = h;
+    }
+  } else {
+    __builtin_memcpy(__builtin_assume_aligned(d, 16), v, 16);
+  }
+}
+template <bool F32>
+__device__ __forceinline__ bool whole_rows(const void* x, int64_t ldx) {
+  return ((uintptr_t)x & 15) == 0 && ldx % (F32 ? 4 : 8) == 0;
+}
+
+template <bool F32>
 __global__ __launch_bounds__(256) void k_ce_copy(const void* __restrict__ x, int64_t ldx, int64_t rows, int64_t D,
                                                  const int* __restrict__ map, const int* __restrict__ n,
                                                  uint16_t* __restrict__ out, int64_t Dp, int64_t plane) {
-  using E = std::conditional_t<F32, float, uint16_t>;
   const int64_t pieces = Dp / 8, have = n ? *n : rows;
-  const bool whole = ((uintptr_t)x & 15) == 0 && ldx % (16 / (int)sizeof(E)) == 0;
+  const bool whole = whole_rows<F32>(x, ldx);
   for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < have * pieces; q += (int64_t)gridDim.x * 256) {
-    const int64_t i = q / pieces, c = (q - i * pieces) * 8;
-    const E* s = static_cast<const E*>(x) + (map ? (int64_t)map[i] : i) * ldx + c;
-    uint16_t* d = out + i * Dp + c;
-    E v[8];
-    if (whole && c + 8 <= D) {
-      __builtin_memcpy(v, __builtin_assume_aligned(s, 16), sizeof(v));
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = c + e < D ? s[e] : (E)0;
-    }
-    if constexpr (F32) {
-#pragma unroll
-      for (int p = 0; p < 3; ++p) {
-        v4u h;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          h[e] = f32x2_to_bf16x2_bits(v[2 * e], v[2 * e + 1]);
-          v[2 * e] -= bf16_lo(h[e]);
-          v[2 * e + 1] -= bf16_hi(h[e]);
-        }
-        *reinterpret_cast<v4u*>(d + p * plane) = h;
-      }
-    } else {
-      __builtin_memcpy(__builtin_assume_aligned(d, 16), v, 16);
-    }
+    const int64_t i = q / pieces;
+    copy_piece<F32>(x, ldx, D, whole, map ? (int64_t)map[i] : i, i, (q - i * pieces) * 8, out, Dp, plane);
   }
 }
 
-// A wave per row: the tiles' maxima and sums joined, the row's loss (NaN for a target outside the
-// vocabulary).
-__global__ __launch_bounds__(256) void k_ce_join(const float2* __restrict__ part, int tiles, const int* __restrict__ n,
-                                                 const int* __restrict__ map, const int* __restrict__ target,
-                                                 const float* __restrict__ ztarget, float* __restrict__ rowmax,
-                                                 float* __restrict__ inv, float* __restrict__ rowloss) {
-  const int lane = threadIdx.x & 63;
-  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (i >= *n) return;
-  float m = -__builtin_inff(), s = 0.0f;
-  for (int t = lane; t < tiles; t += 64) m = fmaxf(m, part[i * tiles + t].x);
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
-  for (int t = lane; t < tiles; t += 64) {
-    const float2 p = part[i * tiles + t];
-    s += p.y * exp_of(p.x - m);
-  }
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) s += __shfl_xor(s, o);
-  if (lane == 0) {
-    rowmax[i] = m;
-    inv[i] = 1.0f / s;
-    rowloss[map[i]] = target[i] < 0 ? __builtin_nanf("") : (m - ztarget[i]) + logf(s);
+// k_ce_rows and k_ce_copy in one launch for few rows: every workgroup finds the rows, the first one
+// writes the state.
+constexpr int kFewRows = 256 * kRowPer;
+template <bool F32>
+__global__ __launch_bounds__(256) void k_ce_rows_copy(const int64_t* __restrict__ y, int64_t T, int64_t V, int64_t ignore,
+                                                      IntState st, float* __restrict__ rowloss, const void* __restrict__ x,
+                                                      int64_t ldx, int64_t D, uint16_t* __restrict__ out, int64_t Dp) {
+  __shared__ int map[kFewRows];
+  const int n = find_rows<256>(y, T, V, ignore, st, rowloss, blockIdx.x == 0, map);
+  const uint32_t pieces = (uint32_t)(Dp / 8), total = n * pieces;  // (at most 2^11 x 2^15)
+  const bool whole = whole_rows<F32>(x, ldx);
+  for (uint32_t q = blockIdx.x * 256 + threadIdx.x; q < total; q += gridDim.x * 256) {
+    const uint32_t i = q / pieces;
+    copy_piece<F32>(x, ldx, D, whole, map[i], i, (q - i * pieces) * 8, out, Dp, T * Dp);
   }
 }
 
@@ -562,13 +598,57 @@ __device__ inline double block_sum(double v) {
   return s;
 }
 
-// The rows' sum, over their number with `mean` (0 / 0 is NaN).
+// The rows' losses added in their order, over their number with `mean` (0 / 0 is NaN).
+__device__ __forceinline__ void add_losses(const float* rowloss, int64_t T, int n, int mean, float* loss) {
+  double sum = 0;
+  for (int64_t t = threadIdx.x; t < T; t += blockDim.x)
+    sum += __hip_atomic_load(&rowloss[t], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  sum = block_sum(sum);
+  if (threadIdx.x == 0) *loss = (float)(mean ? sum / n : sum);
+}
+
+// A wave per row: the tiles' maxima and sums joined, the row's loss (NaN for a target outside the
+// vocabulary).  With `loss`, for few rows, the workgroup that ends last adds them up; for more a
+// launch of its own does, as each workgroup's fence costs more than it (4096 rows: 34 us of forward
+// with the launch, 107 without).
+__global__ __launch_bounds__(256) void k_ce_join(const float2* __restrict__ part, int tiles, int64_t T, IntState st,
+                                                 const float* __restrict__ ztarget, float* __restrict__ rowmax,
+                                                 float* __restrict__ inv, float* __restrict__ rowloss, int mean,
+                                                 float* __restrict__ loss) {
+  const int lane = threadIdx.x & 63, n = *st.n;
+  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (i < n) {
+    float m = -__builtin_inff(), s = 0.0f;
+    for (int t = lane; t < tiles; t += 64) m = fmaxf(m, part[i * tiles + t].x);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+    for (int t = lane; t < tiles; t += 64) {
+      const float2 p = part[i * tiles + t];
+      s += p.y * exp_of(p.x - m);
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) s += __shfl_xor(s, o);
+    if (lane == 0) {
+      rowmax[i] = m;
+      inv[i] = 1.0f / s;
+      rowloss[st.map[i]] = st.target[i] < 0 ? __builtin_nanf("") : (m - ztarget[i]) + logf(s);
+    }
+  }
+  if (!loss) return;
+  __shared__ int before;
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) before = __hip_atomic_fetch_add(st.done, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  if (before != (int)gridDim.x - 1) return;
+  __threadfence();
+  add_losses(rowloss, T, n, mean, loss);
+}
+constexpr int kJoinAlone = 64;  // rows up to which it does
+
 __global__ __launch_bounds__(1024) void k_ce_loss(const float* __restrict__ rowloss, int64_t T, const int* __restrict__ n,
                                                   int mean, float* __restrict__ loss) {
-  double s = 0;
-  for (int64_t t = threadIdx.x; t < T; t += 1024) s += rowloss[t];
-  s = block_sum(s);
-  if (threadIdx.x == 0) *loss = (float)(mean ? s / *n : s);
+  add_losses(rowloss, T, *n, mean, loss);
 }
 
 // What dz is scaled by: coef[i] = g_i 2^a with all products in range (fp16 holds 2^-24 .. 65504,
@@ -650,20 +730,54 @@ __global__ __launch_bounds__(256) void k_ce_dx(const float* __restrict__ slabs, 
 // ---------------------------------------------------------------------------
 // Host
 // ---------------------------------------------------------------------------
-using Big = Cfg<2, 4, 8, 4>;  // 256 x 256, 8 waves of 128 x 64
+// Tiles.  Wide ones read their operands less often and keep the matrix units busier; narrow ones
+// leave fewer compute units idle in a small product, and the narrowest, with more steps on their way,
+// stream w for a few rows.
+using Wide = Cfg<2, 4, 8, 4, 2>;    // 256 x 256, 8 waves of 128 x 64
+using Medium = Cfg<2, 2, 4, 4, 2>;  // 128 x 128, 4 waves of 64 x 64, two workgroups a CU
+using Narrow = Cfg<1, 4, 4, 1, 4>;  // 64 x 64, 4 waves of 64 x 16, two workgroups a CU
+constexpr int kTiles = 3;
+constexpr int kTileM[kTiles] = {Wide::TM, Medium::TM, Narrow::TM};
+constexpr int kTileN[kTiles] = {Wide::TN, Medium::TN, Narrow::TN};
+// a tile's rate against that of the widest, every CU at work
+constexpr double kTileRate[kTiles] = {1.0, 0.75, 0.4};
+
+// The time of m x n outputs in parts of K, in units of one output's share at the widest tile's rate.
+double tile_time(int tile, int64_t m, int64_t n, double parts, double part) {
+  const double count = (double)cdiv(m, kTileM[tile]) * (double)cdiv(n, kTileN[tile]) * parts;
+  const double rounds = ceil(count / cin_device_cus());
+  return rounds * kTileM[tile] * kTileN[tile] / kTileRate[tile] * part;
+}
+int pick_tile(int64_t m, int64_t n) {
+  int best = 0;
+  for (int t = 1; t < kTiles; ++t)
+    if (tile_time(t, m, n, 1, 1) < tile_time(best, m, n, 1, 1)) best = t;
+  return best;
+}
+template <class F>
+void with_tile(int tile, F f) {
+  if (tile == 0)
+    f(Wide{});
+  else if (tile == 1)
+    f(Medium{});
+  else
+    f(Narrow{});
+}
 
 constexpr int64_t kMaxT = (int64_t)1 << 30, kMaxV = (int64_t)1 << 30, kMaxD = (int64_t)1 << 18;
 constexpr int64_t kPieceBytes = (int64_t)1 << 30;  // dz of one piece
 constexpr int64_t kMaxPiece = (int64_t)1 << 20;    // its columns: 256 rows lie within 2^31 bytes
 
 int64_t align_up(int64_t v, int64_t a) { return cdiv(v, a) * a; }
+constexpr int64_t kAlign = 256;  // columns of a piece: whole tiles
 
 struct Plan {
   int planes;           // of an operand: 3 for fp32
   int64_t Dp;           // columns of x and w as the products read them
-  int64_t tiles_n;      // column tiles of the forward product
+  int tile;             // of the forward product
+  int64_t tiles_n;      // its column tiles
   int64_t piece, ldz;   // columns of a piece, elements between rows of dz
-  int splits;           // slabs of dx
+  int splits, slab_tile;  // slabs of dx, the tile of its product
   // bytes
   int64_t part, ztarget, dz, slabs, coef;
 };
@@ -672,18 +786,29 @@ Plan make_plan(int dtype, int64_t T, int64_t D, int64_t V) {
   Plan p;
   p.planes = dtype == CIN_DT_F32 ? 3 : 1;
   p.Dp = align_up(D, BK);
-  p.tiles_n = cdiv(V, Big::TN);
   const int64_t Tp = T > 0 ? T : 1;
-  int64_t most = align_up(kPieceBytes / (Tp * kEs * p.planes) + 1, Big::TN);
+  p.tile = pick_tile(Tp, V);
+  p.tiles_n = cdiv(V, kTileN[p.tile]);
+  int64_t most = align_up(kPieceBytes / (Tp * kEs * p.planes) + 1, kAlign);
   if (most > kMaxPiece) most = kMaxPiece;
   const int64_t pieces = cdiv(V, most);
-  p.piece = align_up(cdiv(V, pieces), Big::TN);
+  p.piece = align_up(cdiv(V, pieces), kAlign);
   p.ldz = p.piece + 64;  // rows not a multiple of 16 KiB apart
-  const int64_t tiles = cdiv(Tp, Big::TM) * cdiv(p.Dp, Big::TN);
-  int64_t s = tiles >= 192 ? 1 : 256 / tiles;
+  // dx: K, the piece, is split where the tiles are fewer than the CUs, in parts of 8 steps at least
   const int64_t steps = p.piece / BK;
-  if (s > steps / 8) s = steps / 8;
-  p.splits = (int)(s < 1 ? 1 : s);
+  double best = 0;
+  for (int t = 0; t < kTiles; ++t) {
+    const int64_t count = cdiv(Tp, kTileM[t]) * cdiv(p.Dp, kTileN[t]);
+    int64_t s = cin_device_cus() / count;
+    if (s > steps / 8) s = steps / 8;
+    if (s < 1) s = 1;
+    const double time = tile_time(t, Tp, p.Dp, (double)s, 1.0 / s);
+    if (t == 0 || time < best) {
+      best = time;
+      p.splits = (int)s;
+      p.slab_tile = t;
+    }
+  }
   p.part = align_up(Tp * p.tiles_n * 8, 256);
   p.ztarget = align_up(Tp * 4, 256);
   p.dz = align_up(p.planes * Tp * p.ldz * kEs, 256);
@@ -697,7 +822,8 @@ int check(const char* name, int dtype, int64_t T, int64_t D, int64_t V) {
   CIN_CHECK_ARG(T >= 0 && T < kMaxT, "%s: T must be in [0, 2^30)", name);
   CIN_CHECK_ARG(V >= 1 && V < kMaxV, "%s: V must be in [1, 2^30)", name);
   CIN_CHECK_ARG(D >= 1 && D <= kMaxD, "%s: D must be in [1, 2^18]", name);
-  CIN_CHECK_ARG(cdiv(T, 256) * cdiv(V, 256) < ((int64_t)1 << 31), "%s: T x V is too large", name);
+  CIN_CHECK_ARG(cdiv(T, 64) * cdiv(V, 64) < ((int64_t)1 << 31) && cdiv(V, 64) * cdiv(D, 64) < ((int64_t)1 << 31),
+                "%s: T x V or V x D is too large", name);
   return CIN_OK;
 }
 
@@ -716,10 +842,13 @@ void with_dtype(int dtype, F f) {
 }
 
 template <int EPI>
-void gemm(int dtype, const GemmArgs& g, int64_t max_m, hipStream_t s) {
-  with_dtype(dtype, [&](auto dt) {
-    const int64_t tiles = cdiv(max_m, Big::TM) * cdiv(g.N, Big::TN);
-    hipLaunchKernelGGL((k_ce_gemm<Big, dt(), EPI>), dim3((unsigned)tiles, (unsigned)g.splits), Big::kThreads, 0, s, g);
+void gemm(int dtype, int tile, const GemmArgs& g, int64_t max_m, hipStream_t s) {
+  with_tile(tile, [&](auto c) {
+    using C = decltype(c);
+    with_dtype(dtype, [&](auto dt) {
+      const int64_t tiles = cdiv(max_m, C::TM) * cdiv(g.N, C::TN);
+      hipLaunchKernelGGL((k_ce_gemm<C, dt(), EPI>), dim3((unsigned)tiles, (unsigned)g.splits), C::kThreads, 0, s, g);
+    });
   });
 }
 
@@ -733,12 +862,6 @@ void copy_rows(bool f32, const void* x, int64_t ldx, int64_t rows, int64_t D, co
   else
     hipLaunchKernelGGL(k_ce_copy<false>, grid, 256, 0, s, x, ldx, rows, D, map, n, o, Dp, rows * Dp);
 }
-
-// The int32 state: n, then map, pos and target of T entries each.
-struct IntState {
-  int *n, *map, *pos, *target;
-  IntState(int32_t* p, int64_t T) : n(p), map(p + 4), pos(map + T), target(pos + T) {}
-};
 
 }  // namespace
 
@@ -767,9 +890,21 @@ int cin_linear_ce_forward(const void* x, int dtype, int64_t T, int64_t D, int64_
   const IntState st(state_i, T);
   float2* part = static_cast<float2*>(workspace);
   float* zt = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.part);
-  hipLaunchKernelGGL(k_ce_rows, 1, kRowThreads, 0, s, target, T, V, ignore_index, st.map, st.pos, st.target, st.n, rowloss);
+  if (T == 0 || T > kFewRows)
+    hipLaunchKernelGGL(k_ce_rows, 1, 1024, 0, s, target, T, V, ignore_index, st, rowloss);
   if (T > 0) {
-    copy_rows(f32, x, ldx, T, D, st.map, st.n, xc, p.Dp, s);
+    if (T > kFewRows) {
+      copy_rows(f32, x, ldx, T, D, st.map, st.n, xc, p.Dp, s);
+    } else {
+      const unsigned grid = (unsigned)cdiv(T * (p.Dp / 8), 256);
+      uint16_t* o = static_cast<uint16_t*>(xc);
+      if (f32)
+        hipLaunchKernelGGL(k_ce_rows_copy<true>, grid < 256 ? grid : 256, 256, 0, s, target, T, V, ignore_index, st, rowloss,
+                           x, ldx, D, o, p.Dp);
+      else
+        hipLaunchKernelGGL(k_ce_rows_copy<false>, grid < 256 ? grid : 256, 256, 0, s, target, T, V, ignore_index, st, rowloss,
+                           x, ldx, D, o, p.Dp);
+    }
     if (wp) copy_rows(f32, w, ldw, V, D, nullptr, nullptr, wp, p.Dp, s);
     GemmArgs g{};
     g.A = xc;
@@ -785,11 +920,12 @@ int cin_linear_ce_forward(const void* x, int dtype, int64_t T, int64_t D, int64_
     g.part = part;
     g.ztarget = zt;
     g.target = st.target;
-    gemm<kStats>(dtype, g, T, s);
-    hipLaunchKernelGGL(k_ce_join, (unsigned)cdiv(T, 4), 256, 0, s, part, (int)p.tiles_n, st.n, st.map, st.target, zt,
-                       state_f, state_f + T, rowloss);
+    gemm<kStats>(dtype, p.tile, g, T, s);
   }
-  if (loss) hipLaunchKernelGGL(k_ce_loss, 1, 1024, 0, s, rowloss, T, st.n, mean, loss);
+  // (without rows one workgroup: the sum of none)
+  hipLaunchKernelGGL(k_ce_join, (unsigned)(T > 0 ? cdiv(T, 4) : 1), 256, 0, s, part, (int)p.tiles_n, T, st, zt, state_f,
+                     state_f + T, rowloss, mean, T <= kJoinAlone ? loss : nullptr);
+  if (loss && T > kJoinAlone) hipLaunchKernelGGL(k_ce_loss, 1, 1024, 0, s, rowloss, T, st.n, mean, loss);
   return cin_check_launch(name);
 }
 
@@ -837,7 +973,7 @@ int cin_linear_ce_backward(const void* xc, int dtype, int64_t T, int64_t D, cons
     g.rowmax = state_f;
     g.inv = state_f + T;
     g.coef = coef;
-    gemm<kGrad>(dtype, g, T, s);
+    gemm<kGrad>(dtype, pick_tile(T, g.N), g, T, s);
     GemmArgs h{};
     h.n = st.n;
     h.A = dz;
@@ -858,7 +994,7 @@ int cin_linear_ce_backward(const void* xc, int dtype, int64_t T, int64_t D, cons
       h.ldc = p.Dp;
       h.slab = T * p.Dp;
       h.add = v0 > 0;
-      gemm<kSlab>(dtype, h, T, s);
+      gemm<kSlab>(dtype, p.slab_tile, h, T, s);
     }
     if (dw) {
       h.B = xc;
@@ -870,7 +1006,7 @@ int cin_linear_ce_backward(const void* xc, int dtype, int64_t T, int64_t D, cons
       h.C = static_cast<char*>(dw) + v0 * D * (dtype == CIN_DT_F32 ? 4 : 2);
       h.ldc = D;
       h.out_scale = out_scale;
-      gemm<kFinal>(dtype, h, cols, s);
+      gemm<kFinal>(dtype, pick_tile(cols, D), h, cols, s);
     }
   }
   if (dx) {

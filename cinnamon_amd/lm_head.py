@@ -8,7 +8,10 @@ fp32 matrix units (csrc/lm_head.hip) without ever keeping the logits.
 """
 from __future__ import annotations
 
+import functools
+
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import call_on, dtype_code, ptr, stream_of
@@ -16,6 +19,7 @@ from .kernels import _cdiv, _plain_eager, _require, custom_op
 
 __all__ = ["linear_cross_entropy"]
 
+_MODES = {"none": 0, "sum": 1, "mean": 2}
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
@@ -42,10 +46,12 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     _require(not target.dtype.is_floating_point and not target.dtype.is_complex and target.dtype != torch.bool,
              "target must hold integers")
     _require(weight.shape[0] >= 1 and weight.shape[1] >= 1, "weight must not be empty")
-    _require(reduction in ("mean", "sum", "none"), "reduction must be 'mean', 'sum' or 'none'")
-    x2 = x.reshape(-1, x.shape[-1])
-    y = target.reshape(-1).to(torch.int64)
-    mode = {"none": 0, "sum": 1, "mean": 2}[reduction]
+    _require(reduction in _MODES, "reduction must be 'mean', 'sum' or 'none'")
+    x2 = x if x.ndim == 2 else x.reshape(-1, x.shape[-1])
+    y = target if target.ndim == 1 else target.reshape(-1)
+    if y.dtype != torch.int64:
+        y = y.to(torch.int64)
+    mode = _MODES[reduction]
     if _plain_eager(x2, weight, y):
         if torch.is_grad_enabled() and (x2.requires_grad or weight.requires_grad):
             loss = _LinearCE.apply(x2, weight, y, int(ignore_index), mode)
@@ -53,23 +59,31 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
             loss = _launch_forward(x2, weight, y, int(ignore_index), mode)[0]
     else:
         loss = _forward_op(x2, weight, y, int(ignore_index), mode)[0]
-    return loss.view(target.shape) if mode == 0 else loss
+    return loss.view(target.shape) if mode == 0 and target.ndim != 1 else loss
 
 
-def _padded(D):
-    """D rounded up to whole K steps of the products."""
-    return _cdiv(D, 64) * 64
+def _layout(T, D, V, dtype):
+    """Bytes of the state that the forward leaves: its rows that count, the weight's copy, integers
+    and floats (csrc/lm_head.hip), each from a multiple of 256 on.  Operands are padded to whole K
+    steps of 64; fp32 ones are three bf16 planes; a 16-bit weight whose width needs no padding is
+    not copied.  Returns (offsets of the four, total, whether the weight is copied)."""
+    Dp = _cdiv(D, 64) * 64
+    planes = 3 if dtype == torch.float32 else 1
+    copied = planes == 3 or Dp != D
+    offsets, at = [], 0
+    for n in (planes * T * Dp * 2, planes * V * Dp * 2 if copied else 0, 4 * (4 + 3 * T), 8 * T):
+        offsets.append(at)
+        at += _cdiv(n, 256) * 256
+    return offsets, at, copied
 
 
-def _operand_shapes(x, V):
-    """Shapes of the compacted rows and of the weight's copy, and their dtype: fp32 operands are three
-    bf16 planes (csrc/lm_head.hip), others the rows padded to whole K steps; no copy of a 16-bit
-    weight whose width needs no padding."""
-    T, D = x.shape
-    Dp = _padded(D)
-    if x.dtype == torch.float32:
-        return (3 * T, Dp), (3 * V, Dp), torch.bfloat16
-    return (T, Dp), (V if Dp != D else 0, Dp), x.dtype
+@functools.lru_cache(maxsize=256)
+def _sizes(T, D, V, dtype):
+    """_layout's, and the workspaces' bytes of the forward and the backward."""
+    ws = [_lib.load().cin_linear_ce_workspace(dtype_code(dtype), T, D, V, back) for back in (0, 1)]
+    if min(ws) < 0:
+        raise ValueError(f"linear_cross_entropy: {_lib.last_error()}")
+    return (*_layout(T, D, V, dtype), *ws)
 
 
 def _rows(t):
@@ -85,48 +99,42 @@ def _weight_rows(w):
     return w.contiguous() if not w.is_contiguous() else w.clone()
 
 
-def _workspace(name, backward, T, D, V, dtype, device):
-    n = _lib.load().cin_linear_ce_workspace(dtype_code(dtype), T, D, V, backward)
-    if n < 0:
-        raise ValueError(f"{name}: {_lib.last_error()}")
-    return torch.empty(max(n, 16), dtype=torch.uint8, device=device)
-
-
 def _launch_forward(x, weight, target, ignore_index, mode):
-    """(loss, compacted rows, padded weight or empty, int state, float state)"""
+    """(loss, state for the backward)"""
     (T, D), V = x.shape, weight.shape[0]
-    dev = x.device
     x = _rows(x)
-    xc, wp, dtype = _operand_shapes(x, V)
-    pad = wp[0] > 0
-    w = _rows(weight) if pad else _weight_rows(weight)
+    (xc, wp, si, sf), total, copied, ws, _ = _sizes(T, D, V, x.dtype)
+    w = _rows(weight) if copied else _weight_rows(weight)
     target = target.contiguous()
-    xc = torch.empty(xc, dtype=dtype, device=dev)
-    wp = torch.empty(wp, dtype=dtype, device=dev)
-    si = torch.empty(4 + 3 * T, dtype=torch.int32, device=dev)
-    sf = torch.empty(2 * T, dtype=torch.float32, device=dev)
-    rows = torch.empty(T, dtype=torch.float32, device=dev)
-    loss = torch.empty((), dtype=torch.float32, device=dev) if mode else rows
-    ws = _workspace("linear_cross_entropy", 0, T, D, V, x.dtype, dev)
-    call_on(x, "cin_linear_ce_forward", ptr(x), dtype_code(x), T, D, x.stride(0), ptr(w), V, w.stride(0), ptr(target),
-            ignore_index, int(mode == 2), ptr(xc), ptr(wp) if pad else 0, ptr(si), ptr(sf), ptr(rows),
-            ptr(loss) if mode else 0, ptr(ws), ws.numel(), stream_of(x))
-    return loss, xc, wp, si, sf
+    state = torch.empty(total, dtype=torch.uint8, device=x.device)
+    work = torch.empty(ws, dtype=torch.uint8, device=x.device)
+    rows = x.new_empty(T, dtype=torch.float32)
+    loss = x.new_empty((), dtype=torch.float32) if mode else rows
+    at = state.data_ptr()
+    call_on(x, "cin_linear_ce_forward", x.data_ptr(), dtype_code(x), T, D, x.stride(0), w.data_ptr(), V, w.stride(0),
+            target.data_ptr(), ignore_index, mode == 2, at + xc, at + wp if copied else 0, at + si, at + sf,
+            rows.data_ptr(), loss.data_ptr() if mode else 0, work.data_ptr(), ws, stream_of(x))
+    return loss, state
 
 
-def _launch_backward(grad, xc, weight, si, sf, D, dtype, mode, need_x, need_w):
-    """(dx, dw) of dtype, None where not needed; weight: its copy where there is one."""
-    T, V = sf.shape[0] // 2, weight.shape[0] // (3 if dtype == torch.float32 else 1)
-    dev = xc.device
-    dx = torch.empty((T, D), dtype=dtype, device=dev) if need_x else None
+def _launch_backward(grad, state, weight, T, mode, need_x, need_w):
+    """(dx, dw), None where not needed."""
+    V, D = weight.shape
+    dtype = weight.dtype
+    dx = weight.new_empty((T, D)) if need_x else None
     if T == 0:
-        return dx, torch.zeros((V, D), dtype=dtype, device=dev) if need_w else None
-    dw = torch.empty((V, D), dtype=dtype, device=dev) if need_w else None
-    w = _weight_rows(weight)
-    ws = _workspace("linear_cross_entropy", 1, T, D, V, dtype, dev)
-    call_on(xc, "cin_linear_ce_backward", ptr(xc), dtype_code(dtype), T, D, ptr(w), V, w.stride(0), ptr(si), ptr(sf),
-            ptr(grad), 0 if mode else grad.stride(0), int(mode == 2), ptr(dx), ptr(dw), ptr(ws), ws.numel(),
-            stream_of(xc))
+        return dx, weight.new_zeros((V, D)) if need_w else None
+    dw = weight.new_empty((V, D)) if need_w else None
+    (xc, wp, si, sf), _, copied, _, ws = _sizes(T, D, V, dtype)
+    at = state.data_ptr()
+    if copied:
+        w, ldw = at + wp, _cdiv(D, 64) * 64
+    else:
+        weight = _weight_rows(weight)
+        w, ldw = weight.data_ptr(), weight.stride(0)
+    work = torch.empty(ws, dtype=torch.uint8, device=weight.device)
+    call_on(weight, "cin_linear_ce_backward", at + xc, dtype_code(dtype), T, D, w, V, ldw, at + si, at + sf, grad.data_ptr(),
+            0 if mode else grad.stride(0), mode == 2, ptr(dx), ptr(dw), work.data_ptr(), ws, stream_of(weight))
     return dx, dw
 
 
@@ -135,55 +143,54 @@ class _LinearCE(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, target, ignore_index, mode):
-        loss, xc, wp, si, sf = _launch_forward(x, weight, target, ignore_index, mode)
-        ctx.save_for_backward(xc, wp if wp.shape[0] else weight, si, sf)
-        ctx.options = x.shape[1], x.dtype, mode
+        loss, state = _launch_forward(x, weight, target, ignore_index, mode)
+        ctx.save_for_backward(state, weight)
+        ctx.options = x.shape[0], mode
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        dx, dw = _launch_backward(grad, *ctx.saved_tensors, *ctx.options, *ctx.needs_input_grad[:2])
-        return dx, dw, None, None, None
+        # (the wrapper costs 4 us of host time a call; only a graph of the gradient needs it)
+        f = _gradients if not torch.is_grad_enabled() else once_differentiable(_gradients)
+        return f(ctx, grad)
 
 
-@custom_op("linear_ce_forward", "(Tensor x, Tensor weight, Tensor target, int ignore_index, int mode) -> "
-           "(Tensor, Tensor, Tensor, Tensor, Tensor)")
+def _gradients(ctx, grad):
+    dx, dw = _launch_backward(grad, *ctx.saved_tensors, *ctx.options, *ctx.needs_input_grad[:2])
+    return dx, dw, None, None, None
+
+
+@custom_op("linear_ce_forward", "(Tensor x, Tensor weight, Tensor target, int ignore_index, int mode) -> (Tensor, Tensor)")
 def _forward_op(x, weight, target, ignore_index, mode):
     return _launch_forward(x, weight, target, ignore_index, mode)
 
 
 @_forward_op.register_fake
 def _(x, weight, target, ignore_index, mode):
-    T = x.shape[0]
-    xc, wp, dtype = _operand_shapes(x, weight.shape[0])
-    return (x.new_empty(() if mode else (T,), dtype=torch.float32), x.new_empty(xc, dtype=dtype),
-            x.new_empty(wp, dtype=dtype), x.new_empty((4 + 3 * T,), dtype=torch.int32),
-            x.new_empty((2 * T,), dtype=torch.float32))
+    (T, D), V = x.shape, weight.shape[0]
+    return (x.new_empty(() if mode else (T,), dtype=torch.float32),
+            x.new_empty((_layout(T, D, V, x.dtype)[1],), dtype=torch.uint8))
 
 
-@custom_op("linear_ce_backward", "(Tensor grad, Tensor xc, Tensor weight, Tensor si, Tensor sf, int D, ScalarType dtype, "
-           "int mode) -> (Tensor, Tensor)")
-def _backward_op(grad, xc, weight, si, sf, D, dtype, mode):
-    return _launch_backward(grad, xc, weight, si, sf, D, dtype, mode, True, True)
+@custom_op("linear_ce_backward", "(Tensor grad, Tensor state, Tensor weight, int T, int mode) -> (Tensor, Tensor)")
+def _backward_op(grad, state, weight, T, mode):
+    return _launch_backward(grad, state, weight, T, mode, True, True)
 
 
 @_backward_op.register_fake
-def _(grad, xc, weight, si, sf, D, dtype, mode):
-    V = weight.shape[0] // (3 if dtype == torch.float32 else 1)
-    return xc.new_empty((sf.shape[0] // 2, D), dtype=dtype), xc.new_empty((V, D), dtype=dtype)
+def _(grad, state, weight, T, mode):
+    return weight.new_empty((T, weight.shape[1])), weight.new_empty(weight.shape)
 
 
 def _setup(ctx, inputs, output):
     x, weight, _target, _ignore, mode = inputs
-    loss, xc, wp, si, sf = output
-    ctx.mark_non_differentiable(xc, wp, si, sf)
-    copied = x.dtype == torch.float32 or _padded(x.shape[1]) != x.shape[1]
-    ctx.save_for_backward(xc, wp if copied else weight, si, sf)
-    ctx.options = x.shape[1], x.dtype, mode
+    _loss, state = output
+    ctx.mark_non_differentiable(state)
+    ctx.save_for_backward(state, weight)
+    ctx.options = x.shape[0], mode
 
 
-def _backward(ctx, grad, *_):
+def _backward(ctx, grad, _state):
     dx, dw = _backward_op(grad, *ctx.saved_tensors, *ctx.options)
     return dx, dw, None, None, None
 
