@@ -101,7 +101,7 @@ struct Operand {
   uint32_t lds;
 
   __device__ static inline int f(int r) {
-    if constexpr (!ACROSS) return swz_f(r);
+    if constexpr (!ACROSS) return (r >> 1) & 7;  // (the 16 rows and two chunks of a pass on 64 banks: no conflicts)
     return ((r & 3) | ((r >> 3 & 1) << 2)) & (kGran - 1);
   }
   // r0: the tile's first row (along) or column (across); valid: rows (along) or columns (across)
