@@ -245,6 +245,19 @@ __device__ inline uint64_t keep_groups(const GateArgs& a, const K* keys, int lan
   }
   uint64_t kept = 0;
   K last = 0;
+  if (a.groups <= LANES) {  // a group a lane
+    for (int r = 0; r < a.top_groups; ++r) {
+      last = lanes_max<LANES>(best[0]);
+      const bool mine = is_first<LANES>(best[0] == last, lane);
+      uint64_t m = __ballot(mine);
+      if constexpr (LANES < 64) m = (m >> (lane & ~(LANES - 1))) & ((1ull << LANES) - 1);
+      kept |= m;
+      if (mine) best[0] = 0;
+    }
+    worst = value_of(last);
+    margin = worst - value_of(lanes_max<LANES>(best[0]));
+    return kept;
+  }
   for (int r = 0; r <= a.top_groups; ++r) {
     // the best group left, the lowest of equals: lane sub holds groups sub, sub + LANES, ..
     K m = 0;
@@ -273,25 +286,46 @@ __device__ inline uint64_t keep_groups(const GateArgs& a, const K* keys, int lan
   return kept;
 }
 
-// The k largest keys, the lowest index of equals: lane r's key, and the expert in chosen[r]; keys
-// taken become 0.
+// Keys with the place in the lane in their lowest bits, the first place largest: neighbours closer
+// than EPL steps of a key count as equal from here on (an equal key's first place comes first).
+template <int EPL>
+constexpr uint32_t kPlace = EPL - 1;
+
+// Bitonic sort of a lane's keys, the largest first.
+template <int EPL>
+__device__ inline void sort_keys(uint32_t (&key)[EPL]) {
+#pragma unroll
+  for (int size = 2; size <= EPL; size *= 2)
+#pragma unroll
+    for (int step = size / 2; step > 0; step /= 2)
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) {
+        const int o = i ^ step;
+        if (o < i) continue;
+        const uint32_t hi = key[i] > key[o] ? key[i] : key[o], lo = key[i] > key[o] ? key[o] : key[i];
+        const bool down = (i & size) == 0 || size == EPL;
+        key[i] = down ? hi : lo;
+        key[o] = down ? lo : hi;
+      }
+}
+
+// The k largest keys, the lowest index of equals: lane r's key, and the expert in chosen[r].  Each
+// lane's keys are sorted once, so that a round is one maximum over the lanes' first keys and a shift in
+// the lane that had it; keys left stay sorted.
 template <int LANES, int EPL>
 __device__ inline uint32_t top_k(int k, int lane, uint32_t (&key)[EPL], int* chosen) {
   const int sub = lane & (LANES - 1);
+  sort_keys(key);
   uint32_t mine = 0;
   for (int r = 0; r < k; ++r) {
-    uint32_t m = key[0];
-#pragma unroll
-    for (int j = 1; j < EPL; ++j) m = key[j] > m ? key[j] : m;
-    const uint32_t top = lanes_max<LANES>(m);
+    const uint32_t head = key[0] & ~kPlace<EPL>;
+    const uint32_t top = lanes_max<LANES>(head);
     mine = sub == r ? top : mine;
-    if (is_first<LANES>(m == top, lane)) {
-      int at = EPL - 1;
+    if (is_first<LANES>(head == top, lane)) {
+      chosen[r] = sub * EPL + (int)(kPlace<EPL> - (key[0] & kPlace<EPL>));
 #pragma unroll
-      for (int j = EPL - 2; j >= 0; --j) at = key[j] == top ? j : at;
-#pragma unroll
-      for (int j = 0; j < EPL; ++j) key[j] = j == at ? 0 : key[j];
-      chosen[r] = sub * EPL + at;
+      for (int j = 0; j + 1 < EPL; ++j) key[j] = key[j + 1];
+      key[EPL - 1] = 0;
     }
   }
   wave_sync();
@@ -393,10 +427,14 @@ __global__ __launch_bounds__(64 * WAVES, EPL <= 16 ? 4 : 1) void k_gate_fwd(Gate
   // Without a bias, and with groups that count by one expert, the logits order as the choices do:
   // exactly, but where 64 bits cannot tell two scores apart (neighbours closer than 1e-10, sigmoids
   // above 10, scores under e^-600).  Else in 32 bits, u = 2^-24: a score is off by less than
-  // (24 + EPL) u of itself, a choice by its rounding too.
+  // (24 + EPL) u of itself, a choice by its rounding too, and ranked keys by 2 EPL u (that of a 16-bit
+  // logit by nothing: those bits are 0).
   const bool direct = !a.bias && (!limited || a.group_top == 1);
-  constexpr float kU = 5.9604644775390625e-8f, kS = (48 + 2 * EPL) * kU, kC = 4 * kU;
-  const auto bound = [&](float c) { return direct ? 1e-10f : kS * (a.bias ? top : fabsf(c)) + kC * fabsf(c); };
+  constexpr float kU = 5.9604644775390625e-8f, kS = (48 + 2 * EPL) * kU, kC = (4 + 2 * EPL) * kU;
+  constexpr float kZ = DT == CIN_DT_F32 ? 2 * EPL * kU : 0.0f;
+  const auto bound = [&](float c) {
+    return direct ? 1e-10f + kZ * fabsf(c) : kS * (a.bias ? top : fabsf(c)) + kC * fabsf(c);
+  };
   const auto blurred = [&](float c) { return direct && !(c - zmax > -600.0f && (a.score == kSoftmax || c < 10.0f)); };
   uint32_t key[EPL];
   bool doubt = false;
@@ -429,6 +467,8 @@ __global__ __launch_bounds__(64 * WAVES, EPL <= 16 ? 4 : 1) void k_gate_fwd(Gate
     most = __uint_as_float(lanes_max<LANES>(__float_as_uint(most)));
     doubt |= !(margin > 4 * bound(most) || (direct && margin == 0.0f)) || blurred(worst);
   }
+#pragma unroll
+  for (int j = 0; j < EPL; ++j) key[j] = key[j] ? (key[j] & ~kPlace<EPL>) | (kPlace<EPL> - j) : 0;
   // lane r < k: the r-th expert, its choice, logit and bias (the lanes from k on as lane k - 1)
   float my_c = value_of(top_k<LANES, EPL>(a.k, lane, key, chosen[slot]));
   const int first = lane & ~(LANES - 1), last = first + a.k - 1;
@@ -444,13 +484,14 @@ __global__ __launch_bounds__(64 * WAVES, EPL <= 16 ? 4 : 1) void k_gate_fwd(Gate
                          my_s < 1e-30f || !(fabsf(my_c) < __builtin_inff()) || blurred(my_c));
   const float cl = __shfl(my_c, last), zl = __shfl(my_z, last), bl = __shfl(my_b, last), least = cl - bound(cl);
   // (a key is 0 for an expert taken or left out: below that of any choice)
-  const uint32_t near = least < __builtin_inff() ? key_of(least) : 1u;
-  uint64_t at = 0;
+  const uint32_t near = least < __builtin_inff() ? key_of(least) & ~kPlace<EPL> : 1u;
+  if (key[0] >= near) {
 #pragma unroll
-  for (int j = 0; j < EPL; ++j) at |= (uint64_t)(key[j] >= near) << j;
-  for (; at; at &= at - 1) {
-    const int e = e0 + (int)__builtin_ctzll(at);
-    doubt |= !(z_of(e) == zl && (a.bias ? a.bias[e] : 0.0f) == bl);
+    for (int j = 0; j < EPL; ++j) {
+      if (key[j] < near || key[j] == 0) break;
+      const int e = e0 + (int)(kPlace<EPL> - (key[j] & kPlace<EPL>));
+      doubt |= !(z_of(e) == zl && (a.bias ? a.bias[e] : 0.0f) == bl);
+    }
   }
   const float total = lanes_sum<LANES>(sub < a.k ? my_s : 0.0f) + (float)kEps;
   float wt = (a.renormalize ? my_s / total : my_s) * a.scale;
