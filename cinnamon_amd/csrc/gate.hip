@@ -438,11 +438,18 @@ __global__ __launch_bounds__(64 * WAVES, EPL <= 16 ? 4 : 1) void k_gate_fwd(Gate
   const auto blurred = [&](float c) { return direct && !(c - zmax > -600.0f && (a.score == kSoftmax || c < 10.0f)); };
   uint32_t key[EPL];
   bool doubt = false;
+  float most = 0.0f;
 #pragma unroll
   for (int j = 0; j < EPL; ++j) {
     const float c = direct ? z[j] : s[j] + b[j];
-    key[j] = e0 + j < a.E ? key_of(c) : 0;
-    doubt |= e0 + j < a.E && !(c < __builtin_inff());  // NaN or infinite
+    key[j] = key_of(c);
+    const bool there = e0 + EPL <= a.E || e0 + j < a.E;
+    doubt |= there && !(c < __builtin_inff());  // NaN or infinite
+    most = fmaxf(most, there ? fabsf(c) : 0.0f);
+  }
+  if (e0 + EPL > a.E) {
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) key[j] = e0 + j < a.E ? key[j] : 0;
   }
   if (limited) {
     uint32_t* keys = keys32[slot];
@@ -451,19 +458,24 @@ __global__ __launch_bounds__(64 * WAVES, EPL <= 16 ? 4 : 1) void k_gate_fwd(Gate
     wave_sync();
     float margin, worst;
     const uint64_t kept = keep_groups<LANES, uint32_t, float>(a, keys, lane, margin, worst);
-    // two choices of up to `most` each on either side
     const int n = a.E / a.groups;
-    int g = e0 / n, left = n - (e0 - g * n);  // the group of e0 + j and its experts from there on
-    float most = 0.0f;
+    int g = e0 / n;  // the group of e0 + j
+    if (n % EPL == 0) {  // a lane's experts are of one group
+      const bool stays = kept >> (g & 63) & 1;
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) {
-      most = fmaxf(most, e0 + j < a.E ? fabsf(value_of(key[j])) : 0.0f);
-      if (!(kept >> g & 1)) key[j] = 0;
-      if (--left == 0) {
-        ++g;
-        left = n;
+      for (int j = 0; j < EPL; ++j) key[j] = stays ? key[j] : 0;
+    } else {
+      int left = n - (e0 - g * n);  // its experts from e0 + j on
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) {
+        if (!(kept >> (g & 63) & 1)) key[j] = 0;
+        if (--left == 0) {
+          ++g;
+          left = n;
+        }
       }
     }
+    // two choices of up to `most` each on either side
     most = __uint_as_float(lanes_max<LANES>(__float_as_uint(most)));
     doubt |= !(margin > 4 * bound(most) || (direct && margin == 0.0f)) || blurred(worst);
   }
