@@ -14,13 +14,18 @@
 //
 // Choices are ordered as they compare in 64 bits: neighbours in the order may differ by less than
 // 32 bits hold.  A token is first ranked in 32 bits; where every difference that decides exceeds
-// the error bound (or is one of equal logits and biases, a true tie), that is the order, else its
-// wave ranks it again in 64 bits (about one token in a thousand with random logits).  NaN counts as the greatest value, in a row and among groups.
+// the error bound (or is one of equal logits and biases, a true tie), that is the order.  Where the
+// chosen experts are sure and their order is not, they are sorted by their choices in 64 bits; else the
+// wave ranks the token again in 64 bits (256 experts with biases in 8 groups, top-8, random logits: the
+// order is in doubt in 1.3 tokens of a thousand, the choice in 0.2).  NaN counts as the greatest value, in a row and among groups.
 //
 // A token's experts lie over LANES lanes, EPL consecutive ones a lane, so that the order of the
 // lanes is the order of the indices: the lowest of equal candidates is the first lane of a ballot.
 // Up to 256 experts a token takes 16 lanes (a DPP row): maxima and sums need no LDS, and the rounds
-// of the top k serve four tokens at once.  Bound by VALU issue: see the rates at the launch.
+// of the top k serve four tokens at once.  65536 tokens, 256 bf16 logits in 8 groups of which 4 stay,
+// top-8, all scores out: 58 us, 1.8 TB/s, of which about 17 are the few waves that rank again in 64 bits
+// (they end last); bound by VALU issue (1600 instructions a wave).  A wave per token with 64-bit keys
+// throughout took 188 us.  The gradient, 22 us, 5.8 TB/s, is bound by HBM.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -426,11 +431,12 @@ __global__ __launch_bounds__(64 * WAVES, EPL <= 16 ? 4 : 1) void k_gate_fwd(Gate
   }
   // Without a bias, and with groups that count by one expert, the logits order as the choices do:
   // exactly, but where 64 bits cannot tell two scores apart (neighbours closer than 1e-10, sigmoids
-  // above 10, scores under e^-600).  Else in 32 bits, u = 2^-24: a score is off by less than
-  // (24 + EPL) u of itself, a choice by its rounding too, and ranked keys by 2 EPL u (that of a 16-bit
-  // logit by nothing: those bits are 0).
+  // above 10, scores under e^-600).  Else in 32 bits, u = 2^-24: a score is off by less than 8 u of
+  // itself (a softmax's by 6 + EPL u more, its sum's), a choice by its rounding too, and ranked keys by
+  // 2 EPL u (that of a 16-bit logit by nothing: those bits are 0).
   const bool direct = !a.bias && (!limited || a.group_top == 1);
-  constexpr float kU = 5.9604644775390625e-8f, kS = (48 + 2 * EPL) * kU, kC = (4 + 2 * EPL) * kU;
+  constexpr float kU = 5.9604644775390625e-8f, kC = (2 + 2 * EPL) * kU;
+  const float kS = (a.score == kSoftmax ? 28 + 2 * EPL : 16) * kU;
   constexpr float kZ = DT == CIN_DT_F32 ? 2 * EPL * kU : 0.0f;
   const auto bound = [&](float c) {
     return direct ? 1e-10f + kZ * fabsf(c) : kS * (a.bias ? top : fabsf(c)) + kC * fabsf(c);
@@ -477,7 +483,7 @@ __global__ __launch_bounds__(64 * WAVES, EPL <= 16 ? 4 : 1) void k_gate_fwd(Gate
     }
     // two choices of up to `most` each on either side
     most = __uint_as_float(lanes_max<LANES>(__float_as_uint(most)));
-    doubt |= !(margin > 4 * bound(most) || (direct && margin == 0.0f)) || blurred(worst);
+    doubt |= !(margin > 2 * bound(most) + 8 * kU * most || (direct && margin == 0.0f)) || blurred(worst);
   }
 #pragma unroll
   for (int j = 0; j < EPL; ++j) key[j] = key[j] ? (key[j] & ~kPlace<EPL>) | (kPlace<EPL> - j) : 0;
@@ -487,13 +493,13 @@ __global__ __launch_bounds__(64 * WAVES, EPL <= 16 ? 4 : 1) void k_gate_fwd(Gate
   int my_e = chosen[slot][sub < a.k ? sub : a.k - 1];
   const auto z_of = [&](int e) { return load_elem(a.logits, DT, t * a.ldl + e); };
   const float my_z = z_of(my_e), my_b = a.bias ? a.bias[my_e] : 0.0f;
-  const float my_s = a.score == kSigmoid ? sigmoid_of(my_z) : exp_of(my_z - zmax) * inv;
+  float my_s = a.score == kSigmoid ? sigmoid_of(my_z) : exp_of(my_z - zmax) * inv;
   // in doubt: neighbours in the order that are near and no true tie, an expert not taken that is
   // near the last one taken, and scores that 32 bits hardly hold
   const int up = sub > 0 ? lane - 1 : lane;
   const float c1 = __shfl(my_c, up), z1 = __shfl(my_z, up), b1 = __shfl(my_b, up);
-  doubt |= sub < a.k && ((sub > 0 && !(c1 - my_c > bound(fmaxf(fabsf(c1), fabsf(my_c)))) && !(z1 == my_z && b1 == my_b)) ||
-                         my_s < 1e-30f || !(fabsf(my_c) < __builtin_inff()) || blurred(my_c));
+  const bool order = sub > 0 && sub < a.k && !(c1 - my_c > bound(fmaxf(fabsf(c1), fabsf(my_c)))) && !(z1 == my_z && b1 == my_b);
+  doubt |= sub < a.k && (my_s < 1e-30f || !(fabsf(my_c) < __builtin_inff()) || blurred(my_c));
   const float cl = __shfl(my_c, last), zl = __shfl(my_z, last), bl = __shfl(my_b, last), least = cl - bound(cl);
   // (a key is 0 for an expert taken or left out: below that of any choice)
   const uint32_t near = least < __builtin_inff() ? key_of(least) & ~kPlace<EPL> : 1u;
@@ -503,6 +509,26 @@ __global__ __launch_bounds__(64 * WAVES, EPL <= 16 ? 4 : 1) void k_gate_fwd(Gate
       if (key[j] < near || key[j] == 0) break;
       const int e = e0 + (int)(kPlace<EPL> - (key[j] & kPlace<EPL>));
       doubt |= !(z_of(e) == zl && (a.bias ? a.bias[e] : 0.0f) == bl);
+    }
+  }
+  if (__ballot(order)) {
+    if (a.score == kSigmoid) {
+      // the experts taken are those, in another order perhaps: sorted by their choices in 64 bits
+      double c = 1 / (1 + exp(-(double)my_z)) + (double)my_b;
+      for (int pass = 0; pass < a.k; ++pass) {
+        const int p = (sub ^ (pass & 1)) & 1 ? sub - 1 : sub + 1;  // odd and even neighbours in turn
+        const bool pair = p >= 0 && p < a.k && sub < a.k;
+        const double pc = __shfl(c, first + (pair ? p : sub));
+        const int pe = __shfl(my_e, first + (pair ? p : sub));
+        const bool ahead = c > pc || (c == pc && my_e < pe);
+        if (pair && (sub < p) != ahead) {
+          c = pc;
+          my_e = pe;
+        }
+      }
+      my_s = sigmoid_of(z_of(my_e));
+    } else {
+      doubt |= order;
     }
   }
   const float total = lanes_sum<LANES>(sub < a.k ? my_s : 0.0f) + (float)kEps;
