@@ -19,6 +19,7 @@ from .kernels import _cdiv, _plain_eager, _require, custom_op
 
 __all__ = ["linear_cross_entropy"]
 
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
 _MODES = {"none": 0, "sum": 1, "mean": 2}
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
@@ -52,7 +53,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     if y.dtype != torch.int64:
         y = y.to(torch.int64)
     mode = _MODES[reduction]
-    if _plain_eager(x2, weight, y):
+    # (a layer's own Parameter is a plain tensor to the autograd Function)
+    if _plain_eager(y) and type(x2) in _PLAIN and type(weight) in _PLAIN:
         if torch.is_grad_enabled() and (x2.requires_grad or weight.requires_grad):
             loss = _LinearCE.apply(x2, weight, y, int(ignore_index), mode)
         else:
@@ -172,14 +174,18 @@ def _(x, weight, target, ignore_index, mode):
             x.new_empty((_layout(T, D, V, x.dtype)[1],), dtype=torch.uint8))
 
 
-@custom_op("linear_ce_backward", "(Tensor grad, Tensor state, Tensor weight, int T, int mode) -> (Tensor, Tensor)")
-def _backward_op(grad, state, weight, T, mode):
-    return _launch_backward(grad, state, weight, T, mode, True, True)
+@custom_op("linear_ce_backward", "(Tensor grad, Tensor state, Tensor weight, int T, int mode, bool need_x, bool need_w) -> "
+           "(Tensor, Tensor)")
+def _backward_op(grad, state, weight, T, mode, need_x, need_w):
+    # a gradient not asked for comes back as an empty placeholder
+    dx, dw = _launch_backward(grad, state, weight, T, mode, need_x, need_w)
+    return dx if need_x else weight.new_empty((0,)), dw if need_w else weight.new_empty((0,))
 
 
 @_backward_op.register_fake
-def _(grad, state, weight, T, mode):
-    return weight.new_empty((T, weight.shape[1])), weight.new_empty(weight.shape)
+def _(grad, state, weight, T, mode, need_x, need_w):
+    return (weight.new_empty((T, weight.shape[1]) if need_x else (0,)),
+            weight.new_empty(weight.shape if need_w else (0,)))
 
 
 def _setup(ctx, inputs, output):
@@ -191,8 +197,9 @@ def _setup(ctx, inputs, output):
 
 
 def _backward(ctx, grad, _state):
-    dx, dw = _backward_op(grad, *ctx.saved_tensors, *ctx.options)
-    return dx, dw, None, None, None
+    need_x, need_w = ctx.needs_input_grad[:2]
+    dx, dw = _backward_op(grad, *ctx.saved_tensors, *ctx.options, need_x, need_w)
+    return dx if need_x else None, dw if need_w else None, None, None, None
 
 
 _forward_op.register_autograd(_backward, setup_context=_setup)
