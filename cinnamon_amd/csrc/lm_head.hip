@@ -56,7 +56,9 @@ struct Cfg {
   static constexpr int kThreads = 64 * WM * WN, TM = 16 * MT * WM, TN = 16 * NT * WN;
   static constexpr int kStage = (TM + TN) * 128;
   static constexpr int kCStride = TN * 2 + 16;  // a staged row of 16-bit results; rows 4 banks apart
-  static constexpr int kBytes = STAGES * kStage > TM * kCStride ? STAGES * kStage : TM * kCStride;
+  // staged rows: all, or one row of waves at a time where all would not fit
+  static constexpr int kParts = TM * kCStride <= 160 * 1024 ? 1 : WM, kPartRows = TM / kParts;
+  static constexpr int kBytes = STAGES * kStage > kPartRows * kCStride ? STAGES * kStage : kPartRows * kCStride;
 };
 
 // What a product ends in.
@@ -414,36 +416,43 @@ __global__ __launch_bounds__(C::kThreads, 2) void k_ce_gemm(GemmArgs g) {
   const bool whole = (g.ldc & 7) == 0 && ((uintptr_t)g.C & 15) == 0;
 #pragma unroll 1
   for (int plane = 0; plane < (DT == CIN_DT_F32 ? 3 : 1); ++plane) {
+    uint16_t* out = static_cast<uint16_t*>(g.C) + plane * g.slab;
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int part = 0; part < C::kParts; ++part) {
+      if (C::kParts == 1 || wm == part) {
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const uint2 h = make_uint2(f32x2_to_half2_bits<kHalf>(acc[i][j][0], acc[i][j][1]),
-                                   f32x2_to_half2_bits<kHalf>(acc[i][j][2], acc[i][j][3]));
-        *reinterpret_cast<uint2*>(smem + ((wm * MT + i) * 16 + l16) * C::kCStride + ((wn * NT + j) * 16 + kq * 4) * 2) = h;
-        if constexpr (DT == CIN_DT_F32) {
-          acc[i][j][0] -= bf16_lo(h.x);
-          acc[i][j][1] -= bf16_hi(h.x);
-          acc[i][j][2] -= bf16_lo(h.y);
-          acc[i][j][3] -= bf16_hi(h.y);
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            const uint2 h = make_uint2(f32x2_to_half2_bits<kHalf>(acc[i][j][0], acc[i][j][1]),
+                                       f32x2_to_half2_bits<kHalf>(acc[i][j][2], acc[i][j][3]));
+            const int row = ((C::kParts == 1 ? wm : 0) * MT + i) * 16 + l16;
+            *reinterpret_cast<uint2*>(smem + row * C::kCStride + ((wn * NT + j) * 16 + kq * 4) * 2) = h;
+            if constexpr (DT == CIN_DT_F32) {
+              acc[i][j][0] -= bf16_lo(h.x);
+              acc[i][j][1] -= bf16_hi(h.x);
+              acc[i][j][2] -= bf16_lo(h.y);
+              acc[i][j][3] -= bf16_hi(h.y);
+            }
+          }
+      }
+      __syncthreads();
+      const int64_t mp = m0 + part * C::kPartRows;
+      for (int q = tid; q < C::kPartRows * kChunks; q += C::kThreads) {
+        const int m = q / kChunks, n = (q % kChunks) * 8;
+        if (mp + m >= M || n0 + n >= N) continue;
+        const v4u v = *reinterpret_cast<const v4u*>(smem + m * C::kCStride + n * 2);
+        uint16_t* d = out + (mp + m) * g.ldc + n0 + n;
+        if (whole && n0 + n + 8 <= N) {
+          *reinterpret_cast<v4u*>(d) = v;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (n0 + n + e < N) d[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
         }
       }
-    __syncthreads();
-    uint16_t* out = static_cast<uint16_t*>(g.C) + plane * g.slab;
-    for (int q = tid; q < C::TM * kChunks; q += C::kThreads) {
-      const int m = q / kChunks, n = (q % kChunks) * 8;
-      if (m0 + m >= M || n0 + n >= N) continue;
-      const v4u v = *reinterpret_cast<const v4u*>(smem + m * C::kCStride + n * 2);
-      uint16_t* d = out + (m0 + m) * g.ldc + n0 + n;
-      if (whole && n0 + n + 8 <= N) {
-        *reinterpret_cast<v4u*>(d) = v;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (n0 + n + e < N) d[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
-      }
+      if (DT == CIN_DT_F32 || part + 1 < C::kParts) __syncthreads();
     }
-    if constexpr (DT == CIN_DT_F32) __syncthreads();
   }
 }
 
@@ -730,19 +739,22 @@ __global__ __launch_bounds__(256) void k_ce_dx(const float* __restrict__ slabs, 
 // ---------------------------------------------------------------------------
 // Host
 // ---------------------------------------------------------------------------
-// Tiles.  Wide ones read their operands less often and keep the matrix units busier; narrow ones
-// leave fewer compute units idle in a small product, and the narrowest, with more steps on their way,
-// stream w for a few rows.
+// Tiles.  Wide ones read their operands less often and keep the matrix units busier (without loads
+// the 256 x 256 tile's loop runs at 1.62 PFLOP/s, with operands that hit the L2 at 1.32, at full length
+// at 1.23); narrow ones leave fewer compute units idle in a small product, and the narrowest, with more
+// steps on their way, stream w for a few rows.  8192 x 131072 x 4096, bf16: x w^T 1.32 and 1.24 PFLOP/s
+// with the two widest; 16368 x 32000 x 1024: 1.07 and 0.97, 0.89 with 128 x 128.
+using Widest = Cfg<2, 4, 8, 6, 2>;  // 256 x 384, 8 waves of 128 x 96: 250 registers, all of the LDS
 using Wide = Cfg<2, 4, 8, 4, 2>;    // 256 x 256, 8 waves of 128 x 64
 using Medium = Cfg<2, 2, 4, 4, 2>;  // 128 x 128, 4 waves of 64 x 64, two workgroups a CU
 using Narrow = Cfg<1, 4, 4, 1, 4>;  // 64 x 64, 4 waves of 64 x 16, two workgroups a CU
-constexpr int kTiles = 3;
-constexpr int kTileM[kTiles] = {Wide::TM, Medium::TM, Narrow::TM};
-constexpr int kTileN[kTiles] = {Wide::TN, Medium::TN, Narrow::TN};
-// a tile's rate against that of the widest, every CU at work
-constexpr double kTileRate[kTiles] = {1.0, 0.75, 0.4};
+constexpr int kTiles = 4;
+constexpr int kTileM[kTiles] = {Widest::TM, Wide::TM, Medium::TM, Narrow::TM};
+constexpr int kTileN[kTiles] = {Widest::TN, Wide::TN, Medium::TN, Narrow::TN};
+// a tile's rate against that of the 256 x 256 ones, every CU at work
+constexpr double kTileRate[kTiles] = {1.08, 1.0, 0.75, 0.4};
 
-// The time of m x n outputs in parts of K, in units of one output's share at the widest tile's rate.
+// The time of m x n outputs in parts of K, in units of one output's share at the 256 x 256 tile's rate.
 double tile_time(int tile, int64_t m, int64_t n, double parts, double part) {
   const double count = (double)cdiv(m, kTileM[tile]) * (double)cdiv(n, kTileN[tile]) * parts;
   const double rounds = ceil(count / cin_device_cus());
@@ -757,8 +769,10 @@ int pick_tile(int64_t m, int64_t n) {
 template <class F>
 void with_tile(int tile, F f) {
   if (tile == 0)
-    f(Wide{});
+    f(Widest{});
   else if (tile == 1)
+    f(Wide{});
+  else if (tile == 2)
     f(Medium{});
   else
     f(Narrow{});
