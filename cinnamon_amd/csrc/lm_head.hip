@@ -476,44 +476,42 @@ __device__ __forceinline__ int find_rows(const int64_t* __restrict__ y, int64_t 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int base = 0;
   for (int64_t t0 = 0; t0 < T; t0 += THREADS * kRowPer) {
-    const int64_t first = t0 + (int64_t)tid * kRowPer;
+    // A wave has 64 kRowPer rows in a run, a lane one of each 64, so that loads and stores are whole lines.
+    const int64_t first = t0 + (int64_t)wave * 64 * kRowPer + lane;
     int64_t v[kRowPer];
-    int mine = 0;
+    int before_me[kRowPer], mine = 0;
+#pragma unroll
+    for (int j = 0; j < kRowPer; ++j) v[j] = first + j * 64 < T ? y[first + j * 64] : ignore;
 #pragma unroll
     for (int j = 0; j < kRowPer; ++j) {
-      v[j] = first + j < T ? y[first + j] : ignore;
-      mine += v[j] != ignore;
+      const uint64_t kept = __ballot(v[j] != ignore);
+      before_me[j] = mine + __popcll(kept & ((1ull << lane) - 1));
+      mine += __popcll(kept);
     }
-    int incl = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int o = __shfl_up(incl, d);
-      if (lane >= d) incl += o;
-    }
-    if (lane == 63) wsum[wave] = incl;
+    if (lane == 0) wsum[wave] = mine;
     __syncthreads();
-    int before = 0, all = 0;
+    int before = base, all = 0;
 #pragma unroll
     for (int w = 0; w < THREADS / 64; ++w) {
       if (w < wave) before += wsum[w];
       all += wsum[w];
     }
-    int i = base + before + incl - mine;
 #pragma unroll
     for (int j = 0; j < kRowPer; ++j) {
-      if (first + j >= T) break;
+      const int64_t t = first + j * 64;
+      if (t >= T) break;
       const bool kept = v[j] != ignore;
-      if (lds_map && kept) lds_map[i] = (int)(first + j);
+      const int i = before + before_me[j];
+      if (lds_map && kept) lds_map[i] = (int)t;
       if (write) {
         if (kept) {
-          st.map[i] = (int)(first + j);
+          st.map[i] = (int)t;
           st.target[i] = v[j] >= 0 && v[j] < V ? (int)v[j] : -1;
         } else {
-          rowloss[first + j] = 0.0f;
+          rowloss[t] = 0.0f;
         }
-        st.pos[first + j] = kept ? i : -1;
+        st.pos[t] = kept ? i : -1;
       }
-      i += kept;
     }
     base += all;
     __syncthreads();
