@@ -670,8 +670,10 @@ int gate_args(const char* name, GateArgs& a, const void* logits, int dtype, int6
               int64_t E, int64_t k, int score, int64_t groups, int64_t top_groups, int group_top, int renormalize,
               float scale) {
   CIN_CHECK_ARG(dtype == CIN_DT_BF16 || dtype == CIN_DT_F32 || dtype == CIN_DT_F16, "%s: bad dtype %d", name, dtype);
-  CIN_CHECK_ARG(T >= 0 && T < ((int64_t)1 << 31), "%s: T must be in [0, 2^31)", name);
+  CIN_CHECK_ARG(T >= 0, "%s: negative size", name);
   CIN_CHECK_ARG(E >= 1 && E <= kGateMaxExperts, "%s: 1 to %d experts", name, kGateMaxExperts);
+  // (a launch has fewer than 2^32 threads: 16 a token up to 256 experts, 64 above)
+  CIN_CHECK_ARG(T <= ((int64_t)1 << (E <= 256 ? 28 : 26)) - 16, "%s: too many tokens", name);
   CIN_CHECK_ARG(k >= 1 && k <= kGateMaxTopK, "%s: top-k of 1 to %d", name, kGateMaxTopK);
   CIN_CHECK_ARG(score == kSigmoid || score == kSoftmax, "%s: bad score function %d", name, score);
   CIN_CHECK_ARG(groups >= 1 && groups <= kGateMaxGroups && E % groups == 0,

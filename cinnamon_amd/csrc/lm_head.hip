@@ -749,6 +749,7 @@ using Narrow = Cfg<1, 4, 4, 1, 4>;  // 64 x 64, 4 waves of 64 x 16, two workgrou
 constexpr int kTiles = 4;
 constexpr int kTileM[kTiles] = {Widest::TM, Wide::TM, Medium::TM, Narrow::TM};
 constexpr int kTileN[kTiles] = {Widest::TN, Wide::TN, Medium::TN, Narrow::TN};
+constexpr int kTileThreads[kTiles] = {Widest::kThreads, Wide::kThreads, Medium::kThreads, Narrow::kThreads};
 // a tile's rate against that of the 256 x 256 ones, every CU at work
 constexpr double kTileRate[kTiles] = {1.08, 1.0, 0.75, 0.4};
 
@@ -776,7 +777,8 @@ void with_tile(int tile, F f) {
     f(Narrow{});
 }
 
-constexpr int64_t kMaxT = (int64_t)1 << 30, kMaxV = (int64_t)1 << 30, kMaxD = (int64_t)1 << 18;
+// A launch has fewer than 2^32 threads: k_ce_join takes 64 a row.
+constexpr int64_t kMaxT = ((int64_t)1 << 26) - 4, kMaxV = (int64_t)1 << 29, kMaxD = (int64_t)1 << 18;
 constexpr int64_t kPieceBytes = (int64_t)1 << 30;  // dz of one piece
 constexpr int64_t kMaxPiece = (int64_t)1 << 20;    // its columns: 256 rows lie within 2^31 bytes
 
@@ -829,18 +831,26 @@ Plan make_plan(int dtype, int64_t T, int64_t D, int64_t V) {
   return p;
 }
 
-int check(const char* name, int dtype, int64_t T, int64_t D, int64_t V) {
+// Whether a product's launch has fewer than 2^32 threads.
+bool grid_fits(int tile, int64_t m, int64_t n) {
+  return (double)cdiv(m, kTileM[tile]) * (double)cdiv(n, kTileN[tile]) * kTileThreads[tile] < 4294967296.0;
+}
+
+int check(const char* name, int dtype, int64_t T, int64_t D, int64_t V, Plan& p) {
   CIN_CHECK_ARG(dtype == CIN_DT_BF16 || dtype == CIN_DT_F32 || dtype == CIN_DT_F16, "%s: bad dtype %d", name, dtype);
-  CIN_CHECK_ARG(T >= 0 && T < kMaxT, "%s: T must be in [0, 2^30)", name);
-  CIN_CHECK_ARG(V >= 1 && V < kMaxV, "%s: V must be in [1, 2^30)", name);
+  CIN_CHECK_ARG(T >= 0 && T <= kMaxT, "%s: T must be in [0, 2^26 - 4]", name);
+  CIN_CHECK_ARG(V >= 1 && V <= kMaxV, "%s: V must be in [1, 2^29]", name);
   CIN_CHECK_ARG(D >= 1 && D <= kMaxD, "%s: D must be in [1, 2^18]", name);
-  CIN_CHECK_ARG(cdiv(T, 64) * cdiv(V, 64) < ((int64_t)1 << 31) && cdiv(V, 64) * cdiv(D, 64) < ((int64_t)1 << 31),
-                "%s: T x V or V x D is too large", name);
+  // (the products over a piece of the vocabulary are smaller: T x piece < 2^30 + 256 T)
+  p = make_plan(dtype, T, D, V);
+  CIN_CHECK_ARG(grid_fits(p.tile, T, V) && grid_fits(p.slab_tile, T, p.Dp) && grid_fits(pick_tile(p.piece, D), p.piece, D),
+                "%s: T x V, T x D or V x D is too large", name);
   return CIN_OK;
 }
 
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 bool w_fits(const void* w, int64_t ldw) {
-  return ((uintptr_t)w & 15) == 0 && ldw * kEs % 16 == 0 && ldw <= 4 * kMaxD;
+  return aligned16(w) && ldw * kEs % 16 == 0 && ldw <= 4 * kMaxD;
 }
 
 template <class F>
@@ -880,8 +890,8 @@ void copy_rows(bool f32, const void* x, int64_t ldx, int64_t rows, int64_t D, co
 extern "C" {
 
 int64_t cin_linear_ce_workspace(int dtype, int64_t T, int64_t D, int64_t V, int backward) {
-  if (check("linear_ce_workspace", dtype, T, D, V)) return -1;
-  const Plan p = make_plan(dtype, T, D, V);
+  Plan p;
+  if (check("linear_ce_workspace", dtype, T, D, V, p)) return -1;
   return backward ? p.dz + p.slabs + p.coef : p.part + p.ztarget;
 }
 
@@ -890,12 +900,13 @@ int cin_linear_ce_forward(const void* x, int dtype, int64_t T, int64_t D, int64_
                           int32_t* state_i, float* state_f, float* rowloss, float* loss, void* workspace,
                           int64_t workspace_bytes, void* stream) {
   const char* name = "linear_ce_forward";
-  if (int rc = check(name, dtype, T, D, V)) return rc;
+  Plan p;
+  if (int rc = check(name, dtype, T, D, V, p)) return rc;
   CIN_CHECK_ARG(ldx >= D && ldw >= D, "%s: rows overlap", name);
   CIN_CHECK_ARG(state_i && w && (T == 0 || (x && target && xc && state_f && rowloss)), "%s: null pointer", name);
-  const Plan p = make_plan(dtype, T, D, V);
   const bool f32 = dtype == CIN_DT_F32;
   CIN_CHECK_ARG(wp || (!f32 && w_fits(w, ldw) && p.Dp == D), "%s: w needs a padded copy", name);
+  CIN_CHECK_ARG(aligned16(xc) && aligned16(wp) && aligned16(workspace), "%s: xc, wp and workspace must lie on 16 bytes", name);
   CIN_CHECK_ARG(workspace_bytes >= p.part + p.ztarget && workspace, "%s: workspace needs %lld bytes", name,
                 (long long)(p.part + p.ztarget));
   hipStream_t s = static_cast<hipStream_t>(stream);
@@ -945,12 +956,13 @@ int cin_linear_ce_backward(const void* xc, int dtype, int64_t T, int64_t D, cons
                            const int32_t* state_i, const float* state_f, const float* grad, int64_t grad_stride,
                            int mean, void* dx, void* dw, void* workspace, int64_t workspace_bytes, void* stream) {
   const char* name = "linear_ce_backward";
-  if (int rc = check(name, dtype, T, D, V)) return rc;
-  const Plan p = make_plan(dtype, T, D, V);
+  Plan p;
+  if (int rc = check(name, dtype, T, D, V, p)) return rc;
   CIN_CHECK_ARG(w_fits(w, ldw) && (dtype == CIN_DT_F32 ? ldw == p.Dp : ldw >= p.Dp),
                 "%s: w's rows must be padded as the forward's", name);
   CIN_CHECK_ARG(grad_stride >= 0, "%s: negative gradient stride", name);
   CIN_CHECK_ARG(T > 0 && state_i && state_f && xc && w && grad, "%s: null pointer", name);
+  CIN_CHECK_ARG(aligned16(xc) && aligned16(dx) && aligned16(workspace), "%s: xc, dx and workspace must lie on 16 bytes", name);
   CIN_CHECK_ARG(workspace && workspace_bytes >= p.dz + p.slabs + p.coef, "%s: workspace needs %lld bytes", name,
                 (long long)(p.dz + p.slabs + p.coef));
   hipStream_t s = static_cast<hipStream_t>(stream);

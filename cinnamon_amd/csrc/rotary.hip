@@ -35,6 +35,7 @@ struct RotaryArgs {
   Side q, k;
   int qheads;
   int64_t n, L;            // units in all, tokens of a sequence
+  int64_t base;            // workgroups of the launches before this one
   const float *cos, *sin;
   int64_t P, ldt;
   int rot, start, turned;  // units of a head that turn: the first ones
@@ -122,7 +123,7 @@ template <int DT, int E, bool INTER>
 __global__ __launch_bounds__(kThreads) void k_rotary(RotaryArgs a) {
   constexpr int kPairs = INTER ? (E > 1 ? E / 2 : 1) : E;  // pairs of a turning unit
   constexpr bool kTwo = !INTER || E == 1;                  // ... which lie in two chunks
-  const int64_t first = (int64_t)blockIdx.x * kSpan;
+  const int64_t first = (a.base + blockIdx.x) * kSpan;
   const int64_t tok0 = div_by(first, (int64_t)a.row, a.wrow);
   const uint32_t rem0 = (uint32_t)(first - tok0 * a.row);
   const int64_t b0 = div_by(tok0, a.L, a.wL), l0 = tok0 - b0 * a.L;
@@ -246,7 +247,7 @@ int cin_rotary(const void* q, int64_t sqb, int64_t sql, int64_t sqh, void* q_out
                 "rotary: null pointer");
   CIN_CHECK_ARG((double)B * L * heads * D < 9e15, "rotary: too many elements");
   const int es = dtype == CIN_DT_F32 ? 4 : 2;
-  RotaryArgs a{{q, q_out, sqb, sql, sqh, soqb, soql, soqh}, {k, k_out, skb, skl, skh, sokb, sokl, sokh}, (int)H, 0, L, cos, sin,
+  RotaryArgs a{{q, q_out, sqb, sql, sqh, soqb, soql, soqh}, {k, k_out, skb, skl, skh, sokb, sokl, sokh}, (int)H, 0, L, 0, cos, sin,
                P, ldt, (int)rot, (int)start, 0, 0, 0, 0, 0, 0, 0, 0, 0, positions, spb, spl, interleaved, inverse};
   // 16 bytes at a time where they hold turning or copied channels only, whatever their alignment:
   // 1 x 32767 x 32 heads, fp16, rot 64: 207 us with heads of 192 channels, 267 with 193 (one
@@ -269,15 +270,20 @@ int cin_rotary(const void* q, int64_t sqb, int64_t sql, int64_t sqh, void* q_out
   a.wrow = magic64(a.row);
   a.wL = magic64((uint64_t)L);
   const int64_t blocks = cdiv(a.n, kSpan);
-  CIN_CHECK_ARG(blocks < ((int64_t)1 << 31) && (double)a.n * a.row < 9e18 && (double)B * L * L < 9e18,
+  CIN_CHECK_ARG((double)a.n * a.row < 9e18 && (double)B * L * L < 9e18,
                 "rotary: too many elements");
   for (int64_t st : {sql, sqh, soql, soqh, skl, skh, sokl, sokh})
     CIN_CHECK_ARG(st < ((int64_t)1 << 31) && st > -((int64_t)1 << 31), "rotary: token and head strides must fit in 32 bits");
+  // (a launch has fewer than 2^32 threads)
+  constexpr int64_t kMost = (int64_t)1 << 23;
   auto go = [&](auto dt, auto e) {
-    if (interleaved)
-      hipLaunchKernelGGL((k_rotary<dt(), e(), true>), (unsigned)blocks, kThreads, 0, static_cast<hipStream_t>(stream), a);
-    else
-      hipLaunchKernelGGL((k_rotary<dt(), e(), false>), (unsigned)blocks, kThreads, 0, static_cast<hipStream_t>(stream), a);
+    for (a.base = 0; a.base < blocks; a.base += kMost) {
+      const unsigned grid = (unsigned)(blocks - a.base < kMost ? blocks - a.base : kMost);
+      if (interleaved)
+        hipLaunchKernelGGL((k_rotary<dt(), e(), true>), grid, kThreads, 0, static_cast<hipStream_t>(stream), a);
+      else
+        hipLaunchKernelGGL((k_rotary<dt(), e(), false>), grid, kThreads, 0, static_cast<hipStream_t>(stream), a);
+    }
   };
   auto with_e = [&](auto dt) {
     if (E > 1)

@@ -89,8 +89,13 @@ def _sizes(T, D, V, dtype):
 
 
 def _rows(t):
-    """Rows of adjacent elements that do not overlap."""
+    """Rows of adjacent elements that do not overlap (_pitch apart)."""
     return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
+
+
+def _pitch(t):
+    """Elements between rows; a single row's stride says nothing."""
+    return max(t.stride(0), t.shape[1])
 
 
 def _weight_rows(w):
@@ -98,7 +103,7 @@ def _weight_rows(w):
     if w.stride(1) == 1 and w.stride(0) >= w.shape[1] and w.stride(0) * w.element_size() % 16 == 0 \
             and w.data_ptr() % 16 == 0 and w.stride(0) <= 1 << 20:
         return w
-    return w.contiguous() if not w.is_contiguous() else w.clone()
+    return w.contiguous() if not w.is_contiguous() else w.clone(memory_format=torch.contiguous_format)
 
 
 def _launch_forward(x, weight, target, ignore_index, mode):
@@ -113,7 +118,7 @@ def _launch_forward(x, weight, target, ignore_index, mode):
     rows = x.new_empty(T, dtype=torch.float32)
     loss = x.new_empty((), dtype=torch.float32) if mode else rows
     at = state.data_ptr()
-    call_on(x, "cin_linear_ce_forward", x.data_ptr(), dtype_code(x), T, D, x.stride(0), w.data_ptr(), V, w.stride(0),
+    call_on(x, "cin_linear_ce_forward", x.data_ptr(), dtype_code(x), T, D, _pitch(x), w.data_ptr(), V, _pitch(w),
             target.data_ptr(), ignore_index, mode == 2, at + xc, at + wp if copied else 0, at + si, at + sf,
             rows.data_ptr(), loss.data_ptr() if mode else 0, work.data_ptr(), ws, stream_of(x))
     return loss, state
@@ -133,7 +138,7 @@ def _launch_backward(grad, state, weight, T, mode, need_x, need_w):
         w, ldw = at + wp, _cdiv(D, 64) * 64
     else:
         weight = _weight_rows(weight)
-        w, ldw = weight.data_ptr(), weight.stride(0)
+        w, ldw = weight.data_ptr(), _pitch(weight)
     work = torch.empty(ws, dtype=torch.uint8, device=weight.device)
     call_on(weight, "cin_linear_ce_backward", at + xc, dtype_code(dtype), T, D, w, V, ldw, at + si, at + sf, grad.data_ptr(),
             0 if mode else grad.stride(0), mode == 2, ptr(dx), ptr(dw), work.data_ptr(), ws, stream_of(weight))

@@ -520,7 +520,7 @@ int cin_moe_combine_backward(const float* dout, int64_t sdm, const void* y, int 
  * lowest index; compared in 64 bits, NaN as the greatest.
  *   logits [T, E] of dtype, row stride ldl; idx [T, k] int64; weights [T, k] fp32 =
  *   scale * s[idx], with renormalize divided by (their sum + 1e-9); scores [T, E] fp32 or null.
- * E <= 4096, k <= 16 and within the kept groups, groups <= 64.
+ * E <= 4096, k <= 16 and within the kept groups, groups <= 64; T below 2^28 (2^26 above 256 experts).
  */
 int cin_moe_gate(const void* logits, int dtype, int64_t ldl, const float* bias, int64_t T, int64_t E,
                  int64_t k, int score, int64_t groups, int64_t top_groups, int group_top,
@@ -563,8 +563,9 @@ int cin_rotary(const void* q, int64_t sqb, int64_t sql, int64_t sqh, void* q_out
  * [2 T] fp32, Dp = D rounded up to 64; and wp [V, Dp] of dtype, a padded copy of w that is needed
  * (else null) where Dp != D or w's rows do not start on 16 bytes.  For fp32, xc is [3, T, Dp] and wp,
  * always needed, [3, V, Dp] bf16: three parts of each value.
- *   workspace: cin_linear_ce_workspace(dtype, T, D, V, backward) bytes, 16-byte aligned (-1 for
- *   sizes that are refused).
+ *   workspace: cin_linear_ce_workspace(dtype, T, D, V, backward) bytes (-1 for sizes that are
+ *   refused: T above 2^26 - 4, V above 2^29, D above 2^18, products of 2^32 threads).  It, xc, wp and
+ *   dx lie on 16 bytes.
  * Backward: w and ldw as the products read them (wp and Dp where there is a copy); grad fp32, of
  * the loss (grad_stride 0, with mean divided by the rows that count) or of each row (grad_stride
  * elements apart); dx [T, D] and dw [V, D] of dtype, contiguous, either null.  Gradients are

@@ -381,6 +381,8 @@ def test_gate_refusals():
     ("cin_moe_gate", (1, 0, 64, None, 4, 64, 2, 0, 1, 1, 2, 1, 1.0, None, 1, None, None)),  # null
     ("cin_moe_gate_backward", (1, 0, 64, 4, 64, 2, 0, 1, 1.0, None, 1, 1, 1, None)),        # null
     ("cin_moe_gate_backward", (1, 0, 64, -1, 64, 2, 0, 1, 1.0, 1, 1, 1, 1, None)),          # T
+    ("cin_moe_gate", (1, 0, 64, None, 1 << 28, 64, 2, 0, 1, 1, 2, 1, 1.0, 1, 1, None, None)),     # 2^32 threads
+    ("cin_moe_gate", (1, 0, 512, None, 1 << 26, 512, 2, 0, 1, 1, 2, 1, 1.0, 1, 1, None, None)),
 ])
 def test_gate_c_refusals(name, args):
     with pytest.raises(ValueError):

@@ -200,6 +200,31 @@ def test_strides_shapes_and_targets_types(dev, dt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 65])
+def test_a_single_row_whose_stride_is_not_its_width(dev, D):
+    """One token, and a vocabulary of one: a transposed column's only row has a stride of 1."""
+    x = torch.randn(D, 1, device=dev).to(torch.bfloat16).t()
+    w = torch.randn(D, 1, device=dev).to(torch.bfloat16).t()
+    y = torch.zeros(1, dtype=torch.int64, device=dev)
+    assert x.stride(0) == w.stride(0) == 1
+    many = torch.randn(37, D, device=dev).to(torch.bfloat16)
+    for a, b, t in ((x, many, y + 5), (many, w, y.expand(37)), (x, w, y)):
+        a, b = a.detach().requires_grad_(), b.detach().requires_grad_()
+        a64, b64 = a.detach().double().requires_grad_(), b.detach().double().requires_grad_()
+        loss = lm_head.linear_cross_entropy(a, b, t, reduction="sum")
+        want = torch.nn.functional.cross_entropy(a64 @ b64.T, t, reduction="sum")
+        da, db = torch.autograd.grad(loss, (a, b))
+        wa, wb = torch.autograd.grad(want, (a64, b64))
+        # (65 products of up to 4 x 4 summed in fp32; exponentials, one more sum and a logarithm)
+        assert abs(loss.item() - want.item()) <= 2e-5 * max(1.0, abs(want.item()))
+        # the gradient of the logits and each gradient are rounded once, by up to 2^-8 of itself; sums of up
+        # to 37 terms of at most 4.5, and fp32's part below
+        for g, r in ((da, wa), (db, wb)):
+            bound = 2 ** -8 * r.abs() + 37 * 4.5 * 2 ** -8 + 1e-4
+            assert g.shape == r.shape and ((g.double() - r).abs() <= bound).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
 def test_no_tokens(dev, dt):
     w = torch.randn(50, 64, device=dev).to(DT[dt]).requires_grad_(True)
@@ -414,6 +439,10 @@ _BWD = [16, 0, 4, 64, 16, 100, 64, 16, 16, 16, 0, 1, 16, 16, 16, 1 << 30, None]
     ("cin_linear_ce_backward", _BWD, 1, 4), ("cin_linear_ce_backward", _BWD, 2, 0), ("cin_linear_ce_backward", _BWD, 6, 65),
     ("cin_linear_ce_backward", _BWD, 4, 18), ("cin_linear_ce_backward", _BWD, 9, None), ("cin_linear_ce_backward", _BWD, 10, -1),
     ("cin_linear_ce_backward", _BWD, 14, None), ("cin_linear_ce_backward", _BWD, 15, 100), ("cin_linear_ce_backward", _BWD, 3, 65),
+    # launches of 2^32 threads, and pointers that 16-byte accesses do not fit
+    ("cin_linear_ce_forward", _FWD, 2, 1 << 26), ("cin_linear_ce_forward", _FWD, 6, (1 << 29) + 1),
+    ("cin_linear_ce_forward", _FWD, 11, 24), ("cin_linear_ce_forward", _FWD, 12, 24), ("cin_linear_ce_forward", _FWD, 17, 24),
+    ("cin_linear_ce_backward", _BWD, 0, 24), ("cin_linear_ce_backward", _BWD, 12, 24), ("cin_linear_ce_backward", _BWD, 14, 24),
 ])
 def test_c_refusals(name, ok, at, value):
     args = list(ok)

@@ -179,6 +179,19 @@ def test_rotary_offsets_past_32_bits(dev):
 
 
 @pytest.mark.gpu
+def test_rotary_more_work_than_one_launch_holds(dev):
+    """2^33 channels copied one at a time, 2^32 threads: one row of heads, repeated by a stride of 0."""
+    B, H, D, rot = (1 << 14) + 1, 4, (1 << 17) - 1, 6
+    cos, sin = (torch.full((1, rot // 2), v, device=dev) for v in (0.6, 0.8))
+    x = torch.randn(1, 1, H, D, device=dev).to(torch.bfloat16).expand(B, 1, H, D)
+    y = rotary.apply_rotary(x, cos, sin, start=3)
+    assert y.numel() > 1 << 33
+    check(y[:1], turn(x[:1], cos, sin, torch.zeros(1, dtype=torch.int64, device=dev), True, 3), "bf16")
+    for b in range(0, B, 1024):
+        assert torch.equal(y[b:b + 1024], y[:1].expand(min(1024, B - b), 1, H, D))
+
+
+@pytest.mark.gpu
 def test_rotary_undoes_itself_and_keeps_lengths(dev):
     cos, sin = rotary.rotary_tables(128, 5000, device=dev)
     x = torch.randn(2, 300, 4, 128, device=dev, requires_grad=True)
