@@ -20,9 +20,15 @@ using namespace cin;
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kUnits = 2;                    // units a thread, their loads in flight together
-constexpr int kSpan = kThreads * kUnits;     // units a workgroup
-constexpr uint32_t kMagicLimit = 60000;      // (kSpan + d) d < 2^32: see div_by
+constexpr int kMaxUnits = 2;
+constexpr uint32_t kMagicLimit = 60000;      // (kThreads kMaxUnits + d) d < 2^32: see div_by
+
+// Units a thread, their loads in flight together.  One is as fast for 16-byte units of 16-bit elements or
+// faster (64 x 1024 x 17 heads of 64: 61 us, with two 64; 16 x 1024: 14.9 and 16.6; heads of 193: 267 and
+// 260); two for fp32 (1 x 32767 x 32 heads of 192: 343 and 325) and for single channels (918 and 770),
+// and four need half as many registers again for the half layout (269 against 207).
+template <int DT, int E>
+constexpr int kUnitsOf = DT != CIN_DT_F32 && E > 1 ? 1 : kMaxUnits;
 
 // One of the two tensors, [B, L, heads, D] with unit channel stride.
 struct Side {
@@ -112,18 +118,19 @@ __device__ __forceinline__ void load_pairs(const float* p, float (&v)[N]) {
 // A unit is 16 bytes of a head's channels (E elements) or one channel (E = 1), and where it turns
 // whole pairs: with the half layout the unit rot / 2 further comes with it, and single interleaved
 // channels come in twos.  The last 16 bytes of the copied channels before or after the turning ones
-// may overlap the ones in front of them (the same values twice); fewer go one by one.  Bound by HBM: each element is read and written once; the tables' rows
-// are shared by a token's heads through the caches.  A workgroup takes kSpan neighbouring units;
-// their token, head, channel and offsets follow from the first one's in 32 bits (with 64-bit
-// divisions and products the vector units bound it: 1 x 32767 x 32 heads of 192, fp16, half layout,
-// 355 us).  That call now takes 207 us, 3.9 TB/s, its interleaved form 170 (4.8), 64 x 1024 x 17
-// heads of 64 in bf16 55 us, 5.2 TB/s.  Two units a thread: four need half as many registers again
-// for the half layout (269 us), one is as fast for it and slower for odd heads (918 us against 770).
+// may overlap the ones in front of them (the same values twice); fewer go one by one.
+// Bound by HBM: each element is read and written once; the tables' rows are shared by a token's heads
+// through the caches.  A workgroup takes neighbouring units; their token, head, channel and offsets
+// follow from the first one's in 32 bits (with 64-bit divisions and products the vector units bound it:
+// 1 x 32767 x 32 heads of 192, fp16, half layout, 355 us).  That call now takes 204 us, 4.0 TB/s, its
+// interleaved form 178 (4.6), 64 x 1024 x 17 heads of 64 in bf16 61 us, 4.7 TB/s.  Stores that bypass
+// the caches take 46 us there, and the next reader of the result as much more.
 template <int DT, int E, bool INTER>
 __global__ __launch_bounds__(kThreads) void k_rotary(RotaryArgs a) {
   constexpr int kPairs = INTER ? (E > 1 ? E / 2 : 1) : E;  // pairs of a turning unit
   constexpr bool kTwo = !INTER || E == 1;                  // ... which lie in two chunks
-  const int64_t first = (a.base + blockIdx.x) * kSpan;
+  constexpr int kUnits = kUnitsOf<DT, E>;
+  const int64_t first = (a.base + blockIdx.x) * (kThreads * kUnits);
   const int64_t tok0 = div_by(first, (int64_t)a.row, a.wrow);
   const uint32_t rem0 = (uint32_t)(first - tok0 * a.row);
   const int64_t b0 = div_by(tok0, a.L, a.wL), l0 = tok0 - b0 * a.L;
@@ -250,7 +257,7 @@ int cin_rotary(const void* q, int64_t sqb, int64_t sql, int64_t sqh, void* q_out
   RotaryArgs a{{q, q_out, sqb, sql, sqh, soqb, soql, soqh}, {k, k_out, skb, skl, skh, sokb, sokl, sokh}, (int)H, 0, L, 0, cos, sin,
                P, ldt, (int)rot, (int)start, 0, 0, 0, 0, 0, 0, 0, 0, 0, positions, spb, spl, interleaved, inverse};
   // 16 bytes at a time where they hold turning or copied channels only, whatever their alignment:
-  // 1 x 32767 x 32 heads, fp16, rot 64: 207 us with heads of 192 channels, 267 with 193 (one
+  // 1 x 32767 x 32 heads, fp16, rot 64: 204 us with heads of 192 channels, 267 with 193 (one
   // channel at a time 770).
   const int64_t e16 = 16 / es;
   const bool odd = (interleaved ? rot : rot / 2) % e16 || ((uintptr_t)cos | (uintptr_t)sin) % 16 || ldt % 4;
@@ -269,7 +276,6 @@ int cin_rotary(const void* q, int64_t sqb, int64_t sql, int64_t sqh, void* q_out
   auto magic64 = [](uint64_t d) { return d < 2 ? 0ull : ~0ull / d + 1; };
   a.wrow = magic64(a.row);
   a.wL = magic64((uint64_t)L);
-  const int64_t blocks = cdiv(a.n, kSpan);
   CIN_CHECK_ARG((double)a.n * a.row < 9e18 && (double)B * L * L < 9e18,
                 "rotary: too many elements");
   for (int64_t st : {sql, sqh, soql, soqh, skl, skh, sokl, sokh})
@@ -277,6 +283,7 @@ int cin_rotary(const void* q, int64_t sqb, int64_t sql, int64_t sqh, void* q_out
   // (a launch has fewer than 2^32 threads)
   constexpr int64_t kMost = (int64_t)1 << 23;
   auto go = [&](auto dt, auto e) {
+    const int64_t blocks = cdiv(a.n, kThreads * kUnitsOf<dt(), e()>);
     for (a.base = 0; a.base < blocks; a.base += kMost) {
       const unsigned grid = (unsigned)(blocks - a.base < kMost ? blocks - a.base : kMost);
       if (interleaved)
