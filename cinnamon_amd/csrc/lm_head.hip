@@ -69,14 +69,29 @@ enum Epi {
   kFinal   // times a device scalar, in x's type
 };
 
+// Slabs of dx: K is split for the rows that count, which only the device knows, where their tiles are
+// fewer than the CUs; in parts of 8 steps at least, and in the memory that was given.
+struct Slabs {
+  int tile_m, tiles_n;  // rows of a tile, tiles of a row
+  int most, parts;      // workgroups, parts of K
+  int64_t room;         // rows of all slabs
+  __device__ int count(int64_t n) const {
+    if (n == 0) return 1;
+    int64_t s = most / (cdiv(n, tile_m) * tiles_n);
+    if (s > room / n) s = room / n;
+    if (s > parts) s = parts;
+    return s < 1 ? 1 : (int)s;
+  }
+};
+
 struct GemmArgs {
   const void *A, *B;
   int64_t lda, ldb;
   int64_t plane_a, plane_b;  // bytes between the planes of an fp32 operand
   int64_t M, N, K;     // N: columns to compute; K: a multiple of a K step where an operand holds K in its rows
   const int* n;        // rows there are, in place of M (or of K for kFinal)
-  int splits;          // parts of K, one slab each
-  int64_t ldc, slab;   // elements between rows of C, between slabs (or planes of dz)
+  const int* slabs;    // how many (kSlab)
+  int64_t ldc, slab;   // elements between rows of C, between planes of dz
   void* C;
   int add;
   int64_t v0, V;       // first column of the piece and columns of the vocabulary
@@ -192,15 +207,19 @@ __global__ __launch_bounds__(C::kThreads, 2) void k_ce_gemm(GemmArgs g) {
   const int64_t rows = __builtin_amdgcn_readfirstlane(*g.n);
   const int64_t M = EPI == kFinal ? g.M : rows, Kall = EPI == kFinal ? rows : g.K;
   const uint32_t tiles_m = (uint32_t)cdiv(M, C::TM), tiles_n = (uint32_t)cdiv(g.N, C::TN);
-  const uint32_t total = tiles_m * tiles_n;
+  const uint32_t tiles = tiles_m * tiles_n, total = EPI == kSlab ? tiles * *g.slabs : tiles;
   if (blockIdx.x >= total) return;
-  uint32_t tm, tn;
-  raster<4>(xcd_remap(blockIdx.x, total), tiles_m, tiles_n, tm, tn);
+  uint32_t tm, tn, tile = xcd_remap(blockIdx.x, total), part = 0;
+  if constexpr (EPI == kSlab) {  // the tiles of a part of K side by side, which share its rows of w
+    part = tile / tiles;
+    tile -= part * tiles;
+  }
+  raster<4>(tile, tiles_m, tiles_n, tm, tn);
   const int64_t m0 = (int64_t)tm * C::TM, n0 = (int64_t)tn * C::TN;
   int64_t k0 = 0, k1 = Kall;
   if constexpr (EPI == kSlab) {
-    const int64_t per = cdiv(cdiv(Kall, BK), g.splits) * BK;
-    k0 = blockIdx.y * per;
+    const int64_t per = cdiv(cdiv(Kall, BK), *g.slabs) * BK;
+    k0 = part * per;
     k1 = k0 + per < Kall ? k0 + per : Kall;
   }
   const int tid = threadIdx.x, lane = tid & 63;
@@ -331,7 +350,7 @@ __global__ __launch_bounds__(C::kThreads, 2) void k_ce_gemm(GemmArgs g) {
     return;
   }
   if constexpr (EPI == kSlab) {
-    float* out = static_cast<float*>(g.C) + blockIdx.y * g.slab;
+    float* out = static_cast<float*>(g.C) + part * rows * g.ldc;
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       const int64_t m = m0 + (wm * MT + i) * 16 + l16;
@@ -530,14 +549,14 @@ __global__ __launch_bounds__(1024) void k_ce_rows(const int64_t* __restrict__ y,
 
 // Rows of x (all, or map's first *n) with zeros up to Dp columns; fp32 rows as three bf16 planes.
 template <bool F32>
-__device__ __forceinline__ void copy_piece(const void* __restrict__ x, int64_t ldx, int64_t D, bool whole, int64_t row, int64_t i,
+__device__ __forceinline__ void copy_piece(const void* __restrict__ x, int64_t ldx, int64_t D, int64_t row, int64_t i,
                                            int64_t c, uint16_t* __restrict__ out, int64_t Dp, int64_t plane) {
   using E = std::conditional_t<F32, float, uint16_t>;
   const E* s = static_cast<const E*>(x) + row * ldx + c;
   uint16_t* d = out + i * Dp + c;
   E v[8];
-  if (whole && c + 8 <= D) {
-    __builtin_memcpy(v, __builtin_assume_aligned(s, 16), sizeof(v));
+  if (c + 8 <= D) {
+    __builtin_memcpy(v, s, sizeof(v));  // (16 bytes at a time from any element's address)
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = c + e < D ? s[e] : (E)0;
@@ -559,19 +578,13 @@ __device__ __forceinline__ void copy_piece(const void* __restrict__ x, int64_t l
   }
 }
 template <bool F32>
-__device__ __forceinline__ bool whole_rows(const void* x, int64_t ldx) {
-  return ((uintptr_t)x & 15) == 0 && ldx % (F32 ? 4 : 8) == 0;
-}
-
-template <bool F32>
 __global__ __launch_bounds__(256) void k_ce_copy(const void* __restrict__ x, int64_t ldx, int64_t rows, int64_t D,
                                                  const int* __restrict__ map, const int* __restrict__ n,
                                                  uint16_t* __restrict__ out, int64_t Dp, int64_t plane) {
   const int64_t pieces = Dp / 8, have = n ? *n : rows;
-  const bool whole = whole_rows<F32>(x, ldx);
   for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < have * pieces; q += (int64_t)gridDim.x * 256) {
     const int64_t i = q / pieces;
-    copy_piece<F32>(x, ldx, D, whole, map ? (int64_t)map[i] : i, i, (q - i * pieces) * 8, out, Dp, plane);
+    copy_piece<F32>(x, ldx, D, map ? (int64_t)map[i] : i, i, (q - i * pieces) * 8, out, Dp, plane);
   }
 }
 
@@ -585,10 +598,9 @@ __global__ __launch_bounds__(256) void k_ce_rows_copy(const int64_t* __restrict_
   __shared__ int map[kFewRows];
   const int n = find_rows<256>(y, T, V, ignore, st, rowloss, blockIdx.x == 0, map);
   const uint32_t pieces = (uint32_t)(Dp / 8), total = n * pieces;  // (at most 2^11 x 2^15)
-  const bool whole = whole_rows<F32>(x, ldx);
   for (uint32_t q = blockIdx.x * 256 + threadIdx.x; q < total; q += gridDim.x * 256) {
     const uint32_t i = q / pieces;
-    copy_piece<F32>(x, ldx, D, whole, map[i], i, (q - i * pieces) * 8, out, Dp, T * Dp);
+    copy_piece<F32>(x, ldx, D, map[i], i, (q - i * pieces) * 8, out, Dp, T * Dp);
   }
 }
 
@@ -660,11 +672,11 @@ __global__ __launch_bounds__(1024) void k_ce_loss(const float* __restrict__ rowl
 
 // What dz is scaled by: coef[i] = g_i 2^a with all products in range (fp16 holds 2^-24 .. 65504,
 // and p - 1 lies in [-1, 1]: top 2^15), and out_scale = 2^-a times what all rows share.  A gradient
-// shared by all rows (stride 0) stays out of coef.  One workgroup.
+// shared by all rows (stride 0) stays out of coef.  And dx's slabs.  One workgroup.
 __global__ __launch_bounds__(1024) void k_ce_coef(const float* __restrict__ grad, int64_t stride, int mean, int half,
                                                   const int* __restrict__ n, const int* __restrict__ map,
                                                   const int* __restrict__ target, float* __restrict__ coef,
-                                                  float* __restrict__ out_scale) {
+                                                  float* __restrict__ out_scale, Slabs slabs, int* __restrict__ slab_count) {
   __shared__ float wmax[16];
   const int rows = *n;
   const float top = half ? 32768.0f : 1.0f;
@@ -691,16 +703,20 @@ __global__ __launch_bounds__(1024) void k_ce_coef(const float* __restrict__ grad
     const float g = stride == 0 ? s : grad[(int64_t)map[i] * stride] * s;
     coef[i] = target[i] < 0 ? __builtin_nanf("") : g;
   }
-  if (threadIdx.x == 0) *out_scale = rows ? out : 0.0f;
+  if (threadIdx.x == 0) {
+    *out_scale = rows ? out : 0.0f;
+    *slab_count = slabs.count(rows);
+  }
 }
 
 // dx[t] = out_scale * the sum of the slabs' row pos[t], zero for an ignored row.
 template <int DT>
-__global__ __launch_bounds__(256) void k_ce_dx(const float* __restrict__ slabs, int64_t slab, int splits, int64_t Dp,
+__global__ __launch_bounds__(256) void k_ce_dx(const float* __restrict__ slabs, const int* __restrict__ count, const int* __restrict__ n, int64_t Dp,
                                                const int* __restrict__ pos, const float* __restrict__ out_scale,
                                                int64_t T, int64_t D, void* __restrict__ dx) {
   const float scale = *out_scale;
-  const int64_t pieces = Dp / 4;
+  const int splits = *count;
+  const int64_t slab = *n * Dp, pieces = Dp / 4;
   const bool whole = D % 4 == 0;
   for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < T * pieces; q += (int64_t)gridDim.x * 256) {
     const int64_t t = q / pieces, c = (q - t * pieces) * 4;
@@ -791,7 +807,8 @@ struct Plan {
   int tile;             // of the forward product
   int64_t tiles_n;      // its column tiles
   int64_t piece, ldz;   // columns of a piece, elements between rows of dz
-  int splits, slab_tile;  // slabs of dx, the tile of its product
+  int splits, slab_tile;  // slabs of dx if all rows count, the tile of its product
+  Slabs split;
   // bytes
   int64_t part, ztarget, dz, slabs, coef;
 };
@@ -823,11 +840,14 @@ Plan make_plan(int dtype, int64_t T, int64_t D, int64_t V) {
       p.slab_tile = t;
     }
   }
+  const int64_t slab_n = cdiv(p.Dp, kTileN[p.slab_tile]), workgroups = cdiv(Tp, kTileM[p.slab_tile]) * slab_n * p.splits;
+  p.split = Slabs{kTileM[p.slab_tile], (int)slab_n, (int)(workgroups < cin_device_cus() ? workgroups : cin_device_cus()),
+                  (int)(steps / 8), Tp * p.splits};
   p.part = align_up(Tp * p.tiles_n * 8, 256);
   p.ztarget = align_up(Tp * 4, 256);
   p.dz = align_up(p.planes * Tp * p.ldz * kEs, 256);
   p.slabs = align_up(p.splits * Tp * p.Dp * 4, 256);
-  p.coef = align_up((Tp + 1) * 4, 256);
+  p.coef = align_up((Tp + 2) * 4, 256);
   return p;
 }
 
@@ -864,12 +884,12 @@ void with_dtype(int dtype, F f) {
 }
 
 template <int EPI>
-void gemm(int dtype, int tile, const GemmArgs& g, int64_t max_m, hipStream_t s) {
+void gemm(int dtype, int tile, const GemmArgs& g, int64_t max_m, int splits, hipStream_t s) {
   with_tile(tile, [&](auto c) {
     using C = decltype(c);
     with_dtype(dtype, [&](auto dt) {
-      const int64_t tiles = cdiv(max_m, C::TM) * cdiv(g.N, C::TN);
-      hipLaunchKernelGGL((k_ce_gemm<C, dt(), EPI>), dim3((unsigned)tiles, (unsigned)g.splits), C::kThreads, 0, s, g);
+      const int64_t tiles = cdiv(max_m, C::TM) * cdiv(g.N, C::TN) * splits;
+      hipLaunchKernelGGL((k_ce_gemm<C, dt(), EPI>), (unsigned)tiles, C::kThreads, 0, s, g);
     });
   });
 }
@@ -939,11 +959,10 @@ int cin_linear_ce_forward(const void* x, int dtype, int64_t T, int64_t D, int64_
     g.N = g.V = V;
     g.K = p.Dp;
     g.n = st.n;
-    g.splits = 1;
     g.part = part;
     g.ztarget = zt;
     g.target = st.target;
-    gemm<kStats>(dtype, p.tile, g, T, s);
+    gemm<kStats>(dtype, p.tile, g, T, 1, s);
   }
   // (without rows one workgroup: the sum of none)
   hipLaunchKernelGGL(k_ce_join, (unsigned)(T > 0 ? cdiv(T, 4) : 1), 256, 0, s, part, (int)p.tiles_n, T, st, zt, state_f,
@@ -971,9 +990,10 @@ int cin_linear_ce_backward(const void* xc, int dtype, int64_t T, int64_t D, cons
   void* dz = ws;
   float* slabs = reinterpret_cast<float*>(ws + p.dz);
   float* out_scale = reinterpret_cast<float*>(ws + p.dz + p.slabs);
-  float* coef = out_scale + 1;
+  int* slab_count = reinterpret_cast<int*>(out_scale + 1);
+  float* coef = out_scale + 2;
   hipLaunchKernelGGL(k_ce_coef, 1, 1024, 0, s, grad, grad_stride, mean, dtype == CIN_DT_F16, st.n, st.map, st.target, coef,
-                     out_scale);
+                     out_scale, p.split, slab_count);
   const char* wb = static_cast<const char*>(w);
   for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
     const int64_t cols = v0 + p.piece < V ? p.piece : V - v0;
@@ -987,7 +1007,6 @@ int cin_linear_ce_backward(const void* xc, int dtype, int64_t T, int64_t D, cons
     g.N = align_up(cols, BK);  // with the zeros that fill the next product's last K step
     g.K = p.Dp;
     g.n = st.n;
-    g.splits = 1;
     g.C = dz;
     g.ldc = p.ldz;
     g.slab = T * p.ldz;
@@ -997,7 +1016,7 @@ int cin_linear_ce_backward(const void* xc, int dtype, int64_t T, int64_t D, cons
     g.rowmax = state_f;
     g.inv = state_f + T;
     g.coef = coef;
-    gemm<kGrad>(dtype, pick_tile(T, g.N), g, T, s);
+    gemm<kGrad>(dtype, pick_tile(T, g.N), g, T, 1, s);
     GemmArgs h{};
     h.n = st.n;
     h.A = dz;
@@ -1013,12 +1032,11 @@ int cin_linear_ce_backward(const void* xc, int dtype, int64_t T, int64_t D, cons
       h.plane_b = g.plane_b;
       h.N = p.Dp;
       h.K = g.N;
-      h.splits = p.splits;
+      h.slabs = slab_count;
       h.C = slabs;
       h.ldc = p.Dp;
-      h.slab = T * p.Dp;
       h.add = v0 > 0;
-      gemm<kSlab>(dtype, p.slab_tile, h, T, s);
+      gemm<kSlab>(dtype, p.slab_tile, h, T, p.splits, s);
     }
     if (dw) {
       h.B = xc;
@@ -1026,17 +1044,16 @@ int cin_linear_ce_backward(const void* xc, int dtype, int64_t T, int64_t D, cons
       h.plane_b = g.plane_a;
       h.M = cols;
       h.N = D;
-      h.splits = 1;
       h.C = static_cast<char*>(dw) + v0 * D * (dtype == CIN_DT_F32 ? 4 : 2);
       h.ldc = D;
       h.out_scale = out_scale;
-      gemm<kFinal>(dtype, pick_tile(cols, D), h, cols, s);
+      gemm<kFinal>(dtype, pick_tile(cols, D), h, cols, 1, s);
     }
   }
   if (dx) {
     const int64_t blocks = cdiv(T * (p.Dp / 4), 256);
     with_dtype(dtype, [&](auto dt) {
-      hipLaunchKernelGGL(k_ce_dx<dt()>, (unsigned)(blocks < 16384 ? blocks : 16384), 256, 0, s, slabs, T * p.Dp, p.splits,
+      hipLaunchKernelGGL(k_ce_dx<dt()>, (unsigned)(blocks < 16384 ? blocks : 16384), 256, 0, s, slabs, slab_count, st.n,
                          p.Dp, st.pos, out_scale, T, D, dx);
     });
   }
