@@ -410,7 +410,6 @@ __global__ __launch_bounds__(C::kThreads, 2) void k_ce_gemm(GemmArgs g) {
   const int64_t N = g.N;
   if constexpr (DT == CIN_DT_F32 && EPI == kFinal) {
     float* out = static_cast<float*>(g.C);
-    const bool whole = (g.ldc & 3) == 0 && ((uintptr_t)out & 15) == 0;
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       const int64_t m = m0 + (wm * MT + i) * 16 + l16;
@@ -418,8 +417,8 @@ __global__ __launch_bounds__(C::kThreads, 2) void k_ce_gemm(GemmArgs g) {
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
         const int64_t n = nl + j * 16;
-        if (whole && n + 4 <= N) {
-          *reinterpret_cast<float4*>(out + m * g.ldc + n) = make_float4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
+        if (n + 4 <= N) {
+          __builtin_memcpy(out + m * g.ldc + n, &acc[i][j], 16);
         } else {
 #pragma unroll
           for (int r = 0; r < 4; ++r)
@@ -432,7 +431,6 @@ __global__ __launch_bounds__(C::kThreads, 2) void k_ce_gemm(GemmArgs g) {
   // 16-bit rows through LDS, so that the stores run along them; for fp32 one plane after the other
   constexpr int kHalf = DT == CIN_DT_F16 ? CIN_DT_F16 : CIN_DT_BF16;
   constexpr int kChunks = C::TN / 8;
-  const bool whole = (g.ldc & 7) == 0 && ((uintptr_t)g.C & 15) == 0;
 #pragma unroll 1
   for (int plane = 0; plane < (DT == CIN_DT_F32 ? 3 : 1); ++plane) {
     uint16_t* out = static_cast<uint16_t*>(g.C) + plane * g.slab;
@@ -462,8 +460,8 @@ __global__ __launch_bounds__(C::kThreads, 2) void k_ce_gemm(GemmArgs g) {
         if (mp + m >= M || n0 + n >= N) continue;
         const v4u v = *reinterpret_cast<const v4u*>(smem + m * C::kCStride + n * 2);
         uint16_t* d = out + (mp + m) * g.ldc + n0 + n;
-        if (whole && n0 + n + 8 <= N) {
-          *reinterpret_cast<v4u*>(d) = v;
+        if (n0 + n + 8 <= N) {
+          __builtin_memcpy(d, &v, 16);  // (from any element's address)
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
@@ -717,7 +715,6 @@ __global__ __launch_bounds__(256) void k_ce_dx(const float* __restrict__ slabs, 
   const float scale = *out_scale;
   const int splits = *count;
   const int64_t slab = *n * Dp, pieces = Dp / 4;
-  const bool whole = D % 4 == 0;
   for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < T * pieces; q += (int64_t)gridDim.x * 256) {
     const int64_t t = q / pieces, c = (q - t * pieces) * 4;
     if (c >= D) continue;
@@ -733,16 +730,16 @@ __global__ __launch_bounds__(256) void k_ce_dx(const float* __restrict__ slabs, 
     const int64_t at = t * D + c;
     if constexpr (DT == CIN_DT_F32) {
       float* d = static_cast<float*>(dx) + at;
-      if (whole)
-        *reinterpret_cast<float4*>(d) = make_float4(v[0], v[1], v[2], v[3]);
+      if (c + 4 <= D)
+        __builtin_memcpy(d, v, 16);
       else
         for (int e = 0; e < 4; ++e)
           if (c + e < D) d[e] = v[e];
     } else {
       uint16_t* d = static_cast<uint16_t*>(dx) + at;
       const uint2 h = make_uint2(f32x2_to_half2_bits<DT>(v[0], v[1]), f32x2_to_half2_bits<DT>(v[2], v[3]));
-      if (whole)
-        *reinterpret_cast<uint2*>(d) = h;
+      if (c + 4 <= D)
+        __builtin_memcpy(d, &h, 8);
       else
         for (int e = 0; e < 4; ++e)
           if (c + e < D) d[e] = (uint16_t)((e < 2 ? h.x : h.y) >> (16 * (e & 1)));
