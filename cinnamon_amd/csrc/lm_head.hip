@@ -91,6 +91,7 @@ struct GemmArgs {
   int64_t M, N, K;     // N: columns to compute; K: a multiple of a K step where an operand holds K in its rows
   const int* n;        // rows there are, in place of M (or of K for kFinal)
   const int* slabs;    // how many (kSlab)
+  int segs;            // planes of a 16-bit B (kFinal)
   int64_t ldc, slab;   // elements between rows of C, between planes of dz
   void* C;
   int add;
@@ -249,6 +250,8 @@ __global__ __launch_bounds__(C::kThreads, 2) void k_ce_gemm(GemmArgs g) {
       planes_of(seg, ia, ib);
       pa = ia * g.plane_a;
       pb = ib * g.plane_b;
+    } else if constexpr (EPI == kFinal) {
+      pb = (g.segs - 1 - seg) * g.plane_b;  // the low parts first
     }
     oa.fetch(fk, pa, stage);
     ob.fetch(fk, pb, stage);
@@ -257,7 +260,7 @@ __global__ __launch_bounds__(C::kThreads, 2) void k_ce_gemm(GemmArgs g) {
       ++seg;
     }
   };
-  const int steps = nk * kSegs;
+  const int steps = nk * (EPI == kFinal && kSegs == 1 ? g.segs : kSegs);
   constexpr int kStages = C::kStages;
   constexpr int kOps = decltype(oa)::kOps + decltype(ob)::kOps;
 #pragma unroll
@@ -630,7 +633,8 @@ __device__ __forceinline__ void add_losses(const float* rowloss, int64_t T, int 
 // with the launch, 107 without).
 __global__ __launch_bounds__(256) void k_ce_join(const float2* __restrict__ part, int tiles, int64_t T, IntState st,
                                                  const float* __restrict__ ztarget, float* __restrict__ rowmax,
-                                                 float* __restrict__ inv, float* __restrict__ rowloss, int mean,
+                                                 float* __restrict__ inv, float* __restrict__ rest,
+                                                 float* __restrict__ rowloss, int mean,
                                                  float* __restrict__ loss) {
   const int lane = threadIdx.x & 63, n = *st.n;
   const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -646,9 +650,11 @@ __global__ __launch_bounds__(256) void k_ce_join(const float2* __restrict__ part
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) s += __shfl_xor(s, o);
     if (lane == 0) {
+      const float loss_i = st.target[i] < 0 ? __builtin_nanf("") : (m - ztarget[i]) + logf(s);
       rowmax[i] = m;
       inv[i] = 1.0f / s;
-      rowloss[st.map[i]] = st.target[i] < 0 ? __builtin_nanf("") : (m - ztarget[i]) + logf(s);
+      rest[i] = -expm1f(-loss_i);
+      rowloss[st.map[i]] = loss_i;
     }
   }
   if (!loss) return;
@@ -670,50 +676,126 @@ __global__ __launch_bounds__(1024) void k_ce_loss(const float* __restrict__ rowl
 
 // What dz is scaled by: coef[i] = g_i 2^a with all products in range (fp16 holds 2^-24 .. 65504,
 // and p - 1 lies in [-1, 1]: top 2^15), and out_scale = 2^-a times what all rows share.  A gradient
-// shared by all rows (stride 0) stays out of coef.  And dx's slabs.  One workgroup.
+// shared by all rows (stride 0) stays out of coef.
+struct Coef {
+  float s, out;
+};
+// By the whole workgroup.
+template <int THREADS>
+__device__ inline Coef coef_of(const float* __restrict__ grad, int64_t stride, int mean, float top, int rows,
+                               const int* __restrict__ map) {
+  __shared__ float wmax[THREADS / 64];
+  Coef c{top, 1.0f / top};
+  if (stride == 0) {
+    c.out *= mean ? grad[0] / (float)rows : grad[0];
+    return c;
+  }
+  float m = 0.0f;
+  for (int i = threadIdx.x; i < rows; i += THREADS) m = fmaxf(m, fabsf(grad[(int64_t)map[i] * stride]));
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+  if ((threadIdx.x & 63) == 0) wmax[threadIdx.x >> 6] = m;
+  __syncthreads();
+  for (int w = 0; w < THREADS / 64; ++w) m = fmaxf(m, wmax[w]);
+  if (m > 0.0f && m < __builtin_inff()) {
+    int e;
+    frexpf(m, &e);  // m <= 2^e
+    e = e < -100 ? -100 : (e > 100 ? 100 : e);
+    c.s = ldexpf(top, -e);
+    c.out = ldexpf(1.0f / top, e);
+  }
+  return c;
+}
+
+// Where the backward leaves what its products are scaled by.
+struct Scales {
+  float *out, *coef, *row;  // row: for few rows, null for many
+  int* slabs;
+};
+
+// And dx's slabs.  One workgroup.
 __global__ __launch_bounds__(1024) void k_ce_coef(const float* __restrict__ grad, int64_t stride, int mean, int half,
                                                   const int* __restrict__ n, const int* __restrict__ map,
-                                                  const int* __restrict__ target, float* __restrict__ coef,
-                                                  float* __restrict__ out_scale, Slabs slabs, int* __restrict__ slab_count) {
-  __shared__ float wmax[16];
+                                                  const int* __restrict__ target, Scales to, Slabs slabs) {
   const int rows = *n;
-  const float top = half ? 32768.0f : 1.0f;
-  float s = top, out = 1.0f / top;
-  if (stride == 0) {
-    out *= mean ? grad[0] / (float)rows : grad[0];
-  } else {
-    float m = 0.0f;
-    for (int i = threadIdx.x; i < rows; i += 1024) m = fmaxf(m, fabsf(grad[(int64_t)map[i] * stride]));
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
-    if ((threadIdx.x & 63) == 0) wmax[threadIdx.x >> 6] = m;
-    __syncthreads();
-    for (int w = 0; w < 16; ++w) m = fmaxf(m, wmax[w]);
-    if (m > 0.0f && m < __builtin_inff()) {
-      int e;
-      frexpf(m, &e);  // m <= 2^e
-      e = e < -100 ? -100 : (e > 100 ? 100 : e);
-      s = ldexpf(top, -e);
-      out = ldexpf(1.0f / top, e);
-    }
-  }
+  const Coef c = coef_of<1024>(grad, stride, mean, half ? 32768.0f : 1.0f, rows, map);
   for (int i = threadIdx.x; i < rows; i += 1024) {
-    const float g = stride == 0 ? s : grad[(int64_t)map[i] * stride] * s;
-    coef[i] = target[i] < 0 ? __builtin_nanf("") : g;
+    const float g = stride == 0 ? c.s : grad[(int64_t)map[i] * stride] * c.s;
+    to.coef[i] = target[i] < 0 ? __builtin_nanf("") : g;
   }
   if (threadIdx.x == 0) {
-    *out_scale = rows ? out : 0.0f;
-    *slab_count = slabs.count(rows);
+    *to.out = rows ? c.out : 0.0f;
+    *to.slabs = slabs.count(rows);
   }
 }
 
-// dx[t] = out_scale * the sum of the slabs' row pos[t], zero for an ignored row.
+// The same for few rows.  A row's largest entry of dz is its target's, g (p - 1), and with few rows the
+// rounding of those few numbers does not average out of dx and dw.  So dz is divided by 1 - p, which
+// makes that entry a power of two, and c = g (1 - p) = 2^e m, m in [1/2, 1), is brought in by other ways:
+// 2^e with dz, m in fp32 with dx's sums and, for dw, with x, held as two 16-bit parts.  The gradients are
+// then as near as their own rounding allows (relative error of 16 x 32000 x 1024, bf16, a gradient for
+// each row: 1.65e-3, without it 2.5e-3).  dw takes twice the products: of x 32000 x 1024 backward 59 -> 63
+// us with 64 rows, 72 -> 82 with 128, 104 -> 121 with 256, and 140 -> 174 with 512, too many for it.
+constexpr int kFewExact = 256;
 template <int DT>
-__global__ __launch_bounds__(256) void k_ce_dx(const float* __restrict__ slabs, const int* __restrict__ count, const int* __restrict__ n, int64_t Dp,
-                                               const int* __restrict__ pos, const float* __restrict__ out_scale,
+__global__ __launch_bounds__(256) void k_ce_coef_few(const float* __restrict__ grad, int64_t stride, int mean,
+                                                     const int* __restrict__ n, const int* __restrict__ map,
+                                                     const int* __restrict__ target, const float* __restrict__ rest,
+                                                     Scales to, Slabs slabs, const uint16_t* __restrict__ x, int64_t Dp,
+                                                     uint16_t* __restrict__ scaled, int64_t plane) {
+  constexpr float top = DT == CIN_DT_F16 ? 32768.0f : 1.0f;
+  constexpr int kLeast = DT == CIN_DT_F16 ? -24 : -60;  // of e: dz's powers of two stay in its type
+  const int rows = *n;
+  const Coef c = coef_of<256>(grad, stride, mean, top, rows, map);
+  // m and e of row i; r: its 1 - p, kept from 0 (the row's other entries are then at most 1 too)
+  const auto row = [&](int i, int& e, float& r) {
+    r = fmaxf(rest[i], 5.9604644775390625e-8f);
+    const float v = (stride == 0 ? 1.0f : grad[(int64_t)map[i] * stride] * (c.s / top)) * r;
+    e = 0;
+    if (!(fabsf(v) < 1.0f)) return v;  // (1, NaN or infinite)
+    frexpf(v, &e);
+    e = v == 0.0f ? 0 : (e < kLeast ? kLeast : (e > 0 ? 0 : e));
+    return ldexpf(v, -e);
+  };
+  if (blockIdx.x == 0) {
+    for (int i = threadIdx.x; i < rows; i += 256) {
+      int e;
+      float r;
+      to.row[i] = row(i, e, r);
+      to.coef[i] = target[i] < 0 ? __builtin_nanf("") : ldexpf(top, e) / r;
+    }
+    if (threadIdx.x == 0) {
+      *to.out = rows ? c.out : 0.0f;
+      *to.slabs = slabs.count(rows);
+    }
+  }
+  const uint32_t pieces = (uint32_t)(Dp / 8), total = rows * pieces;  // (at most 2^8 x 2^15)
+  for (uint32_t q = blockIdx.x * 256 + threadIdx.x; q < total; q += gridDim.x * 256) {
+    const uint32_t i = q / pieces;
+    int e;
+    float r;
+    const float m = row((int)i, e, r);
+    const int64_t at = i * Dp + (q - i * pieces) * 8;
+    const v4u v = *reinterpret_cast<const v4u*>(x + at);
+    v4u hi, lo;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float a = half_bits_to_f32(DT, (uint16_t)v[k]) * m, b = half_bits_to_f32(DT, (uint16_t)(v[k] >> 16)) * m;
+      hi[k] = f32x2_to_half2_bits<DT>(a, b);
+      lo[k] = f32x2_to_half2_bits<DT>(a - half_bits_to_f32(DT, (uint16_t)hi[k]), b - half_bits_to_f32(DT, (uint16_t)(hi[k] >> 16)));
+    }
+    *reinterpret_cast<v4u*>(scaled + at) = hi;
+    *reinterpret_cast<v4u*>(scaled + plane + at) = lo;
+  }
+}
+
+// dx[t] = out_scale (row[pos[t]]) times the sum of the slabs' row pos[t], zero for an ignored row.
+template <int DT>
+__global__ __launch_bounds__(256) void k_ce_dx(const float* __restrict__ slabs, Scales by, const int* __restrict__ n, int64_t Dp,
+                                               const int* __restrict__ pos,
                                                int64_t T, int64_t D, void* __restrict__ dx) {
-  const float scale = *out_scale;
-  const int splits = *count;
+  const float shared = *by.out;
+  const int splits = *by.slabs;
   const int64_t slab = *n * Dp, pieces = Dp / 4;
   for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < T * pieces; q += (int64_t)gridDim.x * 256) {
     const int64_t t = q / pieces, c = (q - t * pieces) * 4;
@@ -726,6 +808,7 @@ __global__ __launch_bounds__(256) void k_ce_dx(const float* __restrict__ slabs, 
         a = make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
       }
     }
+    const float scale = by.row && i >= 0 ? shared * by.row[i] : shared;
     const float v[4] = {a.x * scale, a.y * scale, a.z * scale, a.w * scale};
     const int64_t at = t * D + c;
     if constexpr (DT == CIN_DT_F32) {
@@ -807,7 +890,8 @@ struct Plan {
   int splits, slab_tile;  // slabs of dx if all rows count, the tile of its product
   Slabs split;
   // bytes
-  int64_t part, ztarget, dz, slabs, coef;
+  int64_t part, ztarget, dz, slabs, scaled, coef;
+  bool few;  // rows: k_ce_coef_few
 };
 
 Plan make_plan(int dtype, int64_t T, int64_t D, int64_t V) {
@@ -844,7 +928,9 @@ Plan make_plan(int dtype, int64_t T, int64_t D, int64_t V) {
   p.ztarget = align_up(Tp * 4, 256);
   p.dz = align_up(p.planes * Tp * p.ldz * kEs, 256);
   p.slabs = align_up(p.splits * Tp * p.Dp * 4, 256);
-  p.coef = align_up((Tp + 2) * 4, 256);
+  p.few = p.planes == 1 && Tp <= kFewExact;
+  p.scaled = p.few ? align_up(2 * Tp * p.Dp * kEs, 256) : 0;
+  p.coef = align_up((2 * Tp + 2) * 4, 256);
   return p;
 }
 
@@ -909,7 +995,7 @@ extern "C" {
 int64_t cin_linear_ce_workspace(int dtype, int64_t T, int64_t D, int64_t V, int backward) {
   Plan p;
   if (check("linear_ce_workspace", dtype, T, D, V, p)) return -1;
-  return backward ? p.dz + p.slabs + p.coef : p.part + p.ztarget;
+  return backward ? p.dz + p.slabs + p.scaled + p.coef : p.part + p.ztarget;
 }
 
 int cin_linear_ce_forward(const void* x, int dtype, int64_t T, int64_t D, int64_t ldx, const void* w, int64_t V,
@@ -963,7 +1049,7 @@ int cin_linear_ce_forward(const void* x, int dtype, int64_t T, int64_t D, int64_
   }
   // (without rows one workgroup: the sum of none)
   hipLaunchKernelGGL(k_ce_join, (unsigned)(T > 0 ? cdiv(T, 4) : 1), 256, 0, s, part, (int)p.tiles_n, T, st, zt, state_f,
-                     state_f + T, rowloss, mean, T <= kJoinAlone ? loss : nullptr);
+                     state_f + T, state_f + 2 * T, rowloss, mean, T <= kJoinAlone ? loss : nullptr);
   if (loss && T > kJoinAlone) hipLaunchKernelGGL(k_ce_loss, 1, 1024, 0, s, rowloss, T, st.n, mean, loss);
   return cin_check_launch(name);
 }
@@ -979,18 +1065,27 @@ int cin_linear_ce_backward(const void* xc, int dtype, int64_t T, int64_t D, cons
   CIN_CHECK_ARG(grad_stride >= 0, "%s: negative gradient stride", name);
   CIN_CHECK_ARG(T > 0 && state_i && state_f && xc && w && grad, "%s: null pointer", name);
   CIN_CHECK_ARG(aligned16(xc) && aligned16(dx) && aligned16(workspace), "%s: xc, dx and workspace must lie on 16 bytes", name);
-  CIN_CHECK_ARG(workspace && workspace_bytes >= p.dz + p.slabs + p.coef, "%s: workspace needs %lld bytes", name,
-                (long long)(p.dz + p.slabs + p.coef));
+  CIN_CHECK_ARG(workspace && workspace_bytes >= p.dz + p.slabs + p.scaled + p.coef, "%s: workspace needs %lld bytes", name,
+                (long long)(p.dz + p.slabs + p.scaled + p.coef));
   hipStream_t s = static_cast<hipStream_t>(stream);
   const IntState st(const_cast<int32_t*>(state_i), T);
   char* ws = static_cast<char*>(workspace);
   void* dz = ws;
   float* slabs = reinterpret_cast<float*>(ws + p.dz);
-  float* out_scale = reinterpret_cast<float*>(ws + p.dz + p.slabs);
-  int* slab_count = reinterpret_cast<int*>(out_scale + 1);
-  float* coef = out_scale + 2;
-  hipLaunchKernelGGL(k_ce_coef, 1, 1024, 0, s, grad, grad_stride, mean, dtype == CIN_DT_F16, st.n, st.map, st.target, coef,
-                     out_scale, p.split, slab_count);
+  uint16_t* scaled = reinterpret_cast<uint16_t*>(ws + p.dz + p.slabs);
+  float* f = reinterpret_cast<float*>(ws + p.dz + p.slabs + p.scaled);
+  const Scales by{f, f + 2, p.few ? f + 2 + T : nullptr, reinterpret_cast<int*>(f + 1)};
+  if (p.few) {
+    const unsigned grid = (unsigned)cdiv(T * (p.Dp / 8), 256);
+    with_dtype(dtype, [&](auto dt) {
+      if constexpr (dt() != CIN_DT_F32)
+        hipLaunchKernelGGL(k_ce_coef_few<dt()>, grid < 256 ? grid : 256, 256, 0, s, grad, grad_stride, mean, st.n, st.map,
+                           st.target, state_f + 2 * T, by, p.split, static_cast<const uint16_t*>(xc), p.Dp, scaled, T * p.Dp);
+    });
+  } else {
+    hipLaunchKernelGGL(k_ce_coef, 1, 1024, 0, s, grad, grad_stride, mean, dtype == CIN_DT_F16, st.n, st.map, st.target, by,
+                       p.split);
+  }
   const char* wb = static_cast<const char*>(w);
   for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
     const int64_t cols = v0 + p.piece < V ? p.piece : V - v0;
@@ -1012,7 +1107,7 @@ int cin_linear_ce_backward(const void* xc, int dtype, int64_t T, int64_t D, cons
     g.target = st.target;
     g.rowmax = state_f;
     g.inv = state_f + T;
-    g.coef = coef;
+    g.coef = by.coef;
     gemm<kGrad>(dtype, pick_tile(T, g.N), g, T, 1, s);
     GemmArgs h{};
     h.n = st.n;
@@ -1029,29 +1124,30 @@ int cin_linear_ce_backward(const void* xc, int dtype, int64_t T, int64_t D, cons
       h.plane_b = g.plane_b;
       h.N = p.Dp;
       h.K = g.N;
-      h.slabs = slab_count;
+      h.slabs = by.slabs;
       h.C = slabs;
       h.ldc = p.Dp;
       h.add = v0 > 0;
       gemm<kSlab>(dtype, p.slab_tile, h, T, p.splits, s);
     }
     if (dw) {
-      h.B = xc;
+      h.B = p.few ? scaled : xc;
+      h.segs = p.few ? 2 : 1;
       h.ldb = p.Dp;
       h.plane_b = g.plane_a;
       h.M = cols;
       h.N = D;
       h.C = static_cast<char*>(dw) + v0 * D * (dtype == CIN_DT_F32 ? 4 : 2);
       h.ldc = D;
-      h.out_scale = out_scale;
+      h.out_scale = by.out;
       gemm<kFinal>(dtype, pick_tile(cols, D), h, cols, 1, s);
     }
   }
   if (dx) {
     const int64_t blocks = cdiv(T * (p.Dp / 4), 256);
     with_dtype(dtype, [&](auto dt) {
-      hipLaunchKernelGGL(k_ce_dx<dt()>, (unsigned)(blocks < 16384 ? blocks : 16384), 256, 0, s, slabs, slab_count, st.n,
-                         p.Dp, st.pos, out_scale, T, D, dx);
+      hipLaunchKernelGGL(k_ce_dx<dt()>, (unsigned)(blocks < 16384 ? blocks : 16384), 256, 0, s, slabs, by, st.n,
+                         p.Dp, st.pos, T, D, dx);
     });
   }
   return cin_check_launch(name);

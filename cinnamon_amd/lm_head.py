@@ -32,7 +32,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     each row's loss (0 for an ignored one).  A target outside [0, V) gives NaN, in the gradients too.
 
     Differentiable in x and weight (once), gradients in their dtype.  Products are summed in fp32;
-    the gradient of the logits enters the two gradient products rounded to the inputs' dtype.
+    the gradient of the logits enters the two gradient products rounded to the inputs' dtype, for up
+    to 256 rows scaled so that the targets' entries are exact.
     fp32 inputs are multiplied as three bf16 parts each, to the accuracy of fp32 products.
     Results do not vary from call to call.  The backward recomputes the logits piece by piece:
     beside the inputs it keeps one copy of the rows that count (fp32: 1.5 times their size, and the
@@ -73,7 +74,7 @@ def _layout(T, D, V, dtype):
     planes = 3 if dtype == torch.float32 else 1
     copied = planes == 3 or Dp != D
     offsets, at = [], 0
-    for n in (planes * T * Dp * 2, planes * V * Dp * 2 if copied else 0, 4 * (4 + 3 * T), 8 * T):
+    for n in (planes * T * Dp * 2, planes * V * Dp * 2 if copied else 0, 4 * (4 + 3 * T), 12 * T):
         offsets.append(at)
         at += _cdiv(n, 256) * 256
     return offsets, at, copied

@@ -200,6 +200,38 @@ def test_strides_shapes_and_targets_types(dev, dt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 7, 256])
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+@pytest.mark.parametrize("reduction", ["none", "sum"])
+def test_few_rows_are_rounded_once(dev, T, dt, reduction):
+    """With few rows the targets' part of the gradients is as near as one rounding allows."""
+    V, D = 1000, 128
+    g = torch.Generator().manual_seed(T)
+    y = torch.randperm(V, generator=g)[:T].to(dev)
+    x = torch.randn(T, D, generator=g).to(DT[dt]).to(dev).requires_grad_()
+    w = torch.zeros(V, D)
+    w[y.cpu()] = torch.randn(T, D, generator=g) * 0.3
+    w = w.to(DT[dt]).to(dev).requires_grad_()
+    gr = torch.randn(T, generator=g).to(dev) if reduction == "none" else torch.tensor(0.7, device=dev)
+    loss = lm_head.linear_cross_entropy(x, w, y, reduction=reduction)
+    dx, dw = torch.autograd.grad(loss, (x, w), gr)
+    x64, w64 = x.detach().double(), w.detach().double()
+    p = (x64 @ w64.T).softmax(-1)
+    g64 = gr.double().expand(T)[:, None]
+    at = torch.nn.functional.one_hot(y, V).double()
+    dz, other = g64 * (p - at), (g64 * p).abs() * (1 - at)
+    # the other entries of dz are rounded (fp16: or lie under its steps below 2^-14, 2^-24 of the largest
+    # row's 2^-15), the sums are fp32: 1000 terms of 2^-24 of the products' absolute sum
+    half = torch.finfo(DT[dt]).eps / 2
+    tiny = 2 ** -38 * g64.abs().max()
+    for got, want, off, total in ((dx, dz @ w64, (other * half + tiny) @ w64.abs(), dz.abs() @ w64.abs()),
+                                  (dw, dz.T @ x64, (other * half + tiny).T @ x64.abs(), dz.abs().T @ x64.abs())):
+        # (2^-25: half of fp16's last step)
+        bound = want.abs() * half * 1.001 + off * 1.01 + total * 1000 * 2 ** -24 + 2 ** -25
+        assert ((got.double() - want).abs() <= bound).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("D", [64, 65])
 def test_a_single_row_whose_stride_is_not_its_width(dev, D):
     """One token, and a vocabulary of one: a transposed column's only row has a stride of 1."""
