@@ -17,7 +17,8 @@
 // the error bound (or is one of equal logits and biases, a true tie), that is the order.  Where the
 // chosen experts are sure and their order is not, they are sorted by their choices in 64 bits; else the
 // wave ranks the token again in 64 bits (256 experts with biases in 8 groups, top-8, random logits: the
-// order is in doubt in 1.3 tokens of a thousand, the choice in 0.2).  NaN counts as the greatest value, in a row and among groups.
+// order is in doubt in 1.3 tokens of a thousand, the choice in 0.2).  NaN counts as the greatest value,
+// in a row and among groups.
 //
 // A token's experts lie over LANES lanes, EPL consecutive ones a lane, so that the order of the
 // lanes is the order of the indices: the lowest of equal candidates is the first lane of a ballot.
@@ -109,12 +110,8 @@ __device__ inline float lanes_max_nan(float v) {
 }
 template <int LANES>
 __device__ inline uint64_t lanes_max(uint64_t v) {
-#pragma unroll
-  for (int o = 1; o < LANES; o <<= 1) {
-    const uint64_t u = __shfl_xor(v, o);
-    v = u > v ? u : v;
-  }
-  return v;
+  const uint32_t mine = (uint32_t)(v >> 32), hi = lanes_max<LANES>(mine);
+  return (uint64_t)hi << 32 | lanes_max<LANES>(mine == hi ? (uint32_t)v : 0u);
 }
 template <int LANES>
 __device__ inline double lanes_sum(double v) {
@@ -382,12 +379,8 @@ __device__ inline void rank64(const GateArgs& a, int64_t t, int lane, uint64_t* 
       best = v > best ? v : best;
     }
     const uint64_t top = lanes_max<64>(best);
-    int e = best == top ? at : a.E;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int u = __shfl_xor(e, o);
-      e = u < e ? u : e;
-    }
+    // (the lowest expert: the largest complement)
+    const int e = (int)~lanes_max<64>(~(uint32_t)(best == top ? at : a.E));
     if (lane == r) my_e = e;
     if (lane == 0) keys[e] = 0;
     wave_sync();
@@ -396,8 +389,9 @@ __device__ inline void rank64(const GateArgs& a, int64_t t, int lane, uint64_t* 
 }
 
 template <int LANES, int EPL, int WAVES, int DT>
-__global__ __launch_bounds__(64 * WAVES, EPL <= 16 ? 4 : 1) void k_gate_fwd(GateArgs a, int64_t* __restrict__ idx, float* __restrict__ w,
-                                                         float* __restrict__ all) {
+__global__ __launch_bounds__(64 * WAVES, EPL <= 16 ? 4 : 1) void k_gate_fwd(GateArgs a, int64_t* __restrict__ idx,
+                                                                               float* __restrict__ w,
+                                                                               float* __restrict__ all) {
   constexpr int kTokens = 64 / LANES * WAVES;
   __shared__ uint64_t keys64[WAVES][LANES * EPL];   // of the token a wave ranks in 64 bits
   __shared__ uint32_t keys32[kTokens][LANES * EPL];
