@@ -39,8 +39,13 @@ typedef short s4 __attribute__((ext_vector_type(4)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 
-constexpr int kEs = 2;  // bytes of an operand's element: bf16 or fp16
-constexpr int BK = 64;  // elements of a K step
+// What the products' operands hold: CIN_DT_BF16 or CIN_DT_F16; CIN_DT_F32 for three bf16 planes; kDirect
+// for fp32 as it is, for few rows.
+constexpr int kDirect = 3;
+template <int DT>
+constexpr int kEs = DT == kDirect ? 4 : 2;  // bytes of an operand's element
+constexpr int kStepBytes = 128;
+constexpr int kPadK = 64;  // operands that hold K in their rows have a multiple of it: whole K steps
 
 // s_waitcnt vmcnt(N): everything but the last N vector memory operations has completed
 template <int N>
@@ -107,11 +112,13 @@ struct GemmArgs {
 // Along K: LDS rows are tile rows of 128 bytes, 16-byte chunk c of row r at slot c ^ f(r).
 // Across K: LDS rows are the step's K rows of ROWS elements, in granules of 16 elements, granule
 // q of row r at q ^ f(r): the rows that one transposing read takes together lie on other banks.
-template <int ROWS, int THREADS, bool ACROSS>
+template <int ROWS, int THREADS, bool ACROSS, int ES>
 struct Operand {
+  static constexpr int BK = kStepBytes / ES;
   static constexpr int kOps = ROWS * 8 / THREADS;
-  static constexpr int kCpr = ACROSS ? ROWS * kEs / 16 : 8;  // 16-byte chunks of an LDS row
-  static constexpr int kGran = kCpr / 2;                     // granules of 16 elements (across)
+  static constexpr int kCpr = ACROSS ? ROWS * ES / 16 : 8;  // 16-byte chunks of an LDS row
+  static constexpr int kGc = ES;                            // of a granule of 16 elements (across)
+  static constexpr int kGran = kCpr / kGc;
   static_assert(ROWS * 8 % THREADS == 0, "whole operations");
   uint32_t voff[kOps];
   const uint8_t* p;
@@ -120,28 +127,29 @@ struct Operand {
 
   __device__ static inline int f(int r) {
     if constexpr (!ACROSS) return (r >> 1) & 7;  // (the 16 rows and two chunks of a pass on 64 banks: no conflicts)
+    if constexpr (ES == 4) return (r >> 2) & 3 & (kGran - 1);
     return ((r & 3) | ((r >> 3 & 1) << 2)) & (kGran - 1);
   }
   // r0: the tile's first row (along) or column (across); valid: rows (along) or columns (across)
   // from there on; k0, k1: the K range that there is
   __device__ __forceinline__ void init(const void* base, int64_t ld, int64_t r0, int64_t valid, int64_t k0, int64_t k1,
                                        int tid, uint32_t lds0) {
-    ldb = ld * kEs;
+    ldb = ld * ES;
     lds = lds0 + (uint32_t)__builtin_amdgcn_readfirstlane(tid >> 6) * 1024;
     kleft = k1 - k0;
     if constexpr (ACROSS) {
-      p = static_cast<const uint8_t*>(base) + k0 * ldb + r0 * kEs;
-      bytes = valid * kEs;  // of the last K row
+      p = static_cast<const uint8_t*>(base) + k0 * ldb + r0 * ES;
+      bytes = valid * ES;  // of the last K row
     } else {
       const int rows = (int)(valid < ROWS ? valid : ROWS);
-      p = static_cast<const uint8_t*>(base) + r0 * ldb + k0 * kEs;
-      bytes = (rows - 1) * ldb + kleft * kEs;
+      p = static_cast<const uint8_t*>(base) + r0 * ldb + k0 * ES;
+      bytes = (rows - 1) * ldb + kleft * ES;
     }
 #pragma unroll
     for (int i = 0; i < kOps; ++i) {
       const int slot = i * THREADS + tid, r = slot / kCpr, c = slot % kCpr;
       if constexpr (ACROSS) {
-        voff[i] = (uint32_t)(r * ldb) + (uint32_t)((((c / 2) ^ f(r)) * 2 + c % 2) * 16);
+        voff[i] = (uint32_t)(r * ldb) + (uint32_t)((((c / kGc) ^ f(r)) * kGc + c % kGc) * 16);
       } else {
         voff[i] = r < valid ? (uint32_t)(r * ldb) + (uint32_t)((c ^ f(r)) * 16) : kOut;
       }
@@ -157,15 +165,23 @@ struct Operand {
       rsrc = make_rsrc(p + plane + (int64_t)kt * BK * ldb, left > 0 ? ((left < BK ? left : BK) - 1) * ldb + bytes : 0);
     } else {
       rsrc = make_rsrc(p + plane, bytes);
-      so = (uint32_t)__builtin_amdgcn_readfirstlane(kt) * 128;
+      so = (uint32_t)__builtin_amdgcn_readfirstlane(kt) * kStepBytes;
     }
 #pragma unroll
     for (int i = 0; i < kOps; ++i) dma16(rsrc, voff[i], so, lds + stage + i * THREADS * 16);
   }
-  // 16 bytes a lane: K elements 8 kq .. + 7 of half ks of tile row r16 + l16
+  // 16 bytes a lane: K elements 8 kq .. + 7 of half ks (of 4 bytes: 4 kq .. + 3) of tile row r16 + l16
   __device__ static __forceinline__ v4u frag(const uint8_t* st, int r16, int ks, int l16, int kq) {
     if constexpr (!ACROSS) {
       return *reinterpret_cast<const v4u*>(st + (r16 + l16) * 128 + (((4 * ks + kq) ^ f(r16 + l16)) << 4));
+    } else if constexpr (ES == 4) {
+      v4u v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int k = 16 * ks + 4 * kq + e;
+        v[e] = *reinterpret_cast<const uint32_t*>(st + k * (ROWS * 4) + ((((r16 >> 4)) ^ f(k)) << 6) + l16 * 4);
+      }
+      return v;
     } else {
       v4u v;
 #pragma unroll
@@ -185,6 +201,12 @@ struct Operand {
 // c += a b over a half step: lane (l16, kq) holds column l16 of b and rows 4 kq .. + 3 of a
 template <int DT>
 __device__ __forceinline__ v4f mma(v4u a, v4u b, v4f c) {
+  if constexpr (DT == kDirect) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[e]), __uint_as_float(b[e]), c, 0, 0, 0);
+    return c;
+  } else
   if constexpr (DT == CIN_DT_F16)
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
   else
@@ -203,7 +225,7 @@ __device__ inline float exp_of(float d) { return __builtin_amdgcn_exp2f(d * kLog
 template <class C, int DT, int EPI>
 __global__ __launch_bounds__(C::kThreads, 2) void k_ce_gemm(GemmArgs g) {
   constexpr bool kAcrossA = EPI == kFinal, kAcrossB = EPI == kSlab || EPI == kFinal;
-  constexpr int MT = C::MT, NT = C::NT, kSegs = DT == CIN_DT_F32 ? kPairs32 : 1;
+  constexpr int MT = C::MT, NT = C::NT, kSegs = DT == CIN_DT_F32 ? kPairs32 : 1, BK = kStepBytes / kEs<DT>;
   __shared__ __attribute__((aligned(128))) uint8_t smem[C::kBytes];
   const int64_t rows = __builtin_amdgcn_readfirstlane(*g.n);
   const int64_t M = EPI == kFinal ? g.M : rows, Kall = EPI == kFinal ? rows : g.K;
@@ -228,8 +250,8 @@ __global__ __launch_bounds__(C::kThreads, 2) void k_ce_gemm(GemmArgs g) {
   const int wm = wave / C::WN, wn = wave % C::WN;
   const int l16 = lane & 15, kq = lane >> 4;
   const uint32_t lds0 = (uint32_t)(uintptr_t)smem;
-  Operand<C::TM, C::kThreads, kAcrossA> oa;
-  Operand<C::TN, C::kThreads, kAcrossB> ob;
+  Operand<C::TM, C::kThreads, kAcrossA, kEs<DT>> oa;
+  Operand<C::TN, C::kThreads, kAcrossB, kEs<DT>> ob;
   v4f acc[MT][NT];
 #pragma unroll
   for (int i = 0; i < MT; ++i)
@@ -411,7 +433,7 @@ __global__ __launch_bounds__(C::kThreads, 2) void k_ce_gemm(GemmArgs g) {
         for (int r = 0; r < 4; ++r) acc[i][j][r] *= scale;
   }
   const int64_t N = g.N;
-  if constexpr (DT == CIN_DT_F32 && EPI == kFinal) {
+  if constexpr ((DT == CIN_DT_F32 && EPI == kFinal) || DT == kDirect) {
     float* out = static_cast<float*>(g.C);
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
@@ -548,11 +570,11 @@ __global__ __launch_bounds__(1024) void k_ce_rows(const int64_t* __restrict__ y,
   find_rows<1024>(y, T, V, ignore, st, rowloss, true, nullptr);
 }
 
-// Rows of x (all, or map's first *n) with zeros up to Dp columns; fp32 rows as three bf16 planes.
-template <bool F32>
+// Rows of x (all, or map's first *n) with zeros up to Dp columns, as operands of DT.
+template <int DT>
 __device__ __forceinline__ void copy_piece(const void* __restrict__ x, int64_t ldx, int64_t D, int64_t row, int64_t i,
                                            int64_t c, uint16_t* __restrict__ out, int64_t Dp, int64_t plane) {
-  using E = std::conditional_t<F32, float, uint16_t>;
+  using E = std::conditional_t<DT == CIN_DT_F32 || DT == kDirect, float, uint16_t>;
   const E* s = static_cast<const E*>(x) + row * ldx + c;
   uint16_t* d = out + i * Dp + c;
   E v[8];
@@ -562,7 +584,9 @@ __device__ __forceinline__ void copy_piece(const void* __restrict__ x, int64_t l
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = c + e < D ? s[e] : (E)0;
   }
-  if constexpr (F32) {
+  if constexpr (DT == kDirect) {
+    __builtin_memcpy(__builtin_assume_aligned(reinterpret_cast<float*>(out) + i * Dp + c, 16), v, 32);
+  } else if constexpr (DT == CIN_DT_F32) {
 #pragma unroll
     for (int p = 0; p < 3; ++p) {
       v4u h;
@@ -578,21 +602,21 @@ __device__ __forceinline__ void copy_piece(const void* __restrict__ x, int64_t l
     __builtin_memcpy(__builtin_assume_aligned(d, 16), v, 16);
   }
 }
-template <bool F32>
+template <int DT>
 __global__ __launch_bounds__(256) void k_ce_copy(const void* __restrict__ x, int64_t ldx, int64_t rows, int64_t D,
                                                  const int* __restrict__ map, const int* __restrict__ n,
                                                  uint16_t* __restrict__ out, int64_t Dp, int64_t plane) {
   const int64_t pieces = Dp / 8, have = n ? *n : rows;
   for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < have * pieces; q += (int64_t)gridDim.x * 256) {
     const int64_t i = q / pieces;
-    copy_piece<F32>(x, ldx, D, map ? (int64_t)map[i] : i, i, (q - i * pieces) * 8, out, Dp, plane);
+    copy_piece<DT>(x, ldx, D, map ? (int64_t)map[i] : i, i, (q - i * pieces) * 8, out, Dp, plane);
   }
 }
 
 // k_ce_rows and k_ce_copy in one launch for few rows: every workgroup finds the rows, the first one
 // writes the state.
 constexpr int kFewRows = 256 * kRowPer;
-template <bool F32>
+template <int DT>
 __global__ __launch_bounds__(256) void k_ce_rows_copy(const int64_t* __restrict__ y, int64_t T, int64_t V, int64_t ignore,
                                                       IntState st, float* __restrict__ rowloss, const void* __restrict__ x,
                                                       int64_t ldx, int64_t D, uint16_t* __restrict__ out, int64_t Dp) {
@@ -601,7 +625,7 @@ __global__ __launch_bounds__(256) void k_ce_rows_copy(const int64_t* __restrict_
   const uint32_t pieces = (uint32_t)(Dp / 8), total = n * pieces;  // (at most 2^11 x 2^15)
   for (uint32_t q = blockIdx.x * 256 + threadIdx.x; q < total; q += gridDim.x * 256) {
     const uint32_t i = q / pieces;
-    copy_piece<F32>(x, ldx, D, map[i], i, (q - i * pieces) * 8, out, Dp, T * Dp);
+    copy_piece<DT>(x, ldx, D, map[i], i, (q - i * pieces) * 8, out, Dp, T * Dp);
   }
 }
 
@@ -855,19 +879,21 @@ double tile_time(int tile, int64_t m, int64_t n, double parts, double part) {
   const double rounds = ceil(count / cin_device_cus());
   return rounds * kTileM[tile] * kTileN[tile] / kTileRate[tile] * part;
 }
-int pick_tile(int64_t m, int64_t n) {
-  int best = 0;
-  for (int t = 1; t < kTiles; ++t)
+// fp32 operands of 4 bytes come for few rows only, and in the two smaller tiles.
+int first_tile(int op) { return op == kDirect ? 2 : 0; }
+int pick_tile(int op, int64_t m, int64_t n) {
+  int best = first_tile(op);
+  for (int t = best + 1; t < kTiles; ++t)
     if (tile_time(t, m, n, 1, 1) < tile_time(best, m, n, 1, 1)) best = t;
   return best;
 }
-template <class F>
+template <int DT, class F>
 void with_tile(int tile, F f) {
-  if (tile == 0)
-    f(Widest{});
-  else if (tile == 1)
-    f(Wide{});
-  else if (tile == 2)
+  if constexpr (DT != kDirect) {
+    if (tile == 0) return f(Widest{});
+    if (tile == 1) return f(Wide{});
+  }
+  if (tile <= 2)
     f(Medium{});
   else
     f(Narrow{});
@@ -881,8 +907,13 @@ constexpr int64_t kMaxPiece = (int64_t)1 << 20;    // its columns: 256 rows lie 
 int64_t align_up(int64_t v, int64_t a) { return cdiv(v, a) * a; }
 constexpr int64_t kAlign = 256;  // columns of a piece: whole tiles
 
+// fp32 with so few rows is multiplied as it is: its products are bound by reading w, which three planes
+// more than double, and w needs no copy of three.
+constexpr int64_t kDirectRows = 128;
+
 struct Plan {
-  int planes;           // of an operand: 3 for fp32
+  int op;               // what the operands hold
+  int planes, es;       // of an operand: 3 for fp32 in parts; bytes of an element
   int64_t Dp;           // columns of x and w as the products read them
   int tile;             // of the forward product
   int64_t tiles_n;      // its column tiles
@@ -896,26 +927,28 @@ struct Plan {
 
 Plan make_plan(int dtype, int64_t T, int64_t D, int64_t V) {
   Plan p;
-  p.planes = dtype == CIN_DT_F32 ? 3 : 1;
-  p.Dp = align_up(D, BK);
   const int64_t Tp = T > 0 ? T : 1;
-  p.tile = pick_tile(Tp, V);
+  p.op = dtype == CIN_DT_F32 && Tp <= kDirectRows ? kDirect : dtype;
+  p.planes = p.op == CIN_DT_F32 ? 3 : 1;
+  p.es = p.op == kDirect ? 4 : 2;
+  p.Dp = align_up(D, kPadK);
+  p.tile = pick_tile(p.op, Tp, V);
   p.tiles_n = cdiv(V, kTileN[p.tile]);
-  int64_t most = align_up(kPieceBytes / (Tp * kEs * p.planes) + 1, kAlign);
+  int64_t most = align_up(kPieceBytes / (Tp * p.es * p.planes) + 1, kAlign);
   if (most > kMaxPiece) most = kMaxPiece;
   const int64_t pieces = cdiv(V, most);
   p.piece = align_up(cdiv(V, pieces), kAlign);
   p.ldz = p.piece + 64;  // rows not a multiple of 16 KiB apart
   // dx: K, the piece, is split where the tiles are fewer than the CUs, in parts of 8 steps at least
-  const int64_t steps = p.piece / BK;
+  const int64_t steps = p.piece / kPadK;
   double best = 0;
-  for (int t = 0; t < kTiles; ++t) {
+  for (int t = first_tile(p.op); t < kTiles; ++t) {
     const int64_t count = cdiv(Tp, kTileM[t]) * cdiv(p.Dp, kTileN[t]);
     int64_t s = cin_device_cus() / count;
     if (s > steps / 8) s = steps / 8;
     if (s < 1) s = 1;
     const double time = tile_time(t, Tp, p.Dp, (double)s, 1.0 / s);
-    if (t == 0 || time < best) {
+    if (t == first_tile(p.op) || time < best) {
       best = time;
       p.splits = (int)s;
       p.slab_tile = t;
@@ -926,10 +959,10 @@ Plan make_plan(int dtype, int64_t T, int64_t D, int64_t V) {
                   (int)(steps / 8), Tp * p.splits};
   p.part = align_up(Tp * p.tiles_n * 8, 256);
   p.ztarget = align_up(Tp * 4, 256);
-  p.dz = align_up(p.planes * Tp * p.ldz * kEs, 256);
+  p.dz = align_up(p.planes * Tp * p.ldz * p.es, 256);
   p.slabs = align_up(p.splits * Tp * p.Dp * 4, 256);
-  p.few = p.planes == 1 && Tp <= kFewExact;
-  p.scaled = p.few ? align_up(2 * Tp * p.Dp * kEs, 256) : 0;
+  p.few = dtype != CIN_DT_F32 && Tp <= kFewExact;
+  p.scaled = p.few ? align_up(2 * Tp * p.Dp * p.es, 256) : 0;
   p.coef = align_up((2 * Tp + 2) * 4, 256);
   return p;
 }
@@ -946,14 +979,14 @@ int check(const char* name, int dtype, int64_t T, int64_t D, int64_t V, Plan& p)
   CIN_CHECK_ARG(D >= 1 && D <= kMaxD, "%s: D must be in [1, 2^18]", name);
   // (the products over a piece of the vocabulary are smaller: T x piece < 2^30 + 256 T)
   p = make_plan(dtype, T, D, V);
-  CIN_CHECK_ARG(grid_fits(p.tile, T, V) && grid_fits(p.slab_tile, T, p.Dp) && grid_fits(pick_tile(p.piece, D), p.piece, D),
+  CIN_CHECK_ARG(grid_fits(p.tile, T, V) && grid_fits(p.slab_tile, T, p.Dp) && grid_fits(pick_tile(p.op, p.piece, D), p.piece, D),
                 "%s: T x V, T x D or V x D is too large", name);
   return CIN_OK;
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
-bool w_fits(const void* w, int64_t ldw) {
-  return aligned16(w) && ldw * kEs % 16 == 0 && ldw <= 4 * kMaxD;
+bool w_fits(const void* w, int64_t ldw, int es) {
+  return aligned16(w) && ldw * es % 16 == 0 && ldw <= 4 * kMaxD;
 }
 
 template <class F>
@@ -966,26 +999,34 @@ void with_dtype(int dtype, F f) {
     f(std::integral_constant<int, CIN_DT_BF16>{});
 }
 
+// The same for what the operands hold.
+template <class F>
+void with_op(int op, F f) {
+  if (op == kDirect)
+    f(std::integral_constant<int, kDirect>{});
+  else
+    with_dtype(op, f);
+}
+
 template <int EPI>
-void gemm(int dtype, int tile, const GemmArgs& g, int64_t max_m, int splits, hipStream_t s) {
-  with_tile(tile, [&](auto c) {
-    using C = decltype(c);
-    with_dtype(dtype, [&](auto dt) {
+void gemm(int op, int tile, const GemmArgs& g, int64_t max_m, int splits, hipStream_t s) {
+  with_op(op, [&](auto dt) {
+    with_tile<dt()>(tile, [&](auto c) {
+      using C = decltype(c);
       const int64_t tiles = cdiv(max_m, C::TM) * cdiv(g.N, C::TN) * splits;
       hipLaunchKernelGGL((k_ce_gemm<C, dt(), EPI>), (unsigned)tiles, C::kThreads, 0, s, g);
     });
   });
 }
 
-void copy_rows(bool f32, const void* x, int64_t ldx, int64_t rows, int64_t D, const int* map, const int* n, void* out,
+void copy_rows(int op, const void* x, int64_t ldx, int64_t rows, int64_t D, const int* map, const int* n, void* out,
                int64_t Dp, hipStream_t s) {
   const int64_t blocks = cdiv(rows * (Dp / 8), 256);
   const unsigned grid = (unsigned)(blocks < 8192 ? blocks : 8192);
-  uint16_t* o = static_cast<uint16_t*>(out);
-  if (f32)
-    hipLaunchKernelGGL(k_ce_copy<true>, grid, 256, 0, s, x, ldx, rows, D, map, n, o, Dp, rows * Dp);
-  else
-    hipLaunchKernelGGL(k_ce_copy<false>, grid, 256, 0, s, x, ldx, rows, D, map, n, o, Dp, rows * Dp);
+  // (16-bit elements are copied, whichever they are)
+  with_op(op == CIN_DT_F16 ? CIN_DT_BF16 : op, [&](auto dt) {
+    hipLaunchKernelGGL(k_ce_copy<dt()>, grid, 256, 0, s, x, ldx, rows, D, map, n, static_cast<uint16_t*>(out), Dp, rows * Dp);
+  });
 }
 
 }  // namespace
@@ -1007,8 +1048,7 @@ int cin_linear_ce_forward(const void* x, int dtype, int64_t T, int64_t D, int64_
   if (int rc = check(name, dtype, T, D, V, p)) return rc;
   CIN_CHECK_ARG(ldx >= D && ldw >= D, "%s: rows overlap", name);
   CIN_CHECK_ARG(state_i && w && (T == 0 || (x && target && xc && state_f && rowloss)), "%s: null pointer", name);
-  const bool f32 = dtype == CIN_DT_F32;
-  CIN_CHECK_ARG(wp || (!f32 && w_fits(w, ldw) && p.Dp == D), "%s: w needs a padded copy", name);
+  CIN_CHECK_ARG(wp || (p.planes == 1 && w_fits(w, ldw, p.es) && p.Dp == D), "%s: w needs a padded copy", name);
   CIN_CHECK_ARG(aligned16(xc) && aligned16(wp) && aligned16(workspace), "%s: xc, wp and workspace must lie on 16 bytes", name);
   CIN_CHECK_ARG(workspace_bytes >= p.part + p.ztarget && workspace, "%s: workspace needs %lld bytes", name,
                 (long long)(p.part + p.ztarget));
@@ -1020,32 +1060,29 @@ int cin_linear_ce_forward(const void* x, int dtype, int64_t T, int64_t D, int64_
     hipLaunchKernelGGL(k_ce_rows, 1, 1024, 0, s, target, T, V, ignore_index, st, rowloss);
   if (T > 0) {
     if (T > kFewRows) {
-      copy_rows(f32, x, ldx, T, D, st.map, st.n, xc, p.Dp, s);
+      copy_rows(p.op, x, ldx, T, D, st.map, st.n, xc, p.Dp, s);
     } else {
       const unsigned grid = (unsigned)cdiv(T * (p.Dp / 8), 256);
-      uint16_t* o = static_cast<uint16_t*>(xc);
-      if (f32)
-        hipLaunchKernelGGL(k_ce_rows_copy<true>, grid < 256 ? grid : 256, 256, 0, s, target, T, V, ignore_index, st, rowloss,
-                           x, ldx, D, o, p.Dp);
-      else
-        hipLaunchKernelGGL(k_ce_rows_copy<false>, grid < 256 ? grid : 256, 256, 0, s, target, T, V, ignore_index, st, rowloss,
-                           x, ldx, D, o, p.Dp);
+      with_op(p.op == CIN_DT_F16 ? CIN_DT_BF16 : p.op, [&](auto dt) {
+        hipLaunchKernelGGL(k_ce_rows_copy<dt()>, grid < 256 ? grid : 256, 256, 0, s, target, T, V, ignore_index, st, rowloss,
+                           x, ldx, D, static_cast<uint16_t*>(xc), p.Dp);
+      });
     }
-    if (wp) copy_rows(f32, w, ldw, V, D, nullptr, nullptr, wp, p.Dp, s);
+    if (wp) copy_rows(p.op, w, ldw, V, D, nullptr, nullptr, wp, p.Dp, s);
     GemmArgs g{};
     g.A = xc;
     g.lda = p.Dp;
     g.B = wp ? wp : w;
     g.ldb = wp ? p.Dp : ldw;
-    g.plane_a = T * p.Dp * kEs;
-    g.plane_b = V * p.Dp * kEs;
+    g.plane_a = T * p.Dp * p.es;
+    g.plane_b = V * p.Dp * p.es;
     g.N = g.V = V;
     g.K = p.Dp;
     g.n = st.n;
     g.part = part;
     g.ztarget = zt;
     g.target = st.target;
-    gemm<kStats>(dtype, p.tile, g, T, 1, s);
+    gemm<kStats>(p.op, p.tile, g, T, 1, s);
   }
   // (without rows one workgroup: the sum of none)
   hipLaunchKernelGGL(k_ce_join, (unsigned)(T > 0 ? cdiv(T, 4) : 1), 256, 0, s, part, (int)p.tiles_n, T, st, zt, state_f,
@@ -1060,7 +1097,7 @@ int cin_linear_ce_backward(const void* xc, int dtype, int64_t T, int64_t D, cons
   const char* name = "linear_ce_backward";
   Plan p;
   if (int rc = check(name, dtype, T, D, V, p)) return rc;
-  CIN_CHECK_ARG(w_fits(w, ldw) && (dtype == CIN_DT_F32 ? ldw == p.Dp : ldw >= p.Dp),
+  CIN_CHECK_ARG(w_fits(w, ldw, p.es) && (p.planes > 1 ? ldw == p.Dp : ldw >= p.Dp),
                 "%s: w's rows must be padded as the forward's", name);
   CIN_CHECK_ARG(grad_stride >= 0, "%s: negative gradient stride", name);
   CIN_CHECK_ARG(T > 0 && state_i && state_f && xc && w && grad, "%s: null pointer", name);
@@ -1092,11 +1129,11 @@ int cin_linear_ce_backward(const void* xc, int dtype, int64_t T, int64_t D, cons
     GemmArgs g{};
     g.A = xc;
     g.lda = p.Dp;
-    g.B = wb + v0 * ldw * kEs;
+    g.B = wb + v0 * ldw * p.es;
     g.ldb = ldw;
-    g.plane_a = T * p.Dp * kEs;
-    g.plane_b = V * p.Dp * kEs;
-    g.N = align_up(cols, BK);  // with the zeros that fill the next product's last K step
+    g.plane_a = T * p.Dp * p.es;
+    g.plane_b = V * p.Dp * p.es;
+    g.N = align_up(cols, kPadK);  // with the zeros that fill the next product's last K step
     g.K = p.Dp;
     g.n = st.n;
     g.C = dz;
@@ -1108,14 +1145,14 @@ int cin_linear_ce_backward(const void* xc, int dtype, int64_t T, int64_t D, cons
     g.rowmax = state_f;
     g.inv = state_f + T;
     g.coef = by.coef;
-    gemm<kGrad>(dtype, pick_tile(T, g.N), g, T, 1, s);
+    gemm<kGrad>(p.op, pick_tile(p.op, T, g.N), g, T, 1, s);
     GemmArgs h{};
     h.n = st.n;
     h.A = dz;
     h.lda = p.ldz;
     h.wa = p.ldz;
     h.wb = p.Dp;
-    h.plane_a = T * p.ldz * kEs;
+    h.plane_a = T * p.ldz * p.es;
     h.v0 = v0;
     h.V = V;
     if (dx) {
@@ -1128,7 +1165,7 @@ int cin_linear_ce_backward(const void* xc, int dtype, int64_t T, int64_t D, cons
       h.C = slabs;
       h.ldc = p.Dp;
       h.add = v0 > 0;
-      gemm<kSlab>(dtype, p.slab_tile, h, T, p.splits, s);
+      gemm<kSlab>(p.op, p.slab_tile, h, T, p.splits, s);
     }
     if (dw) {
       h.B = p.few ? scaled : xc;
@@ -1140,7 +1177,7 @@ int cin_linear_ce_backward(const void* xc, int dtype, int64_t T, int64_t D, cons
       h.C = static_cast<char*>(dw) + v0 * D * (dtype == CIN_DT_F32 ? 4 : 2);
       h.ldc = D;
       h.out_scale = by.out;
-      gemm<kFinal>(dtype, pick_tile(cols, D), h, cols, 1, s);
+      gemm<kFinal>(p.op, pick_tile(p.op, cols, D), h, cols, 1, s);
     }
   }
   if (dx) {

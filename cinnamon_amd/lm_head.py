@@ -21,6 +21,7 @@ __all__ = ["linear_cross_entropy"]
 
 _PLAIN = (torch.Tensor, torch.nn.Parameter)
 _MODES = {"none": 0, "sum": 1, "mean": 2}
+_DIRECT_ROWS = 128  # up to which fp32 is multiplied as it is (csrc/lm_head.hip kDirectRows)
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
@@ -34,10 +35,11 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     Differentiable in x and weight (once), gradients in their dtype.  Products are summed in fp32;
     the gradient of the logits enters the two gradient products rounded to the inputs' dtype, for up
     to 256 rows scaled so that the targets' entries are exact.
-    fp32 inputs are multiplied as three bf16 parts each, to the accuracy of fp32 products.
+    fp32 inputs are multiplied as three bf16 parts each, to the accuracy of fp32 products (up to 128
+    rows as they are).
     Results do not vary from call to call.  The backward recomputes the logits piece by piece:
-    beside the inputs it keeps one copy of the rows that count (fp32: 1.5 times their size, and the
-    weight's; a weight whose width is no multiple of 64: a padded copy) and a few words a row, and
+    beside the inputs it keeps one copy of the rows that count (fp32 of more
+    than 128 rows: 1.5 times their size, and the weight's; a weight whose width is no multiple of 64: a padded copy) and a few words a row, and
     works in up to about 1 GiB for a piece of the logits' gradient plus fp32 sums of x's."""
     _require(x.is_cuda and weight.is_cuda and target.is_cuda, "Inputs must be on CUDA")
     _require(x.device == weight.device == target.device, "Inputs must be on one device")
@@ -68,13 +70,14 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
 def _layout(T, D, V, dtype):
     """Bytes of the state that the forward leaves: its rows that count, the weight's copy, integers
     and floats (csrc/lm_head.hip), each from a multiple of 256 on.  Operands are padded to whole K
-    steps of 64; fp32 ones are three bf16 planes; a 16-bit weight whose width needs no padding is
-    not copied.  Returns (offsets of the four, total, whether the weight is copied)."""
+    steps of 64; fp32 ones are three bf16 planes (for few rows as they are); a weight in one plane
+    whose width needs no padding is not copied.  Returns (offsets of the four, total, whether the weight is copied)."""
     Dp = _cdiv(D, 64) * 64
-    planes = 3 if dtype == torch.float32 else 1
+    planes = 3 if dtype == torch.float32 and T > _DIRECT_ROWS else 1
+    es = 4 if dtype == torch.float32 and T <= _DIRECT_ROWS else 2
     copied = planes == 3 or Dp != D
     offsets, at = [], 0
-    for n in (planes * T * Dp * 2, planes * V * Dp * 2 if copied else 0, 4 * (4 + 3 * T), 12 * T):
+    for n in (planes * T * Dp * es, planes * V * Dp * es if copied else 0, 4 * (4 + 3 * T), 12 * T):
         offsets.append(at)
         at += _cdiv(n, 256) * 256
     return offsets, at, copied

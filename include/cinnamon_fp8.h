@@ -561,8 +561,8 @@ int cin_rotary(const void* q, int64_t sqb, int64_t sql, int64_t sqh, void* q_out
  *   rowloss [T] fp32; loss [1] fp32 or null: their sum, with mean over the rows that count.
  * For the backward the forward fills xc [T, Dp] of dtype, state_i [4 + 3 T] int32 and state_f
  * [3 T] fp32, Dp = D rounded up to 64; and wp [V, Dp] of dtype, a padded copy of w that is needed
- * (else null) where Dp != D or w's rows do not start on 16 bytes.  For fp32, xc is [3, T, Dp] and wp,
- * always needed, [3, V, Dp] bf16: three parts of each value.
+ * (else null) where Dp != D or w's rows do not start on 16 bytes.  For fp32 with T above 128, xc is
+ * [3, T, Dp] and wp, always needed, [3, V, Dp] bf16: three parts of each value.
  *   workspace: cin_linear_ce_workspace(dtype, T, D, V, backward) bytes (-1 for sizes that are
  *   refused: T above 2^26 - 4, V above 2^29, D above 2^18, products of 2^32 threads).  It, xc, wp and
  *   dx lie on 16 bytes.
