@@ -64,6 +64,9 @@ struct Cfg {
   // staged rows: all, or one row of waves at a time where all would not fit
   static constexpr int kParts = TM * kCStride <= 160 * 1024 ? 1 : WM, kPartRows = TM / kParts;
   static constexpr int kBytes = STAGES * kStage > kPartRows * kCStride ? STAGES * kStage : kPartRows * kCStride;
+  // Stages that hold all planes of fp32 operands, 0 where two do not fit.  A step then has all six products,
+  // which short runs of steps need (512 x 1500 x 4096: forward 179 -> 85 us, with gradients 457 -> 265).
+  static constexpr int kStages3 = 160 * 1024 / (3 * kStage) < 2 ? 0 : 160 * 1024 / (3 * kStage) < 4 ? 160 * 1024 / (3 * kStage) : 4;
 };
 
 // What a product ends in.
@@ -226,7 +229,9 @@ template <class C, int DT, int EPI>
 __global__ __launch_bounds__(C::kThreads, 2) void k_ce_gemm(GemmArgs g) {
   constexpr bool kAcrossA = EPI == kFinal, kAcrossB = EPI == kSlab || EPI == kFinal;
   constexpr int MT = C::MT, NT = C::NT, kSegs = DT == CIN_DT_F32 ? kPairs32 : 1, BK = kStepBytes / kEs<DT>;
-  __shared__ __attribute__((aligned(128))) uint8_t smem[C::kBytes];
+  constexpr bool kTogether = DT == CIN_DT_F32 && C::kStages3 > 0;
+  constexpr int kStages = kTogether ? C::kStages3 : C::kStages, kPlanes = kTogether ? 3 : 1, kStage = C::kStage * kPlanes;
+  __shared__ __attribute__((aligned(128))) uint8_t smem[kStages * kStage > C::kBytes ? kStages * kStage : C::kBytes];
   const int64_t rows = __builtin_amdgcn_readfirstlane(*g.n);
   const int64_t M = EPI == kFinal ? g.M : rows, Kall = EPI == kFinal ? rows : g.K;
   const uint32_t tiles_m = (uint32_t)cdiv(M, C::TM), tiles_n = (uint32_t)cdiv(g.N, C::TN);
@@ -257,15 +262,25 @@ __global__ __launch_bounds__(C::kThreads, 2) void k_ce_gemm(GemmArgs g) {
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+  v4f low[kTogether ? MT : 1][kTogether ? NT : 1] = {};  // the small products
   const int nk = k1 > k0 ? (int)((k1 - k0 + BK - 1) / BK) : 0;
   if (nk > 0) {
     // w has rows up to the vocabulary's end, as tile rows or as K
     oa.init(g.A, g.lda, m0, (kAcrossA ? g.wa : M) - m0, k0, k1, tid, lds0);
     ob.init(g.B, g.ldb, n0, (kAcrossB ? g.wb : g.V - g.v0) - n0, k0,
-            EPI == kSlab && k1 > g.V - g.v0 ? g.V - g.v0 : k1, tid, lds0 + C::TM * 128);
+            EPI == kSlab && k1 > g.V - g.v0 ? g.V - g.v0 : k1, tid, lds0 + C::TM * 128 * kPlanes);
   }
   int fk = 0, seg = 0;  // the K step and pair of planes that are fetched next
   const auto fetch = [&](uint32_t stage) {
+    if constexpr (kTogether) {
+#pragma unroll
+      for (int p = 0; p < 3; ++p) {
+        oa.fetch(fk, p * g.plane_a, stage + p * C::TM * 128);
+        ob.fetch(fk, p * g.plane_b, stage + p * C::TN * 128);
+      }
+      ++fk;
+      return;
+    }
     int64_t pa = 0, pb = 0;
     if constexpr (kSegs > 1) {
       int ia, ib;
@@ -282,12 +297,11 @@ __global__ __launch_bounds__(C::kThreads, 2) void k_ce_gemm(GemmArgs g) {
       ++seg;
     }
   };
-  const int steps = nk * (EPI == kFinal && kSegs == 1 ? g.segs : kSegs);
-  constexpr int kStages = C::kStages;
-  constexpr int kOps = decltype(oa)::kOps + decltype(ob)::kOps;
+  const int steps = nk * (EPI == kFinal && kSegs == 1 ? g.segs : kTogether ? 1 : kSegs);
+  constexpr int kOps = (decltype(oa)::kOps + decltype(ob)::kOps) * kPlanes;
 #pragma unroll
   for (int q = 0; q < kStages - 1; ++q)
-    if (q < steps) fetch(q * C::kStage);
+    if (q < steps) fetch(q * kStage);
   for (int kt = 0; kt < steps; ++kt) {
     // step kt has landed once no more than the kStages - 2 behind it are on their way
     if (kStages > 2 && kt + kStages - 2 < steps)
@@ -295,23 +309,57 @@ __global__ __launch_bounds__(C::kThreads, 2) void k_ce_gemm(GemmArgs g) {
     else
       wait_dma();
     lds_barrier();
-    const uint32_t st = (kt % kStages) * C::kStage;
+    const uint32_t st = (kt % kStages) * kStage;
     // where step kt - 1 was, read by all
-    if (kt + kStages - 1 < steps) fetch((kt + kStages - 1) % kStages * C::kStage);
+    if (kt + kStages - 1 < steps) fetch((kt + kStages - 1) % kStages * kStage);
     const uint8_t* sa = smem + st;
-    const uint8_t* sb = sa + C::TM * 128;
+    const uint8_t* sb = sa + C::TM * 128 * kPlanes;
+    if constexpr (kTogether) {
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      v4u bf[NT];
+      for (int ks = 0; ks < 2; ++ks) {
+        v4u bf[3][NT];
 #pragma unroll
-      for (int j = 0; j < NT; ++j) bf[j] = ob.frag(sb, (wn * NT + j) * 16, ks, l16, kq);
+        for (int p = 0; p < 3; ++p)
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        const v4u af = oa.frag(sa, (wm * MT + i) * 16, ks, l16, kq);
+          for (int j = 0; j < NT; ++j) bf[p][j] = ob.frag(sb + p * C::TN * 128, (wn * NT + j) * 16, ks, l16, kq);
+        v4u af[3][MT];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = mma<DT>(bf[j], af, acc[i][j]);
+        for (int p = 0; p < 3; ++p)
+#pragma unroll
+          for (int i = 0; i < MT; ++i) af[p][i] = oa.frag(sa + p * C::TM * 128, (wm * MT + i) * 16, ks, l16, kq);
+#pragma unroll
+        for (int q = 0; q < kPairs32; ++q) {
+          int ia, ib;
+          planes_of(q, ia, ib);
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+              v4f& c = q + 1 < kPairs32 ? low[i][j] : acc[i][j];
+              c = mma<DT>(bf[ib][j], af[ia][i], c);
+            }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        v4u bf[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) bf[j] = ob.frag(sb, (wn * NT + j) * 16, ks, l16, kq);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          const v4u af = oa.frag(sa, (wm * MT + i) * 16, ks, l16, kq);
+#pragma unroll
+          for (int j = 0; j < NT; ++j) acc[i][j] = mma<DT>(bf[j], af, acc[i][j]);
+        }
       }
     }
+  }
+  if constexpr (kTogether) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) acc[i][j] += low[i][j];
   }
   lds_barrier();
   // the lane holds rows m0 + (wm MT + i) 16 + l16, columns n0 + (wn NT + j) 16 + 4 kq + r
@@ -860,18 +908,20 @@ __global__ __launch_bounds__(256) void k_ce_dx(const float* __restrict__ slabs, 
 // Tiles.  Wide ones read their operands less often and keep the matrix units busier (without loads
 // the 256 x 256 tile's loop runs at 1.62 PFLOP/s, with operands that hit the L2 at 1.32, at full length
 // at 1.23); narrow ones leave fewer compute units idle in a small product, and the narrowest, with more
-// steps on their way, stream w for a few rows.  8192 x 131072 x 4096, bf16: x w^T 1.32 and 1.24 PFLOP/s
+// steps on their way, stream w for a few rows (16 x 100000 x 2048 of fp32, forward: 188 us with the 32 x 64
+// tile, 266 with 64 x 64).  8192 x 131072 x 4096, bf16: x w^T 1.32 and 1.24 PFLOP/s
 // with the two widest; 16368 x 32000 x 1024: 1.07 and 0.97, 0.89 with 128 x 128.
 using Widest = Cfg<2, 4, 8, 6, 2>;  // 256 x 384, 8 waves of 128 x 96: 250 registers, all of the LDS
 using Wide = Cfg<2, 4, 8, 4, 2>;    // 256 x 256, 8 waves of 128 x 64
 using Medium = Cfg<2, 2, 4, 4, 2>;  // 128 x 128, 4 waves of 64 x 64, two workgroups a CU
 using Narrow = Cfg<1, 4, 4, 1, 4>;  // 64 x 64, 4 waves of 64 x 16, two workgroups a CU
-constexpr int kTiles = 4;
-constexpr int kTileM[kTiles] = {Widest::TM, Wide::TM, Medium::TM, Narrow::TM};
-constexpr int kTileN[kTiles] = {Widest::TN, Wide::TN, Medium::TN, Narrow::TN};
-constexpr int kTileThreads[kTiles] = {Widest::kThreads, Wide::kThreads, Medium::kThreads, Narrow::kThreads};
+using Thin = Cfg<1, 4, 2, 1, 6>;    // 32 x 64, 4 waves of 32 x 16, two workgroups a CU: up to 32 rows, few tiles
+constexpr int kTiles = 5;
+constexpr int kTileM[kTiles] = {Widest::TM, Wide::TM, Medium::TM, Narrow::TM, Thin::TM};
+constexpr int kTileN[kTiles] = {Widest::TN, Wide::TN, Medium::TN, Narrow::TN, Thin::TN};
+constexpr int kTileThreads[kTiles] = {Widest::kThreads, Wide::kThreads, Medium::kThreads, Narrow::kThreads, Thin::kThreads};
 // a tile's rate against that of the 256 x 256 ones, every CU at work
-constexpr double kTileRate[kTiles] = {1.08, 1.0, 0.75, 0.4};
+constexpr double kTileRate[kTiles] = {1.08, 1.0, 0.75, 0.4, 0.25};
 
 // The time of m x n outputs in parts of K, in units of one output's share at the 256 x 256 tile's rate.
 double tile_time(int tile, int64_t m, int64_t n, double parts, double part) {
@@ -895,8 +945,10 @@ void with_tile(int tile, F f) {
   }
   if (tile <= 2)
     f(Medium{});
-  else
+  else if (tile == 3)
     f(Narrow{});
+  else
+    f(Thin{});
 }
 
 // A launch has fewer than 2^32 threads: k_ce_join takes 64 a row.
@@ -908,7 +960,8 @@ int64_t align_up(int64_t v, int64_t a) { return cdiv(v, a) * a; }
 constexpr int64_t kAlign = 256;  // columns of a piece: whole tiles
 
 // fp32 with so few rows is multiplied as it is: its products are bound by reading w, which three planes
-// more than double, and w needs no copy of three.
+// more than double, and w needs no copy of three (forward of 16 x 100000 x 2048: 188 us, in parts 880; with
+// gradients 829 and 2176; of 128: 490 and 1000, 1870 and 2660; of 256: 866 and 1117, but 3390 and 3180).
 constexpr int64_t kDirectRows = 128;
 
 struct Plan {

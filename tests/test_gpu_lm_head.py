@@ -79,7 +79,7 @@ SHAPES = [
     # T, V, D, ignored
     (1, 1, 1, 0.0), (1, 1000, 64, 0.0), (2, 7, 130, 0.0), (16, 3201, 96, 0.0), (65, 64, 8, 0.3), (255, 257, 64, 0.0),
     (257, 513, 129, 0.5), (300, 2049, 192, 0.1), (513, 5003, 320, 0.4), (1000, 300, 777, 0.9), (130, 1024, 1024, 0.0),
-    (3, 20011, 33, 0.0),
+    (3, 20011, 33, 0.0), (128, 3001, 256, 0.2), (129, 700, 2048, 0.0), (33, 5000, 65, 0.0), (20, 260, 4097, 0.1), (32, 9000, 512, 0.0),
 ]
 
 
