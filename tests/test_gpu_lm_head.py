@@ -232,6 +232,37 @@ def test_few_rows_are_rounded_once(dev, T, dt, reduction):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("gap", [0.0, 10.0, 40.0, -40.0])
+def test_sure_rows(dev, dt, gap):
+    """Few rows whose target is nearly sure, or nearly impossible, some with a gradient of 0 or far below the others'."""
+    T, V, D = 5, 600, 64
+    g = torch.Generator().manual_seed(3)
+    x = torch.zeros(T, D)
+    x[:, 0] = 8
+    x[:, 1:] = torch.randn(T, D - 1, generator=g) * 0.1
+    w = torch.randn(V, D, generator=g) * 0.1
+    w[:, 0] = 0
+    y = torch.arange(T) * 7
+    w[y[0], 0] = gap / 8  # the first row's target for all rows
+    y[1:3] = y[0]
+    x, w = (t.to(DT[dt]).to(dev).requires_grad_() for t in (x, w))
+    y, gr = y.to(dev), torch.tensor([1.0, 0.0, -1e-6, 0.5, 1e-12], device=dev)
+    loss = lm_head.linear_cross_entropy(x, w, y, reduction="none")
+    dx, dw = torch.autograd.grad(loss, (x, w), gr)
+    x64, w64, g64 = x.detach().double(), w.detach().double(), gr.double()[:, None]
+    p = (x64 @ w64.T).softmax(-1)
+    dz = g64 * (p - torch.nn.functional.one_hot(y, V).double())
+    # an entry of dz: rounded (fp16: to steps of 2^-38 of the largest); p and p - 1 in fp32, whose exponentials'
+    # arguments, up to 45, are off by 2^-22 of themselves from the sums of 64 products and the scaling: 2^-16
+    half = torch.finfo(DT[dt]).eps / 2
+    off = dz.abs() * (half + 2 ** -16) + g64.abs() * (p * 2 ** -16).clamp(max=2 ** -20) + 2 ** -38
+    for got, want, o in ((dx, dz @ w64, off @ w64.abs()), (dw, dz.T @ x64, off.T @ x64.abs())):
+        bound = want.abs() * (half * 1.001 + 600 * 2 ** -24) + o * 1.01 + 2 ** -25
+        assert torch.isfinite(got).all() and ((got.double() - want).abs() <= bound).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("D", [64, 65])
 def test_a_single_row_whose_stride_is_not_its_width(dev, D):
     """One token, and a vocabulary of one: a transposed column's only row has a stride of 1."""
