@@ -82,8 +82,8 @@ SIGNATURES: dict[str, list] = {
     "cin_moe_gate_backward": [_p, _i32, _i64, _i64, _i64, _i64, _i32, _i32, ctypes.c_float, _p, _p, _p, _p, _p],
     "cin_linear_ce_workspace": [_i32, _i64, _i64, _i64, _i32],
     "cin_linear_ce_forward": [_p, _i32, _i64, _i64, _i64, _p, _i64, _i64, _p, _i64, _i32, _p, _p, _p, _p, _p, _p, _p,
-                              _i64, _p],
-    "cin_linear_ce_backward": [_p, _i32, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _i64, _i32, _p, _p, _p, _i64, _p],
+                              _i64, _p, _p],
+    "cin_linear_ce_backward": [_p, _i32, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _i64, _i32, _p, _p, _p, _i64, _p, _p],
     "cin_rotary": [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i64] * 2 + [_i32, _i64, _i64, _i64, _p, _p, _i64, _i64,
                                                                            _i64, _i64, _p, _i64, _i64, _i32, _i32, _p],
 }

@@ -22,6 +22,7 @@ __all__ = ["linear_cross_entropy"]
 _PLAIN = (torch.Tensor, torch.nn.Parameter)
 _MODES = {"none": 0, "sum": 1, "mean": 2}
 _DIRECT_ROWS = 128  # up to which fp32 is multiplied as it is (csrc/lm_head.hip kDirectRows)
+_KEEP_ROWS = 128    # up to which the logits are kept: fewer bytes than the weight that gives them again
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
@@ -37,10 +38,11 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     to 256 rows scaled so that the targets' entries are exact.
     fp32 inputs are multiplied as three bf16 parts each, to the accuracy of fp32 products (up to 128
     rows as they are).
-    Results do not vary from call to call.  The backward recomputes the logits piece by piece:
-    beside the inputs it keeps one copy of the rows that count (fp32 of more
-    than 128 rows: 1.5 times their size, and the weight's; a weight whose width is no multiple of 64: a padded copy) and a few words a row, and
-    works in up to about 1 GiB for a piece of the logits' gradient plus fp32 sums of x's."""
+    Results do not vary from call to call.  The backward recomputes the logits piece by piece (up to
+    128 rows keep them): beside the inputs it keeps one copy of the rows that count (fp32 of more than
+    128 rows: 1.5 times their size, and the weight's; a weight whose width is no multiple of 64: a
+    padded copy) and a few words a row, and works in up to about 1 GiB for a piece of the logits'
+    gradient plus fp32 sums of x's."""
     _require(x.is_cuda and weight.is_cuda and target.is_cuda, "Inputs must be on CUDA")
     _require(x.device == weight.device == target.device, "Inputs must be on one device")
     _require(weight.ndim == 2 and x.ndim >= 1 and x.shape[-1] == weight.shape[1], "x must be [..., D] and weight [V, D]")
@@ -61,7 +63,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
         if torch.is_grad_enabled() and (x2.requires_grad or weight.requires_grad):
             loss = _LinearCE.apply(x2, weight, y, int(ignore_index), mode)
         else:
-            loss = _launch_forward(x2, weight, y, int(ignore_index), mode)[0]
+            loss = _launch_forward(x2, weight, y, int(ignore_index), mode, False)[0]
     else:
         loss = _forward_op(x2, weight, y, int(ignore_index), mode)[0]
     return loss.view(target.shape) if mode == 0 and target.ndim != 1 else loss
@@ -69,15 +71,16 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
 
 def _layout(T, D, V, dtype):
     """Bytes of the state that the forward leaves: its rows that count, the weight's copy, integers
-    and floats (csrc/lm_head.hip), each from a multiple of 256 on.  Operands are padded to whole K
+    and floats (csrc/lm_head.hip), for few rows the logits, each from a multiple of 256 on.  Operands are padded to whole K
     steps of 64; fp32 ones are three bf16 planes (for few rows as they are); a weight in one plane
-    whose width needs no padding is not copied.  Returns (offsets of the four, total, whether the weight is copied)."""
+    whose width needs no padding is not copied.  Returns (offsets of the five, total, whether the weight is copied)."""
     Dp = _cdiv(D, 64) * 64
     planes = 3 if dtype == torch.float32 and T > _DIRECT_ROWS else 1
     es = 4 if dtype == torch.float32 and T <= _DIRECT_ROWS else 2
     copied = planes == 3 or Dp != D
     offsets, at = [], 0
-    for n in (planes * T * Dp * es, planes * V * Dp * es if copied else 0, 4 * (4 + 3 * T), 12 * T):
+    for n in (planes * T * Dp * es, planes * V * Dp * es if copied else 0, 4 * (4 + 3 * T), 12 * T,
+              4 * T * _cdiv(V, 64) * 64 if T <= _KEEP_ROWS else 0):
         offsets.append(at)
         at += _cdiv(n, 256) * 256
     return offsets, at, copied
@@ -110,21 +113,22 @@ def _weight_rows(w):
     return w.contiguous() if not w.is_contiguous() else w.clone(memory_format=torch.contiguous_format)
 
 
-def _launch_forward(x, weight, target, ignore_index, mode):
-    """(loss, state for the backward)"""
+def _launch_forward(x, weight, target, ignore_index, mode, keep=True):
+    """(loss, state for the backward; not keep: for none)"""
     (T, D), V = x.shape, weight.shape[0]
     x = _rows(x)
-    (xc, wp, si, sf), total, copied, ws, _ = _sizes(T, D, V, x.dtype)
+    (xc, wp, si, sf, sz), total, copied, ws, _ = _sizes(T, D, V, x.dtype)
     w = _rows(weight) if copied else _weight_rows(weight)
     target = target.contiguous()
-    state = torch.empty(total, dtype=torch.uint8, device=x.device)
+    state = torch.empty(total if keep else sz, dtype=torch.uint8, device=x.device)
     work = torch.empty(ws, dtype=torch.uint8, device=x.device)
     rows = x.new_empty(T, dtype=torch.float32)
     loss = x.new_empty((), dtype=torch.float32) if mode else rows
     at = state.data_ptr()
     call_on(x, "cin_linear_ce_forward", x.data_ptr(), dtype_code(x), T, D, _pitch(x), w.data_ptr(), V, _pitch(w),
             target.data_ptr(), ignore_index, mode == 2, at + xc, at + wp if copied else 0, at + si, at + sf,
-            rows.data_ptr(), loss.data_ptr() if mode else 0, work.data_ptr(), ws, stream_of(x))
+            rows.data_ptr(), loss.data_ptr() if mode else 0, work.data_ptr(), ws, at + sz if keep and T <= _KEEP_ROWS else 0,
+            stream_of(x))
     return loss, state
 
 
@@ -136,7 +140,7 @@ def _launch_backward(grad, state, weight, T, mode, need_x, need_w):
     if T == 0:
         return dx, weight.new_zeros((V, D)) if need_w else None
     dw = weight.new_empty((V, D)) if need_w else None
-    (xc, wp, si, sf), _, copied, _, ws = _sizes(T, D, V, dtype)
+    (xc, wp, si, sf, sz), _, copied, _, ws = _sizes(T, D, V, dtype)
     at = state.data_ptr()
     if copied:
         w, ldw = at + wp, _cdiv(D, 64) * 64
@@ -145,7 +149,7 @@ def _launch_backward(grad, state, weight, T, mode, need_x, need_w):
         w, ldw = weight.data_ptr(), _pitch(weight)
     work = torch.empty(ws, dtype=torch.uint8, device=weight.device)
     call_on(weight, "cin_linear_ce_backward", at + xc, dtype_code(dtype), T, D, w, V, ldw, at + si, at + sf, grad.data_ptr(),
-            0 if mode else grad.stride(0), mode == 2, ptr(dx), ptr(dw), work.data_ptr(), ws, stream_of(weight))
+            0 if mode else grad.stride(0), mode == 2, ptr(dx), ptr(dw), work.data_ptr(), ws, at + sz if T <= _KEEP_ROWS else 0, stream_of(weight))
     return dx, dw
 
 

@@ -570,16 +570,19 @@ int cin_rotary(const void* q, int64_t sqb, int64_t sql, int64_t sqh, void* q_out
  * the loss (grad_stride 0, with mean divided by the rows that count) or of each row (grad_stride
  * elements apart); dx [T, D] and dw [V, D] of dtype, contiguous, either null.  Gradients are
  * bit-identical from call to call.
+ *   logits: null, or [T, V rounded up to 64] fp32 that the forward fills with those of the rows that
+ *   count and the backward reads instead of computing them again (not for fp32 with T above 128).
  */
 int64_t cin_linear_ce_workspace(int dtype, int64_t T, int64_t D, int64_t V, int backward);
 int cin_linear_ce_forward(const void* x, int dtype, int64_t T, int64_t D, int64_t ldx, const void* w,
                           int64_t V, int64_t ldw, const int64_t* target, int64_t ignore_index, int mean,
                           void* xc, void* wp, int32_t* state_i, float* state_f, float* rowloss,
-                          float* loss, void* workspace, int64_t workspace_bytes, void* stream);
+                          float* loss, void* workspace, int64_t workspace_bytes, float* logits,
+                          void* stream);
 int cin_linear_ce_backward(const void* xc, int dtype, int64_t T, int64_t D, const void* w, int64_t V,
                            int64_t ldw, const int32_t* state_i, const float* state_f, const float* grad,
                            int64_t grad_stride, int mean, void* dx, void* dw, void* workspace,
-                           int64_t workspace_bytes, void* stream);
+                           int64_t workspace_bytes, const float* logits, void* stream);
 
 #ifdef __cplusplus
 }

@@ -489,8 +489,8 @@ def test_refusals():
         assert f(fake(2, 2, 65), fake(100, 65), fake(2, 2, dtype=i64), reduction="none").shape == (2, 2)
 
 
-_FWD = [16, 0, 4, 64, 64, 16, 100, 64, 16, -100, 1, 16, None, 16, 16, 16, 16, 16, 1 << 30, None]
-_BWD = [16, 0, 4, 64, 16, 100, 64, 16, 16, 16, 0, 1, 16, 16, 16, 1 << 30, None]
+_FWD = [16, 0, 4, 64, 64, 16, 100, 64, 16, -100, 1, 16, None, 16, 16, 16, 16, 16, 1 << 30, None, None]
+_BWD = [16, 0, 4, 64, 16, 100, 64, 16, 16, 16, 0, 1, 16, 16, 16, 1 << 30, None, None]
 
 
 @pytest.mark.parametrize("name,ok,at,value", [
@@ -506,6 +506,7 @@ _BWD = [16, 0, 4, 64, 16, 100, 64, 16, 16, 16, 0, 1, 16, 16, 16, 1 << 30, None]
     ("cin_linear_ce_forward", _FWD, 2, 1 << 26), ("cin_linear_ce_forward", _FWD, 6, (1 << 29) + 1),
     ("cin_linear_ce_forward", _FWD, 11, 24), ("cin_linear_ce_forward", _FWD, 12, 24), ("cin_linear_ce_forward", _FWD, 17, 24),
     ("cin_linear_ce_backward", _BWD, 0, 24), ("cin_linear_ce_backward", _BWD, 12, 24), ("cin_linear_ce_backward", _BWD, 14, 24),
+    ("cin_linear_ce_forward", _FWD, 19, 24), ("cin_linear_ce_backward", _BWD, 16, 24),
 ])
 def test_c_refusals(name, ok, at, value):
     args = list(ok)
