@@ -497,17 +497,22 @@ __global__ __launch_bounds__(64 * WAVES, EPL <= 16 ? 4 : 1) void k_gate_fwd(Gate
   const float cl = __shfl(my_c, last), zl = __shfl(my_z, last), bl = __shfl(my_b, last), least = cl - bound(cl);
   // (a key is 0 for an expert taken or left out: below that of any choice)
   const uint32_t near = least < __builtin_inff() ? key_of(least) & ~kPlace<EPL> : 1u;
+  bool tied = false;  // an expert not taken that equals the last one taken
   if (key[0] >= near) {
 #pragma unroll
     for (int j = 0; j < EPL; ++j) {
       if (key[j] < near || key[j] == 0) break;
       const int e = e0 + (int)(kPlace<EPL> - (key[j] & kPlace<EPL>));
-      doubt |= !(z_of(e) == zl && (a.bias ? a.bias[e] : 0.0f) == bl);
+      const bool same = z_of(e) == zl && (a.bias ? a.bias[e] : 0.0f) == bl;
+      tied |= same;
+      doubt |= !same;
     }
   }
   if (__ballot(order)) {
     if (a.score == kSigmoid) {
-      // the experts taken are those, in another order perhaps: sorted by their choices in 64 bits
+      // The experts taken are those, in another order perhaps: sorted by their choices in 64 bits.  (But
+      // where one taken before the last may be less than the last, so may it be than the last one's equals.)
+      doubt |= any_lane<LANES>(tied, lane) && order;
       double c = 1 / (1 + exp(-(double)my_z)) + (double)my_b;
       for (int pass = 0; pass < a.k; ++pass) {
         const int p = (sub ^ (pass & 1)) & 1 ? sub - 1 : sub + 1;  // odd and even neighbours in turn

@@ -334,6 +334,40 @@ def test_gate_feeds_the_routed_experts(dev):
     assert (dz - dz2).norm() <= 4 * 2.0 ** -19 * dz2.norm() + 64 * U * dout.norm() * out2.norm()
 
 
+@pytest.mark.gpu
+def test_gate_a_tie_behind_a_near_neighbour(dev):
+    """Three sigmoids in one step of the ranked keys: the two equal ones are the greater, the lower
+    index is not."""
+    logits = torch.zeros(3, 256)
+    for t, at in enumerate(([0, 1, 2], [3, 40, 41], [15, 16, 255])):
+        logits[t, at] = torch.tensor([12.125, 12.1875, 12.1875])
+    logits = logits.to(torch.bfloat16).to(dev)
+    for b in (None, torch.zeros(256, device=dev), torch.full((256,), 0.25, device=dev)):
+        assert moe.moe_gate(logits, 2, bias=b)[0].tolist() == [[1, 2], [40, 41], [16, 255]]
+        assert moe.moe_gate(logits, 1, bias=b)[0].tolist() == [[1], [40], [16]]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("E,G,tg", [(64, 1, 1), (256, 1, 1), (256, 8, 4), (1024, 1, 1), (1024, 16, 5)])
+@pytest.mark.parametrize("about,step", [(12.0, 0.0625), (0.0, 2.0 ** -21), (-9.0, 0.0625)])
+def test_gate_equal_logits_among_near_ones(dev, score, E, G, tg, about, step):
+    """Few adjacent values, so that true ties and neighbours within a step of the keys meet at the border of
+    the top k.  (Groups count by one expert where sums of two of the finest steps are equal in 64 bits.)"""
+    g = torch.Generator().manual_seed(14)
+    logits = (about + step * torch.randint(0, 6, (2000, E), generator=g)).to(torch.bfloat16).to(dev)
+    for bias in (None, torch.zeros(E, device=dev), torch.full((E,), 0.5, device=dev)):
+        for k in (2, 8):
+            kw = dict(bias=bias, score=score, n_groups=G, top_groups=tg, group_top=1)
+            check(moe.moe_gate(logits, k, **kw), reference(logits, k, **kw), E, score)
+    spread = (torch.randn(2000, E, generator=g) * 6).to(torch.bfloat16).to(dev)
+    tiny = (torch.randn(2000, E, generator=g) * 1e-4).to(torch.bfloat16).to(dev)
+    for z in (spread, tiny):
+        for bias in (None, torch.zeros(E, device=dev)):
+            kw = dict(bias=bias, score=score)
+            check(moe.moe_gate(z, 8, **kw), reference(z, 8, **kw), E, score)
+
+
 def _fake(*shape, dtype=torch.float32):
     return torch.empty(*shape, dtype=dtype, device="cuda")
 
