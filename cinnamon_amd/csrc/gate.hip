@@ -200,12 +200,30 @@ __device__ inline void scores(int kind, const float (&z)[EPL], float (&s)[EPL], 
   }
 }
 // Groups that stay, as a mask: lanes share a group's keys, `part` of `parts` each.  `margin` gets
-// the difference between the last group that stays, `worst`, and the first that does not.
+// the difference between the last group that stays, `worst`, and the first that does not; where that is 0,
+// `gap` the least difference between `worst` and a group, staying or not, that is not equal to it.
 template <int LANES, class K, class F>
-__device__ inline uint64_t keep_groups(const GateArgs& a, const K* keys, int lane, F& margin, F& worst) {
+__device__ inline uint64_t keep_groups(const GateArgs& a, const K* keys, int lane, F& margin, F& worst, F& gap) {
   constexpr int kPer = kGateMaxGroups / LANES;  // groups of a lane
   const int sub = lane & (LANES - 1), n = a.E / a.groups;
-  K best[kPer];
+  K best[kPer], all[kPer];
+  // (differences are not negative: as integers they compare the same)
+  const auto least_gap = [&] {
+    gap = 0;
+    if (!__ballot(margin == 0)) return;
+    K far = 0;  // the complement of the least
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      F d = value_of(all[i]) - worst;
+      d = d < 0 ? -d : d;
+      if (sub + i * LANES < a.groups && d != 0) {
+        const K c = ~__builtin_bit_cast(K, d);
+        far = c > far ? c : far;
+      }
+    }
+    far = lanes_max<LANES>(far);
+    gap = far ? __builtin_bit_cast(F, (K)~far) : (F)__builtin_inff();
+  };
 #pragma unroll
   for (int i = 0; i < kPer; ++i) best[i] = 0;
   if (2 * a.groups <= LANES) {
@@ -245,6 +263,8 @@ __device__ inline uint64_t keep_groups(const GateArgs& a, const K* keys, int lan
       best[i] = g >= a.groups ? 0 : (a.group_top == 1 || n == 1 ? k1 : key_of(value_of(k1) + value_of(k2)));
     }
   }
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) all[i] = best[i];
   uint64_t kept = 0;
   K last = 0;
   if (a.groups <= LANES) {  // a group a lane
@@ -258,6 +278,7 @@ __device__ inline uint64_t keep_groups(const GateArgs& a, const K* keys, int lan
     }
     worst = value_of(last);
     margin = worst - value_of(lanes_max<LANES>(best[0]));
+    least_gap();
     return kept;
   }
   for (int r = 0; r <= a.top_groups; ++r) {
@@ -285,6 +306,7 @@ __device__ inline uint64_t keep_groups(const GateArgs& a, const K* keys, int lan
       }
     }
   }
+  least_gap();
   return kept;
 }
 
@@ -361,8 +383,8 @@ __device__ inline void rank64(const GateArgs& a, int64_t t, int lane, uint64_t* 
   for (int e = lane; e < a.E; e += 64) keys[e] = key_of(score(e) + (a.bias ? (double)a.bias[e] : 0.0));
   wave_sync();
   if (a.top_groups < a.groups) {
-    double margin, worst;
-    const uint64_t kept = keep_groups<64, uint64_t, double>(a, keys, lane, margin, worst);
+    double margin, worst, gap;
+    const uint64_t kept = keep_groups<64, uint64_t, double>(a, keys, lane, margin, worst, gap);
     const int n = a.E / a.groups;
     wave_sync();
     for (int e = lane; e < a.E; e += 64)
@@ -456,8 +478,8 @@ __global__ __launch_bounds__(64 * WAVES, EPL <= 16 ? 4 : 1) void k_gate_fwd(Gate
 #pragma unroll
     for (int j = 0; j < EPL; ++j) keys[e0 + j] = key[j];
     wave_sync();
-    float margin, worst;
-    const uint64_t kept = keep_groups<LANES, uint32_t, float>(a, keys, lane, margin, worst);
+    float margin, worst, gap;
+    const uint64_t kept = keep_groups<LANES, uint32_t, float>(a, keys, lane, margin, worst, gap);
     const int n = a.E / a.groups;
     int g = e0 / n;  // the group of e0 + j
     if (n % EPL == 0) {  // a lane's experts are of one group
@@ -477,7 +499,9 @@ __global__ __launch_bounds__(64 * WAVES, EPL <= 16 ? 4 : 1) void k_gate_fwd(Gate
     }
     // two choices of up to `most` each on either side
     most = __uint_as_float(lanes_max<LANES>(__float_as_uint(most)));
-    doubt |= !(margin > 2 * bound(most) + 8 * kU * most || (direct && margin == 0.0f)) || blurred(worst);
+    // (equal logits are a true tie, but not where others that 64 bits may not tell from them are near)
+    const float sure = 2 * bound(most) + 8 * kU * most;
+    doubt |= !(margin > sure || (direct && margin == 0.0f && gap > sure)) || blurred(worst);
   }
 #pragma unroll
   for (int j = 0; j < EPL; ++j) key[j] = key[j] ? (key[j] & ~kPlace<EPL>) | (kPlace<EPL> - j) : 0;

@@ -368,6 +368,29 @@ def test_gate_equal_logits_among_near_ones(dev, score, E, G, tg, about, step):
             check(moe.moe_gate(z, 8, **kw), reference(z, 8, **kw), E, score)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("E,G", [(16, 4), (64, 4), (64, 32), (256, 8), (1024, 8), (1024, 64)])
+def test_gate_groups_that_64_bits_cannot_tell_apart(dev, E, G):
+    """Groups whose best logits differ by less than their scores in 64 bits hold are equal, whichever of
+    them are equal in the logits too: the lowest stay."""
+    g = torch.Generator().manual_seed(15)
+    n = E // G
+    best = torch.randint(1, 5, (300, G), generator=g).float() * 1e-18
+    first = torch.tensor([[1.0, 2, 2, 2], [1, 3, 2, 2], [4, 1, 2, 2], [2, 2, 1, 2]]) * 1e-18
+    best[:4, :4] = first
+    best[:4, 4:] = -0.5
+    best[200:] = torch.where(torch.rand(100, G, generator=g) < 0.5, best[200:], -0.25)
+    logits = torch.full((300, G, n), -1.0)
+    logits[torch.arange(300)[:, None], torch.arange(G), torch.randint(0, n, (300, G), generator=g)] = best
+    logits = logits.flatten(1).to(dev)
+    for tg in (1, 2, 3):
+        for k in (1, min(2, tg * n)):
+            kw = dict(n_groups=G, top_groups=tg, group_top=1)
+            check(moe.moe_gate(logits, k, **kw), reference(logits, k, **kw), E, "sigmoid")
+    for t in range(2):
+        assert moe.moe_gate(logits[t:t + 1], 2, n_groups=G, top_groups=2, group_top=1)[0].div(n, rounding_mode="floor").tolist() == [[0, 1]]
+
+
 def _fake(*shape, dtype=torch.float32):
     return torch.empty(*shape, dtype=dtype, device="cuda")
 
