@@ -11,6 +11,8 @@
 // backward, with gw and gs the gradients of w and s:
 //   ds     = gs;  ds[idx_j] += scale * (gw_j - sum_i gw_i s[idx_i] / total) / total
 //   dz     = ds s (1 - s)  or  s (ds - sum_e ds_e s_e)
+// without the differences that cancel: s (1 - s) = t / (1 + t)^2 with t = e^-|z|, and the weights' term
+// is scale * (1e-9 gw_j + sum_i (gw_j - gw_i) s[idx_i]) / total^2.
 //
 // Choices are ordered as they compare in 64 bits: neighbours in the order may differ by less than
 // 32 bits hold.  A token is first ranked in 32 bits; where every difference that decides exceeds
@@ -596,7 +598,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_gate_bwd(GateArgs a, const int64
   const int64_t e = mine ? idx[t * a.k + sub] : 0;
   const bool there = mine && e >= 0 && e < a.E;
   const float ze = there ? load_elem(a.logits, DT, t * a.ldl + e) : 0.0f;
-  const float g = there ? gw[t * a.k + sub] * a.scale : 0.0f;
+  const float g = there ? gw[t * a.k + sub] : 0.0f;
   float z[EPL], s[EPL], ds[EPL];
   load_row<DT, EPL>(a.logits, t * a.ldl, e0, a.E, -__builtin_inff(), z);
   if (gs) {
@@ -605,14 +607,25 @@ __global__ __launch_bounds__(64 * WAVES) void k_gate_bwd(GateArgs a, const int64
 #pragma unroll
     for (int j = 0; j < EPL; ++j) ds[j] = 0.0f;
   }
-  float top, zmax, inv;
-  scores<LANES, EPL>(a.score, z, s, top, zmax, inv);
+  float top, zmax = 0.0f, inv = 1.0f;
+  if (a.score == kSoftmax) {
+    scores<LANES, EPL>(kSoftmax, z, s, top, zmax, inv);
+  } else {  // s (1 - s)
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) {
+      const float t = exp_of(-fabsf(z[j])), r = __builtin_amdgcn_rcpf(1.0f + t);
+      s[j] = t * r * r;
+    }
+  }
   if (gw) {
     const float se = there ? (a.score == kSigmoid ? sigmoid_of(ze) : exp_of(ze - zmax) * inv) : 0.0f;
-    float d = g;
+    float d = g * a.scale;
     if (a.renormalize) {
       const float total = lanes_sum<LANES>(se) + (float)kEps;
-      d = (g - lanes_sum<LANES>(g * se) / total) / total;
+      const int first = lane & ~(LANES - 1);
+      d = (float)kEps * g;
+      for (int i = 0; i < a.k; ++i) d += (g - __shfl(g, first + i)) * __shfl(se, first + i);
+      d = d / total / total * a.scale;
     }
 #pragma unroll
     for (int j = 0; j < EPL; ++j) place[slot][e0 + j] = 0.0f;
@@ -631,7 +644,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_gate_bwd(GateArgs a, const int64
     for (int j = 0; j < EPL; ++j) ds[j] = s[j] * (ds[j] - u);
   } else {
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) ds[j] = ds[j] * s[j] * (1.0f - s[j]);
+    for (int j = 0; j < EPL; ++j) ds[j] *= s[j];
   }
   if (!live) return;
   constexpr int es = DT == CIN_DT_F32 ? 4 : 2;

@@ -391,6 +391,42 @@ def test_gate_groups_that_64_bits_cannot_tell_apart(dev, E, G):
         assert moe.moe_gate(logits[t:t + 1], 2, n_groups=G, top_groups=2, group_top=1)[0].div(n, rounding_mode="floor").tolist() == [[0, 1]]
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("E", [8, 48, 256, 1500])
+def test_gate_gradient_of_saturated_sigmoids(dev, E):
+    """s (1 - s) = t / (1 + t)^2, t = e^-|z|, to the last bits also where s is next to 1.  t is within
+    4 u, 1 + t and its reciprocal within 4 u more, so the factor within 4 + 2 * 5 + 2 u of itself, twice
+    that here; a term of the weights' gradient is a sum over k of (gw_j - gw_i) s_i with errors of 8 u in
+    the scores, 8 in the total and its square, 2 k in the sums."""
+    g = torch.Generator().manual_seed(16)
+    z = (torch.rand(200, E, generator=g) * 60 - 30).to(dev)
+    gs = torch.randn(200, E, generator=g).to(dev)
+    zd = z.double()
+    t = torch.exp(-zd.abs())
+    factor = t / (1 + t) ** 2
+    leaf = z.clone().requires_grad_(True)
+    s = moe.moe_gate(leaf, 2, return_scores=True)[2]
+    (dz,) = torch.autograd.grad(s, [leaf], gs)
+    want = gs.double() * factor
+    assert ((dz.double() - want).abs() <= 32 * U * want.abs() + 1e-37).all()
+    for k in (1, 2, min(8, E)):
+        gw = torch.randn(200, k, generator=g).to(dev)
+        for renormalize, scale in ((True, 1.0), (True, 2.5), (False, 1.0)):
+            idx, w = moe.moe_gate(leaf, k, renormalize=renormalize, scale=scale)
+            (dz,) = torch.autograd.grad(w, [leaf], gw)
+            at = (1 / (1 + torch.exp(-zd))).gather(1, idx)
+            gd = gw.double() * scale
+            ds, size = gd, gd.abs()
+            if renormalize:
+                total = at.sum(1, keepdim=True) + 1e-9
+                apart = gd[:, :, None] - gd[:, None, :]
+                ds = ((apart * at[:, None]).sum(2) + 1e-9 * gd) / total ** 2
+                size = ((apart.abs() * at[:, None]).sum(2) + 1e-9 * gd.abs()) / total ** 2
+            want = torch.zeros_like(zd).scatter(1, idx, ds * factor.gather(1, idx))
+            tol = torch.zeros_like(zd).scatter(1, idx, 2 * (32 + 2 * k) * U * size * factor.gather(1, idx)) + 1e-37
+            assert ((dz.double() - want).abs() <= tol).all(), (k, renormalize)
+
+
 def _fake(*shape, dtype=torch.float32):
     return torch.empty(*shape, dtype=dtype, device="cuda")
 
