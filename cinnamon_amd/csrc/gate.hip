@@ -11,8 +11,8 @@
 // backward, with gw and gs the gradients of w and s:
 //   ds     = gs;  ds[idx_j] += scale * (gw_j - sum_i gw_i s[idx_i] / total) / total
 //   dz     = ds s (1 - s)  or  s (ds - sum_e ds_e s_e)
-// without the differences that cancel: s (1 - s) = t / (1 + t)^2 with t = e^-|z|, and the weights' term
-// is scale * (1e-9 gw_j + sum_i (gw_j - gw_i) s[idx_i]) / total^2.
+// without the differences that cancel: s (1 - s) = t / (1 + t)^2 with t = e^-|z|, a softmax's ds less one
+// of them, and the weights' term is scale * (1e-9 gw_j + sum_i (gw_j - gw_i) s[idx_i]) / total^2.
 //
 // Choices are ordered as they compare in 64 bits: neighbours in the order may differ by less than
 // 32 bits hold.  A token is first ranked in 32 bits; where every difference that decides exceeds
@@ -636,12 +636,16 @@ __global__ __launch_bounds__(64 * WAVES) void k_gate_bwd(GateArgs a, const int64
     for (int j = 0; j < EPL; ++j) ds[j] += place[slot][e0 + j];
   }
   if (a.score == kSoftmax) {
-    float u = 0.0f;
+    // less the largest score's ds, which the sum of the scores, 1, leaves the same: its own term cancels
+    float c = -__builtin_inff(), u = 0.0f;
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) u += e0 + j < a.E ? ds[j] * s[j] : 0.0f;
+    for (int j = 0; j < EPL; ++j) c = z[j] == zmax ? fmaxf(c, ds[j]) : c;
+    c = lanes_max_nan<LANES>(c);
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) u += e0 + j < a.E ? (ds[j] - c) * s[j] : 0.0f;
     u = lanes_sum<LANES>(u);
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) ds[j] = s[j] * (ds[j] - u);
+    for (int j = 0; j < EPL; ++j) ds[j] = s[j] * (ds[j] - c - u);
   } else {
 #pragma unroll
     for (int j = 0; j < EPL; ++j) ds[j] *= s[j];

@@ -427,6 +427,34 @@ def test_gate_gradient_of_saturated_sigmoids(dev, E):
             assert ((dz.double() - want).abs() <= tol).all(), (k, renormalize)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
+@pytest.mark.parametrize("E", [8, 48, 256, 1500])
+def test_gate_gradient_of_saturated_softmaxes(dev, dt, E):
+    """s_j (ds_j - sum_e ds_e s_e) = s_j sum_e (ds_j - ds_e) s_e, also where one s is next to 1.  With c the
+    gradient of the largest score's ds, the terms are |ds_e - c| s_e and |ds_j - c|, each off by a score's
+    bound (8 u and the sum's E / 64 + 6), the sum's and two roundings more; twice that here."""
+    g = torch.Generator().manual_seed(17)
+    z = torch.randn(200, E, generator=g)
+    z[torch.arange(200), torch.randint(0, E, (200,), generator=g)] += torch.rand(200, generator=g) * 60
+    z[7] = 0.0                                             # all equal
+    z = z.to(DT[dt]).to(dev)
+    gs = (torch.randn(200, E, generator=g) + 3).to(dev)
+    leaf = z.clone().requires_grad_(True)
+    s = moe.moe_gate(leaf, 2, score="softmax", return_scores=True)[2]
+    (dz,) = torch.autograd.grad(s, [leaf], gs)
+    p, d = torch.softmax(z.double(), 1), gs.double()
+    top = p.argmax(1, keepdim=True)
+    c = d.gather(1, top)
+    v = ((d - c) * p).sum(1, keepdim=True)
+    want = p * (d - c - v)
+    # (with several largest scores c is one of theirs: the largest difference of them more)
+    same = torch.where(p == p.gather(1, top), (d - c).abs(), 0).amax(1, keepdim=True)
+    size = p * ((d - c).abs() + ((d - c).abs() * p).sum(1, keepdim=True) + 2 * same)
+    tol = 2 * (2 * (8 + E / 64 + 6) + 8) * U * size + 1e-37 + {"fp32": 0, "bf16": 2.0 ** -8}[dt] * want.abs()
+    assert ((dz.double() - want).abs() <= tol).all()
+
+
 def _fake(*shape, dtype=torch.float32):
     return torch.empty(*shape, dtype=dtype, device="cuda")
 
