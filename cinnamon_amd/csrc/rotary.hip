@@ -141,12 +141,12 @@ __global__ __launch_bounds__(kThreads) void k_rotary(RotaryArgs a) {
   int64_t out[kUnits];
   int at0[kUnits], at1[kUnits];
   float cs[kUnits][kPairs], sn[kUnits][kPairs];
-  bool live[kUnits], turns[kUnits], second[kUnits];
+  bool live[kUnits], turns[kUnits], second[kUnits], still[kUnits];  // still: padding, kept bit for bit
 #pragma unroll
   for (int j = 0; j < kUnits; ++j) {
     const uint32_t local = j * kThreads + threadIdx.x;
     live[j] = first + local < a.n;
-    turns[j] = false;
+    turns[j] = still[j] = false;
     if (!live[j]) continue;
     const uint32_t i = rem0 + local, dt = div_by(i, a.row, a.mrow), r = i - dt * a.row;
     const uint32_t h = div_by(r, a.units, a.munits), u = r - h * a.units;
@@ -194,23 +194,20 @@ __global__ __launch_bounds__(kThreads) void k_rotary(RotaryArgs a) {
     if (!turns[j]) continue;
     if constexpr (kTwo) c1[j].load(x, in + at1[j]);
     const int64_t p = a.positions ? a.positions[b0 * a.pb + l0 * a.pl + pos] : l;
-    const bool known = p >= 0 && p < a.P;
-    if (known) {
+    still[j] = p < 0;
+    if (p >= 0 && p < a.P) {
       load_pairs(a.cos + p * a.ldt + (int)u * kPairs, cs[j]);
       load_pairs(a.sin + p * a.ldt + (int)u * kPairs, sn[j]);
     } else {
 #pragma unroll
-      for (int e = 0; e < kPairs; ++e) {
-        cs[j][e] = p < 0 ? 1.0f : __builtin_nanf("");
-        sn[j][e] = p < 0 ? 0.0f : __builtin_nanf("");
-      }
+      for (int e = 0; e < kPairs; ++e) cs[j][e] = sn[j][e] = __builtin_nanf("");
     }
   }
 #pragma unroll
   for (int j = 0; j < kUnits; ++j) {
     if (!live[j]) continue;
     void* y = second[j] ? a.k.y : a.q.y;
-    if (turns[j]) {
+    if (turns[j] && !still[j]) {
       float v0[E], v1[E];
       c0[j].widen(v0);
       if constexpr (kTwo) c1[j].widen(v1);
@@ -224,10 +221,10 @@ __global__ __launch_bounds__(kThreads) void k_rotary(RotaryArgs a) {
         x1 = y1;
       }
       c0[j].round(v0);
-      if constexpr (kTwo) {
-        c1[j].round(v1);
-        c1[j].store(y, out[j] + at1[j]);
-      }
+      if constexpr (kTwo) c1[j].round(v1);
+    }
+    if constexpr (kTwo) {
+      if (turns[j]) c1[j].store(y, out[j] + at1[j]);
     }
     c0[j].store(y, out[j] + at0[j]);
   }

@@ -150,6 +150,36 @@ def test_rotary_padding_and_positions_past_the_table(dev, inter, dt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("inter", [True, False])
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("D,start,rot", [(48, 8, 32), (33, 3, 6), (64, 0, 64)])
+def test_rotary_padding_may_hold_anything(dev, inter, dt, D, start, rot):
+    """A token at a negative position keeps its bits, infinities, NaN and the zeros' signs among them,
+    and so does its gradient."""
+    g = torch.Generator().manual_seed(4)
+    cos, sin = rotary.rotary_tables(rot, 10, device=dev)
+    x = torch.randn(2, 6, 3, D, generator=g).to(DT[dt])
+    odd = torch.tensor([math.inf, -math.inf, math.nan, 0.0, -0.0, 1.0, torch.finfo(DT[dt]).max, 1e-30]).to(DT[dt])
+    x[:, ::2] = odd[torch.randint(0, len(odd), x[:, ::2].shape, generator=g)]
+    x = x.to(dev)
+    p = torch.tensor([[-1, 9, -7, 3, -(2 ** 40), 0], [-1, -1, -2, 5, -(2 ** 62), 2]], device=dev)
+    bits = {2: torch.int16, 4: torch.int32}[x.element_size()]
+    for k in (None, x[:, :, :1]):
+        leaf = x.clone().requires_grad_(True)
+        out = rotary.apply_rotary(leaf, cos, sin, k=k, positions=p, interleaved=inter, start=start)
+        got = out if k is None else out[0]
+        (d,) = torch.autograd.grad(got, [leaf], x)
+        for y in (got.detach(), d):
+            assert torch.equal(y[p < 0].view(bits), x[p < 0].view(bits))
+        if k is not None:
+            assert torch.equal(out[1][p < 0].view(bits), x[:, :, :1][p < 0].view(bits))
+    rest = (p >= 0) & torch.isfinite(x.float()).all(-1).all(-1)
+    y, mag = turn(torch.where(rest[..., None, None], x, 0), cos, sin, p, inter, start)
+    rest = rest.cpu()
+    check(got.detach().cpu()[rest], (y[rest], mag[rest]), dt)
+
+
+@pytest.mark.gpu
 def test_rotary_empty(dev):
     cos, sin = rotary.rotary_tables(32, 10, device=dev)
     for shape in ((0, 5, 2, 64), (2, 0, 2, 64), (2, 5, 0, 64)):
