@@ -563,10 +563,11 @@ __global__ __launch_bounds__(C::kThreads, 2) void k_ce_gemm(GemmArgs g) {
 // ---------------------------------------------------------------------------
 constexpr int kRowPer = 8;  // targets a thread looks at together
 
-// The int32 state: the rows that count, workgroups that are done, and T entries each of map, pos, target.
+// The int32 state: the rows that count, workgroups that are done, whether logits were mended, and T entries
+// each of map, pos, target.
 struct IntState {
-  int *n, *done, *map, *pos, *target;
-  IntState(int32_t* p, int64_t T) : n(p), done(p + 1), map(p + 4), pos(map + T), target(pos + T) {}
+  int *n, *done, *mended, *map, *pos, *target;
+  IntState(int32_t* p, int64_t T) : n(p), done(p + 1), mended(p + 2), map(p + 4), pos(map + T), target(pos + T) {}
 };
 
 // The rows that count, in order: map[i] the row, target[i] its target (-1 outside the vocabulary),
@@ -621,6 +622,7 @@ __device__ __forceinline__ int find_rows(const int64_t* __restrict__ y, int64_t 
   if (write && tid == 0) {
     *st.n = base;
     *st.done = 0;
+    *st.mended = 0;
   }
   return base;
 }
@@ -628,6 +630,16 @@ __device__ __forceinline__ int find_rows(const int64_t* __restrict__ y, int64_t 
 __global__ __launch_bounds__(1024) void k_ce_rows(const int64_t* __restrict__ y, int64_t T, int64_t V, int64_t ignore,
                                                   IntState st, float* __restrict__ rowloss) {
   find_rows<1024>(y, T, V, ignore, st, rowloss, true, nullptr);
+}
+
+// The next bf16 part of a value, which is taken off it.  A finite value has finite parts (one within half a
+// step of 2^128 would round to infinity); an infinity is its own first part and leaves 0.
+__device__ __forceinline__ uint32_t take_part(float& v) {
+  uint32_t b = f32_to_bf16_bits(v);
+  const bool inf = (b & 0x7fff) == 0x7f80;
+  if (inf && fabsf(v) < __builtin_inff()) --b;
+  v = inf && !(fabsf(v) < __builtin_inff()) ? 0.0f : v - __uint_as_float(b << 16);
+  return b;
 }
 
 // Rows of x (all, or map's first *n) with zeros up to Dp columns, as operands of DT.
@@ -649,14 +661,10 @@ __device__ __forceinline__ void copy_piece(const void* __restrict__ x, int64_t l
   } else if constexpr (DT == CIN_DT_F32) {
 #pragma unroll
     for (int p = 0; p < 3; ++p) {
-      v4u h;
+      uint32_t h[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        h[e] = f32x2_to_bf16x2_bits(v[2 * e], v[2 * e + 1]);
-        v[2 * e] -= bf16_lo(h[e]);
-        v[2 * e + 1] -= bf16_hi(h[e]);
-      }
-      *reinterpret_cast<v4u*>(d + p * plane) = h;
+      for (int e = 0; e < 8; ++e) h[e] = take_part(v[e]);
+      *reinterpret_cast<v4u*>(d + p * plane) = v4u{h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16};
     }
   } else {
     __builtin_memcpy(__builtin_assume_aligned(d, 16), v, 16);
@@ -711,11 +719,66 @@ __device__ __forceinline__ void add_losses(const float* rowloss, int64_t T, int 
   if (threadIdx.x == 0) *loss = (float)(mean ? sum / n : sum);
 }
 
+// The product of rows m of x and n of w that are held in parts, by a wave.
+__device__ inline float product_of_parts(const GemmArgs& g, int64_t m, int64_t n, int lane) {
+  const uint8_t* x = static_cast<const uint8_t*>(g.A) + m * g.lda * 2;
+  const uint8_t* w = static_cast<const uint8_t*>(g.B) + n * g.ldb * 2;
+  double s = 0;
+  for (int64_t c = lane * 2; c < g.K; c += 128) {
+    float a[2] = {0.f, 0.f}, b[2] = {0.f, 0.f};
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+      const uint32_t u = *reinterpret_cast<const uint32_t*>(x + p * g.plane_a + c * 2);
+      const uint32_t v = *reinterpret_cast<const uint32_t*>(w + p * g.plane_b + c * 2);
+      a[0] += bf16_lo(u);
+      a[1] += bf16_hi(u);
+      b[0] += bf16_lo(v);
+      b[1] += bf16_hi(v);
+    }
+    s += (double)a[0] * b[0] + (double)a[1] * b[1];
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) s += __shfl_xor(s, o);
+  return (float)s;
+}
+
+// Six products of parts make NaN of an infinity: it meets parts of 0 and of either sign.  (So does a sum
+// that leaves the range on its way.)  Where a tile's sum is NaN its logits are formed again from whole
+// values, here for the statistics and in k_ce_mend for dz: -inf masks an entry of the vocabulary for fp32
+// as it does for 16 bits.  Maximum and sum of row i's such tiles, NaN where the row has a logit that is
+// NaN or +inf, at the first of them; its target's logit if it is theirs.
+__device__ inline float2 mended_tiles(const GemmArgs& g, const float2* __restrict__ part, int tiles, int tile_n, int64_t i,
+                                      int target, int lane, float& ztarget) {
+  float m = -__builtin_inff(), s = 0.0f;
+  for (int t = 0; t < tiles; ++t) {
+    const float y = part[i * tiles + t].y;
+    if (y == y) continue;
+    const int64_t end = (int64_t)(t + 1) * tile_n < g.V ? (int64_t)(t + 1) * tile_n : g.V;
+    for (int64_t v = (int64_t)t * tile_n; v < end; ++v) {
+      const float z = product_of_parts(g, i, v, lane);
+      if (!(z < __builtin_inff())) return make_float2(__builtin_nanf(""), __builtin_nanf(""));
+      if (v == target) ztarget = z;
+      if (z == -__builtin_inff()) continue;
+      if (z > m) {
+        s = s * exp_of(m - z) + 1.0f;
+        m = z;
+      } else {
+        s += exp_of(z - m);
+      }
+    }
+  }
+  return make_float2(m, s);
+}
+
 // A wave per row: the tiles' maxima and sums joined, the row's loss (NaN for a target outside the
 // vocabulary).  With `loss`, for few rows, the workgroup that ends last adds them up; for more a
 // launch of its own does, as each workgroup's fence costs more than it (4096 rows: 34 us of forward
 // with the launch, 107 without).
-__global__ __launch_bounds__(256) void k_ce_join(const float2* __restrict__ part, int tiles, int64_t T, IntState st,
+// PARTS: operands are held in parts, tile_n columns a tile.
+struct NoArgs {};
+template <bool PARTS>
+__global__ __launch_bounds__(256) void k_ce_join(std::conditional_t<PARTS, GemmArgs, NoArgs> g, int tile_n,
+                                                 const float2* __restrict__ part, int tiles, int64_t T, IntState st,
                                                  const float* __restrict__ ztarget, float* __restrict__ rowmax,
                                                  float* __restrict__ inv, float* __restrict__ rest,
                                                  float* __restrict__ rowloss, int mean,
@@ -723,18 +786,40 @@ __global__ __launch_bounds__(256) void k_ce_join(const float2* __restrict__ part
   const int lane = threadIdx.x & 63, n = *st.n;
   const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (i < n) {
-    float m = -__builtin_inff(), s = 0.0f;
-    for (int t = lane; t < tiles; t += 64) m = fmaxf(m, part[i * tiles + t].x);
+    float m = -__builtin_inff(), s = 0.0f, zt = 0.0f;
+    bool mend = false;
+    float2 more;
+    if constexpr (PARTS) {
+      zt = ztarget[i];
+      for (int t = lane; t < tiles; t += 64) {
+        const float2 p = part[i * tiles + t];
+        if (p.y == p.y)
+          m = fmaxf(m, p.x);
+        else
+          mend = true;
+      }
+      mend = __ballot(mend) != 0;
+      if (mend) {
+        more = mended_tiles(g, part, tiles, tile_n, i, st.target[i], lane, zt);
+        m = fmaxf(m, more.x);
+      }
+    } else {
+      for (int t = lane; t < tiles; t += 64) m = fmaxf(m, part[i * tiles + t].x);
+    }
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
     for (int t = lane; t < tiles; t += 64) {
       const float2 p = part[i * tiles + t];
-      s += p.y * exp_of(p.x - m);
+      if (!mend || p.y == p.y) s += p.y * exp_of(p.x - m);
     }
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) s += __shfl_xor(s, o);
+    if (mend) {
+      s += more.y * exp_of(more.x - m);
+      if (lane == 0 && s == s) *st.mended = 1;
+    }
     if (lane == 0) {
-      const float loss_i = st.target[i] < 0 ? __builtin_nanf("") : (m - ztarget[i]) + logf(s);
+      const float loss_i = st.target[i] < 0 ? __builtin_nanf("") : (m - (PARTS ? zt : ztarget[i])) + logf(s);
       rowmax[i] = m;
       inv[i] = 1.0f / s;
       rest[i] = -expm1f(-loss_i);
@@ -870,6 +955,29 @@ __global__ __launch_bounds__(256) void k_ce_coef_few(const float* __restrict__ g
     }
     *reinterpret_cast<v4u*>(scaled + at) = hi;
     *reinterpret_cast<v4u*>(scaled + plane + at) = lo;
+  }
+}
+
+// dz of the logits that are formed again (see mended_tiles), as kGrad's: a wave looks at 64 columns of a row.
+__global__ __launch_bounds__(256) void k_ce_mend(GemmArgs g, const int* __restrict__ mended) {
+  if (!*mended) return;
+  const int lane = threadIdx.x & 63;
+  const int64_t cols = g.N < g.V - g.v0 ? g.N : g.V - g.v0, chunks = cdiv(cols, 64), total = *g.n * chunks;
+  for (int64_t q = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); q < total; q += (int64_t)gridDim.x * 4) {
+    const int64_t i = q / chunks, c0 = (q - i * chunks) * 64;
+    const float mx = g.rowmax[i], inv = g.inv[i], cf = g.coef[i], pc = inv * cf;
+    if (!(pc == pc)) continue;  // the row's own loss or gradient is NaN
+    uint16_t* d = static_cast<uint16_t*>(g.C) + i * g.ldc + c0 + lane;
+    uint64_t nans = __ballot(c0 + lane < cols && (*d & 0x7fff) > 0x7f80);
+    for (; nans; nans &= nans - 1) {
+      const int at = __builtin_ctzll(nans);
+      const float z = product_of_parts(g, i, c0 + at, lane);
+      float v = exp_of(z - mx) * pc - (g.target[i] == g.v0 + c0 + at ? cf : 0.0f);
+      if (lane == at) {
+#pragma unroll
+        for (int p = 0; p < 3; ++p) d[p * g.slab] = (uint16_t)take_part(v);
+      }
+    }
   }
 }
 
@@ -1154,6 +1262,7 @@ int cin_linear_ce_forward(const void* x, int dtype, int64_t T, int64_t D, int64_
   float* zt = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.part);
   if (T == 0 || T > kFewRows)
     hipLaunchKernelGGL(k_ce_rows, 1, 1024, 0, s, target, T, V, ignore_index, st, rowloss);
+  GemmArgs g{};
   if (T > 0) {
     if (T > kFewRows) {
       copy_rows(p.op, x, ldx, T, D, st.map, st.n, xc, p.Dp, s);
@@ -1165,7 +1274,6 @@ int cin_linear_ce_forward(const void* x, int dtype, int64_t T, int64_t D, int64_
       });
     }
     if (wp) copy_rows(p.op, w, ldw, V, D, nullptr, nullptr, wp, p.Dp, s);
-    GemmArgs g{};
     g.A = xc;
     g.lda = p.Dp;
     g.B = wp ? wp : w;
@@ -1183,8 +1291,14 @@ int cin_linear_ce_forward(const void* x, int dtype, int64_t T, int64_t D, int64_
     gemm<kStats>(p.op, p.tile, g, T, 1, s);
   }
   // (without rows one workgroup: the sum of none)
-  hipLaunchKernelGGL(k_ce_join, (unsigned)(T > 0 ? cdiv(T, 4) : 1), 256, 0, s, part, (int)p.tiles_n, T, st, zt, state_f,
-                     state_f + T, state_f + 2 * T, rowloss, mean, T <= kJoinAlone ? loss : nullptr);
+  const unsigned rows4 = (unsigned)(T > 0 ? cdiv(T, 4) : 1);
+  float* here = T <= kJoinAlone ? loss : nullptr;
+  if (p.planes > 1)
+    hipLaunchKernelGGL(k_ce_join<true>, rows4, 256, 0, s, g, kTileN[p.tile], part, (int)p.tiles_n, T, st, zt, state_f, state_f + T,
+                       state_f + 2 * T, rowloss, mean, here);
+  else
+    hipLaunchKernelGGL(k_ce_join<false>, rows4, 256, 0, s, NoArgs{}, 0, part, (int)p.tiles_n, T, st, zt, state_f, state_f + T,
+                       state_f + 2 * T, rowloss, mean, here);
   if (loss && T > kJoinAlone) hipLaunchKernelGGL(k_ce_loss, 1, 1024, 0, s, rowloss, T, st.n, mean, loss);
   return cin_check_launch(name);
 }
@@ -1255,6 +1369,7 @@ int cin_linear_ce_backward(const void* xc, int dtype, int64_t T, int64_t D, cons
       });
     } else {
       gemm<kGrad>(p.op, pick_tile(p.op, T, g.N), g, T, 1, s);
+      if (p.planes > 1) hipLaunchKernelGGL(k_ce_mend, 1024, 256, 0, s, g, st.mended);
     }
     GemmArgs h{};
     h.n = st.n;

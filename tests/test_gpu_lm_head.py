@@ -459,6 +459,78 @@ def test_a_model_step_with_tied_heads(dev):
         assert (a - b).norm() <= 12 * math.sqrt(1000) * U * b.norm()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("T,V,D", [(16, 700, 64), (128, 1500, 96), (129, 1500, 96), (300, 3001, 130), (2100, 900, 64)])
+@pytest.mark.parametrize("value", ["lowest", "-inf"])
+def test_masked_entries_of_the_vocabulary(dev, dt, T, V, D, value):
+    """Entries whose weight holds the type's lowest value or -inf at a constant feature: as if the
+    vocabulary had no such entries, at any number of rows.  With -inf, 0 * inf makes that feature's gradient of x NaN."""
+    low = -math.inf if value == "-inf" else torch.finfo(DT[dt]).min
+    x, w, y, g = make(T, V, D, dt, 0.1, dev)
+    x[:, 5] = 1.0
+    gone = torch.zeros(V, dtype=torch.bool)
+    gone[torch.randperm(V, generator=g)[:9]] = True
+    gone[-1] = True
+    gone[y[y >= 0].cpu()] = False
+    assert gone.any()
+    gone = gone.to(dev)
+    w[gone, 5] = low
+    y2 = torch.where(y >= 0, torch.cumsum(~gone, 0)[y.clamp(min=0)] - 1, y)
+    grad = torch.randn(T, generator=g).to(dev)
+    (loss, ltol), (dx, dxt), (dw, dwt) = reference(x, w[~gone], y2, reduction="none", grad=grad)
+    xl, wl = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    with torch.no_grad():
+        plain = lm_head.linear_cross_entropy(x, w, y, reduction="none")
+    got = lm_head.linear_cross_entropy(xl, wl, y, reduction="none")
+    assert torch.isfinite(got).all() and torch.equal(plain, got.detach())
+    assert ((got.detach().double() - loss).abs() <= ltol).all()
+    a, b = torch.autograd.grad(got, [xl, wl], grad)
+    assert (b[gone] == 0).all()
+    near(b[~gone], dw, dwt, dt, T + D)
+    if value == "-inf":
+        assert torch.isnan(a[y >= 0][:, 5]).all()
+        keep = torch.arange(D, device=dev) != 5
+        a, dx, dxt = a[:, keep], dx[:, keep], dxt[:, keep]
+    near(a, dx, dxt, dt, V + D)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [100, 200])
+def test_infinities_of_fp32_rows(dev, T):
+    """What an infinity or NaN makes of a row's loss does not depend on the number of rows: one row of x
+    holds it, the others' losses and gradients stay."""
+    x, w, y, g = make(T, 1000, 72, "fp32", 0.0, dev)
+    w[:, 7] = w[:, 7].abs() + 0.1
+    w[0, 7] = 0.2
+    want = lm_head.linear_cross_entropy(x, w, y, reduction="none")
+    for value, loss in ((math.inf, "nan"), (-math.inf, "nan"), (math.nan, "nan"), (torch.finfo(torch.float32).max, "any")):
+        z = x.clone()
+        z[3, 7] = value
+        leaf, wl = z.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        got = lm_head.linear_cross_entropy(leaf, wl, y, reduction="none")
+        others = torch.arange(T, device=dev) != 3
+        assert torch.equal(got[others].detach(), want[others])
+        if loss == "nan":
+            assert torch.isnan(got[3])
+        (dx,) = torch.autograd.grad(got[others].sum(), [leaf])
+        assert torch.isfinite(dx[others]).all()
+    # every entry of the vocabulary at -inf for a row: 0 / 0, as in the softmax itself
+    z = x.clone()
+    z[3, 7] = -math.inf
+    assert torch.isnan(lm_head.linear_cross_entropy(z, w, y, reduction="none")[3])
+    # a target at -inf: its loss is inf, and the gradient pushes away from all the others
+    v = w.clone()
+    x[:, 5] = 1.0
+    v[y[0], 5] = -math.inf
+    leaf = v.requires_grad_(True)
+    rows = lm_head.linear_cross_entropy(x, leaf, y, reduction="none")
+    of = y == y[0]
+    assert torch.isposinf(rows[of]).all() and torch.isfinite(rows[~of]).all()
+    (dw,) = torch.autograd.grad(rows.sum(), [leaf])
+    assert torch.isfinite(dw).all()
+
+
 def test_refusals():
     with FakeTensorMode():
         def fake(*shape, dtype=torch.bfloat16):
