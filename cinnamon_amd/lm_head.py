@@ -4,7 +4,8 @@ The reference keeps lm_head out of FP8 (src/kernels.py:863-867) and trains on
 cross_entropy(lm_head(x), targets) for the main and the MTP heads (src/train.py:355-372), which
 writes the logits [n_tokens, vocabulary], their log-softmax and its gradient.
 ``linear_cross_entropy`` computes loss and gradients by pieces of the vocabulary on bf16, fp16 or
-fp32 matrix units (csrc/lm_head.hip) without ever keeping the logits.
+fp32 matrix units (csrc/lm_head.hip); only those of few rows of a wide model, fewer bytes than the
+weight, are ever kept.
 """
 from __future__ import annotations
 
@@ -22,7 +23,7 @@ __all__ = ["linear_cross_entropy"]
 _PLAIN = (torch.Tensor, torch.nn.Parameter)
 _MODES = {"none": 0, "sum": 1, "mean": 2}
 _DIRECT_ROWS = 128  # up to which fp32 is multiplied as it is (csrc/lm_head.hip kDirectRows)
-_KEEP_ROWS = 128    # up to which the logits are kept: fewer bytes than the weight that gives them again
+_KEEP_ROWS = 128    # up to which the logits may be kept for the backward
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
@@ -38,8 +39,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     to 256 rows scaled so that the targets' entries are exact.
     fp32 inputs are multiplied as three bf16 parts each, to the accuracy of fp32 products (up to 128
     rows as they are).
-    Results do not vary from call to call.  The backward recomputes the logits piece by piece (up to
-    128 rows keep them): beside the inputs it keeps one copy of the rows that count (fp32 of more than
+    Results do not vary from call to call.  The backward recomputes the logits piece by piece (those of
+    up to 128 rows are kept where they are at most half the weight's bytes): beside the inputs it keeps one copy of the rows that count (fp32 of more than
     128 rows: 1.5 times their size, and the weight's; a weight whose width is no multiple of 64: a
     padded copy) and a few words a row, and works in up to about 1 GiB for a piece of the logits'
     gradient plus fp32 sums of x's."""
@@ -69,6 +70,14 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     return loss.view(target.shape) if mode == 0 and target.ndim != 1 else loss
 
 
+def _keeps(T, D, dtype):
+    """Whether the backward reads logits that the forward kept: where writing and reading them, 8 T bytes a
+    column, moves no more than reading the weight again (131072 columns, bf16, forward and gradients: 128 x 128
+    169 us kept and 152 formed again, 128 x 512 188 and 188, 128 x 1024 334 and 351, 16 x 512 143 and 156; fp32 gains
+    up to there and loses 4% at most beyond: 128 x 128 252 and 261, 128 x 1024 908 and 1129)."""
+    return T <= _KEEP_ROWS and 8 * T <= D * dtype.itemsize
+
+
 def _layout(T, D, V, dtype):
     """Bytes of the state that the forward leaves: its rows that count, the weight's copy, integers
     and floats (csrc/lm_head.hip), for few rows the logits, each from a multiple of 256 on.  Operands are padded to whole K
@@ -80,7 +89,7 @@ def _layout(T, D, V, dtype):
     copied = planes == 3 or Dp != D
     offsets, at = [], 0
     for n in (planes * T * Dp * es, planes * V * Dp * es if copied else 0, 4 * (4 + 3 * T), 12 * T,
-              4 * T * _cdiv(V, 64) * 64 if T <= _KEEP_ROWS else 0):
+              4 * T * _cdiv(V, 64) * 64 if _keeps(T, D, dtype) else 0):
         offsets.append(at)
         at += _cdiv(n, 256) * 256
     return offsets, at, copied
@@ -127,7 +136,7 @@ def _launch_forward(x, weight, target, ignore_index, mode, keep=True):
     at = state.data_ptr()
     call_on(x, "cin_linear_ce_forward", x.data_ptr(), dtype_code(x), T, D, _pitch(x), w.data_ptr(), V, _pitch(w),
             target.data_ptr(), ignore_index, mode == 2, at + xc, at + wp if copied else 0, at + si, at + sf,
-            rows.data_ptr(), loss.data_ptr() if mode else 0, work.data_ptr(), ws, at + sz if keep and T <= _KEEP_ROWS else 0,
+            rows.data_ptr(), loss.data_ptr() if mode else 0, work.data_ptr(), ws, at + sz if keep and _keeps(T, D, x.dtype) else 0,
             stream_of(x))
     return loss, state
 
@@ -149,7 +158,7 @@ def _launch_backward(grad, state, weight, T, mode, need_x, need_w):
         w, ldw = weight.data_ptr(), _pitch(weight)
     work = torch.empty(ws, dtype=torch.uint8, device=weight.device)
     call_on(weight, "cin_linear_ce_backward", at + xc, dtype_code(dtype), T, D, w, V, ldw, at + si, at + sf, grad.data_ptr(),
-            0 if mode else grad.stride(0), mode == 2, ptr(dx), ptr(dw), work.data_ptr(), ws, at + sz if T <= _KEEP_ROWS else 0, stream_of(weight))
+            0 if mode else grad.stride(0), mode == 2, ptr(dx), ptr(dw), work.data_ptr(), ws, at + sz if _keeps(T, D, dtype) else 0, stream_of(weight))
     return dx, dw
 
 

@@ -531,6 +531,46 @@ def test_infinities_of_fp32_rows(dev, T):
     assert torch.isfinite(dw).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("T,V,D", [(1, 777, 40), (32, 3001, 128), (100, 1500, 64), (128, 2049, 300)])
+def test_kept_logits_and_logits_formed_again(dev, monkeypatch, dt, T, V, D):
+    """Either way gives the gradients; the same ones where the logits are summed in the same order."""
+    x, w, y, g = make(T, V, D, dt, 0.1, dev)
+    grad = torch.randn(T, generator=g).to(dev)
+    _, (dx, dxt), (dw, dwt) = reference(x, w, y, reduction="none", grad=grad)
+    losses = []
+    for kept in (True, False):
+        monkeypatch.setattr(lm_head, "_keeps", lambda T, D, dtype: kept)
+        lm_head._sizes.cache_clear()
+        xl, wl = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        loss = lm_head.linear_cross_entropy(xl, wl, y, reduction="none")
+        a, b = torch.autograd.grad(loss, [xl, wl], grad)
+        near(a, dx, dxt, dt, V + D)
+        near(b, dw, dwt, dt, T + D)
+        losses.append(loss.detach())
+    lm_head._sizes.cache_clear()
+    assert torch.equal(*losses)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+def test_kept_logits_are_fewer_bytes_than_the_weight(dt):
+    """Written and read they are no more than the weight that gives them again."""
+    dtype, es = DT[dt], DT[dt].itemsize
+    V = 131072
+    for D in (8, 64, 128, 256, 512, 1024, 4096):
+        for T in (1, 2, 16, 31, 64, 128, 129, 1000):
+            state = lm_head._layout(T, D, V, dtype)[1]
+            wide = -(-D // 64) * 64
+            rest = 3 * T * wide * es + 64 * T + 4096  # x's copy and the words a row
+            if dtype == torch.float32 and T > 128:
+                rest += 6 * V * wide                  # the weight's, in three parts or padded
+            elif wide != D:
+                rest += V * wide * es
+            assert state <= rest + V * D * es // 2, (D, T)
+    assert lm_head._layout(16, 1024, V, dtype)[1] >= 4 * 16 * V
+
+
 def test_refusals():
     with FakeTensorMode():
         def fake(*shape, dtype=torch.bfloat16):
