@@ -110,6 +110,7 @@ struct GemmArgs {
   float* ztarget;
   const int* target;
   const float *rowmax, *inv, *coef, *out_scale;
+  float* dropped;      // [T], what rounding took off each row's dz of its target (null: not used)
 };
 
 // One operand of ROWS tile rows (of M or N) and a 128-byte K step, moved global -> LDS by DMA.
@@ -226,11 +227,101 @@ __device__ inline void planes_of(int seg, int& a, int& b) {
 
 __device__ inline float exp_of(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
 
+// A row of dx or dw is mostly its targets' entries of dz times rows of w or x, and the rounding of those
+// few numbers to 16 bits does not average out.  So kGrad leaves what it took off each row's target entry;
+// k_ce_dx adds it times the target's row of w, and here the rows of x whose targets are rows m0 .. of a dw
+// tile come once more with it, as further K steps: the targets are looked through, 64 rows found at a time, in
+// their order.  Errors against 64 bits without it, with it, and of the results' own rounding: bf16 16368 x 32000 x
+// 1024 1.82e-3, 1.66e-3, 1.66e-3; fp16 1800 x 50257 x 1001 2.36e-4, 2.08e-4, 2.08e-4.  A step is not fetched ahead
+// and takes about 3 us: forward and gradients of 16384 x V x 1024, bf16, V 32000: 3797 -> 3807 us, 4000: 673 -> 682,
+// 500: 249 -> 271; 8192 x 131072 x 4096: 1%.
+template <class C, int DT>
+__device__ __forceinline__ void add_dropped(const GemmArgs& g, uint8_t* smem, int64_t rows, int64_t m0, int64_t n0, int wave,
+                                            int lane, v4f (&acc)[C::MT][C::NT]) {
+  using A = Operand<C::TM, C::kThreads, true, 2>;
+  using B = Operand<C::TN, C::kThreads, true, 2>;
+  constexpr int kPer = 16, kWaves = C::kThreads / 64;  // targets a thread looks at together
+  static_assert(C::kStage + C::kThreads * kPer * 4 + kWaves * 4 <= C::kBytes, "a K step, the rows found, counts");
+  int* found = reinterpret_cast<int*>(smem + C::kStage);
+  int* counts = found + C::kThreads * kPer;
+  const int tid = wave * 64 + lane;
+  const uint32_t first = (uint32_t)(g.v0 + m0);
+  const uint16_t* x = static_cast<const uint16_t*>(g.B);
+  for (int64_t t0 = 0; t0 < rows; t0 += C::kThreads * kPer) {
+    const int64_t t = t0 + tid * kPer;
+    uint32_t hits = 0;
+    int y[kPer];
+    if (t + kPer <= rows) {
+      __builtin_memcpy(y, g.target + t, sizeof(y));
+    } else {
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) y[e] = t + e < rows ? g.target[t + e] : -1;
+    }
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) hits |= (uint32_t)(y[e] >= 0 && (uint32_t)y[e] - first < (uint32_t)C::TM) << e;
+    int at = __popc(hits);
+    const int mine = at;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int v = __shfl_up(at, o);
+      at += lane >= o ? v : 0;
+    }
+    if (lane == 63) counts[wave] = at;
+    __syncthreads();
+    int all = 0;
+    at -= mine;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const int v = counts[w];
+      at += w < wave ? v : 0;
+      all += v;
+    }
+    for (; hits; hits &= hits - 1) found[at++] = (int)(t + __builtin_ctz(hits));
+    for (int s = 0; s < all; s += 64) {
+      const int left = all - s < 64 ? all - s : 64;
+      for (int q = tid; q < C::TM * 8; q += C::kThreads) reinterpret_cast<v4u*>(smem)[q] = v4u{0, 0, 0, 0};
+      __syncthreads();  // (and the rows found are there)
+      v4u v[B::kOps];
+#pragma unroll
+      for (int i = 0; i < B::kOps; ++i) {
+        const int slot = i * C::kThreads + tid, r = slot / B::kCpr, c = slot % B::kCpr;
+        const int64_t col = n0 + (((c / B::kGc) ^ B::f(r)) * B::kGc + c % B::kGc) * 8;
+        // (any row and column that there are, where it is none)
+        v[i] = *reinterpret_cast<const v4u*>(x + found[r < left ? s + r : s] * g.ldb + (col < g.wb ? col : 0));
+        if (r >= left || col >= g.wb) v[i] = v4u{0, 0, 0, 0};
+      }
+#pragma unroll
+      for (int i = 0; i < B::kOps; ++i)
+        *reinterpret_cast<v4u*>(smem + C::TM * 128 + (i * C::kThreads + tid) * 16) = v[i];
+      if (tid < left) {
+        const int row = found[s + tid], m = g.target[row] - (int)first;
+        *reinterpret_cast<uint16_t*>(smem + tid * (C::TM * 2) + (((m >> 4) ^ A::f(tid)) << 5) + (m & 15) * 2) =
+            (uint16_t)f32_to_half_bits(DT, g.dropped[row]);
+      }
+      __syncthreads();
+#pragma unroll 1
+      for (int ks = 0; ks < 2; ++ks) {
+        v4u b[C::NT];
+#pragma unroll
+        for (int j = 0; j < C::NT; ++j) b[j] = B::frag(smem + C::TM * 128, (wave % C::WN * C::NT + j) * 16, ks, lane & 15, lane >> 4);
+#pragma unroll
+        for (int i = 0; i < C::MT; ++i) {
+          const v4u a = A::frag(smem, (wave / C::WN * C::MT + i) * 16, ks, lane & 15, lane >> 4);
+#pragma unroll
+          for (int j = 0; j < C::NT; ++j) acc[i][j] = mma<DT>(b[j], a, acc[i][j]);
+        }
+      }
+      lds_barrier();
+    }
+    __syncthreads();
+  }
+}
+
 template <class C, int DT, int EPI>
 __global__ __launch_bounds__(C::kThreads, 2) void k_ce_gemm(GemmArgs g) {
   constexpr bool kAcrossA = EPI == kFinal, kAcrossB = EPI == kSlab || EPI == kFinal;
   constexpr int MT = C::MT, NT = C::NT, kSegs = DT == CIN_DT_F32 ? kPairs32 : 1, BK = kStepBytes / kEs<DT>;
-  constexpr bool kTogether = DT == CIN_DT_F32 && C::kStages3 > 0;
+  constexpr bool kTogether = DT == CIN_DT_F32 && C::kStages3 > 0, k16 = DT == CIN_DT_BF16 || DT == CIN_DT_F16;
   constexpr int kStages = kTogether ? C::kStages3 : C::kStages, kPlanes = kTogether ? 3 : 1, kStage = C::kStage * kPlanes;
   __shared__ __attribute__((aligned(128))) uint8_t smem[kStages * kStage > C::kBytes ? kStages * kStage : C::kBytes];
   const int64_t rows = __builtin_amdgcn_readfirstlane(*g.n);
@@ -251,10 +342,10 @@ __global__ __launch_bounds__(C::kThreads, 2) void k_ce_gemm(GemmArgs g) {
     k0 = part * per;
     k1 = k0 + per < Kall ? k0 + per : Kall;
   }
-  const int tid = threadIdx.x, lane = tid & 63;
+  int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / C::WN, wn = wave % C::WN;
-  const int l16 = lane & 15, kq = lane >> 4;
+  int l16 = tid & 15, kq = tid >> 4 & 3;
   const uint32_t lds0 = (uint32_t)(uintptr_t)smem;
   Operand<C::TM, C::kThreads, kAcrossA, kEs<DT>> oa;
   Operand<C::TN, C::kThreads, kAcrossB, kEs<DT>> ob;
@@ -363,6 +454,15 @@ __global__ __launch_bounds__(C::kThreads, 2) void k_ce_gemm(GemmArgs g) {
       for (int j = 0; j < NT; ++j) acc[i][j] += low[i][j];
   }
   lds_barrier();
+  if constexpr (EPI == kFinal && k16)
+    {
+      // the lane's number anew: kept through the loop it would take a register of the operands
+      const int lane = (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+      tid = wave * 64 + lane;
+      l16 = lane & 15;
+      kq = lane >> 4;
+      if (g.dropped) add_dropped<C, DT>(g, smem, Kall, m0, n0, wave, lane, acc);
+    }
   // the lane holds rows m0 + (wm MT + i) 16 + l16, columns n0 + (wn NT + j) 16 + 4 kq + r
   const int64_t nl = n0 + wn * NT * 16 + 4 * kq;
   if constexpr (EPI == kStats) {
@@ -468,10 +568,17 @@ __global__ __launch_bounds__(C::kThreads, 2) void k_ce_gemm(GemmArgs g) {
         for (int r = 0; r < 4; ++r) acc[i][j][r] = exp_of(acc[i][j][r] - mx) * pc;
       const int64_t at = (in ? g.target[m] : -1) - g.v0 - nl;
       if (at >= 0 && at < NT * 16 && (at & 15) < 4) {
+        float v = 0.0f;
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) acc[i][j][r] -= (int)at == j * 16 + r ? cf : 0.0f;
+          for (int r = 0; r < 4; ++r) {
+            const bool here = (int)at == j * 16 + r;
+            acc[i][j][r] -= here ? cf : 0.0f;
+            v = here ? acc[i][j][r] : v;
+          }
+        if constexpr (k16)
+          if (g.dropped) g.dropped[m] = v - half_bits_to_f32(DT, (uint16_t)f32_to_half_bits(DT, v));
       }
     }
     if (g.v0 + n0 + C::TN > g.V) {  // columns past the vocabulary are part of the next products' K
@@ -879,6 +986,7 @@ __device__ inline Coef coef_of(const float* __restrict__ grad, int64_t stride, i
 // Where the backward leaves what its products are scaled by.
 struct Scales {
   float *out, *coef, *row;  // row: for few rows, null for many
+  float* dropped;           // for many of 16 bits, else null
   int* slabs;
 };
 
@@ -904,7 +1012,8 @@ __global__ __launch_bounds__(1024) void k_ce_coef(const float* __restrict__ grad
 // 2^e with dz, m in fp32 with dx's sums and, for dw, with x, held as two 16-bit parts.  The gradients are
 // then as near as their own rounding allows (relative error of 16 x 32000 x 1024, bf16, a gradient for
 // each row: 1.65e-3, without it 2.5e-3).  dw takes twice the products: of x 32000 x 1024 backward 59 -> 63
-// us with 64 rows, 72 -> 82 with 128, 104 -> 121 with 256, and 140 -> 174 with 512, too many for it.
+// us with 64 rows, 72 -> 82 with 128, 104 -> 121 with 256, and 140 -> 174 with 512, too many for it (see
+// add_dropped for those).
 constexpr int kFewExact = 256;
 template <int DT>
 __global__ __launch_bounds__(256) void k_ce_coef_few(const float* __restrict__ grad, int64_t stride, int mean,
@@ -1011,10 +1120,12 @@ __global__ __launch_bounds__(256) void k_ce_grad(const float* __restrict__ z, in
   }
 }
 
-// dx[t] = out_scale (row[pos[t]]) times the sum of the slabs' row pos[t], zero for an ignored row.
+// dx[t] = out_scale (row[pos[t]]) times the sum of the slabs' row pos[t] (and what dz's rounding dropped
+// times the target's row of w), zero for an ignored row.
 template <int DT>
 __global__ __launch_bounds__(256) void k_ce_dx(const float* __restrict__ slabs, Scales by, const int* __restrict__ n, int64_t Dp,
-                                               const int* __restrict__ pos,
+                                               const int* __restrict__ pos, const int* __restrict__ target,
+                                               const void* __restrict__ w, int64_t ldw,
                                                int64_t T, int64_t D, void* __restrict__ dx) {
   const float shared = *by.out;
   const int splits = *by.slabs;
@@ -1028,6 +1139,17 @@ __global__ __launch_bounds__(256) void k_ce_dx(const float* __restrict__ slabs, 
       for (int s = 0; s < splits; ++s) {
         const float4 b = *reinterpret_cast<const float4*>(slabs + s * slab + i * Dp + c);
         a = make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
+      }
+      if constexpr (DT != CIN_DT_F32) {
+        const int y = target[i];
+        if (by.dropped && y >= 0) {
+          const float r = by.dropped[i];
+          const uint2 h = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(w) + y * ldw + c);
+          a.x += r * half_bits_to_f32(DT, (uint16_t)h.x);
+          a.y += r * half_bits_to_f32(DT, (uint16_t)(h.x >> 16));
+          a.z += r * half_bits_to_f32(DT, (uint16_t)h.y);
+          a.w += r * half_bits_to_f32(DT, (uint16_t)(h.y >> 16));
+        }
       }
     }
     const float scale = by.row && i >= 0 ? shared * by.row[i] : shared;
@@ -1081,17 +1203,21 @@ double tile_time(int tile, int64_t m, int64_t n, double parts, double part) {
 }
 // fp32 operands of 4 bytes come for few rows only, and in the two smaller tiles.
 int first_tile(int op) { return op == kDirect ? 2 : 0; }
-int pick_tile(int op, int64_t m, int64_t n) {
-  int best = first_tile(op);
+int pick_tile(int op, int64_t m, int64_t n, int first = 0) {
+  int best = first_tile(op) > first ? first_tile(op) : first;
   for (int t = best + 1; t < kTiles; ++t)
     if (tile_time(t, m, n, 1, 1) < tile_time(best, m, n, 1, 1)) best = t;
   return best;
 }
-template <int DT, class F>
+// dw's: no wider ones, where its product runs as fast (8192 x 65536 x 4096: 3.43 ms with the widest, 3.45 with
+// 256 x 256) and add_dropped would take registers from its loop (3.68 ms).
+int pick_dw_tile(int op, int64_t m, int64_t n) { return pick_tile(op, m, n, 1); }
+template <int DT, int EPI, class F>
 void with_tile(int tile, F f) {
   if constexpr (DT != kDirect) {
-    if (tile == 0) return f(Widest{});
-    if (tile == 1) return f(Wide{});
+    if constexpr (EPI != kFinal)
+      if (tile == 0) return f(Widest{});
+    if (tile <= 1) return f(Wide{});
   }
   if (tile <= 2)
     f(Medium{});
@@ -1182,7 +1308,7 @@ int check(const char* name, int dtype, int64_t T, int64_t D, int64_t V, Plan& p)
   CIN_CHECK_ARG(D >= 1 && D <= kMaxD, "%s: D must be in [1, 2^18]", name);
   // (the products over a piece of the vocabulary are smaller: T x piece < 2^30 + 256 T)
   p = make_plan(dtype, T, D, V);
-  CIN_CHECK_ARG(grid_fits(p.tile, T, V) && grid_fits(p.slab_tile, T, p.Dp) && grid_fits(pick_tile(p.op, p.piece, D), p.piece, D),
+  CIN_CHECK_ARG(grid_fits(p.tile, T, V) && grid_fits(p.slab_tile, T, p.Dp) && grid_fits(pick_dw_tile(p.op, p.piece, D), p.piece, D),
                 "%s: T x V, T x D or V x D is too large", name);
   return CIN_OK;
 }
@@ -1214,7 +1340,7 @@ void with_op(int op, F f) {
 template <int EPI>
 void gemm(int op, int tile, const GemmArgs& g, int64_t max_m, int splits, hipStream_t s) {
   with_op(op, [&](auto dt) {
-    with_tile<dt()>(tile, [&](auto c) {
+    with_tile<dt(), EPI>(tile, [&](auto c) {
       using C = decltype(c);
       const int64_t tiles = cdiv(max_m, C::TM) * cdiv(g.N, C::TN) * splits;
       hipLaunchKernelGGL((k_ce_gemm<C, dt(), EPI>), (unsigned)tiles, C::kThreads, 0, s, g);
@@ -1326,7 +1452,8 @@ int cin_linear_ce_backward(const void* xc, int dtype, int64_t T, int64_t D, cons
   float* slabs = reinterpret_cast<float*>(ws + p.dz);
   uint16_t* scaled = reinterpret_cast<uint16_t*>(ws + p.dz + p.slabs);
   float* f = reinterpret_cast<float*>(ws + p.dz + p.slabs + p.scaled);
-  const Scales by{f, f + 2, p.few ? f + 2 + T : nullptr, reinterpret_cast<int*>(f + 1)};
+  float* rows = f + 2 + T;
+  const Scales by{f, f + 2, p.few ? rows : nullptr, !p.few && dtype != CIN_DT_F32 ? rows : nullptr, reinterpret_cast<int*>(f + 1)};
   if (p.few) {
     const unsigned grid = (unsigned)cdiv(T * (p.Dp / 8), 256);
     with_dtype(dtype, [&](auto dt) {
@@ -1360,6 +1487,7 @@ int cin_linear_ce_backward(const void* xc, int dtype, int64_t T, int64_t D, cons
     g.rowmax = state_f;
     g.inv = state_f + T;
     g.coef = by.coef;
+    g.dropped = by.dropped;
     if (logits) {
       const int64_t blocks = cdiv(T * (g.N / 8), 256);
       with_op(p.op, [&](auto dt) {
@@ -1402,14 +1530,16 @@ int cin_linear_ce_backward(const void* xc, int dtype, int64_t T, int64_t D, cons
       h.C = static_cast<char*>(dw) + v0 * D * (dtype == CIN_DT_F32 ? 4 : 2);
       h.ldc = D;
       h.out_scale = by.out;
-      gemm<kFinal>(p.op, pick_tile(p.op, cols, D), h, cols, 1, s);
+      h.target = st.target;
+      h.dropped = by.dropped;
+      gemm<kFinal>(p.op, pick_dw_tile(p.op, cols, D), h, cols, 1, s);
     }
   }
   if (dx) {
     const int64_t blocks = cdiv(T * (p.Dp / 4), 256);
     with_dtype(dtype, [&](auto dt) {
       hipLaunchKernelGGL(k_ce_dx<dt()>, (unsigned)(blocks < 16384 ? blocks : 16384), 256, 0, s, slabs, by, st.n,
-                         p.Dp, st.pos, T, D, dx);
+                         p.Dp, st.pos, st.target, w, ldw, T, D, dx);
     });
   }
   return cin_check_launch(name);

@@ -35,15 +35,15 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     each row's loss (0 for an ignored one).  A target outside [0, V) gives NaN, in the gradients too.
 
     Differentiable in x and weight (once), gradients in their dtype.  Products are summed in fp32;
-    the gradient of the logits enters the two gradient products rounded to the inputs' dtype, for up
-    to 256 rows scaled so that the targets' entries are exact.
+    the gradient of the logits enters the two gradient products rounded to the inputs' dtype, but for the
+    targets' entries: what rounding takes off them is added back.
     fp32 inputs are multiplied as three bf16 parts each, to the accuracy of fp32 products (up to 128
     rows as they are).
     Results do not vary from call to call.  The backward recomputes the logits piece by piece (those of
-    up to 128 rows are kept where they are at most half the weight's bytes): beside the inputs it keeps one copy of the rows that count (fp32 of more than
-    128 rows: 1.5 times their size, and the weight's; a weight whose width is no multiple of 64: a
-    padded copy) and a few words a row, and works in up to about 1 GiB for a piece of the logits'
-    gradient plus fp32 sums of x's."""
+    up to 128 rows are kept where they are at most half the weight's bytes): beside the inputs it keeps
+    one copy of the rows that count (fp32 of more than 128 rows: 1.5 times their size, and the weight's;
+    a weight whose width is no multiple of 64: a padded copy) and a few words a row, and works in up to
+    about 1 GiB for a piece of the logits' gradient plus fp32 sums of x's."""
     _require(x.is_cuda and weight.is_cuda and target.is_cuda, "Inputs must be on CUDA")
     _require(x.device == weight.device == target.device, "Inputs must be on one device")
     _require(weight.ndim == 2 and x.ndim >= 1 and x.shape[-1] == weight.shape[1], "x must be [..., D] and weight [V, D]")

@@ -571,6 +571,44 @@ def test_kept_logits_are_fewer_bytes_than_the_weight(dt):
     assert lm_head._layout(16, 1024, V, dtype)[1] >= 4 * 16 * V
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,V,D", [(257, 1000, 128), (700, 20000, 200), (1100, 17001, 64), (5000, 16500, 136), (9000, 16400, 64)])
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+@pytest.mark.parametrize("reduction", ["none", "mean"])
+@pytest.mark.parametrize("spread", ["all", "few", "one"])
+def test_many_rows_keep_their_targets_entries(dev, T, V, D, dt, reduction, spread):
+    """What rounding takes off an entry of dz at a target comes back in both gradients: any number of rows with
+    the same target, some ignored."""
+    g = torch.Generator().manual_seed(T)
+    y = {"all": torch.randint(0, V, (T,), generator=g), "few": torch.randint(0, 9, (T,), generator=g) * (V // 9),
+         "one": torch.full((T,), V - 1)}[spread]
+    x = torch.randn(T, D, generator=g) * 0.3
+    w = torch.randn(V, D, generator=g) * 0.3
+    y[torch.rand(T, generator=g) < 0.1] = -100
+    x, w = (t.to(DT[dt]).to(dev).requires_grad_() for t in (x, w))
+    y = y.to(dev)
+    gr = torch.randn(T, generator=g).to(dev) if reduction == "none" else torch.tensor(0.7, device=dev)
+    loss = lm_head.linear_cross_entropy(x, w, y, reduction=reduction)
+    dx, dw = torch.autograd.grad(loss, (x, w), gr)
+    x64, w64 = x.detach().double(), w.detach().double()
+    kept = (y >= 0)[:, None]
+    p = (x64 @ w64.T).softmax(-1)
+    g64 = (gr.double().expand(T)[:, None] / (1 if reduction == "none" else kept.sum())) * kept
+    at = torch.nn.functional.one_hot(y.clamp(min=0), V).double()
+    dz, other, mine = g64 * (p - at), (g64 * p).abs() * (1 - at), (g64 * (p - at) * at).abs()
+    # The other entries are rounded (fp16: or lie under its steps, 2^-24 of the largest row's 2^-15), the
+    # targets' are held to 2 half steps of half a step; p is off by the sums' D 2^-24 of products up to 0.3^2 D 6
+    # and 2^-18; the sums are fp32 chains of K / 32 groups of 32 products and at most 256 slabs
+    half = torch.finfo(DT[dt]).eps / 2
+    tiny = 2 ** -38 * g64.abs().max()
+    off = other * half + mine * 2 * half * half + (g64 * p).abs() * (D * 2 ** -24 * 0.6 * D + 2 ** -18) + tiny * kept
+    for got, want, o, total, K in ((dx, dz @ w64, off @ w64.abs(), dz.abs() @ w64.abs(), V),
+                                   (dw, dz.T @ x64, off.T @ x64.abs(), dz.abs().T @ x64.abs(), T)):
+        bound = want.abs() * half * 1.001 + o * 1.01 + total * (K / 32 + 300) * 2 ** -24 + 2 ** -25
+        d = (got.double() - want).abs()
+        assert (d <= bound).all(), (d / bound).max()
+
+
 def test_refusals():
     with FakeTensorMode():
         def fake(*shape, dtype=torch.bfloat16):
