@@ -766,12 +766,27 @@ __device__ __forceinline__ void copy_piece(const void* __restrict__ x, int64_t l
   if constexpr (DT == kDirect) {
     __builtin_memcpy(__builtin_assume_aligned(reinterpret_cast<float*>(out) + i * Dp + c, 16), v, 32);
   } else if constexpr (DT == CIN_DT_F32) {
+    bool far = false;  // a value that rounds to infinity, or is one
+#pragma unroll
+    for (int e = 0; e < 8; ++e) far |= fabsf(v[e]) >= 0x1.ffp127f;
 #pragma unroll
     for (int p = 0; p < 3; ++p) {
-      uint32_t h[8];
+      v4u h;
+      if (far) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) h[e] = take_part(v[e]);
-      *reinterpret_cast<v4u*>(d + p * plane) = v4u{h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16};
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t lo = take_part(v[2 * e]);
+          h[e] = lo | take_part(v[2 * e + 1]) << 16;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          h[e] = f32x2_to_bf16x2_bits(v[2 * e], v[2 * e + 1]);
+          v[2 * e] -= bf16_lo(h[e]);
+          v[2 * e + 1] -= bf16_hi(h[e]);
+        }
+      }
+      *reinterpret_cast<v4u*>(d + p * plane) = h;
     }
   } else {
     __builtin_memcpy(__builtin_assume_aligned(d, 16), v, 16);
@@ -1497,7 +1512,7 @@ int cin_linear_ce_backward(const void* xc, int dtype, int64_t T, int64_t D, cons
       });
     } else {
       gemm<kGrad>(p.op, pick_tile(p.op, T, g.N), g, T, 1, s);
-      if (p.planes > 1) hipLaunchKernelGGL(k_ce_mend, 1024, 256, 0, s, g, st.mended);
+      if (p.planes > 1) hipLaunchKernelGGL(k_ce_mend, 256, 256, 0, s, g, st.mended);
     }
     GemmArgs h{};
     h.n = st.n;
