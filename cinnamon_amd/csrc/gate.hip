@@ -26,9 +26,9 @@
 // lanes is the order of the indices: the lowest of equal candidates is the first lane of a ballot.
 // Up to 256 experts a token takes 16 lanes (a DPP row): maxima and sums need no LDS, and the rounds
 // of the top k serve four tokens at once.  65536 tokens, 256 bf16 logits in 8 groups of which 4 stay,
-// top-8, all scores out: 55 us, 1.9 TB/s, of which about 14 are the few waves that rank again in 64 bits
+// top-8, all scores out: 56 us, 1.9 TB/s, of which about 14 are the few waves that rank again in 64 bits
 // (they end last); bound by VALU issue (1600 instructions a wave).  A wave per token with 64-bit keys
-// throughout took 188 us.  The gradient, 22 us, 5.8 TB/s, is bound by HBM.
+// throughout took 188 us.  The gradient, 23 us, 5.8 TB/s, is bound by HBM.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

@@ -867,7 +867,8 @@ __device__ inline float product_of_parts(const GemmArgs& g, int64_t m, int64_t n
 // Six products of parts make NaN of an infinity: it meets parts of 0 and of either sign.  (So does a sum
 // that leaves the range on its way.)  Where a tile's sum is NaN its logits are formed again from whole
 // values, here for the statistics and in k_ce_mend for dz: -inf masks an entry of the vocabulary for fp32
-// as it does for 16 bits.  Maximum and sum of row i's such tiles, NaN where the row has a logit that is
+// as it does for 16 bits.  (2046 x 32000 x 1024, forward: 0.83 ms, with one such entry 1.73; with 3200 scattered ones,
+// in every tile, 111.)  Maximum and sum of row i's such tiles, NaN where the row has a logit that is
 // NaN or +inf, at the first of them; its target's logit if it is theirs.
 __device__ inline float2 mended_tiles(const GemmArgs& g, const float2* __restrict__ part, int tiles, int tile_n, int64_t i,
                                       int target, int lane, float& ztarget) {
@@ -1201,13 +1202,18 @@ __global__ __launch_bounds__(256) void k_ce_dx(const float* __restrict__ slabs, 
 using Widest = Cfg<2, 4, 8, 6, 2>;  // 256 x 384, 8 waves of 128 x 96: 250 registers, all of the LDS
 using Wide = Cfg<2, 4, 8, 4, 2>;    // 256 x 256, 8 waves of 128 x 64
 using Medium = Cfg<2, 2, 4, 4, 2>;  // 128 x 128, 4 waves of 64 x 64, two workgroups a CU
-using Narrow = Cfg<1, 4, 4, 1, 4>;  // 64 x 64, 4 waves of 64 x 16, two workgroups a CU
-using Thin = Cfg<1, 4, 2, 1, 6>;    // 32 x 64, 4 waves of 32 x 16, two workgroups a CU: up to 32 rows, few tiles
+// (two workgroups a CU of these where operands are one plane; with all parts of fp32 in a step, one)
+using Narrow = Cfg<1, 4, 4, 1, 4>;  // 64 x 64, 4 waves of 64 x 16
+using Thin = Cfg<1, 4, 2, 1, 6>;    // 32 x 64, 4 waves of 32 x 16: up to 32 rows, few tiles
 constexpr int kTiles = 5;
 constexpr int kTileM[kTiles] = {Widest::TM, Wide::TM, Medium::TM, Narrow::TM, Thin::TM};
 constexpr int kTileN[kTiles] = {Widest::TN, Wide::TN, Medium::TN, Narrow::TN, Thin::TN};
 constexpr int kTileThreads[kTiles] = {Widest::kThreads, Wide::kThreads, Medium::kThreads, Narrow::kThreads, Thin::kThreads};
-// a tile's rate against that of the 256 x 256 ones, every CU at work
+// A tile's rate against that of the 256 x 256 ones.  With full grids, forward of 8192 x 24576 x 4096 in bf16: 1387,
+// 1262, 1095, 631 and 458 TFLOP/s, that is 1.10, 1, 0.87, 0.50 and 0.36 (fp16 the same within 1%; 8192 x 24576 x 1024:
+// 1.11, 1, 0.92, 0.45, 0.32; fp32 in parts, 4096 x 24576 x 1024: 1.08, 1, 0.89, 0.61, 0.48).  The narrower ones have
+// that from several workgroups on a CU; one on each (4096 x 4096, 2048 x 2048, 1024 x 1024 and 512 x 1024 rows and
+// columns, K 8192) gives 0.6, 0.3 and 0.2, as their rounds are counted here, and they are taken in between.
 constexpr double kTileRate[kTiles] = {1.08, 1.0, 0.75, 0.4, 0.25};
 
 // The time of m x n outputs in parts of K, in units of one output's share at the 256 x 256 tile's rate.
@@ -1216,7 +1222,7 @@ double tile_time(int tile, int64_t m, int64_t n, double parts, double part) {
   const double rounds = ceil(count / cin_device_cus());
   return rounds * kTileM[tile] * kTileN[tile] / kTileRate[tile] * part;
 }
-// fp32 operands of 4 bytes come for few rows only, and in the two smaller tiles.
+// fp32 operands of 4 bytes come for few rows only, and in the three smaller tiles.
 int first_tile(int op) { return op == kDirect ? 2 : 0; }
 int pick_tile(int op, int64_t m, int64_t n, int first = 0) {
   int best = first_tile(op) > first ? first_tile(op) : first;

@@ -24,9 +24,10 @@ constexpr int kMaxUnits = 2;
 constexpr uint32_t kMagicLimit = 60000;      // (kThreads kMaxUnits + d) d < 2^32: see div_by
 
 // Units a thread, their loads in flight together.  One is as fast for 16-byte units of 16-bit elements or
-// faster (64 x 1024 x 17 heads of 64: 61 us, with two 64; 16 x 1024: 14.9 and 16.6; heads of 193: 267 and
-// 260); two for fp32 (1 x 32767 x 32 heads of 192: 343 and 325) and for single channels (918 and 770),
-// and four need half as many registers again for the half layout (269 against 207).
+// faster (64 x 1024 x 17 heads of 64: 54 us, with two 58; 16 x 1024: 14.9 and 15.5; 1 x 32767 x 32 heads of 192
+// in the half layout: 169 and 177, interleaved 179 and 177; of 193: 244 and 251); two for single channels (842
+// and 785) and, by a little, for fp32 (1 x 32767 x 32 heads of 192: interleaved 350 and 331, half layout 314 and
+// 320, of 193 416 and 406; 64 x 1024 x 17 heads of 64: 112 and 117).  Four needed half as many registers again.
 template <int DT, int E>
 constexpr int kUnitsOf = DT != CIN_DT_F32 && E > 1 ? 1 : kMaxUnits;
 
@@ -122,9 +123,9 @@ __device__ __forceinline__ void load_pairs(const float* p, float (&v)[N]) {
 // Bound by HBM: each element is read and written once; the tables' rows are shared by a token's heads
 // through the caches.  A workgroup takes neighbouring units; their token, head, channel and offsets
 // follow from the first one's in 32 bits (with 64-bit divisions and products the vector units bound it:
-// 1 x 32767 x 32 heads of 192, fp16, half layout, 355 us).  That call now takes 204 us, 4.0 TB/s, its
-// interleaved form 178 (4.6), 64 x 1024 x 17 heads of 64 in bf16 61 us, 4.7 TB/s.  Stores that bypass
-// the caches take 46 us there, and the next reader of the result as much more.
+// 1 x 32767 x 32 heads of 192, fp16, half layout, 355 us).  That call now takes 169 us, 4.8 TB/s, its
+// interleaved form 179 (4.5), 64 x 1024 x 17 heads of 64 in bf16 54 us, 5.3 TB/s.  Stores that bypass
+// the caches took a quarter less there, and the next reader of the result as much more.
 template <int DT, int E, bool INTER>
 __global__ __launch_bounds__(kThreads) void k_rotary(RotaryArgs a) {
   constexpr int kPairs = INTER ? (E > 1 ? E / 2 : 1) : E;  // pairs of a turning unit
@@ -254,8 +255,8 @@ int cin_rotary(const void* q, int64_t sqb, int64_t sql, int64_t sqh, void* q_out
   RotaryArgs a{{q, q_out, sqb, sql, sqh, soqb, soql, soqh}, {k, k_out, skb, skl, skh, sokb, sokl, sokh}, (int)H, 0, L, 0, cos, sin,
                P, ldt, (int)rot, (int)start, 0, 0, 0, 0, 0, 0, 0, 0, 0, positions, spb, spl, interleaved, inverse};
   // 16 bytes at a time where they hold turning or copied channels only, whatever their alignment:
-  // 1 x 32767 x 32 heads, fp16, rot 64: 204 us with heads of 192 channels, 267 with 193 (one
-  // channel at a time 770).
+  // 1 x 32767 x 32 heads, fp16, rot 64: 169 us with heads of 192 channels, 244 with 193 (one
+  // channel at a time 785).
   const int64_t e16 = 16 / es;
   const bool odd = (interleaved ? rot : rot / 2) % e16 || ((uintptr_t)cos | (uintptr_t)sin) % 16 || ldt % 4;
   const int64_t E = odd ? 1 : e16;
