@@ -609,6 +609,61 @@ def test_many_rows_keep_their_targets_entries(dev, T, V, D, dt, reduction, sprea
         assert (d <= bound).all(), (d / bound).max()
 
 
+@pytest.mark.gpu
+def test_masked_entries_of_a_later_piece(dev):
+    """fp32, two pieces of the vocabulary, a masked entry in each."""
+    T, V, D = 9000, 35001, 64
+    x, w, y, g = make(T, V, D, "fp32", 0.1, dev)
+    x[:, 5] = 1.0
+    gone = torch.zeros(V, dtype=torch.bool, device=dev)
+    gone[[10, V - 3]] = True
+    y[(y == 10) | (y == V - 3)] = 0
+    w[gone, 5] = -math.inf
+    y2 = torch.where(y >= 0, torch.cumsum(~gone, 0)[y.clamp(min=0)] - 1, y)
+    grad = torch.tensor(0.7, device=dev)
+    (loss, ltol), (dx, dxt), (dw, dwt) = reference(x, w[~gone], y2, reduction="sum", grad=grad)
+    xl, wl = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    got = lm_head.linear_cross_entropy(xl, wl, y, reduction="sum")
+    assert abs(got.item() - loss.item()) <= ltol.item()
+    a, b = torch.autograd.grad(got, [xl, wl], grad)
+    assert (b[gone] == 0).all()
+    near(b[~gone], dw, dwt, "fp32", T + D)
+    keep = torch.arange(D, device=dev) != 5
+    near(a[:, keep], dx[:, keep], dxt[:, keep], "fp32", V + D)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+def test_a_graph_whose_weight_is_masked_in_some_replays(dev, dt):
+    T, V, D = 300, 2000, 128
+    x, w, y, g = make(T, V, D, dt, 0.2, dev)
+    x[:, 5] = 1.0
+    masked = w.clone()
+    masked[[3, 700, 1999], 5] = -math.inf
+
+    def step(x, w):
+        loss = lm_head.linear_cross_entropy(x, w, y, reduction="none")
+        return (loss, *torch.autograd.grad(loss.sum(), [x, w]))
+
+    def leaves(w):
+        return x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+
+    step(*leaves(w))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    sx, sw = leaves(w)
+    with torch.cuda.graph(graph):
+        out = step(sx, sw)
+    for v in (w, masked, w, masked, masked, w):
+        with torch.no_grad():
+            sw.copy_(v)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step(*leaves(v))
+        for a, b in zip(out, want):
+            assert torch.equal(a.nan_to_num(nan=7.0), b.nan_to_num(nan=7.0))
+
+
 def test_refusals():
     with FakeTensorMode():
         def fake(*shape, dtype=torch.bfloat16):
