@@ -14,7 +14,7 @@
 // One kernel runs the three products on the matrix units, with fp32 sums.  fp32 values are held as
 // three bf16 ones (x = x0 + x1 + x2, each the rounding of what is left, exact to 2^-26), and their
 // product is the six products of planes down to x0 y2, the small ones first: what is dropped lies
-// under 2^-26 of |x y|, and the sums are those of fp32 products (2046 x 32000 x 1024: 0.62 ms, 215
+// under 2^-26 of |x y|, and the sums are those of fp32 products (2046 x 32000 x 1024: 0.64 ms, 208
 // TFLOP/s; on the fp32 matrix units, in the same tiles, 1.04 ms).  An operand is read along K (its rows
 // hold K) or across it (its rows are K), so no transposed copy of x, w or dz is ever made.
 #include <hip/hip_runtime.h>
@@ -454,15 +454,14 @@ __global__ __launch_bounds__(C::kThreads, 2) void k_ce_gemm(GemmArgs g) {
       for (int j = 0; j < NT; ++j) acc[i][j] += low[i][j];
   }
   lds_barrier();
-  if constexpr (EPI == kFinal && k16)
-    {
-      // the lane's number anew: kept through the loop it would take a register of the operands
-      const int lane = (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
-      tid = wave * 64 + lane;
-      l16 = lane & 15;
-      kq = lane >> 4;
-      if (g.dropped) add_dropped<C, DT>(g, smem, Kall, m0, n0, wave, lane, acc);
-    }
+  if constexpr (EPI == kFinal && k16) {
+    // the lane's number anew: kept through the loop it would take a register of the operands
+    const int lane = (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+    tid = wave * 64 + lane;
+    l16 = lane & 15;
+    kq = lane >> 4;
+    if (g.dropped) add_dropped<C, DT>(g, smem, Kall, m0, n0, wave, lane, acc);
+  }
   // the lane holds rows m0 + (wm MT + i) 16 + l16, columns n0 + (wn NT + j) 16 + 4 kq + r
   const int64_t nl = n0 + wn * NT * 16 + 4 * kq;
   if constexpr (EPI == kStats) {
