@@ -433,6 +433,11 @@ __global__ __launch_bounds__(C::kThreads, 2) void k_ce_gemm(GemmArgs g) {
         }
       }
     } else {
+      // The fp32 matrix units add one product after the other, each sum rounded: a sum of its own for each step
+      // of 32 leaves a fifth of the error where K is long (logits of 4096 products of variance 1: 4.2e-5 to 7.9e-5
+      // -> 0.8e-5 to 1.4e-5; K of dw is the rows).  Forward of 16 x 100000 x 2048 181 -> 186 us, of 128 489 -> 534.
+      constexpr bool kOwn = DT == kDirect && EPI != kFinal;
+      v4f own[kOwn ? MT : 1][kOwn ? NT : 1] = {};
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
         v4u bf[NT];
@@ -442,8 +447,17 @@ __global__ __launch_bounds__(C::kThreads, 2) void k_ce_gemm(GemmArgs g) {
         for (int i = 0; i < MT; ++i) {
           const v4u af = oa.frag(sa, (wm * MT + i) * 16, ks, l16, kq);
 #pragma unroll
-          for (int j = 0; j < NT; ++j) acc[i][j] = mma<DT>(bf[j], af, acc[i][j]);
+          for (int j = 0; j < NT; ++j) {
+            v4f& c = kOwn ? own[kOwn ? i : 0][kOwn ? j : 0] : acc[i][j];
+            c = mma<DT>(bf[j], af, c);
+          }
         }
+      }
+      if constexpr (kOwn) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int j = 0; j < NT; ++j) acc[i][j] += own[i][j];
       }
     }
   }
@@ -1256,8 +1270,8 @@ int64_t align_up(int64_t v, int64_t a) { return cdiv(v, a) * a; }
 constexpr int64_t kAlign = 256;  // columns of a piece: whole tiles
 
 // fp32 with so few rows is multiplied as it is: its products are bound by reading w, which three planes
-// more than double, and w needs no copy of three (forward of 16 x 100000 x 2048: 188 us, in parts 880; with
-// gradients 829 and 2176; of 128: 490 and 1000, 1870 and 2660; of 256: 866 and 1117, but 3390 and 3180).
+// more than double, and w needs no copy of three (forward of 16 x 100000 x 2048: 187 us, in parts 675; with
+// gradients 678 and 1435; of 128: 533 and 998, 1504 and 2668; of 256: 938 and 1113, but 3614 and 3178).
 constexpr int64_t kDirectRows = 128;
 
 struct Plan {

@@ -38,7 +38,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     the gradient of the logits enters the two gradient products rounded to the inputs' dtype, but for the
     targets' entries: what rounding takes off them is added back.
     fp32 inputs are multiplied as three bf16 parts each, to the accuracy of fp32 products (up to 128
-    rows as they are).
+    rows as they are, 32 products to a sum).
     Results do not vary from call to call.  The backward recomputes the logits piece by piece (those of
     up to 128 rows are kept where they are at most half the weight's bytes): beside the inputs it keeps
     one copy of the rows that count (fp32 of more than 128 rows: 1.5 times their size, and the weight's;

@@ -664,6 +664,28 @@ def test_a_graph_whose_weight_is_masked_in_some_replays(dev, dt):
             assert torch.equal(a.nan_to_num(nan=7.0), b.nan_to_num(nan=7.0))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [20, 64, 128])
+def test_long_fp32_sums(dev, T):
+    """Logits of 4096 products.  A rounding of a sum s is off by u |s| / sqrt(3) in the mean square at most; the sum of
+    k products of variance v has mean square k v.  Sums of 32 products each, then of the 128 of them:
+    u sqrt(v) times 32 sqrt(128 / 6) and 128 sqrt(32 / 6), 150 and 300 (one after the other all the way: 4096 / sqrt(6) =
+    1670).  Their root of squares here, 0.3 of it more for the few rows, and two roundings of the loss itself."""
+    D = 4096
+    g = torch.Generator().manual_seed(T)
+    x = torch.randn(T, D, generator=g)
+    w = torch.zeros(2, D)
+    w[0] = torch.randn(D, generator=g)
+    x = torch.where((x @ w[0])[:, None] < 0, -x, x).to(dev)   # the first logit positive, the second one 0
+    w = w.to(dev)
+    loss = lm_head.linear_cross_entropy(x, w, torch.ones(T, dtype=torch.int64, device=dev), reduction="none")
+    z = x.double() @ w[0].double()
+    want = torch.nn.functional.softplus(z, threshold=1e9)
+    rms = (loss.double() - want).square().mean().sqrt()
+    v = (x.double() * w[0].double()).square().mean().sqrt()
+    assert rms <= 1.3 * math.hypot(150, 300) * U * v + 2 * U * z.square().mean().sqrt()
+
+
 def test_refusals():
     with FakeTensorMode():
         def fake(*shape, dtype=torch.bfloat16):
