@@ -22,6 +22,10 @@ _DTYPE_CODE = {torch.bfloat16: CIN_DT_BF16, torch.float32: CIN_DT_F32, torch.flo
 
 _p, _i64, _i32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int
 
+_f32 = ctypes.c_float
+# the inputs of cin_block_norm and its backward: y, residual, sizes, the two weights, the gate, the residual's scale
+_NORM = [_p, _i32, _i64] * 2 + [_i64, _i64] + [_p, _i32] * 2 + [_p, _i32, _i32, _i64] + [_p, _i32, _i32, _f32]
+
 # name -> argtypes (all return int)
 SIGNATURES: dict[str, list] = {
     "cin_abi_version": [],
@@ -86,10 +90,14 @@ SIGNATURES: dict[str, list] = {
     "cin_linear_ce_backward": [_p, _i32, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _i64, _i32, _p, _p, _p, _i64, _p, _p],
     "cin_rotary": [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i64] * 2 + [_i32, _i64, _i64, _i64, _p, _p, _i64, _i64,
                                                                            _i64, _i64, _p, _i64, _i64, _i32, _i32, _p],
+    "cin_block_norm": _NORM + [_f32, _p, _p, _p, _p],
+    "cin_block_norm_backward": _NORM + [_p] + [_p, _i64] * 2 + [_p] * 6 + [_p, _i64, _p],
+    "cin_block_norm_workspace": [_i64, _i64],
 }
 
 # entry points that return something other than an int status
-RESTYPES = {"cin_indexer_weights_grad_workspace": ctypes.c_int64, "cin_linear_ce_workspace": ctypes.c_int64}
+RESTYPES = {"cin_indexer_weights_grad_workspace": ctypes.c_int64, "cin_linear_ce_workspace": ctypes.c_int64,
+            "cin_block_norm_workspace": ctypes.c_int64}
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None

@@ -1,0 +1,826 @@
+// The norms around a block with its gate and residual scale on gfx950 (reference src/norm.py:15-17 and the
+// residual sums of src/layers.py:202), forward and backward.
+//
+//   u  = y / rms(y) * pw        rms(v) = sqrt(mean(v^2) + eps) over a row's D channels (u = y without pw)
+//   x  = a r + g u              the new residual stream: a a number, one learned value or one a channel,
+//                               g none, one a channel, one a row or one an element
+//   n  = x / rms(x) * w         what the next block reads
+// backward, with gn and gx the gradients of n and x, i = 1 / rms(x) and j = 1 / rms(y):
+//   t  = gn w;   dx = gx + i (t - x i^2 mean(t x));   dr = a dx;   du = g dx
+//   s  = du pw;  dy = j (s - y j^2 mean(s y))         (dy = du without pw)
+//   dw = sum gn x i,  dpw = sum du y j,  dg = dx u,  da = dx r over the rows, a row or an element
+//
+// x is formed again from y and r in the backward, in fp32 as in the forward: that reads as many bytes as
+// a stored x and has no rounding to x's type in it.  All arithmetic and the sums are fp32, each output is
+// rounded once.
+//
+// A row is read once into registers, 8 channels a thread and chunk, by one wave (up to 1024 channels, the
+// sums by DPP and swaps, no barrier) or by one workgroup.  Workgroups walk over rows, so that the channels'
+// vectors are loaded once and a channel's sums over the rows stay in registers; each workgroup leaves one
+// row of partial sums, which k_norm_columns adds up in a fixed order.  Bound by HBM.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "cin_common.h"
+#include "cin_runtime.h"
+
+using namespace cin;
+
+namespace {
+
+constexpr int kMaxThreads = 1024;
+constexpr int kMaxChunks = 2;
+constexpr int64_t kMaxWidth = (int64_t)kMaxThreads * kMaxChunks * 8;
+constexpr int kWaveRows = 4;  // rows at a time of a workgroup whose waves take a row each
+
+enum Gate { kNoGate = 0, kChannel = 1, kRow = 2, kElement = 3 };
+enum Scale { kNumber = 0, kOneValue = 1, kPerChannel = 2 };
+enum Sum { kSumW = 0, kSumPw = 1, kSumGate = 2, kSumScale = 3, kSums = 4 };
+
+struct Vec {  // a vector over the channels
+  const void* p;
+  int dtype;
+};
+
+struct NormArgs {
+  const void *y, *r;
+  int64_t ldy, ldr;
+  int64_t T;
+  int D, threads;  // threads of a row
+  Vec w, pw, gate, scale;
+  int gate_kind, scale_kind;
+  int64_t ldg;
+  float scale_value, eps;
+  void *n, *x;
+  float* stats;  // [2, T]: 1 / rms(x), 1 / rms(y)
+  // backward
+  const void *gn, *gx;
+  int64_t ldgn, ldgx;
+  void *dy, *dr, *dgate;
+  float* partial;  // [kSums, workgroups, D], then one value a workgroup for the learned scale
+};
+
+template <int DT>
+constexpr int kWords = DT == CIN_DT_F32 ? 8 : 4;
+
+// 8 adjacent elements as they lie in memory, at any element's address; cnt of them are there.
+template <int DT>
+struct Unit {
+  uint32_t w[kWords<DT>];
+  __device__ __forceinline__ void load(const void* p, int64_t i, int cnt) {
+    constexpr int es = DT == CIN_DT_F32 ? 4 : 2;
+    const uint8_t* q = static_cast<const uint8_t*>(p) + i * es;
+    if (__builtin_expect(cnt == 8, 1)) {
+      __builtin_memcpy(w, q, 16);
+      if constexpr (DT == CIN_DT_F32) __builtin_memcpy(w + 4, q + 16, 16);
+      return;
+    }
+#pragma unroll
+    for (int k = 0; k < kWords<DT>; ++k) w[k] = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < cnt) {
+        if constexpr (DT == CIN_DT_F32)
+          w[e] = reinterpret_cast<const uint32_t*>(q)[e];
+        else
+          w[e / 2] |= (uint32_t) reinterpret_cast<const uint16_t*>(q)[e] << (16 * (e & 1));
+      }
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int k = 0; k < kWords<DT>; ++k) w[k] = 0;
+  }
+  // What was widened before is widened again, instead of staying in twice the registers.
+  __device__ __forceinline__ void forget() {
+    if constexpr (DT != CIN_DT_F32) {
+#pragma unroll
+      for (int k = 0; k < kWords<DT>; ++k) asm volatile("" : "+v"(w[k]));
+    }
+  }
+  __device__ __forceinline__ float at(int e) const {
+    if constexpr (DT == CIN_DT_F32) return __uint_as_float(w[e]);
+    return half_bits_to_f32(DT, (uint16_t)(w[e / 2] >> (16 * (e & 1))));
+  }
+};
+
+template <int DT>
+__device__ __forceinline__ void store_unit(void* p, int64_t i, int cnt, const float (&v)[8]) {
+  constexpr int es = DT == CIN_DT_F32 ? 4 : 2;
+  uint8_t* q = static_cast<uint8_t*>(p) + i * es;
+  uint32_t w[kWords<DT>];
+#pragma unroll
+  for (int k = 0; k < kWords<DT>; ++k) {
+    if constexpr (DT == CIN_DT_F32)
+      w[k] = __float_as_uint(v[k]);
+    else
+      w[k] = f32x2_to_half2_bits<DT>(v[2 * k], v[2 * k + 1]);
+  }
+  if (__builtin_expect(cnt == 8, 1)) {
+    __builtin_memcpy(q, w, 16);
+    if constexpr (DT == CIN_DT_F32) __builtin_memcpy(q + 16, w + 4, 16);
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (e < cnt) {
+      if constexpr (DT == CIN_DT_F32)
+        reinterpret_cast<uint32_t*>(q)[e] = w[e];
+      else
+        reinterpret_cast<uint16_t*>(q)[e] = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
+    }
+}
+
+__device__ inline void store_elem(void* p, int dt, int64_t i, float v) {
+  if (dt == CIN_DT_F32)
+    static_cast<float*>(p)[i] = v;
+  else
+    static_cast<uint16_t*>(p)[i] = (uint16_t)f32_to_half_bits(dt, v);
+}
+
+// 8 channels of a vector, `none` where there is no vector.
+__device__ __forceinline__ void load_channels(const Vec& vec, int i, int cnt, float none, float (&v)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = none;
+  if (!vec.p) return;
+  if (vec.dtype == CIN_DT_F32) {
+    Unit<CIN_DT_F32> u;
+    u.load(vec.p, i, cnt);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = u.at(e);
+  } else {
+    Unit<CIN_DT_BF16> u;
+    u.load(vec.p, i, cnt);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = half_bits_to_f32(vec.dtype, (uint16_t)(u.w[e / 2] >> (16 * (e & 1))));
+  }
+}
+
+__device__ __forceinline__ float row16_sum(float v) {
+  v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0xB1, 0xF, 0xF, true));
+  v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x4E, 0xF, 0xF, true));
+  v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x141, 0xF, 0xF, true));
+  v += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x140, 0xF, 0xF, true));
+  return v;
+}
+__device__ __forceinline__ float wave_sum(float v) {
+  v = row16_sum(v);
+  v += __shfl_xor(v, 16);
+  v += __shfl_xor(v, 32);
+  return v;
+}
+
+// Sums of a row's values over its threads, every thread getting them.  A workgroup's sums go through LDS: the
+// buffers take turns, and two reductions lie between a buffer's readers and its next writers, of which
+// each passes a barrier.
+template <bool WAVE, int N>
+struct RowSum {
+  float (*lds)[N][kMaxThreads / 64];  // [2]
+  int turn = 0;
+  __device__ __forceinline__ void operator()(float (&v)[N], int waves) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = wave_sum(v[k]);
+    if constexpr (!WAVE) {
+      const int wave = threadIdx.x >> 6;
+      if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) lds[turn][k][wave] = v[k];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        float s = 0.0f;
+        for (int i = 0; i < waves; ++i) s += lds[turn][k][i];
+        v[k] = s;
+      }
+      turn ^= 1;
+    }
+  }
+};
+
+// Channels of one thread: CH chunks of 8, `threads` chunks apart.
+template <int CH>
+struct Span {
+  int at[CH], cnt[CH];
+  __device__ __forceinline__ void set(int lane, int threads, int D) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      at[c] = (c * threads + lane) * 8;
+      cnt[c] = min(max(D - at[c], 0), 8);
+    }
+  }
+};
+
+// FULL: with post norm, gate or learned scale; else x = scale_value r + y.  WAVE: a row a wave.
+template <int DT, int DR, int CH, bool WAVE, bool FULL>
+__global__ __launch_bounds__(WAVE ? 64 * kWaveRows : kMaxThreads) void k_norm_forward(NormArgs a) {
+  __shared__ float lds[2][1][kMaxThreads / 64];
+  RowSum<WAVE, 1> sum{lds};
+  const int lane = WAVE ? threadIdx.x & 63 : threadIdx.x;
+  const int waves = blockDim.x >> 6;
+  const int64_t step = WAVE ? (int64_t)gridDim.x * kWaveRows : gridDim.x;
+  int64_t row = WAVE ? (int64_t)blockIdx.x * kWaveRows + (threadIdx.x >> 6) : blockIdx.x;
+  if (row >= a.T) return;
+  Span<CH> s;
+  s.set(lane, a.threads, a.D);
+  float w[CH][8], pw[FULL ? CH : 1][8], g[FULL ? CH : 1][8], sc[FULL ? CH : 1][8];
+  const float inv_d = 1.0f / (float)a.D;
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    load_channels(a.w, s.at[c], s.cnt[c], 1.0f, w[c]);
+    if constexpr (FULL) {
+      load_channels(a.pw, s.at[c], s.cnt[c], 1.0f, pw[c]);
+      load_channels(a.gate_kind == kChannel ? a.gate : Vec{nullptr, 0}, s.at[c], s.cnt[c], 1.0f, g[c]);
+      load_channels(a.scale_kind == kPerChannel ? a.scale : Vec{nullptr, 0}, s.at[c], s.cnt[c], a.scale_value, sc[c]);
+    }
+  }
+  float scale = a.scale_value;
+  if (FULL && a.scale_kind == kOneValue) {
+    scale = load_elem(a.scale.p, a.scale.dtype, 0);
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sc[c][e] = scale;
+  }
+  for (; row < a.T; row += step) {
+    Unit<DT> y[CH], ge[FULL ? CH : 1];
+    Unit<DR> r[CH];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      y[c].load(a.y, row * a.ldy + s.at[c], s.cnt[c]);
+      if (a.r)
+        r[c].load(a.r, row * a.ldr + s.at[c], s.cnt[c]);
+      else
+        r[c].zero();
+      if constexpr (FULL)
+        if (a.gate_kind == kElement) ge[c].load(a.gate.p, row * a.ldg + s.at[c], s.cnt[c]);
+    }
+    float grow = 1.0f, j = 1.0f;
+    if constexpr (FULL) {
+      if (a.gate_kind == kRow) grow = load_elem(a.gate.p, a.gate.dtype, row * a.ldg);
+      if (a.pw.p) {
+        float q[1] = {0.0f};
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) q[0] = __builtin_fmaf(y[c].at(e), y[c].at(e), q[0]);
+        sum(q, waves);
+        j = 1.0f / sqrtf(q[0] * inv_d + a.eps);
+      }
+    }
+    float x[CH][8], q[1] = {0.0f};
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float u = y[c].at(e);
+        if constexpr (FULL) {
+          if (a.pw.p) u = u * j * pw[c][e];
+          u *= a.gate_kind == kElement ? ge[c].at(e) : a.gate_kind == kRow ? grow : g[c][e];
+          x[c][e] = a.r ? __builtin_fmaf(sc[c][e], r[c].at(e), u) : u;
+        } else {
+          x[c][e] = a.r ? __builtin_fmaf(scale, r[c].at(e), u) : u;
+        }
+        q[0] = __builtin_fmaf(x[c][e], x[c][e], q[0]);
+      }
+      if (a.x && s.cnt[c] > 0) store_unit<DR>(a.x, row * a.D + s.at[c], s.cnt[c], x[c]);
+    }
+    sum(q, waves);
+    const float i = 1.0f / sqrtf(q[0] * inv_d + a.eps);
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[c][e] = x[c][e] * i * w[c][e];
+      if (s.cnt[c] > 0) store_unit<DT>(a.n, row * a.D + s.at[c], s.cnt[c], x[c]);
+    }
+    if (a.stats && lane == 0) {
+      a.stats[row] = i;
+      a.stats[a.T + row] = j;
+    }
+  }
+}
+
+// Partial sums of one workgroup: of its waves' rows together where each has its own.
+template <int CH, bool WAVE>
+__device__ __forceinline__ void leave_partial(const NormArgs& a, int which, const float (&v)[CH][8], const Span<CH>& s,
+                                              float* lds) {
+  float* out = a.partial + ((int64_t)which * gridDim.x + blockIdx.x) * a.D;
+  if constexpr (WAVE) {
+    constexpr int kW = 64 * CH * 8;
+    __syncthreads();  // (the buffer's readers before)
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) lds[(threadIdx.x >> 6) * kW + s.at[c] + e] = v[c][e];
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.D; i += 64 * kWaveRows) {
+      float t = lds[i];
+#pragma unroll
+      for (int k = 1; k < kWaveRows; ++k) t += lds[k * kW + i];
+      out[i] = t;
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+      if (s.cnt[c] > 0) store_unit<CIN_DT_F32>(out, s.at[c], s.cnt[c], v[c]);
+  }
+}
+
+// What a row of the backward reads.
+template <int DT, int DR, int CH, bool FULL>
+struct RowIn {
+  Unit<DT> y[CH], gn[CH], ge[FULL ? CH : 1];
+  Unit<DR> r[CH], gx[CH];
+  float i, j, gate;
+  __device__ __forceinline__ void load(const NormArgs& a, int64_t row, const Span<CH>& s) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      y[c].load(a.y, row * a.ldy + s.at[c], s.cnt[c]);
+      if (a.r)
+        r[c].load(a.r, row * a.ldr + s.at[c], s.cnt[c]);
+      else
+        r[c].zero();
+      if (a.gn)
+        gn[c].load(a.gn, row * a.ldgn + s.at[c], s.cnt[c]);
+      else
+        gn[c].zero();
+      if (a.gx)
+        gx[c].load(a.gx, row * a.ldgx + s.at[c], s.cnt[c]);
+      else
+        gx[c].zero();
+      if constexpr (FULL)
+        if (a.gate_kind == kElement) ge[c].load(a.gate.p, row * a.ldg + s.at[c], s.cnt[c]);
+    }
+    i = a.stats[row];
+    j = FULL ? a.stats[a.T + row] : 1.0f;
+    gate = FULL && a.gate_kind == kRow ? load_elem(a.gate.p, a.gate.dtype, row * a.ldg) : 1.0f;
+  }
+};
+
+// A channel's sums for the gate and the scale lie in LDS, each thread's own (they are rare, and in
+// registers they would halve the waves of a CU): 8 of chunk c at [(which CH + c) 2 + half][thread].
+template <int CH>
+struct LdsSums {
+  float4* at;
+  __device__ __forceinline__ float4& part(int which, int c, int half) const {
+    return at[((which * CH + c) * 2 + half) * blockDim.x + threadIdx.x];
+  }
+  __device__ __forceinline__ void clear() const {
+#pragma unroll
+    for (int k = 0; k < 4 * CH; ++k) at[k * blockDim.x + threadIdx.x] = float4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  __device__ __forceinline__ void add(int which, int c, const float (&v)[8]) const {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float4 t = part(which, c, h);
+      t.x += v[4 * h];
+      t.y += v[4 * h + 1];
+      t.z += v[4 * h + 2];
+      t.w += v[4 * h + 3];
+      part(which, c, h) = t;
+    }
+  }
+  __device__ __forceinline__ void get(int which, float (&v)[CH][8]) const {
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float4 t = part(which, c, h);
+        v[c][4 * h] = t.x;
+        v[c][4 * h + 1] = t.y;
+        v[c][4 * h + 2] = t.z;
+        v[c][4 * h + 3] = t.w;
+      }
+  }
+};
+
+template <int DT, int DR, int CH, bool WAVE, bool FULL>
+__global__ __launch_bounds__(WAVE ? 64 * kWaveRows : kMaxThreads) void k_norm_backward(NormArgs a) {
+  __shared__ float lds1[2][1][kMaxThreads / 64], lds2[2][2][kMaxThreads / 64];
+  __shared__ float joined[WAVE ? kWaveRows * 64 * CH * 8 : 1];
+  extern __shared__ float4 channel_sums[];  // where the gate or the scale is one a channel
+  RowSum<WAVE, 1> sum1{lds1};
+  RowSum<WAVE, 2> sum2{lds2};
+  const LdsSums<CH> sums{channel_sums};
+  const int lane = WAVE ? threadIdx.x & 63 : threadIdx.x;
+  const int waves = blockDim.x >> 6;
+  const int64_t step = WAVE ? (int64_t)gridDim.x * kWaveRows : gridDim.x;
+  int64_t row = WAVE ? (int64_t)blockIdx.x * kWaveRows + (threadIdx.x >> 6) : blockIdx.x;
+  Span<CH> s;
+  s.set(lane, a.threads, a.D);
+  constexpr int F = FULL ? CH : 1;
+  float w[CH][8], pw[F][8], one = a.scale_value;
+  float sw[CH][8], spw[F][8], sone = 0.0f;
+  const float inv_d = 1.0f / (float)a.D;
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    load_channels(a.w, s.at[c], s.cnt[c], 1.0f, w[c]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sw[c][e] = 0.0f;
+    if constexpr (FULL) {
+      load_channels(a.pw, s.at[c], s.cnt[c], 1.0f, pw[c]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) spw[c][e] = 0.0f;
+    }
+  }
+  if constexpr (FULL) {
+    if (a.gate_kind == kChannel || a.scale_kind == kPerChannel) sums.clear();
+    if (a.scale_kind == kOneValue) one = load_elem(a.scale.p, a.scale.dtype, 0);
+  }
+  // A workgroup's waves wait for each other twice a row, so the next row's loads go out before; waves with rows
+  // of their own cover each other's (and fp32 rows are as many bytes without).
+  constexpr bool kAhead = !WAVE && CH == 1 && DR != CIN_DT_F32;
+  RowIn<DT, DR, CH, FULL> in, next;
+  if (kAhead && row < a.T) next.load(a, row, s);
+  for (; row < a.T; row += step) {
+    if constexpr (kAhead) {
+      in = next;
+      if (row + step < a.T) next.load(a, row + step, s);
+    } else {
+      in.load(a, row, s);
+    }
+    const float i = in.i, j = in.j;
+    // (a gate or scale per channel is read again each row, from L2: in registers they would cost half the waves)
+    float g[F][8], sc[F][8];
+    if constexpr (FULL) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        if (a.gate_kind == kElement) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) g[c][e] = in.ge[c].at(e);
+        } else {
+          load_channels(a.gate_kind == kChannel ? a.gate : Vec{nullptr, 0}, s.at[c], s.cnt[c], in.gate, g[c]);
+        }
+        load_channels(a.scale_kind == kPerChannel ? a.scale : Vec{nullptr, 0}, s.at[c], s.cnt[c], one, sc[c]);
+      }
+    }
+    auto unit = [&](int c, int e) {  // u, without its gate
+      if constexpr (FULL) return in.y[c].at(e) * j * pw[c][e];
+      return in.y[c].at(e);
+    };
+    auto gate = [&](int c, int e) {
+      if constexpr (FULL) return g[c][e];
+      return 1.0f;
+    };
+    auto scale = [&](int c, int e) {
+      if constexpr (FULL) return sc[c][e];
+      return a.scale_value;
+    };
+    float x[CH][8], q[1] = {0.0f};
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float u = unit(c, e);
+        if constexpr (FULL) u *= gate(c, e);
+        x[c][e] = a.r ? __builtin_fmaf(scale(c, e), in.r[c].at(e), u) : u;
+        q[0] = __builtin_fmaf(in.gn[c].at(e) * w[c][e], x[c][e], q[0]);
+      }
+    sum1(q, waves);
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      in.y[c].forget();
+      in.r[c].forget();
+      in.gn[c].forget();
+    }
+    const float c1 = i * i * (q[0] * inv_d);
+    // x becomes dx
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float t = in.gn[c].at(e);
+        sw[c][e] = __builtin_fmaf(t, x[c][e] * i, sw[c][e]);
+        x[c][e] = __builtin_fmaf(i, __builtin_fmaf(-x[c][e], c1, t * w[c][e]), in.gx[c].at(e));
+      }
+      if (a.dr && s.cnt[c] > 0) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = scale(c, e) * x[c][e];
+        store_unit<DR>(a.dr, row * a.D + s.at[c], s.cnt[c], v);
+      }
+    }
+    if constexpr (FULL) {
+      float p[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        if (a.scale_kind != kNumber) {
+          float v[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            v[e] = x[c][e] * in.r[c].at(e);
+            sone += v[e];
+          }
+          if (a.scale_kind == kPerChannel) sums.add(1, c, v);
+        }
+        if (a.gate_kind != kNoGate) {
+          float v[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            v[e] = x[c][e] * unit(c, e);
+            p[1] += v[e];
+          }
+          if (a.gate_kind == kElement && a.dgate && s.cnt[c] > 0) store_unit<DT>(a.dgate, row * a.D + s.at[c], s.cnt[c], v);
+          if (a.gate_kind == kChannel) sums.add(0, c, v);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x[c][e] *= gate(c, e);  // du
+          if (a.pw.p) {
+            spw[c][e] = __builtin_fmaf(x[c][e], in.y[c].at(e) * j, spw[c][e]);
+            p[0] = __builtin_fmaf(x[c][e] * pw[c][e], in.y[c].at(e), p[0]);
+          }
+        }
+      }
+      if (a.pw.p || a.gate_kind == kRow) sum2(p, waves);
+      if (a.pw.p) {
+        const float c2 = j * j * (p[0] * inv_d);
+#pragma unroll
+        for (int c = 0; c < CH; ++c) in.y[c].forget();
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[c][e] = j * __builtin_fmaf(-in.y[c].at(e), c2, x[c][e] * pw[c][e]);
+      }
+      if (a.gate_kind == kRow && a.dgate && lane == 0) store_elem(a.dgate, a.gate.dtype, row, p[1]);
+    }
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+      if (a.dy && s.cnt[c] > 0) store_unit<DT>(a.dy, row * a.D + s.at[c], s.cnt[c], x[c]);
+  }
+  if (!a.partial) return;
+  leave_partial<CH, WAVE>(a, kSumW, sw, s, joined);
+  if constexpr (FULL) {
+    if (a.pw.p) leave_partial<CH, WAVE>(a, kSumPw, spw, s, joined);
+    if (a.gate_kind == kChannel) {
+      sums.get(0, sw);
+      leave_partial<CH, WAVE>(a, kSumGate, sw, s, joined);
+    }
+    if (a.scale_kind == kPerChannel) {
+      sums.get(1, sw);
+      leave_partial<CH, WAVE>(a, kSumScale, sw, s, joined);
+    }
+    if (a.scale_kind == kOneValue) {
+      __shared__ float ones[kMaxThreads / 64];
+      const float t = wave_sum(sone);
+      if ((threadIdx.x & 63) == 0) ones[threadIdx.x >> 6] = t;
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        float v = 0.0f;
+        for (int k = 0; k < waves; ++k) v += ones[k];
+        a.partial[(int64_t)kSums * gridDim.x * a.D + blockIdx.x] = v;
+      }
+    }
+  }
+}
+
+struct ColumnArgs {
+  const float* partial;
+  int64_t G;  // partial rows
+  int D;
+  void* out[kSums];
+  int dtype[kSums];
+  void* one;
+  int one_dtype;
+};
+
+// The partial rows' sums, each in the order of the rows: 32 channels a workgroup, 32 lines of rows; the
+// last workgroup of blockIdx.x has the learned scale's.
+__global__ __launch_bounds__(1024) void k_norm_columns(ColumnArgs a) {
+  __shared__ float lds[32][33];
+  const int col = threadIdx.x & 31, line = threadIdx.x >> 5;
+  const int groups = (a.D + 31) / 32;
+  if ((int)blockIdx.x == groups) {
+    if (blockIdx.y != 0 || !a.one) return;
+    const float* p = a.partial + (int64_t)kSums * a.G * a.D;
+    float t = 0.0f;
+    for (int64_t i = threadIdx.x; i < a.G; i += 1024) t += p[i];
+    lds[line][col] = t;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      float v = 0.0f;
+      for (int l = 0; l < 32; ++l)
+        for (int c = 0; c < 32; ++c) v += lds[l][c];
+      store_elem(a.one, a.one_dtype, 0, v);
+    }
+    return;
+  }
+  void* out = a.out[blockIdx.y];
+  if (!out) return;
+  const int d = blockIdx.x * 32 + col;
+  float t = 0.0f;
+  if (d < a.D) {
+    const float* p = a.partial + (int64_t)blockIdx.y * a.G * a.D + d;
+#pragma unroll 8
+    for (int64_t i = line; i < a.G; i += 32) t += p[i * a.D];
+  }
+  lds[line][col] = t;
+  __syncthreads();
+  if (line == 0 && d < a.D) {
+    for (int l = 1; l < 32; ++l) t += lds[l][col];
+    store_elem(out, a.dtype[blockIdx.y], d, t);
+  }
+}
+
+// Chunks of a thread, threads of a row and whether a wave takes a row.
+struct Shape {
+  int chunks, threads;
+  bool wave;
+};
+Shape shape_of(int64_t D) {
+  const int64_t units = cdiv(D, 8);
+  if (units <= 64) return {1, 64, true};
+  if (units <= 128) return {2, 64, true};
+  const int chunks = units <= kMaxThreads ? 1 : 2;
+  return {chunks, (int)(cdiv(cdiv(units, chunks), 64) * 64), false};
+}
+
+// Workgroups that walk over the rows.
+int64_t groups_of(int64_t T, const Shape& s, bool backward) {
+  const int64_t rows = s.wave ? cdiv(T, kWaveRows) : T;
+  const int64_t waves = s.wave ? kWaveRows : s.threads / 64;
+  const int64_t each = (backward ? 16 : 32) / waves;
+  const int64_t most = (int64_t)cin_device_cus() * (each > 1 ? each : 1);
+  return rows < most ? rows : most;
+}
+
+template <class K>
+void allow_lds(K kernel, size_t bytes) {
+  if (bytes > 65536) (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+}
+
+template <int DT, int DR, int CH, bool WAVE>
+void launch(const NormArgs& a, const Shape& s, int64_t groups, bool full, bool backward, hipStream_t stream) {
+  const dim3 grid((uint32_t)groups), block(s.wave ? 64 * kWaveRows : s.threads);
+  if (backward) {
+    if (full) {
+      const bool sums = a.gate_kind == kChannel || a.scale_kind == kPerChannel;
+      const size_t lds = sums ? (size_t)block.x * CH * 64 : 0;
+      allow_lds(k_norm_backward<DT, DR, CH, WAVE, true>, lds);
+      hipLaunchKernelGGL((k_norm_backward<DT, DR, CH, WAVE, true>), grid, block, lds, stream, a);
+    } else {
+      hipLaunchKernelGGL((k_norm_backward<DT, DR, CH, WAVE, false>), grid, block, 0, stream, a);
+    }
+  } else {
+    if (full)
+      hipLaunchKernelGGL((k_norm_forward<DT, DR, CH, WAVE, true>), grid, block, 0, stream, a);
+    else
+      hipLaunchKernelGGL((k_norm_forward<DT, DR, CH, WAVE, false>), grid, block, 0, stream, a);
+  }
+}
+
+template <int DT, int DR>
+void launch_shape(const NormArgs& a, const Shape& s, int64_t groups, bool full, bool backward, hipStream_t stream) {
+  if (s.wave && s.chunks == 1)
+    launch<DT, DR, 1, true>(a, s, groups, full, backward, stream);
+  else if (s.wave)
+    launch<DT, DR, 2, true>(a, s, groups, full, backward, stream);
+  else if (s.chunks == 1)
+    launch<DT, DR, 1, false>(a, s, groups, full, backward, stream);
+  else
+    launch<DT, DR, 2, false>(a, s, groups, full, backward, stream);
+}
+
+void launch_types(const NormArgs& a, int dt, int dr, const Shape& s, int64_t groups, bool full, bool backward,
+                  hipStream_t stream) {
+  if (dt == CIN_DT_BF16 && dr == CIN_DT_BF16)
+    launch_shape<CIN_DT_BF16, CIN_DT_BF16>(a, s, groups, full, backward, stream);
+  else if (dt == CIN_DT_BF16)
+    launch_shape<CIN_DT_BF16, CIN_DT_F32>(a, s, groups, full, backward, stream);
+  else if (dt == CIN_DT_F16 && dr == CIN_DT_F16)
+    launch_shape<CIN_DT_F16, CIN_DT_F16>(a, s, groups, full, backward, stream);
+  else if (dt == CIN_DT_F16)
+    launch_shape<CIN_DT_F16, CIN_DT_F32>(a, s, groups, full, backward, stream);
+  else
+    launch_shape<CIN_DT_F32, CIN_DT_F32>(a, s, groups, full, backward, stream);
+}
+
+bool is_type(int dt) { return dt == CIN_DT_BF16 || dt == CIN_DT_F16 || dt == CIN_DT_F32; }
+
+// Checks of what both directions take; fills the arguments.
+int common_args(NormArgs& a, const char* name, const void* y, int dtype, int64_t ldy, const void* r, int r_dtype,
+                int64_t ldr, int64_t T, int64_t D, const void* w, int w_dtype, const void* pw, int pw_dtype, const void* gate,
+                int gate_dtype, int gate_kind, int64_t ldg, const void* scale, int scale_dtype, int scale_kind,
+                float scale_value, float eps) {
+  CIN_CHECK_ARG(is_type(dtype) && is_type(r_dtype), "%s: dtype must be bf16, fp16 or fp32", name);
+  CIN_CHECK_ARG(r_dtype == dtype || r_dtype == CIN_DT_F32, "%s: the residual must have y's dtype or fp32", name);
+  CIN_CHECK_ARG(T >= 0 && T < (1LL << 40) && D >= 1 && D <= kMaxWidth, "%s: D must be in [1, %lld]", name, (long long)kMaxWidth);
+  CIN_CHECK_ARG(ldy >= D && (!r || ldr >= D), "%s: row stride below D", name);
+  CIN_CHECK_ARG((!w || is_type(w_dtype)) && (!pw || is_type(pw_dtype)), "%s: weights must be bf16, fp16 or fp32", name);
+  CIN_CHECK_ARG(gate_kind >= kNoGate && gate_kind <= kElement && (gate != nullptr) == (gate_kind != kNoGate) &&
+                    (!gate || is_type(gate_dtype)),
+                "%s: bad gate", name);
+  CIN_CHECK_ARG(gate_kind != kElement || (gate_dtype == dtype && ldg >= D), "%s: a gate of elements must have y's dtype and rows of D",
+                name);
+  CIN_CHECK_ARG(gate_kind != kRow || ldg >= 1, "%s: bad gate stride", name);
+  CIN_CHECK_ARG(scale_kind >= kNumber && scale_kind <= kPerChannel && (scale != nullptr) == (scale_kind != kNumber) &&
+                    (!scale || is_type(scale_dtype)),
+                "%s: bad residual scale", name);
+  a = {};
+  a.y = y;
+  a.r = r;
+  a.ldy = ldy;
+  a.ldr = ldr;
+  a.T = T;
+  a.D = (int)D;
+  a.w = {w, w_dtype};
+  a.pw = {pw, pw_dtype};
+  a.gate = {gate, gate_dtype};
+  a.scale = {scale, scale_dtype};
+  a.gate_kind = gate_kind;
+  a.scale_kind = scale_kind;
+  a.ldg = ldg;
+  a.scale_value = scale_value;
+  a.eps = eps;
+  return CIN_OK;
+}
+
+bool is_full(const NormArgs& a) { return a.pw.p || a.gate_kind != kNoGate || a.scale_kind != kNumber; }
+
+}  // namespace
+
+extern "C" {
+
+int cin_block_norm(const void* y, int dtype, int64_t ldy, const void* r, int r_dtype, int64_t ldr, int64_t T, int64_t D,
+                   const void* w, int w_dtype, const void* pw, int pw_dtype, const void* gate, int gate_dtype, int gate_kind,
+                   int64_t ldg, const void* scale, int scale_dtype, int scale_kind, float scale_value, float eps, void* n,
+                   void* x, float* stats, void* stream) {
+  NormArgs a;
+  const int rc = common_args(a, "cin_block_norm", y, dtype, ldy, r, r_dtype, ldr, T, D, w, w_dtype, pw, pw_dtype, gate,
+                             gate_dtype, gate_kind, ldg, scale, scale_dtype, scale_kind, scale_value, eps);
+  if (rc != CIN_OK || T == 0) return rc;
+  CIN_CHECK_ARG(y && n, "cin_block_norm: null pointer");
+  a.n = n;
+  a.x = x;
+  a.stats = stats;
+  const Shape s = shape_of(D);
+  a.threads = s.threads;
+  launch_types(a, dtype, r_dtype, s, groups_of(T, s, false), is_full(a), false, (hipStream_t)stream);
+  return cin_check_launch("cin_block_norm");
+}
+
+int64_t cin_block_norm_workspace(int64_t T, int64_t D) {
+  if (T < 0 || D < 1 || D > kMaxWidth) {
+    cin_set_error(CIN_ERR_ARG, "cin_block_norm_workspace: D must be in [1, %lld]", (long long)kMaxWidth);
+    return -1;
+  }
+  return 4 * groups_of(T, shape_of(D), true) * (kSums * D + 1);
+}
+
+int cin_block_norm_backward(const void* y, int dtype, int64_t ldy, const void* r, int r_dtype, int64_t ldr, int64_t T,
+                            int64_t D, const void* w, int w_dtype, const void* pw, int pw_dtype, const void* gate,
+                            int gate_dtype, int gate_kind, int64_t ldg, const void* scale, int scale_dtype, int scale_kind,
+                            float scale_value, const float* stats, const void* gn, int64_t ldgn, const void* gx,
+                            int64_t ldgx, void* dy, void* dr, void* dw, void* dpw, void* dgate, void* dscale,
+                            void* workspace, int64_t workspace_bytes, void* stream) {
+  NormArgs a;
+  const int rc = common_args(a, "cin_block_norm_backward", y, dtype, ldy, r, r_dtype, ldr, T, D, w, w_dtype, pw, pw_dtype,
+                             gate, gate_dtype, gate_kind, ldg, scale, scale_dtype, scale_kind, scale_value, 0.0f);
+  if (rc != CIN_OK || T == 0) return rc;
+  CIN_CHECK_ARG(y && stats, "cin_block_norm_backward: null pointer");
+  CIN_CHECK_ARG((!gn || ldgn >= D) && (!gx || ldgx >= D), "cin_block_norm_backward: row stride below D");
+  CIN_CHECK_ARG((!dw || w) && (!dpw || pw) && (!dgate || gate) && (!dscale || scale) && (!dr || r),
+                "cin_block_norm_backward: a gradient of an input that is not there");
+  CIN_CHECK_ARG(!dscale || r, "cin_block_norm_backward: a scale without a residual");
+  ColumnArgs c = {};
+  c.out[kSumW] = dw;
+  c.dtype[kSumW] = w_dtype;
+  c.out[kSumPw] = dpw;
+  c.dtype[kSumPw] = pw_dtype;
+  if (gate_kind == kChannel) {
+    c.out[kSumGate] = dgate;
+    c.dtype[kSumGate] = gate_dtype;
+  }
+  if (scale_kind == kPerChannel) {
+    c.out[kSumScale] = dscale;
+    c.dtype[kSumScale] = scale_dtype;
+  } else if (scale_kind == kOneValue) {
+    c.one = dscale;
+    c.one_dtype = scale_dtype;
+  }
+  const bool sums = c.out[0] || c.out[1] || c.out[2] || c.out[3] || c.one;
+  CIN_CHECK_ARG(!sums || (workspace && workspace_bytes >= cin_block_norm_workspace(T, D)),
+                "cin_block_norm_backward: workspace below cin_block_norm_workspace bytes");
+  a.stats = const_cast<float*>(stats);
+  a.gn = gn;
+  a.gx = gx;
+  a.ldgn = ldgn;
+  a.ldgx = ldgx;
+  a.dy = dy;
+  a.dr = dr;
+  a.dgate = dgate;
+  a.partial = sums ? static_cast<float*>(workspace) : nullptr;
+  const Shape s = shape_of(D);
+  a.threads = s.threads;
+  const int64_t groups = groups_of(T, s, true);
+  launch_types(a, dtype, r_dtype, s, groups, is_full(a), true, (hipStream_t)stream);
+  if (sums) {
+    c.partial = a.partial;
+    c.G = groups;
+    c.D = (int)D;
+    const int rows = c.out[3] ? 4 : c.out[2] ? 3 : c.out[1] ? 2 : 1;
+    hipLaunchKernelGGL(k_norm_columns, dim3((uint32_t)(cdiv(D, 32) + (c.one ? 1 : 0)), rows), dim3(1024), 0, (hipStream_t)stream, c);
+  }
+  return cin_check_launch("cin_block_norm_backward");
+}
+
+}  // extern "C"

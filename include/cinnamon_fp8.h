@@ -584,6 +584,39 @@ int cin_linear_ce_backward(const void* xc, int dtype, int64_t T, int64_t D, cons
                            int64_t grad_stride, int mean, void* dx, void* dw, void* workspace,
                            int64_t workspace_bytes, const float* logits, void* stream);
 
+/*
+ * The end of a block and the norm in front of the next (reference src/norm.py:15-17 and the residual sums of
+ * src/layers.py:202), with norm(v) = v / sqrt(mean(v^2) + eps) over a row:
+ *   x = a r + g u,  u = norm(y) pw (u = y where pw is null);   n = norm(x) w (w null: ones)
+ *   y [T, D] of dtype (row stride ldy); r [T, D] of r_dtype, dtype or fp32 (row stride ldr), or null: x = g u;
+ *   w, pw [D]; gate by gate_kind: 0 none, 1 [D], 2 one a row (ldg apart), 3 [T, D] of dtype (row stride ldg);
+ *   scale by scale_kind: 0 the number scale_value, 1 one value, 2 [D]; each vector with its own type.
+ *   n [T, D] of dtype and x [T, D] of r_dtype (or null), contiguous; stats [2, T] fp32 for the backward, or null.
+ * D <= 16384.  Outputs must not overlap the inputs.
+ */
+int cin_block_norm(const void* y, int dtype, int64_t ldy, const void* r, int r_dtype, int64_t ldr,
+                   int64_t T, int64_t D, const void* w, int w_dtype, const void* pw, int pw_dtype,
+                   const void* gate, int gate_dtype, int gate_kind, int64_t ldg, const void* scale,
+                   int scale_dtype, int scale_kind, float scale_value, float eps, void* n, void* x,
+                   float* stats, void* stream);
+
+/*
+ * Gradients of cin_block_norm from those of n (gn [T, D] of dtype) and x (gx [T, D] of r_dtype), either
+ * null for none; stats as the forward left them.  dy, dr, dw, dpw, dgate, dscale: contiguous, shape and type
+ * of their input, any of them null.  The workspace, cin_block_norm_workspace(T, D) bytes for the current
+ * device on 16 bytes, is needed for dw, dpw, dscale and a dgate of channels (-1 for sizes that are refused).
+ * Bit-identical from call to call.
+ */
+int64_t cin_block_norm_workspace(int64_t T, int64_t D);
+int cin_block_norm_backward(const void* y, int dtype, int64_t ldy, const void* r, int r_dtype,
+                            int64_t ldr, int64_t T, int64_t D, const void* w, int w_dtype,
+                            const void* pw, int pw_dtype, const void* gate, int gate_dtype,
+                            int gate_kind, int64_t ldg, const void* scale, int scale_dtype,
+                            int scale_kind, float scale_value, const float* stats, const void* gn,
+                            int64_t ldgn, const void* gx, int64_t ldgx, void* dy, void* dr, void* dw,
+                            void* dpw, void* dgate, void* dscale, void* workspace,
+                            int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
