@@ -93,11 +93,13 @@ SIGNATURES: dict[str, list] = {
     "cin_block_norm": _NORM + [_f32, _p, _p, _p, _p],
     "cin_block_norm_backward": _NORM + [_p] + [_p, _i64] * 2 + [_p] * 6 + [_p, _i64, _p],
     "cin_block_norm_workspace": [_i64, _i64],
+    "cin_verify_drafts": [_p, _i64, _i64] * 3 + [_i32, _i64, _i64, _i64, _p, _i32, _i64, _i64, _p, _i64, _p, _p, _p, _i64, _p],
+    "cin_verify_drafts_workspace": [_i64, _i64, _i64],
 }
 
 # entry points that return something other than an int status
 RESTYPES = {"cin_indexer_weights_grad_workspace": ctypes.c_int64, "cin_linear_ce_workspace": ctypes.c_int64,
-            "cin_block_norm_workspace": ctypes.c_int64}
+            "cin_block_norm_workspace": ctypes.c_int64, "cin_verify_drafts_workspace": ctypes.c_int64}
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None

@@ -1,4 +1,5 @@
-"""The output projection and the softmax cross entropy over a large vocabulary in one operator.
+"""The vocabulary's end of the model: the output projection with its cross entropy, and the verification of
+drafted tokens.
 
 The reference keeps lm_head out of FP8 (src/kernels.py:863-867) and trains on
 cross_entropy(lm_head(x), targets) for the main and the MTP heads (src/train.py:355-372), which
@@ -6,6 +7,10 @@ writes the logits [n_tokens, vocabulary], their log-softmax and its gradient.
 ``linear_cross_entropy`` computes loss and gradients by pieces of the vocabulary on bf16, fp16 or
 fp32 matrix units (csrc/lm_head.hip); only those of few rows of a wide model, fewer bytes than the
 weight, are ever kept.
+
+The reference trains heads that predict further tokens (MTP, src/layers.py:215-241).  ``verify_drafts`` is the step
+that uses them: drafted tokens are kept or replaced so that the result is distributed as the target's
+(csrc/verify.hip).
 """
 from __future__ import annotations
 
@@ -16,9 +21,9 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import call_on, dtype_code, ptr, stream_of
-from .kernels import _cdiv, _plain_eager, _require, custom_op
+from .kernels import _cdiv, _plain_eager, _require, _run, custom_op
 
-__all__ = ["linear_cross_entropy"]
+__all__ = ["linear_cross_entropy", "verify_drafts"]
 
 _PLAIN = (torch.Tensor, torch.nn.Parameter)
 _MODES = {"none": 0, "sum": 1, "mean": 2}
@@ -225,3 +230,82 @@ def _backward(ctx, grad, _state):
 
 
 _forward_op.register_autograd(_backward, setup_context=_setup)
+
+
+# ---------------------------------------------------------------------------
+# Drafted tokens
+# ---------------------------------------------------------------------------
+MAX_DRAFTS = 63
+
+
+def verify_drafts(draft_tokens: torch.Tensor, draft_probs: torch.Tensor | None, target_probs: torch.Tensor,
+                  uniforms: torch.Tensor, n_drafts: torch.Tensor | None = None):
+    """Drafted tokens against the target's probabilities, from given random numbers: (tokens int64
+    [B, K + 1], accepted int64 [B]), distributed as tokens drawn from target_probs one by one.
+
+    draft_tokens [B, K] integers, drawn from draft_probs [B, K, V]; target_probs [B, K + 1, V], the target's
+    at each draft's position and after the last; bf16, fp16 or fp32, one type for both.  uniforms [B, K + 1] in
+    [0, 1), fp32 or fp64.  n_drafts [B] integers: sequence b has that many drafts (default K, clamped to
+    [0, K]); its row n_drafts[b] of target_probs is the one after the last.  draft_probs None: the drafts were certain of
+    their tokens (a greedy draft).  K may be 0: a draw from target_probs[:, 0].
+
+    Position i keeps its token x while uniforms[i] * draft_probs[i, x] < target_probs[i, x] (a token
+    outside [0, V) is not kept).  With n = accepted tokens kept, tokens[n] is drawn by uniforms[K] from
+    max(target_probs[n] - draft_probs[n], 0), or from target_probs[n] past the last draft or where nothing is left:
+    the first token at which the running sum exceeds uniforms[K] times the whole.  Behind it tokens is -1; it is
+    -1 itself where the sum is not positive and finite.  Products, differences and sums are in 64 bits; rows need not
+    sum to one.  No gradient."""
+    for t in (draft_tokens, draft_probs, target_probs, uniforms, n_drafts):
+        _require(t is None or (t.is_cuda and t.device == target_probs.device), "Inputs must be on one CUDA device")
+    _require(draft_tokens.ndim == 2 and target_probs.ndim == 3, "draft_tokens must be [B, K] and target_probs [B, K + 1, V]")
+    (B, K), V = draft_tokens.shape, target_probs.shape[2]
+    _require(K <= MAX_DRAFTS, f"at most {MAX_DRAFTS} drafts")
+    _require(target_probs.shape == (B, K + 1, V) and V >= 1, "target_probs must be [B, K + 1, V]")
+    _require(target_probs.dtype in _DTYPES, "probabilities must be bf16, fp16 or fp32")
+    _require(draft_probs is None or (draft_probs.shape == (B, K, V) and draft_probs.dtype == target_probs.dtype),
+             "draft_probs must be [B, K, V] in target_probs' dtype")
+    _require(uniforms.shape == (B, K + 1) and uniforms.dtype in (torch.float32, torch.float64),
+             "uniforms must be [B, K + 1] in fp32 or fp64")
+    for t, shape in ((draft_tokens, (B, K)), (n_drafts, (B,))):
+        _require(t is None or (t.shape == shape and not t.dtype.is_floating_point and not t.dtype.is_complex
+                               and t.dtype != torch.bool), "draft_tokens and n_drafts must hold integers, n_drafts [B] of them")
+    if draft_tokens.dtype != torch.int64:
+        draft_tokens = draft_tokens.to(torch.int64)
+    if n_drafts is not None and n_drafts.dtype != torch.int64:
+        n_drafts = n_drafts.to(torch.int64)
+    return _run(_verify_op, draft_tokens, None if draft_probs is None else draft_probs.detach(), target_probs.detach(),
+                uniforms.detach(), n_drafts)
+
+
+@functools.lru_cache(maxsize=256)
+def _verify_workspace(B, K, V, device):
+    with torch.cuda.device(device):  # (the device's CUs decide)
+        n = _lib.load().cin_verify_drafts_workspace(B, K, V)
+    if n < 0:
+        raise ValueError(f"verify_drafts: {_lib.last_error()}")
+    return n
+
+
+def _channels(t):
+    return t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+@custom_op("verify_drafts", "(Tensor tokens, Tensor? draft, Tensor target, Tensor uniforms, Tensor? counts) -> (Tensor, Tensor)")
+def _verify_op(tokens, draft, target, uniforms, counts):
+    draft, target = _channels(draft), _channels(target)
+    (B, K), V = tokens.shape, target.shape[2]
+    out = tokens.new_empty((B, K + 1))
+    accepted = tokens.new_empty((B,))
+    ws = _verify_workspace(B, K, V, target.device)
+    work = torch.empty(ws, dtype=torch.uint8, device=target.device)
+    q = (0, 0, 0) if draft is None else (draft.data_ptr(), draft.stride(0), draft.stride(1))
+    call_on(target, "cin_verify_drafts", tokens.data_ptr(), tokens.stride(0), tokens.stride(1), *q, target.data_ptr(),
+            target.stride(0), target.stride(1), dtype_code(target), B, K, V, uniforms.data_ptr(),
+            uniforms.dtype == torch.float64, uniforms.stride(0), uniforms.stride(1), ptr(counts),
+            0 if counts is None else counts.stride(0), out.data_ptr(), accepted.data_ptr(), work.data_ptr(), ws, stream_of(target))
+    return out, accepted
+
+
+@_verify_op.register_fake
+def _(tokens, draft, target, uniforms, counts):
+    return tokens.new_empty((tokens.shape[0], tokens.shape[1] + 1)), tokens.new_empty((tokens.shape[0],))

@@ -617,6 +617,27 @@ int cin_block_norm_backward(const void* y, int dtype, int64_t ldy, const void* r
                             void* dpw, void* dgate, void* dscale, void* workspace,
                             int64_t workspace_bytes, void* stream);
 
+/*
+ * Drafted tokens against the target's probabilities, from given uniform numbers (the reference trains the
+ * draft heads, src/layers.py:215-241).  Of sequence b, position i < min(counts[b], K) keeps its token x while
+ * u[b, i] q[b, i, x] < p[b, i, x] and x lies in [0, V); with n tokens kept, the next is drawn by u[b, K] from
+ * max(p[b, n] - q[b, n], 0), or where that is all 0, and past the last draft, from max(p[b, n], 0): the first token
+ * at which the running sum exceeds u[b, K] times the whole.  All of it in 64 bits.
+ *   tokens [B, K] int64 (strides stb, stk); q [B, K, V] (strides sqb, sqk, channels adjacent), or null: a draft
+ *   is certain of its token; p [B, K + 1, V] (spb, spk); both of dtype; u [B, K + 1] fp32 or (u_double)
+ *   fp64 (sub, suk); counts [B] int64 (scb apart) or null for K.
+ *   out [B, K + 1] int64: the kept tokens, the drawn one (-1 where the row's sum is not positive and
+ *   finite), then -1; accepted [B] int64: n.
+ * Workspace: cin_verify_drafts_workspace(B, K, V) bytes for the current device, on 16 (-1 for sizes that are
+ * refused).  B <= 65536, K <= 63, V < 2^30, B V < 2^37.
+ */
+int64_t cin_verify_drafts_workspace(int64_t B, int64_t K, int64_t V);
+int cin_verify_drafts(const int64_t* tokens, int64_t stb, int64_t stk, const void* q, int64_t sqb,
+                      int64_t sqk, const void* p, int64_t spb, int64_t spk, int dtype, int64_t B,
+                      int64_t K, int64_t V, const void* u, int u_double, int64_t sub, int64_t suk,
+                      const int64_t* counts, int64_t scb, int64_t* out, int64_t* accepted,
+                      void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
