@@ -84,6 +84,9 @@ SIGNATURES: dict[str, list] = {
     "cin_moe_gate": [_p, _i32, _i64, _p, _i64, _i64, _i64, _i32, _i64, _i64, _i32, _i32, ctypes.c_float, _p, _p,
                      _p, _p],
     "cin_moe_gate_backward": [_p, _i32, _i64, _i64, _i64, _i64, _i32, _i32, ctypes.c_float, _p, _p, _p, _p, _p],
+    "cin_moe_decode": [_p, _i32, _i64, _i64, _i64, _p, _i32, _i64, _i64, _p, _i64, _i32, _i64, _i64, _i32, _i32, _f32, _i32]
+                      + [_p, _p, _p, _p, _i64] * 2 + [_p, _p, _p, _p, _i64, _p],
+    "cin_moe_decode_workspace": [_i32, _i64, _i64, _i64, _i64, _i64, _i64],
     "cin_linear_ce_workspace": [_i32, _i64, _i64, _i64, _i32],
     "cin_linear_ce_forward": [_p, _i32, _i64, _i64, _i64, _p, _i64, _i64, _p, _i64, _i32, _p, _p, _p, _p, _p, _p, _p,
                               _i64, _p, _p],
@@ -99,7 +102,8 @@ SIGNATURES: dict[str, list] = {
 
 # entry points that return something other than an int status
 RESTYPES = {"cin_indexer_weights_grad_workspace": ctypes.c_int64, "cin_linear_ce_workspace": ctypes.c_int64,
-            "cin_block_norm_workspace": ctypes.c_int64, "cin_verify_drafts_workspace": ctypes.c_int64}
+            "cin_block_norm_workspace": ctypes.c_int64, "cin_verify_drafts_workspace": ctypes.c_int64,
+            "cin_moe_decode_workspace": ctypes.c_int64}
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None

@@ -12,7 +12,8 @@ MoE.forward (src/layers.py:126-157):
   sorted_out * sorted_scores, scatter_add_       moe_combine: per-token sum in sorted order
 
 ``routed_experts`` chains those after moe_gate with layers.experts_forward/backward; its gradients reach
-x, the expert weights and the routing scores.  Every launch is a cinnamon_amd:: torch
+x, the expert weights and the routing scores.  ``moe_decode`` is the whole layer, router and shared expert
+included, for the few tokens of a generation step (csrc/moe_decode.hip).  Every launch is a cinnamon_amd:: torch
 operator (torch.compile traces through it).  The sort is stable, so within an expert the
 rows keep token order (the reference's unstable sort may order them differently; each
 row's result does not depend on its position, and the combine adds a token's terms in
@@ -20,10 +21,12 @@ sorted position order, the order of a sequential scatter_add_).
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import layers
+from . import _lib, layers
 from ._lib import call, call_on, dtype_code, ptr, stream_of
 from .kernels import _cdiv, _plain_eager, _require, _run_detached, _scale_buf, custom_op
 
@@ -31,9 +34,11 @@ _ROUTE_CHUNK = 1024  # assignments per route workgroup (csrc/moe.hip kChunk)
 MAX_EXPERTS = 4096
 MAX_TOP_K = 16
 MAX_GROUPS = 64
+MAX_DECODE_TOKENS = 128
+MAX_DECODE_EXPERTS = 1024
 
 __all__ = ["moe_gate", "moe_route", "moe_gather_quantize", "moe_gather_sum", "moe_combine",
-           "moe_combine_backward", "RoutedExpertsFunction", "routed_experts"]
+           "moe_combine_backward", "RoutedExpertsFunction", "routed_experts", "moe_decode"]
 
 
 # ---------------------------------------------------------------------------
@@ -488,3 +493,134 @@ def routed_experts(experts: layers.GroupedExperts, x: torch.Tensor, top_idx: tor
     out = RoutedExpertsFunction.apply(x, experts.w12, experts.w3, top_scores, perm, inv, starts, ends, k,
                                       experts.quantized_weights())
     return out, counts
+
+
+# ---------------------------------------------------------------------------
+# The whole layer for a few tokens (reference src/layers.py:113-157 at generation)
+# ---------------------------------------------------------------------------
+def moe_decode(x: torch.Tensor, router_weight: torch.Tensor, experts, top_k: int, bias: torch.Tensor | None = None,
+               score: str = "sigmoid", n_groups: int = 1, top_groups: int | None = None, group_top: int = 2,
+               renormalize: bool = True, scale: float = 1.0, shared=None, return_routing: bool = False):
+    """The mixture-of-experts layer of a generation step: x [n_tokens, D] (bf16, fp16 or fp32, at most 128
+    tokens) -> out of the same shape and dtype,
+
+      top_idx, top_scores = moe_gate(x @ router_weight.T, top_k, bias, score, n_groups, ...)
+      out_t = sum_j top_scores[t, j] * expert_{top_idx[t, j]}(x_t) + shared(x_t)
+      expert(v) = W3 (silu(W1 v) * (W2 v))
+
+    and with return_routing (out, top_idx int64, top_scores fp32 [n_tokens, top_k]).
+
+    router_weight [E, D] in bf16, fp16 or fp32 (E at most 1024), the other options as in moe_gate; the logits are summed
+    and the experts chosen in 64 bits.  experts: a layers.GroupedExperts, whose FP8 weights are used (kept between
+    calls with its weight cache, else quantized in every call), or (w12, w12_scales, w3, w3_scales): w12
+    [E, 2 H, D] (W1 above W2) and w3 [E, D, H], either e4m3 codes with fp32 scales of 128 x 128 blocks
+    ([E, ceil(2 H / 128), ceil(D / 128)] and [E, ceil(D / 128), ceil(H / 128)], as
+    layers.quantize_expert_weights returns them) or bf16 with None for the scales.  shared: None or such a tuple of one
+    expert, without E and with an H of its own.  D and H are multiples of 16.
+
+    Only the chosen experts' weights are read.  Activations stay in 16 bits or more: unlike in routed_experts
+    they are not quantized, products are summed in fp32 and the result is rounded once.  Inference only: no
+    gradient.  Bit-identical from call to call."""
+    _require(x.is_cuda, "Input must be on CUDA")
+    _require(x.ndim == 2 and x.shape[0] <= MAX_DECODE_TOKENS, f"x must be [n_tokens, D] with at most {MAX_DECODE_TOKENS} tokens")
+    _require(x.dtype in (torch.bfloat16, torch.float16, torch.float32), "x must be bf16, fp16 or fp32")
+    D = x.shape[1]
+    _require(router_weight.ndim == 2 and router_weight.shape[1] == D and router_weight.device == x.device
+             and router_weight.dtype in (torch.bfloat16, torch.float16, torch.float32),
+             "router_weight must be [E, D] on x's device, in bf16, fp16 or fp32")
+    E = router_weight.shape[0]
+    _require(1 <= E <= MAX_DECODE_EXPERTS, f"n_experts must be in [1, {MAX_DECODE_EXPERTS}]")
+    _require(score in _SCORES, "score must be 'sigmoid' or 'softmax'")
+    _require(1 <= n_groups <= MAX_GROUPS and E % n_groups == 0, f"n_groups must divide n_experts and be in [1, {MAX_GROUPS}]")
+    top_groups = n_groups if top_groups is None else top_groups
+    _require(1 <= top_groups <= n_groups, "top_groups must be in [1, n_groups]")
+    _require(group_top in (1, 2), "group_top must be 1 or 2")
+    _require(1 <= top_k <= min(MAX_TOP_K, top_groups * (E // n_groups)),
+             f"top_k must be in [1, {MAX_TOP_K}] and within the experts of the kept groups")
+    if bias is not None:
+        _require(bias.shape == (E,) and bias.device == x.device and bias.dtype == torch.float32,
+                 "bias must be fp32 [n_experts] on x's device")
+        bias = bias.detach()
+    if isinstance(experts, layers.GroupedExperts):
+        _require(experts.n_experts == E, "the router and the experts differ in number")
+        w12, w3 = experts.w12.detach(), experts.w3.detach()
+        H = experts.hidden_dim
+        q = experts.quantized_weights()
+        (w12q, _, w12s), (w3q, _, w3s) = q if q is not None else layers.quantize_expert_weights(w12, w3)
+        experts = (w12q.view(E, 2 * H, D), w12s.view(E, 2 * H // 128, -1), w3q.view(E, D, H), w3s.view(E, D // 128, -1))
+    weights = _decode_weights(experts, x, (E,))
+    if shared is not None:
+        extra = _decode_weights(shared, x, ())
+        _require(extra[0].dtype == weights[0].dtype, "the shared expert's weights must have the experts' type")
+    else:
+        extra = (None,) * 4
+    out = _run_detached(_decode_op, x, router_weight, bias, *weights, *extra, int(top_k), _SCORES[score], int(n_groups),
+                        int(top_groups), int(group_top), bool(renormalize), float(scale))
+    return out if return_routing else out[0]
+
+
+def _decode_weights(weights, x, lead):
+    """The four tensors of stacked experts (lead (E,)) or of one (()), checked."""
+    _require(isinstance(weights, (tuple, list)) and len(weights) == 4, "expert weights must be (w12, w12_scales, w3, w3_scales)")
+    w12, s12, w3, s3 = weights
+    n = len(lead)
+    D = x.shape[1]
+    _require(w12.ndim == n + 2 and w3.ndim == n + 2, "w12 must be [E, 2 H, D] and w3 [E, D, H]")
+    H = w3.shape[-1]
+    _require(tuple(w12.shape) == (*lead, 2 * H, D) and tuple(w3.shape) == (*lead, D, H), "w12 must be [E, 2 H, D] and w3 [E, D, H]")
+    _require(D >= 16 and H >= 16 and D % 16 == 0 and H % 16 == 0 and max(D, H) <= 65536, "D and H must be multiples of 16 up to 65536")
+    _require(w12.dtype == w3.dtype and w12.dtype in (torch.float8_e4m3fn, torch.bfloat16), "weights must be e4m3 codes or bf16")
+    if w12.dtype == torch.bfloat16:
+        _require(s12 is None and s3 is None, "bf16 weights have no scales")
+    else:
+        _require(s12 is not None and s3 is not None and s12.dtype == s3.dtype == torch.float32
+                 and tuple(s12.shape) == (*lead, _cdiv(2 * H, 128), _cdiv(D, 128))
+                 and tuple(s3.shape) == (*lead, _cdiv(D, 128), _cdiv(H, 128)), "codes need fp32 scales of their 128 x 128 blocks")
+    for t in (w12, s12, w3, s3):
+        _require(t is None or t.device == x.device, "weights must be on x's device")
+    return tuple(None if t is None else t.detach() for t in (w12, s12, w3, s3))
+
+
+@functools.lru_cache(maxsize=256)
+def _decode_workspace(dtype, *sizes):
+    n = _lib.load().cin_moe_decode_workspace(dtype_code(dtype), *sizes)
+    if n < 0:
+        raise ValueError(f"moe_decode: {_lib.last_error()}")
+    return n
+
+
+def _on16(t):
+    """Contiguous, its first element on 16 bytes."""
+    if t is None or (t.is_contiguous() and t.data_ptr() % 16 == 0):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+@custom_op("moe_decode", "(Tensor x, Tensor router, Tensor? bias, Tensor w12, Tensor? s12, Tensor w3, Tensor? s3, Tensor? shared_w12, "
+           "Tensor? shared_s12, Tensor? shared_w3, Tensor? shared_s3, int top_k, int score, int n_groups, int top_groups, "
+           "int group_top, bool renormalize, float scale) -> (Tensor, Tensor, Tensor)")
+def _decode_op(x, router, bias, w12, s12, w3, s3, sw12, ss12, sw3, ss3, top_k, score, n_groups, top_groups, group_top, renormalize,
+               scale):
+    x, router = _gate_rows(x), _gate_rows(router)
+    T, D = x.shape
+    E, H = router.shape[0], w3.shape[-1]
+    Hs = 0 if sw3 is None else sw3.shape[-1]
+    held = [_on16(t) for t in (w12, s12, w3, s3, sw12, ss12, sw3, ss3)]
+    bias = None if bias is None else bias.contiguous()
+    out = x.new_empty((T, D))
+    idx = x.new_empty((T, top_k), dtype=torch.int64)
+    weights = x.new_empty((T, top_k), dtype=torch.float32)
+    ws = _decode_workspace(x.dtype, T, D, E, top_k, H, Hs)
+    work = torch.empty(ws, dtype=torch.uint8, device=x.device)
+    p = [ptr(t) for t in held]
+    call_on(x, "cin_moe_decode", x.data_ptr(), dtype_code(x), max(x.stride(0), D), T, D, router.data_ptr(), dtype_code(router),
+            max(router.stride(0), D), E, ptr(bias), top_k, score, n_groups, top_groups, group_top, renormalize, scale,
+            w12.dtype == torch.float8_e4m3fn, *p[:4], H, *p[4:], Hs, out.data_ptr(), idx.data_ptr(), weights.data_ptr(),
+            work.data_ptr(), ws, stream_of(x))
+    return out, idx, weights
+
+
+@_decode_op.register_fake
+def _(x, router, bias, w12, s12, w3, s3, sw12, ss12, sw3, ss3, top_k, *options):
+    T, D = x.shape
+    return (x.new_empty((T, D)), x.new_empty((T, top_k), dtype=torch.int64), x.new_empty((T, top_k), dtype=torch.float32))

@@ -536,6 +536,30 @@ int cin_moe_gate_backward(const void* logits, int dtype, int64_t ldl, int64_t T,
                           const float* gweights, const float* gscores, void* dlogits, void* stream);
 
 /*
+ * A whole mixture-of-experts layer for a few tokens (reference src/layers.py:113-157 at generation): the
+ * router's logits x R^T, the gate as in cin_moe_gate, SwiGLU experts, their weighted sum, and a shared expert
+ * of weight 1:  out_t = sum_j w_tj W3_e (silu(W1_e x_t) * (W2_e x_t)) + the shared expert's.
+ *   x [T, D] of dtype (row stride ldx); router [E, D] of router_dtype (row stride ldr); bias [E] fp32 or null
+ *   and the options after it as in cin_moe_gate; logits and gate in 64 bits
+ *   w12 [E, 2 H, D] (W1 above W2) and w3 [E, D, H], contiguous, on 16 bytes: with weights_fp8 e4m3 codes with fp32
+ *   scales of 128 x 128 blocks, s12 [E, ceil(2 H / 128), ceil(D / 128)] and s3 [E, ceil(D / 128),
+ *   ceil(H / 128)]; else bf16 (s12 and s3 null).  The shared expert's four the same without E, null with shared_H 0.
+ *   out [T, D] of dtype, idx [T, k] int64 and weights [T, k] fp32, contiguous
+ * T <= 128, E <= 1024, k <= 16; D, H and shared_H multiples of 16 up to 65536.  The workspace,
+ * cin_moe_decode_workspace bytes (-1 for sizes that are refused), lies on 16 bytes.  Bit-identical from call to
+ * call.
+ */
+int64_t cin_moe_decode_workspace(int dtype, int64_t T, int64_t D, int64_t E, int64_t k, int64_t H,
+                                 int64_t shared_H);
+int cin_moe_decode(const void* x, int dtype, int64_t ldx, int64_t T, int64_t D, const void* router,
+                   int router_dtype, int64_t ldr, int64_t E, const float* bias, int64_t k, int score,
+                   int64_t groups, int64_t top_groups, int group_top, int renormalize, float scale,
+                   int weights_fp8, const void* w12, const float* s12, const void* w3, const float* s3,
+                   int64_t H, const void* shared_w12, const float* shared_s12, const void* shared_w3,
+                   const float* shared_s3, int64_t shared_H, void* out, int64_t* idx, float* weights,
+                   void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
  * Rotary positions (reference src/attention.py:9-128): the channel pairs of [start, start + rot)
  * of q [B, L, H, D] and k [B, L, Hk, D] turned by the angle of the token's position,
  *   y0 = x0 cos - x1 sin, y1 = x0 sin + x1 cos    (inverse: sin negated, the gradient),
