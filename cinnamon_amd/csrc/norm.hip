@@ -9,6 +9,8 @@
 //   t  = gn w;   dx = gx + i (t - x i^2 mean(t x));   dr = a dx;   du = g dx
 //   s  = du pw;  dy = j (s - y j^2 mean(s y))         (dy = du without pw)
 //   dw = sum gn x i,  dpw = sum du y j,  dg = dx u,  da = dx r over the rows, a row or an element
+// A gate per channel only meets pw as the product g pw, and both have their gradient from one sum over the rows:
+// S = sum dx y j;  dpw = g S,  dg = pw S.
 //
 // x is formed again from y and r in the backward, in fp32 as in the forward: that reads as many bytes as
 // a stored x and has no rounding to x's type in it.  All arithmetic and the sums are fp32, each output is
@@ -28,14 +30,14 @@ using namespace cin;
 
 namespace {
 
-constexpr int kMaxThreads = 1024;
-constexpr int kMaxChunks = 2;
+constexpr int kMaxThreads = 512;
+constexpr int kMaxChunks = 4;
 constexpr int64_t kMaxWidth = (int64_t)kMaxThreads * kMaxChunks * 8;
 constexpr int kWaveRows = 4;  // rows at a time of a workgroup whose waves take a row each
 
 enum Gate { kNoGate = 0, kChannel = 1, kRow = 2, kElement = 3 };
 enum Scale { kNumber = 0, kOneValue = 1, kPerChannel = 2 };
-enum Sum { kSumW = 0, kSumPw = 1, kSumGate = 2, kSumScale = 3, kSums = 4 };
+enum Sum { kSumW = 0, kSumU = 1, kSumScale = 2, kSums = 3 };
 
 struct Vec {  // a vector over the channels
   const void* p;
@@ -63,28 +65,58 @@ struct NormArgs {
 template <int DT>
 constexpr int kWords = DT == CIN_DT_F32 ? 8 : 4;
 
+// A row of a matrix, the same for all lanes: loads and stores then take a 32-bit offset a lane.
+template <int DT>
+__device__ __forceinline__ const uint8_t* row_at(const void* p, int64_t row, int64_t ld) {
+  return static_cast<const uint8_t*>(p) + row * ld * (DT == CIN_DT_F32 ? 4 : 2);
+}
+
 // 8 adjacent elements as they lie in memory, at any element's address; cnt of them are there.
 template <int DT>
 struct Unit {
   uint32_t w[kWords<DT>];
-  __device__ __forceinline__ void load(const void* p, int64_t i, int cnt) {
-    constexpr int es = DT == CIN_DT_F32 ? 4 : 2;
-    const uint8_t* q = static_cast<const uint8_t*>(p) + i * es;
-    if (__builtin_expect(cnt == 8, 1)) {
-      __builtin_memcpy(w, q, 16);
-      if constexpr (DT == CIN_DT_F32) __builtin_memcpy(w + 4, q + 16, 16);
-      return;
+  static constexpr int kEs = DT == CIN_DT_F32 ? 4 : 2;
+  __device__ __forceinline__ void load(const uint8_t* row, uint32_t at) {
+    const uint8_t* q = row + at * kEs;
+    __builtin_memcpy(w, q, 16);
+    if constexpr (DT == CIN_DT_F32) __builtin_memcpy(w + 4, q + 16, 16);
+  }
+  __device__ __forceinline__ void load(const uint8_t* row, uint32_t at, int cnt) {
+    if (__builtin_expect(cnt == 8, 1)) return load(row, at);
+    zero();
+    // the rest as 4, 2 and 1 elements
+    const uint8_t* q = row + at * kEs;
+    if constexpr (DT == CIN_DT_F32) {
+      uint4 four = {0, 0, 0, 0};
+      uint2 two = {0, 0};
+      uint32_t one = 0;
+      if (cnt & 4) __builtin_memcpy(&four, q, 16);
+      if (cnt & 2) __builtin_memcpy(&two, q + (cnt & 4) * 4, 8);
+      if (cnt & 1) __builtin_memcpy(&one, q + (cnt & 6) * 4, 4);
+      const uint32_t a = cnt & 2 ? two.x : one, b = cnt & 2 ? two.y : 0u, c = cnt & 2 ? one : 0u;
+      const bool low = !(cnt & 4);
+      w[0] = low ? a : four.x;
+      w[1] = low ? b : four.y;
+      w[2] = low ? c : four.z;
+      w[3] = four.w;
+      w[4] = low ? 0u : a;
+      w[5] = low ? 0u : b;
+      w[6] = low ? 0u : c;
+      w[7] = 0u;
+    } else {
+      uint2 four = {0, 0};
+      uint32_t two = 0;
+      uint16_t one = 0;
+      if (cnt & 4) __builtin_memcpy(&four, q, 8);
+      if (cnt & 2) __builtin_memcpy(&two, q + (cnt & 4) * 2, 4);
+      if (cnt & 1) __builtin_memcpy(&one, q + (cnt & 6) * 2, 2);
+      const uint32_t a = cnt & 2 ? two : one, b = cnt & 2 ? one : 0u;
+      const bool low = !(cnt & 4);
+      w[0] = low ? a : four.x;
+      w[1] = low ? b : four.y;
+      w[2] = low ? 0u : a;
+      w[3] = low ? 0u : b;
     }
-#pragma unroll
-    for (int k = 0; k < kWords<DT>; ++k) w[k] = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (e < cnt) {
-        if constexpr (DT == CIN_DT_F32)
-          w[e] = reinterpret_cast<const uint32_t*>(q)[e];
-        else
-          w[e / 2] |= (uint32_t) reinterpret_cast<const uint16_t*>(q)[e] << (16 * (e & 1));
-      }
   }
   __device__ __forceinline__ void zero() {
 #pragma unroll
@@ -104,9 +136,9 @@ struct Unit {
 };
 
 template <int DT>
-__device__ __forceinline__ void store_unit(void* p, int64_t i, int cnt, const float (&v)[8]) {
+__device__ __forceinline__ void store_unit(const uint8_t* row, uint32_t at, int cnt, const float (&v)[8]) {
   constexpr int es = DT == CIN_DT_F32 ? 4 : 2;
-  uint8_t* q = static_cast<uint8_t*>(p) + i * es;
+  uint8_t* q = const_cast<uint8_t*>(row) + at * es;
   uint32_t w[kWords<DT>];
 #pragma unroll
   for (int k = 0; k < kWords<DT>; ++k) {
@@ -120,14 +152,22 @@ __device__ __forceinline__ void store_unit(void* p, int64_t i, int cnt, const fl
     if constexpr (DT == CIN_DT_F32) __builtin_memcpy(q + 16, w + 4, 16);
     return;
   }
-#pragma unroll
-  for (int e = 0; e < 8; ++e)
-    if (e < cnt) {
-      if constexpr (DT == CIN_DT_F32)
-        reinterpret_cast<uint32_t*>(q)[e] = w[e];
-      else
-        reinterpret_cast<uint16_t*>(q)[e] = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
-    }
+  const bool low = !(cnt & 4);
+  if constexpr (DT == CIN_DT_F32) {
+    const uint4 four = {w[0], w[1], w[2], w[3]};
+    const uint2 two = {low ? w[0] : w[4], low ? w[1] : w[5]};
+    const uint32_t third = low ? w[2] : w[6], one = cnt & 2 ? third : two.x;
+    if (cnt & 4) __builtin_memcpy(q, &four, 16);
+    if (cnt & 2) __builtin_memcpy(q + (cnt & 4) * 4, &two, 8);
+    if (cnt & 1) __builtin_memcpy(q + (cnt & 6) * 4, &one, 4);
+  } else {
+    const uint2 four = {w[0], w[1]};
+    const uint32_t two = low ? w[0] : w[2];
+    const uint16_t one = (uint16_t)(cnt & 2 ? (low ? w[1] : w[3]) : two);
+    if (cnt & 4) __builtin_memcpy(q, &four, 8);
+    if (cnt & 2) __builtin_memcpy(q + (cnt & 4) * 2, &two, 4);
+    if (cnt & 1) __builtin_memcpy(q + (cnt & 6) * 2, &one, 2);
+  }
 }
 
 __device__ inline void store_elem(void* p, int dt, int64_t i, float v) {
@@ -144,12 +184,12 @@ __device__ __forceinline__ void load_channels(const Vec& vec, int i, int cnt, fl
   if (!vec.p) return;
   if (vec.dtype == CIN_DT_F32) {
     Unit<CIN_DT_F32> u;
-    u.load(vec.p, i, cnt);
+    u.load(static_cast<const uint8_t*>(vec.p), (uint32_t)i, cnt);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = u.at(e);
   } else {
     Unit<CIN_DT_BF16> u;
-    u.load(vec.p, i, cnt);
+    u.load(static_cast<const uint8_t*>(vec.p), (uint32_t)i, cnt);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = half_bits_to_f32(vec.dtype, (uint16_t)(u.w[e / 2] >> (16 * (e & 1))));
   }
@@ -218,7 +258,7 @@ __global__ __launch_bounds__(WAVE ? 64 * kWaveRows : kMaxThreads) void k_norm_fo
   const int lane = WAVE ? threadIdx.x & 63 : threadIdx.x;
   const int waves = blockDim.x >> 6;
   const int64_t step = WAVE ? (int64_t)gridDim.x * kWaveRows : gridDim.x;
-  int64_t row = WAVE ? (int64_t)blockIdx.x * kWaveRows + (threadIdx.x >> 6) : blockIdx.x;
+  int64_t row = WAVE ? (int64_t)blockIdx.x * kWaveRows + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) : blockIdx.x;
   if (row >= a.T) return;
   Span<CH> s;
   s.set(lane, a.threads, a.D);
@@ -246,13 +286,13 @@ __global__ __launch_bounds__(WAVE ? 64 * kWaveRows : kMaxThreads) void k_norm_fo
     Unit<DR> r[CH];
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      y[c].load(a.y, row * a.ldy + s.at[c], s.cnt[c]);
+      y[c].load(row_at<DT>(a.y, row, a.ldy), s.at[c], s.cnt[c]);
       if (a.r)
-        r[c].load(a.r, row * a.ldr + s.at[c], s.cnt[c]);
+        r[c].load(row_at<DR>(a.r, row, a.ldr), s.at[c], s.cnt[c]);
       else
         r[c].zero();
       if constexpr (FULL)
-        if (a.gate_kind == kElement) ge[c].load(a.gate.p, row * a.ldg + s.at[c], s.cnt[c]);
+        if (a.gate_kind == kElement) ge[c].load(row_at<DT>(a.gate.p, row, a.ldg), s.at[c], s.cnt[c]);
     }
     float grow = 1.0f, j = 1.0f;
     if constexpr (FULL) {
@@ -282,7 +322,7 @@ __global__ __launch_bounds__(WAVE ? 64 * kWaveRows : kMaxThreads) void k_norm_fo
         }
         q[0] = __builtin_fmaf(x[c][e], x[c][e], q[0]);
       }
-      if (a.x && s.cnt[c] > 0) store_unit<DR>(a.x, row * a.D + s.at[c], s.cnt[c], x[c]);
+      if (a.x && s.cnt[c] > 0) store_unit<DR>(row_at<DR>(a.x, row, a.D), s.at[c], s.cnt[c], x[c]);
     }
     sum(q, waves);
     const float i = 1.0f / sqrtf(q[0] * inv_d + a.eps);
@@ -290,7 +330,7 @@ __global__ __launch_bounds__(WAVE ? 64 * kWaveRows : kMaxThreads) void k_norm_fo
     for (int c = 0; c < CH; ++c) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[c][e] = x[c][e] * i * w[c][e];
-      if (s.cnt[c] > 0) store_unit<DT>(a.n, row * a.D + s.at[c], s.cnt[c], x[c]);
+      if (s.cnt[c] > 0) store_unit<DT>(row_at<DT>(a.n, row, a.D), s.at[c], s.cnt[c], x[c]);
     }
     if (a.stats && lane == 0) {
       a.stats[row] = i;
@@ -321,242 +361,299 @@ __device__ __forceinline__ void leave_partial(const NormArgs& a, int which, cons
   } else {
 #pragma unroll
     for (int c = 0; c < CH; ++c)
-      if (s.cnt[c] > 0) store_unit<CIN_DT_F32>(out, s.at[c], s.cnt[c], v[c]);
+      if (s.cnt[c] > 0) store_unit<CIN_DT_F32>(reinterpret_cast<const uint8_t*>(out), s.at[c], s.cnt[c], v[c]);
   }
 }
 
-// What a row of the backward reads.
-template <int DT, int DR, int CH, bool FULL>
+// What the backward knows of a call when it is compiled: neither post norm nor gate nor learned scale, no gate but of
+// channels, anything.
+enum Mode { kPlain = 0, kChannels = 1, kAny = 2 };
+
+// What a row of the backward reads; ANY: a gate a row or an element with it.
+template <int DT, int DR, int CH, bool ANY>
 struct RowIn {
-  Unit<DT> y[CH], gn[CH], ge[FULL ? CH : 1];
+  Unit<DT> y[CH], gn[CH], ge[ANY ? CH : 1];
   Unit<DR> r[CH], gx[CH];
   float i, j, gate;
   __device__ __forceinline__ void load(const NormArgs& a, int64_t row, const Span<CH>& s) {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      y[c].load(a.y, row * a.ldy + s.at[c], s.cnt[c]);
-      if (a.r)
-        r[c].load(a.r, row * a.ldr + s.at[c], s.cnt[c]);
-      else
-        r[c].zero();
-      if (a.gn)
-        gn[c].load(a.gn, row * a.ldgn + s.at[c], s.cnt[c]);
-      else
-        gn[c].zero();
-      if (a.gx)
-        gx[c].load(a.gx, row * a.ldgx + s.at[c], s.cnt[c]);
-      else
-        gx[c].zero();
-      if constexpr (FULL)
-        if (a.gate_kind == kElement) ge[c].load(a.gate.p, row * a.ldg + s.at[c], s.cnt[c]);
+      if (__builtin_expect(s.cnt[c] == 8, 1)) {
+        y[c].load(row_at<DT>(a.y, row, a.ldy), s.at[c]);
+        if (a.r) r[c].load(row_at<DR>(a.r, row, a.ldr), s.at[c]);
+        if (a.gn) gn[c].load(row_at<DT>(a.gn, row, a.ldgn), s.at[c]);
+        if (a.gx) gx[c].load(row_at<DR>(a.gx, row, a.ldgx), s.at[c]);
+        if (ANY && a.gate_kind == kElement) ge[ANY ? c : 0].load(row_at<DT>(a.gate.p, row, a.ldg), s.at[c]);
+      } else {
+        y[c].load(row_at<DT>(a.y, row, a.ldy), s.at[c], s.cnt[c]);
+        if (a.r) r[c].load(row_at<DR>(a.r, row, a.ldr), s.at[c], s.cnt[c]);
+        if (a.gn) gn[c].load(row_at<DT>(a.gn, row, a.ldgn), s.at[c], s.cnt[c]);
+        if (a.gx) gx[c].load(row_at<DR>(a.gx, row, a.ldgx), s.at[c], s.cnt[c]);
+        if (ANY && a.gate_kind == kElement) ge[ANY ? c : 0].load(row_at<DT>(a.gate.p, row, a.ldg), s.at[c], s.cnt[c]);
+      }
+      if (!a.r) r[c].zero();
+      if (!a.gn) gn[c].zero();
+      if (!a.gx) gx[c].zero();
     }
     i = a.stats[row];
-    j = FULL ? a.stats[a.T + row] : 1.0f;
-    gate = FULL && a.gate_kind == kRow ? load_elem(a.gate.p, a.gate.dtype, row * a.ldg) : 1.0f;
+    j = a.stats[a.T + row];
+    gate = ANY && a.gate_kind == kRow ? load_elem(a.gate.p, a.gate.dtype, row * a.ldg) : 1.0f;
   }
 };
 
-// A channel's sums for the gate and the scale lie in LDS, each thread's own (they are rare, and in
-// registers they would halve the waves of a CU): 8 of chunk c at [(which CH + c) 2 + half][thread].
-template <int CH>
-struct LdsSums {
+// 8 channels of a thread's chunk c in LDS, each thread's own: two 16-byte words, threads side by side.
+struct Slots {
   float4* at;
-  __device__ __forceinline__ float4& part(int which, int c, int half) const {
-    return at[((which * CH + c) * 2 + half) * blockDim.x + threadIdx.x];
+  int threads, mine, chunks;
+  __device__ __forceinline__ float4& half(int which, int c, int h) const {
+    return at[((which * chunks + c) * 2 + h) * threads + mine];
   }
-  __device__ __forceinline__ void clear() const {
+  __device__ __forceinline__ void set(int which, int c, const float (&v)[8]) const {
 #pragma unroll
-    for (int k = 0; k < 4 * CH; ++k) at[k * blockDim.x + threadIdx.x] = float4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int h = 0; h < 2; ++h) half(which, c, h) = float4{v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]};
   }
-  __device__ __forceinline__ void add(int which, int c, const float (&v)[8]) const {
+  __device__ __forceinline__ void get(int which, int c, float (&v)[8]) const {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      float4 t = part(which, c, h);
-      t.x += v[4 * h];
-      t.y += v[4 * h + 1];
-      t.z += v[4 * h + 2];
-      t.w += v[4 * h + 3];
-      part(which, c, h) = t;
+      const float4 t = half(which, c, h);
+      v[4 * h] = t.x;
+      v[4 * h + 1] = t.y;
+      v[4 * h + 2] = t.z;
+      v[4 * h + 3] = t.w;
     }
   }
-  __device__ __forceinline__ void get(int which, float (&v)[CH][8]) const {
+  __device__ __forceinline__ void add(int which, int c, const float (&v)[8]) const {
+    float t[8];
+    get(which, c, t);
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float4 t = part(which, c, h);
-        v[c][4 * h] = t.x;
-        v[c][4 * h + 1] = t.y;
-        v[c][4 * h + 2] = t.z;
-        v[c][4 * h + 3] = t.w;
-      }
+    for (int e = 0; e < 8; ++e) t[e] += v[e];
+    set(which, c, t);
   }
 };
 
-template <int DT, int DR, int CH, bool WAVE, bool FULL>
+// FULL keeps the channels' vectors in LDS between the rows (w, g pw and the scale, up to 8192 channels of each) and the
+// scale's sums too: in registers they would cost the next row's loads, and read again from L2 they would have to
+// be waited for behind those.
+template <int CH>
+constexpr bool kVectorsInLds = CH <= 2;
+template <int CH, bool WAVE>
+size_t backward_lds(bool scale_channels, int block) {
+  const size_t row = (WAVE ? 64 : block) * CH * 32, own = (size_t)block * CH * 32;
+  return (kVectorsInLds<CH> ? (scale_channels ? 3 : 2) * row : 0) + (scale_channels ? own : 0);
+}
+
+template <int DT, int DR, int CH, bool WAVE, Mode MODE>
 __global__ __launch_bounds__(WAVE ? 64 * kWaveRows : kMaxThreads) void k_norm_backward(NormArgs a) {
+  constexpr bool FULL = MODE != kPlain;
   __shared__ float lds1[2][1][kMaxThreads / 64], lds2[2][2][kMaxThreads / 64];
   __shared__ float joined[WAVE ? kWaveRows * 64 * CH * 8 : 1];
-  extern __shared__ float4 channel_sums[];  // where the gate or the scale is one a channel
+  extern __shared__ float4 slots[];
   RowSum<WAVE, 1> sum1{lds1};
   RowSum<WAVE, 2> sum2{lds2};
-  const LdsSums<CH> sums{channel_sums};
   const int lane = WAVE ? threadIdx.x & 63 : threadIdx.x;
   const int waves = blockDim.x >> 6;
   const int64_t step = WAVE ? (int64_t)gridDim.x * kWaveRows : gridDim.x;
-  int64_t row = WAVE ? (int64_t)blockIdx.x * kWaveRows + (threadIdx.x >> 6) : blockIdx.x;
+  int64_t row = WAVE ? (int64_t)blockIdx.x * kWaveRows + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) : blockIdx.x;
   Span<CH> s;
   s.set(lane, a.threads, a.D);
-  constexpr int F = FULL ? CH : 1;
-  float w[CH][8], pw[F][8], one = a.scale_value;
-  float sw[CH][8], spw[F][8], sone = 0.0f;
+  const bool scale_channels = FULL && a.scale_kind == kPerChannel;
+  constexpr bool kInLds = FULL && kVectorsInLds<CH>;
+  constexpr int R = kInLds ? 1 : CH;
+  const Slots vectors{slots, WAVE ? 64 : (int)blockDim.x, lane, CH};
+  const Slots scale_sums{slots + (kInLds ? 6 * CH * vectors.threads : 0), (int)blockDim.x, (int)threadIdx.x, CH};
+  float w[R][8], gp[FULL ? R : 1][8], value = a.scale_value;
+  float sw[CH][8], su[FULL ? CH : 1][8], sone = 0.0f;
   const float inv_d = 1.0f / (float)a.D;
+  if (FULL && a.scale_kind == kOneValue) value = load_elem(a.scale.p, a.scale.dtype, 0);
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
-    load_channels(a.w, s.at[c], s.cnt[c], 1.0f, w[c]);
+    float v[8];
+    load_channels(a.w, s.at[c], s.cnt[c], 1.0f, v);
+    if constexpr (kInLds) vectors.set(0, c, v);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sw[c][e] = 0.0f;
+    for (int e = 0; e < 8; ++e) {
+      if constexpr (!kInLds) w[c][e] = v[e];
+      sw[c][e] = 0.0f;
+    }
     if constexpr (FULL) {
-      load_channels(a.pw, s.at[c], s.cnt[c], 1.0f, pw[c]);
+      float g[8];
+      load_channels(a.pw, s.at[c], s.cnt[c], 1.0f, v);
+      load_channels(a.gate_kind == kChannel ? a.gate : Vec{nullptr, 0}, s.at[c], s.cnt[c], 1.0f, g);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) spw[c][e] = 0.0f;
+      for (int e = 0; e < 8; ++e) {
+        v[e] *= g[e];
+        if constexpr (!kInLds) gp[c][e] = v[e];
+        su[c][e] = 0.0f;
+      }
+      if constexpr (kInLds) vectors.set(1, c, v);
+      if (scale_channels) {
+        load_channels(a.scale, s.at[c], s.cnt[c], 0.0f, v);
+        if constexpr (kInLds) vectors.set(2, c, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+        scale_sums.set(0, c, v);
+      }
     }
   }
-  if constexpr (FULL) {
-    if (a.gate_kind == kChannel || a.scale_kind == kPerChannel) sums.clear();
-    if (a.scale_kind == kOneValue) one = load_elem(a.scale.p, a.scale.dtype, 0);
-  }
+  auto weights = [&](int c, float (&v)[8]) {
+    if constexpr (kInLds) {
+      vectors.get(0, c, v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = w[c][e];
+    }
+  };
+  auto products = [&](int c, float (&v)[8]) {  // g pw
+    if constexpr (kInLds) {
+      vectors.get(1, c, v);
+    } else if constexpr (FULL) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = gp[c][e];
+    }
+  };
+  auto scales = [&](int c, float (&v)[8]) {
+    if (!scale_channels) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = value;
+    } else if constexpr (kInLds) {
+      vectors.get(2, c, v);
+    } else {
+      load_channels(a.scale, s.at[c], s.cnt[c], 0.0f, v);
+    }
+  };
   // A workgroup's waves wait for each other twice a row, so the next row's loads go out before; waves with rows
   // of their own cover each other's (and fp32 rows are as many bytes without).
-  constexpr bool kAhead = !WAVE && CH == 1 && DR != CIN_DT_F32;
-  RowIn<DT, DR, CH, FULL> in, next;
-  if (kAhead && row < a.T) next.load(a, row, s);
-  for (; row < a.T; row += step) {
+  constexpr bool kAhead = !WAVE && CH <= 2 && DR != CIN_DT_F32;
+  const bool post = FULL && a.pw.p, gated = MODE == kAny && (a.gate_kind == kRow || a.gate_kind == kElement);
+  const bool inner = FULL && (a.pw.p || a.gate_kind == kChannel);  // S is summed
+  using In = RowIn<DT, DR, CH, MODE == kAny>;
+  auto one_row = [&](In& in, In& next) {
     if constexpr (kAhead) {
-      in = next;
       if (row + step < a.T) next.load(a, row + step, s);
     } else {
       in.load(a, row, s);
     }
     const float i = in.i, j = in.j;
-    // (a gate or scale per channel is read again each row, from L2: in registers they would cost half the waves)
-    float g[F][8], sc[F][8];
-    if constexpr (FULL) {
-#pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        if (a.gate_kind == kElement) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) g[c][e] = in.ge[c].at(e);
-        } else {
-          load_channels(a.gate_kind == kChannel ? a.gate : Vec{nullptr, 0}, s.at[c], s.cnt[c], in.gate, g[c]);
-        }
-        load_channels(a.scale_kind == kPerChannel ? a.scale : Vec{nullptr, 0}, s.at[c], s.cnt[c], one, sc[c]);
-      }
-    }
-    auto unit = [&](int c, int e) {  // u, without its gate
-      if constexpr (FULL) return in.y[c].at(e) * j * pw[c][e];
-      return in.y[c].at(e);
-    };
-    auto gate = [&](int c, int e) {
-      if constexpr (FULL) return g[c][e];
-      return 1.0f;
-    };
-    auto scale = [&](int c, int e) {
-      if constexpr (FULL) return sc[c][e];
-      return a.scale_value;
-    };
     float x[CH][8], q[1] = {0.0f};
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
+    for (int c = 0; c < CH; ++c) {
+      float wc[8], pc[8], sc[8];
+      weights(c, wc);
+      products(c, pc);
+      scales(c, sc);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        float u = unit(c, e);
-        if constexpr (FULL) u *= gate(c, e);
-        x[c][e] = a.r ? __builtin_fmaf(scale(c, e), in.r[c].at(e), u) : u;
-        q[0] = __builtin_fmaf(in.gn[c].at(e) * w[c][e], x[c][e], q[0]);
+        x[c][e] = in.y[c].at(e);
+        if constexpr (FULL) x[c][e] = x[c][e] * j * pc[e];
       }
+      if (gated) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[c][e] *= a.gate_kind == kElement ? in.ge[MODE == kAny ? c : 0].at(e) : in.gate;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[c][e] = __builtin_fmaf(sc[e], in.r[c].at(e), x[c][e]);  // (r is 0 without a residual)
+        q[0] = __builtin_fmaf(in.gn[c].at(e) * wc[e], x[c][e], q[0]);
+      }
+    }
     sum1(q, waves);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       in.y[c].forget();
       in.r[c].forget();
       in.gn[c].forget();
+      if constexpr (MODE == kAny) in.ge[c].forget();
     }
-    const float c1 = i * i * (q[0] * inv_d);
-    // x becomes dx
+    const float c1 = -(q[0] * inv_d * i * i * i);
+    float p[2] = {0.0f, 0.0f};
+    // x becomes dx, then du without a channel's gate
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
+      float v[8], wc[8], pc[8];
+      weights(c, wc);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float t = in.gn[c].at(e);
-        sw[c][e] = __builtin_fmaf(t, x[c][e] * i, sw[c][e]);
-        x[c][e] = __builtin_fmaf(i, __builtin_fmaf(-x[c][e], c1, t * w[c][e]), in.gx[c].at(e));
+        const float t = in.gn[c].at(e) * i;
+        sw[c][e] = __builtin_fmaf(t, x[c][e], sw[c][e]);
+        x[c][e] = __builtin_fmaf(t, wc[e], __builtin_fmaf(x[c][e], c1, in.gx[c].at(e)));
       }
-      if (a.dr && s.cnt[c] > 0) {
-        float v[8];
+      if (a.dr) {
+        scales(c, v);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = scale(c, e) * x[c][e];
-        store_unit<DR>(a.dr, row * a.D + s.at[c], s.cnt[c], v);
+        for (int e = 0; e < 8; ++e) v[e] *= x[c][e];
+        if (s.cnt[c] > 0) store_unit<DR>(row_at<DR>(a.dr, row, a.D), s.at[c], s.cnt[c], v);
+      }
+      if constexpr (FULL) {
+        if (a.scale_kind == kOneValue) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sone = __builtin_fmaf(x[c][e], in.r[c].at(e), sone);
+        } else if (scale_channels) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = x[c][e] * in.r[c].at(e);
+          scale_sums.add(0, c, v);
+        }
+        products(c, pc);
+        if (gated) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            v[e] = x[c][e] * (in.y[c].at(e) * j * pc[e]);
+            p[1] += v[e];
+            x[c][e] *= a.gate_kind == kElement ? in.ge[MODE == kAny ? c : 0].at(e) : in.gate;
+          }
+          if (a.gate_kind == kElement && a.dgate && s.cnt[c] > 0)
+            store_unit<DT>(row_at<DT>(a.dgate, row, a.D), s.at[c], s.cnt[c], v);
+        }
+        if (inner) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float t = x[c][e] * in.y[c].at(e);
+            su[c][e] = __builtin_fmaf(t, j, su[c][e]);
+            p[0] = __builtin_fmaf(t, pc[e], p[0]);
+          }
+        }
       }
     }
     if constexpr (FULL) {
-      float p[2] = {0.0f, 0.0f};
+      if (post || (MODE == kAny && a.gate_kind == kRow)) sum2(p, waves);
+      if (inner) {
+        const float c2 = post ? -(p[0] * inv_d * j * j * j) : 0.0f;
 #pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        if (a.scale_kind != kNumber) {
-          float v[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            v[e] = x[c][e] * in.r[c].at(e);
-            sone += v[e];
-          }
-          if (a.scale_kind == kPerChannel) sums.add(1, c, v);
-        }
-        if (a.gate_kind != kNoGate) {
-          float v[8];
+        for (int c = 0; c < CH; ++c) {
+          in.y[c].forget();
+          float pc[8];
+          products(c, pc);
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            v[e] = x[c][e] * unit(c, e);
-            p[1] += v[e];
-          }
-          if (a.gate_kind == kElement && a.dgate && s.cnt[c] > 0) store_unit<DT>(a.dgate, row * a.D + s.at[c], s.cnt[c], v);
-          if (a.gate_kind == kChannel) sums.add(0, c, v);
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          x[c][e] *= gate(c, e);  // du
-          if (a.pw.p) {
-            spw[c][e] = __builtin_fmaf(x[c][e], in.y[c].at(e) * j, spw[c][e]);
-            p[0] = __builtin_fmaf(x[c][e] * pw[c][e], in.y[c].at(e), p[0]);
+            x[c][e] = x[c][e] * j * pc[e];
+            if (post) x[c][e] = __builtin_fmaf(in.y[c].at(e), c2, x[c][e]);
           }
         }
       }
-      if (a.pw.p || a.gate_kind == kRow) sum2(p, waves);
-      if (a.pw.p) {
-        const float c2 = j * j * (p[0] * inv_d);
-#pragma unroll
-        for (int c = 0; c < CH; ++c) in.y[c].forget();
-#pragma unroll
-        for (int c = 0; c < CH; ++c)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[c][e] = j * __builtin_fmaf(-in.y[c].at(e), c2, x[c][e] * pw[c][e]);
-      }
-      if (a.gate_kind == kRow && a.dgate && lane == 0) store_elem(a.dgate, a.gate.dtype, row, p[1]);
+      if (MODE == kAny && a.gate_kind == kRow && a.dgate && lane == 0) store_elem(a.dgate, a.gate.dtype, row, p[1]);
     }
 #pragma unroll
     for (int c = 0; c < CH; ++c)
-      if (a.dy && s.cnt[c] > 0) store_unit<DT>(a.dy, row * a.D + s.at[c], s.cnt[c], x[c]);
+      if (a.dy && s.cnt[c] > 0) store_unit<DT>(row_at<DT>(a.dy, row, a.D), s.at[c], s.cnt[c], x[c]);
+    row += step;
+  };
+  In even, odd;
+  if constexpr (kAhead) {
+    if (row < a.T) even.load(a, row, s);
+    while (row < a.T) {
+      one_row(even, odd);
+      if (row >= a.T) break;
+      one_row(odd, even);
+    }
+  } else {
+    while (row < a.T) one_row(even, odd);
   }
   if (!a.partial) return;
   leave_partial<CH, WAVE>(a, kSumW, sw, s, joined);
   if constexpr (FULL) {
-    if (a.pw.p) leave_partial<CH, WAVE>(a, kSumPw, spw, s, joined);
-    if (a.gate_kind == kChannel) {
-      sums.get(0, sw);
-      leave_partial<CH, WAVE>(a, kSumGate, sw, s, joined);
-    }
-    if (a.scale_kind == kPerChannel) {
-      sums.get(1, sw);
+    if (inner) leave_partial<CH, WAVE>(a, kSumU, su, s, joined);
+    if (scale_channels) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c) scale_sums.get(0, c, sw[c]);
       leave_partial<CH, WAVE>(a, kSumScale, sw, s, joined);
     }
     if (a.scale_kind == kOneValue) {
@@ -573,12 +670,17 @@ __global__ __launch_bounds__(WAVE ? 64 * kWaveRows : kMaxThreads) void k_norm_ba
   }
 }
 
+// One output of a sum over the rows: times a vector where there is one.
+struct ColumnOut {
+  void* p;
+  int dtype;
+  Vec times;
+};
 struct ColumnArgs {
   const float* partial;
   int64_t G;  // partial rows
   int D;
-  void* out[kSums];
-  int dtype[kSums];
+  ColumnOut out[kSums][2];
   void* one;
   int one_dtype;
 };
@@ -604,8 +706,9 @@ __global__ __launch_bounds__(1024) void k_norm_columns(ColumnArgs a) {
     }
     return;
   }
-  void* out = a.out[blockIdx.y];
-  if (!out) return;
+  const ColumnOut& first = a.out[blockIdx.y][0];
+  const ColumnOut& second = a.out[blockIdx.y][1];
+  if (!first.p && !second.p) return;
   const int d = blockIdx.x * 32 + col;
   float t = 0.0f;
   if (d < a.D) {
@@ -617,7 +720,10 @@ __global__ __launch_bounds__(1024) void k_norm_columns(ColumnArgs a) {
   __syncthreads();
   if (line == 0 && d < a.D) {
     for (int l = 1; l < 32; ++l) t += lds[l][col];
-    store_elem(out, a.dtype[blockIdx.y], d, t);
+    for (int k = 0; k < 2; ++k) {
+      const ColumnOut& o = a.out[blockIdx.y][k];
+      if (o.p) store_elem(o.p, o.dtype, d, o.times.p ? t * load_elem(o.times.p, o.times.dtype, d) : t);
+    }
   }
 }
 
@@ -630,7 +736,7 @@ Shape shape_of(int64_t D) {
   const int64_t units = cdiv(D, 8);
   if (units <= 64) return {1, 64, true};
   if (units <= 128) return {2, 64, true};
-  const int chunks = units <= kMaxThreads ? 1 : 2;
+  const int chunks = units <= kMaxThreads ? 1 : units <= 2 * kMaxThreads ? 2 : 4;
   return {chunks, (int)(cdiv(cdiv(units, chunks), 64) * 64), false};
 }
 
@@ -648,23 +754,27 @@ void allow_lds(K kernel, size_t bytes) {
   if (bytes > 65536) (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
 }
 
+template <int DT, int DR, int CH, bool WAVE, Mode MODE>
+void launch_backward(const NormArgs& a, dim3 grid, dim3 block, hipStream_t stream) {
+  const size_t lds = MODE == kPlain ? 0 : backward_lds<CH, WAVE>(a.scale_kind == kPerChannel, (int)block.x);
+  allow_lds(k_norm_backward<DT, DR, CH, WAVE, MODE>, lds);
+  hipLaunchKernelGGL((k_norm_backward<DT, DR, CH, WAVE, MODE>), grid, block, lds, stream, a);
+}
+
 template <int DT, int DR, int CH, bool WAVE>
 void launch(const NormArgs& a, const Shape& s, int64_t groups, bool full, bool backward, hipStream_t stream) {
   const dim3 grid((uint32_t)groups), block(s.wave ? 64 * kWaveRows : s.threads);
-  if (backward) {
-    if (full) {
-      const bool sums = a.gate_kind == kChannel || a.scale_kind == kPerChannel;
-      const size_t lds = sums ? (size_t)block.x * CH * 64 : 0;
-      allow_lds(k_norm_backward<DT, DR, CH, WAVE, true>, lds);
-      hipLaunchKernelGGL((k_norm_backward<DT, DR, CH, WAVE, true>), grid, block, lds, stream, a);
-    } else {
-      hipLaunchKernelGGL((k_norm_backward<DT, DR, CH, WAVE, false>), grid, block, 0, stream, a);
-    }
-  } else {
+  if (!backward) {
     if (full)
       hipLaunchKernelGGL((k_norm_forward<DT, DR, CH, WAVE, true>), grid, block, 0, stream, a);
     else
       hipLaunchKernelGGL((k_norm_forward<DT, DR, CH, WAVE, false>), grid, block, 0, stream, a);
+  } else if (!full) {
+    launch_backward<DT, DR, CH, WAVE, kPlain>(a, grid, block, stream);
+  } else if (a.gate_kind == kRow || a.gate_kind == kElement) {
+    launch_backward<DT, DR, CH, WAVE, kAny>(a, grid, block, stream);
+  } else {
+    launch_backward<DT, DR, CH, WAVE, kChannels>(a, grid, block, stream);
   }
 }
 
@@ -676,8 +786,10 @@ void launch_shape(const NormArgs& a, const Shape& s, int64_t groups, bool full, 
     launch<DT, DR, 2, true>(a, s, groups, full, backward, stream);
   else if (s.chunks == 1)
     launch<DT, DR, 1, false>(a, s, groups, full, backward, stream);
-  else
+  else if (s.chunks == 2)
     launch<DT, DR, 2, false>(a, s, groups, full, backward, stream);
+  else
+    launch<DT, DR, 4, false>(a, s, groups, full, backward, stream);
 }
 
 void launch_types(const NormArgs& a, int dt, int dr, const Shape& s, int64_t groups, bool full, bool backward,
@@ -782,22 +894,18 @@ int cin_block_norm_backward(const void* y, int dtype, int64_t ldy, const void* r
                 "cin_block_norm_backward: a gradient of an input that is not there");
   CIN_CHECK_ARG(!dscale || r, "cin_block_norm_backward: a scale without a residual");
   ColumnArgs c = {};
-  c.out[kSumW] = dw;
-  c.dtype[kSumW] = w_dtype;
-  c.out[kSumPw] = dpw;
-  c.dtype[kSumPw] = pw_dtype;
-  if (gate_kind == kChannel) {
-    c.out[kSumGate] = dgate;
-    c.dtype[kSumGate] = gate_dtype;
-  }
+  const Vec none = {nullptr, 0};
+  c.out[kSumW][0] = {dw, w_dtype, none};
+  c.out[kSumU][0] = {dpw, pw_dtype, gate_kind == kChannel ? a.gate : none};
+  if (gate_kind == kChannel) c.out[kSumU][1] = {dgate, gate_dtype, a.pw};
   if (scale_kind == kPerChannel) {
-    c.out[kSumScale] = dscale;
-    c.dtype[kSumScale] = scale_dtype;
+    c.out[kSumScale][0] = {dscale, scale_dtype, none};
   } else if (scale_kind == kOneValue) {
     c.one = dscale;
     c.one_dtype = scale_dtype;
   }
-  const bool sums = c.out[0] || c.out[1] || c.out[2] || c.out[3] || c.one;
+  const bool inner = c.out[kSumU][0].p || c.out[kSumU][1].p;
+  const bool sums = dw || inner || dscale;
   CIN_CHECK_ARG(!sums || (workspace && workspace_bytes >= cin_block_norm_workspace(T, D)),
                 "cin_block_norm_backward: workspace below cin_block_norm_workspace bytes");
   a.stats = const_cast<float*>(stats);
@@ -817,7 +925,7 @@ int cin_block_norm_backward(const void* y, int dtype, int64_t ldy, const void* r
     c.partial = a.partial;
     c.G = groups;
     c.D = (int)D;
-    const int rows = c.out[3] ? 4 : c.out[2] ? 3 : c.out[1] ? 2 : 1;
+    const int rows = c.out[kSumScale][0].p ? 3 : inner ? 2 : 1;
     hipLaunchKernelGGL(k_norm_columns, dim3((uint32_t)(cdiv(D, 32) + (c.one ? 1 : 0)), rows), dim3(1024), 0, (hipStream_t)stream, c);
   }
   return cin_check_launch("cin_block_norm_backward");
