@@ -16,10 +16,15 @@
 // large as the output's own rounding.  All sums are fp32.  Logits and the gate are in 64 bits: choices next to
 // the border of the top k differ by less than 32 bits hold.
 //
-// Four launches: k_router (logits by slices of D on the fp64 matrix units, and x's parts), k_gate (a workgroup a
-// token), k_up (a workgroup an expert and 16 or 32 of its hidden channels, the waves sharing D), k_down (a workgroup
-// 16 or 32 output channels, the waves sharing the chosen experts' hidden channels; each wave's sums per token
-// lie in LDS and are joined in a fixed order).  No atomics on results.
+// Launches: k_router (logits by slices of D on the fp64 matrix units, and x's parts), k_gate (a workgroup a token), then
+//   up to 16 tokens: k_up_few (a workgroup an expert and 16 of its hidden channels, the waves sharing D) and
+//   k_down_few (a workgroup 16 output channels, the waves sharing the chosen experts' hidden channels; each
+//   wave's sums per token lie in LDS and are joined in a fixed order): with so few columns a product the work is
+//   the weights', and each is spread over the whole chip;
+//   more: k_products twice (a workgroup a unit of an expert's tokens and 16 or 32 rows a wave; the tokens' parts
+//   go through LDS once for all waves, as they would be more bytes than the weights), which leaves h, then
+//   each expert's output rows, and k_join (their sum per token in the order of top k).
+// No atomics on results.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -38,10 +43,11 @@ constexpr int kMaxTopK = 16;
 constexpr int kMaxGroups = 64;
 constexpr int kBlock = 128;        // of a scale, and a step of K
 constexpr int kMaxAssigned = kMaxTokens * kMaxTopK;
-constexpr int kLeastUnit = 32;
-constexpr int kMaxUnits = kMaxExperts + kMaxAssigned / kLeastUnit;
+constexpr int kUnitTokens = 32;    // of an expert, multiplied at once
+constexpr int kMaxUnits = kMaxExperts + kMaxAssigned / kUnitTokens;
 constexpr int kRouterSlice = 512;  // channels of a k_router workgroup
-constexpr int kUpWaves = 4, kDownWaves = 8;
+constexpr int kUpWaves = 4, kDownWaves = 8, kTileWaves = 4;
+constexpr int kFewTokens = 16;
 
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
@@ -54,8 +60,6 @@ template <int DT>
 constexpr int kXParts = DT == CIN_DT_BF16 ? 1 : DT == CIN_DT_F16 ? 2 : 3;
 template <int DT>
 constexpr int kHParts = DT == CIN_DT_F32 ? 3 : 2;
-// Tokens of an expert multiplied at once: what the registers hold of their parts.
-constexpr int unit_tokens(int dtype) { return dtype == CIN_DT_F32 ? kLeastUnit : 64; }
 
 struct Expert {  // stacked experts, or a shared one
   const uint8_t *w12, *w3;
@@ -81,8 +85,21 @@ struct LayerArgs {
   double* logits;  // [slices, T, E]
   int slices;
   uint16_t *xb, *hb, *hs;  // parts of x [P, T, Dp], of h [P, T k, H], of the shared expert's [P, T, Hs]
+  float* y;                // past kFewTokens: the experts' outputs [T k, D], the shared one's [T, D]
   int units;               // the most that the routed experts can have
 };
+
+// Scales, the same for all lanes and nowhere written here: scalar loads.
+typedef const __attribute__((address_space(4))) float* floats_at;
+
+// 16 bytes at an offset into a buffer; zeros from kNothing on.  No load of the products is behind a branch: one
+// that may not have been issued would have to be counted as issued last, and all before it waited for.
+constexpr uint32_t kNothing = 0x80000000u;
+template <int AUX = 0>
+__device__ __forceinline__ u4 load16(__amdgpu_buffer_rsrc_t from, uint32_t at) {
+  return __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(from, at, 0, AUX));
+}
+constexpr int kStream = 2;  // read once: not kept in the caches
 
 // ---------------------------------------------------------------------------------------------
 // Router and gate
@@ -293,12 +310,13 @@ __global__ __launch_bounds__(256) void k_gate(LayerArgs a) {
 // ---------------------------------------------------------------------------------------------
 // Which expert multiplies which tokens
 // ---------------------------------------------------------------------------------------------
-// The assignments (t k + j) by expert, in units of up to unit_tokens of one expert.
+// The assignments (t k + j) by expert, in units of up to UNIT of one expert.
 struct Plan {
   int count[kMaxExperts];           // assignments of an expert, then where its next one goes
   uint32_t unit[kMaxUnits];         // expert, first entry
   uint8_t tokens[kMaxUnits];
   uint16_t list[kMaxAssigned];
+  uint16_t expert[kMaxAssigned];    // of an assignment
   uint32_t waves[kDownWaves];
   int units;
 };
@@ -312,7 +330,11 @@ __device__ __forceinline__ void make_plan(Plan& p, const int64_t* idx, int n, in
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   for (int e = tid; e < E; e += THREADS) p.count[e] = 0;
   __syncthreads();
-  for (int i = tid; i < n; i += THREADS) atomicAdd(&p.count[(int)idx[i]], 1);
+  for (int i = tid; i < n; i += THREADS) {
+    const int e = (int)idx[i];
+    p.expert[i] = (uint16_t)e;
+    atomicAdd(&p.count[e], 1);
+  }
   __syncthreads();
   // units (upper half) and assignments of the experts before this thread's
   uint32_t own = 0;
@@ -350,14 +372,14 @@ __device__ __forceinline__ void make_plan(Plan& p, const int64_t* idx, int n, in
   if (tid == 0) p.units = (int)(all >> 16);
   __syncthreads();
   if constexpr (ALL) {
-    for (int i = tid; i < n; i += THREADS) p.list[atomicAdd(&p.count[(int)idx[i]], 1)] = (uint16_t)i;
+    for (int i = tid; i < n; i += THREADS) p.list[atomicAdd(&p.count[p.expert[i]], 1)] = (uint16_t)i;
     __syncthreads();
     for (int u = wave; u + 1 < p.units; u += THREADS / 64) {
       const uint32_t e = p.unit[u] >> 16;
       if (p.unit[u + 1] >> 16 != e || (u > 0 && p.unit[u - 1] >> 16 == e)) continue;
       uint32_t to = p.unit[u] & 0xffffu;
       for (int i0 = 0; i0 < n; i0 += 64) {
-        const bool mine = i0 + lane < n && (uint32_t)idx[i0 + lane] == e;
+        const bool mine = i0 + lane < n && p.expert[i0 + lane] == e;
         const uint64_t m = __ballot(mine);
         if (mine) p.list[to + (uint32_t)__builtin_popcountll(m & ((1ull << lane) - 1))] = (uint16_t)(i0 + lane);
         to += (uint32_t)__builtin_popcountll(m);
@@ -369,33 +391,33 @@ __device__ __forceinline__ void make_plan(Plan& p, const int64_t* idx, int n, in
 
 // The list of one expert in increasing order: workgroups that take its units each find the same.
 template <int THREADS>
-__device__ __forceinline__ void list_of(Plan& p, const int64_t* idx, int n, int expert) {
-  constexpr int kWaves = THREADS / 64, kOwn = kMaxAssigned / THREADS;
+__device__ __forceinline__ void list_of(Plan& p, int n, int expert) {
+  constexpr int kWaves = THREADS / 64;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int each = (n + kWaves * 64 - 1) / (kWaves * 64);  // 64 assignments a round, a wave's one behind the other
-  uint64_t mine[kOwn];
+  const int each = (n + kWaves * 64 - 1) / (kWaves * 64);  // rounds of 64 assignments, a wave's one behind the other
   uint32_t found = 0;
-#pragma unroll
-  for (int o = 0; o < kOwn; ++o) {
+  for (int o = 0; o < each; ++o) {
     const int i = (wave * each + o) * 64 + lane;
-    mine[o] = __ballot(o < each && i < n && (int)idx[i < n ? i : 0] == expert);
-    found += (uint32_t)__builtin_popcountll(mine[o]);
+    found += (uint32_t)__builtin_popcountll(__ballot(i < n && p.expert[i < n ? i : 0] == expert));
   }
   if (lane == 0) p.waves[wave] = found;
   __syncthreads();
   uint32_t at = 0;
   for (int w = 0; w < wave; ++w) at += p.waves[w];
-#pragma unroll
-  for (int o = 0; o < kOwn; ++o) {
-    if (mine[o] >> lane & 1)
-      p.list[at + (uint32_t)__builtin_popcountll(mine[o] & ((1ull << lane) - 1))] = (uint16_t)((wave * each + o) * 64 + lane);
-    at += (uint32_t)__builtin_popcountll(mine[o]);
+  for (int o = 0; o < each; ++o) {
+    const int i = (wave * each + o) * 64 + lane;
+    const bool mine = i < n && p.expert[i < n ? i : 0] == expert;
+    const uint64_t m = __ballot(mine);
+    if (mine) p.list[at + (uint32_t)__builtin_popcountll(m & ((1ull << lane) - 1))] = (uint16_t)i;
+    at += (uint32_t)__builtin_popcountll(m);
   }
   __syncthreads();
 }
 
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
 // ---------------------------------------------------------------------------------------------
-// Products of M times 16 weight rows with NC times 16 tokens
+// Products of 16 weight rows with 16 tokens
 // ---------------------------------------------------------------------------------------------
 // In a step of 128 of K a lane has row (or token) lane % 16 and the 32 neighbours from 32 (lane / 16) on; both
 // operands take the same ones, so that their order in a product does not matter.
@@ -405,21 +427,20 @@ struct Weights {
   static constexpr int kEach = FP8 ? 16 : 8;   // elements of one
   u4 w[M][kWords];
   float scale[FP8 ? M : 1];
-  // rows[m] + off: this lane's; left: elements of K from this lane's first on
-  __device__ __forceinline__ void load(const uint8_t* const (&rows)[M], int64_t off, int left) {
-    if (__builtin_expect(left >= 32, 1)) {
+  // step b of 16 rows[m] from this lane's offset on, scaled by scales[m]; left: elements of K from there on
+  __device__ __forceinline__ void load(const __amdgpu_buffer_rsrc_t (&rows)[M], uint32_t mine, const floats_at (&scales)[M], int b,
+                                       int left) {
+    const uint32_t off = mine + (uint32_t)b * (FP8 ? kBlock : 2 * kBlock);
+    left -= b * kBlock;
 #pragma unroll
-      for (int m = 0; m < M; ++m)
+    for (int j = 0; j < kWords; ++j) {
+      const uint32_t at = j * kEach < left ? off + 16 * j : kNothing;
 #pragma unroll
-        for (int j = 0; j < kWords; ++j) w[m][j] = __builtin_nontemporal_load(reinterpret_cast<const u4*>(rows[m] + off) + j);
-    } else {
+      for (int m = 0; m < M; ++m) w[m][j] = load16<kStream>(rows[m], at);
+    }
+    if constexpr (FP8) {
 #pragma unroll
-      for (int m = 0; m < M; ++m)
-#pragma unroll
-        for (int j = 0; j < kWords; ++j) {
-          w[m][j] = u4{0, 0, 0, 0};
-          if (j * kEach < left) w[m][j] = *(reinterpret_cast<const u4*>(rows[m] + off) + j);
-        }
+      for (int m = 0; m < M; ++m) scale[m] = scales[m][b];
     }
   }
   // the q-th 8 elements of row m as bf16
@@ -437,323 +458,390 @@ struct Weights {
   }
 };
 
-template <int NC, int P>
-struct Tokens {
-  u4 b[NC][P][4];
-  // cols[c]: this lane's token's, null for none; parts `plane` elements apart
-  __device__ __forceinline__ void load(const uint16_t* const (&cols)[NC], int64_t plane, int64_t off, int left) {
+// 16 rows of an expert's stacked weights from `row` on, a lane's offset into them, and their blocks' scales.
+template <bool FP8>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(const uint8_t* w, int64_t row, int K) {
+  const int64_t pitch = (int64_t)K * (FP8 ? 1 : 2);
+  return make_rsrc(w + row * pitch, 16 * pitch);
+}
+template <bool FP8>
+__device__ __forceinline__ uint32_t offset_in_rows(int K) {
+  const int lane = threadIdx.x & 63;
+  return (uint32_t)((lane & 15) * K * (FP8 ? 1 : 2) + (lane >> 4) * (FP8 ? 32 : 64));
+}
+__device__ __forceinline__ floats_at scales_at(const float* s, int64_t expert, int64_t row, int rows, int K) {
+  return (floats_at)(uintptr_t)s + (expert * ((rows + kBlock - 1) / kBlock) + row / kBlock) * ((K + kBlock - 1) / kBlock);
+}
+
+template <bool FP8, int M, int NC>
+__device__ __forceinline__ void clear(f4 (&acc)[M][NC]) {
+#pragma unroll
+  for (int m = 0; m < M; ++m)
+#pragma unroll
+    for (int c = 0; c < NC; ++c) acc[m][c] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+}
+// A step's sums join the others by their block's scale (16 rows share it).
+template <bool FP8, int M, int NC>
+__device__ __forceinline__ void join_step(f4 (&acc)[M][NC], const f4 (&sum)[M][NC], const Weights<FP8, M>& w) {
+#pragma unroll
+  for (int m = 0; m < M; ++m)
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
-      for (int p = 0; p < P; ++p)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          b[c][p][q] = u4{0, 0, 0, 0};
-          if (cols[c] && q * 8 < left) b[c][p][q] = *(reinterpret_cast<const u4*>(cols[c] + p * plane + off) + q);
-        }
-  }
-};
+      for (int i = 0; i < 4; ++i) acc[m][c][i] = __builtin_fmaf(w.scale[m], sum[m][c][i], acc[m][c][i]);
+}
 
-template <bool FP8, int M, int NC, int P>
-__device__ __forceinline__ void multiply(f4 (&acc)[M][NC], const Weights<FP8, M>& w, const Tokens<NC, P>& x) {
-  f4 sum[M][NC];
-  if constexpr (FP8) {
+// h = weight silu(h1) h2 of four neighbouring channels, its parts stored `plane` elements apart.
+template <int PH>
+__device__ __forceinline__ void store_h(uint16_t* to, int64_t plane, f4 h1, f4 h2, float weight) {
+  float h[8];
 #pragma unroll
-    for (int m = 0; m < M; ++m)
-#pragma unroll
-      for (int c = 0; c < NC; ++c) sum[m][c] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int e = 0; e < 4; ++e) {
+    h[e] = weight * (h1[e] / (1.0f + expf(-h1[e])) * h2[e]);
+    h[4 + e] = 0.0f;
   }
+  u4 part[PH];
+  split8<PH>(h, part);
 #pragma unroll
-  for (int m = 0; m < M; ++m)
+  for (int p = 0; p < PH; ++p) {
+    const uint2 v = {part[p][0], part[p][1]};
+    *reinterpret_cast<uint2*>(to + p * plane) = v;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Up to 16 tokens
+// ---------------------------------------------------------------------------------------------
+template <int P>
+struct Tokens {
+  u4 b[P][4];
+  // step's part of this lane's token, which begins at `mine` of parts[p] (kNothing for none)
+  __device__ __forceinline__ void load(const __amdgpu_buffer_rsrc_t (&parts)[P], uint32_t mine, int step, int left) {
+    left -= step * kBlock;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const bf8 row = w.frag(m, q);
+      const uint32_t at = q * 8 < left ? mine + (uint32_t)step * 2 * kBlock + 16 * q : kNothing;
 #pragma unroll
-      for (int c = 0; c < NC; ++c)
-#pragma unroll
-        for (int p = P - 1; p >= 0; --p) {
-          f4& s = FP8 ? sum[m][c] : acc[m][c];
-          s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(row, __builtin_bit_cast(bf8, x.b[c][p][q]), s, 0, 0, 0);
-        }
+      for (int p = 0; p < P; ++p) b[p][q] = load16(parts[p], at);
     }
-  if constexpr (FP8) {
-#pragma unroll
-    for (int m = 0; m < M; ++m)
-#pragma unroll
-      for (int c = 0; c < NC; ++c)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[m][c][i] = __builtin_fmaf(w.scale[m], sum[m][c][i], acc[m][c][i]);
   }
-}
-
-// acc += rows[.., first : end : step steps of K] times the tokens; the next step's loads go out before a step's
-// products (the tokens' too, where they are few registers; else theirs of this step go first, as loads are waited
-// for in their order).
-template <bool FP8, int M, int NC, int P>
-__device__ __forceinline__ void sum_steps(f4 (&acc)[M][NC], const uint8_t* const (&rows)[M], const float* const (&scales)[M],
-                                          const uint16_t* const (&cols)[NC], int64_t plane, int K, int first, int end,
-                                          int step) {
-  constexpr bool kAhead = NC * P <= 2;
-  if (first >= end) return;
-  const int mine = (threadIdx.x >> 4 & 3) * 32;
-  Weights<FP8, M> w, next;
-  Tokens<NC, P> x, ahead;
-  auto load = [&](Weights<FP8, M>& to, int b) {
-    to.load(rows, (int64_t)b * (FP8 ? kBlock : 2 * kBlock), K - b * kBlock - mine);
-    if constexpr (FP8) {
-#pragma unroll
-      for (int m = 0; m < M; ++m) to.scale[m] = scales[m][b];
-    }
-  };
-  auto tokens = [&](Tokens<NC, P>& to, int b) { to.load(cols, plane, (int64_t)b * kBlock, K - b * kBlock - mine); };
-  load(w, first);
-  if constexpr (kAhead) tokens(x, first);
-  for (int b = first; b < end; b += 2 * step) {
-    if constexpr (!kAhead) tokens(x, b);
-    if (b + step < end) {
-      load(next, b + step);
-      if constexpr (kAhead) tokens(ahead, b + step);
-    }
-    multiply<FP8, M, NC, P>(acc, w, x);
-    if (b + step >= end) break;
-    if constexpr (!kAhead) tokens(x, b + step);
-    if (b + 2 * step < end) {
-      load(w, b + 2 * step);
-      if constexpr (kAhead) tokens(x, b + 2 * step);
-    }
-    multiply<FP8, M, NC, P>(acc, next, kAhead ? ahead : x);
-  }
-}
-
-// ---------------------------------------------------------------------------------------------
-// Up: h = weight * silu(W1 x) * (W2 x)
-// ---------------------------------------------------------------------------------------------
-template <int R>
-struct UpShared {
-  Plan plan;
-  f4 sum[kUpWaves][2 * R][64];
 };
 
-template <int DT, bool FP8, int R, int NC, class LDS>
-__device__ __forceinline__ void up_unit(const LayerArgs& a, LDS& lds, const Expert w, int expert, int h0, int first, int n,
-                                        bool shared) {
-  constexpr int M = 2 * R, P = kXParts<DT>, PH = kHParts<DT>;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
-  const int H = w.H, KB = (a.D + kBlock - 1) / kBlock, RB = (2 * H + kBlock - 1) / kBlock;
-  const int64_t pitch = (int64_t)a.D * (FP8 ? 1 : 2);
-  const uint8_t* rows[M];
-  const float* scales[M];
-  const uint16_t* cols[NC];
+template <bool FP8, int M, int P>
+__device__ __forceinline__ void multiply(f4 (&acc)[M][1], const Weights<FP8, M>& w, const Tokens<P>& x) {
+  f4 sum[M][1];
+  if constexpr (FP8) clear<FP8, M, 1>(sum);
 #pragma unroll
-  for (int m = 0; m < M; ++m) {
-    const int row = (m < R ? 0 : H) + h0 + 16 * (m < R ? m : m - R);
-    rows[m] = w.w12 + ((int64_t)expert * 2 * H + row + r) * pitch + g * (FP8 ? 32 : 64);
-    scales[m] = FP8 ? w.s12 + ((int64_t)expert * RB + row / kBlock) * KB : nullptr;
-  }
+  for (int q = 0; q < 4; ++q)
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    const int i = c * 16 + r;
-    cols[c] = nullptr;
-    if (i < n) {
-      const int t = shared ? first + i : lds.plan.list[first + i] / a.k;
-      cols[c] = a.xb + (int64_t)t * a.Dp + g * 32;
+    for (int m = 0; m < M; ++m) {
+      const bf8 row = w.frag(m, q);
+#pragma unroll
+      for (int p = P - 1; p >= 0; --p) {
+        f4& s = FP8 ? sum[m][0] : acc[m][0];
+        s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(row, __builtin_bit_cast(bf8, x.b[p][q]), s, 0, 0, 0);
+      }
     }
-  }
-  f4 acc[M][NC];
-#pragma unroll
-  for (int m = 0; m < M; ++m)
-#pragma unroll
-    for (int c = 0; c < NC; ++c) acc[m][c] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-  sum_steps<FP8, M, NC, P>(acc, rows, scales, cols, (int64_t)a.T * a.Dp, a.D, wave, KB, kUpWaves);
-  const int64_t plane = (int64_t)(shared ? a.T : a.T * a.k) * H;
-#pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    if (c * 16 >= n) break;
-    if (c) __syncthreads();  // (the readers before)
-#pragma unroll
-    for (int m = 0; m < M; ++m) lds.sum[wave][m][lane] = acc[m][c];
-    __syncthreads();
-    // (four neighbouring channels of one token each)
-    const int m = wave, at = c * 16 + r;
-    if (m >= R || at >= n) continue;
-    f4 h1 = lds.sum[0][m][lane], h2 = lds.sum[0][m + R][lane];
-#pragma unroll
-    for (int v = 1; v < kUpWaves; ++v) {
-      h1 += lds.sum[v][m][lane];
-      h2 += lds.sum[v][m + R][lane];
+  if constexpr (FP8) join_step<FP8, M, 1>(acc, sum, w);
+}
+
+// acc += rows[.., steps first : end : step of K] times the tokens; the loads of the next step go out before a step's
+// products.
+template <bool FP8, int M, int P>
+__device__ __forceinline__ void sum_steps(f4 (&acc)[M][1], const __amdgpu_buffer_rsrc_t (&rows)[M], const floats_at (&scales)[M],
+                                          const __amdgpu_buffer_rsrc_t (&parts)[P], uint32_t token, int K, int first, int end,
+                                          int step) {
+  if (first >= end) return;
+  const int left = K - (threadIdx.x >> 4 & 3) * 32;
+  const uint32_t mine = offset_in_rows<FP8>(K);
+  Weights<FP8, M> w, next;
+  Tokens<P> x, ahead;
+  w.load(rows, mine, scales, first, left);
+  x.load(parts, token, first, left);
+  for (int b = first; b < end; b += 2 * step) {
+    const int b1 = b + step, b2 = b1 + step;
+    if (b1 < end) {
+      next.load(rows, mine, scales, b1, left);
+      ahead.load(parts, token, b1, left);
     }
-    const int row = shared ? first + at : lds.plan.list[first + at];
-    const float weight = shared ? 1.0f : a.weights[row];
-    float h[8];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      h[e] = weight * (h1[e] / (1.0f + expf(-h1[e])) * h2[e]);
-      h[4 + e] = 0.0f;
+    multiply<FP8, M, P>(acc, w, x);
+    if (b1 >= end) break;
+    if (b2 < end) {
+      w.load(rows, mine, scales, b2, left);
+      x.load(parts, token, b2, left);
     }
-    u4 part[PH];
-    split8<PH>(h, part);
-    uint16_t* to = (shared ? a.hs : a.hb) + (int64_t)row * H + h0 + 16 * m + 4 * g;
-#pragma unroll
-    for (int p = 0; p < PH; ++p) {
-      const uint2 v = {part[p][0], part[p][1]};
-      *reinterpret_cast<uint2*>(to + p * plane) = v;
-    }
+    multiply<FP8, M, P>(acc, next, ahead);
   }
 }
 
-template <int DT, bool FP8, int R, bool FEW>
-__global__ __launch_bounds__(64 * kUpWaves) void k_up(LayerArgs a) {
-  constexpr int UNIT = unit_tokens(DT);
-  __shared__ UpShared<R> lds;
-  const int tiles = (a.experts.H + 16 * R - 1) / (16 * R);
-  const int routed = a.units * tiles;
+template <int DT, bool FP8>
+__global__ __launch_bounds__(64 * kUpWaves) void k_up_few(LayerArgs a) {
+  constexpr int P = kXParts<DT>;
+  __shared__ Plan plan;
+  __shared__ f4 sum[kUpWaves][2][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+  const int tiles = a.experts.H / 16, routed = a.units * tiles;
   const bool shared = (int)blockIdx.x >= routed;
-  int expert = 0, tile, first, n, H;
+  int expert = 0, tile = blockIdx.x - routed, n = a.T;
   if (!shared) {
     const int u = blockIdx.x / tiles;
     tile = blockIdx.x - u * tiles;
-    make_plan<64 * kUpWaves, UNIT, false>(lds.plan, a.idx, a.T * a.k, a.E);
-    if (u >= lds.plan.units) return;
-    expert = (int)(lds.plan.unit[u] >> 16);
-    first = (int)(lds.plan.unit[u] & 0xffffu);
-    n = lds.plan.tokens[u];
-    list_of<64 * kUpWaves>(lds.plan, a.idx, a.T * a.k, expert);
-    H = a.experts.H;
-  } else {
-    H = a.shared.H;
-    const int i = blockIdx.x - routed, per = (H + 16 * R - 1) / (16 * R);
-    tile = i % per;
-    first = i / per * UNIT;
-    n = min(a.T - first, UNIT);
+    make_plan<64 * kUpWaves, kFewTokens, false>(plan, a.idx, a.T * a.k, a.E);
+    if (u >= plan.units) return;
+    expert = uniform((int)(plan.unit[u] >> 16));
+    n = uniform(plan.tokens[u]);
+    list_of<64 * kUpWaves>(plan, a.T * a.k, expert);
   }
-  const Expert w = shared ? a.shared : a.experts;
-  const int h0 = tile * 16 * R;
-  auto run = [&](auto rows, auto columns) {
-    up_unit<DT, FP8, decltype(rows)::value, decltype(columns)::value>(a, lds, w, expert, h0, first, n, shared);
-  };
-  auto with = [&](auto rows) {
-    if (FEW || n <= 16)
-      run(rows, std::integral_constant<int, 1>{});
-    else if (UNIT == 32 || n <= 32)
-      run(rows, std::integral_constant<int, FEW ? 1 : 2>{});
-    else
-      run(rows, std::integral_constant<int, FEW ? 1 : UNIT / 16>{});
-  };
-  if (R == 1 || h0 + 16 * R <= H)
-    with(std::integral_constant<int, R>{});
-  else
-    with(std::integral_constant<int, 1>{});  // the last 16 channels of an odd number of them
-}
-
-// ---------------------------------------------------------------------------------------------
-// Down: out = sum W3 h
-// ---------------------------------------------------------------------------------------------
-template <int R>
-constexpr int kDownPitch = 16 * R + 4;  // floats of a token's sums in LDS
-
-template <int DT, bool FP8, int R, int NC>
-__device__ __forceinline__ void down_unit(const LayerArgs& a, const Plan& plan, float* sums, const Expert w, int expert, int d0,
-                                          int first, int n, bool shared, int kb0, int kb1) {
-  constexpr int P = kHParts<DT>;
-  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const int H = w.H, KB = (H + kBlock - 1) / kBlock, RB = (a.D + kBlock - 1) / kBlock;
-  const int64_t pitch = (int64_t)H * (FP8 ? 1 : 2);
-  const uint8_t* rows[R];
-  const float* scales[R];
-  const uint16_t* cols[NC];
-  int token[NC];
+  const int H = shared ? a.shared.H : a.experts.H, h0 = tile * 16, KB = (a.D + kBlock - 1) / kBlock;
+  const uint8_t* w12 = shared ? a.shared.w12 : a.experts.w12;
+  const float* s12 = shared ? a.shared.s12 : a.experts.s12;
+  __amdgpu_buffer_rsrc_t rows[2], parts[P];
+  floats_at scales[2];
 #pragma unroll
-  for (int m = 0; m < R; ++m) {
-    const int row = d0 + 16 * m;
-    rows[m] = w.w3 + ((int64_t)expert * a.D + row + r) * pitch + g * (FP8 ? 32 : 64);
-    scales[m] = FP8 ? w.s3 + ((int64_t)expert * RB + row / kBlock) * KB : nullptr;
+  for (int m = 0; m < 2; ++m) {
+    rows[m] = rows_at<FP8>(w12, (int64_t)expert * 2 * H + m * H + h0, a.D);
+    scales[m] = scales_at(s12, expert, m * H + h0, 2 * H, a.D);
   }
+  const int64_t plane = (int64_t)a.T * a.Dp;
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    const int i = c * 16 + r;
-    cols[c] = nullptr;
-    token[c] = -1;
-    if (i < n) {
-      const int at = shared ? first + i : plan.list[first + i];
-      token[c] = shared ? at : at / a.k;
-      cols[c] = (shared ? a.hs : a.hb) + (int64_t)at * H + g * 32;
-    }
-  }
-  f4 acc[R][NC];
+  for (int p = 0; p < P; ++p) parts[p] = make_rsrc(a.xb + p * plane, 2 * plane);
+  const int at = r < n ? (shared ? r : plan.list[r]) : 0;
+  const uint32_t token = r < n ? (uint32_t)((shared ? at : at / a.k) * a.Dp + g * 32) * 2 : kNothing;
+  f4 acc[2][1];
+  clear<FP8, 2, 1>(acc);
+  sum_steps<FP8, 2, P>(acc, rows, scales, parts, token, a.D, uniform(wave), KB, kUpWaves);
 #pragma unroll
-  for (int m = 0; m < R; ++m)
-#pragma unroll
-    for (int c = 0; c < NC; ++c) acc[m][c] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-  sum_steps<FP8, R, NC, P>(acc, rows, scales, cols, (int64_t)(shared ? a.T : a.T * a.k) * H, H, kb0, kb1, 1);
-  // (a token has an expert once, so a wave adds to a value once a unit)
-#pragma unroll
-  for (int c = 0; c < NC; ++c)
-    if (token[c] >= 0) {
-#pragma unroll
-      for (int m = 0; m < R; ++m) {
-        f4* to = reinterpret_cast<f4*>(sums + token[c] * kDownPitch<R> + 16 * m + 4 * g);
-        *to += acc[m][c];
-      }
-    }
-}
-
-template <int DT, bool FP8, int R, bool FEW>
-__global__ __launch_bounds__(64 * kDownWaves) void k_down(LayerArgs a) {
-  constexpr int UNIT = unit_tokens(DT);
-  __shared__ Plan plan;
-  extern __shared__ f4 joined[];  // [waves][T][kDownPitch] floats
-  float* const sums = reinterpret_cast<float*>(joined);
-  const int wave = threadIdx.x >> 6;
-  const int d0 = blockIdx.x * 16 * R;
-  const bool half = R == 2 && d0 + 32 > a.D;  // the last 16 channels of an odd number of them
-  make_plan<64 * kDownWaves, UNIT, true>(plan, a.idx, a.T * a.k, a.E);
-  const int each = a.T * kDownPitch<R>;
-  for (int i = threadIdx.x; i < kDownWaves * each; i += 64 * kDownWaves) sums[i] = 0.0f;
+  for (int m = 0; m < 2; ++m) sum[wave][m][lane] = acc[m][0];
   __syncthreads();
+  if (wave > 0 || r >= n) return;
+  f4 h1 = sum[0][0][lane], h2 = sum[0][1][lane];
+#pragma unroll
+  for (int v = 1; v < kUpWaves; ++v) {
+    h1 += sum[v][0][lane];
+    h2 += sum[v][1][lane];
+  }
+  store_h<kHParts<DT>>((shared ? a.hs : a.hb) + (int64_t)at * H + h0 + 4 * g, (int64_t)(shared ? a.T : a.T * a.k) * H, h1, h2,
+                       shared ? 1.0f : a.weights[at]);
+}
+
+constexpr int kSumPitch = 20;  // floats of a token's 16 sums in LDS
+
+template <int DT, bool FP8>
+__global__ __launch_bounds__(64 * kDownWaves) void k_down_few(LayerArgs a) {
+  constexpr int P = kHParts<DT>;
+  __shared__ Plan plan;
+  __shared__ f4 sums[kDownWaves][kFewTokens][kSumPitch / 4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+  const int d0 = blockIdx.x * 16;
+  make_plan<64 * kDownWaves, kFewTokens, true>(plan, a.idx, a.T * a.k, a.E);
+  for (int t = g; t < a.T; t += 4)
+    if (r < kSumPitch / 4) sums[wave][t][r] = f4{0.0f, 0.0f, 0.0f, 0.0f};
   // the waves share the steps of all units, the shared expert's behind the others'
-  const int KB = (a.experts.H + kBlock - 1) / kBlock;
-  const int routed = plan.units * KB;
-  const int KS = a.shared.w12 ? (a.shared.H + kBlock - 1) / kBlock : 0;
-  const int all = routed + (KS ? (a.T + UNIT - 1) / UNIT * KS : 0);
-  int at = (int)((int64_t)all * wave / kDownWaves);
-  const int end = (int)((int64_t)all * (wave + 1) / kDownWaves);
+  const int KB = (a.experts.H + kBlock - 1) / kBlock, routed = uniform(plan.units) * KB;
+  const int all = routed + (a.shared.H + kBlock - 1) / kBlock;
+  int at = uniform(all * wave / kDownWaves);
+  const int end = uniform(all * (wave + 1) / kDownWaves);
   while (at < end) {
     const bool shared = at >= routed;
-    const int per = shared ? KS : KB, from = shared ? at - routed : at;
-    const int u = from / per, kb0 = from - u * per, kb1 = min(per, kb0 + end - at);
-    const int expert = shared ? 0 : (int)(plan.unit[u] >> 16);
-    const int first = shared ? u * UNIT : (int)(plan.unit[u] & 0xffffu);
-    const int n = shared ? min(a.T - first, UNIT) : plan.tokens[u];
-    const Expert w = shared ? a.shared : a.experts;
-    auto run = [&](auto columns) {
-      constexpr int NC = decltype(columns)::value;
-      if (half) {
-        // rows past D would lie outside: one fragment, its sums at the same pitch
-        down_unit<DT, FP8, 1, NC>(a, plan, sums + wave * each, w, expert, d0, first, n, shared, kb0, kb1);
-      } else {
-        down_unit<DT, FP8, R, NC>(a, plan, sums + wave * each, w, expert, d0, first, n, shared, kb0, kb1);
-      }
-    };
-    if (FEW || n <= 16)
-      run(std::integral_constant<int, 1>{});
-    else if (UNIT == 32 || n <= 32)
-      run(std::integral_constant<int, FEW ? 1 : 2>{});
-    else
-      run(std::integral_constant<int, FEW ? 1 : UNIT / 16>{});
+    const int u = shared ? 0 : at / KB, kb0 = shared ? at - routed : at - u * KB;
+    const int kb1 = shared ? kb0 + end - at : min(KB, kb0 + end - at);
+    const int expert = shared ? 0 : uniform((int)(plan.unit[u] >> 16)), first = shared ? 0 : uniform((int)(plan.unit[u] & 0xffffu));
+    const int n = shared ? a.T : uniform(plan.tokens[u]), H = shared ? a.shared.H : a.experts.H;
+    const __amdgpu_buffer_rsrc_t rows[1] = {rows_at<FP8>(shared ? a.shared.w3 : a.experts.w3, (int64_t)expert * a.D + d0, H)};
+    const floats_at scales[1] = {scales_at(shared ? a.shared.s3 : a.experts.s3, expert, d0, a.D, H)};
+    __amdgpu_buffer_rsrc_t parts[P];
+    const int64_t plane = (int64_t)(shared ? a.T : a.T * a.k) * H;
+#pragma unroll
+    for (int p = 0; p < P; ++p) parts[p] = make_rsrc((shared ? a.hs : a.hb) + p * plane, 2 * plane);
+    const int row = r < n ? (shared ? r : plan.list[first + r]) : 0;
+    const uint32_t token = r < n ? (uint32_t)(row * H + g * 32) * 2 : kNothing;
+    f4 acc[1][1];
+    clear<FP8, 1, 1>(acc);
+    sum_steps<FP8, 1, P>(acc, rows, scales, parts, token, H, kb0, kb1, 1);
+    // (a token has an expert once, so a wave adds to a value once a unit)
+    if (r < n) sums[wave][shared ? row : row / a.k][g] += acc[0][0];
     at += kb1 - kb0;
   }
   __syncthreads();
-  const int width = half ? 16 : 16 * R, row_pitch = half ? kDownPitch<1> : kDownPitch<R>;
-  for (int i = threadIdx.x; i < a.T * width; i += 64 * kDownWaves) {
-    const int t = i / width, d = i - t * width;
+  for (int i = threadIdx.x; i < a.T * 16; i += 64 * kDownWaves) {
+    const int t = i >> 4, d = i & 15;
     float s = 0.0f;
 #pragma unroll
-    for (int v = 0; v < kDownWaves; ++v) s += sums[v * each + t * row_pitch + d];
+    for (int v = 0; v < kDownWaves; ++v) s += sums[v][t][d >> 2][d & 3];
     const int64_t o = (int64_t)t * a.D + d0 + d;
     if constexpr (DT == CIN_DT_F32)
       static_cast<float*>(a.out)[o] = s;
     else
       static_cast<uint16_t*>(a.out)[o] = (uint16_t)f32_to_half_bits(DT, s);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// More tokens
+// ---------------------------------------------------------------------------------------------
+constexpr int kTokenPitch = kBlock + 8;  // elements of a token's step in LDS: 16 lanes' 16 bytes on all banks
+
+// Rows of a workgroup: 16 hidden channels (of W1 and W2 each) a wave, or 32 output channels.
+template <bool UP>
+constexpr int kTileRows = kTileWaves * (UP ? 16 : 32);
+
+template <int DT, bool FP8, bool UP, int NC>
+__device__ __forceinline__ void tile_unit(const LayerArgs& a, const Plan& plan, uint16_t* lds, int expert, int tile, int first, int n,
+                                          bool shared) {
+  constexpr int P = UP ? kXParts<DT> : kHParts<DT>;
+  constexpr int kChunks = NC * 16 * P * (kBlock / 8), kThreads = 64 * kTileWaves;  // of 16 bytes, a step
+  constexpr int kOwn = (kChunks + kThreads - 1) / kThreads;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
+  const int H = shared ? a.shared.H : a.experts.H, K = UP ? a.D : H, KB = (K + kBlock - 1) / kBlock;
+  const int row0 = tile * kTileRows<UP> + wave * (UP ? 16 : 32), rows_all = UP ? H : a.D;
+  const bool active = row0 < rows_all, both = UP || row0 + 16 < rows_all;
+  // this lane's weight rows; those past the end are the first ones again and not stored
+  __amdgpu_buffer_rsrc_t rows[2];
+  floats_at scales[2];
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    const int row = UP ? (active ? row0 : 0) + m * H : (!active ? 0 : row0 + (m && both ? 16 : 0));
+    const uint8_t* w = UP ? (shared ? a.shared.w12 : a.experts.w12) : (shared ? a.shared.w3 : a.experts.w3);
+    const float* s = UP ? (shared ? a.shared.s12 : a.experts.s12) : (shared ? a.shared.s3 : a.experts.s3);
+    const int stacked = UP ? 2 * H : a.D;
+    rows[m] = rows_at<FP8>(w, (int64_t)expert * stacked + row, K);
+    scales[m] = scales_at(s, expert, row, stacked, K);
+  }
+  // this thread's 16 bytes of the tokens' parts (of all of them at most 128 x 16 x 65536 x 3 x 2 bytes)
+  const int pitch = UP ? a.Dp : H;
+  const int64_t plane = (int64_t)(UP ? a.T : shared ? a.T : a.T * a.k) * pitch;
+  const __amdgpu_buffer_rsrc_t parts = make_rsrc(UP ? a.xb : shared ? a.hs : a.hb, 2 * P * plane);
+  uint32_t from[kOwn], to[kOwn];
+#pragma unroll
+  for (int o = 0; o < kOwn; ++o) {
+    const int q = threadIdx.x + o * kThreads, chunk = q & 15, i = (q >> 4) % (NC * 16), p = (q >> 4) / (NC * 16);
+    from[o] = kNothing;
+    to[o] = (uint32_t)((p * NC * 16 + i) * kTokenPitch + chunk * 8);
+    if (q < kChunks && i < n) {
+      const int at = shared ? first + i : plan.list[first + i];
+      from[o] = (uint32_t)(2 * (p * plane + (int64_t)(UP && !shared ? at / a.k : at) * pitch + chunk * 8));
+    }
+  }
+  u4 part[kOwn];
+  const int end = pitch - (int)(threadIdx.x & 15) * 8;
+  auto fetch = [&](int b) {
+    const bool there = b * kBlock < end;
+#pragma unroll
+    for (int o = 0; o < kOwn; ++o) part[o] = load16(parts, there ? from[o] + (uint32_t)b * 2 * kBlock : kNothing);
+  };
+  auto leave = [&]() {
+#pragma unroll
+    for (int o = 0; o < kOwn; ++o)
+      if (kChunks % kThreads == 0 || threadIdx.x + o * kThreads < kChunks) *reinterpret_cast<u4*>(lds + to[o]) = part[o];
+  };
+  f4 acc[2][NC];
+  clear<FP8, 2, NC>(acc);
+  const int left = K - g * 32;
+  Weights<FP8, 2> w, next;
+  fetch(0);
+  const uint32_t mine = offset_in_rows<FP8>(K);
+  w.load(rows, mine, scales, 0, left);
+  leave();
+  __syncthreads();
+  // one step: the next one's loads go out first (its tokens' before its weights', as loads are waited for in their order)
+  auto one_step = [&](int b, const Weights<FP8, 2>& now, Weights<FP8, 2>& later) {
+    const bool more = b + 1 < KB;
+    if (more) {
+      fetch(b + 1);
+      later.load(rows, mine, scales, b + 1, left);
+    }
+    if (active) {
+      f4 sum[2][NC];
+      if constexpr (FP8) clear<FP8, 2, NC>(sum);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const bf8 f[2] = {now.frag(0, q), now.frag(1, q)};
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int p = P - 1; p >= 0; --p) {
+            const bf8 x = *reinterpret_cast<const bf8*>(lds + (p * NC * 16 + c * 16 + r) * kTokenPitch + g * 32 + q * 8);
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+              f4& s = FP8 ? sum[m][c] : acc[m][c];
+              s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[m], x, s, 0, 0, 0);
+            }
+          }
+      }
+      if constexpr (FP8) join_step<FP8, 2, NC>(acc, sum, now);
+    }
+    __syncthreads();
+    if (more) leave();
+    __syncthreads();
+  };
+  for (int b = 0; b < KB; b += 2) {
+    one_step(b, w, next);
+    if (b + 1 < KB) one_step(b + 1, next, w);
+  }
+  if (!active) return;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int i = c * 16 + r;
+    if (i >= n) continue;
+    const int at = shared ? first + i : plan.list[first + i];
+    if constexpr (UP) {
+      store_h<kHParts<DT>>((shared ? a.hs : a.hb) + (int64_t)at * H + row0 + 4 * g, (int64_t)(shared ? a.T : a.T * a.k) * H,
+                           acc[0][c], acc[1][c], shared ? 1.0f : a.weights[at]);
+    } else {
+      float* y = a.y + (int64_t)(shared ? a.T * a.k + at : at) * a.D + row0 + 4 * g;
+      *reinterpret_cast<f4*>(y) = acc[0][c];
+      if (both) *reinterpret_cast<f4*>(y + 16) = acc[1][c];
+    }
+  }
+}
+
+// The units of a tile are neighbours: those of one expert read its weights at the same time, from the cache.
+template <int DT, bool FP8, bool UP>
+__global__ __launch_bounds__(64 * kTileWaves, 4) void k_products(LayerArgs a) {
+  constexpr int UNIT = kUnitTokens, ROWS = kTileRows<UP>;
+  __shared__ Plan plan;
+  extern __shared__ u4 tokens[];  // [parts, columns][kTokenPitch] of 16 bits
+  const int tiles = ((UP ? a.experts.H : a.D) + ROWS - 1) / ROWS, routed = a.units * tiles;
+  const bool shared = (int)blockIdx.x >= routed;
+  int expert = 0, tile, first, n;
+  if (!shared) {
+    tile = blockIdx.x / a.units;
+    const int u = blockIdx.x - tile * a.units;
+    make_plan<64 * kTileWaves, UNIT, false>(plan, a.idx, a.T * a.k, a.E);
+    if (u >= plan.units) return;
+    expert = uniform((int)(plan.unit[u] >> 16));
+    first = uniform((int)(plan.unit[u] & 0xffffu));
+    n = uniform(plan.tokens[u]);
+    list_of<64 * kTileWaves>(plan, a.T * a.k, expert);
+  } else {
+    const int i = blockIdx.x - routed, units = (a.T + UNIT - 1) / UNIT;
+    tile = i / units;
+    first = (i - tile * units) * UNIT;
+    n = min(a.T - first, UNIT);
+  }
+  uint16_t* lds = reinterpret_cast<uint16_t*>(tokens);
+  if (n <= 16)
+    tile_unit<DT, FP8, UP, 1>(a, plan, lds, expert, tile, first, n, shared);
+  else
+    tile_unit<DT, FP8, UP, UNIT / 16>(a, plan, lds, expert, tile, first, n, shared);
+}
+
+// out = the sum of a token's rows of y, in the order of its experts, the shared one's last.
+template <int DT>
+__global__ __launch_bounds__(256) void k_join(LayerArgs a) {
+  const int per = a.D / 4, i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= a.T * per) return;
+  const int t = i / per, d = (i - t * per) * 4;
+  const float* y = a.y + (int64_t)t * a.k * a.D + d;
+  f4 s = *reinterpret_cast<const f4*>(y);
+  for (int j = 1; j < a.k; ++j) s += *reinterpret_cast<const f4*>(y + (int64_t)j * a.D);
+  if (a.shared.H) s += *reinterpret_cast<const f4*>(a.y + (int64_t)(a.T * a.k + t) * a.D + d);
+  const int64_t o = (int64_t)t * a.D + d;
+  if constexpr (DT == CIN_DT_F32) {
+    *reinterpret_cast<f4*>(static_cast<float*>(a.out) + o) = s;
+  } else {
+    const uint2 v = {f32x2_to_half2_bits<DT>(s[0], s[1]), f32x2_to_half2_bits<DT>(s[2], s[3])};
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + o) = v;
   }
 }
 
@@ -775,6 +863,7 @@ int64_t layout(LayerArgs& a, int dtype, char* base) {
   a.xb = reinterpret_cast<uint16_t*>(take(2 * px * a.T * a.Dp));
   a.hb = reinterpret_cast<uint16_t*>(take(2 * ph * a.T * a.k * a.experts.H));
   a.hs = reinterpret_cast<uint16_t*>(take(2 * ph * a.T * a.shared.H));
+  a.y = reinterpret_cast<float*>(take(a.T > kFewTokens ? 4LL * a.T * (a.k + 1) * a.D : 0));
   return at;
 }
 
@@ -786,7 +875,7 @@ bool sizes_ok(int dtype, int64_t T, int64_t D, int64_t E, int64_t k, int64_t H, 
 const char* const kSizes =
     "dtype must be bf16, fp16 or fp32, T <= 128, E <= 1024, k <= min(16, E), D, H and the shared expert's H multiples of 16 up to 65536";
 
-void set_sizes(LayerArgs& a, int dtype, int64_t T, int64_t D, int64_t E, int64_t k, int64_t H, int64_t Hs) {
+void set_sizes(LayerArgs& a, int64_t T, int64_t D, int64_t E, int64_t k, int64_t H, int64_t Hs) {
   a.T = (int)T;
   a.D = (int)D;
   a.Dp = (int)(cdiv(D, kBlock) * kBlock);
@@ -796,34 +885,38 @@ void set_sizes(LayerArgs& a, int dtype, int64_t T, int64_t D, int64_t E, int64_t
   a.shared.H = (int)Hs;
   a.slices = (int)cdiv(a.Dp, kRouterSlice);
   const int64_t n = T * k;
-  a.units = (int)((n < E ? n : E) + n / unit_tokens(dtype));
+  a.units = (int)((n < E ? n : E) + n / kUnitTokens);
 }
 
-// FEW: at most 16 tokens, RD times 16 rows a workgroup of k_down.
-template <int DT, bool FP8, bool FEW>
+template <int DT, bool FP8, bool UP>
 void launch_products(const LayerArgs& a, hipStream_t stream) {
-  constexpr int RU = 1, RD = FEW ? 1 : 2;
-  const int per = (a.experts.H + 16 * RU - 1) / (16 * RU), unit = unit_tokens(DT);
-  const int shared = a.shared.w12 ? (a.shared.H + 16 * RU - 1) / (16 * RU) * ((a.T + unit - 1) / unit) : 0;
-  hipLaunchKernelGGL((k_up<DT, FP8, RU, FEW>), dim3(a.units * per + shared), dim3(64 * kUpWaves), 0, stream, a);
-  const size_t lds = sizeof(float) * kDownWaves * a.T * kDownPitch<RD>;
-  if (lds + sizeof(Plan) > 65536)
-    (void)hipFuncSetAttribute((const void*)k_down<DT, FP8, RD, FEW>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-  hipLaunchKernelGGL((k_down<DT, FP8, RD, FEW>), dim3((a.D + 16 * RD - 1) / (16 * RD)), dim3(64 * kDownWaves), lds, stream, a);
+  constexpr int P = UP ? kXParts<DT> : kHParts<DT>, ROWS = kTileRows<UP>, UNIT = kUnitTokens;
+  const int per = ((UP ? a.experts.H : a.D) + ROWS - 1) / ROWS;
+  const int shared = a.shared.H ? ((UP ? a.shared.H : a.D) + ROWS - 1) / ROWS * ((a.T + UNIT - 1) / UNIT) : 0;
+  const size_t lds = 2 * P * UNIT * kTokenPitch;
+  hipLaunchKernelGGL((k_products<DT, FP8, UP>), dim3(a.units * per + shared), dim3(64 * kTileWaves), lds, stream, a);
+}
+
+template <int DT, bool FP8>
+void launch_experts(const LayerArgs& a, hipStream_t stream) {
+  if (a.T <= kFewTokens) {
+    hipLaunchKernelGGL((k_up_few<DT, FP8>), dim3((a.units * a.experts.H + a.shared.H) / 16), dim3(64 * kUpWaves), 0, stream, a);
+    hipLaunchKernelGGL((k_down_few<DT, FP8>), dim3(a.D / 16), dim3(64 * kDownWaves), 0, stream, a);
+    return;
+  }
+  launch_products<DT, FP8, true>(a, stream);
+  launch_products<DT, FP8, false>(a, stream);
+  hipLaunchKernelGGL((k_join<DT>), dim3((a.T * (a.D / 4) + 255) / 256), dim3(256), 0, stream, a);
 }
 
 template <int DT>
 void launch(const LayerArgs& a, bool fp8, hipStream_t stream) {
   hipLaunchKernelGGL((k_router<DT>), dim3(a.slices * ((a.E + 15) / 16), (a.T + 15) / 16), dim3(256), 0, stream, a);
   hipLaunchKernelGGL(k_gate, dim3(a.T), dim3(256), 0, stream, a);
-  if (fp8 && a.T <= 16)
-    launch_products<DT, true, true>(a, stream);
-  else if (fp8)
-    launch_products<DT, true, false>(a, stream);
-  else if (a.T <= 16)
-    launch_products<DT, false, true>(a, stream);
+  if (fp8)
+    launch_experts<DT, true>(a, stream);
   else
-    launch_products<DT, false, false>(a, stream);
+    launch_experts<DT, false>(a, stream);
 }
 
 }  // namespace
@@ -836,7 +929,7 @@ int64_t cin_moe_decode_workspace(int dtype, int64_t T, int64_t D, int64_t E, int
     return -1;
   }
   LayerArgs a = {};
-  set_sizes(a, dtype, T, D, E, k, H, shared_H);
+  set_sizes(a, T, D, E, k, H, shared_H);
   return layout(a, dtype, nullptr);
 }
 
@@ -864,7 +957,7 @@ int cin_moe_decode(const void* x, int dtype, int64_t ldx, int64_t T, int64_t D, 
   CIN_CHECK_ARG(workspace_bytes >= cin_moe_decode_workspace(dtype, T, D, E, k, H, shared_H),
                 "cin_moe_decode: workspace below cin_moe_decode_workspace bytes");
   LayerArgs a = {};
-  set_sizes(a, dtype, T, D, E, k, H, shared_H);
+  set_sizes(a, T, D, E, k, H, shared_H);
   layout(a, dtype, static_cast<char*>(workspace));
   a.x = x;
   a.ldx = ldx;
