@@ -44,7 +44,6 @@ constexpr int kMaxGroups = 64;
 constexpr int kBlock = 128;        // of a scale, and a step of K
 constexpr int kMaxAssigned = kMaxTokens * kMaxTopK;
 constexpr int kUnitTokens = 32;    // of an expert, multiplied at once
-constexpr int kMaxUnits = kMaxExperts + kMaxAssigned / kUnitTokens;
 constexpr int kRouterSlice = 512;  // channels of a k_router workgroup
 constexpr int kUpWaves = 4, kDownWaves = 8, kTileWaves = 4;
 constexpr int kFewTokens = 16;
@@ -311,31 +310,21 @@ __global__ __launch_bounds__(256) void k_gate(LayerArgs a) {
 // Which expert multiplies which tokens
 // ---------------------------------------------------------------------------------------------
 // The assignments (t k + j) by expert, in units of up to UNIT of one expert.
-struct Plan {
-  int count[kMaxExperts];           // assignments of an expert, then where its next one goes
-  uint32_t unit[kMaxUnits];         // expert, first entry
-  uint8_t tokens[kMaxUnits];
-  uint16_t list[kMaxAssigned];
-  uint16_t expert[kMaxAssigned];    // of an assignment
+template <int UNITS>
+struct Counts {
+  int count[kMaxExperts];  // assignments of an expert, then where its next one goes
   uint32_t waves[kDownWaves];
   int units;
+  uint32_t unit[UNITS];    // expert, first entry
+  uint8_t tokens[UNITS];
 };
 
-// ALL: units begin at their place in the list of all experts, which follows: an expert's in the atomics' order, as it
-// only decides which column of a product a token has, but in increasing order where the expert has several units, whose
-// steps are summed apart.  Else units begin at their place among their expert's assignments.
-template <int THREADS, int UNIT, bool ALL>
-__device__ __forceinline__ void make_plan(Plan& p, const int64_t* idx, int n, int E) {
+// The units of all experts in the order of the experts, from each one's count; only unit `one` where UNITS is 1.  BASE:
+// a unit's first entry counts the assignments of the experts before, and so does count from then on.
+template <int THREADS, int UNIT, int UNITS, bool BASE>
+__device__ __forceinline__ void make_units(Counts<UNITS>& p, int E, int one) {
   constexpr int kOwn = kMaxExperts / THREADS;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  for (int e = tid; e < E; e += THREADS) p.count[e] = 0;
-  __syncthreads();
-  for (int i = tid; i < n; i += THREADS) {
-    const int e = (int)idx[i];
-    p.expert[i] = (uint16_t)e;
-    atomicAdd(&p.count[e], 1);
-  }
-  __syncthreads();
   // units (upper half) and assignments of the experts before this thread's
   uint32_t own = 0;
   int c[kOwn];
@@ -361,80 +350,109 @@ __device__ __forceinline__ void make_plan(Plan& p, const int64_t* idx, int n, in
 #pragma unroll
   for (int o = 0; o < kOwn; ++o) {
     const int e = tid * kOwn + o;
-    if (e < E) p.count[e] = (int)(at & 0xffffu);
+    if (BASE && e < E) p.count[e] = (int)(at & 0xffffu);
     for (int i = 0; i < c[o]; i += UNIT) {
-      p.unit[at >> 16] = (uint32_t)e << 16 | ((ALL ? at & 0xffffu : 0u) + i);
-      p.tokens[at >> 16] = (uint8_t)min(c[o] - i, UNIT);
+      const int u = (int)(at >> 16);
+      if (UNITS > 1 || u == one) {
+        p.unit[UNITS > 1 ? u : 0] = (uint32_t)e << 16 | ((BASE ? at & 0xffffu : 0u) + i);
+        p.tokens[UNITS > 1 ? u : 0] = (uint8_t)min(c[o] - i, UNIT);
+      }
       at += 1u << 16;
     }
     at += (uint32_t)c[o];
   }
   if (tid == 0) p.units = (int)(all >> 16);
   __syncthreads();
-  if constexpr (ALL) {
-    for (int i = tid; i < n; i += THREADS) p.list[atomicAdd(&p.count[p.expert[i]], 1)] = (uint16_t)i;
-    __syncthreads();
-    for (int u = wave; u + 1 < p.units; u += THREADS / 64) {
-      const uint32_t e = p.unit[u] >> 16;
-      if (p.unit[u + 1] >> 16 != e || (u > 0 && p.unit[u - 1] >> 16 == e)) continue;
-      uint32_t to = p.unit[u] & 0xffffu;
-      for (int i0 = 0; i0 < n; i0 += 64) {
-        const bool mine = i0 + lane < n && p.expert[i0 + lane] == e;
-        const uint64_t m = __ballot(mine);
-        if (mine) p.list[to + (uint32_t)__builtin_popcountll(m & ((1ull << lane) - 1))] = (uint16_t)(i0 + lane);
-        to += (uint32_t)__builtin_popcountll(m);
-      }
-    }
-    __syncthreads();
-  }
 }
 
-// The list of one expert in increasing order: workgroups that take its units each find the same.
-template <int THREADS>
-__device__ __forceinline__ void list_of(Plan& p, int n, int expert) {
-  constexpr int kWaves = THREADS / 64;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int each = (n + kWaves * 64 - 1) / (kWaves * 64);  // rounds of 64 assignments, a wave's one behind the other
-  uint32_t found = 0;
-  for (int o = 0; o < each; ++o) {
-    const int i = (wave * each + o) * 64 + lane;
-    found += (uint32_t)__builtin_popcountll(__ballot(i < n && p.expert[i < n ? i : 0] == expert));
-  }
-  if (lane == 0) p.waves[wave] = found;
+template <int THREADS, class Plan>
+__device__ __forceinline__ void count_experts(Plan& p, const int64_t* idx, int n, int E) {
+  for (int e = threadIdx.x; e < E; e += THREADS) p.counts.count[e] = 0;
   __syncthreads();
-  uint32_t at = 0;
-  for (int w = 0; w < wave; ++w) at += p.waves[w];
-  for (int o = 0; o < each; ++o) {
-    const int i = (wave * each + o) * 64 + lane;
-    const bool mine = i < n && p.expert[i < n ? i : 0] == expert;
-    const uint64_t m = __ballot(mine);
-    if (mine) p.list[at + (uint32_t)__builtin_popcountll(m & ((1ull << lane) - 1))] = (uint16_t)i;
-    at += (uint32_t)__builtin_popcountll(m);
+  for (int i = threadIdx.x; i < n; i += THREADS) {
+    const int e = (int)idx[i];
+    p.expert[i] = (uint16_t)e;
+    atomicAdd(&p.counts.count[e], 1);
   }
   __syncthreads();
 }
+
+// All units of up to kFewTokens tokens, with the list of all assignments by expert, an expert's in the atomics' order: it
+// only decides which column of a product a token has.
+struct Plan {
+  static constexpr int kMost = kFewTokens * kMaxTopK;
+  Counts<kMost> counts;
+  uint16_t expert[kMost], list[kMost];
+  template <int THREADS>
+  __device__ __forceinline__ void make(const int64_t* idx, int n, int E) {
+    count_experts<THREADS>(*this, idx, n, E);
+    make_units<THREADS, kFewTokens, kMost, true>(counts, E, 0);
+    for (int i = threadIdx.x; i < n; i += THREADS) list[atomicAdd(&counts.count[expert[i]], 1)] = (uint16_t)i;
+    __syncthreads();
+  }
+};
+
+// One unit of UNIT tokens, with the list of its expert in increasing order: workgroups that take the expert's units each
+// find the same.
+template <int UNIT, int MOST>
+struct OneUnit {
+  Counts<1> counts;
+  uint16_t expert[MOST], list[kMaxTokens];
+  // false where there is no such unit
+  template <int THREADS>
+  __device__ __forceinline__ bool make(const int64_t* idx, int n, int E, int u) {
+    constexpr int kWaves = THREADS / 64;
+    count_experts<THREADS>(*this, idx, n, E);
+    make_units<THREADS, UNIT, 1, false>(counts, E, u);
+    if (u >= counts.units) return false;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, mine = (int)(counts.unit[0] >> 16);
+    const int each = (n + kWaves * 64 - 1) / (kWaves * 64);  // rounds of 64 assignments, a wave's one behind the other
+    uint32_t found = 0;
+    for (int o = 0; o < each; ++o) {
+      const int i = (wave * each + o) * 64 + lane;
+      found += (uint32_t)__builtin_popcountll(__ballot(i < n && expert[i < n ? i : 0] == mine));
+    }
+    if (lane == 0) counts.waves[wave] = found;
+    __syncthreads();
+    uint32_t at = 0;
+    for (int w = 0; w < wave; ++w) at += counts.waves[w];
+    for (int o = 0; o < each; ++o) {
+      const int i = (wave * each + o) * 64 + lane;
+      const bool here = i < n && expert[i < n ? i : 0] == mine;
+      const uint64_t m = __ballot(here);
+      if (here) list[at + (uint32_t)__builtin_popcountll(m & ((1ull << lane) - 1))] = (uint16_t)i;
+      at += (uint32_t)__builtin_popcountll(m);
+    }
+    __syncthreads();
+    return true;
+  }
+};
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // ---------------------------------------------------------------------------------------------
 // Products of 16 weight rows with 16 tokens
 // ---------------------------------------------------------------------------------------------
-// In a step of 128 of K a lane has row (or token) lane % 16 and the 32 neighbours from 32 (lane / 16) on; both
-// operands take the same ones, so that their order in a product does not matter.
+// In a step of 128 of K a lane has row (or token) lane % 16 and of it four times 8 elements, the q-th from
+// k_of(q, lane / 16) on: words of 16 bytes, so that the four lanes of a row load 64 adjacent bytes at once.  Both operands
+// take the same elements, so their order in a product does not matter.
+template <bool FP8>
+__device__ __forceinline__ constexpr int k_of(int q, int g) {
+  return FP8 ? (q >> 1) * 64 + g * 16 + (q & 1) * 8 : q * 32 + g * 8;
+}
 template <bool FP8, int M>
 struct Weights {
-  static constexpr int kWords = FP8 ? 2 : 4;   // of 16 bytes
-  static constexpr int kEach = FP8 ? 16 : 8;   // elements of one
+  static constexpr int kWords = FP8 ? 2 : 4;  // of 16 bytes
   u4 w[M][kWords];
   float scale[FP8 ? M : 1];
-  // step b of 16 rows[m] from this lane's offset on, scaled by scales[m]; left: elements of K from there on
+  // step b of 16 rows[m] from this lane's offset on, scaled by scales[m]
   __device__ __forceinline__ void load(const __amdgpu_buffer_rsrc_t (&rows)[M], uint32_t mine, const floats_at (&scales)[M], int b,
-                                       int left) {
+                                       int K) {
     const uint32_t off = mine + (uint32_t)b * (FP8 ? kBlock : 2 * kBlock);
-    left -= b * kBlock;
+    const int left = K - b * kBlock, g = threadIdx.x >> 4 & 3;
 #pragma unroll
     for (int j = 0; j < kWords; ++j) {
-      const uint32_t at = j * kEach < left ? off + 16 * j : kNothing;
+      const uint32_t at = k_of<FP8>(FP8 ? 2 * j : j, g) < left ? off + 64 * j : kNothing;
 #pragma unroll
       for (int m = 0; m < M; ++m) w[m][j] = load16<kStream>(rows[m], at);
     }
@@ -467,7 +485,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(const uint8_t* w, int6
 template <bool FP8>
 __device__ __forceinline__ uint32_t offset_in_rows(int K) {
   const int lane = threadIdx.x & 63;
-  return (uint32_t)((lane & 15) * K * (FP8 ? 1 : 2) + (lane >> 4) * (FP8 ? 32 : 64));
+  return (uint32_t)((lane & 15) * K * (FP8 ? 1 : 2) + (lane >> 4) * 16);
 }
 __device__ __forceinline__ floats_at scales_at(const float* s, int64_t expert, int64_t row, int rows, int K) {
   return (floats_at)(uintptr_t)s + (expert * ((rows + kBlock - 1) / kBlock) + row / kBlock) * ((K + kBlock - 1) / kBlock);
@@ -512,15 +530,16 @@ __device__ __forceinline__ void store_h(uint16_t* to, int64_t plane, f4 h1, f4 h
 // ---------------------------------------------------------------------------------------------
 // Up to 16 tokens
 // ---------------------------------------------------------------------------------------------
-template <int P>
+template <bool FP8, int P>
 struct Tokens {
   u4 b[P][4];
-  // step's part of this lane's token, which begins at `mine` of parts[p] (kNothing for none)
-  __device__ __forceinline__ void load(const __amdgpu_buffer_rsrc_t (&parts)[P], uint32_t mine, int step, int left) {
-    left -= step * kBlock;
+  // a step of this lane's token, which begins at `token` of parts[p] (kNothing for none)
+  __device__ __forceinline__ void load(const __amdgpu_buffer_rsrc_t (&parts)[P], uint32_t token, int step, int K) {
+    const int left = K - step * kBlock, g = threadIdx.x >> 4 & 3;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const uint32_t at = q * 8 < left ? mine + (uint32_t)step * 2 * kBlock + 16 * q : kNothing;
+      const int k = k_of<FP8>(q, g);
+      const uint32_t at = k < left ? token + (uint32_t)(step * kBlock + k) * 2 : kNothing;
 #pragma unroll
       for (int p = 0; p < P; ++p) b[p][q] = load16(parts[p], at);
     }
@@ -528,7 +547,7 @@ struct Tokens {
 };
 
 template <bool FP8, int M, int P>
-__device__ __forceinline__ void multiply(f4 (&acc)[M][1], const Weights<FP8, M>& w, const Tokens<P>& x) {
+__device__ __forceinline__ void multiply(f4 (&acc)[M][1], const Weights<FP8, M>& w, const Tokens<FP8, P>& x) {
   f4 sum[M][1];
   if constexpr (FP8) clear<FP8, M, 1>(sum);
 #pragma unroll
@@ -552,23 +571,22 @@ __device__ __forceinline__ void sum_steps(f4 (&acc)[M][1], const __amdgpu_buffer
                                           const __amdgpu_buffer_rsrc_t (&parts)[P], uint32_t token, int K, int first, int end,
                                           int step) {
   if (first >= end) return;
-  const int left = K - (threadIdx.x >> 4 & 3) * 32;
   const uint32_t mine = offset_in_rows<FP8>(K);
   Weights<FP8, M> w, next;
-  Tokens<P> x, ahead;
-  w.load(rows, mine, scales, first, left);
-  x.load(parts, token, first, left);
+  Tokens<FP8, P> x, ahead;
+  w.load(rows, mine, scales, first, K);
+  x.load(parts, token, first, K);
   for (int b = first; b < end; b += 2 * step) {
     const int b1 = b + step, b2 = b1 + step;
     if (b1 < end) {
-      next.load(rows, mine, scales, b1, left);
-      ahead.load(parts, token, b1, left);
+      next.load(rows, mine, scales, b1, K);
+      ahead.load(parts, token, b1, K);
     }
     multiply<FP8, M, P>(acc, w, x);
     if (b1 >= end) break;
     if (b2 < end) {
-      w.load(rows, mine, scales, b2, left);
-      x.load(parts, token, b2, left);
+      w.load(rows, mine, scales, b2, K);
+      x.load(parts, token, b2, K);
     }
     multiply<FP8, M, P>(acc, next, ahead);
   }
@@ -577,7 +595,7 @@ __device__ __forceinline__ void sum_steps(f4 (&acc)[M][1], const __amdgpu_buffer
 template <int DT, bool FP8>
 __global__ __launch_bounds__(64 * kUpWaves) void k_up_few(LayerArgs a) {
   constexpr int P = kXParts<DT>;
-  __shared__ Plan plan;
+  __shared__ OneUnit<kFewTokens, kFewTokens * kMaxTopK> plan;
   __shared__ f4 sum[kUpWaves][2][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
   const int tiles = a.experts.H / 16, routed = a.units * tiles;
@@ -586,11 +604,9 @@ __global__ __launch_bounds__(64 * kUpWaves) void k_up_few(LayerArgs a) {
   if (!shared) {
     const int u = blockIdx.x / tiles;
     tile = blockIdx.x - u * tiles;
-    make_plan<64 * kUpWaves, kFewTokens, false>(plan, a.idx, a.T * a.k, a.E);
-    if (u >= plan.units) return;
-    expert = uniform((int)(plan.unit[u] >> 16));
-    n = uniform(plan.tokens[u]);
-    list_of<64 * kUpWaves>(plan, a.T * a.k, expert);
+    if (!plan.make<64 * kUpWaves>(a.idx, a.T * a.k, a.E, u)) return;
+    expert = uniform((int)(plan.counts.unit[0] >> 16));
+    n = uniform(plan.counts.tokens[0]);
   }
   const int H = shared ? a.shared.H : a.experts.H, h0 = tile * 16, KB = (a.D + kBlock - 1) / kBlock;
   const uint8_t* w12 = shared ? a.shared.w12 : a.experts.w12;
@@ -606,7 +622,7 @@ __global__ __launch_bounds__(64 * kUpWaves) void k_up_few(LayerArgs a) {
 #pragma unroll
   for (int p = 0; p < P; ++p) parts[p] = make_rsrc(a.xb + p * plane, 2 * plane);
   const int at = r < n ? (shared ? r : plan.list[r]) : 0;
-  const uint32_t token = r < n ? (uint32_t)((shared ? at : at / a.k) * a.Dp + g * 32) * 2 : kNothing;
+  const uint32_t token = r < n ? (uint32_t)((shared ? at : at / a.k) * a.Dp) * 2 : kNothing;
   f4 acc[2][1];
   clear<FP8, 2, 1>(acc);
   sum_steps<FP8, 2, P>(acc, rows, scales, parts, token, a.D, uniform(wave), KB, kUpWaves);
@@ -633,11 +649,11 @@ __global__ __launch_bounds__(64 * kDownWaves) void k_down_few(LayerArgs a) {
   __shared__ f4 sums[kDownWaves][kFewTokens][kSumPitch / 4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
   const int d0 = blockIdx.x * 16;
-  make_plan<64 * kDownWaves, kFewTokens, true>(plan, a.idx, a.T * a.k, a.E);
+  plan.make<64 * kDownWaves>(a.idx, a.T * a.k, a.E);
   for (int t = g; t < a.T; t += 4)
     if (r < kSumPitch / 4) sums[wave][t][r] = f4{0.0f, 0.0f, 0.0f, 0.0f};
   // the waves share the steps of all units, the shared expert's behind the others'
-  const int KB = (a.experts.H + kBlock - 1) / kBlock, routed = uniform(plan.units) * KB;
+  const int KB = (a.experts.H + kBlock - 1) / kBlock, routed = uniform(plan.counts.units) * KB;
   const int all = routed + (a.shared.H + kBlock - 1) / kBlock;
   int at = uniform(all * wave / kDownWaves);
   const int end = uniform(all * (wave + 1) / kDownWaves);
@@ -645,8 +661,8 @@ __global__ __launch_bounds__(64 * kDownWaves) void k_down_few(LayerArgs a) {
     const bool shared = at >= routed;
     const int u = shared ? 0 : at / KB, kb0 = shared ? at - routed : at - u * KB;
     const int kb1 = shared ? kb0 + end - at : min(KB, kb0 + end - at);
-    const int expert = shared ? 0 : uniform((int)(plan.unit[u] >> 16)), first = shared ? 0 : uniform((int)(plan.unit[u] & 0xffffu));
-    const int n = shared ? a.T : uniform(plan.tokens[u]), H = shared ? a.shared.H : a.experts.H;
+    const int expert = shared ? 0 : uniform((int)(plan.counts.unit[u] >> 16)), first = shared ? 0 : uniform((int)(plan.counts.unit[u] & 0xffffu));
+    const int n = shared ? a.T : uniform(plan.counts.tokens[u]), H = shared ? a.shared.H : a.experts.H;
     const __amdgpu_buffer_rsrc_t rows[1] = {rows_at<FP8>(shared ? a.shared.w3 : a.experts.w3, (int64_t)expert * a.D + d0, H)};
     const floats_at scales[1] = {scales_at(shared ? a.shared.s3 : a.experts.s3, expert, d0, a.D, H)};
     __amdgpu_buffer_rsrc_t parts[P];
@@ -654,7 +670,7 @@ __global__ __launch_bounds__(64 * kDownWaves) void k_down_few(LayerArgs a) {
 #pragma unroll
     for (int p = 0; p < P; ++p) parts[p] = make_rsrc((shared ? a.hs : a.hb) + p * plane, 2 * plane);
     const int row = r < n ? (shared ? r : plan.list[first + r]) : 0;
-    const uint32_t token = r < n ? (uint32_t)(row * H + g * 32) * 2 : kNothing;
+    const uint32_t token = r < n ? (uint32_t)(row * H) * 2 : kNothing;
     f4 acc[1][1];
     clear<FP8, 1, 1>(acc);
     sum_steps<FP8, 1, P>(acc, rows, scales, parts, token, H, kb0, kb1, 1);
@@ -685,8 +701,10 @@ constexpr int kTokenPitch = kBlock + 8;  // elements of a token's step in LDS: 1
 template <bool UP>
 constexpr int kTileRows = kTileWaves * (UP ? 16 : 32);
 
+using TilePlan = OneUnit<kUnitTokens, kMaxAssigned>;
+
 template <int DT, bool FP8, bool UP, int NC>
-__device__ __forceinline__ void tile_unit(const LayerArgs& a, const Plan& plan, uint16_t* lds, int expert, int tile, int first, int n,
+__device__ __forceinline__ void tile_unit(const LayerArgs& a, const TilePlan& plan, uint16_t* lds, int expert, int tile, int first, int n,
                                           bool shared) {
   constexpr int P = UP ? kXParts<DT> : kHParts<DT>;
   constexpr int kChunks = NC * 16 * P * (kBlock / 8), kThreads = 64 * kTileWaves;  // of 16 bytes, a step
@@ -736,11 +754,10 @@ __device__ __forceinline__ void tile_unit(const LayerArgs& a, const Plan& plan, 
   };
   f4 acc[2][NC];
   clear<FP8, 2, NC>(acc);
-  const int left = K - g * 32;
   Weights<FP8, 2> w, next;
   fetch(0);
   const uint32_t mine = offset_in_rows<FP8>(K);
-  w.load(rows, mine, scales, 0, left);
+  w.load(rows, mine, scales, 0, K);
   leave();
   __syncthreads();
   // one step: the next one's loads go out first (its tokens' before its weights', as loads are waited for in their order)
@@ -748,7 +765,7 @@ __device__ __forceinline__ void tile_unit(const LayerArgs& a, const Plan& plan, 
     const bool more = b + 1 < KB;
     if (more) {
       fetch(b + 1);
-      later.load(rows, mine, scales, b + 1, left);
+      later.load(rows, mine, scales, b + 1, K);
     }
     if (active) {
       f4 sum[2][NC];
@@ -760,7 +777,7 @@ __device__ __forceinline__ void tile_unit(const LayerArgs& a, const Plan& plan, 
         for (int c = 0; c < NC; ++c)
 #pragma unroll
           for (int p = P - 1; p >= 0; --p) {
-            const bf8 x = *reinterpret_cast<const bf8*>(lds + (p * NC * 16 + c * 16 + r) * kTokenPitch + g * 32 + q * 8);
+            const bf8 x = *reinterpret_cast<const bf8*>(lds + (p * NC * 16 + c * 16 + r) * kTokenPitch + k_of<FP8>(q, g));
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
               f4& s = FP8 ? sum[m][c] : acc[m][c];
@@ -799,7 +816,7 @@ __device__ __forceinline__ void tile_unit(const LayerArgs& a, const Plan& plan, 
 template <int DT, bool FP8, bool UP>
 __global__ __launch_bounds__(64 * kTileWaves, 4) void k_products(LayerArgs a) {
   constexpr int UNIT = kUnitTokens, ROWS = kTileRows<UP>;
-  __shared__ Plan plan;
+  __shared__ TilePlan plan;
   extern __shared__ u4 tokens[];  // [parts, columns][kTokenPitch] of 16 bits
   const int tiles = ((UP ? a.experts.H : a.D) + ROWS - 1) / ROWS, routed = a.units * tiles;
   const bool shared = (int)blockIdx.x >= routed;
@@ -807,12 +824,10 @@ __global__ __launch_bounds__(64 * kTileWaves, 4) void k_products(LayerArgs a) {
   if (!shared) {
     tile = blockIdx.x / a.units;
     const int u = blockIdx.x - tile * a.units;
-    make_plan<64 * kTileWaves, UNIT, false>(plan, a.idx, a.T * a.k, a.E);
-    if (u >= plan.units) return;
-    expert = uniform((int)(plan.unit[u] >> 16));
-    first = uniform((int)(plan.unit[u] & 0xffffu));
-    n = uniform(plan.tokens[u]);
-    list_of<64 * kTileWaves>(plan, a.T * a.k, expert);
+    if (!plan.make<64 * kTileWaves>(a.idx, a.T * a.k, a.E, u)) return;
+    expert = uniform((int)(plan.counts.unit[0] >> 16));
+    first = uniform((int)(plan.counts.unit[0] & 0xffffu));
+    n = uniform(plan.counts.tokens[0]);
   } else {
     const int i = blockIdx.x - routed, units = (a.T + UNIT - 1) / UNIT;
     tile = i / units;
