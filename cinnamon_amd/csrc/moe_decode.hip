@@ -433,33 +433,53 @@ __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirs
 // ---------------------------------------------------------------------------------------------
 // Products of 16 weight rows with 16 tokens
 // ---------------------------------------------------------------------------------------------
-// In a step of 128 of K a lane has row (or token) lane % 16 and of it four times 8 elements, the q-th from
-// k_of(q, lane / 16) on: words of 16 bytes, so that the four lanes of a row load 64 adjacent bytes at once.  Both operands
-// take the same elements, so their order in a product does not matter.
+// In a step of 128 of K a lane multiplies row (or token) lane % 16, and of it four times 8 elements, the q-th from
+// k_of(q, lane / 16) on.  Both operands take the same elements, so their order in a product does not matter.
+//
+// A load takes 8 rows' 128 adjacent bytes (lane: row lane % 8, 16 bytes from 16 (lane / 8) on), a whole line of each,
+// streamed past the caches: 969 MB of codes in rows of 7168 arrive at 6.2 TB/s, against 4.8 with 64 bytes of 16 rows a load
+// and 5.5 with those kept in the caches (linear reads: 7.0).  Two loads, of rows 0-7 and 8-15, then hold every lane's
+// two words, half of them in the lane 8 further in its row of 16: settle() swaps those.
 template <bool FP8>
 __device__ __forceinline__ constexpr int k_of(int q, int g) {
-  return FP8 ? (q >> 1) * 64 + g * 16 + (q & 1) * 8 : q * 32 + g * 8;
+  return FP8 ? g * 32 + q * 8 : (q >> 1) * 64 + g * 16 + (q & 1) * 8;
 }
 template <bool FP8, int M>
 struct Weights {
   static constexpr int kWords = FP8 ? 2 : 4;  // of 16 bytes
   u4 w[M][kWords];
   float scale[FP8 ? M : 1];
-  // step b of 16 rows[m] from this lane's offset on, scaled by scales[m]
-  __device__ __forceinline__ void load(const __amdgpu_buffer_rsrc_t (&rows)[M], uint32_t mine, const floats_at (&scales)[M], int b,
+  // step b of 8 rows[m][i] from this lane's offset on, scaled by scales[m]
+  __device__ __forceinline__ void load(const __amdgpu_buffer_rsrc_t (&rows)[M][2], uint32_t mine, const floats_at (&scales)[M], int b,
                                        int K) {
     const uint32_t off = mine + (uint32_t)b * (FP8 ? kBlock : 2 * kBlock);
-    const int left = K - b * kBlock, g = threadIdx.x >> 4 & 3;
+    const int left = K - b * kBlock, c = threadIdx.x >> 3 & 7;
 #pragma unroll
-    for (int j = 0; j < kWords; ++j) {
-      const uint32_t at = k_of<FP8>(FP8 ? 2 * j : j, g) < left ? off + 64 * j : kNothing;
+    for (int j = 0; j < kWords / 2; ++j) {
+      const uint32_t at = (FP8 ? c * 16 : j * 64 + c * 8) < left ? off + 128 * j : kNothing;
 #pragma unroll
-      for (int m = 0; m < M; ++m) w[m][j] = load16<kStream>(rows[m], at);
+      for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) w[m][2 * j + i] = load16<kStream>(rows[m][i], at);
     }
     if constexpr (FP8) {
 #pragma unroll
-      for (int m = 0; m < M; ++m) scale[m] = scales[m][b];
+      for (int m = 0; m < M; ++m) scale[m] = scales[m][left > 0 ? b : 0];  // (past the end: any)
     }
+  }
+  // from the loads' order to the lanes' rows: lanes 0-7 of 16 keep the first load's word and take the other's from
+  // 8 lanes on, lanes 8-15 the other way round
+  __device__ __forceinline__ void settle() {
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+      for (int j = 0; j < kWords; j += 2)
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          const int a = (int)w[m][j][d], b = (int)w[m][j + 1][d];
+          w[m][j][d] = (uint32_t)__builtin_amdgcn_update_dpp(a, b, 0x128, 0xF, 0xC, false);      // row_ror:8
+          w[m][j + 1][d] = (uint32_t)__builtin_amdgcn_update_dpp(b, a, 0x128, 0xF, 0x3, false);
+        }
   }
   // the q-th 8 elements of row m as bf16
   __device__ __forceinline__ bf8 frag(int m, int q) const {
@@ -476,16 +496,17 @@ struct Weights {
   }
 };
 
-// 16 rows of an expert's stacked weights from `row` on, a lane's offset into them, and their blocks' scales.
+// 16 rows of an expert's stacked weights from `row` on, a lane's offset into their halves, and their blocks' scales.
 template <bool FP8>
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(const uint8_t* w, int64_t row, int K) {
+__device__ __forceinline__ void rows_at(__amdgpu_buffer_rsrc_t (&rows)[2], const uint8_t* w, int64_t row, int K) {
   const int64_t pitch = (int64_t)K * (FP8 ? 1 : 2);
-  return make_rsrc(w + row * pitch, 16 * pitch);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) rows[i] = make_rsrc(w + (row + 8 * i) * pitch, 8 * pitch);
 }
 template <bool FP8>
 __device__ __forceinline__ uint32_t offset_in_rows(int K) {
   const int lane = threadIdx.x & 63;
-  return (uint32_t)((lane & 15) * K * (FP8 ? 1 : 2) + (lane >> 4) * 16);
+  return (uint32_t)((lane & 7) * K * (FP8 ? 1 : 2) + (lane >> 3) * 16);
 }
 __device__ __forceinline__ floats_at scales_at(const float* s, int64_t expert, int64_t row, int rows, int K) {
   return (floats_at)(uintptr_t)s + (expert * ((rows + kBlock - 1) / kBlock) + row / kBlock) * ((K + kBlock - 1) / kBlock);
@@ -547,7 +568,8 @@ struct Tokens {
 };
 
 template <bool FP8, int M, int P>
-__device__ __forceinline__ void multiply(f4 (&acc)[M][1], const Weights<FP8, M>& w, const Tokens<FP8, P>& x) {
+__device__ __forceinline__ void multiply(f4 (&acc)[M][1], Weights<FP8, M>& w, const Tokens<FP8, P>& x) {
+  w.settle();
   f4 sum[M][1];
   if constexpr (FP8) clear<FP8, M, 1>(sum);
 #pragma unroll
@@ -567,8 +589,8 @@ __device__ __forceinline__ void multiply(f4 (&acc)[M][1], const Weights<FP8, M>&
 // acc += rows[.., steps first : end : step of K] times the tokens; the loads of the next step go out before a step's
 // products.
 template <bool FP8, int M, int P>
-__device__ __forceinline__ void sum_steps(f4 (&acc)[M][1], const __amdgpu_buffer_rsrc_t (&rows)[M], const floats_at (&scales)[M],
-                                          const __amdgpu_buffer_rsrc_t (&parts)[P], uint32_t token, int K, int first, int end,
+__device__ __forceinline__ void sum_steps(f4 (&acc)[M][1], const __amdgpu_buffer_rsrc_t (&rows)[M][2],
+                                          const floats_at (&scales)[M], const __amdgpu_buffer_rsrc_t (&parts)[P], uint32_t token, int K, int first, int end,
                                           int step) {
   if (first >= end) return;
   const uint32_t mine = offset_in_rows<FP8>(K);
@@ -611,11 +633,11 @@ __global__ __launch_bounds__(64 * kUpWaves) void k_up_few(LayerArgs a) {
   const int H = shared ? a.shared.H : a.experts.H, h0 = tile * 16, KB = (a.D + kBlock - 1) / kBlock;
   const uint8_t* w12 = shared ? a.shared.w12 : a.experts.w12;
   const float* s12 = shared ? a.shared.s12 : a.experts.s12;
-  __amdgpu_buffer_rsrc_t rows[2], parts[P];
+  __amdgpu_buffer_rsrc_t rows[2][2], parts[P];
   floats_at scales[2];
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
-    rows[m] = rows_at<FP8>(w12, (int64_t)expert * 2 * H + m * H + h0, a.D);
+    rows_at<FP8>(rows[m], w12, (int64_t)expert * 2 * H + m * H + h0, a.D);
     scales[m] = scales_at(s12, expert, m * H + h0, 2 * H, a.D);
   }
   const int64_t plane = (int64_t)a.T * a.Dp;
@@ -663,7 +685,8 @@ __global__ __launch_bounds__(64 * kDownWaves) void k_down_few(LayerArgs a) {
     const int kb1 = shared ? kb0 + end - at : min(KB, kb0 + end - at);
     const int expert = shared ? 0 : uniform((int)(plan.counts.unit[u] >> 16)), first = shared ? 0 : uniform((int)(plan.counts.unit[u] & 0xffffu));
     const int n = shared ? a.T : uniform(plan.counts.tokens[u]), H = shared ? a.shared.H : a.experts.H;
-    const __amdgpu_buffer_rsrc_t rows[1] = {rows_at<FP8>(shared ? a.shared.w3 : a.experts.w3, (int64_t)expert * a.D + d0, H)};
+    __amdgpu_buffer_rsrc_t rows[1][2];
+    rows_at<FP8>(rows[0], shared ? a.shared.w3 : a.experts.w3, (int64_t)expert * a.D + d0, H);
     const floats_at scales[1] = {scales_at(shared ? a.shared.s3 : a.experts.s3, expert, d0, a.D, H)};
     __amdgpu_buffer_rsrc_t parts[P];
     const int64_t plane = (int64_t)(shared ? a.T : a.T * a.k) * H;
@@ -697,6 +720,10 @@ __global__ __launch_bounds__(64 * kDownWaves) void k_down_few(LayerArgs a) {
 // ---------------------------------------------------------------------------------------------
 constexpr int kTokenPitch = kBlock + 8;  // elements of a token's step in LDS: 16 lanes' 16 bytes on all banks
 
+// Elements of a step's parts in LDS.
+template <int P, int NC>
+constexpr int kTokenStep = P * NC * 16 * kTokenPitch;
+
 // Rows of a workgroup: 16 hidden channels (of W1 and W2 each) a wave, or 32 output channels.
 template <bool UP>
 constexpr int kTileRows = kTileWaves * (UP ? 16 : 32);
@@ -714,7 +741,7 @@ __device__ __forceinline__ void tile_unit(const LayerArgs& a, const TilePlan& pl
   const int row0 = tile * kTileRows<UP> + wave * (UP ? 16 : 32), rows_all = UP ? H : a.D;
   const bool active = row0 < rows_all, both = UP || row0 + 16 < rows_all;
   // this lane's weight rows; those past the end are the first ones again and not stored
-  __amdgpu_buffer_rsrc_t rows[2];
+  __amdgpu_buffer_rsrc_t rows[2][2];
   floats_at scales[2];
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
@@ -722,7 +749,7 @@ __device__ __forceinline__ void tile_unit(const LayerArgs& a, const TilePlan& pl
     const uint8_t* w = UP ? (shared ? a.shared.w12 : a.experts.w12) : (shared ? a.shared.w3 : a.experts.w3);
     const float* s = UP ? (shared ? a.shared.s12 : a.experts.s12) : (shared ? a.shared.s3 : a.experts.s3);
     const int stacked = UP ? 2 * H : a.D;
-    rows[m] = rows_at<FP8>(w, (int64_t)expert * stacked + row, K);
+    rows_at<FP8>(rows[m], w, (int64_t)expert * stacked + row, K);
     scales[m] = scales_at(s, expert, row, stacked, K);
   }
   // this thread's 16 bytes of the tokens' parts (of all of them at most 128 x 16 x 65536 x 3 x 2 bytes)
@@ -740,34 +767,37 @@ __device__ __forceinline__ void tile_unit(const LayerArgs& a, const TilePlan& pl
       from[o] = (uint32_t)(2 * (p * plane + (int64_t)(UP && !shared ? at / a.k : at) * pitch + chunk * 8));
     }
   }
-  u4 part[kOwn];
   const int end = pitch - (int)(threadIdx.x & 15) * 8;
-  auto fetch = [&](int b) {
+  auto fetch = [&](u4 (&part)[kOwn], int b) {
     const bool there = b * kBlock < end;
 #pragma unroll
     for (int o = 0; o < kOwn; ++o) part[o] = load16(parts, there ? from[o] + (uint32_t)b * 2 * kBlock : kNothing);
   };
-  auto leave = [&]() {
+  auto leave = [&](const u4 (&part)[kOwn], int b) {
+    uint16_t* tile_b = lds + (b & 1) * kTokenStep<P, NC>;
 #pragma unroll
     for (int o = 0; o < kOwn; ++o)
-      if (kChunks % kThreads == 0 || threadIdx.x + o * kThreads < kChunks) *reinterpret_cast<u4*>(lds + to[o]) = part[o];
+      if (kChunks % kThreads == 0 || threadIdx.x + o * kThreads < kChunks) *reinterpret_cast<u4*>(tile_b + to[o]) = part[o];
   };
   f4 acc[2][NC];
   clear<FP8, 2, NC>(acc);
-  Weights<FP8, 2> w, next;
-  fetch(0);
   const uint32_t mine = offset_in_rows<FP8>(K);
-  w.load(rows, mine, scales, 0, K);
-  leave();
+  // Two steps' loads are on their way while one is multiplied, a step's tokens before its weights, as loads are waited
+  // for in their order; the tokens' parts of two steps lie in LDS, so that a step has one barrier.
+  Weights<FP8, 2> w[3];
+  u4 part[2][kOwn];
+  fetch(part[0], 0);
+  w[0].load(rows, mine, scales, 0, K);
+  fetch(part[1], 1);  // (past the end: zeros)
+  w[1].load(rows, mine, scales, 1, K);
+  leave(part[0], 0);
   __syncthreads();
-  // one step: the next one's loads go out first (its tokens' before its weights', as loads are waited for in their order)
-  auto one_step = [&](int b, const Weights<FP8, 2>& now, Weights<FP8, 2>& later) {
-    const bool more = b + 1 < KB;
-    if (more) {
-      fetch(b + 1);
-      later.load(rows, mine, scales, b + 1, K);
-    }
+  auto one_step = [&](int b, Weights<FP8, 2>& now, Weights<FP8, 2>& later, const u4 (&next)[kOwn], u4 (&after)[kOwn]) {
+    fetch(after, b + 2);
+    later.load(rows, mine, scales, b + 2, K);
     if (active) {
+      now.settle();
+      const uint16_t* tile_b = lds + (b & 1) * kTokenStep<P, NC>;
       f4 sum[2][NC];
       if constexpr (FP8) clear<FP8, 2, NC>(sum);
 #pragma unroll
@@ -777,7 +807,7 @@ __device__ __forceinline__ void tile_unit(const LayerArgs& a, const TilePlan& pl
         for (int c = 0; c < NC; ++c)
 #pragma unroll
           for (int p = P - 1; p >= 0; --p) {
-            const bf8 x = *reinterpret_cast<const bf8*>(lds + (p * NC * 16 + c * 16 + r) * kTokenPitch + k_of<FP8>(q, g));
+            const bf8 x = *reinterpret_cast<const bf8*>(tile_b + (p * NC * 16 + c * 16 + r) * kTokenPitch + k_of<FP8>(q, g));
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
               f4& s = FP8 ? sum[m][c] : acc[m][c];
@@ -787,13 +817,21 @@ __device__ __forceinline__ void tile_unit(const LayerArgs& a, const TilePlan& pl
       }
       if constexpr (FP8) join_step<FP8, 2, NC>(acc, sum, now);
     }
-    __syncthreads();
-    if (more) leave();
+    leave(next, b + 1);
     __syncthreads();
   };
-  for (int b = 0; b < KB; b += 2) {
-    one_step(b, w, next);
-    if (b + 1 < KB) one_step(b + 1, next, w);
+  for (int b = 0; b < KB; b += 6) {
+    one_step(b, w[0], w[2], part[1], part[0]);
+    if (b + 1 >= KB) break;
+    one_step(b + 1, w[1], w[0], part[0], part[1]);
+    if (b + 2 >= KB) break;
+    one_step(b + 2, w[2], w[1], part[1], part[0]);
+    if (b + 3 >= KB) break;
+    one_step(b + 3, w[0], w[2], part[0], part[1]);
+    if (b + 4 >= KB) break;
+    one_step(b + 4, w[1], w[0], part[1], part[0]);
+    if (b + 5 >= KB) break;
+    one_step(b + 5, w[2], w[1], part[0], part[1]);
   }
   if (!active) return;
 #pragma unroll
@@ -814,7 +852,7 @@ __device__ __forceinline__ void tile_unit(const LayerArgs& a, const TilePlan& pl
 
 // The units of a tile are neighbours: those of one expert read its weights at the same time, from the cache.
 template <int DT, bool FP8, bool UP>
-__global__ __launch_bounds__(64 * kTileWaves, 4) void k_products(LayerArgs a) {
+__global__ __launch_bounds__(64 * kTileWaves, !FP8 || DT == CIN_DT_F32 ? 2 : UP && DT == CIN_DT_BF16 ? 4 : 3) void k_products(LayerArgs a) {
   constexpr int UNIT = kUnitTokens, ROWS = kTileRows<UP>;
   __shared__ TilePlan plan;
   extern __shared__ u4 tokens[];  // [parts, columns][kTokenPitch] of 16 bits
@@ -908,7 +946,7 @@ void launch_products(const LayerArgs& a, hipStream_t stream) {
   constexpr int P = UP ? kXParts<DT> : kHParts<DT>, ROWS = kTileRows<UP>, UNIT = kUnitTokens;
   const int per = ((UP ? a.experts.H : a.D) + ROWS - 1) / ROWS;
   const int shared = a.shared.H ? ((UP ? a.shared.H : a.D) + ROWS - 1) / ROWS * ((a.T + UNIT - 1) / UNIT) : 0;
-  const size_t lds = 2 * P * UNIT * kTokenPitch;
+  const size_t lds = 2 * sizeof(uint16_t) * kTokenStep<P, UNIT / 16>;
   hipLaunchKernelGGL((k_products<DT, FP8, UP>), dim3(a.units * per + shared), dim3(64 * kTileWaves), lds, stream, a);
 }
 
