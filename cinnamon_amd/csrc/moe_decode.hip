@@ -16,14 +16,12 @@
 // large as the output's own rounding.  All sums are fp32.  Logits and the gate are in 64 bits: choices next to
 // the border of the top k differ by less than 32 bits hold.
 //
-// Launches: k_router (logits by slices of D on the fp64 matrix units, and x's parts), k_gate (a workgroup a token), then
-//   up to 16 tokens: k_up_few (a workgroup an expert and 16 of its hidden channels, the waves sharing D) and
-//   k_down_few (a workgroup 16 output channels, the waves sharing the chosen experts' hidden channels; each
-//   wave's sums per token lie in LDS and are joined in a fixed order): with so few columns a product the work is
-//   the weights', and each is spread over the whole chip;
-//   more: k_products twice (a workgroup a unit of an expert's tokens and 16 or 32 rows a wave; the tokens' parts
-//   go through LDS once for all waves, as they would be more bytes than the weights), which leaves h, then
-//   each expert's output rows, and k_join (their sum per token in the order of top k).
+// Five launches: k_router (logits by slices of D on the fp64 matrix units, and x's parts), k_gate (a workgroup a
+// token), the products up to h and down to each expert's output rows, and k_join (a token's rows in the order of top
+// k).  The products take a workgroup an expert's tokens and some of its rows:
+//   k_few, up to 16 tokens and where the others would leave CUs idle: 16 rows of W1 and W2, or 32 of W3, the waves sharing K;
+//   k_products: as many rows a wave; the tokens' parts go through LDS once for all waves, as they
+//   would be more bytes than the weights.
 // No atomics on results.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -45,7 +43,7 @@ constexpr int kBlock = 128;        // of a scale, and a step of K
 constexpr int kMaxAssigned = kMaxTokens * kMaxTopK;
 constexpr int kUnitTokens = 32;    // of an expert, multiplied at once
 constexpr int kRouterSlice = 512;  // channels of a k_router workgroup
-constexpr int kUpWaves = 4, kDownWaves = 8, kTileWaves = 4;
+constexpr int kFewWaves = 4, kTileWaves = 4;
 constexpr int kFewTokens = 16;
 
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
@@ -84,7 +82,7 @@ struct LayerArgs {
   double* logits;  // [slices, T, E]
   int slices;
   uint16_t *xb, *hb, *hs;  // parts of x [P, T, Dp], of h [P, T k, H], of the shared expert's [P, T, Hs]
-  float* y;                // past kFewTokens: the experts' outputs [T k, D], the shared one's [T, D]
+  float* y;                // the experts' outputs [T k, D], the shared one's [T, D]
   int units;               // the most that the routed experts can have
 };
 
@@ -209,9 +207,14 @@ __global__ __launch_bounds__(256) void k_gate(LayerArgs a) {
     z[o] = -__builtin_inf();
     if (e < a.E) {
       const double* p = a.logits + (int64_t)t * a.E + e;
-      double s = p[0];
-#pragma unroll 8
-      for (int i = 1; i < a.slices; ++i) s += p[(int64_t)i * a.T * a.E];
+      double s = 0.0;
+      for (int i = 0; i < a.slices; i += 16) {
+        double v[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] = p[(int64_t)min(i + j, a.slices - 1) * a.T * a.E];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s += i + j < a.slices ? v[j] : 0.0;
+      }
       z[o] = s;
     }
   }
@@ -309,119 +312,85 @@ __global__ __launch_bounds__(256) void k_gate(LayerArgs a) {
 // ---------------------------------------------------------------------------------------------
 // Which expert multiplies which tokens
 // ---------------------------------------------------------------------------------------------
-// The assignments (t k + j) by expert, in units of up to UNIT of one expert.
-template <int UNITS>
-struct Counts {
-  int count[kMaxExperts];  // assignments of an expert, then where its next one goes
-  uint32_t waves[kDownWaves];
-  int units;
-  uint32_t unit[UNITS];    // expert, first entry
-  uint8_t tokens[UNITS];
-};
-
-// The units of all experts in the order of the experts, from each one's count; only unit `one` where UNITS is 1.  BASE:
-// a unit's first entry counts the assignments of the experts before, and so does count from then on.
-template <int THREADS, int UNIT, int UNITS, bool BASE>
-__device__ __forceinline__ void make_units(Counts<UNITS>& p, int E, int one) {
-  constexpr int kOwn = kMaxExperts / THREADS;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  // units (upper half) and assignments of the experts before this thread's
-  uint32_t own = 0;
-  int c[kOwn];
-#pragma unroll
-  for (int o = 0; o < kOwn; ++o) {
-    const int e = tid * kOwn + o;
-    c[o] = e < E ? p.count[e] : 0;
-    own += (uint32_t)((c[o] + UNIT - 1) / UNIT) << 16 | (uint32_t)c[o];
-  }
-  uint32_t s = own;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint32_t u = (uint32_t)__shfl_up((int)s, o);
-    if (lane >= o) s += u;
-  }
-  if (lane == 63) p.waves[wave] = s;
-  __syncthreads();
-  uint32_t at = s - own, all = 0;
-  for (int w = 0; w < THREADS / 64; ++w) {
-    if (w < wave) at += p.waves[w];
-    all += p.waves[w];
-  }
-#pragma unroll
-  for (int o = 0; o < kOwn; ++o) {
-    const int e = tid * kOwn + o;
-    if (BASE && e < E) p.count[e] = (int)(at & 0xffffu);
-    for (int i = 0; i < c[o]; i += UNIT) {
-      const int u = (int)(at >> 16);
-      if (UNITS > 1 || u == one) {
-        p.unit[UNITS > 1 ? u : 0] = (uint32_t)e << 16 | ((BASE ? at & 0xffffu : 0u) + i);
-        p.tokens[UNITS > 1 ? u : 0] = (uint8_t)min(c[o] - i, UNIT);
-      }
-      at += 1u << 16;
-    }
-    at += (uint32_t)c[o];
-  }
-  if (tid == 0) p.units = (int)(all >> 16);
-  __syncthreads();
-}
-
-template <int THREADS, class Plan>
-__device__ __forceinline__ void count_experts(Plan& p, const int64_t* idx, int n, int E) {
-  for (int e = threadIdx.x; e < E; e += THREADS) p.counts.count[e] = 0;
-  __syncthreads();
-  for (int i = threadIdx.x; i < n; i += THREADS) {
-    const int e = (int)idx[i];
-    p.expert[i] = (uint16_t)e;
-    atomicAdd(&p.counts.count[e], 1);
-  }
-  __syncthreads();
-}
-
-// All units of up to kFewTokens tokens, with the list of all assignments by expert, an expert's in the atomics' order: it
-// only decides which column of a product a token has.
-struct Plan {
-  static constexpr int kMost = kFewTokens * kMaxTopK;
-  Counts<kMost> counts;
-  uint16_t expert[kMost], list[kMost];
-  template <int THREADS>
-  __device__ __forceinline__ void make(const int64_t* idx, int n, int E) {
-    count_experts<THREADS>(*this, idx, n, E);
-    make_units<THREADS, kFewTokens, kMost, true>(counts, E, 0);
-    for (int i = threadIdx.x; i < n; i += THREADS) list[atomicAdd(&counts.count[expert[i]], 1)] = (uint16_t)i;
-    __syncthreads();
-  }
-};
-
-// One unit of UNIT tokens, with the list of its expert in increasing order: workgroups that take the expert's units each
-// find the same.
-template <int UNIT, int MOST>
+// One unit: up to UNIT tokens of one expert.  The assignments (t k + j) are counted by expert, and the experts' units
+// follow each other; the unit's list holds its expert's assignments in increasing order, so that the workgroups that take
+// the expert's units each find the same.
+template <int THREADS, int UNIT, int MOST>
 struct OneUnit {
-  Counts<1> counts;
+  int count[kMaxExperts];  // assignments of an expert
+  uint32_t waves[THREADS / 64];
+  uint32_t unit;           // expert, first entry of the list
+  int tokens;
   uint16_t expert[MOST], list[kMaxTokens];
-  // false where there is no such unit
-  template <int THREADS>
-  __device__ __forceinline__ bool make(const int64_t* idx, int n, int E, int u) {
+
+  // false where there is no unit u
+  __device__ __forceinline__ bool make(const int64_t* idx, int T, int k, int E, int u) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = T * k;
+    if (T == 1) {  // every assignment is a unit
+      if (tid == 0) {
+        unit = (uint32_t)idx[u] << 16;
+        tokens = 1;
+        list[0] = (uint16_t)u;
+      }
+      __syncthreads();
+      return true;
+    }
+    for (int e = tid; e < E; e += THREADS) count[e] = 0;
+    __syncthreads();
+    for (int i = tid; i < n; i += THREADS) {
+      const int e = (int)idx[i];
+      expert[i] = (uint16_t)e;
+      atomicAdd(&count[e], 1);
+    }
+    __syncthreads();
+    // units of the experts before this thread's
+    constexpr int kOwn = kMaxExperts / THREADS;
+    int own = 0, c[kOwn];
+#pragma unroll
+    for (int o = 0; o < kOwn; ++o) {
+      c[o] = tid * kOwn + o < E ? count[tid * kOwn + o] : 0;
+      own += (c[o] + UNIT - 1) / UNIT;
+    }
+    int s = own;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int v = __shfl_up(s, o);
+      if (lane >= o) s += v;
+    }
+    if (lane == 63) waves[wave] = (uint32_t)s;
+    __syncthreads();
+    int at = s - own, all = 0;
+    for (int w = 0; w < THREADS / 64; ++w) {
+      if (w < wave) at += (int)waves[w];
+      all += (int)waves[w];
+    }
+    if (u >= all) return false;
+#pragma unroll
+    for (int o = 0; o < kOwn; ++o)
+      for (int i = 0; i < c[o]; i += UNIT, ++at)
+        if (at == u) {
+          unit = (uint32_t)(tid * kOwn + o) << 16 | (uint32_t)i;
+          tokens = min(c[o] - i, UNIT);
+        }
+    __syncthreads();
+    const int mine = (int)(unit >> 16);
     constexpr int kWaves = THREADS / 64;
-    count_experts<THREADS>(*this, idx, n, E);
-    make_units<THREADS, UNIT, 1, false>(counts, E, u);
-    if (u >= counts.units) return false;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, mine = (int)(counts.unit[0] >> 16);
     const int each = (n + kWaves * 64 - 1) / (kWaves * 64);  // rounds of 64 assignments, a wave's one behind the other
     uint32_t found = 0;
     for (int o = 0; o < each; ++o) {
       const int i = (wave * each + o) * 64 + lane;
       found += (uint32_t)__builtin_popcountll(__ballot(i < n && expert[i < n ? i : 0] == mine));
     }
-    if (lane == 0) counts.waves[wave] = found;
+    if (lane == 0) waves[wave] = found;
     __syncthreads();
-    uint32_t at = 0;
-    for (int w = 0; w < wave; ++w) at += counts.waves[w];
+    uint32_t to = 0;
+    for (int w = 0; w < wave; ++w) to += waves[w];
     for (int o = 0; o < each; ++o) {
       const int i = (wave * each + o) * 64 + lane;
       const bool here = i < n && expert[i < n ? i : 0] == mine;
       const uint64_t m = __ballot(here);
-      if (here) list[at + (uint32_t)__builtin_popcountll(m & ((1ull << lane) - 1))] = (uint16_t)i;
-      at += (uint32_t)__builtin_popcountll(m);
+      if (here) list[to + (uint32_t)__builtin_popcountll(m & ((1ull << lane) - 1))] = (uint16_t)i;
+      to += (uint32_t)__builtin_popcountll(m);
     }
     __syncthreads();
     return true;
@@ -548,8 +517,22 @@ __device__ __forceinline__ void store_h(uint16_t* to, int64_t plane, f4 h1, f4 h
   }
 }
 
+// What a lane has of a row (an assignment's, or a shared expert's token's): four h, or four outputs of each 16 rows.
+template <int DT, bool UP>
+__device__ __forceinline__ void leave_rows(const LayerArgs& a, bool shared, int at, int row, bool both, f4 first, f4 second) {
+  if constexpr (UP) {
+    const int H = shared ? a.shared.H : a.experts.H;
+    store_h<kHParts<DT>>((shared ? a.hs : a.hb) + (int64_t)at * H + row, (int64_t)(shared ? a.T : a.T * a.k) * H, first, second,
+                         shared ? 1.0f : a.weights[at]);
+  } else {
+    float* y = a.y + (int64_t)(shared ? a.T * a.k + at : at) * a.D + row;
+    *reinterpret_cast<f4*>(y) = first;
+    if (both) *reinterpret_cast<f4*>(y + 16) = second;
+  }
+}
+
 // ---------------------------------------------------------------------------------------------
-// Up to 16 tokens
+// Few tokens
 // ---------------------------------------------------------------------------------------------
 template <bool FP8, int P>
 struct Tokens {
@@ -614,105 +597,55 @@ __device__ __forceinline__ void sum_steps(f4 (&acc)[M][1], const __amdgpu_buffer
   }
 }
 
-template <int DT, bool FP8>
-__global__ __launch_bounds__(64 * kUpWaves) void k_up_few(LayerArgs a) {
-  constexpr int P = kXParts<DT>;
-  __shared__ OneUnit<kFewTokens, kFewTokens * kMaxTopK> plan;
-  __shared__ f4 sum[kUpWaves][2][64];
+template <int DT, bool FP8, bool UP>
+__global__ __launch_bounds__(64 * kFewWaves) void k_few(LayerArgs a) {
+  constexpr int P = UP ? kXParts<DT> : kHParts<DT>, ROWS = UP ? 16 : 32;
+  __shared__ OneUnit<64 * kFewWaves, kFewTokens, kFewTokens * kMaxTopK> plan;
+  __shared__ f4 sum[kFewWaves][2][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
-  const int tiles = a.experts.H / 16, routed = a.units * tiles;
+  const int tiles = ((UP ? a.experts.H : a.D) + ROWS - 1) / ROWS, routed = a.units * tiles;
   const bool shared = (int)blockIdx.x >= routed;
   int expert = 0, tile = blockIdx.x - routed, n = a.T;
   if (!shared) {
     const int u = blockIdx.x / tiles;
     tile = blockIdx.x - u * tiles;
-    if (!plan.make<64 * kUpWaves>(a.idx, a.T * a.k, a.E, u)) return;
-    expert = uniform((int)(plan.counts.unit[0] >> 16));
-    n = uniform(plan.counts.tokens[0]);
+    if (!plan.make(a.idx, a.T, a.k, a.E, u)) return;
+    expert = uniform((int)(plan.unit >> 16));
+    n = uniform(plan.tokens);
   }
-  const int H = shared ? a.shared.H : a.experts.H, h0 = tile * 16, KB = (a.D + kBlock - 1) / kBlock;
-  const uint8_t* w12 = shared ? a.shared.w12 : a.experts.w12;
-  const float* s12 = shared ? a.shared.s12 : a.experts.s12;
+  const int H = shared ? a.shared.H : a.experts.H, K = UP ? a.D : H, KB = (K + kBlock - 1) / kBlock;
+  const int row0 = tile * ROWS, stacked = UP ? 2 * H : a.D;
+  const bool both = UP || row0 + 16 < a.D;  // else the second 16 rows are the first ones again and not stored
+  const uint8_t* w = UP ? (shared ? a.shared.w12 : a.experts.w12) : (shared ? a.shared.w3 : a.experts.w3);
+  const float* s = UP ? (shared ? a.shared.s12 : a.experts.s12) : (shared ? a.shared.s3 : a.experts.s3);
   __amdgpu_buffer_rsrc_t rows[2][2], parts[P];
   floats_at scales[2];
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
-    rows_at<FP8>(rows[m], w12, (int64_t)expert * 2 * H + m * H + h0, a.D);
-    scales[m] = scales_at(s12, expert, m * H + h0, 2 * H, a.D);
+    const int row = row0 + (UP ? m * H : m && both ? 16 : 0);
+    rows_at<FP8>(rows[m], w, (int64_t)expert * stacked + row, K);
+    scales[m] = scales_at(s, expert, row, stacked, K);
   }
-  const int64_t plane = (int64_t)a.T * a.Dp;
+  const int pitch = UP ? a.Dp : H;
+  const int64_t plane = (int64_t)(UP || shared ? a.T : a.T * a.k) * pitch;
 #pragma unroll
-  for (int p = 0; p < P; ++p) parts[p] = make_rsrc(a.xb + p * plane, 2 * plane);
+  for (int p = 0; p < P; ++p) parts[p] = make_rsrc((UP ? a.xb : shared ? a.hs : a.hb) + p * plane, 2 * plane);
   const int at = r < n ? (shared ? r : plan.list[r]) : 0;
-  const uint32_t token = r < n ? (uint32_t)((shared ? at : at / a.k) * a.Dp) * 2 : kNothing;
+  const uint32_t token = r < n ? (uint32_t)(UP && !shared ? at / a.k : at) * (uint32_t)pitch * 2 : kNothing;
   f4 acc[2][1];
   clear<FP8, 2, 1>(acc);
-  sum_steps<FP8, 2, P>(acc, rows, scales, parts, token, a.D, uniform(wave), KB, kUpWaves);
+  sum_steps<FP8, 2, P>(acc, rows, scales, parts, token, K, uniform(wave), KB, kFewWaves);
 #pragma unroll
   for (int m = 0; m < 2; ++m) sum[wave][m][lane] = acc[m][0];
   __syncthreads();
   if (wave > 0 || r >= n) return;
-  f4 h1 = sum[0][0][lane], h2 = sum[0][1][lane];
+  f4 v[2] = {sum[0][0][lane], sum[0][1][lane]};
 #pragma unroll
-  for (int v = 1; v < kUpWaves; ++v) {
-    h1 += sum[v][0][lane];
-    h2 += sum[v][1][lane];
+  for (int i = 1; i < kFewWaves; ++i) {
+    v[0] += sum[i][0][lane];
+    v[1] += sum[i][1][lane];
   }
-  store_h<kHParts<DT>>((shared ? a.hs : a.hb) + (int64_t)at * H + h0 + 4 * g, (int64_t)(shared ? a.T : a.T * a.k) * H, h1, h2,
-                       shared ? 1.0f : a.weights[at]);
-}
-
-constexpr int kSumPitch = 20;  // floats of a token's 16 sums in LDS
-
-template <int DT, bool FP8>
-__global__ __launch_bounds__(64 * kDownWaves) void k_down_few(LayerArgs a) {
-  constexpr int P = kHParts<DT>;
-  __shared__ Plan plan;
-  __shared__ f4 sums[kDownWaves][kFewTokens][kSumPitch / 4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
-  const int d0 = blockIdx.x * 16;
-  plan.make<64 * kDownWaves>(a.idx, a.T * a.k, a.E);
-  for (int t = g; t < a.T; t += 4)
-    if (r < kSumPitch / 4) sums[wave][t][r] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-  // the waves share the steps of all units, the shared expert's behind the others'
-  const int KB = (a.experts.H + kBlock - 1) / kBlock, routed = uniform(plan.counts.units) * KB;
-  const int all = routed + (a.shared.H + kBlock - 1) / kBlock;
-  int at = uniform(all * wave / kDownWaves);
-  const int end = uniform(all * (wave + 1) / kDownWaves);
-  while (at < end) {
-    const bool shared = at >= routed;
-    const int u = shared ? 0 : at / KB, kb0 = shared ? at - routed : at - u * KB;
-    const int kb1 = shared ? kb0 + end - at : min(KB, kb0 + end - at);
-    const int expert = shared ? 0 : uniform((int)(plan.counts.unit[u] >> 16)), first = shared ? 0 : uniform((int)(plan.counts.unit[u] & 0xffffu));
-    const int n = shared ? a.T : uniform(plan.counts.tokens[u]), H = shared ? a.shared.H : a.experts.H;
-    __amdgpu_buffer_rsrc_t rows[1][2];
-    rows_at<FP8>(rows[0], shared ? a.shared.w3 : a.experts.w3, (int64_t)expert * a.D + d0, H);
-    const floats_at scales[1] = {scales_at(shared ? a.shared.s3 : a.experts.s3, expert, d0, a.D, H)};
-    __amdgpu_buffer_rsrc_t parts[P];
-    const int64_t plane = (int64_t)(shared ? a.T : a.T * a.k) * H;
-#pragma unroll
-    for (int p = 0; p < P; ++p) parts[p] = make_rsrc((shared ? a.hs : a.hb) + p * plane, 2 * plane);
-    const int row = r < n ? (shared ? r : plan.list[first + r]) : 0;
-    const uint32_t token = r < n ? (uint32_t)(row * H) * 2 : kNothing;
-    f4 acc[1][1];
-    clear<FP8, 1, 1>(acc);
-    sum_steps<FP8, 1, P>(acc, rows, scales, parts, token, H, kb0, kb1, 1);
-    // (a token has an expert once, so a wave adds to a value once a unit)
-    if (r < n) sums[wave][shared ? row : row / a.k][g] += acc[0][0];
-    at += kb1 - kb0;
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < a.T * 16; i += 64 * kDownWaves) {
-    const int t = i >> 4, d = i & 15;
-    float s = 0.0f;
-#pragma unroll
-    for (int v = 0; v < kDownWaves; ++v) s += sums[v][t][d >> 2][d & 3];
-    const int64_t o = (int64_t)t * a.D + d0 + d;
-    if constexpr (DT == CIN_DT_F32)
-      static_cast<float*>(a.out)[o] = s;
-    else
-      static_cast<uint16_t*>(a.out)[o] = (uint16_t)f32_to_half_bits(DT, s);
-  }
+  leave_rows<DT, UP>(a, shared, at, row0 + 4 * g, both, v[0], v[1]);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -728,7 +661,7 @@ constexpr int kTokenStep = P * NC * 16 * kTokenPitch;
 template <bool UP>
 constexpr int kTileRows = kTileWaves * (UP ? 16 : 32);
 
-using TilePlan = OneUnit<kUnitTokens, kMaxAssigned>;
+using TilePlan = OneUnit<64 * kTileWaves, kUnitTokens, kMaxAssigned>;
 
 template <int DT, bool FP8, bool UP, int NC>
 __device__ __forceinline__ void tile_unit(const LayerArgs& a, const TilePlan& plan, uint16_t* lds, int expert, int tile, int first, int n,
@@ -768,12 +701,13 @@ __device__ __forceinline__ void tile_unit(const LayerArgs& a, const TilePlan& pl
     }
   }
   const int end = pitch - (int)(threadIdx.x & 15) * 8;
-  auto fetch = [&](u4 (&part)[kOwn], int b) {
+  u4 part[kOwn];
+  auto fetch = [&](int b) {
     const bool there = b * kBlock < end;
 #pragma unroll
     for (int o = 0; o < kOwn; ++o) part[o] = load16(parts, there ? from[o] + (uint32_t)b * 2 * kBlock : kNothing);
   };
-  auto leave = [&](const u4 (&part)[kOwn], int b) {
+  auto leave = [&](int b) {
     uint16_t* tile_b = lds + (b & 1) * kTokenStep<P, NC>;
 #pragma unroll
     for (int o = 0; o < kOwn; ++o)
@@ -782,18 +716,16 @@ __device__ __forceinline__ void tile_unit(const LayerArgs& a, const TilePlan& pl
   f4 acc[2][NC];
   clear<FP8, 2, NC>(acc);
   const uint32_t mine = offset_in_rows<FP8>(K);
-  // Two steps' loads are on their way while one is multiplied, a step's tokens before its weights, as loads are waited
-  // for in their order; the tokens' parts of two steps lie in LDS, so that a step has one barrier.
+  // The weights of two steps are on their way while one is multiplied; the next step's tokens go out before the latter
+  // of them, as loads are waited for in their order.  Two steps' tokens lie in LDS, so that a step has one barrier.
   Weights<FP8, 2> w[3];
-  u4 part[2][kOwn];
-  fetch(part[0], 0);
+  fetch(0);
   w[0].load(rows, mine, scales, 0, K);
-  fetch(part[1], 1);  // (past the end: zeros)
-  w[1].load(rows, mine, scales, 1, K);
-  leave(part[0], 0);
+  w[1].load(rows, mine, scales, 1, K);  // (past the end: zeros)
+  leave(0);
   __syncthreads();
-  auto one_step = [&](int b, Weights<FP8, 2>& now, Weights<FP8, 2>& later, const u4 (&next)[kOwn], u4 (&after)[kOwn]) {
-    fetch(after, b + 2);
+  auto one_step = [&](int b, Weights<FP8, 2>& now, Weights<FP8, 2>& later) {
+    fetch(b + 1);
     later.load(rows, mine, scales, b + 2, K);
     if (active) {
       now.settle();
@@ -817,21 +749,15 @@ __device__ __forceinline__ void tile_unit(const LayerArgs& a, const TilePlan& pl
       }
       if constexpr (FP8) join_step<FP8, 2, NC>(acc, sum, now);
     }
-    leave(next, b + 1);
+    leave(b + 1);
     __syncthreads();
   };
-  for (int b = 0; b < KB; b += 6) {
-    one_step(b, w[0], w[2], part[1], part[0]);
+  for (int b = 0; b < KB; b += 3) {
+    one_step(b, w[0], w[2]);
     if (b + 1 >= KB) break;
-    one_step(b + 1, w[1], w[0], part[0], part[1]);
+    one_step(b + 1, w[1], w[0]);
     if (b + 2 >= KB) break;
-    one_step(b + 2, w[2], w[1], part[1], part[0]);
-    if (b + 3 >= KB) break;
-    one_step(b + 3, w[0], w[2], part[0], part[1]);
-    if (b + 4 >= KB) break;
-    one_step(b + 4, w[1], w[0], part[1], part[0]);
-    if (b + 5 >= KB) break;
-    one_step(b + 5, w[2], w[1], part[0], part[1]);
+    one_step(b + 2, w[2], w[1]);
   }
   if (!active) return;
 #pragma unroll
@@ -839,20 +765,13 @@ __device__ __forceinline__ void tile_unit(const LayerArgs& a, const TilePlan& pl
     const int i = c * 16 + r;
     if (i >= n) continue;
     const int at = shared ? first + i : plan.list[first + i];
-    if constexpr (UP) {
-      store_h<kHParts<DT>>((shared ? a.hs : a.hb) + (int64_t)at * H + row0 + 4 * g, (int64_t)(shared ? a.T : a.T * a.k) * H,
-                           acc[0][c], acc[1][c], shared ? 1.0f : a.weights[at]);
-    } else {
-      float* y = a.y + (int64_t)(shared ? a.T * a.k + at : at) * a.D + row0 + 4 * g;
-      *reinterpret_cast<f4*>(y) = acc[0][c];
-      if (both) *reinterpret_cast<f4*>(y + 16) = acc[1][c];
-    }
+    leave_rows<DT, UP>(a, shared, at, row0 + 4 * g, both, acc[0][c], acc[1][c]);
   }
 }
 
 // The units of a tile are neighbours: those of one expert read its weights at the same time, from the cache.
 template <int DT, bool FP8, bool UP>
-__global__ __launch_bounds__(64 * kTileWaves, !FP8 || DT == CIN_DT_F32 ? 2 : UP && DT == CIN_DT_BF16 ? 4 : 3) void k_products(LayerArgs a) {
+__global__ __launch_bounds__(64 * kTileWaves, !FP8 ? 2 : UP && DT == CIN_DT_BF16 ? 4 : 3) void k_products(LayerArgs a) {
   constexpr int UNIT = kUnitTokens, ROWS = kTileRows<UP>;
   __shared__ TilePlan plan;
   extern __shared__ u4 tokens[];  // [parts, columns][kTokenPitch] of 16 bits
@@ -862,10 +781,10 @@ __global__ __launch_bounds__(64 * kTileWaves, !FP8 || DT == CIN_DT_F32 ? 2 : UP 
   if (!shared) {
     tile = blockIdx.x / a.units;
     const int u = blockIdx.x - tile * a.units;
-    if (!plan.make<64 * kTileWaves>(a.idx, a.T * a.k, a.E, u)) return;
-    expert = uniform((int)(plan.counts.unit[0] >> 16));
-    first = uniform((int)(plan.counts.unit[0] & 0xffffu));
-    n = uniform(plan.counts.tokens[0]);
+    if (!plan.make(a.idx, a.T, a.k, a.E, u)) return;
+    expert = uniform((int)(plan.unit >> 16));
+    first = uniform((int)(plan.unit & 0xffffu));
+    n = uniform(plan.tokens);
   } else {
     const int i = blockIdx.x - routed, units = (a.T + UNIT - 1) / UNIT;
     tile = i / units;
@@ -886,9 +805,17 @@ __global__ __launch_bounds__(256) void k_join(LayerArgs a) {
   if (i >= a.T * per) return;
   const int t = i / per, d = (i - t * per) * 4;
   const float* y = a.y + (int64_t)t * a.k * a.D + d;
-  f4 s = *reinterpret_cast<const f4*>(y);
-  for (int j = 1; j < a.k; ++j) s += *reinterpret_cast<const f4*>(y + (int64_t)j * a.D);
-  if (a.shared.H) s += *reinterpret_cast<const f4*>(a.y + (int64_t)(a.T * a.k + t) * a.D + d);
+  f4 s = {0.0f, 0.0f, 0.0f, 0.0f}, last = s;
+  if (a.shared.H) last = *reinterpret_cast<const f4*>(a.y + (int64_t)(a.T * a.k + t) * a.D + d);
+  for (int j = 0; j < a.k; j += 8) {
+    f4 v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = *reinterpret_cast<const f4*>(y + (int64_t)min(j + i, a.k - 1) * a.D);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (j + i < a.k) s += v[i];
+  }
+  s += last;
   const int64_t o = (int64_t)t * a.D + d;
   if constexpr (DT == CIN_DT_F32) {
     *reinterpret_cast<f4*>(static_cast<float*>(a.out) + o) = s;
@@ -916,7 +843,7 @@ int64_t layout(LayerArgs& a, int dtype, char* base) {
   a.xb = reinterpret_cast<uint16_t*>(take(2 * px * a.T * a.Dp));
   a.hb = reinterpret_cast<uint16_t*>(take(2 * ph * a.T * a.k * a.experts.H));
   a.hs = reinterpret_cast<uint16_t*>(take(2 * ph * a.T * a.shared.H));
-  a.y = reinterpret_cast<float*>(take(a.T > kFewTokens ? 4LL * a.T * (a.k + 1) * a.D : 0));
+  a.y = reinterpret_cast<float*>(take(4LL * a.T * (a.k + 1) * a.D));
   return at;
 }
 
@@ -941,22 +868,33 @@ void set_sizes(LayerArgs& a, int64_t T, int64_t D, int64_t E, int64_t k, int64_t
   a.units = (int)((n < E ? n : E) + n / kUnitTokens);
 }
 
+// Whether the waves share K: where k_products would have fewer than one and a half workgroups a CU.  One token, 8 of 32 experts
+// of 7168 x 2048 and a shared one: up, 288 of them, 48 us against 65, down, 504, 29 against 25; 16 tokens, 16 experts of
+// 1024 x 1024, 320 and 136: 43 against 51 a call.
+bool splits_k(const LayerArgs& a, bool up) {
+  const int64_t rows = up ? kTileRows<true> : kTileRows<false>;
+  const int64_t groups = a.units * cdiv(up ? a.experts.H : a.D, rows) + (a.shared.H ? cdiv(up ? a.shared.H : a.D, rows) : 0);
+  return a.T <= kFewTokens && 2 * groups < 3 * cin_device_cus();
+}
+
 template <int DT, bool FP8, bool UP>
 void launch_products(const LayerArgs& a, hipStream_t stream) {
-  constexpr int P = UP ? kXParts<DT> : kHParts<DT>, ROWS = kTileRows<UP>, UNIT = kUnitTokens;
-  const int per = ((UP ? a.experts.H : a.D) + ROWS - 1) / ROWS;
-  const int shared = a.shared.H ? ((UP ? a.shared.H : a.D) + ROWS - 1) / ROWS * ((a.T + UNIT - 1) / UNIT) : 0;
-  const size_t lds = 2 * sizeof(uint16_t) * kTokenStep<P, UNIT / 16>;
-  hipLaunchKernelGGL((k_products<DT, FP8, UP>), dim3(a.units * per + shared), dim3(64 * kTileWaves), lds, stream, a);
+  const bool few = splits_k(a, UP);
+  const int64_t rows = few ? (UP ? 16 : 32) : kTileRows<UP>, units = few ? 1 : cdiv(a.T, kUnitTokens);
+  const int64_t routed = a.units * cdiv(UP ? a.experts.H : a.D, rows);
+  const int64_t shared = a.shared.H ? units * cdiv(UP ? a.shared.H : a.D, rows) : 0;
+  const dim3 grid((uint32_t)(routed + shared));
+  if (few) {
+    hipLaunchKernelGGL((k_few<DT, FP8, UP>), grid, dim3(64 * kFewWaves), 0, stream, a);
+  } else {
+    constexpr int P = UP ? kXParts<DT> : kHParts<DT>;
+    const size_t lds = 2 * sizeof(uint16_t) * kTokenStep<P, kUnitTokens / 16>;
+    hipLaunchKernelGGL((k_products<DT, FP8, UP>), grid, dim3(64 * kTileWaves), lds, stream, a);
+  }
 }
 
 template <int DT, bool FP8>
 void launch_experts(const LayerArgs& a, hipStream_t stream) {
-  if (a.T <= kFewTokens) {
-    hipLaunchKernelGGL((k_up_few<DT, FP8>), dim3((a.units * a.experts.H + a.shared.H) / 16), dim3(64 * kUpWaves), 0, stream, a);
-    hipLaunchKernelGGL((k_down_few<DT, FP8>), dim3(a.D / 16), dim3(64 * kDownWaves), 0, stream, a);
-    return;
-  }
   launch_products<DT, FP8, true>(a, stream);
   launch_products<DT, FP8, false>(a, stream);
   hipLaunchKernelGGL((k_join<DT>), dim3((a.T * (a.D / 4) + 255) / 256), dim3(256), 0, stream, a);
