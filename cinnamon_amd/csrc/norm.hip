@@ -59,7 +59,7 @@ struct NormArgs {
   const void *gn, *gx;
   int64_t ldgn, ldgx;
   void *dy, *dr, *dgate;
-  float* partial;  // [kSums, workgroups, D], then one value a workgroup for the learned scale
+  float* partial;  // [kSums, workgroups, D], then one double a workgroup for the learned scale
 };
 
 template <int DT>
@@ -339,6 +339,11 @@ __global__ __launch_bounds__(WAVE ? 64 * kWaveRows : kMaxThreads) void k_norm_fo
   }
 }
 
+// Behind the partial rows: a workgroup's sum for the learned scale of one value.
+__host__ __device__ inline double* one_sums(const float* partial, int64_t groups, int D) {
+  return reinterpret_cast<double*>(const_cast<float*>(partial) + (kSums * groups * D + 1) / 2 * 2);
+}
+
 // Partial sums of one workgroup: of its waves' rows together where each has its own.
 template <int CH, bool WAVE>
 __device__ __forceinline__ void leave_partial(const NormArgs& a, int which, const float (&v)[CH][8], const Span<CH>& s,
@@ -462,7 +467,8 @@ __global__ __launch_bounds__(WAVE ? 64 * kWaveRows : kMaxThreads) void k_norm_ba
   const Slots vectors{slots, WAVE ? 64 : (int)blockDim.x, lane, CH};
   const Slots scale_sums{slots + (kInLds ? 6 * CH * vectors.threads : 0), (int)blockDim.x, (int)threadIdx.x, CH};
   float w[R][8], gp[FULL ? R : 1][8], value = a.scale_value;
-  float sw[CH][8], su[FULL ? CH : 1][8], sone = 0.0f;
+  float sw[CH][8], su[FULL ? CH : 1][8];
+  double sone = 0.0;  // over all channels of all rows: in fp32 it would lose half its digits
   const float inv_d = 1.0f / (float)a.D;
   if (FULL && a.scale_kind == kOneValue) value = load_elem(a.scale.p, a.scale.dtype, 0);
 #pragma unroll
@@ -565,7 +571,7 @@ __global__ __launch_bounds__(WAVE ? 64 * kWaveRows : kMaxThreads) void k_norm_ba
       if constexpr (MODE == kAny) in.ge[c].forget();
     }
     const float c1 = -(q[0] * inv_d * i * i * i);
-    float p[2] = {0.0f, 0.0f};
+    float p[2] = {0.0f, 0.0f}, one_sum = 0.0f;
     // x becomes dx, then du without a channel's gate
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
@@ -586,7 +592,7 @@ __global__ __launch_bounds__(WAVE ? 64 * kWaveRows : kMaxThreads) void k_norm_ba
       if constexpr (FULL) {
         if (a.scale_kind == kOneValue) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) sone = __builtin_fmaf(x[c][e], in.r[c].at(e), sone);
+          for (int e = 0; e < 8; ++e) one_sum = __builtin_fmaf(x[c][e], in.r[c].at(e), one_sum);
         } else if (scale_channels) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[e] = x[c][e] * in.r[c].at(e);
@@ -614,6 +620,7 @@ __global__ __launch_bounds__(WAVE ? 64 * kWaveRows : kMaxThreads) void k_norm_ba
       }
     }
     if constexpr (FULL) {
+      sone += (double)one_sum;
       if (post || (MODE == kAny && a.gate_kind == kRow)) sum2(p, waves);
       if (inner) {
         const float c2 = post ? -(p[0] * inv_d * j * j * j) : 0.0f;
@@ -657,14 +664,15 @@ __global__ __launch_bounds__(WAVE ? 64 * kWaveRows : kMaxThreads) void k_norm_ba
       leave_partial<CH, WAVE>(a, kSumScale, sw, s, joined);
     }
     if (a.scale_kind == kOneValue) {
-      __shared__ float ones[kMaxThreads / 64];
-      const float t = wave_sum(sone);
-      if ((threadIdx.x & 63) == 0) ones[threadIdx.x >> 6] = t;
+      __shared__ double ones[kMaxThreads / 64];
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) sone += __shfl_xor(sone, o);
+      if ((threadIdx.x & 63) == 0) ones[threadIdx.x >> 6] = sone;
       __syncthreads();
       if (threadIdx.x == 0) {
-        float v = 0.0f;
+        double v = 0.0;
         for (int k = 0; k < waves; ++k) v += ones[k];
-        a.partial[(int64_t)kSums * gridDim.x * a.D + blockIdx.x] = v;
+        one_sums(a.partial, gridDim.x, a.D)[blockIdx.x] = v;
       }
     }
   }
@@ -693,16 +701,18 @@ __global__ __launch_bounds__(1024) void k_norm_columns(ColumnArgs a) {
   const int groups = (a.D + 31) / 32;
   if ((int)blockIdx.x == groups) {
     if (blockIdx.y != 0 || !a.one) return;
-    const float* p = a.partial + (int64_t)kSums * a.G * a.D;
-    float t = 0.0f;
+    const double* p = one_sums(a.partial, a.G, a.D);
+    __shared__ double sums[16];
+    double t = 0.0;
     for (int64_t i = threadIdx.x; i < a.G; i += 1024) t += p[i];
-    lds[line][col] = t;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) t += __shfl_xor(t, o);
+    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = t;
     __syncthreads();
     if (threadIdx.x == 0) {
-      float v = 0.0f;
-      for (int l = 0; l < 32; ++l)
-        for (int c = 0; c < 32; ++c) v += lds[l][c];
-      store_elem(a.one, a.one_dtype, 0, v);
+      double v = 0.0;
+      for (int w = 0; w < 16; ++w) v += sums[w];
+      store_elem(a.one, a.one_dtype, 0, (float)v);
     }
     return;
   }
@@ -875,7 +885,8 @@ int64_t cin_block_norm_workspace(int64_t T, int64_t D) {
     cin_set_error(CIN_ERR_ARG, "cin_block_norm_workspace: D must be in [1, %lld]", (long long)kMaxWidth);
     return -1;
   }
-  return 4 * groups_of(T, shape_of(D), true) * (kSums * D + 1);
+  const int64_t groups = groups_of(T, shape_of(D), true);
+  return 4 * ((kSums * groups * D + 1) / 2 * 2) + 8 * groups;
 }
 
 int cin_block_norm_backward(const void* y, int dtype, int64_t ldy, const void* r, int r_dtype, int64_t ldr, int64_t T,

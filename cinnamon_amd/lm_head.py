@@ -255,26 +255,33 @@ def verify_drafts(draft_tokens: torch.Tensor, draft_probs: torch.Tensor | None, 
     the first token at which the running sum exceeds uniforms[K] times the whole.  Behind it tokens is -1; it is
     -1 itself where the sum is not positive and finite.  Products, differences and sums are in 64 bits; rows need not
     sum to one.  No gradient."""
-    for t in (draft_tokens, draft_probs, target_probs, uniforms, n_drafts):
-        _require(t is None or (t.is_cuda and t.device == target_probs.device), "Inputs must be on one CUDA device")
+    dev = target_probs.device
+    _require(target_probs.is_cuda and draft_tokens.device == dev and uniforms.device == dev
+             and (draft_probs is None or draft_probs.device == dev) and (n_drafts is None or n_drafts.device == dev),
+             "Inputs must be on one CUDA device")
     _require(draft_tokens.ndim == 2 and target_probs.ndim == 3, "draft_tokens must be [B, K] and target_probs [B, K + 1, V]")
     (B, K), V = draft_tokens.shape, target_probs.shape[2]
-    _require(K <= MAX_DRAFTS, f"at most {MAX_DRAFTS} drafts")
+    _require(K <= MAX_DRAFTS, "at most 63 drafts")
     _require(target_probs.shape == (B, K + 1, V) and V >= 1, "target_probs must be [B, K + 1, V]")
     _require(target_probs.dtype in _DTYPES, "probabilities must be bf16, fp16 or fp32")
     _require(draft_probs is None or (draft_probs.shape == (B, K, V) and draft_probs.dtype == target_probs.dtype),
              "draft_probs must be [B, K, V] in target_probs' dtype")
     _require(uniforms.shape == (B, K + 1) and uniforms.dtype in (torch.float32, torch.float64),
              "uniforms must be [B, K + 1] in fp32 or fp64")
-    for t, shape in ((draft_tokens, (B, K)), (n_drafts, (B,))):
-        _require(t is None or (t.shape == shape and not t.dtype.is_floating_point and not t.dtype.is_complex
-                               and t.dtype != torch.bool), "draft_tokens and n_drafts must hold integers, n_drafts [B] of them")
-    if draft_tokens.dtype != torch.int64:
-        draft_tokens = draft_tokens.to(torch.int64)
-    if n_drafts is not None and n_drafts.dtype != torch.int64:
-        n_drafts = n_drafts.to(torch.int64)
-    return _run(_verify_op, draft_tokens, None if draft_probs is None else draft_probs.detach(), target_probs.detach(),
-                uniforms.detach(), n_drafts)
+    draft_tokens = _integers(draft_tokens)
+    if n_drafts is not None:
+        _require(n_drafts.shape == (B,), "n_drafts must be [B]")
+        n_drafts = _integers(n_drafts)
+    return _run(_verify_op, draft_tokens, draft_probs, target_probs, uniforms, n_drafts)
+
+
+def _integers(t):
+    """int64, of integers."""
+    if t.dtype == torch.int64:
+        return t
+    _require(not t.dtype.is_floating_point and not t.dtype.is_complex and t.dtype != torch.bool,
+             "draft_tokens and n_drafts must hold integers")
+    return t.to(torch.int64)
 
 
 @functools.lru_cache(maxsize=256)

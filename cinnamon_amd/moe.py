@@ -45,6 +45,7 @@ __all__ = ["moe_gate", "moe_route", "moe_gather_quantize", "moe_gather_sum", "mo
 # The gate (reference src/layers.py:122-126)
 # ---------------------------------------------------------------------------
 _SCORES = {"sigmoid": 0, "softmax": 1}
+_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
 def moe_gate(logits: torch.Tensor, top_k: int, bias: torch.Tensor | None = None, score: str = "sigmoid",
@@ -522,23 +523,22 @@ def moe_decode(x: torch.Tensor, router_weight: torch.Tensor, experts, top_k: int
     they are not quantized, products are summed in fp32 and the result is rounded once.  Inference only: no
     gradient.  Bit-identical from call to call."""
     _require(x.is_cuda, "Input must be on CUDA")
-    _require(x.ndim == 2 and x.shape[0] <= MAX_DECODE_TOKENS, f"x must be [n_tokens, D] with at most {MAX_DECODE_TOKENS} tokens")
-    _require(x.dtype in (torch.bfloat16, torch.float16, torch.float32), "x must be bf16, fp16 or fp32")
-    D = x.shape[1]
-    _require(router_weight.ndim == 2 and router_weight.shape[1] == D and router_weight.device == x.device
-             and router_weight.dtype in (torch.bfloat16, torch.float16, torch.float32),
-             "router_weight must be [E, D] on x's device, in bf16, fp16 or fp32")
+    _require(x.ndim == 2 and x.shape[0] <= MAX_DECODE_TOKENS, "x must be [n_tokens, D] with at most 128 tokens")
+    _require(x.dtype in _DTYPES, "x must be bf16, fp16 or fp32")
+    dev, D = x.device, x.shape[1]
+    _require(router_weight.ndim == 2 and router_weight.shape[1] == D and router_weight.device == dev
+             and router_weight.dtype in _DTYPES, "router_weight must be [E, D] on x's device, in bf16, fp16 or fp32")
     E = router_weight.shape[0]
-    _require(1 <= E <= MAX_DECODE_EXPERTS, f"n_experts must be in [1, {MAX_DECODE_EXPERTS}]")
+    _require(1 <= E <= MAX_DECODE_EXPERTS, "n_experts must be in [1, 1024]")
     _require(score in _SCORES, "score must be 'sigmoid' or 'softmax'")
-    _require(1 <= n_groups <= MAX_GROUPS and E % n_groups == 0, f"n_groups must divide n_experts and be in [1, {MAX_GROUPS}]")
+    _require(1 <= n_groups <= MAX_GROUPS and E % n_groups == 0, "n_groups must divide n_experts and be in [1, 64]")
     top_groups = n_groups if top_groups is None else top_groups
     _require(1 <= top_groups <= n_groups, "top_groups must be in [1, n_groups]")
     _require(group_top in (1, 2), "group_top must be 1 or 2")
     _require(1 <= top_k <= min(MAX_TOP_K, top_groups * (E // n_groups)),
-             f"top_k must be in [1, {MAX_TOP_K}] and within the experts of the kept groups")
+             "top_k must be in [1, 16] and within the experts of the kept groups")
     if bias is not None:
-        _require(bias.shape == (E,) and bias.device == x.device and bias.dtype == torch.float32,
+        _require(bias.shape == (E,) and bias.device == dev and bias.dtype == torch.float32,
                  "bias must be fp32 [n_experts] on x's device")
         bias = bias.detach()
     if isinstance(experts, layers.GroupedExperts):
@@ -549,11 +549,10 @@ def moe_decode(x: torch.Tensor, router_weight: torch.Tensor, experts, top_k: int
         (w12q, _, w12s), (w3q, _, w3s) = q if q is not None else layers.quantize_expert_weights(w12, w3)
         experts = (w12q.view(E, 2 * H, D), w12s.view(E, 2 * H // 128, -1), w3q.view(E, D, H), w3s.view(E, D // 128, -1))
     weights = _decode_weights(experts, x, (E,))
+    extra = (None,) * 4
     if shared is not None:
         extra = _decode_weights(shared, x, ())
         _require(extra[0].dtype == weights[0].dtype, "the shared expert's weights must have the experts' type")
-    else:
-        extra = (None,) * 4
     out = _run_detached(_decode_op, x, router_weight, bias, *weights, *extra, int(top_k), _SCORES[score], int(n_groups),
                         int(top_groups), int(group_top), bool(renormalize), float(scale))
     return out if return_routing else out[0]
@@ -563,22 +562,20 @@ def _decode_weights(weights, x, lead):
     """The four tensors of stacked experts (lead (E,)) or of one (()), checked."""
     _require(isinstance(weights, (tuple, list)) and len(weights) == 4, "expert weights must be (w12, w12_scales, w3, w3_scales)")
     w12, s12, w3, s3 = weights
-    n = len(lead)
-    D = x.shape[1]
-    _require(w12.ndim == n + 2 and w3.ndim == n + 2, "w12 must be [E, 2 H, D] and w3 [E, D, H]")
-    H = w3.shape[-1]
-    _require(tuple(w12.shape) == (*lead, 2 * H, D) and tuple(w3.shape) == (*lead, D, H), "w12 must be [E, 2 H, D] and w3 [E, D, H]")
-    _require(D >= 16 and H >= 16 and D % 16 == 0 and H % 16 == 0 and max(D, H) <= 65536, "D and H must be multiples of 16 up to 65536")
-    _require(w12.dtype == w3.dtype and w12.dtype in (torch.float8_e4m3fn, torch.bfloat16), "weights must be e4m3 codes or bf16")
-    if w12.dtype == torch.bfloat16:
+    D, dev, dt = x.shape[1], x.device, w12.dtype
+    H = w3.shape[-1] if w3.ndim else 0
+    _require(w12.shape == (*lead, 2 * H, D) and w3.shape == (*lead, D, H), "w12 must be [E, 2 H, D] and w3 [E, D, H]")
+    _require(D >= 16 and H >= 16 and D % 16 == 0 and H % 16 == 0 and D <= 65536 and H <= 65536,
+             "D and H must be multiples of 16 up to 65536")
+    _require(dt == w3.dtype and w12.device == dev and w3.device == dev, "weights must share one dtype, on x's device")
+    if dt == torch.bfloat16:
         _require(s12 is None and s3 is None, "bf16 weights have no scales")
-    else:
-        _require(s12 is not None and s3 is not None and s12.dtype == s3.dtype == torch.float32
-                 and tuple(s12.shape) == (*lead, _cdiv(2 * H, 128), _cdiv(D, 128))
-                 and tuple(s3.shape) == (*lead, _cdiv(D, 128), _cdiv(H, 128)), "codes need fp32 scales of their 128 x 128 blocks")
-    for t in (w12, s12, w3, s3):
-        _require(t is None or t.device == x.device, "weights must be on x's device")
-    return tuple(None if t is None else t.detach() for t in (w12, s12, w3, s3))
+        return w12.detach(), None, w3.detach(), None
+    _require(dt == torch.float8_e4m3fn, "weights must be e4m3 codes or bf16")
+    _require(s12 is not None and s3 is not None and s12.dtype == torch.float32 and s3.dtype == torch.float32
+             and s12.device == dev and s3.device == dev and s12.shape == (*lead, _cdiv(2 * H, 128), _cdiv(D, 128))
+             and s3.shape == (*lead, _cdiv(D, 128), _cdiv(H, 128)), "codes need fp32 scales of their 128 x 128 blocks, on x's device")
+    return w12, s12.detach(), w3, s3.detach()
 
 
 @functools.lru_cache(maxsize=256)
@@ -590,10 +587,14 @@ def _decode_workspace(dtype, *sizes):
 
 
 def _on16(t):
-    """Contiguous, its first element on 16 bytes."""
-    if t is None or (t.is_contiguous() and t.data_ptr() % 16 == 0):
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+    """(contiguous, its first element on 16 bytes; its address)"""
+    if t is None:
+        return None, 0
+    at = t.data_ptr()
+    if at % 16 or not t.is_contiguous():
+        t = t.clone(memory_format=torch.contiguous_format)
+        at = t.data_ptr()
+    return t, at
 
 
 @custom_op("moe_decode", "(Tensor x, Tensor router, Tensor? bias, Tensor w12, Tensor? s12, Tensor w3, Tensor? s3, Tensor? shared_w12, "
@@ -605,14 +606,13 @@ def _decode_op(x, router, bias, w12, s12, w3, s3, sw12, ss12, sw3, ss3, top_k, s
     T, D = x.shape
     E, H = router.shape[0], w3.shape[-1]
     Hs = 0 if sw3 is None else sw3.shape[-1]
-    held = [_on16(t) for t in (w12, s12, w3, s3, sw12, ss12, sw3, ss3)]
+    held, p = zip(*[_on16(t) for t in (w12, s12, w3, s3, sw12, ss12, sw3, ss3)])
     bias = None if bias is None else bias.contiguous()
     out = x.new_empty((T, D))
     idx = x.new_empty((T, top_k), dtype=torch.int64)
     weights = x.new_empty((T, top_k), dtype=torch.float32)
     ws = _decode_workspace(x.dtype, T, D, E, top_k, H, Hs)
     work = torch.empty(ws, dtype=torch.uint8, device=x.device)
-    p = [ptr(t) for t in held]
     call_on(x, "cin_moe_decode", x.data_ptr(), dtype_code(x), max(x.stride(0), D), T, D, router.data_ptr(), dtype_code(router),
             max(router.stride(0), D), E, ptr(bias), top_k, score, n_groups, top_groups, group_top, renormalize, scale,
             w12.dtype == torch.float8_e4m3fn, *p[:4], H, *p[4:], Hs, out.data_ptr(), idx.data_ptr(), weights.data_ptr(),

@@ -13,7 +13,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import call_on, dtype_code, ptr, stream_of
+from ._lib import _DTYPE_CODE, call_on, ptr, stream_of
 from .kernels import _plain_eager, _require, custom_op
 
 __all__ = ["block_norm", "rms_norm"]
@@ -47,31 +47,36 @@ def block_norm(y: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | N
 
     Computed in fp32 and each output rounded once: the norm is that of the sum before its rounding.
     Differentiable (once) in every tensor, gradients in their dtype, bit-identical from call to call.  The backward
-    keeps the inputs and two words a row, forms the sum again, and works in up to 16 D bytes a workgroup."""
+    keeps the inputs and two words a row, forms the sum again, and works in up to 12 D bytes a workgroup."""
     _require(residual is not None, "residual must be a tensor (rms_norm takes none)")
-    scale, value = (residual_scale, 1.0) if torch.is_tensor(residual_scale) else \
-        (None, 1.0 if residual_scale is None else float(residual_scale))
+    if residual_scale is None:
+        scale, value = None, 1.0
+    elif isinstance(residual_scale, torch.Tensor):
+        scale, value = residual_scale, 1.0
+    else:
+        scale, value = None, float(residual_scale)
     _check(y, residual, weight, post_weight, gate, scale)
     return _call(y, residual, weight, post_weight, gate, scale, value, eps)[:2]
 
 
 def _check(y, residual, weight, post_weight, gate, scale):
     _require(y.is_cuda, "Input must be on CUDA")
-    _require(y.ndim >= 1 and 1 <= y.shape[-1] <= MAX_WIDTH, f"the last dimension must be in [1, {MAX_WIDTH}]")
-    _require(y.dtype in _DTYPES, "y must be bf16, fp16 or fp32")
-    D, dev = y.shape[-1], y.device
+    shape, dt, dev = y.shape, y.dtype, y.device
+    _require(len(shape) >= 1 and 1 <= shape[-1] <= MAX_WIDTH, "the last dimension must be in [1, 16384]")
+    _require(dt in _DTYPES, "y must be bf16, fp16 or fp32")
+    D = shape[-1]
     if residual is not None:
-        _require(residual.shape == y.shape and residual.device == dev, "residual must have y's shape and device")
-        _require(residual.dtype == y.dtype or residual.dtype == torch.float32, "residual must have y's dtype or fp32")
-    for name, t in (("weight", weight), ("post_weight", post_weight)):
+        _require(residual.shape == shape and residual.device == dev, "residual must have y's shape and device")
+        _require(residual.dtype == dt or residual.dtype == torch.float32, "residual must have y's dtype or fp32")
+    for t in (weight, post_weight):
         if t is not None:
-            _require(t.shape == (D,) and t.device == dev and t.dtype in _DTYPES,
-                     f"{name} must be [D] on y's device, in bf16, fp16 or fp32")
+            _require(t.ndim == 1 and t.shape[0] == D and t.device == dev and t.dtype in _DTYPES,
+                     "weight and post_weight must be [D] on y's device, in bf16, fp16 or fp32")
     if gate is not None:
         kind = _gate_kind(gate, y)
         _require(kind != _NO_GATE and gate.device == dev and gate.dtype in _DTYPES,
                  "gate must be [D], [..., 1] or of y's shape, on y's device")
-        _require(kind != _ELEMENT or gate.dtype == y.dtype, "a gate of y's shape must have y's dtype")
+        _require(kind != _ELEMENT or gate.dtype == dt, "a gate of y's shape must have y's dtype")
     if scale is not None:
         _require((scale.numel() == 1 or scale.shape == (D,)) and scale.device == dev and scale.dtype in _DTYPES,
                  "residual_scale must be a number, or one value or [D] on y's device")
@@ -89,67 +94,75 @@ def _gate_kind(gate, y):
 
 
 def _call(y, residual, weight, post_weight, gate, scale, value, eps):
-    args = (y, residual, weight, post_weight, gate, scale)
-    tensors = [t for t in args if t is not None]
+    tensors = [t for t in (y, residual, weight, post_weight, gate, scale) if t is not None]
     if _plain_eager() and all(type(t) in _PLAIN for t in tensors):
         if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-            return _BlockNorm.apply(*args, value, float(eps))
-        return _launch(*args, value, float(eps), False)
-    n, x, stats = _norm_op(*args, value, float(eps))
-    return n, x, stats
+            return _BlockNorm.apply(y, residual, weight, post_weight, gate, scale, value, float(eps))
+        return _launch(y, residual, weight, post_weight, gate, scale, value, float(eps), False)
+    return _norm_op(y, residual, weight, post_weight, gate, scale, value, float(eps))
 
 
-def _rows(t):
-    """(t as rows of adjacent elements, elements between them)"""
-    D = t.shape[-1]
-    t2 = t if t.ndim == 2 else t.reshape(-1, D)
-    if not t2.is_contiguous() and (t2.stride(1) != 1 or t2.stride(0) < D):
-        t2 = t2.contiguous()
-    return t2, max(t2.stride(0), D)
+def _rows(t, D):
+    """(what holds t's rows of adjacent elements, their address, the elements between them)"""
+    if t.is_contiguous():
+        return t, t.data_ptr(), D
+    t = t if t.ndim == 2 else t.reshape(-1, D)
+    if t.stride(1) != 1 or t.stride(0) < D:
+        t = t.contiguous()
+    return t, t.data_ptr(), max(t.stride(0), D)
 
 
-def _side(t):
-    """(what holds the rows, the arguments of one tensor [.., D]: pointer, type, stride)"""
+def _vector(t):
+    """(what holds the vector, its address, its type's code)"""
     if t is None:
-        return None, (0, 0, 0)
-    rows, ld = _rows(t)
-    return rows, (rows.data_ptr(), dtype_code(rows), ld)
+        return None, 0, 0
+    t = t if t.is_contiguous() else t.contiguous()
+    return t, t.data_ptr(), _DTYPE_CODE[t.dtype]
 
 
 def _inputs(y, residual, weight, post_weight, gate, scale, value):
     """(what must live until the launch, the arguments both directions share)"""
-    y2, ya = _side(y)
-    r2, ra = _side(residual)
+    D = y.shape[-1]
+    T = y.numel() // D
+    code = _DTYPE_CODE[y.dtype]
+    kind = _NO_GATE if gate is None else _gate_kind(gate, y)
+    if kind == _NO_GATE:
+        gp = gcode = ldg = 0
+    else:
+        gcode = _DTYPE_CODE[gate.dtype]
+        if kind == _ELEMENT:
+            gate, gp, ldg = _rows(gate, D)
+        else:
+            if kind == _ROW:
+                gate = gate.reshape(-1)
+            if kind == _CHANNEL or gate.stride(0) < 1:
+                gate = gate.contiguous()
+            gp, ldg = gate.data_ptr(), gate.stride(0)
+    y, yp, ldy = _rows(y, D)
     if residual is None:
-        ra = (0, ya[1], ya[2])
-    w = None if weight is None else weight.contiguous()
-    pw = None if post_weight is None else post_weight.contiguous()
-    kind = _gate_kind(gate, y)
-    ldg, g = 0, gate
-    if kind == _ELEMENT:
-        g, ldg = _rows(gate)
-    elif kind == _ROW:
-        g = gate.reshape(-1)
-        ldg = g.stride(0)
-        if ldg < 1:
-            g, ldg = g.contiguous(), 1
-    elif kind == _CHANNEL:
-        g = gate.contiguous()
-    s = None if scale is None else scale.contiguous()
+        rp, rcode, ldr = 0, code, D
+    else:
+        rcode = _DTYPE_CODE[residual.dtype]
+        residual, rp, ldr = _rows(residual, D)
+    weight, wp, wcode = _vector(weight)
+    post_weight, pp, pcode = _vector(post_weight)
+    scale, sp, scode = _vector(scale)
     # (a scale of one value stays one where D is 1 too)
-    skind = 0 if s is None else 1 if s.numel() == 1 else 2
-    code = lambda t: 0 if t is None else dtype_code(t)  # noqa: E731
-    return (y2, r2, w, pw, g, s), (*ya, *ra, y2.shape[0], y2.shape[1], ptr(w), code(w), ptr(pw), code(pw), ptr(g), code(g),
-                                   kind, ldg, ptr(s), code(s), skind, value)
+    skind = 0 if scale is None else 1 if scale.numel() == 1 else 2
+    return (y, residual, weight, post_weight, gate, scale), (yp, code, ldy, rp, rcode, ldr, T, D, wp, wcode, pp, pcode, gp, gcode,
+                                                             kind, ldg, sp, scode, skind, value)
+
+
+_T, _KIND = 6, 14  # of the arguments
 
 
 def _launch(y, residual, weight, post_weight, gate, scale, value, eps, train=True):
     """(normed, new residual or None, what the backward needs of the rows or None)"""
-    keep, args = _inputs(y, residual, weight, post_weight, gate, scale, value)
+    held, args = _inputs(y, residual, weight, post_weight, gate, scale, value)
     n = torch.empty(y.shape, dtype=y.dtype, device=y.device)
     x = None if residual is None else torch.empty(y.shape, dtype=residual.dtype, device=y.device)
-    stats = torch.empty(2 * args[6], dtype=torch.float32, device=y.device) if train else None
-    call_on(y, "cin_block_norm", *args, eps, n.data_ptr(), ptr(x), ptr(stats), stream_of(y))
+    stats = torch.empty(2 * args[_T], dtype=torch.float32, device=y.device) if train else None
+    call_on(n, "cin_block_norm", *args, eps, n.data_ptr(), ptr(x), ptr(stats), stream_of(n))
     return n, x, stats
 
 
@@ -161,19 +174,22 @@ def _workspace(T, D, device):
 
 def _launch_backward(gn, gx, y, residual, weight, post_weight, gate, scale, stats, value, needs):
     """Gradients of the six tensors, None where not needed."""
-    keep, args = _inputs(y, residual, weight, post_weight, gate, scale, value)
-    T, D = args[6:8]
-    grads = [torch.empty(t.shape, dtype=t.dtype, device=y.device) if need and t is not None else None
+    held, args = _inputs(y, residual, weight, post_weight, gate, scale, value)
+    T, D = args[_T], args[_T + 1]
+    dev = y.device
+    grads = [torch.empty(t.shape, dtype=t.dtype, device=dev) if need and t is not None else None
              for t, need in zip((y, residual, weight, post_weight, gate, scale), needs)]
     if T == 0:  # sums over no rows
         return [g if g is None else g.zero_() for g in grads]
-    gn2, gna = _side(gn)
-    gx2, gxa = _side(gx)
-    sums = any(g is not None for g in (grads[2], grads[3], grads[5])) or (grads[4] is not None and args[14] == _CHANNEL)
-    ws = _workspace(T, D, y.device) if sums else 0
-    work = torch.empty(ws, dtype=torch.uint8, device=y.device) if sums else None
-    call_on(y, "cin_block_norm_backward", *args, stats.data_ptr(), gna[0], gna[2], gxa[0], gxa[2], *(ptr(g) for g in grads),
-            ptr(work), ws, stream_of(y))
+    gn, gnp, ldgn = (None, 0, 0) if gn is None else _rows(gn, D)
+    gx, gxp, ldgx = (None, 0, 0) if gx is None else _rows(gx, D)
+    dy, dr, dw, dpw, dgate, dscale = grads
+    ws, work = 0, None
+    if dw is not None or dpw is not None or dscale is not None or (dgate is not None and args[_KIND] == _CHANNEL):
+        ws = _workspace(T, D, y.get_device())
+        work = torch.empty(ws, dtype=torch.uint8, device=dev)
+    call_on(y, "cin_block_norm_backward", *args, stats.data_ptr(), gnp, ldgn, gxp, ldgx, ptr(dy), ptr(dr), ptr(dw), ptr(dpw),
+            ptr(dgate), ptr(dscale), ptr(work), ws, stream_of(y))
     return grads
 
 
@@ -198,7 +214,7 @@ class _BlockNorm(torch.autograd.Function):
 def _gradients(ctx, gn, gx):
     if gn is None and gx is None:
         return (None,) * 8
-    return (*_launch_backward(gn, gx, *ctx.saved_tensors, ctx.value, ctx.needs_input_grad[:6]), None, None)
+    return (*_launch_backward(gn, gx, *ctx.saved_tensors, ctx.value, ctx.needs_input_grad), None, None)
 
 
 @custom_op("block_norm", "(Tensor y, Tensor? residual, Tensor? weight, Tensor? post_weight, Tensor? gate, Tensor? scale, "
