@@ -406,14 +406,14 @@ __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirs
 // k_of(q, lane / 16) on.  Both operands take the same elements, so their order in a product does not matter.
 //
 // A load takes 8 rows' 128 adjacent bytes (lane: row lane % 8, 16 bytes from 16 (lane / 8) on), a whole line of each,
-// streamed past the caches: 969 MB of codes in rows of 7168 arrive at 6.2 TB/s, against 4.8 with 64 bytes of 16 rows a load
+// streamed past the caches where rows begin on lines: 969 MB of codes in rows of 7168 arrive at 6.2 TB/s, against 4.8 with 64 bytes of 16 rows a load
 // and 5.5 with those kept in the caches (linear reads: 7.0).  Two loads, of rows 0-7 and 8-15, then hold every lane's
 // two words, half of them in the lane 8 further in its row of 16: settle() swaps those.
 template <bool FP8>
 __device__ __forceinline__ constexpr int k_of(int q, int g) {
   return FP8 ? g * 32 + q * 8 : (q >> 1) * 64 + g * 16 + (q & 1) * 8;
 }
-template <bool FP8, int M>
+template <bool FP8, bool STREAM, int M>
 struct Weights {
   static constexpr int kWords = FP8 ? 2 : 4;  // of 16 bytes
   u4 w[M][kWords];
@@ -429,7 +429,7 @@ struct Weights {
 #pragma unroll
       for (int m = 0; m < M; ++m)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) w[m][2 * j + i] = load16<kStream>(rows[m][i], at);
+        for (int i = 0; i < 2; ++i) w[m][2 * j + i] = load16<STREAM ? kStream : 0>(rows[m][i], at);
     }
     if constexpr (FP8) {
 #pragma unroll
@@ -489,8 +489,8 @@ __device__ __forceinline__ void clear(f4 (&acc)[M][NC]) {
     for (int c = 0; c < NC; ++c) acc[m][c] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 }
 // A step's sums join the others by their block's scale (16 rows share it).
-template <bool FP8, int M, int NC>
-__device__ __forceinline__ void join_step(f4 (&acc)[M][NC], const f4 (&sum)[M][NC], const Weights<FP8, M>& w) {
+template <bool FP8, bool STREAM, int M, int NC>
+__device__ __forceinline__ void join_step(f4 (&acc)[M][NC], const f4 (&sum)[M][NC], const Weights<FP8, STREAM, M>& w) {
 #pragma unroll
   for (int m = 0; m < M; ++m)
 #pragma unroll
@@ -550,8 +550,8 @@ struct Tokens {
   }
 };
 
-template <bool FP8, int M, int P>
-__device__ __forceinline__ void multiply(f4 (&acc)[M][1], Weights<FP8, M>& w, const Tokens<FP8, P>& x) {
+template <bool FP8, bool STREAM, int M, int P>
+__device__ __forceinline__ void multiply(f4 (&acc)[M][1], Weights<FP8, STREAM, M>& w, const Tokens<FP8, P>& x) {
   w.settle();
   f4 sum[M][1];
   if constexpr (FP8) clear<FP8, M, 1>(sum);
@@ -566,18 +566,18 @@ __device__ __forceinline__ void multiply(f4 (&acc)[M][1], Weights<FP8, M>& w, co
         s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(row, __builtin_bit_cast(bf8, x.b[p][q]), s, 0, 0, 0);
       }
     }
-  if constexpr (FP8) join_step<FP8, M, 1>(acc, sum, w);
+  if constexpr (FP8) join_step<FP8, STREAM, M, 1>(acc, sum, w);
 }
 
 // acc += rows[.., steps first : end : step of K] times the tokens; the loads of the next step go out before a step's
 // products.
-template <bool FP8, int M, int P>
+template <bool FP8, bool STREAM, int M, int P>
 __device__ __forceinline__ void sum_steps(f4 (&acc)[M][1], const __amdgpu_buffer_rsrc_t (&rows)[M][2],
                                           const floats_at (&scales)[M], const __amdgpu_buffer_rsrc_t (&parts)[P], uint32_t token, int K, int first, int end,
                                           int step) {
   if (first >= end) return;
   const uint32_t mine = offset_in_rows<FP8>(K);
-  Weights<FP8, M> w, next;
+  Weights<FP8, STREAM, M> w, next;
   Tokens<FP8, P> x, ahead;
   w.load(rows, mine, scales, first, K);
   x.load(parts, token, first, K);
@@ -587,17 +587,17 @@ __device__ __forceinline__ void sum_steps(f4 (&acc)[M][1], const __amdgpu_buffer
       next.load(rows, mine, scales, b1, K);
       ahead.load(parts, token, b1, K);
     }
-    multiply<FP8, M, P>(acc, w, x);
+    multiply<FP8, STREAM, M, P>(acc, w, x);
     if (b1 >= end) break;
     if (b2 < end) {
       w.load(rows, mine, scales, b2, K);
       x.load(parts, token, b2, K);
     }
-    multiply<FP8, M, P>(acc, next, ahead);
+    multiply<FP8, STREAM, M, P>(acc, next, ahead);
   }
 }
 
-template <int DT, bool FP8, bool UP>
+template <int DT, bool FP8, bool UP, bool STREAM>
 __global__ __launch_bounds__(64 * kFewWaves) void k_few(LayerArgs a) {
   constexpr int P = UP ? kXParts<DT> : kHParts<DT>, ROWS = UP ? 16 : 32;
   __shared__ OneUnit<64 * kFewWaves, kFewTokens, kFewTokens * kMaxTopK> plan;
@@ -634,7 +634,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_few(LayerArgs a) {
   const uint32_t token = r < n ? (uint32_t)(UP && !shared ? at / a.k : at) * (uint32_t)pitch * 2 : kNothing;
   f4 acc[2][1];
   clear<FP8, 2, 1>(acc);
-  sum_steps<FP8, 2, P>(acc, rows, scales, parts, token, K, uniform(wave), KB, kFewWaves);
+  sum_steps<FP8, STREAM, 2, P>(acc, rows, scales, parts, token, K, uniform(wave), KB, kFewWaves);
 #pragma unroll
   for (int m = 0; m < 2; ++m) sum[wave][m][lane] = acc[m][0];
   __syncthreads();
@@ -663,7 +663,7 @@ constexpr int kTileRows = kTileWaves * (UP ? 16 : 32);
 
 using TilePlan = OneUnit<64 * kTileWaves, kUnitTokens, kMaxAssigned>;
 
-template <int DT, bool FP8, bool UP, int NC>
+template <int DT, bool FP8, bool UP, bool STREAM, int NC>
 __device__ __forceinline__ void tile_unit(const LayerArgs& a, const TilePlan& plan, uint16_t* lds, int expert, int tile, int first, int n,
                                           bool shared) {
   constexpr int P = UP ? kXParts<DT> : kHParts<DT>;
@@ -718,15 +718,17 @@ __device__ __forceinline__ void tile_unit(const LayerArgs& a, const TilePlan& pl
   const uint32_t mine = offset_in_rows<FP8>(K);
   // The weights of two steps are on their way while one is multiplied; the next step's tokens go out before the latter
   // of them, as loads are waited for in their order.  Two steps' tokens lie in LDS, so that a step has one barrier.
-  Weights<FP8, 2> w[3];
+  // (bf16 weights, of twice the bytes a step: one step's)
+  constexpr int kSteps = FP8 ? 2 : 1;
+  Weights<FP8, STREAM, 2> w[kSteps + 1];
   fetch(0);
   w[0].load(rows, mine, scales, 0, K);
-  w[1].load(rows, mine, scales, 1, K);  // (past the end: zeros)
+  if constexpr (kSteps == 2) w[1].load(rows, mine, scales, 1, K);  // (past the end: zeros)
   leave(0);
   __syncthreads();
-  auto one_step = [&](int b, Weights<FP8, 2>& now, Weights<FP8, 2>& later) {
+  auto one_step = [&](int b, Weights<FP8, STREAM, 2>& now, Weights<FP8, STREAM, 2>& later) {
     fetch(b + 1);
-    later.load(rows, mine, scales, b + 2, K);
+    later.load(rows, mine, scales, b + kSteps, K);
     if (active) {
       now.settle();
       const uint16_t* tile_b = lds + (b & 1) * kTokenStep<P, NC>;
@@ -747,17 +749,19 @@ __device__ __forceinline__ void tile_unit(const LayerArgs& a, const TilePlan& pl
             }
           }
       }
-      if constexpr (FP8) join_step<FP8, 2, NC>(acc, sum, now);
+      if constexpr (FP8) join_step<FP8, STREAM, 2, NC>(acc, sum, now);
     }
     leave(b + 1);
     __syncthreads();
   };
-  for (int b = 0; b < KB; b += 3) {
-    one_step(b, w[0], w[2]);
+  for (int b = 0; b < KB; b += kSteps + 1) {
+    one_step(b, w[0], w[kSteps]);
     if (b + 1 >= KB) break;
     one_step(b + 1, w[1], w[0]);
-    if (b + 2 >= KB) break;
-    one_step(b + 2, w[2], w[1]);
+    if constexpr (kSteps == 2) {
+      if (b + 2 >= KB) break;
+      one_step(b + 2, w[2], w[1]);
+    }
   }
   if (!active) return;
 #pragma unroll
@@ -770,8 +774,8 @@ __device__ __forceinline__ void tile_unit(const LayerArgs& a, const TilePlan& pl
 }
 
 // The units of a tile are neighbours: those of one expert read its weights at the same time, from the cache.
-template <int DT, bool FP8, bool UP>
-__global__ __launch_bounds__(64 * kTileWaves, !FP8 ? 2 : UP && DT == CIN_DT_BF16 ? 4 : 3) void k_products(LayerArgs a) {
+template <int DT, bool FP8, bool UP, bool STREAM>
+__global__ __launch_bounds__(64 * kTileWaves, FP8 && UP && DT == CIN_DT_BF16 ? 4 : 3) void k_products(LayerArgs a) {
   constexpr int UNIT = kUnitTokens, ROWS = kTileRows<UP>;
   __shared__ TilePlan plan;
   extern __shared__ u4 tokens[];  // [parts, columns][kTokenPitch] of 16 bits
@@ -793,9 +797,9 @@ __global__ __launch_bounds__(64 * kTileWaves, !FP8 ? 2 : UP && DT == CIN_DT_BF16
   }
   uint16_t* lds = reinterpret_cast<uint16_t*>(tokens);
   if (n <= 16)
-    tile_unit<DT, FP8, UP, 1>(a, plan, lds, expert, tile, first, n, shared);
+    tile_unit<DT, FP8, UP, STREAM, 1>(a, plan, lds, expert, tile, first, n, shared);
   else
-    tile_unit<DT, FP8, UP, UNIT / 16>(a, plan, lds, expert, tile, first, n, shared);
+    tile_unit<DT, FP8, UP, STREAM, UNIT / 16>(a, plan, lds, expert, tile, first, n, shared);
 }
 
 // out = the sum of a token's rows of y, in the order of its experts, the shared one's last.
@@ -877,7 +881,7 @@ bool splits_k(const LayerArgs& a, bool up) {
   return a.T <= kFewTokens && 2 * groups < 3 * cin_device_cus();
 }
 
-template <int DT, bool FP8, bool UP>
+template <int DT, bool FP8, bool UP, bool STREAM>
 void launch_products(const LayerArgs& a, hipStream_t stream) {
   const bool few = splits_k(a, UP);
   const int64_t rows = few ? (UP ? 16 : 32) : kTileRows<UP>, units = few ? 1 : cdiv(a.T, kUnitTokens);
@@ -885,18 +889,32 @@ void launch_products(const LayerArgs& a, hipStream_t stream) {
   const int64_t shared = a.shared.H ? units * cdiv(UP ? a.shared.H : a.D, rows) : 0;
   const dim3 grid((uint32_t)(routed + shared));
   if (few) {
-    hipLaunchKernelGGL((k_few<DT, FP8, UP>), grid, dim3(64 * kFewWaves), 0, stream, a);
+    hipLaunchKernelGGL((k_few<DT, FP8, UP, STREAM>), grid, dim3(64 * kFewWaves), 0, stream, a);
   } else {
     constexpr int P = UP ? kXParts<DT> : kHParts<DT>;
     const size_t lds = 2 * sizeof(uint16_t) * kTokenStep<P, kUnitTokens / 16>;
-    hipLaunchKernelGGL((k_products<DT, FP8, UP>), grid, dim3(64 * kTileWaves), lds, stream, a);
+    hipLaunchKernelGGL((k_products<DT, FP8, UP, STREAM>), grid, dim3(64 * kTileWaves), lds, stream, a);
   }
+}
+
+// Rows that begin on lines of 128 bytes are streamed: a load takes whole lines, and none need be kept.  Else a line's
+// parts are of two steps (17 tokens, rows of 7152 codes: streamed 419 us a call, kept 341; 64 tokens, rows of 7168: 323 and 336).
+template <int DT, bool FP8, bool UP>
+void launch_products(const LayerArgs& a, bool on_lines, hipStream_t stream) {
+  constexpr int line = FP8 ? 128 : 64;
+  const bool whole = UP ? a.D % line == 0 : a.experts.H % line == 0 && a.shared.H % line == 0;
+  if (on_lines && whole)
+    launch_products<DT, FP8, UP, true>(a, stream);
+  else
+    launch_products<DT, FP8, UP, false>(a, stream);
 }
 
 template <int DT, bool FP8>
 void launch_experts(const LayerArgs& a, hipStream_t stream) {
-  launch_products<DT, FP8, true>(a, stream);
-  launch_products<DT, FP8, false>(a, stream);
+  const bool on_lines =
+      ((uintptr_t)a.experts.w12 | (uintptr_t)a.experts.w3 | (uintptr_t)a.shared.w12 | (uintptr_t)a.shared.w3) % 128 == 0;
+  launch_products<DT, FP8, true>(a, on_lines, stream);
+  launch_products<DT, FP8, false>(a, on_lines, stream);
   hipLaunchKernelGGL((k_join<DT>), dim3((a.T * (a.D / 4) + 255) / 256), dim3(256), 0, stream, a);
 }
 
