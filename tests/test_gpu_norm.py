@@ -267,8 +267,9 @@ def test_offsets_past_32_bits(dev):
 
 
 @pytest.mark.gpu
-def test_another_stream_and_a_graph(dev):
-    s, value, gn, gx = inputs(dev, (130, 1536), "bf16", "bf16", "fp32", True, "channel", "value")
+@pytest.mark.parametrize("shape,scale", [((130, 1536), "value"), ((9, 8192), "channel"), ((70, 256), "channel")])
+def test_another_stream_and_a_graph(dev, shape, scale):
+    s, value, gn, gx = inputs(dev, shape, "bf16", "bf16", "fp32", True, "channel", scale)
     leaves = {k: t.clone().requires_grad_() for k, t in s.items()}
     n, x = call(leaves, value)
     eager = torch.autograd.grad([n, x], list(leaves.values()), [gn, gx], retain_graph=True)
@@ -280,12 +281,15 @@ def test_another_stream_and_a_graph(dev):
         on_side = torch.autograd.grad([n2, x2], list(held.values()), [gn, gx])
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(n, n2) and all(torch.equal(a, b) for a, b in zip(eager, on_side))
+    # (leaves that no eager graph holds any more: torch cannot capture a backward through such)
+    held = {k: t.clone().requires_grad_() for k, t in s.items()}
+    torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         n3, x3 = call(held, value)
         captured = torch.autograd.grad([n3, x3], list(held.values()), [gn, gx])
     for seed in range(3):
-        fresh, _, _, _ = inputs(dev, (130, 1536), "bf16", "bf16", "fp32", True, "channel", "value", seed=seed)
+        fresh, _, _, _ = inputs(dev, shape, "bf16", "bf16", "fp32", True, "channel", scale, seed=seed)
         with torch.no_grad():
             for k in held:
                 held[k].copy_(fresh[k])
