@@ -41,8 +41,8 @@ constexpr int kMaxTopK = 16;
 constexpr int kMaxGroups = 64;
 constexpr int kBlock = 128;        // of a scale, and a step of K
 constexpr int kMaxAssigned = kMaxTokens * kMaxTopK;
-constexpr int kUnitTokens = 32;    // of an expert, multiplied at once
-constexpr int kRouterSlice = 512;  // channels of a k_router workgroup
+constexpr int kUnitTokens = 32;    // of an expert, multiplied at once, or twice as many (unit_tokens)
+constexpr int kRouterSlice = 256;  // channels of a k_router workgroup
 constexpr int kFewWaves = 4, kTileWaves = 4;
 constexpr int kFewTokens = 16;
 
@@ -83,7 +83,7 @@ struct LayerArgs {
   int slices;
   uint16_t *xb, *hb, *hs;  // parts of x [P, T, Dp], of h [P, T k, H], of the shared expert's [P, T, Hs]
   float* y;                // the experts' outputs [T k, D], the shared one's [T, D]
-  int units;               // the most that the routed experts can have
+  int unit, units;         // tokens of a unit, and the most units that the routed experts can have
 };
 
 // Scales, the same for all lanes and nowhere written here: scalar loads.
@@ -661,10 +661,11 @@ constexpr int kTokenStep = P * NC * 16 * kTokenPitch;
 template <bool UP>
 constexpr int kTileRows = kTileWaves * (UP ? 16 : 32);
 
-using TilePlan = OneUnit<64 * kTileWaves, kUnitTokens, kMaxAssigned>;
+template <int UNIT>
+using TilePlan = OneUnit<64 * kTileWaves, UNIT, kMaxAssigned>;
 
-template <int DT, bool FP8, bool UP, bool STREAM, int NC>
-__device__ __forceinline__ void tile_unit(const LayerArgs& a, const TilePlan& plan, uint16_t* lds, int expert, int tile, int first, int n,
+template <int DT, bool FP8, bool UP, bool STREAM, int NC, class Plan>
+__device__ __forceinline__ void tile_unit(const LayerArgs& a, const Plan& plan, uint16_t* lds, int expert, int tile, int first, int n,
                                           bool shared) {
   constexpr int P = UP ? kXParts<DT> : kHParts<DT>;
   constexpr int kChunks = NC * 16 * P * (kBlock / 8), kThreads = 64 * kTileWaves;  // of 16 bytes, a step
@@ -774,10 +775,10 @@ __device__ __forceinline__ void tile_unit(const LayerArgs& a, const TilePlan& pl
 }
 
 // The units of a tile are neighbours: those of one expert read its weights at the same time, from the cache.
-template <int DT, bool FP8, bool UP, bool STREAM>
-__global__ __launch_bounds__(64 * kTileWaves, FP8 && UP && DT == CIN_DT_BF16 ? 4 : 3) void k_products(LayerArgs a) {
-  constexpr int UNIT = kUnitTokens, ROWS = kTileRows<UP>;
-  __shared__ TilePlan plan;
+template <int DT, bool FP8, bool UP, bool STREAM, int UNIT>
+__global__ __launch_bounds__(64 * kTileWaves, UNIT > kUnitTokens ? 2 : FP8 && UP && DT == CIN_DT_BF16 ? 4 : 3) void k_products(LayerArgs a) {
+  constexpr int ROWS = kTileRows<UP>;
+  __shared__ TilePlan<UNIT> plan;
   extern __shared__ u4 tokens[];  // [parts, columns][kTokenPitch] of 16 bits
   const int tiles = ((UP ? a.experts.H : a.D) + ROWS - 1) / ROWS, routed = a.units * tiles;
   const bool shared = (int)blockIdx.x >= routed;
@@ -798,6 +799,8 @@ __global__ __launch_bounds__(64 * kTileWaves, FP8 && UP && DT == CIN_DT_BF16 ? 4
   uint16_t* lds = reinterpret_cast<uint16_t*>(tokens);
   if (n <= 16)
     tile_unit<DT, FP8, UP, STREAM, 1>(a, plan, lds, expert, tile, first, n, shared);
+  else if (UNIT == 32 || n <= 32)
+    tile_unit<DT, FP8, UP, STREAM, 2>(a, plan, lds, expert, tile, first, n, shared);
   else
     tile_unit<DT, FP8, UP, STREAM, UNIT / 16>(a, plan, lds, expert, tile, first, n, shared);
 }
@@ -859,7 +862,15 @@ bool sizes_ok(int dtype, int64_t T, int64_t D, int64_t E, int64_t k, int64_t H, 
 const char* const kSizes =
     "dtype must be bf16, fp16 or fp32, T <= 128, E <= 1024, k <= min(16, E), D, H and the shared expert's H multiples of 16 up to 65536";
 
-void set_sizes(LayerArgs& a, int64_t T, int64_t D, int64_t E, int64_t k, int64_t H, int64_t Hs) {
+// Tokens of a unit.  A second unit of an expert reads its weights again, from the cache at best; more tokens at once
+// cost the registers of a third workgroup a CU, and with fp32's parts the LDS of a second.  8 of 32 experts of 7168 x 2048:
+// 80 tokens with units of 32 335 us, of 64 386; 96 393 and 392; 112 445 and 404; 96 tokens, 6 of 8 experts 264 and 199; 96
+// fp32 tokens 520 and 722.
+int64_t unit_tokens(int dtype, int64_t T, int64_t E, int64_t k) {
+  return dtype != CIN_DT_F32 && T > kUnitTokens && T * k > 24 * E ? 2 * kUnitTokens : kUnitTokens;
+}
+
+void set_sizes(LayerArgs& a, int dtype, int64_t T, int64_t D, int64_t E, int64_t k, int64_t H, int64_t Hs) {
   a.T = (int)T;
   a.D = (int)D;
   a.Dp = (int)(cdiv(D, kBlock) * kBlock);
@@ -869,7 +880,8 @@ void set_sizes(LayerArgs& a, int64_t T, int64_t D, int64_t E, int64_t k, int64_t
   a.shared.H = (int)Hs;
   a.slices = (int)cdiv(a.Dp, kRouterSlice);
   const int64_t n = T * k;
-  a.units = (int)((n < E ? n : E) + n / kUnitTokens);
+  a.unit = (int)unit_tokens(dtype, T, E, k);
+  a.units = (int)((n < E ? n : E) + n / a.unit);
 }
 
 // Whether the waves share K: where k_products would have fewer than one and a half workgroups a CU.  One token, 8 of 32 experts
@@ -882,18 +894,32 @@ bool splits_k(const LayerArgs& a, bool up) {
 }
 
 template <int DT, bool FP8, bool UP, bool STREAM>
+void launch_tiles(const LayerArgs& a, dim3 grid, hipStream_t stream) {
+  constexpr int P = UP ? kXParts<DT> : kHParts<DT>;
+  const size_t lds = 2 * sizeof(uint16_t) * kTokenStep<P, kUnitTokens / 16>;
+  if (DT == CIN_DT_F32 || a.unit == kUnitTokens) {
+    hipLaunchKernelGGL((k_products<DT, FP8, UP, STREAM, kUnitTokens>), grid, dim3(64 * kTileWaves), lds, stream, a);
+    return;
+  }
+  if constexpr (DT != CIN_DT_F32) {
+    auto kernel = k_products<DT, FP8, UP, STREAM, 2 * kUnitTokens>;
+    if (2 * lds + sizeof(TilePlan<2 * kUnitTokens>) > 65536)
+      (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)(2 * lds));
+    hipLaunchKernelGGL(kernel, grid, dim3(64 * kTileWaves), 2 * lds, stream, a);
+  }
+}
+
+template <int DT, bool FP8, bool UP, bool STREAM>
 void launch_products(const LayerArgs& a, hipStream_t stream) {
   const bool few = splits_k(a, UP);
-  const int64_t rows = few ? (UP ? 16 : 32) : kTileRows<UP>, units = few ? 1 : cdiv(a.T, kUnitTokens);
+  const int64_t rows = few ? (UP ? 16 : 32) : kTileRows<UP>, units = few ? 1 : cdiv(a.T, a.unit);
   const int64_t routed = a.units * cdiv(UP ? a.experts.H : a.D, rows);
   const int64_t shared = a.shared.H ? units * cdiv(UP ? a.shared.H : a.D, rows) : 0;
   const dim3 grid((uint32_t)(routed + shared));
   if (few) {
     hipLaunchKernelGGL((k_few<DT, FP8, UP, STREAM>), grid, dim3(64 * kFewWaves), 0, stream, a);
   } else {
-    constexpr int P = UP ? kXParts<DT> : kHParts<DT>;
-    const size_t lds = 2 * sizeof(uint16_t) * kTokenStep<P, kUnitTokens / 16>;
-    hipLaunchKernelGGL((k_products<DT, FP8, UP, STREAM>), grid, dim3(64 * kTileWaves), lds, stream, a);
+    launch_tiles<DT, FP8, UP, STREAM>(a, grid, stream);
   }
 }
 
@@ -938,7 +964,7 @@ int64_t cin_moe_decode_workspace(int dtype, int64_t T, int64_t D, int64_t E, int
     return -1;
   }
   LayerArgs a = {};
-  set_sizes(a, T, D, E, k, H, shared_H);
+  set_sizes(a, dtype, T, D, E, k, H, shared_H);
   return layout(a, dtype, nullptr);
 }
 
@@ -966,7 +992,7 @@ int cin_moe_decode(const void* x, int dtype, int64_t ldx, int64_t T, int64_t D, 
   CIN_CHECK_ARG(workspace_bytes >= cin_moe_decode_workspace(dtype, T, D, E, k, H, shared_H),
                 "cin_moe_decode: workspace below cin_moe_decode_workspace bytes");
   LayerArgs a = {};
-  set_sizes(a, T, D, E, k, H, shared_H);
+  set_sizes(a, dtype, T, D, E, k, H, shared_H);
   layout(a, dtype, static_cast<char*>(workspace));
   a.x = x;
   a.ldx = ldx;
