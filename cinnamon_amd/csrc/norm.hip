@@ -19,7 +19,9 @@
 // A row is read once into registers, 8 channels a thread and chunk, by one wave (up to 1024 channels, the
 // sums by DPP and swaps, no barrier) or by one workgroup.  Workgroups walk over rows, so that the channels'
 // vectors are loaded once and a channel's sums over the rows stay in registers; each workgroup leaves one
-// row of partial sums, which k_norm_columns adds up in a fixed order.  Bound by HBM.
+// row of partial sums, which k_norm_columns adds up in a fixed order.  Bound by HBM: 8192 x 7168 bf16 with post norm,
+// gate and learned scale a channel, forward 175 us (470 MB, 2.7 TB/s; 97 us for 16384 x 4096, 5.5 TB/s without these),
+// backward 305 us (705 MB in, 235 out); 8192 x 1000 bf16 with an fp32 stream 34 and 54 us.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -31,8 +33,8 @@ using namespace cin;
 namespace {
 
 constexpr int kMaxThreads = 512;
-constexpr int kMaxChunks = 4;
-constexpr int64_t kMaxWidth = (int64_t)kMaxThreads * kMaxChunks * 8;
+constexpr int kWideThreads = 1024;  // of the backward past 8192 channels
+constexpr int64_t kMaxWidth = kWideThreads * 2 * 8;
 constexpr int kWaveRows = 4;  // rows at a time of a workgroup whose waves take a row each
 
 enum Gate { kNoGate = 0, kChannel = 1, kRow = 2, kElement = 3 };
@@ -214,7 +216,7 @@ __device__ __forceinline__ float wave_sum(float v) {
 // each passes a barrier.
 template <bool WAVE, int N>
 struct RowSum {
-  float (*lds)[N][kMaxThreads / 64];  // [2]
+  float (*lds)[N][kWideThreads / 64];  // [2]
   int turn = 0;
   __device__ __forceinline__ void operator()(float (&v)[N], int waves) {
 #pragma unroll
@@ -253,7 +255,7 @@ struct Span {
 // FULL: with post norm, gate or learned scale; else x = scale_value r + y.  WAVE: a row a wave.
 template <int DT, int DR, int CH, bool WAVE, bool FULL>
 __global__ __launch_bounds__(WAVE ? 64 * kWaveRows : kMaxThreads) void k_norm_forward(NormArgs a) {
-  __shared__ float lds[2][1][kMaxThreads / 64];
+  __shared__ float lds[2][1][kWideThreads / 64];
   RowSum<WAVE, 1> sum{lds};
   const int lane = WAVE ? threadIdx.x & 63 : threadIdx.x;
   const int waves = blockDim.x >> 6;
@@ -438,19 +440,25 @@ struct Slots {
 
 // FULL keeps the channels' vectors in LDS between the rows (w, g pw and the scale, up to 8192 channels of each) and the
 // scale's sums too: in registers they would cost the next row's loads, and read again from L2 they would have to
-// be waited for behind those.
-template <int CH>
-constexpr bool kVectorsInLds = CH <= 2;
-template <int CH, bool WAVE>
+// be waited for behind those.  WIDE, of more channels, has 1024 threads, no room for the vectors in LDS nor for the next
+// row in registers: it reads the vectors again, from L2, and its sums spill (4096 x 16384 bf16, gate a channel: 566 us;
+// 745 with 512 threads of four chunks).
+template <int CH, bool WAVE, bool WIDE>
 size_t backward_lds(bool scale_channels, int block) {
   const size_t row = (WAVE ? 64 : block) * CH * 32, own = (size_t)block * CH * 32;
-  return (kVectorsInLds<CH> ? (scale_channels ? 3 : 2) * row : 0) + (scale_channels ? own : 0);
+  return (WIDE ? 0 : (scale_channels ? 3 : 2) * row) + (scale_channels ? own : 0);
 }
 
-template <int DT, int DR, int CH, bool WAVE, Mode MODE>
-__global__ __launch_bounds__(WAVE ? 64 * kWaveRows : kMaxThreads) void k_norm_backward(NormArgs a) {
+// Waves a SIMD that the registers are kept to: up to 4096 channels a workgroup is small, and others cover its waits
+// (4999 x 1111 fp16, gate per element: 49 us with three, 66 with two).
+template <int CH, bool WAVE, Mode MODE>
+constexpr int kBackwardWaves = WAVE || CH > 1 ? 1 : MODE == kAny ? 3 : 4;
+
+template <int DT, int DR, int CH, bool WAVE, bool WIDE, Mode MODE>
+__global__ __launch_bounds__(WAVE ? 64 * kWaveRows : WIDE ? kWideThreads : kMaxThreads, (kBackwardWaves<CH, WAVE, MODE>))
+void k_norm_backward(NormArgs a) {
   constexpr bool FULL = MODE != kPlain;
-  __shared__ float lds1[2][1][kMaxThreads / 64], lds2[2][2][kMaxThreads / 64];
+  __shared__ float lds1[2][1][kWideThreads / 64], lds2[2][2][kWideThreads / 64];
   __shared__ float joined[WAVE ? kWaveRows * 64 * CH * 8 : 1];
   extern __shared__ float4 slots[];
   RowSum<WAVE, 1> sum1{lds1};
@@ -462,35 +470,35 @@ __global__ __launch_bounds__(WAVE ? 64 * kWaveRows : kMaxThreads) void k_norm_ba
   Span<CH> s;
   s.set(lane, a.threads, a.D);
   const bool scale_channels = FULL && a.scale_kind == kPerChannel;
-  constexpr bool kInLds = FULL && kVectorsInLds<CH>;
-  constexpr int R = kInLds ? 1 : CH;
+  constexpr bool kInLds = FULL && !WIDE, kInRegisters = !FULL && !WIDE;
   const Slots vectors{slots, WAVE ? 64 : (int)blockDim.x, lane, CH};
   const Slots scale_sums{slots + (kInLds ? 6 * CH * vectors.threads : 0), (int)blockDim.x, (int)threadIdx.x, CH};
-  float w[R][8], gp[FULL ? R : 1][8], value = a.scale_value;
+  float w[kInRegisters ? CH : 1][8], value = a.scale_value;
   float sw[CH][8], su[FULL ? CH : 1][8];
   double sone = 0.0;  // over all channels of all rows: in fp32 it would lose half its digits
   const float inv_d = 1.0f / (float)a.D;
   if (FULL && a.scale_kind == kOneValue) value = load_elem(a.scale.p, a.scale.dtype, 0);
+  auto load_products = [&](int c, float (&v)[8]) {  // g pw
+    float g[8];
+    load_channels(a.pw, s.at[c], s.cnt[c], 1.0f, v);
+    load_channels(a.gate_kind == kChannel ? a.gate : Vec{nullptr, 0}, s.at[c], s.cnt[c], 1.0f, g);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] *= g[e];
+  };
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
     float v[8];
-    load_channels(a.w, s.at[c], s.cnt[c], 1.0f, v);
+    if constexpr (!WIDE) load_channels(a.w, s.at[c], s.cnt[c], 1.0f, v);
     if constexpr (kInLds) vectors.set(0, c, v);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      if constexpr (!kInLds) w[c][e] = v[e];
+      if constexpr (kInRegisters) w[c][e] = v[e];
       sw[c][e] = 0.0f;
     }
     if constexpr (FULL) {
-      float g[8];
-      load_channels(a.pw, s.at[c], s.cnt[c], 1.0f, v);
-      load_channels(a.gate_kind == kChannel ? a.gate : Vec{nullptr, 0}, s.at[c], s.cnt[c], 1.0f, g);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        v[e] *= g[e];
-        if constexpr (!kInLds) gp[c][e] = v[e];
-        su[c][e] = 0.0f;
-      }
+      for (int e = 0; e < 8; ++e) su[c][e] = 0.0f;
+      if constexpr (kInLds) load_products(c, v);
       if constexpr (kInLds) vectors.set(1, c, v);
       if (scale_channels) {
         load_channels(a.scale, s.at[c], s.cnt[c], 0.0f, v);
@@ -504,18 +512,18 @@ __global__ __launch_bounds__(WAVE ? 64 * kWaveRows : kMaxThreads) void k_norm_ba
   auto weights = [&](int c, float (&v)[8]) {
     if constexpr (kInLds) {
       vectors.get(0, c, v);
+    } else if constexpr (WIDE) {
+      load_channels(a.w, s.at[c], s.cnt[c], 1.0f, v);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = w[c][e];
     }
   };
-  auto products = [&](int c, float (&v)[8]) {  // g pw
-    if constexpr (kInLds) {
+  auto products = [&](int c, float (&v)[8]) {
+    if constexpr (kInLds)
       vectors.get(1, c, v);
-    } else if constexpr (FULL) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = gp[c][e];
-    }
+    else if constexpr (FULL)
+      load_products(c, v);
   };
   auto scales = [&](int c, float (&v)[8]) {
     if (!scale_channels) {
@@ -529,7 +537,7 @@ __global__ __launch_bounds__(WAVE ? 64 * kWaveRows : kMaxThreads) void k_norm_ba
   };
   // A workgroup's waves wait for each other twice a row, so the next row's loads go out before; waves with rows
   // of their own cover each other's (and fp32 rows are as many bytes without).
-  constexpr bool kAhead = !WAVE && CH <= 2 && DR != CIN_DT_F32;
+  constexpr bool kAhead = !WAVE && !WIDE && DR != CIN_DT_F32;
   const bool post = FULL && a.pw.p, gated = MODE == kAny && (a.gate_kind == kRow || a.gate_kind == kElement);
   const bool inner = FULL && (a.pw.p || a.gate_kind == kChannel);  // S is summed
   using In = RowIn<DT, DR, CH, MODE == kAny>;
@@ -664,7 +672,7 @@ __global__ __launch_bounds__(WAVE ? 64 * kWaveRows : kMaxThreads) void k_norm_ba
       leave_partial<CH, WAVE>(a, kSumScale, sw, s, joined);
     }
     if (a.scale_kind == kOneValue) {
-      __shared__ double ones[kMaxThreads / 64];
+      __shared__ double ones[kWideThreads / 64];
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) sone += __shfl_xor(sone, o);
       if ((threadIdx.x & 63) == 0) ones[threadIdx.x >> 6] = sone;
@@ -740,14 +748,15 @@ __global__ __launch_bounds__(1024) void k_norm_columns(ColumnArgs a) {
 // Chunks of a thread, threads of a row and whether a wave takes a row.
 struct Shape {
   int chunks, threads;
-  bool wave;
+  bool wave, wide;
 };
-Shape shape_of(int64_t D) {
+Shape shape_of(int64_t D, bool backward) {
   const int64_t units = cdiv(D, 8);
-  if (units <= 64) return {1, 64, true};
-  if (units <= 128) return {2, 64, true};
-  const int chunks = units <= kMaxThreads ? 1 : units <= 2 * kMaxThreads ? 2 : 4;
-  return {chunks, (int)(cdiv(cdiv(units, chunks), 64) * 64), false};
+  if (units <= 64) return {1, 64, true, false};
+  if (units <= 128) return {2, 64, true, false};
+  const bool wide = backward && units > 2 * kMaxThreads;
+  const int chunks = units <= kMaxThreads ? 1 : units <= 2 * kMaxThreads || wide ? 2 : 4;
+  return {chunks, (int)(cdiv(cdiv(units, chunks), 64) * 64), false, wide};
 }
 
 // Workgroups that walk over the rows.
@@ -764,42 +773,57 @@ void allow_lds(K kernel, size_t bytes) {
   if (bytes > 65536) (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
 }
 
-template <int DT, int DR, int CH, bool WAVE, Mode MODE>
-void launch_backward(const NormArgs& a, dim3 grid, dim3 block, hipStream_t stream) {
-  const size_t lds = MODE == kPlain ? 0 : backward_lds<CH, WAVE>(a.scale_kind == kPerChannel, (int)block.x);
-  allow_lds(k_norm_backward<DT, DR, CH, WAVE, MODE>, lds);
-  hipLaunchKernelGGL((k_norm_backward<DT, DR, CH, WAVE, MODE>), grid, block, lds, stream, a);
+template <int DT, int DR, int CH, bool WAVE, bool WIDE, Mode MODE>
+void launch_mode(const NormArgs& a, dim3 grid, dim3 block, hipStream_t stream) {
+  const size_t lds = MODE == kPlain ? 0 : backward_lds<CH, WAVE, WIDE>(a.scale_kind == kPerChannel, (int)block.x);
+  allow_lds(k_norm_backward<DT, DR, CH, WAVE, WIDE, MODE>, lds);
+  hipLaunchKernelGGL((k_norm_backward<DT, DR, CH, WAVE, WIDE, MODE>), grid, block, lds, stream, a);
+}
+
+template <int DT, int DR, int CH, bool WAVE, bool WIDE>
+void launch_backward(const NormArgs& a, const Shape& s, int64_t groups, bool full, hipStream_t stream) {
+  const dim3 grid((uint32_t)groups), block(s.wave ? 64 * kWaveRows : s.threads);
+  if (!full)
+    launch_mode<DT, DR, CH, WAVE, WIDE, kPlain>(a, grid, block, stream);
+  else if (a.gate_kind == kRow || a.gate_kind == kElement)
+    launch_mode<DT, DR, CH, WAVE, WIDE, kAny>(a, grid, block, stream);
+  else
+    launch_mode<DT, DR, CH, WAVE, WIDE, kChannels>(a, grid, block, stream);
 }
 
 template <int DT, int DR, int CH, bool WAVE>
-void launch(const NormArgs& a, const Shape& s, int64_t groups, bool full, bool backward, hipStream_t stream) {
+void launch_forward(const NormArgs& a, const Shape& s, int64_t groups, bool full, hipStream_t stream) {
   const dim3 grid((uint32_t)groups), block(s.wave ? 64 * kWaveRows : s.threads);
-  if (!backward) {
-    if (full)
-      hipLaunchKernelGGL((k_norm_forward<DT, DR, CH, WAVE, true>), grid, block, 0, stream, a);
-    else
-      hipLaunchKernelGGL((k_norm_forward<DT, DR, CH, WAVE, false>), grid, block, 0, stream, a);
-  } else if (!full) {
-    launch_backward<DT, DR, CH, WAVE, kPlain>(a, grid, block, stream);
-  } else if (a.gate_kind == kRow || a.gate_kind == kElement) {
-    launch_backward<DT, DR, CH, WAVE, kAny>(a, grid, block, stream);
-  } else {
-    launch_backward<DT, DR, CH, WAVE, kChannels>(a, grid, block, stream);
-  }
+  if (full)
+    hipLaunchKernelGGL((k_norm_forward<DT, DR, CH, WAVE, true>), grid, block, 0, stream, a);
+  else
+    hipLaunchKernelGGL((k_norm_forward<DT, DR, CH, WAVE, false>), grid, block, 0, stream, a);
 }
 
 template <int DT, int DR>
 void launch_shape(const NormArgs& a, const Shape& s, int64_t groups, bool full, bool backward, hipStream_t stream) {
-  if (s.wave && s.chunks == 1)
-    launch<DT, DR, 1, true>(a, s, groups, full, backward, stream);
-  else if (s.wave)
-    launch<DT, DR, 2, true>(a, s, groups, full, backward, stream);
-  else if (s.chunks == 1)
-    launch<DT, DR, 1, false>(a, s, groups, full, backward, stream);
-  else if (s.chunks == 2)
-    launch<DT, DR, 2, false>(a, s, groups, full, backward, stream);
-  else
-    launch<DT, DR, 4, false>(a, s, groups, full, backward, stream);
+  if (!backward) {
+    if (s.wave && s.chunks == 1)
+      launch_forward<DT, DR, 1, true>(a, s, groups, full, stream);
+    else if (s.wave)
+      launch_forward<DT, DR, 2, true>(a, s, groups, full, stream);
+    else if (s.chunks == 1)
+      launch_forward<DT, DR, 1, false>(a, s, groups, full, stream);
+    else if (s.chunks == 2)
+      launch_forward<DT, DR, 2, false>(a, s, groups, full, stream);
+    else
+      launch_forward<DT, DR, 4, false>(a, s, groups, full, stream);
+  } else if (s.wave && s.chunks == 1) {
+    launch_backward<DT, DR, 1, true, false>(a, s, groups, full, stream);
+  } else if (s.wave) {
+    launch_backward<DT, DR, 2, true, false>(a, s, groups, full, stream);
+  } else if (s.wide) {
+    launch_backward<DT, DR, 2, false, true>(a, s, groups, full, stream);
+  } else if (s.chunks == 1) {
+    launch_backward<DT, DR, 1, false, false>(a, s, groups, full, stream);
+  } else {
+    launch_backward<DT, DR, 2, false, false>(a, s, groups, full, stream);
+  }
 }
 
 void launch_types(const NormArgs& a, int dt, int dr, const Shape& s, int64_t groups, bool full, bool backward,
@@ -874,7 +898,7 @@ int cin_block_norm(const void* y, int dtype, int64_t ldy, const void* r, int r_d
   a.n = n;
   a.x = x;
   a.stats = stats;
-  const Shape s = shape_of(D);
+  const Shape s = shape_of(D, false);
   a.threads = s.threads;
   launch_types(a, dtype, r_dtype, s, groups_of(T, s, false), is_full(a), false, (hipStream_t)stream);
   return cin_check_launch("cin_block_norm");
@@ -885,7 +909,7 @@ int64_t cin_block_norm_workspace(int64_t T, int64_t D) {
     cin_set_error(CIN_ERR_ARG, "cin_block_norm_workspace: D must be in [1, %lld]", (long long)kMaxWidth);
     return -1;
   }
-  const int64_t groups = groups_of(T, shape_of(D), true);
+  const int64_t groups = groups_of(T, shape_of(D, true), true);
   return 4 * ((kSums * groups * D + 1) / 2 * 2) + 8 * groups;
 }
 
@@ -928,7 +952,7 @@ int cin_block_norm_backward(const void* y, int dtype, int64_t ldy, const void* r
   a.dr = dr;
   a.dgate = dgate;
   a.partial = sums ? static_cast<float*>(workspace) : nullptr;
-  const Shape s = shape_of(D);
+  const Shape s = shape_of(D, true);
   a.threads = s.threads;
   const int64_t groups = groups_of(T, s, true);
   launch_types(a, dtype, r_dtype, s, groups, is_full(a), true, (hipStream_t)stream);
