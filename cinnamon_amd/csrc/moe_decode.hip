@@ -19,10 +19,15 @@
 // Five launches: k_router (logits by slices of D on the fp64 matrix units, and x's parts), k_gate (a workgroup a
 // token), the products up to h and down to each expert's output rows, and k_join (a token's rows in the order of top
 // k).  The products take a workgroup an expert's tokens and some of its rows:
-//   k_few, up to 16 tokens and where the others would leave CUs idle: 16 rows of W1 and W2, or 32 of W3, the waves sharing K;
+//   k_few, up to 16 tokens and where the others would leave CUs idle: 16 rows of W1 and W2, or 32 of W3, the waves
+//   sharing K;
 //   k_products: as many rows a wave; the tokens' parts go through LDS once for all waves, as they
 //   would be more bytes than the weights.
 // No atomics on results.
+//
+// Bound by the weights' bytes.  32 experts of 7168 x 2048 in codes, 8 a token, and a shared one: one token 84 us (0.40 GB,
+// 4.7 TB/s: up 47, down 23), 64 tokens 345 (1.46 GB, 4.2: up 204, down 125).  16 experts of 1024 x 1024, one token: 24, the
+// latency of five launches.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -406,9 +411,9 @@ __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirs
 // k_of(q, lane / 16) on.  Both operands take the same elements, so their order in a product does not matter.
 //
 // A load takes 8 rows' 128 adjacent bytes (lane: row lane % 8, 16 bytes from 16 (lane / 8) on), a whole line of each,
-// streamed past the caches where rows begin on lines: 969 MB of codes in rows of 7168 arrive at 6.2 TB/s, against 4.8 with 64 bytes of 16 rows a load
-// and 5.5 with those kept in the caches (linear reads: 7.0).  Two loads, of rows 0-7 and 8-15, then hold every lane's
-// two words, half of them in the lane 8 further in its row of 16: settle() swaps those.
+// streamed past the caches where rows begin on lines: 969 MB of codes in rows of 7168 arrive at 6.2 TB/s, against 4.8
+// with 64 bytes of 16 rows a load and 5.5 with those kept in the caches (linear reads: 7.0).  Two loads, of rows 0-7 and
+// 8-15, then hold every lane's two words, half of them in the lane 8 further in its row of 16: settle() swaps those.
 template <bool FP8>
 __device__ __forceinline__ constexpr int k_of(int q, int g) {
   return FP8 ? g * 32 + q * 8 : (q >> 1) * 64 + g * 16 + (q & 1) * 8;

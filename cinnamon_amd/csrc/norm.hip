@@ -19,9 +19,10 @@
 // A row is read once into registers, 8 channels a thread and chunk, by one wave (up to 1024 channels, the
 // sums by DPP and swaps, no barrier) or by one workgroup.  Workgroups walk over rows, so that the channels'
 // vectors are loaded once and a channel's sums over the rows stay in registers; each workgroup leaves one
-// row of partial sums, which k_norm_columns adds up in a fixed order.  Bound by HBM: 8192 x 7168 bf16 with post norm,
-// gate and learned scale a channel, forward 175 us (470 MB, 2.7 TB/s; 97 us for 16384 x 4096, 5.5 TB/s without these),
-// backward 305 us (705 MB in, 235 out); 8192 x 1000 bf16 with an fp32 stream 34 and 54 us.
+// row of partial sums, which k_norm_columns adds up in a fixed order.  Bound by HBM: 16384 x 7168 bf16 with post norm,
+// a gate and a learned scale, forward 175 us (0.94 GB, 5.4 TB/s), backward 300 (1.41 GB, 4.7); 16384 x 1024 bf16
+// with an fp32 stream 34 us (0.20 GB, 5.9) and 54 (0.30 GB, 5.6).  Rows of odd lengths lie on no 16 bytes: 4999 x 1111 fp16
+// with a gate an element 23 us (56 MB, 2.5) and 49 (89 MB, 1.8).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

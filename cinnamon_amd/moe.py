@@ -542,7 +542,8 @@ def moe_decode(x: torch.Tensor, router_weight: torch.Tensor, experts, top_k: int
                  "bias must be fp32 [n_experts] on x's device")
         bias = bias.detach()
     if isinstance(experts, layers.GroupedExperts):
-        _require(experts.n_experts == E, "the router and the experts differ in number")
+        _require(experts.n_experts == E and experts.d_model == D, "the router and the experts differ in number or width")
+        _require(D % 128 == 0 and experts.hidden_dim % 64 == 0, "GroupedExperts' FP8 blocks need D in multiples of 128, H of 64")
         w12, w3 = experts.w12.detach(), experts.w3.detach()
         H = experts.hidden_dim
         q = experts.quantized_weights()

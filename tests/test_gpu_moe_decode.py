@@ -359,6 +359,9 @@ def test_shapes_and_refusals():
                          ((x, r, e16, 2), {"group_top": 3}), ((x, r, e16, 2), {"n_groups": 2, "top_groups": 3})]:
             with pytest.raises(AssertionError):
                 moe.moe_decode(*args, **kw)
+        for sizes in [(7, 256, 128), (8, 128, 128), (8, 256, 96)]:  # the experts, the width, blocks of two experts
+            with pytest.raises(AssertionError):
+                moe.moe_decode(x, r, layers.GroupedExperts(*sizes), 2)
 
 
 def test_c_entry_refuses_bad_arguments():

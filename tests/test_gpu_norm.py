@@ -120,6 +120,15 @@ CASES = [
     ((600, 2048), "fp32", None, "fp32", False, "none", "one"),
     ((4, 130, 1536), "bf16", None, "fp32", False, "none", "one"),
     ((3000, 768), "fp16", "fp32", "fp32", False, "none", "one"),
+    # several rows a workgroup
+    ((5001, 1000), "bf16", "fp32", "fp32", True, "channel", "value"),
+    ((2700, 1111), "fp16", "fp16", "fp16", True, "element", "channel"),
+    ((1300, 4096), "bf16", "bf16", "fp32", True, "channel", "value"),
+    ((1100, 3001), "bf16", "fp32", "bf16", False, "row", "number"),
+    ((600, 6000), "bf16", "bf16", "fp32", True, "row", "channel"),
+    ((520, 12000), "bf16", "bf16", "fp32", True, "channel", "channel"),
+    ((515, 9001), "fp32", "fp32", "fp32", True, "element", "value"),
+    ((530, 16384), "fp16", "fp32", "fp32", False, "none", "one"),
 ]
 
 
