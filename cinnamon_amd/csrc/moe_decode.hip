@@ -17,16 +17,17 @@
 // the border of the top k differ by less than 32 bits hold.
 //
 // Five launches: k_router (logits by slices of D on the fp64 matrix units, and x's parts), k_gate (a workgroup a
-// token), the products up to h and down to each expert's output rows, and k_join (a token's rows in the order of top
-// k).  The products take a workgroup an expert's tokens and some of its rows:
+// token, and the shared expert's h where that is little work), the products up to h and down to each expert's output
+// rows, and k_join (a token's rows in the order of top k).  The products take a workgroup an expert's tokens and some
+// of its rows:
 //   k_few, up to 16 tokens and where the others would leave CUs idle: 16 rows of W1 and W2, or 32 of W3, the waves
 //   sharing K;
 //   k_products: as many rows a wave; the tokens' parts go through LDS once for all waves, as they
 //   would be more bytes than the weights.
 // No atomics on results.
 //
-// Bound by the weights' bytes.  32 experts of 7168 x 2048 in codes, 8 a token, and a shared one: one token 84 us (0.40 GB,
-// 4.7 TB/s: up 47, down 23), 64 tokens 345 (1.46 GB, 4.2: up 204, down 125).  16 experts of 1024 x 1024, one token: 24, the
+// Bound by the weights' bytes.  32 experts of 7168 x 2048 in codes, 8 a token, and a shared one: one token 80 us (0.40 GB,
+// 5.0 TB/s: up 39, down 23), 64 tokens 304 (1.46 GB, 4.8: up 163, down 120).  16 experts of 1024 x 1024, one token: 24, the
 // latency of five launches.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -185,6 +186,7 @@ __device__ inline double of_key(uint64_t k) {
   return __longlong_as_double((long long)(k >> 63 ? k & ~(1ull << 63) : ~k));
 }
 
+template <int WAVES>
 __device__ inline double block_reduce(double v, bool maximum, double* lds) {
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -194,21 +196,23 @@ __device__ inline double block_reduce(double v, bool maximum, double* lds) {
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
   __syncthreads();
   double r = lds[0];
-  for (int w = 1; w < 4; ++w) r = maximum ? (lds[w] > r || lds[w] != lds[w] ? lds[w] : r) : r + lds[w];
+  for (int w = 1; w < WAVES; ++w) r = maximum ? (lds[w] > r || lds[w] != lds[w] ? lds[w] : r) : r + lds[w];
   __syncthreads();
   return r;
 }
 
-__global__ __launch_bounds__(256) void k_gate(LayerArgs a) {
-  __shared__ double score[kMaxExperts], reduce[4];
+// A token's experts and weights, by one workgroup.
+template <int WAVES>
+__device__ __forceinline__ void choose(const LayerArgs& a, int t) {
+  __shared__ double score[kMaxExperts], reduce[WAVES];
   __shared__ uint64_t key[kMaxExperts], group_key[kMaxGroups];
   __shared__ int chosen[kMaxTopK], kept[kMaxGroups];
-  constexpr int kOwn = kMaxExperts / 256;
-  const int t = blockIdx.x, tid = threadIdx.x;
+  constexpr int kThreads = 64 * WAVES, kOwn = kMaxExperts / kThreads;
+  const int tid = threadIdx.x;
   double z[kOwn];
 #pragma unroll
   for (int o = 0; o < kOwn; ++o) {
-    const int e = tid + o * 256;
+    const int e = tid + o * kThreads;
     z[o] = -__builtin_inf();
     if (e < a.E) {
       const double* p = a.logits + (int64_t)t * a.E + e;
@@ -227,20 +231,20 @@ __global__ __launch_bounds__(256) void k_gate(LayerArgs a) {
     double m = z[0];
 #pragma unroll
     for (int o = 1; o < kOwn; ++o) m = z[o] > m || z[o] != z[o] ? z[o] : m;
-    m = block_reduce(m, true, reduce);
+    m = block_reduce<WAVES>(m, true, reduce);
     double sum = 0.0;
 #pragma unroll
     for (int o = 0; o < kOwn; ++o) {
-      z[o] = tid + o * 256 < a.E ? exp(z[o] - m) : 0.0;
+      z[o] = tid + o * kThreads < a.E ? exp(z[o] - m) : 0.0;
       sum += z[o];
     }
-    sum = block_reduce(sum, false, reduce);
+    sum = block_reduce<WAVES>(sum, false, reduce);
 #pragma unroll
     for (int o = 0; o < kOwn; ++o) z[o] /= sum;
   } else {
 #pragma unroll
     for (int o = 0; o < kOwn; ++o) {
-      if (tid + o * 256 < a.E) {
+      if (tid + o * kThreads < a.E) {
         const double q = exp(-fabs(z[o]));
         z[o] = z[o] < 0 ? q / (1.0 + q) : 1.0 / (1.0 + q);
       }
@@ -248,7 +252,7 @@ __global__ __launch_bounds__(256) void k_gate(LayerArgs a) {
   }
 #pragma unroll
   for (int o = 0; o < kOwn; ++o) {
-    const int e = tid + o * 256;
+    const int e = tid + o * kThreads;
     if (e < a.E) {
       score[e] = z[o];
       key[e] = order_key(a.bias ? z[o] + (double)a.bias[e] : z[o]);
@@ -278,7 +282,7 @@ __global__ __launch_bounds__(256) void k_gate(LayerArgs a) {
       kept[tid] = rank < a.top_groups;
     }
     __syncthreads();
-    for (int e = tid; e < a.E; e += 256)
+    for (int e = tid; e < a.E; e += kThreads)
       if (!kept[e / n]) key[e] = 0;
     __syncthreads();
   }
@@ -287,23 +291,23 @@ __global__ __launch_bounds__(256) void k_gate(LayerArgs a) {
   int rank[kOwn];
 #pragma unroll
   for (int o = 0; o < kOwn; ++o) {
-    const int e = tid + o * 256;
+    const int e = tid + o * kThreads;
     mine[o] = e < a.E ? key[e] : 0;
     rank[o] = 0;
   }
-  const int own = (a.E + 255) / 256;
+  const int own = (a.E + kThreads - 1) / kThreads;
 #pragma unroll 8
   for (int j = 0; j < a.E; ++j) {
     const uint64_t other = key[j];
     rank[0] += other > mine[0] || (other == mine[0] && j < tid);
     if (own > 1) {
 #pragma unroll
-      for (int o = 1; o < kOwn; ++o) rank[o] += other > mine[o] || (other == mine[o] && j < tid + o * 256);
+      for (int o = 1; o < kOwn; ++o) rank[o] += other > mine[o] || (other == mine[o] && j < tid + o * kThreads);
     }
   }
 #pragma unroll
   for (int o = 0; o < kOwn; ++o)
-    if (tid + o * 256 < a.E && rank[o] < a.k) chosen[rank[o]] = tid + o * 256;
+    if (tid + o * kThreads < a.E && rank[o] < a.k) chosen[rank[o]] = tid + o * kThreads;
   __syncthreads();
   if (tid < a.k) {
     double total = 0.0;
@@ -539,51 +543,55 @@ __device__ __forceinline__ void leave_rows(const LayerArgs& a, bool shared, int 
 // ---------------------------------------------------------------------------------------------
 // Few tokens
 // ---------------------------------------------------------------------------------------------
-template <bool FP8, int P>
+template <bool FP8, int P, int NC>
 struct Tokens {
-  u4 b[P][4];
-  // a step of this lane's token, which begins at `token` of parts[p] (kNothing for none)
-  __device__ __forceinline__ void load(const __amdgpu_buffer_rsrc_t (&parts)[P], uint32_t token, int step, int K) {
+  u4 b[NC][P][4];
+  // a step of this lane's tokens, which begin at token[c] of parts[p] (kNothing for none)
+  __device__ __forceinline__ void load(const __amdgpu_buffer_rsrc_t (&parts)[P], const uint32_t (&token)[NC], int step, int K) {
     const int left = K - step * kBlock, g = threadIdx.x >> 4 & 3;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int k = k_of<FP8>(q, g);
-      const uint32_t at = k < left ? token + (uint32_t)(step * kBlock + k) * 2 : kNothing;
+    for (int c = 0; c < NC; ++c)
 #pragma unroll
-      for (int p = 0; p < P; ++p) b[p][q] = load16(parts[p], at);
-    }
+      for (int q = 0; q < 4; ++q) {
+        const int k = k_of<FP8>(q, g);
+        const uint32_t at = k < left ? token[c] + (uint32_t)(step * kBlock + k) * 2 : kNothing;
+#pragma unroll
+        for (int p = 0; p < P; ++p) b[c][p][q] = load16(parts[p], at);
+      }
   }
 };
 
-template <bool FP8, bool STREAM, int M, int P>
-__device__ __forceinline__ void multiply(f4 (&acc)[M][1], Weights<FP8, STREAM, M>& w, const Tokens<FP8, P>& x) {
+template <bool FP8, bool STREAM, int M, int P, int NC>
+__device__ __forceinline__ void multiply(f4 (&acc)[M][NC], Weights<FP8, STREAM, M>& w, const Tokens<FP8, P, NC>& x) {
   w.settle();
-  f4 sum[M][1];
-  if constexpr (FP8) clear<FP8, M, 1>(sum);
+  f4 sum[M][NC];
+  if constexpr (FP8) clear<FP8, M, NC>(sum);
 #pragma unroll
   for (int q = 0; q < 4; ++q)
 #pragma unroll
     for (int m = 0; m < M; ++m) {
       const bf8 row = w.frag(m, q);
 #pragma unroll
-      for (int p = P - 1; p >= 0; --p) {
-        f4& s = FP8 ? sum[m][0] : acc[m][0];
-        s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(row, __builtin_bit_cast(bf8, x.b[p][q]), s, 0, 0, 0);
-      }
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int p = P - 1; p >= 0; --p) {
+          f4& s = FP8 ? sum[m][c] : acc[m][c];
+          s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(row, __builtin_bit_cast(bf8, x.b[c][p][q]), s, 0, 0, 0);
+        }
     }
-  if constexpr (FP8) join_step<FP8, STREAM, M, 1>(acc, sum, w);
+  if constexpr (FP8) join_step<FP8, STREAM, M, NC>(acc, sum, w);
 }
 
 // acc += rows[.., steps first : end : step of K] times the tokens; the loads of the next step go out before a step's
 // products.
-template <bool FP8, bool STREAM, int M, int P>
-__device__ __forceinline__ void sum_steps(f4 (&acc)[M][1], const __amdgpu_buffer_rsrc_t (&rows)[M][2],
-                                          const floats_at (&scales)[M], const __amdgpu_buffer_rsrc_t (&parts)[P], uint32_t token, int K, int first, int end,
-                                          int step) {
+template <bool FP8, bool STREAM, int M, int P, int NC>
+__device__ __forceinline__ void sum_steps(f4 (&acc)[M][NC], const __amdgpu_buffer_rsrc_t (&rows)[M][2],
+                                          const floats_at (&scales)[M], const __amdgpu_buffer_rsrc_t (&parts)[P],
+                                          const uint32_t (&token)[NC], int K, int first, int end, int step) {
   if (first >= end) return;
   const uint32_t mine = offset_in_rows<FP8>(K);
   Weights<FP8, STREAM, M> w, next;
-  Tokens<FP8, P> x, ahead;
+  Tokens<FP8, P, NC> x, ahead;
   w.load(rows, mine, scales, first, K);
   x.load(parts, token, first, K);
   for (int b = first; b < end; b += 2 * step) {
@@ -592,34 +600,27 @@ __device__ __forceinline__ void sum_steps(f4 (&acc)[M][1], const __amdgpu_buffer
       next.load(rows, mine, scales, b1, K);
       ahead.load(parts, token, b1, K);
     }
-    multiply<FP8, STREAM, M, P>(acc, w, x);
+    multiply<FP8, STREAM, M, P, NC>(acc, w, x);
     if (b1 >= end) break;
     if (b2 < end) {
       w.load(rows, mine, scales, b2, K);
       x.load(parts, token, b2, K);
     }
-    multiply<FP8, STREAM, M, P>(acc, next, ahead);
+    multiply<FP8, STREAM, M, P, NC>(acc, next, ahead);
   }
 }
 
-template <int DT, bool FP8, bool UP, bool STREAM>
-__global__ __launch_bounds__(64 * kFewWaves) void k_few(LayerArgs a) {
-  constexpr int P = UP ? kXParts<DT> : kHParts<DT>, ROWS = UP ? 16 : 32;
-  __shared__ OneUnit<64 * kFewWaves, kFewTokens, kFewTokens * kMaxTopK> plan;
-  __shared__ f4 sum[kFewWaves][2][64];
+template <bool UP>
+constexpr int kFewRows = UP ? 16 : 32;  // of a workgroup
+
+// kFewRows rows times n <= 16 NC tokens: the shared expert's from `first` on, or the assignments of a list.
+template <int DT, bool FP8, bool UP, bool STREAM, int NC, int WAVES>
+__device__ __forceinline__ void few_rows(const LayerArgs& a, const uint16_t* list, int expert, int tile, int first, int n, bool shared) {
+  constexpr int P = UP ? kXParts<DT> : kHParts<DT>;
+  __shared__ f4 sum[WAVES][2][NC][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
-  const int tiles = ((UP ? a.experts.H : a.D) + ROWS - 1) / ROWS, routed = a.units * tiles;
-  const bool shared = (int)blockIdx.x >= routed;
-  int expert = 0, tile = blockIdx.x - routed, n = a.T;
-  if (!shared) {
-    const int u = blockIdx.x / tiles;
-    tile = blockIdx.x - u * tiles;
-    if (!plan.make(a.idx, a.T, a.k, a.E, u)) return;
-    expert = uniform((int)(plan.unit >> 16));
-    n = uniform(plan.tokens);
-  }
   const int H = shared ? a.shared.H : a.experts.H, K = UP ? a.D : H, KB = (K + kBlock - 1) / kBlock;
-  const int row0 = tile * ROWS, stacked = UP ? 2 * H : a.D;
+  const int row0 = tile * kFewRows<UP>, stacked = UP ? 2 * H : a.D;
   const bool both = UP || row0 + 16 < a.D;  // else the second 16 rows are the first ones again and not stored
   const uint8_t* w = UP ? (shared ? a.shared.w12 : a.experts.w12) : (shared ? a.shared.w3 : a.experts.w3);
   const float* s = UP ? (shared ? a.shared.s12 : a.experts.s12) : (shared ? a.shared.s3 : a.experts.s3);
@@ -635,22 +636,60 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_few(LayerArgs a) {
   const int64_t plane = (int64_t)(UP || shared ? a.T : a.T * a.k) * pitch;
 #pragma unroll
   for (int p = 0; p < P; ++p) parts[p] = make_rsrc((UP ? a.xb : shared ? a.hs : a.hb) + p * plane, 2 * plane);
-  const int at = r < n ? (shared ? r : plan.list[r]) : 0;
-  const uint32_t token = r < n ? (uint32_t)(UP && !shared ? at / a.k : at) * (uint32_t)pitch * 2 : kNothing;
-  f4 acc[2][1];
-  clear<FP8, 2, 1>(acc);
-  sum_steps<FP8, STREAM, 2, P>(acc, rows, scales, parts, token, K, uniform(wave), KB, kFewWaves);
+  int at[NC];
+  uint32_t token[NC];
 #pragma unroll
-  for (int m = 0; m < 2; ++m) sum[wave][m][lane] = acc[m][0];
-  __syncthreads();
-  if (wave > 0 || r >= n) return;
-  f4 v[2] = {sum[0][0][lane], sum[0][1][lane]};
-#pragma unroll
-  for (int i = 1; i < kFewWaves; ++i) {
-    v[0] += sum[i][0][lane];
-    v[1] += sum[i][1][lane];
+  for (int c = 0; c < NC; ++c) {
+    const int i = c * 16 + r;
+    at[c] = i < n ? (shared ? first + i : list[i]) : 0;
+    token[c] = i < n ? (uint32_t)(UP && !shared ? at[c] / a.k : at[c]) * (uint32_t)pitch * 2 : kNothing;
   }
-  leave_rows<DT, UP>(a, shared, at, row0 + 4 * g, both, v[0], v[1]);
+  f4 acc[2][NC];
+  clear<FP8, 2, NC>(acc);
+  sum_steps<FP8, STREAM, 2, P, NC>(acc, rows, scales, parts, token, K, uniform(wave), KB, WAVES);
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int c = 0; c < NC; ++c) sum[wave][m][c][lane] = acc[m][c];
+  __syncthreads();
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    if (wave != c || c * 16 + r >= n) continue;
+    f4 v[2] = {sum[0][0][c][lane], sum[0][1][c][lane]};
+#pragma unroll
+    for (int i = 1; i < WAVES; ++i) {
+      v[0] += sum[i][0][c][lane];
+      v[1] += sum[i][1][c][lane];
+    }
+    leave_rows<DT, UP>(a, shared, at[c], row0 + 4 * g, both, v[0], v[1]);
+  }
+}
+
+// The gate, a workgroup a token, and the shared expert's h, which needs no gate (its workgroups read their tokens
+// from the cache, each for itself: see early_shared).  With up to 16 tokens the waves have fewer steps each to wait for.
+template <int NC>
+constexpr int kGateWaves = NC == 1 ? 8 : 4;
+template <int DT, bool FP8, bool STREAM, int NC>
+__global__ __launch_bounds__(64 * kGateWaves<NC>) void k_gate(LayerArgs a) {
+  if ((int)blockIdx.x < a.T) return choose<kGateWaves<NC>>(a, blockIdx.x);
+  const int i = blockIdx.x - a.T, units = (a.T + 16 * NC - 1) / (16 * NC), tile = i / units, first = (i - tile * units) * 16 * NC;
+  few_rows<DT, FP8, true, STREAM, NC, kGateWaves<NC>>(a, nullptr, 0, tile, first, min(a.T - first, 16 * NC), true);
+}
+
+template <int DT, bool FP8, bool UP, bool STREAM>
+__global__ __launch_bounds__(64 * kFewWaves) void k_few(LayerArgs a) {
+  __shared__ OneUnit<64 * kFewWaves, kFewTokens, kFewTokens * kMaxTopK> plan;
+  const int tiles = ((UP ? a.experts.H : a.D) + kFewRows<UP> - 1) / kFewRows<UP>, routed = a.units * tiles;
+  const bool shared = (int)blockIdx.x >= routed;
+  int expert = 0, tile = blockIdx.x - routed, n = a.T;
+  if (!shared) {
+    const int u = blockIdx.x / tiles;
+    tile = blockIdx.x - u * tiles;
+    if (!plan.make(a.idx, a.T, a.k, a.E, u)) return;
+    expert = uniform((int)(plan.unit >> 16));
+    n = uniform(plan.tokens);
+  }
+  few_rows<DT, FP8, UP, STREAM, 1, kFewWaves>(a, plan.list, expert, tile, 0, n, shared);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -889,12 +928,12 @@ void set_sizes(LayerArgs& a, int dtype, int64_t T, int64_t D, int64_t E, int64_t
   a.units = (int)((n < E ? n : E) + n / a.unit);
 }
 
-// Whether the waves share K: where k_products would have fewer than one and a half workgroups a CU.  One token, 8 of 32 experts
-// of 7168 x 2048 and a shared one: up, 288 of them, 48 us against 65, down, 504, 29 against 25; 16 tokens, 16 experts of
-// 1024 x 1024, 320 and 136: 43 against 51 a call.
+// Whether the waves share K: where k_products would have fewer than one and a half workgroups a CU.  One token, 8 of 32
+// experts of 7168 x 2048 and a shared one: up, 288 of them with the shared one's, 47 us against 65, down, 504, 29 against
+// 25; 16 tokens, 16 experts of 1024 x 1024, 320 and 136: 43 against 51 a call.
 bool splits_k(const LayerArgs& a, bool up) {
   const int64_t rows = up ? kTileRows<true> : kTileRows<false>;
-  const int64_t groups = a.units * cdiv(up ? a.experts.H : a.D, rows) + (a.shared.H ? cdiv(up ? a.shared.H : a.D, rows) : 0);
+  const int64_t groups = a.units * cdiv(up ? a.experts.H : a.D, rows) + (!up && a.shared.H ? cdiv(a.D, rows) : 0);
   return a.T <= kFewTokens && 2 * groups < 3 * cin_device_cus();
 }
 
@@ -914,12 +953,21 @@ void launch_tiles(const LayerArgs& a, dim3 grid, hipStream_t stream) {
   }
 }
 
+// Whether the shared expert's h is formed beside the gate: where its workgroups among the products, which come last and
+// are waited for, would leave most CUs idle, and while the tokens' parts that each 16 rows read for themselves are few.
+// Gate and up together, 32 experts of 7168 x 2048 and a shared one: one bf16 token 50 us, 52 with it among the products;
+// 16 163 and 177; 64 190 and 201; with 64 tokens in fp16 248 and 229, with a shared one of 8192 243 and 225.
+template <int DT>
+bool early_shared(const LayerArgs& a) {
+  return a.T * kXParts<DT> <= 64 && 2 * cdiv(a.shared.H, kTileRows<true>) * cdiv(a.T, a.unit) <= cin_device_cus();
+}
+
 template <int DT, bool FP8, bool UP, bool STREAM>
 void launch_products(const LayerArgs& a, hipStream_t stream) {
   const bool few = splits_k(a, UP);
-  const int64_t rows = few ? (UP ? 16 : 32) : kTileRows<UP>, units = few ? 1 : cdiv(a.T, a.unit);
+  const int64_t rows = few ? kFewRows<UP> : kTileRows<UP>, units = few ? 1 : cdiv(a.T, a.unit);
   const int64_t routed = a.units * cdiv(UP ? a.experts.H : a.D, rows);
-  const int64_t shared = a.shared.H ? units * cdiv(UP ? a.shared.H : a.D, rows) : 0;
+  const int64_t shared = a.shared.H && !(UP && early_shared<DT>(a)) ? units * cdiv(UP ? a.shared.H : a.D, rows) : 0;
   const dim3 grid((uint32_t)(routed + shared));
   if (few) {
     hipLaunchKernelGGL((k_few<DT, FP8, UP, STREAM>), grid, dim3(64 * kFewWaves), 0, stream, a);
@@ -940,10 +988,27 @@ void launch_products(const LayerArgs& a, bool on_lines, hipStream_t stream) {
     launch_products<DT, FP8, UP, false>(a, stream);
 }
 
+template <int DT, bool FP8, bool STREAM, int NC>
+void launch_gate(const LayerArgs& a, hipStream_t stream) {
+  const int64_t shared = early_shared<DT>(a) ? cdiv(a.shared.H, kFewRows<true>) * cdiv(a.T, 16 * NC) : 0;
+  hipLaunchKernelGGL((k_gate<DT, FP8, STREAM, NC>), dim3((uint32_t)(a.T + shared)), dim3(64 * kGateWaves<NC>), 0, stream, a);
+}
+template <int DT, bool FP8, bool STREAM>
+void launch_gate(const LayerArgs& a, hipStream_t stream) {
+  if (a.T <= 16)
+    launch_gate<DT, FP8, STREAM, 1>(a, stream);
+  else
+    launch_gate<DT, FP8, STREAM, 2>(a, stream);
+}
+
 template <int DT, bool FP8>
 void launch_experts(const LayerArgs& a, hipStream_t stream) {
   const bool on_lines =
       ((uintptr_t)a.experts.w12 | (uintptr_t)a.experts.w3 | (uintptr_t)a.shared.w12 | (uintptr_t)a.shared.w3) % 128 == 0;
+  if (on_lines && a.D % (FP8 ? 128 : 64) == 0)
+    launch_gate<DT, FP8, true>(a, stream);
+  else
+    launch_gate<DT, FP8, false>(a, stream);
   launch_products<DT, FP8, true>(a, on_lines, stream);
   launch_products<DT, FP8, false>(a, on_lines, stream);
   hipLaunchKernelGGL((k_join<DT>), dim3((a.T * (a.D / 4) + 255) / 256), dim3(256), 0, stream, a);
@@ -952,7 +1017,6 @@ void launch_experts(const LayerArgs& a, hipStream_t stream) {
 template <int DT>
 void launch(const LayerArgs& a, bool fp8, hipStream_t stream) {
   hipLaunchKernelGGL((k_router<DT>), dim3(a.slices * ((a.E + 15) / 16), (a.T + 15) / 16), dim3(256), 0, stream, a);
-  hipLaunchKernelGGL(k_gate, dim3(a.T), dim3(256), 0, stream, a);
   if (fp8)
     launch_experts<DT, true>(a, stream);
   else

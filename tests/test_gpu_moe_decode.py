@@ -135,6 +135,13 @@ CASES = [
     (128, 96, 64, 1024, 16, "bf16", "fp8", 32, {"n_groups": 64, "top_groups": 7}),
     (40, 2000, 720, 60, 4, "bf16", "bf16", 0, {}),
     (128, 256, 128, 2, 1, "fp16", "fp8", 128, {}),
+    # the shared expert's first product beside the gate in several units, and among the others where it is large
+    (19, 1040, 272, 5, 2, "fp32", "bf16", 144, {}),
+    (37, 784, 128, 12, 3, "bf16", "bf16", 208, {}),
+    (29, 2048, 160, 6, 2, "fp16", "fp8", 1040, {}),
+    (49, 1152, 128, 700, 2, "bf16", "fp8", 128, {}),
+    (20, 512, 128, 4, 2, "bf16", "fp8", 8208, {}),
+    (2, 256, 128, 4, 2, "fp16", "bf16", 8256, {}),
 ]
 
 
