@@ -70,6 +70,12 @@ struct Expert {  // stacked experts, or a shared one
   int H;
 };
 
+// A unit: up to kUnitTokens or twice as many tokens of one expert, as assignments t k + j.
+struct UnitPlan {
+  uint32_t expert, tokens;  // no tokens: no such unit
+  uint16_t list[2 * kUnitTokens];
+};
+
 struct LayerArgs {
   const void* x;
   int64_t ldx;
@@ -89,6 +95,7 @@ struct LayerArgs {
   int slices;
   uint16_t *xb, *hb, *hs;  // parts of x [P, T, Dp], of h [P, T k, H], of the shared expert's [P, T, Hs]
   float* y;                // the experts' outputs [T k, D], the shared one's [T, D]
+  UnitPlan* plans;         // [units]
   int unit, units;         // tokens of a unit, and the most units that the routed experts can have
 };
 
@@ -408,6 +415,45 @@ struct OneUnit {
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
+// What a workgroup of the products keeps of its unit: the first product finds it from the chosen experts, and leaves it for
+// the second.
+template <bool UP, int THREADS, int UNIT, int MOST>
+struct Unit : OneUnit<THREADS, UNIT, MOST> {};
+template <int THREADS, int UNIT, int MOST>
+struct Unit<false, THREADS, UNIT, MOST> {
+  uint16_t list[UNIT];
+};
+// False where there is no unit u; else its expert and n tokens, list[first] and on.
+template <int THREADS, int UNIT, int MOST>
+__device__ __forceinline__ bool find_unit(const LayerArgs& a, Unit<true, THREADS, UNIT, MOST>& plan, int u, bool leave, int& expert,
+                                          int& first, int& n) {
+  const bool there = plan.make(a.idx, a.T, a.k, a.E, u);
+  expert = there ? uniform((int)(plan.unit >> 16)) : 0;
+  first = there ? uniform((int)(plan.unit & 0xffffu)) : 0;
+  n = there ? uniform(plan.tokens) : 0;
+  if (leave) {
+    UnitPlan& p = a.plans[u];
+    if (threadIdx.x == 0) {
+      p.expert = (uint32_t)expert;
+      p.tokens = (uint32_t)n;
+    }
+    if ((int)threadIdx.x < n) p.list[threadIdx.x] = plan.list[first + threadIdx.x];
+  }
+  return there;
+}
+template <int THREADS, int UNIT, int MOST>
+__device__ __forceinline__ bool find_unit(const LayerArgs& a, Unit<false, THREADS, UNIT, MOST>& plan, int u, bool, int& expert,
+                                          int& first, int& n) {
+  const UnitPlan& p = a.plans[u];
+  expert = uniform((int)p.expert);
+  first = 0;
+  n = uniform((int)p.tokens);
+  if (n == 0) return false;
+  if ((int)threadIdx.x < UNIT) plan.list[threadIdx.x] = p.list[threadIdx.x];
+  __syncthreads();
+  return true;
+}
+
 // ---------------------------------------------------------------------------------------------
 // Products of 16 weight rows with 16 tokens
 // ---------------------------------------------------------------------------------------------
@@ -678,16 +724,14 @@ __global__ __launch_bounds__(64 * kGateWaves<NC>) void k_gate(LayerArgs a) {
 
 template <int DT, bool FP8, bool UP, bool STREAM>
 __global__ __launch_bounds__(64 * kFewWaves) void k_few(LayerArgs a) {
-  __shared__ OneUnit<64 * kFewWaves, kFewTokens, kFewTokens * kMaxTopK> plan;
+  __shared__ Unit<UP, 64 * kFewWaves, kFewTokens, kFewTokens * kMaxTopK> plan;
   const int tiles = ((UP ? a.experts.H : a.D) + kFewRows<UP> - 1) / kFewRows<UP>, routed = a.units * tiles;
   const bool shared = (int)blockIdx.x >= routed;
-  int expert = 0, tile = blockIdx.x - routed, n = a.T;
+  int expert = 0, tile = blockIdx.x - routed, first = 0, n = a.T;
   if (!shared) {
     const int u = blockIdx.x / tiles;
     tile = blockIdx.x - u * tiles;
-    if (!plan.make(a.idx, a.T, a.k, a.E, u)) return;
-    expert = uniform((int)(plan.unit >> 16));
-    n = uniform(plan.tokens);
+    if (!find_unit(a, plan, u, tile == 0, expert, first, n)) return;
   }
   few_rows<DT, FP8, UP, STREAM, 1, kFewWaves>(a, plan.list, expert, tile, 0, n, shared);
 }
@@ -705,8 +749,8 @@ constexpr int kTokenStep = P * NC * 16 * kTokenPitch;
 template <bool UP>
 constexpr int kTileRows = kTileWaves * (UP ? 16 : 32);
 
-template <int UNIT>
-using TilePlan = OneUnit<64 * kTileWaves, UNIT, kMaxAssigned>;
+template <bool UP, int UNIT>
+using TilePlan = Unit<UP, 64 * kTileWaves, UNIT, kMaxAssigned>;
 
 template <int DT, bool FP8, bool UP, bool STREAM, int NC, class Plan>
 __device__ __forceinline__ void tile_unit(const LayerArgs& a, const Plan& plan, uint16_t* lds, int expert, int tile, int first, int n,
@@ -822,7 +866,7 @@ __device__ __forceinline__ void tile_unit(const LayerArgs& a, const Plan& plan, 
 template <int DT, bool FP8, bool UP, bool STREAM, int UNIT>
 __global__ __launch_bounds__(64 * kTileWaves, UNIT > kUnitTokens ? 2 : FP8 && UP && DT == CIN_DT_BF16 ? 4 : 3) void k_products(LayerArgs a) {
   constexpr int ROWS = kTileRows<UP>;
-  __shared__ TilePlan<UNIT> plan;
+  __shared__ TilePlan<UP, UNIT> plan;
   extern __shared__ u4 tokens[];  // [parts, columns][kTokenPitch] of 16 bits
   const int tiles = ((UP ? a.experts.H : a.D) + ROWS - 1) / ROWS, routed = a.units * tiles;
   const bool shared = (int)blockIdx.x >= routed;
@@ -830,10 +874,7 @@ __global__ __launch_bounds__(64 * kTileWaves, UNIT > kUnitTokens ? 2 : FP8 && UP
   if (!shared) {
     tile = blockIdx.x / a.units;
     const int u = blockIdx.x - tile * a.units;
-    if (!plan.make(a.idx, a.T, a.k, a.E, u)) return;
-    expert = uniform((int)(plan.unit >> 16));
-    first = uniform((int)(plan.unit & 0xffffu));
-    n = uniform(plan.tokens);
+    if (!find_unit(a, plan, u, tile == 0, expert, first, n)) return;
   } else {
     const int i = blockIdx.x - routed, units = (a.T + UNIT - 1) / UNIT;
     tile = i / units;
@@ -895,6 +936,7 @@ int64_t layout(LayerArgs& a, int dtype, char* base) {
   a.hb = reinterpret_cast<uint16_t*>(take(2 * ph * a.T * a.k * a.experts.H));
   a.hs = reinterpret_cast<uint16_t*>(take(2 * ph * a.T * a.shared.H));
   a.y = reinterpret_cast<float*>(take(4LL * a.T * (a.k + 1) * a.D));
+  a.plans = reinterpret_cast<UnitPlan*>(take((int64_t)sizeof(UnitPlan) * a.units));
   return at;
 }
 
@@ -947,7 +989,7 @@ void launch_tiles(const LayerArgs& a, dim3 grid, hipStream_t stream) {
   }
   if constexpr (DT != CIN_DT_F32) {
     auto kernel = k_products<DT, FP8, UP, STREAM, 2 * kUnitTokens>;
-    if (2 * lds + sizeof(TilePlan<2 * kUnitTokens>) > 65536)
+    if (2 * lds + sizeof(TilePlan<UP, 2 * kUnitTokens>) > 65536)
       (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)(2 * lds));
     hipLaunchKernelGGL(kernel, grid, dim3(64 * kTileWaves), 2 * lds, stream, a);
   }
