@@ -540,7 +540,7 @@ def moe_decode(x: torch.Tensor, router_weight: torch.Tensor, experts, top_k: int
     if bias is not None:
         _require(bias.shape == (E,) and bias.device == dev and bias.dtype == torch.float32,
                  "bias must be fp32 [n_experts] on x's device")
-        bias = bias.detach()
+        bias = _without_grad(bias)
     if isinstance(experts, layers.GroupedExperts):
         _require(experts.n_experts == E and experts.d_model == D, "the router and the experts differ in number or width")
         _require(D % 128 == 0 and experts.hidden_dim % 64 == 0, "GroupedExperts' FP8 blocks need D in multiples of 128, H of 64")
@@ -571,12 +571,17 @@ def _decode_weights(weights, x, lead):
     _require(dt == w3.dtype and w12.device == dev and w3.device == dev, "weights must share one dtype, on x's device")
     if dt == torch.bfloat16:
         _require(s12 is None and s3 is None, "bf16 weights have no scales")
-        return w12.detach(), None, w3.detach(), None
+        return _without_grad(w12), None, _without_grad(w3), None
     _require(dt == torch.float8_e4m3fn, "weights must be e4m3 codes or bf16")
     _require(s12 is not None and s3 is not None and s12.dtype == torch.float32 and s3.dtype == torch.float32
              and s12.device == dev and s3.device == dev and s12.shape == (*lead, _cdiv(2 * H, 128), _cdiv(D, 128))
              and s3.shape == (*lead, _cdiv(D, 128), _cdiv(H, 128)), "codes need fp32 scales of their 128 x 128 blocks, on x's device")
-    return w12, s12.detach(), w3, s3.detach()
+    return w12, _without_grad(s12), w3, _without_grad(s3)
+
+
+def _without_grad(t):
+    # (detach costs 0.6 us of host time each)
+    return t if type(t) is torch.Tensor and not t.requires_grad else t.detach()
 
 
 @functools.lru_cache(maxsize=256)
