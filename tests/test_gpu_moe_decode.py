@@ -324,7 +324,7 @@ def test_compiled(dev):
     want = f(x, r, *experts, *shared)
     got = torch.compile(f, fullgraph=True, backend="aot_eager")(x, r, *experts, *shared)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
-    # (the checker itself cannot compute with codes)
+    # (opcheck itself cannot compute with codes)
     x, r, experts, shared = inputs(dev, 5, 144, 64, 6, "bf16", "bf16", 32)
     torch.library.opcheck(torch.ops.cinnamon_amd.moe_decode.default, (x, r, None, *experts, *shared, 2, 0, 1, 1, 2, True, 1.0))
 
