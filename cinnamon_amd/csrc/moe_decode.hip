@@ -102,7 +102,7 @@ struct LayerArgs {
 // Scales, the same for all lanes and nowhere written here: scalar loads.
 typedef const __attribute__((address_space(4))) float* floats_at;
 
-// 16 bytes at an offset into a buffer; zeros from kNothing on.  No load of the products is behind a branch: one
+// 16 bytes at an offset into a buffer; zeros from kNothing on.  No load of k_products is behind a branch: one
 // that may not have been issued would have to be counted as issued last, and all before it waited for.
 constexpr uint32_t kNothing = 0x80000000u;
 template <int AUX = 0>
