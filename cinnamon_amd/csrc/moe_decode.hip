@@ -11,9 +11,9 @@
 // 16 x 16 x 32 units, 16 weight rows by up to 16 tokens at a time.  The tokens of an expert are gathered, so
 // that no column is wasted; a block's scale multiplies its fp32 sum.
 //
-// Rounding: x is split into bf16 parts that hold it exactly (one for bf16, two for fp16, three for fp32); h is
-// split into two parts (2^-17 of a value; three, 2^-25, where the output is fp32), as one bf16 part would add an error as
-// large as the output's own rounding.  All sums are fp32.  Logits and the gate are in 64 bits: choices next to
+// Rounding: x is split into bf16 parts that hold it exactly (one for bf16, two for fp16, three for fp32); h, formed in
+// fp32, into three (2^-25 of a value): two parts' 2^-17 would show wherever an output's terms cancel, in 16 bits too,
+// for 1 to 6% of the time (64 tokens 308 us with two, 327 with three).  All sums are fp32.  Logits and the gate are in 64 bits: choices next to
 // the border of the top k differ by less than 32 bits hold.
 //
 // Five launches: k_router (logits by slices of D on the fp64 matrix units, and x's parts), k_gate (a workgroup a
@@ -58,11 +58,10 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 typedef double d4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
-// Parts of x and of h for an input type.
+// Parts of x for its type, and of h.
 template <int DT>
 constexpr int kXParts = DT == CIN_DT_BF16 ? 1 : DT == CIN_DT_F16 ? 2 : 3;
-template <int DT>
-constexpr int kHParts = DT == CIN_DT_F32 ? 3 : 2;
+constexpr int kHParts = 3;
 
 struct Expert {  // stacked experts, or a shared one
   const uint8_t *w12, *w3;
@@ -577,7 +576,7 @@ template <int DT, bool UP>
 __device__ __forceinline__ void leave_rows(const LayerArgs& a, bool shared, int at, int row, bool both, f4 first, f4 second) {
   if constexpr (UP) {
     const int H = shared ? a.shared.H : a.experts.H;
-    store_h<kHParts<DT>>((shared ? a.hs : a.hb) + (int64_t)at * H + row, (int64_t)(shared ? a.T : a.T * a.k) * H, first, second,
+    store_h<kHParts>((shared ? a.hs : a.hb) + (int64_t)at * H + row, (int64_t)(shared ? a.T : a.T * a.k) * H, first, second,
                          shared ? 1.0f : a.weights[at]);
   } else {
     float* y = a.y + (int64_t)(shared ? a.T * a.k + at : at) * a.D + row;
@@ -662,7 +661,7 @@ constexpr int kFewRows = UP ? 16 : 32;  // of a workgroup
 // kFewRows rows times n <= 16 NC tokens: the shared expert's from `first` on, or the assignments of a list.
 template <int DT, bool FP8, bool UP, bool STREAM, int NC, int WAVES>
 __device__ __forceinline__ void few_rows(const LayerArgs& a, const uint16_t* list, int expert, int tile, int first, int n, bool shared) {
-  constexpr int P = UP ? kXParts<DT> : kHParts<DT>;
+  constexpr int P = UP ? kXParts<DT> : kHParts;
   __shared__ f4 sum[WAVES][2][NC][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
   const int H = shared ? a.shared.H : a.experts.H, K = UP ? a.D : H, KB = (K + kBlock - 1) / kBlock;
@@ -741,9 +740,11 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_few(LayerArgs a) {
 // ---------------------------------------------------------------------------------------------
 constexpr int kTokenPitch = kBlock + 8;  // elements of a token's step in LDS: 16 lanes' 16 bytes on all banks
 
-// Elements of a step's parts in LDS.
+// Elements of a step's parts in LDS, and the steps that lie there: two, or one where two would leave a CU one workgroup.
 template <int P, int NC>
 constexpr int kTokenStep = P * NC * 16 * kTokenPitch;
+template <int P, int NC>
+constexpr int kStepsInLds = P * NC > 8 ? 1 : 2;
 
 // Rows of a workgroup: 16 hidden channels (of W1 and W2 each) a wave, or 32 output channels.
 template <bool UP>
@@ -755,9 +756,9 @@ using TilePlan = Unit<UP, 64 * kTileWaves, UNIT, kMaxAssigned>;
 template <int DT, bool FP8, bool UP, bool STREAM, int NC, class Plan>
 __device__ __forceinline__ void tile_unit(const LayerArgs& a, const Plan& plan, uint16_t* lds, int expert, int tile, int first, int n,
                                           bool shared) {
-  constexpr int P = UP ? kXParts<DT> : kHParts<DT>;
+  constexpr int P = UP ? kXParts<DT> : kHParts;
   constexpr int kChunks = NC * 16 * P * (kBlock / 8), kThreads = 64 * kTileWaves;  // of 16 bytes, a step
-  constexpr int kOwn = (kChunks + kThreads - 1) / kThreads;
+  constexpr int kOwn = (kChunks + kThreads - 1) / kThreads, kInLds = kStepsInLds<P, NC>;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
   const int H = shared ? a.shared.H : a.experts.H, K = UP ? a.D : H, KB = (K + kBlock - 1) / kBlock;
   const int row0 = tile * kTileRows<UP> + wave * (UP ? 16 : 32), rows_all = UP ? H : a.D;
@@ -797,7 +798,7 @@ __device__ __forceinline__ void tile_unit(const LayerArgs& a, const Plan& plan, 
     for (int o = 0; o < kOwn; ++o) part[o] = load16(parts, there ? from[o] + (uint32_t)b * 2 * kBlock : kNothing);
   };
   auto leave = [&](int b) {
-    uint16_t* tile_b = lds + (b & 1) * kTokenStep<P, NC>;
+    uint16_t* tile_b = lds + b % kInLds * kTokenStep<P, NC>;
 #pragma unroll
     for (int o = 0; o < kOwn; ++o)
       if (kChunks % kThreads == 0 || threadIdx.x + o * kThreads < kChunks) *reinterpret_cast<u4*>(tile_b + to[o]) = part[o];
@@ -820,7 +821,7 @@ __device__ __forceinline__ void tile_unit(const LayerArgs& a, const Plan& plan, 
     later.load(rows, mine, scales, b + kSteps, K);
     if (active) {
       now.settle();
-      const uint16_t* tile_b = lds + (b & 1) * kTokenStep<P, NC>;
+      const uint16_t* tile_b = lds + b % kInLds * kTokenStep<P, NC>;
       f4 sum[2][NC];
       if constexpr (FP8) clear<FP8, 2, NC>(sum);
 #pragma unroll
@@ -840,6 +841,7 @@ __device__ __forceinline__ void tile_unit(const LayerArgs& a, const Plan& plan, 
       }
       if constexpr (FP8) join_step<FP8, STREAM, 2, NC>(acc, sum, now);
     }
+    if constexpr (kInLds == 1) __syncthreads();  // (this step's readers)
     leave(b + 1);
     __syncthreads();
   };
@@ -924,7 +926,7 @@ constexpr int64_t padded(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
 // Bytes of the workspace; fills its pointers where `base` is given.
 int64_t layout(LayerArgs& a, int dtype, char* base) {
-  const int64_t px = dtype == CIN_DT_BF16 ? 1 : dtype == CIN_DT_F16 ? 2 : 3, ph = dtype == CIN_DT_F32 ? 3 : 2;
+  const int64_t px = dtype == CIN_DT_BF16 ? 1 : dtype == CIN_DT_F16 ? 2 : 3, ph = kHParts;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     char* p = base ? base + at : nullptr;
@@ -949,9 +951,9 @@ const char* const kSizes =
     "dtype must be bf16, fp16 or fp32, T <= 128, E <= 1024, k <= min(16, E), D, H and the shared expert's H multiples of 16 up to 65536";
 
 // Tokens of a unit.  A second unit of an expert reads its weights again, from the cache at best; more tokens at once
-// cost the registers of a third workgroup a CU, and with fp32's parts the LDS of a second.  8 of 32 experts of 7168 x 2048:
-// 80 tokens with units of 32 335 us, of 64 386; 96 393 and 392; 112 445 and 404; 96 tokens, 6 of 8 experts 264 and 199; 96
-// fp32 tokens 520 and 722.
+// cost the registers of a third workgroup a CU, and with the parts of an fp32 x the LDS of a second.  8 of 32 experts of
+// 7168 x 2048 and a shared one: 80 tokens with units of 32 350 us, of 64 411; 96 408 and 436; 112 458 and 450; 96 tokens, 6
+// of 8 experts 284 and 262; 64 tokens, 8 of 16 in bf16 518 and 330; 96 fp32 tokens 520 and 722.
 int64_t unit_tokens(int dtype, int64_t T, int64_t E, int64_t k) {
   return dtype != CIN_DT_F32 && T > kUnitTokens && T * k > 24 * E ? 2 * kUnitTokens : kUnitTokens;
 }
@@ -981,17 +983,18 @@ bool splits_k(const LayerArgs& a, bool up) {
 
 template <int DT, bool FP8, bool UP, bool STREAM>
 void launch_tiles(const LayerArgs& a, dim3 grid, hipStream_t stream) {
-  constexpr int P = UP ? kXParts<DT> : kHParts<DT>;
-  const size_t lds = 2 * sizeof(uint16_t) * kTokenStep<P, kUnitTokens / 16>;
+  constexpr int P = UP ? kXParts<DT> : kHParts;
+  constexpr size_t lds = 2 * sizeof(uint16_t) * kTokenStep<P, kUnitTokens / 16>;
   if (DT == CIN_DT_F32 || a.unit == kUnitTokens) {
     hipLaunchKernelGGL((k_products<DT, FP8, UP, STREAM, kUnitTokens>), grid, dim3(64 * kTileWaves), lds, stream, a);
     return;
   }
   if constexpr (DT != CIN_DT_F32) {
+    constexpr size_t more = lds * kStepsInLds<P, 2 * kUnitTokens / 16>;  // (twice the tokens, in one or two steps)
     auto kernel = k_products<DT, FP8, UP, STREAM, 2 * kUnitTokens>;
-    if (2 * lds + sizeof(TilePlan<UP, 2 * kUnitTokens>) > 65536)
-      (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)(2 * lds));
-    hipLaunchKernelGGL(kernel, grid, dim3(64 * kTileWaves), 2 * lds, stream, a);
+    if (more + sizeof(TilePlan<UP, 2 * kUnitTokens>) > 65536)
+      (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)more);
+    hipLaunchKernelGGL(kernel, grid, dim3(64 * kTileWaves), more, stream, a);
   }
 }
 

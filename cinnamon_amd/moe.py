@@ -519,8 +519,8 @@ def moe_decode(x: torch.Tensor, router_weight: torch.Tensor, experts, top_k: int
     layers.quantize_expert_weights returns them) or bf16 with None for the scales.  shared: None or such a tuple of one
     expert, without E and with an H of its own.  D and H are multiples of 16.
 
-    Only the chosen experts' weights are read.  Activations stay in 16 bits or more: unlike in routed_experts
-    they are not quantized, products are summed in fp32 and the result is rounded once.  Inference only: no
+    Only the chosen experts' weights are read.  Unlike in routed_experts activations are not quantized: x is exact in the
+    products, silu(W1 v) * (W2 v) keeps 24 bits, products are summed in fp32 and the result is rounded once.  Inference only: no
     gradient.  Bit-identical from call to call."""
     _require(x.is_cuda, "Input must be on CUDA")
     _require(x.ndim == 2 and x.shape[0] <= MAX_DECODE_TOKENS, "x must be [n_tokens, D] with at most 128 tokens")
