@@ -167,6 +167,16 @@ __device__ inline uint32_t f32_to_bf16_bits(float f) {
   return f32x2_to_bf16x2_bits(f, 0.0f) & 0xffffu;
 }
 
+// The next bf16 part of a value, which is taken off it.  A finite value has finite parts (one within half a
+// step of 2^128 would round to infinity); an infinity is its own first part and leaves 0.
+__device__ __forceinline__ uint32_t take_part(float& v) {
+  uint32_t b = f32_to_bf16_bits(v);
+  const bool inf = (b & 0x7fff) == 0x7f80;
+  if (inf && fabsf(v) < __builtin_inff()) --b;
+  v = inf && !(fabsf(v) < __builtin_inff()) ? 0.0f : v - __uint_as_float(b << 16);
+  return b;
+}
+
 // fp32 -> fp16 bits, round to nearest even (overflow to inf, as a torch .half()).  The
 // empty asm pins f as an fp32 value: otherwise the compiler may fuse the multiply or FMA
 // that produced it with this conversion into one mixed-precision instruction (one rounding

@@ -752,16 +752,6 @@ __global__ __launch_bounds__(1024) void k_ce_rows(const int64_t* __restrict__ y,
   find_rows<1024>(y, T, V, ignore, st, rowloss, true, nullptr);
 }
 
-// The next bf16 part of a value, which is taken off it.  A finite value has finite parts (one within half a
-// step of 2^128 would round to infinity); an infinity is its own first part and leaves 0.
-__device__ __forceinline__ uint32_t take_part(float& v) {
-  uint32_t b = f32_to_bf16_bits(v);
-  const bool inf = (b & 0x7fff) == 0x7f80;
-  if (inf && fabsf(v) < __builtin_inff()) --b;
-  v = inf && !(fabsf(v) < __builtin_inff()) ? 0.0f : v - __uint_as_float(b << 16);
-  return b;
-}
-
 // Rows of x (all, or map's first *n) with zeros up to Dp columns, as operands of DT.
 template <int DT>
 __device__ __forceinline__ void copy_piece(const void* __restrict__ x, int64_t ldx, int64_t D, int64_t row, int64_t i,

@@ -125,22 +125,28 @@ __device__ __forceinline__ void load8(const void* p, int dt, int64_t i, float (&
   }
 }
 
-// bf16 parts of 8 values: each the rounding of what the ones before leave; an infinity or NaN has one.
+// bf16 parts of 8 values: each the rounding of what the ones before leave, kept finite for a finite value; an infinity has
+// one.
 template <int P>
 __device__ __forceinline__ void split8(const float (&v)[8], u4 (&part)[P]) {
   float r[8];
+  bool far = false;  // a value that rounds to infinity, or is one
 #pragma unroll
-  for (int e = 0; e < 8; ++e) r[e] = v[e];
+  for (int e = 0; e < 8; ++e) {
+    r[e] = v[e];
+    far |= fabsf(v[e]) >= 0x1.ffp127f;
+  }
 #pragma unroll
   for (int p = 0; p < P; ++p) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t w = f32x2_to_bf16x2_bits(r[2 * i], r[2 * i + 1]);
-      part[p][i] = w;
-      if (p + 1 < P) {
-        const float lo = bf16_lo(w), hi = bf16_hi(w);
-        r[2 * i] = __builtin_isfinite(lo) ? r[2 * i] - lo : 0.0f;
-        r[2 * i + 1] = __builtin_isfinite(hi) ? r[2 * i + 1] - hi : 0.0f;
+      if (P > 1 && far) {
+        const uint32_t lo = take_part(r[2 * i]);
+        part[p][i] = lo | take_part(r[2 * i + 1]) << 16;
+      } else {
+        part[p][i] = f32x2_to_bf16x2_bits(r[2 * i], r[2 * i + 1]);
+        r[2 * i] -= bf16_lo(part[p][i]);
+        r[2 * i + 1] -= bf16_hi(part[p][i]);
       }
     }
   }

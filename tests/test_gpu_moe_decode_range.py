@@ -1,13 +1,12 @@
-"""moe.moe_decode where its inner values need all their digits, next to the others in tests/test_gpu_moe_decode.py."""
+"""moe.moe_decode where its inner values need all their digits or come near the largest ones, next to the others in
+tests/test_gpu_moe_decode.py."""
+import math
+
 import pytest
 import torch
 
 from cinnamon_amd import moe
-
-U = 2.0 ** -24
-STEP = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
-DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
-E4M3 = torch.float8_e4m3fn
+from tests.test_gpu_moe_decode import DT, E4M3, STEP, U, check, definition, inputs
 
 
 def pairs(dev, T, D, dt, wt, lead, gen):
@@ -59,3 +58,53 @@ def test_h_keeps_24_bits(dev, T, dt, wt, where):
     tol = (24 + 1 + 4) * U * size + (1 + 2.0 ** -8) * STEP[got.dtype] * want.abs() + 2.0 ** -25
     bad = ~((got.double() - want).abs() <= tol)
     assert not bad.any(), ((got.double() - want).abs() / tol)[bad].max()
+
+
+LARGEST = torch.finfo(torch.float32).max
+LARGEST16 = 2.0 ** 128 - 2.0 ** 120  # of bf16
+FAR = 2.0 ** 128 - 2.0 ** 119  # from here on rounding to bf16 gives infinity
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("wt", ["fp8", "bf16"])
+@pytest.mark.parametrize("T", [1, 20])
+@pytest.mark.parametrize("big", [LARGEST16, FAR - 2.0 ** 104, FAR, -FAR, LARGEST, -LARGEST])
+def test_states_next_to_the_largest(dev, big, T, wt):
+    """Finite fp32 states whose rounding to bf16 is infinite: their weights are zero, or (bf16 weights) bring them
+    back to the others' size."""
+    D, H, E = 144, 64, 2
+    x, r, experts, shared = inputs(dev, T, D, H, E, "fp32", wt, H)
+    r[:, 3] = 0
+    for w in (experts, shared):
+        w[0].view(torch.uint8 if wt == "fp8" else w[0].dtype)[..., 3] = 0
+        if wt == "bf16":
+            w[0][..., 3] = 2.0 ** -126 * torch.randint(-2, 3, w[0].shape[:-1], generator=torch.Generator().manual_seed(4)).to(dev)
+    x[T - 1, 3] = big
+    got = moe.moe_decode(x, r, experts, 2, shared=shared, return_routing=True)
+    assert torch.isfinite(got[0]).all()
+    check(got, definition(x, r, experts, 2, shared=shared))
+    x[T - 1, 3] = math.copysign(math.inf, big)
+    assert not torch.isfinite(moe.moe_decode(x, r, experts, 2, shared=shared)[T - 1]).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("T", [1, 20, 100])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_h_next_to_the_largest(dev, T, dt, sign):
+    """h = 2^64 (2^64 - 2^56 + 2^55 v), v in [1, 2): finite, rounding to infinity in bf16.  Its three products and one sum
+    are within 8 u (silu of 2^64 is exact), its parts and the output's product within 4 u more."""
+    D, H = 64, 32
+    x = torch.zeros(T, D, device=dev)
+    x[:, 0] = 1
+    x[:, 1] = 1 + torch.arange(T, device=dev) / 128
+    x = x.to(DT[dt])
+    w12, w3 = torch.zeros(1, 2 * H, D, device=dev), torch.zeros(1, D, H, device=dev)
+    w12[:, 0, 0] = 2.0 ** 64
+    w12[:, H, 0], w12[:, H, 1] = sign * (2.0 ** 64 - 2.0 ** 56), sign * 2.0 ** 55
+    w3[:, :, 0] = 2.0 ** -120
+    r = torch.zeros(1, D, device=dev)
+    got = moe.moe_decode(x, r, (w12.bfloat16(), None, w3.bfloat16(), None), 1)
+    want = sign * 2.0 ** -56 * (2.0 ** 64 - 2.0 ** 56 + 2.0 ** 55 * x[:, 1:2].double()).expand(T, D)
+    assert (want.abs() * 2.0 ** 120 >= FAR).all() and (want.abs() * 2.0 ** 120 <= LARGEST).all()
+    assert ((got.double() - want).abs() <= (12 * U + (1 + 2.0 ** -8) * STEP[got.dtype]) * want.abs()).all()
