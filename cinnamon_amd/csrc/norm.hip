@@ -853,7 +853,8 @@ int common_args(NormArgs& a, const char* name, const void* y, int dtype, int64_t
   CIN_CHECK_ARG(T >= 0 && T < (1LL << 40) && D >= 1 && D <= kMaxWidth, "%s: D must be in [1, %lld]", name, (long long)kMaxWidth);
   CIN_CHECK_ARG(ldy >= D && (!r || ldr >= D), "%s: row stride below D", name);
   CIN_CHECK_ARG((!w || is_type(w_dtype)) && (!pw || is_type(pw_dtype)), "%s: weights must be bf16, fp16 or fp32", name);
-  CIN_CHECK_ARG(gate_kind >= kNoGate && gate_kind <= kElement && (gate != nullptr) == (gate_kind != kNoGate) &&
+  const bool no_gates = T == 0 && (gate_kind == kRow || gate_kind == kElement);  // one for each of no rows: maybe null
+  CIN_CHECK_ARG(gate_kind >= kNoGate && gate_kind <= kElement && (no_gates || (gate != nullptr) == (gate_kind != kNoGate)) &&
                     (!gate || is_type(gate_dtype)),
                 "%s: bad gate", name);
   CIN_CHECK_ARG(gate_kind != kElement || (gate_dtype == dtype && ldg >= D), "%s: a gate of elements must have y's dtype and rows of D",

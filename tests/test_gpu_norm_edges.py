@@ -1,0 +1,31 @@
+"""norm.block_norm and norm.rms_norm at the edges of what they take, next to the cases of tests/test_gpu_norm.py."""
+import pytest
+import torch
+
+from cinnamon_amd import _lib
+from tests.test_gpu_norm import EPS, NAMES, call, inputs
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gate", ["none", "channel", "row", "element"])
+@pytest.mark.parametrize("shape", [(0, 128), (3, 0, 70)])
+def test_no_rows_with_every_gate(dev, shape, gate):
+    s, value, gn, gx = inputs(dev, shape, "bf16", "fp32", "fp32", True, gate, "channel")
+    leaves = {k: t.clone().requires_grad_() for k, t in s.items() if t is not None}
+    with torch.no_grad():
+        n, x = call(s, value)
+    assert n.shape == x.shape == shape and n.dtype == torch.bfloat16 and x.dtype == torch.float32
+    n, x = call({**s, **leaves}, value)
+    grads = dict(zip(leaves, torch.autograd.grad([n, x], list(leaves.values()), [gn, gx])))
+    assert all(g.shape == s[k].shape and g.dtype == s[k].dtype for k, g in grads.items())
+    assert all((grads[k] == 0).all() for k in NAMES[2:] if k in grads)
+
+
+def test_c_entry_takes_no_rows_without_a_gate_pointer():
+    lib = _lib.load()
+    scale = (None, 0, 0, 1.0)
+    for rows, kind, ok in ((0, 2, True), (0, 3, True), (0, 1, False), (4, 2, False), (4, 3, False)):
+        args = (None, 0, 64, None, 0, 64, rows, 64, None, 0, None, 0, None, 0, kind, 64, *scale)
+        want = 0 if ok else _lib.CIN_ERR_ARG
+        assert lib.cin_block_norm(*args, EPS, None, None, None, None) == want, (rows, kind)
+        assert lib.cin_block_norm_backward(*args, None, None, 0, None, 0, *(None,) * 6, None, 0, None) == want, (rows, kind)
