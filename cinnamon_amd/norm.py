@@ -137,7 +137,7 @@ def _inputs(y, residual, weight, post_weight, gate, scale, value):
                 gate = gate.reshape(-1)
             if kind == _CHANNEL or gate.stride(0) < 1:
                 gate = gate.contiguous()
-            gp, ldg = gate.data_ptr(), gate.stride(0)
+            gp, ldg = gate.data_ptr(), max(gate.stride(0), 1)  # (one expanded value stays as it is, with 0)
     y, yp, ldy = _rows(y, D)
     if residual is None:
         rp, rcode, ldr = 0, code, D

@@ -29,3 +29,19 @@ def test_c_entry_takes_no_rows_without_a_gate_pointer():
         want = 0 if ok else _lib.CIN_ERR_ARG
         assert lib.cin_block_norm(*args, EPS, None, None, None, None) == want, (rows, kind)
         assert lib.cin_block_norm_backward(*args, None, None, 0, None, 0, *(None,) * 6, None, 0, None) == want, (rows, kind)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(1, 128), (1, 1, 1100), (128,)])
+def test_one_row_with_an_expanded_gate(dev, shape):
+    """A gate that repeats one value has no stride, and of one row none that a copy would give it."""
+    s, value, gn, gx = inputs(dev, shape, "bf16", "bf16", "fp32", False, "none", "one")
+    gate = torch.full((), 0.625, device=dev).expand(*shape[:-1], 1)
+    assert gate.stride()[-1] == 0
+    results = []
+    for g in (gate.clone(), gate.detach()):
+        s["gate"] = g.requires_grad_()
+        n, x = call(s, value)
+        results.append((n, x, *torch.autograd.grad([n, x], [g], [gn, gx])))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    assert results[1][2].shape == gate.shape
