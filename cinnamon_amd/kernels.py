@@ -32,6 +32,7 @@ kernels.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import call, dtype_code, ptr, stream_of
@@ -110,9 +111,28 @@ def _run(op, *args):
     return _LAUNCH[op](*args) if _plain_eager(*args) else op(*args)
 
 
+def _refuse_tangents(*args) -> None:
+    """Raise where an argument carries a forward-mode derivative: a launch, or an operator's, would
+    give a result without one."""
+    if forward_ad._current_level >= 0 and any(isinstance(a, torch.Tensor) and _has_tangent(a) for a in args):
+        raise NotImplementedError("no forward-mode derivative of this operator")
+
+
+def _has_tangent(t) -> bool:
+    ft = torch._C._functorch
+    while ft.is_batchedtensor(t):
+        t = ft.get_unwrapped(t)
+    # (of a transform inside another only the inner one's tangents are to be seen)
+    if ft.is_functorch_wrapped_tensor(t) and (ft.is_functorch_wrapped_tensor(ft.get_unwrapped(t))
+                                              or ft.peek_interpreter_stack().key() != ft.TransformType.Jvp):
+        return True
+    return forward_ad.unpack_dual(t).tangent is not None
+
+
 def _run_detached(op, *args):
     """_run for an operator whose result could be mistaken for a differentiable one: with an
-    input that records a graph, the operator runs (and refuses the backward)."""
+    input that records a graph, the operator runs (and refuses the backward); tangents are refused here."""
+    _refuse_tangents(*args)
     if _grad_enabled():
         for a in args:
             if type(a) is torch.Tensor and a.requires_grad:

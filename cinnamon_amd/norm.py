@@ -14,7 +14,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import _DTYPE_CODE, call_on, ptr, stream_of
-from .kernels import _plain_eager, _require, custom_op
+from .kernels import _plain_eager, _refuse_tangents, _require, custom_op
 
 __all__ = ["block_norm", "rms_norm"]
 
@@ -27,7 +27,7 @@ _NO_GATE, _CHANNEL, _ROW, _ELEMENT = range(4)
 def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-6) -> torch.Tensor:
     """x / sqrt(mean(x^2) + eps) * weight over the last dimension (weight [D], default ones): x [..., D]
     in bf16, fp16 or fp32, at most 16384 wide; squares and sums in fp32, the result rounded once to x's
-    dtype.  Differentiable (once) in x and weight."""
+    dtype.  Differentiable (once, in reverse mode) in x and weight."""
     _check(x, None, weight, None, None, None)
     return _call(x, None, weight, None, None, None, 1.0, eps)[0]
 
@@ -46,8 +46,8 @@ def block_norm(y: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | N
     Returns (normed in y's dtype, new_residual in residual's).
 
     Computed in fp32 and each output rounded once: the norm is that of the sum before its rounding.
-    Differentiable (once) in every tensor, gradients in their dtype, bit-identical from call to call.  The backward
-    keeps the inputs and two words a row, forms the sum again, and works in up to 12 D bytes a workgroup."""
+    Differentiable (once, in reverse mode) in every tensor, gradients in their dtype, bit-identical from call to call.
+    The backward keeps the inputs and two words a row, forms the sum again, and works in up to 12 D bytes a workgroup."""
     _require(residual is not None, "residual must be a tensor (rms_norm takes none)")
     if residual_scale is None:
         scale, value = None, 1.0
@@ -95,6 +95,7 @@ def _gate_kind(gate, y):
 
 def _call(y, residual, weight, post_weight, gate, scale, value, eps):
     tensors = [t for t in (y, residual, weight, post_weight, gate, scale) if t is not None]
+    _refuse_tangents(*tensors)
     if _plain_eager() and all(type(t) in _PLAIN for t in tensors):
         if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
             return _BlockNorm.apply(y, residual, weight, post_weight, gate, scale, value, float(eps))
@@ -214,6 +215,7 @@ class _BlockNorm(torch.autograd.Function):
 def _gradients(ctx, gn, gx):
     if gn is None and gx is None:
         return (None,) * 8
+    _refuse_tangents(gn, gx)
     return (*_launch_backward(gn, gx, *ctx.saved_tensors, ctx.value, ctx.needs_input_grad), None, None)
 
 
@@ -259,6 +261,7 @@ def _setup(ctx, inputs, output):
 
 def _backward(ctx, gn, gx, _gstats):
     *tensors, stats = ctx.saved_tensors
+    _refuse_tangents(gn, gx, *tensors)
     needs = [bool(n) and t is not None for n, t in zip(ctx.needs_input_grad[:6], tensors)]
     grads = _norm_bwd_op(gn, gx if tensors[1] is not None else None, *tensors, stats, ctx.value, needs)
     return (*(g if need else None for g, need in zip(grads, needs)), None, None)
