@@ -921,6 +921,7 @@ def indexer_scores_fp8(q: torch.Tensor, k: torch.Tensor, weights: torch.Tensor,
     _require(d % 32 == 0 and 32 <= d <= 256, "head dim must be a multiple of 32 in [32, 256]")
     S = k.shape[1]
     w = weights.float().contiguous()
+    _refuse_tangents(w)
     if H <= (4 if d <= 128 else 2):
         # the q codes are kept only for the weights' gradient
         save_q = torch.is_grad_enabled() and w.requires_grad
@@ -1016,6 +1017,7 @@ class _IndexerScoresQ(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad):
         q8, qs, k8, ks = ctx.saved_tensors
+        _refuse_tangents(grad)
         return None, None, _launch_wgrad(q8, qs, k8, ks, grad, ctx.softmax_scale), None, None
 
 
@@ -1062,6 +1064,7 @@ def _indexer_q_backward(ctx, grad, _grad_q8, _grad_qs):
     if ctx.needs_input_grad[3]:
         _require(ctx.save_q, "indexer_scores_fp8_q: the weights' gradient needs save_q=True")
         q8, q_scale, k8, k_scale = ctx.saved_tensors
+        _refuse_tangents(grad)
         dw = _indexer_wgrad_op(q8, q_scale, k8, k_scale, grad, ctx.softmax_scale)
     return None, None, None, dw, None, None
 
@@ -1107,6 +1110,7 @@ def _indexer_backward(ctx, grad):
     q8, q_scale, k8, k_scale = ctx.saved_tensors
     dw = None
     if ctx.needs_input_grad[4]:
+        _refuse_tangents(grad)
         dw = _indexer_wgrad_op(q8, q_scale, k8, k_scale, grad, ctx.softmax_scale)
     return None, None, None, None, dw, None
 

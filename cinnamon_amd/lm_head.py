@@ -21,7 +21,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import call_on, dtype_code, ptr, stream_of
-from .kernels import _cdiv, _plain_eager, _require, _run, custom_op
+from .kernels import _cdiv, _plain_eager, _refuse_tangents, _require, _run, custom_op
 
 __all__ = ["linear_cross_entropy", "verify_drafts"]
 
@@ -64,6 +64,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     if y.dtype != torch.int64:
         y = y.to(torch.int64)
     mode = _MODES[reduction]
+    _refuse_tangents(x2, weight)
     # (a layer's own Parameter is a plain tensor to the autograd Function)
     if _plain_eager(y) and type(x2) in _PLAIN and type(weight) in _PLAIN:
         if torch.is_grad_enabled() and (x2.requires_grad or weight.requires_grad):
@@ -185,6 +186,7 @@ class _LinearCE(torch.autograd.Function):
 
 
 def _gradients(ctx, grad):
+    _refuse_tangents(grad)
     dx, dw = _launch_backward(grad, *ctx.saved_tensors, *ctx.options, *ctx.needs_input_grad[:2])
     return dx, dw, None, None, None
 
@@ -225,6 +227,7 @@ def _setup(ctx, inputs, output):
 
 def _backward(ctx, grad, _state):
     need_x, need_w = ctx.needs_input_grad[:2]
+    _refuse_tangents(grad, *ctx.saved_tensors)
     dx, dw = _backward_op(grad, *ctx.saved_tensors, *ctx.options, need_x, need_w)
     return dx if need_x else None, dw if need_w else None, None, None, None
 

@@ -28,7 +28,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib, layers
 from ._lib import call, call_on, dtype_code, ptr, stream_of
-from .kernels import _cdiv, _plain_eager, _require, _run_detached, _scale_buf, custom_op
+from .kernels import _cdiv, _plain_eager, _refuse_tangents, _require, _run_detached, _scale_buf, custom_op
 
 _ROUTE_CHUNK = 1024  # assignments per route workgroup (csrc/moe.hip kChunk)
 MAX_EXPERTS = 4096
@@ -81,6 +81,7 @@ def moe_gate(logits: torch.Tensor, top_k: int, bias: torch.Tensor | None = None,
         bias = bias.detach()
     options = (int(top_k), _SCORES[score], int(n_groups), int(top_groups), int(group_top), bool(renormalize),
                float(scale), bool(return_scores))
+    _refuse_tangents(logits)
     if _plain_eager(logits, bias):
         if torch.is_grad_enabled() and logits.requires_grad:
             out = _MoeGate.apply(logits, bias, *options)
@@ -143,6 +144,7 @@ class _MoeGate(torch.autograd.Function):
 def _gate_gradient(ctx, _gidx, gw, gs):
     if gw is None and gs is None:
         return (None,) * 10
+    _refuse_tangents(gw, gs)
     _k, score, _g, _tg, _gt, renormalize, scale, _rs = ctx.options
     return (_launch_gate_backward(*ctx.saved_tensors, gw, gs, score, renormalize, scale),) + (None,) * 9
 
@@ -183,6 +185,7 @@ def _gate_setup(ctx, inputs, output):
 
 def _gate_backward(ctx, _gidx, gw, gs):
     logits, idx = ctx.saved_tensors
+    _refuse_tangents(gw, gs, logits)
     score, renormalize, scale, return_scores = ctx.options
     dz = _gate_bwd_op(logits, idx, gw, gs if return_scores else None, score, renormalize, scale)
     return (dz,) + (None,) * 9

@@ -13,7 +13,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from ._lib import call_on, dtype_code, ptr, stream_of
-from .kernels import _plain_eager, _require, custom_op
+from .kernels import _plain_eager, _refuse_tangents, _require, custom_op
 
 __all__ = ["rotary_tables", "apply_rotary"]
 
@@ -99,6 +99,7 @@ def apply_rotary(q: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k: torch
         if positions.dtype != torch.int64:
             positions = positions.to(torch.int64)
     args = (q, k, cos, sin, positions, bool(interleaved), int(start))
+    _refuse_tangents(*args)
     if _plain_eager(*args):
         if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
             out = _Rotary.apply(*args)
@@ -181,6 +182,7 @@ def _rotary_turn_back(ctx, gq, gk):
     gq, gk = gq if need_q else None, gk if need_k else None
     if gq is None and gk is None:
         return (None,) * 7
+    _refuse_tangents(gq, gk)
     return (*_launch(gq, gk, *ctx.saved_tensors, *ctx.options, True), None, None, None, None, None)
 
 
@@ -207,6 +209,7 @@ def _rotary_setup(ctx, inputs, output):
 def _rotary_backward(ctx, gq, gk):
     cos, sin, positions = ctx.saved_tensors
     interleaved, start, inverse = ctx.options
+    _refuse_tangents(gq, gk)
     dq, dk = _rotary_op(gq, gk if ctx.with_k else None, cos, sin, positions, interleaved, start, not inverse)
     return dq, dk if ctx.with_k else None, None, None, None, None, None, None
 

@@ -4,7 +4,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from cinnamon_amd import kernels, norm
+from cinnamon_amd import kernels, lm_head, moe, norm, rotary
 
 
 @pytest.fixture
@@ -76,3 +76,39 @@ def test_operators_without_a_gradient_refuse_tangents():
         torch.func.jvp(lambda x: kernels._run_detached(op, x), (X,), (X,))
     with forward_ad.dual_level(), pytest.raises(NotImplementedError):
         kernels._run_detached(op, forward_ad.make_dual(X, X))
+
+
+class OnDevice(torch.Tensor):
+    """A CPU tensor that says it is on a device, for the public functions' checks."""
+    is_cuda = True
+
+
+def on_device(t):
+    return t.as_subclass(OnDevice)
+
+
+def test_differentiable_operators_refuse_tangents(monkeypatch):
+    """moe_gate, apply_rotary, linear_cross_entropy and indexer_scores_fp8 (its weights), at the call and in the backward."""
+    logits, x, y = on_device(torch.randn(3, 8)), torch.randn(1, 3, 2, 32), torch.zeros(3, dtype=torch.int64)
+    cos = on_device(torch.ones(3, 16))
+    calls = [(logits, lambda t: moe.moe_gate(t, 2)[1]), (on_device(x), lambda t: rotary.apply_rotary(t, cos, cos)),
+             (on_device(x), lambda t: rotary.apply_rotary(on_device(x), cos, cos, k=t)[1]),
+             (logits, lambda t: lm_head.linear_cross_entropy(t, on_device(torch.randn(5, 8)), on_device(y))),
+             (logits, lambda t: lm_head.linear_cross_entropy(on_device(torch.randn(3, 8)), t, on_device(y))),
+             (on_device(torch.randn(1, 3, 2)), lambda t: kernels.indexer_scores_fp8(on_device(x), on_device(x[:, :, 0]), t, 1.0))]
+    for t, f in calls:
+        with forward_ad.dual_level(), pytest.raises(NotImplementedError):
+            f(forward_ad.make_dual(t, torch.ones_like(t)))
+    for module, name in ((moe, "_launch_gate_backward"), (rotary, "_launch"), (lm_head, "_launch_backward"), (kernels, "_launch_wgrad")):
+        monkeypatch.setattr(module, name, lambda *a: pytest.fail("launched"))
+
+    class Ctx:
+        saved_tensors, options, needs_input_grad, softmax_scale, with_k, save_q = (X, X, X, X), (0,) * 8, (True,) * 8, 1.0, False, True
+
+    with forward_ad.dual_level():
+        g = forward_ad.make_dual(X, X)
+        for f in (lambda: moe._gate_gradient(Ctx, None, g, None), lambda: rotary._rotary_turn_back(Ctx, g, None),
+                  lambda: lm_head._gradients(Ctx, g), lambda: kernels._IndexerScoresQ.backward(Ctx, g),
+                  lambda: kernels._indexer_backward(Ctx, g), lambda: kernels._indexer_q_backward(Ctx, g, None, None)):
+            with pytest.raises(NotImplementedError):
+                f()
