@@ -523,8 +523,9 @@ def moe_decode(x: torch.Tensor, router_weight: torch.Tensor, experts, top_k: int
     expert, without E and with an H of its own.  D and H are multiples of 16.
 
     Only the chosen experts' weights are read.  Unlike in routed_experts activations are not quantized: x is exact in the
-    products, silu(W1 v) * (W2 v) keeps 24 bits, products are summed in fp32 and the result is rounded once.  Inference only: no
-    gradient.  Bit-identical from call to call."""
+    products, silu(W1 v) * (W2 v) keeps 24 bits, products are summed in fp32 and the result is rounded once.
+    Bit-identical from call to call.  Inference only: where x, a weight (also of a GroupedExperts), a scale or the bias
+    requires a gradient, the backward is refused; torch.no_grad() saves the host work of that."""
     _require(x.is_cuda, "Input must be on CUDA")
     _require(x.ndim == 2 and x.shape[0] <= MAX_DECODE_TOKENS, "x must be [n_tokens, D] with at most 128 tokens")
     _require(x.dtype in _DTYPES, "x must be bf16, fp16 or fp32")
@@ -544,11 +545,14 @@ def moe_decode(x: torch.Tensor, router_weight: torch.Tensor, experts, top_k: int
         _require(bias.shape == (E,) and bias.device == dev and bias.dtype == torch.float32,
                  "bias must be fp32 [n_experts] on x's device")
         bias = _without_grad(bias)
+    trained = None
     if isinstance(experts, layers.GroupedExperts):
         _require(experts.n_experts == E and experts.d_model == D, "the router and the experts differ in number or width")
         _require(D % 128 == 0 and experts.hidden_dim % 64 == 0, "GroupedExperts' FP8 blocks need D in multiples of 128, H of 64")
         w12, w3 = experts.w12.detach(), experts.w3.detach()
         H = experts.hidden_dim
+        if torch.is_grad_enabled():  # (their codes record no graph)
+            trained = next((w for w in (experts.w12, experts.w3) if w.requires_grad), None)
         q = experts.quantized_weights()
         (w12q, _, w12s), (w3q, _, w3s) = q if q is not None else layers.quantize_expert_weights(w12, w3)
         experts = (w12q.view(E, 2 * H, D), w12s.view(E, 2 * H // 128, -1), w3q.view(E, D, H), w3s.view(E, D // 128, -1))
@@ -558,7 +562,7 @@ def moe_decode(x: torch.Tensor, router_weight: torch.Tensor, experts, top_k: int
         extra = _decode_weights(shared, x, ())
         _require(extra[0].dtype == weights[0].dtype, "the shared expert's weights must have the experts' type")
     out = _run_detached(_decode_op, x, router_weight, bias, *weights, *extra, int(top_k), _SCORES[score], int(n_groups),
-                        int(top_groups), int(group_top), bool(renormalize), float(scale))
+                        int(top_groups), int(group_top), bool(renormalize), float(scale), trained)
     return out if return_routing else out[0]
 
 
@@ -583,8 +587,11 @@ def _decode_weights(weights, x, lead):
 
 
 def _without_grad(t):
+    """A plain tensor; but what records a graph stays, so that the operator refuses its backward."""
     # (detach costs 0.6 us of host time each)
-    return t if type(t) is torch.Tensor and not t.requires_grad else t.detach()
+    if t.requires_grad:
+        return t if torch.is_grad_enabled() else t.detach()
+    return t if type(t) is torch.Tensor else t.detach()
 
 
 @functools.lru_cache(maxsize=256)
@@ -608,9 +615,10 @@ def _on16(t):
 
 @custom_op("moe_decode", "(Tensor x, Tensor router, Tensor? bias, Tensor w12, Tensor? s12, Tensor w3, Tensor? s3, Tensor? shared_w12, "
            "Tensor? shared_s12, Tensor? shared_w3, Tensor? shared_s3, int top_k, int score, int n_groups, int top_groups, "
-           "int group_top, bool renormalize, float scale) -> (Tensor, Tensor, Tensor)")
+           "int group_top, bool renormalize, float scale, Tensor? trained=None) -> (Tensor, Tensor, Tensor)")
 def _decode_op(x, router, bias, w12, s12, w3, s3, sw12, ss12, sw3, ss3, top_k, score, n_groups, top_groups, group_top, renormalize,
-               scale):
+               scale, trained=None):
+    # trained: a weight behind the codes that records a graph, for the refusal of its backward alone
     x, router = _gate_rows(x), _gate_rows(router)
     T, D = x.shape
     E, H = router.shape[0], w3.shape[-1]

@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from cinnamon_amd import moe
+from cinnamon_amd import kernels, layers, moe
 from tests.test_gpu_moe_decode import DT, E4M3, STEP, U, check, definition, inputs
 
 
@@ -108,3 +108,53 @@ def test_h_next_to_the_largest(dev, T, dt, sign):
     want = sign * 2.0 ** -56 * (2.0 ** 64 - 2.0 ** 56 + 2.0 ** 55 * x[:, 1:2].double()).expand(T, D)
     assert (want.abs() * 2.0 ** 120 >= FAR).all() and (want.abs() * 2.0 ** 120 <= LARGEST).all()
     assert ((got.double() - want).abs() <= (12 * U + (1 + 2.0 ** -8) * STEP[got.dtype]) * want.abs()).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("wt", ["fp8", "bf16"])
+def test_whatever_requires_a_gradient_has_its_backward_refused(dev, wt):
+    """One tensor of the call at a time; the result is that of the call without."""
+    x, r, experts, shared = inputs(dev, 3, 256, 128, 4, "bf16", wt, 128)
+    bias = torch.zeros(4, device=dev)
+
+    def call(x, r, bias, *w):
+        return moe.moe_decode(x, r, w[:4], 2, bias=bias, shared=w[4:], return_routing=True)
+
+    tensors = [x, r, bias, *experts, *shared]
+    want = call(*tensors)
+    assert not want[0].requires_grad
+    for i, t in enumerate(tensors):
+        if t is None or t.dtype == E4M3:
+            continue
+        for leaf in (t.clone().requires_grad_(), torch.nn.Parameter(t.clone())):
+            args = [leaf if j == i else v for j, v in enumerate(tensors)]
+            got = call(*args)
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+            with pytest.raises(RuntimeError, match="autograd"):
+                got[0].sum().backward()
+            with torch.no_grad():
+                got = call(*args)
+            assert not got[0].requires_grad and torch.equal(got[0], want[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cached", [False, True])
+def test_trainable_experts_have_their_backward_refused(dev, cached):
+    torch.manual_seed(5)
+    experts = layers.GroupedExperts(4, 256, 128).to(dev)
+    x, r = torch.randn(3, 256, device=dev).bfloat16(), torch.randn(4, 256, device=dev)
+    if cached:
+        kernels.set_weight_cache(experts)
+    with torch.no_grad():
+        want = moe.moe_decode(x, r, experts, 2)
+    assert not want.requires_grad
+    for frozen in ((), ("w12",), ("w3",)):
+        for name in ("w12", "w3"):
+            getattr(experts, name).requires_grad_(name not in frozen)
+        out = moe.moe_decode(x, r, experts, 2)
+        assert torch.equal(out, want)
+        with pytest.raises(RuntimeError, match="autograd"):
+            out.sum().backward()
+    experts.requires_grad_(False)
+    out = moe.moe_decode(x, r, experts, 2)
+    assert not out.requires_grad and torch.equal(out, want)
