@@ -1,9 +1,11 @@
 """norm.block_norm and norm.rms_norm at the edges of what they take, next to the cases of tests/test_gpu_norm.py."""
+import math
+
 import pytest
 import torch
 
 from cinnamon_amd import _lib
-from tests.test_gpu_norm import EPS, NAMES, call, inputs
+from tests.test_gpu_norm import CASES, EPS, NAMES, call, check, definition, inputs
 
 
 @pytest.mark.gpu
@@ -45,3 +47,27 @@ def test_one_row_with_an_expanded_gate(dev, shape):
         results.append((n, x, *torch.autograd.grad([n, x], [g], [gn, gx])))
     assert all(torch.equal(a, b) for a, b in zip(*results))
     assert results[1][2].shape == gate.shape
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", CASES, ids=lambda c: "-".join(map(str, c)))
+def test_gradients_within_their_own_sums(dev, case):
+    """Each gradient by the roundings on its own way, beside the K of tests/test_gpu_norm.py (there a sum over a row is along
+    16 + 6 + 16 of them; the forward's past 8192 channels is along 32 + 6 + 8, which K covers too):
+      y, residual and a gate an element: none more;
+      a gate a row: a sum over a row, 32 + 6 + 16;
+      vectors: a workgroup's T / workgroups rows (at least 256 workgroups), a wave's three others, the
+      partial rows in lines of 32 (at most 4096 / 32 a line) and the lines;
+      a scale of one value: a thread's 16 channels of a row, the rest in 64 bits."""
+    s, value, gn, gx = inputs(dev, *case)
+    ref = definition(s, value, EPS, gn, gx)
+    leaves = {k: t.clone().requires_grad_() for k, t in s.items() if t is not None}
+    n, x = call({**s, **leaves}, value)
+    outs, gs = ([n], [gn]) if x is None else ([n, x], [gn, gx])
+    T = math.prod(case[0][:-1])
+    vector = T / min(T, 256) + 3 + 4096 / 32 + 32
+    more = {"y": 0, "residual": 0, "weight": vector, "post_weight": vector,
+            "gate": {"channel": vector, "row": 32 + 6 + 16, "element": 0}.get(case[5]),
+            "residual_scale": vector if case[6] == "channel" else 16}
+    for k, g in zip(leaves, torch.autograd.grad(outs, list(leaves.values()), gs)):
+        check(g, ref[k], more[k])
