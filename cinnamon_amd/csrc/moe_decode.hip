@@ -27,8 +27,8 @@
 // No atomics on results.
 //
 // Bound by the weights' bytes.  32 experts of 7168 x 2048 in codes, 8 a token, and a shared one: one token 80 us (0.40 GB,
-// 5.0 TB/s: up 39, down 23), 64 tokens 304 (1.46 GB, 4.8: up 163, down 120).  16 experts of 1024 x 1024, one token: 24, the
-// latency of five launches.
+// 5.0 TB/s: up 40, down 24), 64 tokens 327 (1.46 GB, 4.5: up 163-180, down 131-146), 128 tokens 481.  16 experts of
+// 1024 x 1024, one token: 26, the latency of five launches.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -979,8 +979,9 @@ void set_sizes(LayerArgs& a, int dtype, int64_t T, int64_t D, int64_t E, int64_t
 }
 
 // Whether the waves share K: where k_products would have fewer than one and a half workgroups a CU.  One token, 8 of 32
-// experts of 7168 x 2048 and a shared one: up, 288 of them with the shared one's, 47 us against 65, down, 504, 29 against
-// 25; 16 tokens, 16 experts of 1024 x 1024, 320 and 136: 43 against 51 a call.
+// experts of 7168 x 2048 and a shared one: up, 256 of them, 40 us against 52, down, 504, 35 against 24; 2 of 16 experts of
+// 1024 x 1024 and a shared one: up, 32, 5.5 against 9.5, down, 24, 9.8 against 26; 16 tokens of these, 272 and 144: 51
+// against 60 a call.
 bool splits_k(const LayerArgs& a, bool up) {
   const int64_t rows = up ? kTileRows<true> : kTileRows<false>;
   const int64_t groups = a.units * cdiv(up ? a.experts.H : a.D, rows) + (!up && a.shared.H ? cdiv(a.D, rows) : 0);

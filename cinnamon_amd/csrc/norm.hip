@@ -13,16 +13,17 @@
 // S = sum dx y j;  dpw = g S,  dg = pw S.
 //
 // x is formed again from y and r in the backward, in fp32 as in the forward: that reads as many bytes as
-// a stored x and has no rounding to x's type in it.  All arithmetic and the sums are fp32, each output is
-// rounded once.
+// a stored x and has no rounding to x's type in it.  Arithmetic and sums are fp32, the sum over all channels and rows for a
+// learned scale of one value fp64; each output is rounded once.
 //
 // A row is read once into registers, 8 channels a thread and chunk, by one wave (up to 1024 channels, the
 // sums by DPP and swaps, no barrier) or by one workgroup.  Workgroups walk over rows, so that the channels'
-// vectors are loaded once and a channel's sums over the rows stay in registers; each workgroup leaves one
-// row of partial sums, which k_norm_columns adds up in a fixed order.  Bound by HBM: 16384 x 7168 bf16 with post norm,
-// a gate and a learned scale, forward 175 us (0.94 GB, 5.4 TB/s), backward 300 (1.41 GB, 4.7); 16384 x 1024 bf16
-// with an fp32 stream 34 us (0.20 GB, 5.9) and 54 (0.30 GB, 5.6).  Rows of odd lengths lie on no 16 bytes: 4999 x 1111 fp16
-// with a gate an element 23 us (56 MB, 2.5) and 49 (89 MB, 1.8).
+// vectors are loaded once (the backward past 8192 channels reads them again, from L2) and a channel's sums over the rows stay
+// in registers; each workgroup leaves one row of partial sums, which k_norm_columns adds up in a fixed order.
+// Bound by HBM.  16384 rows, bf16 with post norm, a gate a channel and a learned scale, forward and backward: 7168 channels
+// 178-187 us (0.94 GB, 5.0-5.3 TB/s) and 297-316 (1.41 GB, 4.5-4.7), 4096 121 (4.5) and 172 (4.7), 2048 53 (5.1) and 100 (4.0);
+// bf16 with an fp32 stream, 1024 channels 34 (0.20 GB, 5.9) and 54 (0.30 GB, 5.6).  fp16 with a gate an element, 4999 rows: 1112
+// channels 22 (56 MB, 2.5) and 46 (89 MB, 1.9); 1111, whose rows lie on no 16 bytes, 22-27 and 50-61.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -451,7 +452,8 @@ size_t backward_lds(bool scale_channels, int block) {
 }
 
 // Waves a SIMD that the registers are kept to: up to 4096 channels a workgroup is small, and others cover its waits
-// (4999 x 1111 fp16, gate per element: 49 us with three, 66 with two).
+// (4999 x 1111 fp16, gate per element: 49 us with three, 66 with two).  With a 16-bit stream three waves spill 2 registers
+// and four (kChannels) 8.
 template <int CH, bool WAVE, Mode MODE>
 constexpr int kBackwardWaves = WAVE || CH > 1 ? 1 : MODE == kAny ? 3 : 4;
 

@@ -520,7 +520,8 @@ def moe_decode(x: torch.Tensor, router_weight: torch.Tensor, experts, top_k: int
     [E, 2 H, D] (W1 above W2) and w3 [E, D, H], either e4m3 codes with fp32 scales of 128 x 128 blocks
     ([E, ceil(2 H / 128), ceil(D / 128)] and [E, ceil(D / 128), ceil(H / 128)], as
     layers.quantize_expert_weights returns them) or bf16 with None for the scales.  shared: None or such a tuple of one
-    expert, without E and with an H of its own.  D and H are multiples of 16.
+    expert, without E and with an H of its own.  D and H are multiples of 16.  Weights and scales that are not contiguous, or
+    whose first element is not on 16 bytes, are copied whole in every call.
 
     Only the chosen experts' weights are read.  Unlike in routed_experts activations are not quantized: x is exact in the
     products, silu(W1 v) * (W2 v) keeps 24 bits, products are summed in fp32 and the result is rounded once.
