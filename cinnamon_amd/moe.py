@@ -526,7 +526,8 @@ def moe_decode(x: torch.Tensor, router_weight: torch.Tensor, experts, top_k: int
     Only the chosen experts' weights are read.  Unlike in routed_experts activations are not quantized: x is exact in the
     products, silu(W1 v) * (W2 v) keeps 24 bits, products are summed in fp32 and the result is rounded once.
     Bit-identical from call to call.  Inference only: where x, a weight (also of a GroupedExperts), a scale or the bias
-    requires a gradient, the backward is refused; torch.no_grad() saves the host work of that."""
+    requires a gradient, the backward is refused (under torch.compile, which forms it at once, the call is); torch.no_grad()
+    saves the host work of that."""
     _require(x.is_cuda, "Input must be on CUDA")
     _require(x.ndim == 2 and x.shape[0] <= MAX_DECODE_TOKENS, "x must be [n_tokens, D] with at most 128 tokens")
     _require(x.dtype in _DTYPES, "x must be bf16, fp16 or fp32")
