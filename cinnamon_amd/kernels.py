@@ -123,9 +123,10 @@ def _has_tangent(t) -> bool:
     while ft.is_batchedtensor(t):
         t = ft.get_unwrapped(t)
     # (of a transform inside another only the inner one's tangents are to be seen)
-    if ft.is_functorch_wrapped_tensor(t) and (ft.is_functorch_wrapped_tensor(ft.get_unwrapped(t))
-                                              or ft.peek_interpreter_stack().key() != ft.TransformType.Jvp):
-        return True
+    if ft.is_functorch_wrapped_tensor(t):
+        inner = ft.peek_interpreter_stack()
+        if inner is None or inner.key() != ft.TransformType.Jvp or ft.is_functorch_wrapped_tensor(ft.get_unwrapped(t)):
+            return True
     return forward_ad.unpack_dual(t).tangent is not None
 
 
